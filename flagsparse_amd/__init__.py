@@ -68,6 +68,15 @@ from .alpha_spmm import (
     prepare_alpha_spmm_alg1_tle_opt,
     prepare_alpha_spmm_alg1_tle_opt2,
 )
+from .embedding import flagsparse_embedding, flagsparse_embedding_grad
+from .expert import (
+    PreparedExpertRoute,
+    flagsparse_expert_combine,
+    flagsparse_expert_combine_grad,
+    flagsparse_expert_dispatch,
+    flagsparse_expert_dispatch_grad,
+    prepare_expert_route,
+)
 
 __all__ = [
     "benchmark_spmv_case",
@@ -122,4 +131,12 @@ __all__ = [
     "alpha_spmm_alg1_tle_unavailable_reason",
     "alpha_spmm_alg1_tle_opt_unavailable_reason",
     "alpha_spmm_alg1_tle_opt2_unavailable_reason",
+    "flagsparse_embedding",
+    "flagsparse_embedding_grad",
+    "PreparedExpertRoute",
+    "prepare_expert_route",
+    "flagsparse_expert_dispatch",
+    "flagsparse_expert_dispatch_grad",
+    "flagsparse_expert_combine",
+    "flagsparse_expert_combine_grad",
 ]

@@ -94,6 +94,14 @@ EXPORTED_SYMBOLS = (
     "fs_spmm_sell",
     "fs_spmm_sell_staged_fits",
     "fs_spmm_sell_staged",
+    "fs_embedding",
+    "fs_embedding_grad_workspace_bytes",
+    "fs_embedding_grad",
+    "fs_expert_route_workspace_bytes",
+    "fs_expert_route",
+    "fs_expert_dispatch",
+    "fs_expert_combine",
+    "fs_expert_combine_grad",
 )
 
 
@@ -131,6 +139,7 @@ _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _sz = ctypes.c_size_t
+_f64 = ctypes.c_double
 
 
 def _declare(lib):
@@ -254,6 +263,24 @@ def _declare(lib):
     lib.fs_spmm_sell.restype = _i32
     lib.fs_spmm_sell.argtypes = [_i32, _i32, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64,
                                  _vp]
+    lib.fs_embedding.restype = _i32
+    lib.fs_embedding.argtypes = [_i32, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _f64, _vp, _vp]
+    lib.fs_embedding_grad_workspace_bytes.restype = _sz
+    lib.fs_embedding_grad_workspace_bytes.argtypes = [_i32, _i64, _i64, _i64]
+    lib.fs_embedding_grad.restype = _i32
+    lib.fs_embedding_grad.argtypes = [_i32, _i32, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _f64, _i64, _vp, _vp, _sz,
+                                      _vp]
+    lib.fs_expert_route_workspace_bytes.restype = _sz
+    lib.fs_expert_route_workspace_bytes.argtypes = [_i64, _i64]
+    lib.fs_expert_route.restype = _i32
+    lib.fs_expert_route.argtypes = [_i32, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]
+    lib.fs_expert_dispatch.restype = _i32
+    lib.fs_expert_dispatch.argtypes = [_i32, _i64, _i32, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp]
+    lib.fs_expert_combine.restype = _i32
+    lib.fs_expert_combine.argtypes = [_i32, _i64, _i32, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp]
+    lib.fs_expert_combine_grad.restype = _i32
+    lib.fs_expert_combine_grad.argtypes = [_i32, _i64, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
+                                           _vp]
     lib.fs_last_kernel.restype = ctypes.c_char_p
     lib.fs_last_kernel.argtypes = []
 

@@ -1,0 +1,40 @@
+"""Checks and layouts that the row operators share (embedding.py, expert.py)."""
+
+import torch
+
+from . import _lib
+
+ROW_VALUE_CODES = {
+    torch.float16: _lib.FS_F16,
+    torch.bfloat16: _lib.FS_BF16,
+    torch.float32: _lib.FS_F32,
+    torch.float64: _lib.FS_F64,
+}
+ROW_DTYPE_MESSAGE = "float16, bfloat16, float32, float64"
+
+
+def row_major(t):
+    """(t, stride of its rows) of a 2D tensor whose rows are contiguous; a copy
+    where they are not, or where rows overlap or run backwards."""
+    if t.is_contiguous():
+        return t, t.shape[1]
+    if t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
+        return t, t.stride(0)
+    t = t.contiguous()
+    return t, t.shape[1]
+
+
+def wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def check_out(out, device, shape, dtype):
+    """Same checks and messages as the sparse products' (spmm_coo.py:619-625)."""
+    if not isinstance(out, torch.Tensor):
+        raise TypeError("out must be a torch.Tensor")
+    if not out.is_cuda:
+        raise ValueError("out must be a CUDA tensor")
+    if out.device != device:
+        raise ValueError("out must be on the same CUDA device as the inputs")
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
+        raise ValueError("out shape/dtype must match result")

@@ -1,0 +1,216 @@
+// expert_rows.hip — token rows into expert order and back.
+//
+// With inverse[t, j] the place of slot j of token t and `routed` the number of
+// slots that name an expert (places from there on belong to none):
+//   dispatch      rows[inverse[t, j]] = x[t], 0 for slots of no expert
+//   combine       out[t] = sum_j w[t, j] rows[inverse[t, j]] over routed slots
+//                 (w = 1: the gradient of dispatch)
+//   combine_grad  grad_rows[inverse[t, j]] = w[t, j] grad[t];
+//                 grad_w[t, j] = sum_h grad[t, h] rows[inverse[t, j], h]
+// Products with the routing matrix, tokens by rows, and its transpose; all are
+// bound by the rows' bytes.  Sums run in slot order in 32 bits (64 for float64)
+// and are rounded once; a slot of no expert is left out, whatever its row holds.
+#include "select_rows.hpp"
+
+namespace fs {
+namespace {
+
+template <class V, bool ALIGNED>
+__global__ __launch_bounds__(256) void expert_dispatch_kernel(const V* __restrict__ x, int64_t ldx, int64_t n_tokens,
+                                                              int slots, int64_t width, int lpr,
+                                                              const int32_t* __restrict__ inverse,
+                                                              const int32_t* __restrict__ routed_at,
+                                                              V* __restrict__ out) {
+  constexpr int E = Slice<V>::n;
+  const int lane = threadIdx.x & (lpr - 1);
+  const int64_t t = (int64_t)blockIdx.x * (256 / lpr) + threadIdx.x / lpr;
+  if (t >= n_tokens) return;
+  const int routed = *routed_at;
+  const V* row = x + t * ldx;
+  const int32_t* inv = inverse + t * slots;
+  const int64_t full = width / E;
+  for (int64_t c = lane; c < full; c += lpr) {
+    const Slice<V> s = load_slice<ALIGNED>(row + c * E);
+    for (int j = 0; j < slots; ++j) {
+      const int at = inv[j];
+      Slice<V> o = s;
+      if (at >= routed)
+#pragma unroll
+        for (int e = 0; e < E; ++e) o.v[e] = (V)0;
+      store_slice<ALIGNED>(out + at * width + c * E, o);
+    }
+  }
+  for (int64_t h = full * E + lane; h < width; h += lpr)
+    for (int j = 0; j < slots; ++j) out[(int64_t)inv[j] * width + h] = inv[j] < routed ? row[h] : (V)0;
+}
+
+template <class V, bool ALIGNED>
+__global__ __launch_bounds__(256) void expert_combine_kernel(const V* __restrict__ rows, int64_t ldr, int64_t n_tokens,
+                                                             int slots, int64_t width, int lpr,
+                                                             const int32_t* __restrict__ inverse,
+                                                             const int32_t* __restrict__ routed_at,
+                                                             const typename Elem<V>::acc* __restrict__ weights,
+                                                             V* __restrict__ out) {
+  using A = typename Elem<V>::acc;
+  constexpr int E = Slice<V>::n;
+  const int lane = threadIdx.x & (lpr - 1);
+  const int64_t t = (int64_t)blockIdx.x * (256 / lpr) + threadIdx.x / lpr;
+  if (t >= n_tokens) return;
+  const int routed = *routed_at;
+  const int32_t* inv = inverse + t * slots;
+  const A* wt = weights != nullptr ? weights + t * slots : nullptr;
+  const int64_t full = width / E;
+  for (int64_t c = lane; c < full; c += lpr) {
+    A acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0;
+#pragma unroll 4
+    for (int j = 0; j < slots; ++j) {
+      const int at = inv[j];
+      if (at >= routed) continue;
+      const A w = wt != nullptr ? wt[j] : (A)1;
+      const Slice<V> s = load_slice<ALIGNED>(rows + at * ldr + c * E);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += w * widen(s.v[e]);
+    }
+    Slice<V> o;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o.v[e] = (V)acc[e];
+    store_slice<ALIGNED>(out + t * width + c * E, o);
+  }
+  for (int64_t h = full * E + lane; h < width; h += lpr) {
+    A acc = 0;
+    for (int j = 0; j < slots; ++j)
+      if (inv[j] < routed) acc += (wt != nullptr ? wt[j] : (A)1) * widen(rows[inv[j] * ldr + h]);
+    out[t * width + h] = (V)acc;
+  }
+}
+
+// One wave a slot: the token's gradient row, read by its slots in turn, comes
+// from cache after the first.
+template <class V, bool ALIGNED>
+__global__ __launch_bounds__(256) void expert_combine_grad_kernel(
+    const V* __restrict__ grad, int64_t ldg, const V* __restrict__ rows, int64_t ldr, int64_t n, int slots,
+    int64_t width, const int32_t* __restrict__ inverse, const int32_t* __restrict__ routed_at,
+    const typename Elem<V>::acc* __restrict__ weights, V* __restrict__ grad_rows,
+    typename Elem<V>::acc* __restrict__ grad_w) {
+  using A = typename Elem<V>::acc;
+  constexpr int E = Slice<V>::n;
+  const int lane = threadIdx.x & 63;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= n) return;
+  const int at = inverse[i];
+  const bool in = at < *routed_at;
+  const A w = in ? weights[i] : (A)0;
+  const V* g = grad + i / slots * ldg;
+  const V* y = rows + at * ldr;
+  V* o = grad_rows + at * width;
+  const int64_t full = width / E;
+  A dot = 0;
+  for (int64_t c = lane; c < full; c += 64) {
+    Slice<V> out;
+    if (in) {
+      const Slice<V> sg = load_slice<ALIGNED>(g + c * E), sy = load_slice<ALIGNED>(y + c * E);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const A ge = widen(sg.v[e]);
+        dot += ge * widen(sy.v[e]);
+        out.v[e] = (V)(w * ge);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) out.v[e] = (V)0;
+    }
+    store_slice<ALIGNED>(o + c * E, out);
+  }
+  for (int64_t h = full * E + lane; h < width; h += 64) {
+    if (in) dot += widen(g[h]) * widen(y[h]);
+    o[h] = in ? (V)(w * widen(g[h])) : (V)0;
+  }
+  dot = wave_sum(dot);
+  if (lane == 0) grad_w[i] = dot;
+}
+
+int check_rows(const char* who, int64_t n_tokens, int slots, int64_t width, int64_t n_experts) {
+  if (n_tokens < 0 || slots < 1 || width < 0 || n_experts < 1 || n_tokens > INT32_MAX / slots)
+    return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
+  return FS_OK;
+}
+
+}  // namespace
+}  // namespace fs
+
+extern "C" int fs_expert_dispatch(int val_t, int64_t n_tokens, int slots, int64_t width, int64_t n_experts,
+                                  const void* x, int64_t ldx, const int32_t* inverse, const int32_t* offsets,
+                                  void* out, hipStream_t stream) {
+  using namespace fs;
+  if (int rc = check_rows("fs_expert_dispatch", n_tokens, slots, width, n_experts)) return rc;
+  if (n_tokens == 0 || width == 0) return FS_OK;
+  if (!x || !inverse || !offsets || !out || ldx < 0) return fail(FS_E_INVALID, "fs_expert_dispatch: bad pointer or stride");
+  return with_value_type(val_t, "fs_expert_dispatch", [&](auto v) -> int {
+    using V = decltype(v);
+    const int64_t s = sizeof(V);
+    const int lpr = lanes_per_row(width / Slice<V>::n);
+    const dim3 grid((uint32_t)ceil_div(n_tokens, 256 / lpr));
+    if (aligned16(x, ldx * s) && aligned16(out, width * s))
+      hipLaunchKernelGGL((expert_dispatch_kernel<V, true>), grid, dim3(256), 0, stream, (const V*)x, ldx, n_tokens,
+                         slots, width, lpr, inverse, offsets + n_experts, (V*)out);
+    else
+      hipLaunchKernelGGL((expert_dispatch_kernel<V, false>), grid, dim3(256), 0, stream, (const V*)x, ldx, n_tokens,
+                         slots, width, lpr, inverse, offsets + n_experts, (V*)out);
+    FS_CHECK_MAIN_LAUNCH("expert_dispatch_kernel");
+    return FS_OK;
+  });
+}
+
+extern "C" int fs_expert_combine(int val_t, int64_t n_tokens, int slots, int64_t width, int64_t n_experts,
+                                 const void* rows, int64_t ldr, const int32_t* inverse, const int32_t* offsets,
+                                 const void* weights, void* out, hipStream_t stream) {
+  using namespace fs;
+  if (int rc = check_rows("fs_expert_combine", n_tokens, slots, width, n_experts)) return rc;
+  if (n_tokens == 0 || width == 0) return FS_OK;
+  if (!rows || !inverse || !offsets || !out || ldr < 0) return fail(FS_E_INVALID, "fs_expert_combine: bad pointer or stride");
+  return with_value_type(val_t, "fs_expert_combine", [&](auto v) -> int {
+    using V = decltype(v);
+    using A = typename Elem<V>::acc;
+    const int64_t s = sizeof(V);
+    const int lpr = lanes_per_row(width / Slice<V>::n);
+    const dim3 grid((uint32_t)ceil_div(n_tokens, 256 / lpr));
+    if (aligned16(rows, ldr * s) && aligned16(out, width * s))
+      hipLaunchKernelGGL((expert_combine_kernel<V, true>), grid, dim3(256), 0, stream, (const V*)rows, ldr, n_tokens,
+                         slots, width, lpr, inverse, offsets + n_experts, (const A*)weights, (V*)out);
+    else
+      hipLaunchKernelGGL((expert_combine_kernel<V, false>), grid, dim3(256), 0, stream, (const V*)rows, ldr, n_tokens,
+                         slots, width, lpr, inverse, offsets + n_experts, (const A*)weights, (V*)out);
+    FS_CHECK_MAIN_LAUNCH("expert_combine_kernel");
+    return FS_OK;
+  });
+}
+
+extern "C" int fs_expert_combine_grad(int val_t, int64_t n_tokens, int slots, int64_t width, int64_t n_experts,
+                                      const void* grad, int64_t ldg, const void* rows, int64_t ldr,
+                                      const int32_t* inverse, const int32_t* offsets, const void* weights,
+                                      void* grad_rows, void* grad_weights, hipStream_t stream) {
+  using namespace fs;
+  if (int rc = check_rows("fs_expert_combine_grad", n_tokens, slots, width, n_experts)) return rc;
+  if (n_tokens == 0) return FS_OK;
+  if (!inverse || !offsets || !weights || !grad_weights || ldg < 0 || ldr < 0 ||
+      (width > 0 && (!grad || !rows || !grad_rows)))
+    return fail(FS_E_INVALID, "fs_expert_combine_grad: bad pointer or stride");
+  return with_value_type(val_t, "fs_expert_combine_grad", [&](auto v) -> int {
+    using V = decltype(v);
+    using A = typename Elem<V>::acc;
+    const int64_t s = sizeof(V), n = n_tokens * slots;
+    const dim3 grid((uint32_t)ceil_div(n, 4));
+    if (aligned16(grad, ldg * s) && aligned16(rows, ldr * s) && aligned16(grad_rows, width * s))
+      hipLaunchKernelGGL((expert_combine_grad_kernel<V, true>), grid, dim3(256), 0, stream, (const V*)grad, ldg,
+                         (const V*)rows, ldr, n, slots, width, inverse, offsets + n_experts, (const A*)weights,
+                         (V*)grad_rows, (A*)grad_weights);
+    else
+      hipLaunchKernelGGL((expert_combine_grad_kernel<V, false>), grid, dim3(256), 0, stream, (const V*)grad, ldg,
+                         (const V*)rows, ldr, n, slots, width, inverse, offsets + n_experts, (const A*)weights,
+                         (V*)grad_rows, (A*)grad_weights);
+    FS_CHECK_MAIN_LAUNCH("expert_combine_grad_kernel");
+    return FS_OK;
+  });
+}

@@ -1,0 +1,315 @@
+// select_sort.hip — positions sorted by a small key: the transpose of a
+// selection matrix (one entry a row, in column ids[i]).
+//
+// order lists the positions 0..n-1 by key, equal keys in position order;
+// inverse is its inverse.  The key of an id outside [0, n_keys) is n_keys, so
+// such positions come last.  A token's experts and a batch's tokens are sorted
+// by this one routine (expert order; the embedding gradient's segments).
+//
+// Counting sort, least significant digit first: up to 10 key bits a pass, one
+// pass for experts, two for a vocabulary.  A pass is a count (digits of each
+// tile of 4096 positions) and a scatter, which ranks its tile stably: a wave
+// takes 64 positions at a time, the lanes with its digit found by ballots, and
+// waves own consecutive sub-tiles, so ranks need no order of atomics.  One tile
+// counts for itself and is one launch a pass.
+#include "fs_common.hpp"
+#include "radix_tile.hpp"
+
+namespace fs {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / 64;
+constexpr int kChunks = 8;
+constexpr int kSub = 64 * kChunks;
+constexpr int kTile = kWaves * kSub;
+constexpr int kMaxBits = 10;
+constexpr int kMaxDigits = 1 << kMaxBits;
+// Up to this many tiles a scatter adds up the counts of the tiles before it
+// itself (reads all counts, 4 nd bytes a tile); more are scanned by launches.
+constexpr int64_t kSelfScanTiles = 512;
+
+template <class Id>
+__device__ inline uint32_t key_of(Id id, uint32_t n_keys) {
+  // (a negative id is a large unsigned one)
+  return sizeof(Id) == 8 ? ((uint64_t)id < n_keys ? (uint32_t)id : n_keys)
+                         : ((uint32_t)id < n_keys ? (uint32_t)id : n_keys);
+}
+
+// Keys from the ids themselves (KEYS = false) or from an earlier pass.
+template <class Id, bool KEYS>
+__device__ inline uint32_t load_key(const void* __restrict__ src, int64_t i, uint32_t n_keys) {
+  if constexpr (KEYS) return static_cast<const uint32_t*>(src)[i];
+  else return key_of(static_cast<const Id*>(src)[i], n_keys);
+}
+
+template <class Id, bool KEYS>
+__global__ __launch_bounds__(kThreads) void select_count_kernel(const void* __restrict__ src, int64_t n,
+                                                                uint32_t n_keys, int shift, int nd,
+                                                                uint32_t* __restrict__ cnt) {
+  __shared__ uint32_t s_cnt[kMaxDigits];
+  for (int d = threadIdx.x; d < nd; d += kThreads) s_cnt[d] = 0u;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * kTile;
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
+    const int64_t i = base + c * kThreads + threadIdx.x;
+    if (i < n) atomicAdd(&s_cnt[(load_key<Id, KEYS>(src, i, n_keys) >> shift) & (uint32_t)(nd - 1)], 1u);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < nd; d += kThreads) cnt[(int64_t)blockIdx.x * nd + d] = s_cnt[d];
+}
+
+// mode 0: one tile; 1: the tiles before this one are added up here; 2: cnt
+// holds each tile's first place per digit.  LAST: writes order, inverse and
+// offsets, where asked for, besides the sorted keys.
+template <class Id, bool KEYS>
+__global__ __launch_bounds__(kThreads) void select_scatter_kernel(
+    const void* __restrict__ src, const int32_t* __restrict__ pos_in, int64_t n, uint32_t n_keys, int shift, int nd,
+    const uint32_t* __restrict__ cnt, int64_t n_tiles, int mode, uint32_t* __restrict__ keys_out,
+    int32_t* __restrict__ pos_out, int32_t* __restrict__ inverse, int32_t* __restrict__ offsets) {
+  __shared__ uint32_t s_cnt[kWaves][kMaxDigits];
+  __shared__ uint32_t s_base[kMaxDigits];
+  __shared__ uint32_t s_part[2 * kThreads];
+  __shared__ int64_t s_wave[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int64_t tile = blockIdx.x;
+  const int64_t first = tile * kTile + w * kSub + lane;
+  for (int d = tid; d < nd; d += kThreads)
+    for (int k = 0; k < kWaves; ++k) s_cnt[k][d] = 0u;
+
+  uint32_t key[kChunks];
+  int32_t pos[kChunks];
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
+    const int64_t i = first + c * 64;
+    key[c] = i < n ? load_key<Id, KEYS>(src, i, n_keys) : 0u;
+    pos[c] = pos_in != nullptr && i < n ? pos_in[i] : (int32_t)i;
+  }
+  __syncthreads();
+  uint32_t rank[kChunks];
+  const uint32_t mask = (uint32_t)(nd - 1);
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
+    const bool active = first + c * 64 < n;
+    const uint32_t digit = (key[c] >> shift) & mask;
+    const uint64_t peers = match_lanes<kMaxBits>(digit, __ballot(active), mask);
+    const int below = count_below_t(peers);
+    uint32_t before = 0u;
+    if (active) before = s_cnt[w][digit];
+    wave_sync_t();
+    if (active && below == 0) s_cnt[w][digit] = before + (uint32_t)__popcll(peers);
+    wave_sync_t();
+    rank[c] = before + (uint32_t)below;
+  }
+  __syncthreads();
+  // counts of the waves -> places within the tile's run of each digit, and the
+  // first place of the run
+  for (int d = tid; d < nd; d += kThreads) {
+    uint32_t run = 0u;
+    for (int k = 0; k < kWaves; ++k) {
+      const uint32_t v = s_cnt[k][d];
+      s_cnt[k][d] = run;
+      run += v;
+    }
+    s_base[d] = run;
+  }
+  if (mode == 2) {
+    __syncthreads();
+    for (int d = tid; d < nd; d += kThreads) s_base[d] = cnt[tile * nd + d];
+  } else {
+    // per digit: all tiles' count (tot) and that of the tiles before (pre)
+    uint32_t tot[kMaxDigits / kThreads + 1], pre[kMaxDigits / kThreads + 1];
+    const int per = nd > kThreads ? nd / kThreads : 1;
+    if (mode == 1) {
+      const int groups = nd < kThreads ? kThreads / nd : 1;
+      for (int j = 0; j < per; ++j) {
+        const int d = nd < kThreads ? tid % nd : tid * per + j;
+        uint32_t a = 0u, b = 0u;
+#pragma unroll 8
+        for (int64_t t = nd < kThreads ? tid / nd : 0; t < n_tiles; t += groups) {
+          const uint32_t v = cnt[t * nd + d];
+          a += v;
+          b += t < tile ? v : 0u;
+        }
+        tot[j] = a;
+        pre[j] = b;
+      }
+      if (groups > 1) {
+        s_part[tid] = tot[0];
+        s_part[kThreads + tid] = pre[0];
+        __syncthreads();
+        if (tid < nd)
+          for (int g = 1; g < groups; ++g) {
+            tot[0] += s_part[g * nd + tid];
+            pre[0] += s_part[kThreads + g * nd + tid];
+          }
+      }
+    } else {
+      __syncthreads();
+      for (int j = 0; j < per; ++j) {
+        const int d = tid * per + j;
+        tot[j] = d < nd ? s_base[d] : 0u;
+        pre[j] = 0u;
+      }
+    }
+    int64_t mine = 0, all;
+    if (tid * per < nd)
+      for (int j = 0; j < per; ++j) mine += tot[j];
+    uint32_t run = (uint32_t)block_exclusive_scan(mine, s_wave, all);
+    if (tid * per < nd)
+      for (int j = 0; j < per; ++j) {
+        s_base[tid * per + j] = run + pre[j];
+        // one pass: the digit is the key
+        if (offsets != nullptr && tile == 0 && (uint32_t)(tid * per + j) <= n_keys) offsets[tid * per + j] = (int32_t)run;
+        run += tot[j];
+      }
+  }
+  __syncthreads();
+  if (mode == 2 && offsets != nullptr && tile == 0)
+    for (uint32_t d = tid; d <= n_keys; d += kThreads) offsets[d] = (int32_t)s_base[d];
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
+    const int64_t i = first + c * 64;
+    if (i >= n) continue;
+    const uint32_t digit = (key[c] >> shift) & mask;
+    const uint32_t at = s_base[digit] + s_cnt[w][digit] + rank[c];
+    if (keys_out != nullptr) keys_out[at] = key[c];
+    if (pos_out != nullptr) pos_out[at] = pos[c];
+    if (inverse != nullptr) inverse[pos[c]] = (int32_t)at;
+  }
+}
+
+// Passes over keys 0..n_keys: equal shares of their bits.
+struct Passes {
+  int count, bits;
+};
+Passes passes_of(int64_t n_keys) {
+  int bits = 1;
+  while (bits < 32 && (n_keys >> bits) != 0) ++bits;
+  const int count = (bits + kMaxBits - 1) / kMaxBits;
+  return {count, (bits + count - 1) / count};
+}
+
+struct SortLayout {
+  size_t cnt, partial, totals, keys[2], pos[2], bytes;
+};
+SortLayout sort_layout(int64_t n, int64_t n_keys) {
+  const Passes p = passes_of(n_keys);
+  const int64_t tiles = ceil_div(n, kTile), nd = (int64_t)1 << p.bits;
+  SortLayout l{};
+  size_t at = 0;
+  auto take = [&](size_t b) {
+    const size_t a = at;
+    at += (b + 255) / 256 * 256;
+    return a;
+  };
+  if (tiles > 1) l.cnt = take((size_t)(tiles * nd) * 4);
+  if (tiles > kSelfScanTiles) {
+    l.partial = take((size_t)(ceil_div(tiles, kWgScanTiles) * nd) * 4);
+    l.totals = take((size_t)nd * 4);
+  }
+  // passes before the last write keys and positions, in turn
+  for (int k = 0; k < 2 && k + 1 < p.count; ++k) {
+    l.keys[k] = take((size_t)n * 4);
+    l.pos[k] = take((size_t)n * 4);
+  }
+  l.bytes = at;
+  return l;
+}
+
+template <class Id, bool KEYS>
+int sort_pass(const void* src, const int32_t* pos_in, int64_t n, uint32_t n_keys, int shift, int nd, uint8_t* ws,
+              const SortLayout& l, uint32_t* keys_out, int32_t* pos_out, int32_t* inverse, int32_t* offsets,
+              hipStream_t s) {
+  const int64_t tiles = ceil_div(n, kTile);
+  uint32_t* cnt = reinterpret_cast<uint32_t*>(ws + l.cnt);
+  int mode = 0;
+  if (tiles > 1) {
+    hipLaunchKernelGGL((select_count_kernel<Id, KEYS>), dim3((uint32_t)tiles), dim3(kThreads), 0, s, src, n, n_keys,
+                       shift, nd, cnt);
+    FS_CHECK_LAUNCH("select_count_kernel");
+    mode = 1;
+    if (tiles > kSelfScanTiles) {
+      mode = 2;
+      uint32_t* partial = reinterpret_cast<uint32_t*>(ws + l.partial);
+      uint32_t* totals = reinterpret_cast<uint32_t*>(ws + l.totals);
+      const int64_t blocks = ceil_div(tiles, kWgScanTiles);
+      hipLaunchKernelGGL(wg_scan_reduce_kernel, dim3((uint32_t)blocks), dim3(256), 0, s, cnt, tiles, nd, partial);
+      FS_CHECK_LAUNCH("wg_scan_reduce_kernel");
+      hipLaunchKernelGGL(wg_scan_column_kernel, dim3((uint32_t)nd), dim3(256), 0, s, partial, blocks, nd, totals);
+      FS_CHECK_LAUNCH("wg_scan_column_kernel");
+      hipLaunchKernelGGL(wg_scan_down_kernel, dim3((uint32_t)blocks), dim3(256), 0, s, cnt, tiles, nd, partial, totals);
+      FS_CHECK_LAUNCH("wg_scan_down_kernel");
+    }
+  }
+  hipLaunchKernelGGL((select_scatter_kernel<Id, KEYS>), dim3((uint32_t)tiles), dim3(kThreads), 0, s, src, pos_in, n,
+                     n_keys, shift, nd, cnt, tiles, mode, keys_out, pos_out, inverse, offsets);
+  FS_CHECK_MAIN_LAUNCH("select_scatter_kernel");
+  return FS_OK;
+}
+
+__global__ __launch_bounds__(256) void zero_offsets_kernel(int32_t* __restrict__ p, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = 0;
+}
+
+}  // namespace
+
+size_t select_sort_bytes(int64_t n, int64_t n_keys) { return n > 0 ? sort_layout(n, n_keys).bytes : 0; }
+
+// keys_out, inverse and offsets may be null; offsets needs one pass.
+int select_sort(const void* ids, int id_t, int64_t n, int64_t n_keys, uint32_t* keys_out, int32_t* order,
+                int32_t* inverse, int32_t* offsets, uint8_t* ws, hipStream_t s) {
+  if (n == 0) {
+    if (offsets != nullptr) {
+      hipLaunchKernelGGL(zero_offsets_kernel, dim3((uint32_t)ceil_div(n_keys + 1, 256)), dim3(256), 0, s, offsets,
+                         n_keys + 1);
+      FS_CHECK_LAUNCH("zero_offsets_kernel");
+    }
+    return FS_OK;
+  }
+  const Passes p = passes_of(n_keys);
+  const SortLayout l = sort_layout(n, n_keys);
+  const int nd = 1 << p.bits;
+  const void* src = ids;
+  const int32_t* pos = nullptr;
+  for (int k = 0; k < p.count; ++k) {
+    const bool last = k + 1 == p.count;
+    uint32_t* ko = last ? keys_out : reinterpret_cast<uint32_t*>(ws + l.keys[k & 1]);
+    int32_t* po = last ? order : reinterpret_cast<int32_t*>(ws + l.pos[k & 1]);
+    int32_t* inv = last ? inverse : nullptr;
+    int rc;
+    if (k > 0) rc = sort_pass<int32_t, true>(src, pos, n, (uint32_t)n_keys, k * p.bits, nd, ws, l, ko, po, inv, offsets, s);
+    else if (id_t == FS_I64) rc = sort_pass<int64_t, false>(src, pos, n, (uint32_t)n_keys, 0, nd, ws, l, ko, po, inv, offsets, s);
+    else rc = sort_pass<int32_t, false>(src, pos, n, (uint32_t)n_keys, 0, nd, ws, l, ko, po, inv, offsets, s);
+    if (rc != FS_OK) return rc;
+    src = ko;
+    pos = po;
+  }
+  return FS_OK;
+}
+
+int select_max_one_pass_keys() { return kMaxDigits - 1; }
+
+}  // namespace fs
+
+extern "C" size_t fs_expert_route_workspace_bytes(int64_t n, int64_t n_experts) {
+  if (n <= 0 || n > INT32_MAX || n_experts < 1 || n_experts > fs::select_max_one_pass_keys()) return 0;
+  return fs::select_sort_bytes(n, n_experts);
+}
+
+extern "C" int fs_expert_route(int id_t, int64_t n, int64_t n_experts, const void* experts, int32_t* order,
+                               int32_t* inverse, int32_t* offsets, void* ws, size_t ws_bytes, hipStream_t stream) {
+  if (id_t != FS_I32 && id_t != FS_I64) return fs::fail(FS_E_INVALID, "fs_expert_route: bad type code");
+  if (n < 0 || n > INT32_MAX) return fs::fail(FS_E_INVALID, "fs_expert_route: slots out of range");
+  if (n_experts < 1 || n_experts > fs::select_max_one_pass_keys())
+    return fs::fail(FS_E_INVALID, "fs_expert_route: n_experts out of range");
+  if (offsets == nullptr || (n > 0 && (experts == nullptr || order == nullptr || inverse == nullptr)))
+    return fs::fail(FS_E_INVALID, "fs_expert_route: null pointer");
+  const size_t need = fs_expert_route_workspace_bytes(n, n_experts);
+  if (need > 0 && (ws == nullptr || ws_bytes < need))
+    return fs::fail(FS_E_WORKSPACE, "fs_expert_route: workspace too small");
+  return fs::select_sort(experts, id_t, n, n_experts, nullptr, order, inverse, offsets, static_cast<uint8_t*>(ws),
+                         stream);
+}

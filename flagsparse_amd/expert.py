@@ -1,0 +1,268 @@
+"""Tokens routed to experts: rows sorted by expert, the experts' products, and
+the rows back with weights applied, each with its gradient.
+
+``prepare_expert_route`` sorts the slots of T tokens, k slots a token, by the
+expert each names; equal experts keep slot order.  A slot whose expert is
+outside [0, num_experts) belongs to none (over capacity, or an expert that
+another process holds: subtract the first expert held here): its place is
+behind all others, its row is zero and it adds nothing to a token.  Places run
+from 0 to T k whatever the experts are, so no shape depends on the data and
+nothing synchronises.
+
+    dispatch   rows[inverse[t, j]] = x[t]
+    product    y[r] = rows[r] op(W[e]), e the expert of place r
+    combine    out[t] = sum_j weights[t, j] y[inverse[t, j]]
+
+Products with the routing matrix, with a block-diagonal matrix and with the
+routing matrix's transpose (csrc/select_sort.hip, expert_rows.hip,
+expert_product.hip).  Values: float16, bfloat16, float32 (float64 too but for
+the product); sums run in 32 bits (64 for float64), in a fixed order, and are
+rounded once.  Routing weights are float32 (float64 with float64 rows).
+
+The reference has no counterpart; names, checks and errors follow its other
+operators (sparse_operations/spmm_coo.py:335-395, 619-625).
+"""
+
+import torch
+
+from . import _lib
+from ._common import _INDEX_LIMIT_INT32, SUPPORTED_INDEX_DTYPES
+from ._rows import ROW_DTYPE_MESSAGE, ROW_VALUE_CODES, check_out, row_major, wants_grad
+
+MAX_EXPERTS = 1023
+
+
+class PreparedExpertRoute:
+    """Slots of tokens sorted by expert (``prepare_expert_route``).
+
+    order     int32 (T k,): slot t k + j at each place
+    inverse   int32 (T, k): place of each slot
+    offsets   int32 (num_experts + 1,): first place of each expert; the last is
+              the number of slots that name one
+    """
+
+    __slots__ = ("n_tokens", "slots", "num_experts", "order", "inverse", "offsets", "device")
+
+    def __init__(self, n_tokens, slots, num_experts, order, inverse, offsets):
+        self.n_tokens, self.slots, self.num_experts = n_tokens, slots, num_experts
+        self.order, self.inverse, self.offsets = order, inverse, offsets
+        self.device = offsets.device
+
+    @property
+    def n_rows(self):
+        return self.n_tokens * self.slots
+
+
+def prepare_expert_route(experts, num_experts):
+    """Sort the slots of ``experts``, (T, k) int32 or int64, by expert."""
+    if not isinstance(experts, torch.Tensor):
+        raise TypeError("experts must be a torch.Tensor")
+    if experts.ndim != 2:
+        raise ValueError("experts must be a 2D tensor: (tokens, slots)")
+    if experts.dtype not in SUPPORTED_INDEX_DTYPES:
+        raise TypeError("experts dtype must be torch.int32 or torch.int64")
+    if not experts.is_cuda:
+        raise ValueError("experts must be a CUDA tensor")
+    num_experts = int(num_experts)
+    if not 1 <= num_experts <= MAX_EXPERTS:
+        raise ValueError(f"num_experts must be in 1..{MAX_EXPERTS}, got {num_experts}")
+    n_tokens, slots = experts.shape
+    if slots < 1:
+        raise ValueError("experts must have at least one slot a token")
+    n = n_tokens * slots
+    if n > _INDEX_LIMIT_INT32:
+        raise ValueError("tokens * slots exceeds the int32 range")
+    experts = experts.contiguous()
+    device = experts.device
+    # one allocation for the three: the smallest calls are what it costs to make them
+    buf = torch.empty(2 * n + num_experts + 1, dtype=torch.int32, device=device)
+    order, inverse, offsets = buf[:n], buf[n : 2 * n].view(n_tokens, slots), buf[2 * n :]
+    lib = _lib.lib()
+    need = lib.fs_expert_route_workspace_bytes(n, num_experts)
+    ws = _lib.workspace(need, device) if need else None
+    _lib.check(
+        lib.fs_expert_route(_lib.INDEX_TYPE_CODES[experts.dtype], n, num_experts, _lib.ptr(experts), _lib.ptr(order),
+                            _lib.ptr(inverse), _lib.ptr(offsets), _lib.ptr(ws), need, _lib.stream_handle(device)),
+        "fs_expert_route",
+    )
+    return PreparedExpertRoute(n_tokens, slots, num_experts, order, inverse, offsets)
+
+
+def _check_rows(rows, what, route, n_rows):
+    if not isinstance(route, PreparedExpertRoute):
+        raise TypeError("route must be a PreparedExpertRoute")
+    if not isinstance(rows, torch.Tensor):
+        raise TypeError(f"{what} must be a torch.Tensor")
+    if rows.dtype not in ROW_VALUE_CODES:
+        raise TypeError(f"{what} dtype must be one of: {ROW_DTYPE_MESSAGE}")
+    if not rows.is_cuda:
+        raise ValueError(f"{what} must be a CUDA tensor")
+    if rows.device != route.device:
+        raise ValueError(f"{what} must be on the same CUDA device as the route")
+    if rows.ndim != 2 or rows.shape[0] != n_rows:
+        raise ValueError(f"{what} must be a 2D tensor with {n_rows} rows, got shape {tuple(rows.shape)}")
+
+
+def _check_weights(weights, rows, route):
+    wide = torch.float64 if rows.dtype == torch.float64 else torch.float32
+    if not isinstance(weights, torch.Tensor):
+        raise TypeError("weights must be a torch.Tensor")
+    if weights.dtype != wide:
+        raise TypeError(f"weights dtype must be {wide} for {rows.dtype} rows")
+    if weights.device != route.device:
+        raise ValueError("weights must be on the same CUDA device as the route")
+    if tuple(weights.shape) != (route.n_tokens, route.slots):
+        raise ValueError(f"weights must have shape {(route.n_tokens, route.slots)}, got {tuple(weights.shape)}")
+
+
+def _into(out, shape, like):
+    """The tensor to write: out itself where it is contiguous."""
+    if out is not None and out.is_contiguous():
+        return out
+    return torch.empty(shape, dtype=like.dtype, device=like.device)
+
+
+def _done(out, result):
+    if out is not None and result is not out:
+        out.copy_(result)
+        return out
+    return result
+
+
+def _dispatch(x, route, out=None):
+    x, ld = row_major(x)
+    result = _into(out, (route.n_rows, x.shape[1]), x)
+    _lib.check(
+        _lib.lib().fs_expert_dispatch(ROW_VALUE_CODES[x.dtype], route.n_tokens, route.slots, x.shape[1],
+                                      route.num_experts, _lib.ptr(x), ld, _lib.ptr(route.inverse),
+                                      _lib.ptr(route.offsets), _lib.ptr(result), _lib.stream_handle(x.device)),
+        "fs_expert_dispatch",
+    )
+    return _done(out, result)
+
+
+def _combine(rows, route, weights, out=None):
+    rows, ld = row_major(rows)
+    weights = None if weights is None else weights.contiguous()
+    result = _into(out, (route.n_tokens, rows.shape[1]), rows)
+    _lib.check(
+        _lib.lib().fs_expert_combine(ROW_VALUE_CODES[rows.dtype], route.n_tokens, route.slots, rows.shape[1],
+                                     route.num_experts, _lib.ptr(rows), ld, _lib.ptr(route.inverse),
+                                     _lib.ptr(route.offsets), _lib.ptr(weights), _lib.ptr(result),
+                                     _lib.stream_handle(rows.device)),
+        "fs_expert_combine",
+    )
+    return _done(out, result)
+
+
+class _Dispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, route):
+        ctx.route = route
+        return _dispatch(x, route)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return _combine(grad, ctx.route, None), None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, route, weights):
+        ctx.route = route
+        ctx.save_for_backward(rows, weights)
+        return _combine(rows, route, weights)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        rows, weights = ctx.saved_tensors
+        if weights is None:
+            return _dispatch(grad, ctx.route), None, None
+        grad_rows, grad_weights = flagsparse_expert_combine_grad(grad, rows, ctx.route, weights)
+        return grad_rows, None, grad_weights
+
+
+def flagsparse_expert_dispatch(x, route, out=None):
+    """Rows of ``x``, (T, width), in expert order: (T k, width).
+
+    Differentiable in ``x``.
+    """
+    n_tokens = route.n_tokens if isinstance(route, PreparedExpertRoute) else 0
+    _check_rows(x, "x", route, n_tokens)
+    if wants_grad(x):
+        if out is not None:
+            raise ValueError("out cannot be given where a gradient is recorded")
+        return _Dispatch.apply(x, route)
+    if out is not None:
+        check_out(out, x.device, (route.n_rows, x.shape[1]), x.dtype)
+    return _dispatch(x, route, out)
+
+
+def flagsparse_expert_dispatch_grad(grad, route, out=None):
+    """Gradient of ``flagsparse_expert_dispatch`` in x: a token's routed rows of ``grad`` summed, (T, width)."""
+    n_rows = route.n_rows if isinstance(route, PreparedExpertRoute) else 0
+    _check_rows(grad, "grad", route, n_rows)
+    if out is not None:
+        check_out(out, grad.device, (route.n_tokens, grad.shape[1]), grad.dtype)
+    return _combine(grad, route, None, out)
+
+
+def flagsparse_expert_combine(rows, route, weights=None, out=None):
+    """Tokens' rows back from expert order, weighted and summed: (T, width).
+
+    rows is (T k, width), weights (T, k), or None for ones.  Differentiable in
+    both.
+    """
+    n_rows = route.n_rows if isinstance(route, PreparedExpertRoute) else 0
+    _check_rows(rows, "rows", route, n_rows)
+    if weights is not None:
+        _check_weights(weights, rows, route)
+    if wants_grad(rows, weights):
+        if out is not None:
+            raise ValueError("out cannot be given where a gradient is recorded")
+        return _Combine.apply(rows, route, weights)
+    if out is not None:
+        check_out(out, rows.device, (route.n_tokens, rows.shape[1]), rows.dtype)
+    return _combine(rows, route, weights, out)
+
+
+def flagsparse_expert_combine_grad(grad, rows, route, weights):
+    """Gradients of ``flagsparse_expert_combine`` in its rows and weights, in one pass.
+
+    grad is (T, width).  Slots of no expert get zeros in both.
+    """
+    n_rows = route.n_rows if isinstance(route, PreparedExpertRoute) else 0
+    _check_rows(rows, "rows", route, n_rows)
+    _check_rows(grad, "grad", route, route.n_tokens)
+    if grad.dtype != rows.dtype:
+        raise TypeError("grad dtype must match rows dtype")
+    if grad.shape[1] != rows.shape[1]:
+        raise ValueError(f"grad must have width {rows.shape[1]}, got {grad.shape[1]}")
+    _check_weights(weights, rows, route)
+    grad, ldg = row_major(grad)
+    rows, ldr = row_major(rows)
+    weights = weights.contiguous()
+    grad_rows = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
+    grad_weights = torch.empty_like(weights)
+    _lib.check(
+        _lib.lib().fs_expert_combine_grad(ROW_VALUE_CODES[rows.dtype], route.n_tokens, route.slots, rows.shape[1],
+                                          route.num_experts, _lib.ptr(grad), ldg, _lib.ptr(rows), ldr,
+                                          _lib.ptr(route.inverse), _lib.ptr(route.offsets), _lib.ptr(weights),
+                                          _lib.ptr(grad_rows), _lib.ptr(grad_weights),
+                                          _lib.stream_handle(rows.device)),
+        "fs_expert_combine_grad",
+    )
+    return grad_rows, grad_weights
+
+
+__all__ = [
+    "MAX_EXPERTS",
+    "PreparedExpertRoute",
+    "prepare_expert_route",
+    "flagsparse_expert_dispatch",
+    "flagsparse_expert_dispatch_grad",
+    "flagsparse_expert_combine",
+    "flagsparse_expert_combine_grad",
+]

@@ -573,6 +573,63 @@ int fs_spmv_sell(int val_t, int sell_idx_t, int ptr_t, int layout, int64_t n_row
                  const int32_t* code_table, const int64_t* slice_ptr,
                  const void* indptr, const void* x, void* y, hipStream_t stream);
 
+/* ---- products with selection matrices (rows moved, never multiplied out) ----
+ *
+ * The reference has no counterpart of the entry points below.  Their value
+ * types are FS_F16, FS_BF16, FS_F32 and FS_F64; sums run in 32 bits (64 for
+ * FS_F64) in a fixed order and are rounded once.  Rows are contiguous; ld*
+ * is the distance between rows in elements, results are dense.  Nothing
+ * synchronises.
+ */
+
+/*
+ * Embedding lookup: out[t] = scale * table[ids[t]] for n ids (id_t FS_I32 /
+ * FS_I64) and a table of n_rows rows; a zero row for ids outside it.
+ */
+int fs_embedding(int val_t, int id_t, int64_t n, int64_t n_rows, int64_t width,
+                 const void* table, int64_t ldt, const void* ids, double scale,
+                 void* out, hipStream_t stream);
+/*
+ * Its gradient: out[v] = scale * (sum of grad[t] over ids[t] == v, in order of
+ * t), every row of out written; row `padding` (-1: none) is zero.  out_t is
+ * val_t, or FS_F32 for 16-bit values.
+ */
+size_t fs_embedding_grad_workspace_bytes(int val_t, int64_t n, int64_t n_rows, int64_t width);
+int fs_embedding_grad(int val_t, int out_t, int id_t, int64_t n, int64_t n_rows, int64_t width,
+                      const void* grad, int64_t ldg, const void* ids, double scale,
+                      int64_t padding, void* out, void* ws, size_t ws_bytes, hipStream_t stream);
+
+/*
+ * Slots sorted by expert: experts holds n ids; order lists the slots by expert
+ * (equal experts in slot order, ids outside [0, n_experts) last), inverse gives
+ * each slot's place and offsets[0..n_experts] the experts' first places, the
+ * last the number of slots that name an expert.  1 <= n_experts <= 1023.
+ */
+size_t fs_expert_route_workspace_bytes(int64_t n, int64_t n_experts);
+int fs_expert_route(int id_t, int64_t n, int64_t n_experts, const void* experts, int32_t* order,
+                    int32_t* inverse, int32_t* offsets, void* ws, size_t ws_bytes, hipStream_t stream);
+/*
+ * Rows into expert order and back; inverse (n_tokens x slots) and offsets are
+ * fs_expert_route's.  weights and grad_weights (n_tokens x slots) are float,
+ * double with FS_F64.
+ *   dispatch      out[inverse[t, j]] = x[t]; zero rows for slots of no expert
+ *   combine       out[t] = sum over j of weights[t, j] rows[inverse[t, j]], slots
+ *                 of no expert left out; weights may be null (ones)
+ *   combine_grad  grad_rows[inverse[t, j]] = weights[t, j] grad[t] and
+ *                 grad_weights[t, j] = <grad[t], rows[inverse[t, j]]>; zeros for
+ *                 slots of no expert
+ */
+int fs_expert_dispatch(int val_t, int64_t n_tokens, int slots, int64_t width, int64_t n_experts,
+                       const void* x, int64_t ldx, const int32_t* inverse, const int32_t* offsets,
+                       void* out, hipStream_t stream);
+int fs_expert_combine(int val_t, int64_t n_tokens, int slots, int64_t width, int64_t n_experts,
+                      const void* rows, int64_t ldr, const int32_t* inverse, const int32_t* offsets,
+                      const void* weights, void* out, hipStream_t stream);
+int fs_expert_combine_grad(int val_t, int64_t n_tokens, int slots, int64_t width, int64_t n_experts,
+                           const void* grad, int64_t ldg, const void* rows, int64_t ldr,
+                           const int32_t* inverse, const int32_t* offsets, const void* weights,
+                           void* grad_rows, void* grad_weights, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
