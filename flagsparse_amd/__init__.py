@@ -75,6 +75,8 @@ from .expert import (
     flagsparse_expert_combine_grad,
     flagsparse_expert_dispatch,
     flagsparse_expert_dispatch_grad,
+    flagsparse_expert_product,
+    flagsparse_expert_product_grad,
     prepare_expert_route,
 )
 
@@ -139,4 +141,6 @@ __all__ = [
     "flagsparse_expert_dispatch_grad",
     "flagsparse_expert_combine",
     "flagsparse_expert_combine_grad",
+    "flagsparse_expert_product",
+    "flagsparse_expert_product_grad",
 ]

@@ -23,7 +23,8 @@ OUT = os.path.join(PKG, "libflagsparse_hip.so")
 BUILD_DIR = os.path.join(HERE, "_build")
 
 SOURCES = ["abi.cpp", "spmv.hip", "spmv_opt.hip", "spmv_scatter.hip", "spmv_gather.hip", "spmm.hip", "spmm_group.hip",
-           "spmm_half.hip", "transpose.hip", "sell.hip", "select_sort.hip", "embedding.hip", "expert_rows.hip"]
+           "spmm_half.hip", "transpose.hip", "sell.hip", "select_sort.hip", "embedding.hip", "expert_rows.hip",
+           "expert_product.hip"]
 # the measurement-only library (bench.py --gather-floor), with its own copy of
 # the error reporting
 DIAG_OUT = os.path.join(PKG, "libflagsparse_diag.so")

@@ -1,0 +1,415 @@
+// expert_product.hip — the experts' products on matrix cores.
+//
+// Rows of expert order, a block of consecutive rows an expert (offsets, from
+// fs_expert_route), times the expert's matrix: a block-diagonal product.
+//   rows    C[r, n] = sum_k A[r, k] B_e(k, n), e the expert of row r, with
+//           B_e stored (N, K) ("trans", k contiguous) or (K, N) ("non")
+//   matrix  C_e[m, n] = sum over the rows r of e of A[r, m] B[r, n], the
+//           gradient of the matrices
+// Rows of no expert (from offsets[n_experts] on) are written as zeros.
+//
+// A workgroup computes one BM x BN tile of one expert, 128 bytes of k at a
+// time: both operands' slices go to LDS, 16-byte pieces exchanged within a row
+// so that fragment reads meet no bank twice, double buffered, and feed 16x16
+// matrix instructions that accumulate in 32 bits.  Results are rounded once.
+// Where an operand is contiguous in k a fragment is one 16-byte LDS read; where
+// it is contiguous along the tile, 16-bit fragments are transposed by the LDS
+// read itself and 32-bit ones are read element by element.
+// How many rows an expert has is known on the device only: the grid is an upper
+// bound, each workgroup finds its tile from the offsets, and those beyond the
+// last tile leave.
+#include <type_traits>
+
+#include "select_rows.hpp"
+
+namespace fs {
+namespace {
+
+constexpr int kRowBytes = 128;  // k of one step, of an operand contiguous in k
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) uint8_t lds_byte;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) float lds_float;
+
+template <class T>
+struct Mma;
+template <>
+struct Mma<_Float16> {
+  using frag = f16x8;
+  __device__ static f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Mma<__bf16> {
+  using frag = bf16x8;
+  __device__ static f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Mma<float> {
+  using frag = f32x4;  // four steps of one k a lane
+  __device__ static f32x4 run(frag a, frag b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// One operand's slice in LDS, and the way there.  KC: contiguous in k, R rows
+// of the tile by 128 bytes of k; otherwise BK rows of k by R elements.
+template <class T, bool KC, int R, int THREADS>
+struct Operand {
+  static constexpr int E = 16 / (int)sizeof(T);        // elements a piece
+  static constexpr int BK = kRowBytes / (int)sizeof(T);
+  static constexpr int kBytes = R * kRowBytes;
+  static constexpr int kPieces = kBytes / 16 / THREADS;  // a thread's, each step
+  static constexpr int kPerRow = KC ? 8 : R * (int)sizeof(T) / 16;
+  static_assert(kBytes % (16 * THREADS) == 0, "whole pieces a thread");
+
+  // Exchange of the pieces of LDS row `row`.
+  __device__ static int swizzle(int row) {
+    if constexpr (KC) return row & 7;
+    else if constexpr (sizeof(T) == 4) return ((row >> 2) & 1) * 4;
+    else return ((row & 3) + (kPerRow >= 16 ? ((row >> 3) & 1) * 4 : 0)) * 2;
+  }
+  __device__ static int row_of(int i, int tid) { return (i * THREADS + tid) / kPerRow; }
+  __device__ static int piece_of(int i, int tid) {
+    return ((i * THREADS + tid) % kPerRow) ^ swizzle(row_of(i, tid));
+  }
+
+  // Fragment of 16 tile rows (from j * 16 past the wave's first) and the kk-th
+  // half of the step's k: lane l has tile row l % 16, k piece l / 16.
+  __device__ static uint32_t frag_offset(int r0, int lane) {
+    const int g = lane >> 4, i = lane & 15;
+    if constexpr (KC) {
+      return (uint32_t)((r0 + i) * kRowBytes + ((g ^ (i & 7)) * 16));
+    } else if constexpr (sizeof(T) == 4) {
+      const int row = 4 * g;
+      return (uint32_t)(row * R * 4 + ((r0 / 4 + i / 4) ^ swizzle(row)) * 16 + (i & 3) * 4);
+    } else {
+      const int row = 8 * g + i / 4;
+      return (uint32_t)(row * R * 2 + ((r0 / 8 + (i & 3) / 2) ^ swizzle(row)) * 16 + (i & 1) * 8);
+    }
+  }
+  __device__ static typename Mma<T>::frag frag(uint32_t at, int kk) {
+    typename Mma<T>::frag f;
+    if constexpr (KC) {
+      // (piece g ^ (i & 7) of the first half is piece (g + 4) ^ (i & 7) of the second, 64 bytes away either way)
+      const u32x4 v = *(const lds_u32x4*)(lds_byte*)(uintptr_t)(at ^ (uint32_t)(kk * 64));
+      __builtin_memcpy(&f, &v, 16);
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        f[i] = *(const lds_float*)(lds_byte*)(uintptr_t)(at + (uint32_t)((kk * 16 + i) * R * 4));
+    } else {
+      const uint32_t p = at + (uint32_t)(kk * 32 * R * 2);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_byte*)(uintptr_t)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_byte*)(uintptr_t)(p + 4 * R * 2));
+      __builtin_memcpy(&f, &lo, 8);
+      __builtin_memcpy((char*)&f + 8, &hi, 8);
+    }
+    return f;
+  }
+};
+
+// What one operand's loads need: the tile's first element, the distance of its
+// rows (of the tile if KC, of k otherwise), and how many there are of each.
+template <class T>
+struct Source {
+  const T* base;
+  int64_t ld;
+  int tile_rows;  // tile rows within the operand
+  int64_t k;      // k within it
+};
+
+// A thread's pieces of step kt in registers, zeros outside the operand.
+template <class O, class T, bool KC>
+__device__ inline void load_pieces(const Source<T>& s, int64_t kt, int tid, u32x4 (&r)[O::kPieces]) {
+  constexpr int E = O::E;
+#pragma unroll
+  for (int i = 0; i < O::kPieces; ++i) {
+    const int row = O::row_of(i, tid), piece = O::piece_of(i, tid);
+    const int64_t k0 = kt * O::BK;
+    const int64_t line = KC ? row : k0 + row;                       // row of memory
+    const int64_t first = KC ? k0 + (int64_t)piece * E : piece * E;  // element in it
+    const bool in = KC ? row < s.tile_rows : k0 + row < s.k;
+    const int64_t left = (KC ? s.k : (int64_t)s.tile_rows) - first;
+    const T* p = s.base + line * s.ld + first;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (in && left >= E) {
+      __builtin_memcpy(&v, p, 16);
+    } else if (in && left > 0) {
+      T e[E];
+#pragma unroll
+      for (int q = 0; q < E; ++q) e[q] = q < left ? p[q] : (T)0;
+      __builtin_memcpy(&v, e, 16);
+    }
+    r[i] = v;
+  }
+}
+template <class O>
+__device__ inline void store_pieces(uint32_t lds, int tid, const u32x4 (&r)[O::kPieces], int threads) {
+#pragma unroll
+  for (int i = 0; i < O::kPieces; ++i) *(lds_u32x4*)(lds_byte*)(uintptr_t)(lds + (uint32_t)(i * threads + tid) * 16) = r[i];
+}
+
+struct ProductArgs {
+  const void* a;
+  const void* b;
+  void* c;
+  const int32_t* offsets;
+  int64_t lda, ldb, ldc;   // distances of rows
+  int64_t b_expert, c_expert;  // distances of experts' matrices
+  int64_t n_rows;          // rows of A
+  int64_t m, n, k;         // m: of a matrix gradient; k: of a product of rows
+  int n_experts;
+};
+
+struct TileAt {
+  int expert;  // n_experts: rows of no expert
+  int64_t row0;
+  int rows;
+  int m, n;  // tile within the expert
+};
+
+constexpr int kGroupN = 4;  // neighbouring tiles share 4 column panels
+
+// Tile r of an expert with mt x nt tiles: groups of kGroupN columns, rows first.
+__device__ inline void tile_in_group(uint32_t r, uint32_t mt, uint32_t nt, TileAt& t) {
+  const uint32_t g = r / (mt * kGroupN), left = nt - g * kGroupN, gn = left < kGroupN ? left : kGroupN;
+  const uint32_t q = r - g * mt * kGroupN;
+  t.m = (int)(q / gn);
+  t.n = (int)(g * kGroupN + q % gn);
+}
+
+__device__ inline int wave_scan(int v, int lane) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int u = __shfl_up(v, off);
+    if (lane >= off) v += u;
+  }
+  return v;
+}
+
+// The workgroup's tile of a product of rows, or false.  All waves alike.
+template <int BM>
+__device__ inline bool find_tile(const ProductArgs& p, uint32_t nt, int lane, TileAt& t) {
+  const int E = p.n_experts;
+  auto tiles_of = [&](int e) {
+    if (e > E) return 0;
+    const int64_t a = p.offsets[e], b = e < E ? (int64_t)p.offsets[e + 1] : p.n_rows;
+    return (int)((b - a + BM - 1) / BM);
+  };
+  int total = 0;
+  for (int e = 0; e <= E; e += 64) total += __builtin_amdgcn_readlane(wave_scan(tiles_of(e + lane), lane), 63);
+  const uint32_t all = (uint32_t)total * nt;
+  if (blockIdx.x >= all) return false;
+  const uint32_t id = (uint32_t)xcd_range_block(blockIdx.x, all), q = id / nt;
+  int before = 0;
+  for (int e = 0; e <= E; e += 64) {
+    const int own = tiles_of(e + lane), upto = wave_scan(own, lane) + before;
+    const uint64_t m = __ballot((uint32_t)upto > q);
+    if (m != 0) {
+      const int l = __builtin_ctzll(m);
+      const int mt = __builtin_amdgcn_readlane(own, l), first = __builtin_amdgcn_readlane(upto, l) - mt;
+      t.expert = e + l;
+      tile_in_group(id - (uint32_t)first * nt, (uint32_t)mt, nt, t);
+      const int64_t a = p.offsets[t.expert], b = t.expert < E ? (int64_t)p.offsets[t.expert + 1] : p.n_rows;
+      t.row0 = a + (int64_t)t.m * BM;
+      t.rows = (int)(b - t.row0 < BM ? b - t.row0 : BM);
+      return true;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+enum Mode { kRowsTrans = 0, kRowsNon = 1, kMatrix = 2 };
+
+template <class T, int MODE, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const ProductArgs p) {
+  constexpr int THREADS = 64 * WM * WN;
+  constexpr bool AKC = MODE != kMatrix, BKC = MODE == kRowsTrans;
+  using OA = Operand<T, AKC, BM, THREADS>;
+  using OB = Operand<T, BKC, BN, THREADS>;
+  constexpr int BK = OA::BK;
+  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  __shared__ alignas(1024) uint8_t s_mem[2][OA::kBytes + OB::kBytes];
+
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t nt = (uint32_t)((p.n + BN - 1) / BN);
+  TileAt t;
+  Source<T> sa, sb;
+  T* c;
+  int c_rows;
+  if constexpr (MODE == kMatrix) {
+    const uint32_t mt = (uint32_t)((p.m + BM - 1) / BM), id = (uint32_t)xcd_range_block(blockIdx.x, gridDim.x);
+    t.expert = (int)(id / (mt * nt));
+    tile_in_group(id % (mt * nt), mt, nt, t);
+    const int64_t r0 = p.offsets[t.expert], m0 = (int64_t)t.m * BM;
+    sa.k = sb.k = p.offsets[t.expert + 1] - r0;
+    sa.base = (const T*)p.a + r0 * p.lda + m0;
+    sb.base = (const T*)p.b + r0 * p.ldb;
+    sa.tile_rows = (int)(p.m - m0 < BM ? p.m - m0 : BM);
+    c = (T*)p.c + (int64_t)t.expert * p.c_expert + m0 * p.ldc;
+    c_rows = sa.tile_rows;
+  } else {
+    if (!find_tile<BM>(p, nt, lane, t)) return;
+    sa.k = sb.k = t.expert < p.n_experts ? p.k : 0;
+    sa.base = (const T*)p.a + t.row0 * p.lda;
+    sb.base = (const T*)p.b + (int64_t)t.expert * p.b_expert;
+    sa.tile_rows = c_rows = t.rows;
+    c = (T*)p.c + t.row0 * p.ldc;
+  }
+  const int64_t n0 = (int64_t)t.n * BN;
+  sb.base += BKC ? n0 * p.ldb : n0;
+  sb.tile_rows = (int)(p.n - n0 < BN ? p.n - n0 : BN);
+  sa.ld = p.lda;
+  sb.ld = p.ldb;
+  c += n0;
+
+  const int wm = w / WN, wn = w % WN;
+  const uint32_t lds = (uint32_t)(uintptr_t)(lds_byte*)&s_mem[0][0];
+  uint32_t at_a[FM], at_b[FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i) at_a[i] = OA::frag_offset(wm * (BM / WM) + i * 16, lane);
+#pragma unroll
+  for (int j = 0; j < FN; ++j) at_b[j] = OB::frag_offset(wn * (BN / WN) + j * 16, lane) + OA::kBytes;
+
+  f32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const int64_t steps = (sa.k + BK - 1) / BK;
+  u32x4 ra[OA::kPieces], rb[OB::kPieces];
+  if (steps > 0) {
+    load_pieces<OA, T, AKC>(sa, 0, tid, ra);
+    load_pieces<OB, T, BKC>(sb, 0, tid, rb);
+  }
+  for (int64_t kt = 0; kt < steps; ++kt) {
+    const uint32_t buf = lds + (uint32_t)(kt & 1) * (OA::kBytes + OB::kBytes);
+    store_pieces<OA>(buf, tid, ra, THREADS);
+    store_pieces<OB>(buf + OA::kBytes, tid, rb, THREADS);
+    if (kt + 1 < steps) {
+      load_pieces<OA, T, AKC>(sa, kt + 1, tid, ra);
+      load_pieces<OB, T, BKC>(sb, kt + 1, tid, rb);
+    }
+    // one barrier a step: the buffer written next was last read before it
+    __syncthreads();
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      typename Mma<T>::frag fa[FM], fb[FN];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fa[i] = OA::frag(buf + at_a[i], kk);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fb[j] = OB::frag(buf + at_b[j], kk);
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::run(fb[j], fa[i], acc[i][j]);
+    }
+  }
+
+  // lane l holds row l % 16 and 4 neighbouring columns of each 16x16 result
+  const int cm = wm * (BM / WM) + (lane & 15), cn = wn * (BN / WN) + (lane >> 4) * 4;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int m = cm + i * 16;
+    if (m >= c_rows) continue;
+    T* row = c + (int64_t)m * p.ldc;
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = cn + j * 16 + e;
+        if (n < sb.tile_rows) row[n] = (T)acc[i][j][e];
+      }
+  }
+}
+
+template <class T, int MODE>
+int launch_product(const ProductArgs& p, hipStream_t stream) {
+  constexpr int BM = 128, BN = 128;
+  const int64_t nt = ceil_div(p.n, BN);
+  const int64_t tiles = MODE == kMatrix ? ceil_div(p.m, BM) * nt * p.n_experts
+                                        : (p.n_rows / BM + p.n_experts + 1) * nt;
+  if (tiles > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
+  hipLaunchKernelGGL((expert_product_kernel<T, MODE, BM, BN, 2, 2>), dim3((uint32_t)tiles), dim3(256), 0, stream, p);
+  FS_CHECK_MAIN_LAUNCH("expert_product_kernel");
+  return FS_OK;
+}
+
+template <int MODE>
+int launch_product_type(int val_t, const ProductArgs& p, hipStream_t stream) {
+  switch (val_t) {
+    case FS_F16: return launch_product<_Float16, MODE>(p, stream);
+    case FS_BF16: return launch_product<__bf16, MODE>(p, stream);
+    case FS_F32: return launch_product<float, MODE>(p, stream);
+  }
+  return fail(FS_E_INVALID, "fs_expert_product: value types are FS_F16, FS_BF16 and FS_F32");
+}
+
+int check_product(const char* who, int64_t n_rows, int64_t n_experts, int64_t a, int64_t b, int trans) {
+  if (n_rows < 0 || n_rows > INT32_MAX || n_experts < 1 || n_experts > INT32_MAX || a < 0 || b < 0 ||
+      a > INT32_MAX || b > INT32_MAX || (trans != 0 && trans != 1))
+    return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
+  return FS_OK;
+}
+
+}  // namespace
+}  // namespace fs
+
+extern "C" int fs_expert_product(int val_t, int trans, int64_t n_rows, int64_t n_experts, int64_t inner, int64_t outer,
+                                 const void* rows, int64_t ldr, const void* matrices, const int32_t* offsets, void* out,
+                                 hipStream_t stream) {
+  using namespace fs;
+  if (int rc = check_product("fs_expert_product", n_rows, n_experts, inner, outer, trans)) return rc;
+  if (n_rows == 0 || outer == 0) return FS_OK;
+  if (!offsets || !out || ldr < 0 || (inner > 0 && (!rows || !matrices)))
+    return fail(FS_E_INVALID, "fs_expert_product: bad pointer or stride");
+  ProductArgs p{};
+  p.a = rows;
+  p.b = matrices;
+  p.c = out;
+  p.offsets = offsets;
+  p.lda = ldr;
+  p.ldb = trans ? inner : outer;
+  p.ldc = outer;
+  p.b_expert = inner * outer;
+  p.n_rows = n_rows;
+  p.n = outer;
+  p.k = inner;
+  p.n_experts = (int)n_experts;
+  return trans ? launch_product_type<kRowsTrans>(val_t, p, stream) : launch_product_type<kRowsNon>(val_t, p, stream);
+}
+
+extern "C" int fs_expert_product_grad_matrices(int val_t, int trans, int64_t n_rows, int64_t n_experts, int64_t inner,
+                                               int64_t outer, const void* grad, int64_t ldg, const void* rows,
+                                               int64_t ldr, const int32_t* offsets, void* grad_matrices,
+                                               hipStream_t stream) {
+  using namespace fs;
+  if (int rc = check_product("fs_expert_product_grad_matrices", n_rows, n_experts, inner, outer, trans)) return rc;
+  if (inner == 0 || outer == 0) return FS_OK;
+  if (!offsets || !grad_matrices || ldg < 0 || ldr < 0 || (n_rows > 0 && (!grad || !rows)))
+    return fail(FS_E_INVALID, "fs_expert_product_grad_matrices: bad pointer or stride");
+  ProductArgs p{};
+  p.a = trans ? grad : rows;
+  p.lda = trans ? ldg : ldr;
+  p.b = trans ? rows : grad;
+  p.ldb = trans ? ldr : ldg;
+  p.m = trans ? outer : inner;
+  p.n = trans ? inner : outer;
+  p.c = grad_matrices;
+  p.ldc = p.n;
+  p.c_expert = inner * outer;
+  p.offsets = offsets;
+  p.n_rows = n_rows;
+  p.n_experts = (int)n_experts;
+  return launch_product_type<kMatrix>(val_t, p, stream);
+}

@@ -28,6 +28,7 @@ import torch
 from . import _lib
 from ._common import _INDEX_LIMIT_INT32, SUPPORTED_INDEX_DTYPES
 from ._rows import ROW_DTYPE_MESSAGE, ROW_VALUE_CODES, check_out, row_major, wants_grad
+from .spmm_csr import _normalize_spmm_op, _spmm_op_transposes
 
 MAX_EXPERTS = 1023
 
@@ -257,6 +258,121 @@ def flagsparse_expert_combine_grad(grad, rows, route, weights):
     return grad_rows, grad_weights
 
 
+PRODUCT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+
+
+def _check_product(rows, matrices, route, op):
+    """(trans, inner, outer) of a product's arguments."""
+    n_rows = route.n_rows if isinstance(route, PreparedExpertRoute) else 0
+    _check_rows(rows, "rows", route, n_rows)
+    if rows.dtype not in PRODUCT_DTYPES:
+        raise TypeError("rows dtype must be one of: float16, bfloat16, float32")
+    if not isinstance(matrices, torch.Tensor):
+        raise TypeError("matrices must be a torch.Tensor")
+    if matrices.dtype != rows.dtype:
+        raise TypeError("matrices dtype must match rows dtype")
+    if matrices.device != route.device:
+        raise ValueError("matrices must be on the same CUDA device as the route")
+    if matrices.ndim != 3 or matrices.shape[0] != route.num_experts:
+        raise ValueError(f"matrices must be a 3D tensor with {route.num_experts} matrices, got shape "
+                         f"{tuple(matrices.shape)}")
+    trans = _spmm_op_transposes(_normalize_spmm_op(op))
+    inner, outer = matrices.shape[2 if trans else 1], matrices.shape[1 if trans else 2]
+    if rows.shape[1] != inner:
+        raise ValueError(f"rows must have width {inner}, got {rows.shape[1]}")
+    return trans, inner, outer
+
+
+def _dense_matrices(matrices, trans):
+    """(matrices, trans) of a contiguous tensor: a transposed view is taken as it lies."""
+    if matrices.is_contiguous():
+        return matrices, trans
+    flipped = matrices.transpose(1, 2)
+    if flipped.is_contiguous():
+        return flipped, not trans
+    return matrices.contiguous(), trans
+
+
+def _product(rows, matrices, route, trans, inner, outer, out=None):
+    rows, ld = row_major(rows)
+    matrices, trans = _dense_matrices(matrices, trans)
+    result = _into(out, (route.n_rows, outer), rows)
+    _lib.check(
+        _lib.lib().fs_expert_product(ROW_VALUE_CODES[rows.dtype], int(trans), route.n_rows, route.num_experts, inner,
+                                     outer, _lib.ptr(rows), ld, _lib.ptr(matrices), _lib.ptr(route.offsets),
+                                     _lib.ptr(result), _lib.stream_handle(rows.device)),
+        "fs_expert_product",
+    )
+    return _done(out, result)
+
+
+def _product_grad_matrices(grad, rows, route, trans, inner, outer):
+    grad, ldg = row_major(grad)
+    rows, ldr = row_major(rows)
+    shape = (route.num_experts, outer, inner) if trans else (route.num_experts, inner, outer)
+    result = torch.empty(shape, dtype=rows.dtype, device=rows.device)
+    _lib.check(
+        _lib.lib().fs_expert_product_grad_matrices(
+            ROW_VALUE_CODES[rows.dtype], int(trans), route.n_rows, route.num_experts, inner, outer, _lib.ptr(grad), ldg,
+            _lib.ptr(rows), ldr, _lib.ptr(route.offsets), _lib.ptr(result), _lib.stream_handle(rows.device)),
+        "fs_expert_product_grad_matrices",
+    )
+    return result
+
+
+class _Product(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, matrices, route, trans, inner, outer):
+        ctx.save_for_backward(rows, matrices)
+        ctx.route, ctx.sizes = route, (trans, inner, outer)
+        return _product(rows, matrices, route, trans, inner, outer)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        rows, matrices = ctx.saved_tensors
+        trans, inner, outer = ctx.sizes
+        grad_rows = grad_matrices = None
+        if ctx.needs_input_grad[0]:
+            grad_rows = _product(grad, matrices, ctx.route, not trans, outer, inner)
+        if ctx.needs_input_grad[1]:
+            grad_matrices = _product_grad_matrices(grad, rows, ctx.route, trans, inner, outer)
+        return grad_rows, grad_matrices, None, None, None, None
+
+
+def flagsparse_expert_product(rows, matrices, route, op="non", out=None):
+    """Each row times its expert's matrix: (T k, outer).
+
+    rows is (T k, inner) in expert order; matrices is (num_experts, inner,
+    outer), or (num_experts, outer, inner) with op="trans" ("conj" is the same
+    for these real types).  Rows of no expert are zero.  Differentiable in both.
+    """
+    trans, inner, outer = _check_product(rows, matrices, route, op)
+    if wants_grad(rows, matrices):
+        if out is not None:
+            raise ValueError("out cannot be given where a gradient is recorded")
+        return _Product.apply(rows, matrices, route, trans, inner, outer)
+    if out is not None:
+        check_out(out, rows.device, (route.n_rows, outer), rows.dtype)
+    return _product(rows, matrices, route, trans, inner, outer, out)
+
+
+def flagsparse_expert_product_grad(grad, rows, matrices, route, op="non"):
+    """Gradients of ``flagsparse_expert_product`` in its rows and its matrices.
+
+    grad is (T k, outer).  Rows of no expert get zeros, as do the matrices of
+    experts without rows.
+    """
+    trans, inner, outer = _check_product(rows, matrices, route, op)
+    _check_rows(grad, "grad", route, route.n_rows)
+    if grad.dtype != rows.dtype:
+        raise TypeError("grad dtype must match rows dtype")
+    if grad.shape[1] != outer:
+        raise ValueError(f"grad must have width {outer}, got {grad.shape[1]}")
+    return (_product(grad, matrices, route, not trans, outer, inner),
+            _product_grad_matrices(grad, rows, route, trans, inner, outer))
+
+
 __all__ = [
     "MAX_EXPERTS",
     "PreparedExpertRoute",
@@ -265,4 +381,6 @@ __all__ = [
     "flagsparse_expert_dispatch_grad",
     "flagsparse_expert_combine",
     "flagsparse_expert_combine_grad",
+    "flagsparse_expert_product",
+    "flagsparse_expert_product_grad",
 ]

@@ -629,6 +629,22 @@ int fs_expert_combine_grad(int val_t, int64_t n_tokens, int slots, int64_t width
                            const void* grad, int64_t ldg, const void* rows, int64_t ldr,
                            const int32_t* inverse, const int32_t* offsets, const void* weights,
                            void* grad_rows, void* grad_weights, hipStream_t stream);
+/*
+ * The experts' products, FS_F16, FS_BF16 and FS_F32, accumulated in 32 bits:
+ * out[r] = rows[r] op(matrices[e]) for the rows r of expert e (offsets, as
+ * above), zeros for rows of none.  matrices holds n_experts dense matrices,
+ * inner x outer each, or outer x inner with trans = 1.  The gradient of the
+ * matrices, in their layout, sums rows[r]^T grad[r] (trans: grad[r]^T rows[r])
+ * over each expert's rows; that of the rows is the product of grad with the
+ * other trans, and inner and outer exchanged.
+ */
+int fs_expert_product(int val_t, int trans, int64_t n_rows, int64_t n_experts, int64_t inner,
+                      int64_t outer, const void* rows, int64_t ldr, const void* matrices,
+                      const int32_t* offsets, void* out, hipStream_t stream);
+int fs_expert_product_grad_matrices(int val_t, int trans, int64_t n_rows, int64_t n_experts,
+                                    int64_t inner, int64_t outer, const void* grad, int64_t ldg,
+                                    const void* rows, int64_t ldr, const int32_t* offsets,
+                                    void* grad_matrices, hipStream_t stream);
 
 #ifdef __cplusplus
 }
