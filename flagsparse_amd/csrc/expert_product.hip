@@ -8,10 +8,10 @@
 //           gradient of the matrices
 // Rows of no expert (from offsets[n_experts] on) are written as zeros.
 //
-// A workgroup computes one BM x BN tile of one expert, 128 bytes of k at a
-// time: both operands' slices go to LDS, 16-byte pieces exchanged within a row
-// so that fragment reads meet no bank twice, double buffered, and feed 16x16
-// matrix instructions that accumulate in 32 bits.  Results are rounded once.
+// A workgroup computes one BM x BN tile of one expert, 64 bytes of k (one
+// fragment) a step: both operands' slices go to LDS, 16-byte pieces exchanged
+// within a row so that fragment reads meet no bank twice, and feed 16x16 matrix
+// instructions that accumulate in 32 bits.  Results are rounded once.
 // Where an operand is contiguous in k a fragment is one 16-byte LDS read; where
 // it is contiguous along the tile, 16-bit fragments are transposed by the LDS
 // read itself and 32-bit ones are read element by element.
@@ -25,7 +25,7 @@
 namespace fs {
 namespace {
 
-constexpr int kRowBytes = 128;  // k of one step, of an operand contiguous in k
+constexpr int kRowBytes = 64;  // k of one step, of an operand contiguous in k
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -60,19 +60,19 @@ struct Mma<float> {
 };
 
 // One operand's slice in LDS, and the way there.  KC: contiguous in k, R rows
-// of the tile by 128 bytes of k; otherwise BK rows of k by R elements.
+// of the tile by 64 bytes of k; otherwise BK rows of k by R elements.
 template <class T, bool KC, int R, int THREADS>
 struct Operand {
   static constexpr int E = 16 / (int)sizeof(T);        // elements a piece
   static constexpr int BK = kRowBytes / (int)sizeof(T);
   static constexpr int kBytes = R * kRowBytes;
   static constexpr int kPieces = kBytes / 16 / THREADS;  // a thread's, each step
-  static constexpr int kPerRow = KC ? 8 : R * (int)sizeof(T) / 16;
+  static constexpr int kPerRow = KC ? 4 : R * (int)sizeof(T) / 16;
   static_assert(kBytes % (16 * THREADS) == 0, "whole pieces a thread");
 
   // Exchange of the pieces of LDS row `row`.
   __device__ static int swizzle(int row) {
-    if constexpr (KC) return row & 7;
+    if constexpr (KC) return (row >> 1) & 3;
     else if constexpr (sizeof(T) == 4) return ((row >> 2) & 1) * 4;
     else return ((row & 3) + (kPerRow >= 16 ? ((row >> 3) & 1) * 4 : 0)) * 2;
   }
@@ -81,12 +81,11 @@ struct Operand {
     return ((i * THREADS + tid) % kPerRow) ^ swizzle(row_of(i, tid));
   }
 
-  // Fragment of 16 tile rows (from j * 16 past the wave's first) and the kk-th
-  // half of the step's k: lane l has tile row l % 16, k piece l / 16.
+  // Fragment of 16 tile rows from r0: lane l has tile row l % 16, k piece l / 16.
   __device__ static uint32_t frag_offset(int r0, int lane) {
     const int g = lane >> 4, i = lane & 15;
     if constexpr (KC) {
-      return (uint32_t)((r0 + i) * kRowBytes + ((g ^ (i & 7)) * 16));
+      return (uint32_t)((r0 + i) * kRowBytes + ((g ^ ((i >> 1) & 3)) * 16));
     } else if constexpr (sizeof(T) == 4) {
       const int row = 4 * g;
       return (uint32_t)(row * R * 4 + ((r0 / 4 + i / 4) ^ swizzle(row)) * 16 + (i & 3) * 4);
@@ -95,24 +94,37 @@ struct Operand {
       return (uint32_t)(row * R * 2 + ((r0 / 8 + (i & 3) / 2) ^ swizzle(row)) * 16 + (i & 1) * 8);
     }
   }
-  __device__ static typename Mma<T>::frag frag(uint32_t at, int kk) {
+  __device__ static typename Mma<T>::frag frag(const lds_byte* p) {
     typename Mma<T>::frag f;
     if constexpr (KC) {
-      // (piece g ^ (i & 7) of the first half is piece (g + 4) ^ (i & 7) of the second, 64 bytes away either way)
-      const u32x4 v = *(const lds_u32x4*)(lds_byte*)(uintptr_t)(at ^ (uint32_t)(kk * 64));
+      const u32x4 v = *(const lds_u32x4*)p;
       __builtin_memcpy(&f, &v, 16);
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        f[i] = *(const lds_float*)(lds_byte*)(uintptr_t)(at + (uint32_t)((kk * 16 + i) * R * 4));
+      for (int i = 0; i < 4; ++i) f[i] = *(const lds_float*)(p + i * R * 4);
     } else {
-      const uint32_t p = at + (uint32_t)(kk * 32 * R * 2);
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_byte*)(uintptr_t)p);
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_byte*)(uintptr_t)(p + 4 * R * 2));
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * R * 2));
       __builtin_memcpy(&f, &lo, 8);
       __builtin_memcpy((char*)&f + 8, &hi, 8);
     }
     return f;
+  }
+};
+
+// A wave's fragments of one operand: F of them, from tile row r0 on.
+template <class O, bool KC, int F>
+struct Frags {
+  uint32_t at[KC ? 1 : F];
+  __device__ void init(int r0, int lane) {
+#pragma unroll
+    for (int j = 0; j < (KC ? 1 : F); ++j) at[j] = O::frag_offset(r0 + j * 16, lane);
+  }
+  template <class X>
+  __device__ void read(uint32_t slice, X (&f)[F]) const {
+#pragma unroll
+    for (int j = 0; j < F; ++j)
+      f[j] = O::frag((const lds_byte*)(uintptr_t)(slice + at[KC ? 0 : j]) + (KC ? j * 16 * kRowBytes : 0));
   }
 };
 
@@ -155,6 +167,71 @@ template <class O>
 __device__ inline void store_pieces(uint32_t lds, int tid, const u32x4 (&r)[O::kPieces], int threads) {
 #pragma unroll
   for (int i = 0; i < O::kPieces; ++i) *(lds_u32x4*)(lds_byte*)(uintptr_t)(lds + (uint32_t)(i * threads + tid) * 16) = r[i];
+}
+
+// The same pieces straight to LDS (buffer loads that write LDS, 64 lanes x 16
+// bytes from the address in M0): nothing in registers but an offset a piece.
+// Offsets below kInBuffer count from the step's base, which moves; a piece
+// outside the operand gets one beyond it, and the load writes zeros.
+constexpr uint32_t kInBuffer = 1u << 30;
+
+__device__ inline void lds_dma16(uint32_t lds, uint32_t offset, u32x4 rsrc) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds"
+      :
+      : "s"(lds), "v"(offset), "s"(rsrc)
+      : "memory");  // (nothing else here uses M0)
+}
+__device__ inline u32x4 buffer_at(const void* p) {
+  const uint64_t a = (uint64_t)(uintptr_t)p;
+  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)) & 0xffffu, kInBuffer, 0x00020000u};
+}
+
+template <class O, class T, bool KC, int THREADS>
+struct Dma {
+  uint32_t off[O::kPieces];
+  const char* base;
+  int64_t step;  // bytes from one step to the next
+  __device__ void init(const Source<T>& s, int tid) {
+    base = (const char*)s.base;
+    step = KC ? (int64_t)kRowBytes : s.ld * (int64_t)sizeof(T) * O::BK;
+#pragma unroll
+    for (int i = 0; i < O::kPieces; ++i) {
+      const int row = O::row_of(i, tid), piece = O::piece_of(i, tid);
+      const bool in = KC ? row < s.tile_rows : piece * O::E < s.tile_rows;
+      off[i] = in ? (uint32_t)(row * s.ld * (int64_t)sizeof(T)) + (uint32_t)piece * 16u : 2u * kInBuffer;
+    }
+  }
+  // Before the loads of a step that has only `left` of k (none or less: zeros).
+  __device__ void cut(int64_t left, int tid) {
+#pragma unroll
+    for (int i = 0; i < O::kPieces; ++i) {
+      const int k0 = KC ? O::piece_of(i, tid) * O::E : O::row_of(i, tid);
+      if (k0 >= left) off[i] |= kInBuffer;
+    }
+  }
+  __device__ u32x4 at(int64_t kt) const { return buffer_at(base + kt * step); }
+  __device__ void issue(uint32_t lds, u32x4 rsrc, int i, int w) const {
+    lds_dma16(lds + (uint32_t)(i * THREADS + w * 64) * 16, off[i], rsrc);
+  }
+};
+
+// Waits and the barrier, which nothing is moved across.
+template <int LEFT>
+__device__ inline void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+}
+__device__ inline void wait_reads() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+__device__ inline void barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 struct ProductArgs {
@@ -230,7 +307,7 @@ __device__ inline bool find_tile(const ProductArgs& p, uint32_t nt, int lane, Ti
 
 enum Mode { kRowsTrans = 0, kRowsNon = 1, kMatrix = 2 };
 
-template <class T, int MODE, int BM, int BN, int WM, int WN>
+template <class T, int MODE, bool DMA, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const ProductArgs p) {
   constexpr int THREADS = 64 * WM * WN;
   constexpr bool AKC = MODE != kMatrix, BKC = MODE == kRowsTrans;
@@ -238,7 +315,8 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
   using OB = Operand<T, BKC, BN, THREADS>;
   constexpr int BK = OA::BK;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  __shared__ alignas(1024) uint8_t s_mem[2][OA::kBytes + OB::kBytes];
+  constexpr int kSlots = DMA ? 4 : 2, kSlot = OA::kBytes + OB::kBytes;
+  __shared__ alignas(1024) uint8_t s_mem[kSlots][kSlot];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t nt = (uint32_t)((p.n + BN - 1) / BN);
@@ -274,11 +352,10 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
 
   const int wm = w / WN, wn = w % WN;
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_byte*)&s_mem[0][0];
-  uint32_t at_a[FM], at_b[FN];
-#pragma unroll
-  for (int i = 0; i < FM; ++i) at_a[i] = OA::frag_offset(wm * (BM / WM) + i * 16, lane);
-#pragma unroll
-  for (int j = 0; j < FN; ++j) at_b[j] = OB::frag_offset(wn * (BN / WN) + j * 16, lane) + OA::kBytes;
+  Frags<OA, AKC, FM> from_a;
+  Frags<OB, BKC, FN> from_b;
+  from_a.init(wm * (BM / WM), lane);
+  from_b.init(wn * (BN / WN), lane);
 
   f32x4 acc[FM][FN];
 #pragma unroll
@@ -287,32 +364,91 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   const int64_t steps = (sa.k + BK - 1) / BK;
-  u32x4 ra[OA::kPieces], rb[OB::kPieces];
-  if (steps > 0) {
-    load_pieces<OA, T, AKC>(sa, 0, tid, ra);
-    load_pieces<OB, T, BKC>(sb, 0, tid, rb);
-  }
-  for (int64_t kt = 0; kt < steps; ++kt) {
-    const uint32_t buf = lds + (uint32_t)(kt & 1) * (OA::kBytes + OB::kBytes);
-    store_pieces<OA>(buf, tid, ra, THREADS);
-    store_pieces<OB>(buf + OA::kBytes, tid, rb, THREADS);
-    if (kt + 1 < steps) {
-      load_pieces<OA, T, AKC>(sa, kt + 1, tid, ra);
-      load_pieces<OB, T, BKC>(sb, kt + 1, tid, rb);
+  typename Mma<T>::frag fa[FM], fb[FN];
+  auto read_frags = [&](uint32_t slot) {
+    from_b.read(slot + OA::kBytes, fb);
+    from_a.read(slot, fa);
+  };
+  auto multiply_row = [&](int i) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::run(fb[j], fa[i], acc[i][j]);
+  };
+  if constexpr (DMA) {
+    // Two groups of four waves, one wave a SIMD each, half a step apart: one
+    // multiplies and starts the loads of three steps ahead while the other
+    // reads fragments.  Every wave starts its share of every step's loads, also
+    // of the three steps past the last (zeros), so that counting the loads
+    // still under way tells which step has arrived.
+    static_assert(WM * WN == 8, "two waves a SIMD");
+    constexpr int kLoads = OA::kPieces + OB::kPieces;
+    static_assert(kLoads <= FM, "a load between the products of two rows");
+    const bool second = w >= 4;
+    Dma<OA, T, AKC, THREADS> da;
+    Dma<OB, T, BKC, THREADS> db;
+    da.init(sa, tid);
+    db.init(sb, tid);
+    u32x4 rsrc_a, rsrc_b;
+    uint32_t next;
+    auto begin_loads = [&](int64_t kt) {
+      const int64_t left = sa.k - kt * BK;
+      if (left < BK) {
+        da.cut(left, tid);
+        db.cut(left, tid);
+      }
+      rsrc_a = da.at(kt);
+      rsrc_b = db.at(kt);
+      next = lds + (uint32_t)(kt & 3) * kSlot;
+    };
+    auto load = [&](int i) {
+      if (i < OA::kPieces) da.issue(next, rsrc_a, i, w);
+      else db.issue(next + OA::kBytes, rsrc_b, i - OA::kPieces, w);
+    };
+    for (int64_t kt = 0; kt < 3; ++kt) {
+      begin_loads(kt);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) load(i);
     }
-    // one barrier a step: the buffer written next was last read before it
-    __syncthreads();
+    wait_loads<2 * kLoads>();
+    barrier();
+    if (second) barrier();
+    for (int64_t kt = 0; kt < steps; ++kt) {
+      read_frags(lds + (uint32_t)(kt & 3) * kSlot);
+      begin_loads(kt + 3);
+      wait_reads();
+      if (second) wait_loads<kLoads>();  // step kt + 1, which the first group reads next
+      barrier();
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      typename Mma<T>::frag fa[FM], fb[FN];
+      for (int i = 0; i < FM; ++i) {
+        multiply_row(i);
+        if (i < kLoads) load(i);  // its slot was last read two phases ago
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_s_setprio(0);
+      if (!second) wait_loads<2 * kLoads>();
+      barrier();
+    }
+    if (!second) barrier();
+    wait_loads<0>();
+  } else {
+    u32x4 ra[OA::kPieces], rb[OB::kPieces];
+    if (steps > 0) {
+      load_pieces<OA, T, AKC>(sa, 0, tid, ra);
+      load_pieces<OB, T, BKC>(sb, 0, tid, rb);
+    }
+    for (int64_t kt = 0; kt < steps; ++kt) {
+      const uint32_t slot = lds + (uint32_t)(kt & 1) * kSlot;
+      store_pieces<OA>(slot, tid, ra, THREADS);
+      store_pieces<OB>(slot + OA::kBytes, tid, rb, THREADS);
+      if (kt + 1 < steps) {
+        load_pieces<OA, T, AKC>(sa, kt + 1, tid, ra);
+        load_pieces<OB, T, BKC>(sb, kt + 1, tid, rb);
+      }
+      // one barrier a step: the slot written next was last read before it
+      __syncthreads();
+      read_frags(slot);
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = OA::frag(buf + at_a[i], kk);
-#pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = OB::frag(buf + at_b[j], kk);
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::run(fb[j], fa[i], acc[i][j]);
+      for (int i = 0; i < FM; ++i) multiply_row(i);
     }
   }
 
@@ -324,25 +460,44 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
     if (m >= c_rows) continue;
     T* row = c + (int64_t)m * p.ldc;
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
+    for (int j = 0; j < FN; ++j) {
+      const int n = cn + j * 16;
+      T out[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int n = cn + j * 16 + e;
-        if (n < sb.tile_rows) row[n] = (T)acc[i][j][e];
+      for (int e = 0; e < 4; ++e) out[e] = (T)acc[i][j][e];
+      if constexpr (DMA) {  // (whole 16-byte pieces)
+        if (n < sb.tile_rows) __builtin_memcpy(__builtin_assume_aligned(row + n, sizeof out), out, sizeof out);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < sb.tile_rows) row[n + e] = out[e];
       }
+    }
   }
 }
 
-template <class T, int MODE>
-int launch_product(const ProductArgs& p, hipStream_t stream) {
-  constexpr int BM = 128, BN = 128;
+template <class T, int MODE, bool DMA, int BM, int BN, int WM, int WN>
+int launch_tiles(const ProductArgs& p, hipStream_t stream) {
   const int64_t nt = ceil_div(p.n, BN);
   const int64_t tiles = MODE == kMatrix ? ceil_div(p.m, BM) * nt * p.n_experts
                                         : (p.n_rows / BM + p.n_experts + 1) * nt;
   if (tiles > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
-  hipLaunchKernelGGL((expert_product_kernel<T, MODE, BM, BN, 2, 2>), dim3((uint32_t)tiles), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((expert_product_kernel<T, MODE, DMA, BM, BN, WM, WN>), dim3((uint32_t)tiles),
+                     dim3(64 * WM * WN), 0, stream, p);
   FS_CHECK_MAIN_LAUNCH("expert_product_kernel");
   return FS_OK;
+}
+
+template <class T, int MODE>
+int launch_product(const ProductArgs& p, hipStream_t stream) {
+  // straight to LDS: whole 16-byte pieces, and offsets within a step that fit
+  const int64_t s = sizeof(T), reach = MODE == kMatrix ? kRowBytes / s : 256;
+  const bool dma = aligned16(p.a, p.lda * s) && aligned16(p.b, p.ldb * s) && p.b_expert * s % 16 == 0 &&
+                   aligned16(p.c, p.ldc * s) &&
+                   (MODE == kMatrix ? p.m : p.k) * s % 16 == 0 && (MODE == kRowsTrans ? p.k : p.n) * s % 16 == 0 &&
+                   reach * std::max(p.lda, p.ldb) * s < (int64_t)kInBuffer;
+  if (!dma) return launch_tiles<T, MODE, false, 128, 128, 2, 2>(p, stream);
+  return launch_tiles<T, MODE, true, 256, 256, 2, 4>(p, stream);
 }
 
 template <int MODE>
