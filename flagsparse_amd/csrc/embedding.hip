@@ -7,7 +7,7 @@
 // table row over its segment, in position order, so results do not change from
 // run to run.  Rows without tokens are written as zeros in the same pass.
 //
-// A row of up to 64 tokens is summed by one wave.  A longer segment (tokens
+// A row of up to 64 tokens is summed at once.  A longer segment (tokens
 // follow a Zipf law: the first ones occur thousands of times in a batch) is cut
 // at multiples of 64 sorted positions; each chunk sums its part into the
 // workspace and a second launch adds a row's parts in order.
@@ -16,11 +16,10 @@
 namespace fs {
 namespace {
 
-constexpr int kLong = 64;       // tokens of a row that one wave sums, and positions a chunk
-constexpr int kRowsPerWave = 4; // table rows of a wave
-constexpr int kU = 4;           // slices a lane sums at a time
+constexpr int kLong = 64;      // tokens of a row that are summed at once, and positions a chunk
+constexpr int kBlockRows = 16; // table rows that a wave goes through
 
-template <class V, class Id, bool ALIGNED>
+template <class V, class Id>
 __global__ __launch_bounds__(256) void embedding_kernel(const V* __restrict__ table, int64_t ldt, int64_t n_rows,
                                                         const Id* __restrict__ ids, int64_t n, int64_t width, int lpr,
                                                         typename Elem<V>::acc scale, V* __restrict__ out) {
@@ -32,15 +31,17 @@ __global__ __launch_bounds__(256) void embedding_kernel(const V* __restrict__ ta
   const bool in = (uint64_t)id < (uint64_t)n_rows;
   const V* row = table + (in ? id : 0) * ldt;
   V* o = out + t * width;
-  const int64_t full = width / E;
-  for (int64_t c = lane; c < full; c += lpr) {
-    Slice<V> s;
-    if (in) s = load_slice<ALIGNED>(row + c * E);
+  const int64_t slices = slices_of<V>(width);
+#pragma unroll 2
+  for (int64_t c = lane; c < slices; c += lpr) {
+    const int64_t h = slice_start<V>(c, width);
+    Slice<V> s{};
+    if (in) s = load_slice(row + h);
 #pragma unroll
     for (int e = 0; e < E; ++e) s.v[e] = in ? (V)(widen(s.v[e]) * scale) : (V)0;
-    store_slice<ALIGNED>(o + c * E, s);
+    store_slice(o + h, s);
   }
-  for (int64_t h = full * E + lane; h < width; h += lpr) o[h] = in ? (V)(widen(row[h]) * scale) : (V)0;
+  for (int64_t h = slices > 0 ? width : lane; h < width; h += lpr) o[h] = in ? (V)(widen(row[h]) * scale) : (V)0;
 }
 
 // First index with keys[i] >= key (n if none), by the whole wave: 64 probes a step.
@@ -57,43 +58,38 @@ __device__ inline int64_t wave_lower_bound(const uint32_t* __restrict__ keys, in
   return lo + __popcll(__ballot(p < hi && keys[p < hi ? p : 0] < key));
 }
 
-// acc[u] = sum over positions t0..t1 (held by the lanes) of the lane's slices
-// c0 + u * 64 of the rows, two rows' loads in flight.
-template <class V, bool ALIGNED>
-__device__ inline void sum_slices(const V* __restrict__ grad, int64_t ldg, int pos, int t0, int t1, int64_t c0,
-                                  int64_t full, typename Elem<V>::acc (&acc)[kU][Slice<V>::n]) {
-  constexpr int E = Slice<V>::n;
+// Sum over the positions t0..t1 (held by the lanes) of the rows' slices from
+// element h, eight rows' loads in flight, in position order.
+template <class V>
+__device__ inline void sum_slices(const V* __restrict__ grad, int64_t ldg, int pos, int t0, int t1, int64_t h,
+                                  typename Elem<V>::acc (&acc)[Slice<V>::n]) {
+  constexpr int E = Slice<V>::n, kAtOnce = 8;
 #pragma unroll
-  for (int u = 0; u < kU; ++u)
+  for (int e = 0; e < E; ++e) acc[e] = 0;
+  auto row = [&](int t) { return load_slice(grad + (int64_t)__builtin_amdgcn_readlane(pos, t) * ldg + h); };
+  auto add = [&](const Slice<V>& s) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[u][e] = 0;
-  auto load = [&](int t, Slice<V> (&s)[kU]) {
-    const V* row = grad + (int64_t)__builtin_amdgcn_readlane(pos, t) * ldg;
-#pragma unroll
-    for (int u = 0; u < kU; ++u)
-      if (c0 + u * 64 < full) s[u] = load_slice<ALIGNED>(row + (c0 + u * 64) * E);
-  };
-  auto add = [&](const Slice<V> (&s)[kU]) {
-#pragma unroll
-    for (int u = 0; u < kU; ++u)
-      if (c0 + u * 64 < full)
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[u][e] += widen(s[u].v[e]);
+    for (int e = 0; e < E; ++e) acc[e] += widen(s.v[e]);
   };
   int t = t0;
-  for (; t + 1 < t1; t += 2) {
-    Slice<V> a[kU], b[kU];
-    load(t, a);
-    load(t + 1, b);
-    add(a);
-    add(b);
+  for (; t + kAtOnce <= t1; t += kAtOnce) {
+    Slice<V> s[kAtOnce];
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) s[q] = row(t + q);
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) add(s[q]);
   }
   if (t < t1) {
-    Slice<V> a[kU];
-    load(t, a);
-    add(a);
+    Slice<V> s[kAtOnce];
+#pragma unroll
+    for (int q = 0; q < kAtOnce - 1; ++q)
+      if (t + q < t1) s[q] = row(t + q);
+#pragma unroll
+    for (int q = 0; q < kAtOnce - 1; ++q)
+      if (t + q < t1) add(s[q]);
   }
 }
+// The same of one element, for rows shorter than a slice.
 template <class V>
 __device__ inline typename Elem<V>::acc sum_element(const V* __restrict__ grad, int64_t ldg, int pos, int t0, int t1,
                                                     int64_t h, bool in) {
@@ -106,7 +102,7 @@ __device__ inline typename Elem<V>::acc sum_element(const V* __restrict__ grad, 
 }
 
 // O = V, or float for 16-bit V: a slice of sums leaves as one or two stores.
-template <bool ALIGNED, class V, class O, class A>
+template <class V, class O, class A>
 __device__ inline void store_sums(O* p, const A (&acc)[Slice<V>::n], A scale) {
   constexpr int E = Slice<V>::n, EO = Slice<O>::n;
 #pragma unroll
@@ -114,138 +110,151 @@ __device__ inline void store_sums(O* p, const A (&acc)[Slice<V>::n], A scale) {
     Slice<O> s;
 #pragma unroll
     for (int e = 0; e < EO; ++e) s.v[e] = (O)(acc[k * EO + e] * scale);
-    store_slice<ALIGNED>(p + k * EO, s);
+    store_slice(p + k * EO, s);
   }
 }
 
-template <class V, class O, bool ALIGNED>
+// A wave's share of one sum of rows: slices first, first + stride, ...
+template <class V, class O>
+__device__ inline void sum_rows(const V* __restrict__ grad, int64_t ldg, int pos, int t0, int t1, int64_t width,
+                                int64_t first, int64_t stride, int lane, typename Elem<V>::acc scale, O* out) {
+  const int64_t slices = slices_of<V>(width);
+  typename Elem<V>::acc acc[Slice<V>::n];
+  for (int64_t c = first; c < slices; c += stride) {  // (the same number of times for the lanes that go on)
+    const int64_t h = slice_start<V>(c + lane < slices ? c + lane : slices - 1, width);
+    sum_slices(grad, ldg, pos, t0, t1, h, acc);
+    store_sums<V>(out + h, acc, scale);
+  }
+  if (slices == 0 && first == 0) {
+    const auto a = sum_element(grad, ldg, pos, t0, t1, lane, lane < width);
+    if (lane < width) out[lane] = (O)(a * scale);
+  }
+}
+
+// wpr waves share a row (or a chunk), 64 slices each at a time.
+template <class V, class O>
 __global__ __launch_bounds__(256) void embedding_grad_kernel(
     const V* __restrict__ grad, int64_t ldg, const uint32_t* __restrict__ keys, const int32_t* __restrict__ order,
-    int64_t n, int64_t n_rows, int64_t width, typename Elem<V>::acc scale, int64_t padding, uint32_t chunk_blocks,
-    int64_t n_chunks, O* __restrict__ out, typename Elem<V>::acc* __restrict__ parts) {
+    int64_t n, int64_t n_rows, int64_t width, typename Elem<V>::acc scale, int64_t padding, int wpr,
+    uint32_t chunk_blocks, int64_t n_chunks, O* __restrict__ out, typename Elem<V>::acc* __restrict__ parts) {
   using A = typename Elem<V>::acc;
-  constexpr int E = Slice<V>::n;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t full = width / E;
-  A acc[kU][E];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t first = (int64_t)(w % wpr) * 64, stride = (int64_t)wpr * 64;
+  const int groups = 4 / wpr;
 
-  if (blockIdx.x < chunk_blocks) {  // parts of long segments, a wave a chunk
-    const int64_t chunk = (int64_t)blockIdx.x * 4 + w;
+  if (blockIdx.x < chunk_blocks) {  // parts of long segments
+    const int64_t chunk = (int64_t)blockIdx.x * groups + w / wpr;
     if (chunk >= n_chunks) return;
     const int64_t c0 = chunk * kLong;
     const int cnt = (int)(n - c0 < kLong ? n - c0 : kLong);
     const uint32_t kk = lane < cnt ? keys[c0 + lane] : 0xffffffffu;
+    const int pos = lane < cnt ? order[c0 + lane] : 0;
     const uint32_t kl = (uint32_t)__builtin_amdgcn_readfirstlane((int)kk);
     const uint32_t kr = (uint32_t)__builtin_amdgcn_readlane((int)kk, cnt - 1);
     const uint64_t at_l = __ballot(kk == kl), at_r = __ballot(kk == kr);
     int64_t start = c0;
-    if (c0 > 0) {  // (c0 is a multiple of 64)
-      const uint64_t before = __ballot(keys[c0 - 64 + lane] == kl);
-      start = c0 - __popcll(before);
-    }
+    if (c0 > 0) start = c0 - __popcll(__ballot(keys[c0 - 64 + lane] == kl));  // (c0 is a multiple of 64)
     const bool enters = start < c0;
-    auto is_long = [&](int64_t s, uint32_t k) {
-      return (int64_t)k < n_rows && (int64_t)k != padding && s + kLong < n && keys[s + kLong] == k;
-    };
-    const bool left = enters && (start == c0 - 64 ? (int64_t)kl < n_rows && (int64_t)kl != padding : is_long(start, kl));
+    auto is_summed = [&](uint32_t k) { return (int64_t)k < n_rows && (int64_t)k != padding; };
+    auto is_long = [&](int64_t s, uint32_t k) { return is_summed(k) && s + kLong < n && keys[s + kLong] == k; };
+    const bool left = enters && (start == c0 - 64 ? is_summed(kl) : is_long(start, kl));
     const int f = __builtin_ctzll(at_r);
     const bool right = (f > 0 || !enters) && is_long(c0 + f, kr);
-    if (!left && !right) return;
-    const int pos = lane < cnt ? order[c0 + lane] : 0;
-    for (int side = 0; side < 2; ++side) {
-      if (side == 0 ? !left : !right) continue;
-      const int t0 = side == 0 ? 0 : f, t1 = side == 0 ? __popcll(at_l) : cnt;
-      A* part = parts + (chunk * 2 + side) * width;
-      for (int64_t c = lane; c - lane < full; c += 64 * kU) {
-        sum_slices<V, ALIGNED>(grad, ldg, pos, t0, t1, c, full, acc);
-#pragma unroll
-        for (int u = 0; u < kU; ++u)
-          if (c + u * 64 < full) store_sums<ALIGNED, V>(part + (c + u * 64) * E, acc[u], (A)1);
-      }
-      const int64_t h = full * E + lane;
-      const A a = sum_element(grad, ldg, pos, t0, t1, h, h < width);
-      if (h < width) part[h] = a;
-    }
+    A* part = parts + chunk * 2 * width;
+    if (left) sum_rows(grad, ldg, pos, 0, __popcll(at_l), width, first, stride, lane, (A)1, part);
+    if (right) sum_rows(grad, ldg, pos, f, cnt, width, first, stride, lane, (A)1, part + width);
     return;
   }
 
-  const int64_t v0 = ((int64_t)(blockIdx.x - chunk_blocks) * 4 + w) * kRowsPerWave;
+  const int64_t v0 = ((int64_t)(blockIdx.x - chunk_blocks) * groups + w / wpr) * kBlockRows;
   if (v0 >= n_rows) return;
+  // a window of 64 sorted positions from the first row's on
   int64_t wb = wave_lower_bound(keys, n, (uint32_t)v0, lane);
-  uint32_t kk = wb + lane < n ? keys[wb + lane] : 0xffffffffu;
-  for (int r = 0; r < kRowsPerWave && v0 + r < n_rows; ++r) {
+  uint32_t kk;
+  int pos;
+  auto window = [&] {
+    kk = wb + lane < n ? keys[wb + lane] : 0xffffffffu;
+    pos = wb + lane < n ? order[wb + lane] : 0;
+  };
+  window();
+  for (int r = 0; r < kBlockRows && v0 + r < n_rows; ++r) {
     const uint32_t v = (uint32_t)(v0 + r);
     while (__ballot(kk < v) == ~0ull) {
       wb += 64;
-      kk = wb + lane < n ? keys[wb + lane] : 0xffffffffu;
+      window();
     }
     uint64_t m = __ballot(kk == v);
     if (m >> 63) {  // the window may cut the segment: begin it there
       wb += __builtin_ctzll(m);
-      kk = wb + lane < n ? keys[wb + lane] : 0xffffffffu;
+      window();
       m = __ballot(kk == v);
       if (m == ~0ull && wb + kLong < n && keys[wb + kLong] == v) {
-        if ((int64_t)v != padding) {  // a long segment: the chunks sum it
-          wb = wave_lower_bound(keys, n, v + 1, lane);
-          kk = wb + lane < n ? keys[wb + lane] : 0xffffffffu;
-          continue;
-        }
+        // a long segment: the chunks sum it, or nobody
+        if ((int64_t)v == padding) sum_rows(grad, ldg, pos, 0, 0, width, first, stride, lane, scale, out + (int64_t)v * width);
+        wb = wave_lower_bound(keys, n, v + 1, lane);
+        window();
+        continue;
       }
     }
     const int t0 = m != 0 ? __builtin_ctzll(m) : 0;
     const int t1 = (int64_t)v == padding ? t0 : t0 + __popcll(m);
-    const int pos = lane >= t0 && lane < t1 ? order[wb + lane] : 0;
-    O* o = out + (int64_t)v * width;
-    for (int64_t c = lane; c - lane < full; c += 64 * kU) {
-      sum_slices<V, ALIGNED>(grad, ldg, pos, t0, t1, c, full, acc);
-#pragma unroll
-      for (int u = 0; u < kU; ++u)
-        if (c + u * 64 < full) store_sums<ALIGNED, V>(o + (c + u * 64) * E, acc[u], scale);
-    }
-    const int64_t h = full * E + lane;
-    const A a = sum_element(grad, ldg, pos, t0, t1, h, h < width);
-    if (h < width) o[h] = (O)(a * scale);
+    sum_rows(grad, ldg, pos, t0, t1, width, first, stride, lane, scale, out + (int64_t)v * width);
   }
 }
 
 // Rows of long segments: the chunk in which one starts adds its parts, the
-// first chunk's second slot and the first slots of the chunks after it.  The 4
-// waves of a workgroup take every fourth part of 256 columns and are added in
-// wave order.
+// first chunk's second slot and the first slots of the chunks after it.  The
+// waves of a workgroup take every kJoinWaves-th part of 256 columns, eight
+// loads in flight, and are added in wave order.
+constexpr int kJoinWaves = 4;
 template <class O, class A>
-__global__ __launch_bounds__(256) void embedding_grad_join_kernel(const uint32_t* __restrict__ keys, int64_t n,
-                                                                  int64_t n_rows, int64_t width, A scale,
-                                                                  int64_t padding, const A* __restrict__ parts,
-                                                                  O* __restrict__ out) {
-  constexpr int C = 4;
-  __shared__ A s_sum[3][C][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+__global__ __launch_bounds__(64 * kJoinWaves) void embedding_grad_join_kernel(
+    const uint32_t* __restrict__ keys, int64_t n, int64_t n_rows, int64_t width, A scale, int64_t padding,
+    const A* __restrict__ parts, O* __restrict__ out) {
+  constexpr int C = 4, kAtOnce = 8;
+  __shared__ A s_sum[kJoinWaves - 1][C][64];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t c0 = (int64_t)blockIdx.x * kLong;
   if (c0 + kLong >= n) return;  // the last chunk starts none that leaves it
   const uint32_t kr = keys[c0 + kLong - 1];
   if (keys[c0 + kLong] != kr || (int64_t)kr >= n_rows || (int64_t)kr == padding) return;
   if (c0 > 0 && keys[c0 - 1] == kr) return;  // starts before
   const int f = __builtin_ctzll(__ballot(keys[c0 + lane] == kr));
-  if (c0 + f + kLong >= n || keys[c0 + f + kLong] != kr) return;  // one wave summed it
+  if (c0 + f + kLong >= n || keys[c0 + f + kLong] != kr) return;  // summed at once
   const int64_t end = wave_lower_bound(keys, n, kr + 1, lane);
   const int64_t count = (end - 1) / kLong - blockIdx.x + 1;  // chunks that hold it
-  const int64_t h0 = (int64_t)blockIdx.y * 64 * C + lane;
-  A sum[C] = {};
-#pragma unroll 8
-  for (int64_t k = w; k < count; k += 4) {
-    const A* p = parts + ((blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * width;
+  int64_t h[C];
 #pragma unroll
-    for (int u = 0; u < C; ++u)
-      if (h0 + u * 64 < width) sum[u] += p[h0 + u * 64];
+  for (int u = 0; u < C; ++u) {
+    const int64_t own = (int64_t)blockIdx.y * 64 * C + u * 64 + lane;
+    h[u] = own < width ? own : width - 1;
+  }
+  auto part = [&](int64_t k) { return parts + ((blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * width; };
+  A sum[C] = {};
+  for (int64_t k = w; k < count; k += kJoinWaves * kAtOnce) {
+    A v[kAtOnce][C];
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q)
+      if (k + q * kJoinWaves < count)
+#pragma unroll
+        for (int u = 0; u < C; ++u) v[q][u] = part(k + q * kJoinWaves)[h[u]];
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q)
+      if (k + q * kJoinWaves < count)
+#pragma unroll
+        for (int u = 0; u < C; ++u) sum[u] += v[q][u];
   }
   if (w > 0)
+#pragma unroll
     for (int u = 0; u < C; ++u) s_sum[w - 1][u][lane] = sum[u];
   __syncthreads();
   if (w > 0) return;
 #pragma unroll
   for (int u = 0; u < C; ++u) {
-    const A total = sum[u] + s_sum[0][u][lane] + s_sum[1][u][lane] + s_sum[2][u][lane];
-    if (h0 + u * 64 < width) out[(int64_t)kr * width + h0 + u * 64] = (O)(total * scale);
+    A total = sum[u];
+#pragma unroll
+    for (int k = 0; k < kJoinWaves - 1; ++k) total += s_sum[k][u][lane];
+    out[(int64_t)kr * width + h[u]] = (O)(total * scale);
   }
 }
 
@@ -283,17 +292,15 @@ extern "C" int fs_embedding(int val_t, int id_t, int64_t n, int64_t n_rows, int6
   return with_value_type(val_t, "fs_embedding", [&](auto v) -> int {
     using V = decltype(v);
     using A = typename Elem<V>::acc;
-    const int64_t s = sizeof(V);
-    const int lpr = lanes_per_row(width / Slice<V>::n);
+    const int lpr = lanes_per_row(slices_of<V>(width));
     const dim3 grid((uint32_t)ceil_div(n, 256 / lpr));
-    auto launch = [&](auto id, auto al) {
+    auto launch = [&](auto id) {
       using Id = decltype(id);
-      hipLaunchKernelGGL((embedding_kernel<V, Id, decltype(al)::value>), grid, dim3(256), 0, stream, (const V*)table,
-                         ldt, n_rows, (const Id*)ids, n, width, lpr, (A)scale, (V*)out);
+      hipLaunchKernelGGL((embedding_kernel<V, Id>), grid, dim3(256), 0, stream, (const V*)table, ldt, n_rows,
+                         (const Id*)ids, n, width, lpr, (A)scale, (V*)out);
     };
-    const bool al = aligned16(table, ldt * s) && aligned16(out, width * s);
-    if (id_t == FS_I64) al ? launch(int64_t(0), std::true_type{}) : launch(int64_t(0), std::false_type{});
-    else al ? launch(int32_t(0), std::true_type{}) : launch(int32_t(0), std::false_type{});
+    if (id_t == FS_I64) launch(int64_t(0));
+    else launch(int32_t(0));
     FS_CHECK_MAIN_LAUNCH("embedding_kernel");
     return FS_OK;
   });
@@ -331,22 +338,16 @@ extern "C" int fs_embedding_grad(int val_t, int out_t, int id_t, int64_t n, int6
     auto run = [&](auto o) -> int {
       using O = decltype(o);
       A* parts = n > 0 ? reinterpret_cast<A*>(w + l.parts) : nullptr;
-      const int64_t chunks = n > kLong ? ceil_div(n, kLong) : 0;
-      const uint32_t chunk_blocks = (uint32_t)ceil_div(chunks, 4);
-      const dim3 grid(chunk_blocks + (uint32_t)ceil_div(n_rows, 4 * kRowsPerWave));
-      // (parts: rows of `width` sums from a 256-byte boundary)
-      const bool al = aligned16(grad, ldg * sizeof(V)) && aligned16(out, width * sizeof(O)) &&
-                      aligned16(parts, width * sizeof(A));
-      if (al)
-        hipLaunchKernelGGL((embedding_grad_kernel<V, O, true>), grid, dim3(256), 0, stream, (const V*)grad, ldg, keys,
-                           order, n, n_rows, width, (A)scale, padding, chunk_blocks, chunks, (O*)out, parts);
-      else
-        hipLaunchKernelGGL((embedding_grad_kernel<V, O, false>), grid, dim3(256), 0, stream, (const V*)grad, ldg, keys,
-                           order, n, n_rows, width, (A)scale, padding, chunk_blocks, chunks, (O*)out, parts);
+      const int64_t chunks = n > kLong ? ceil_div(n, kLong) : 0, slices = slices_of<V>(width);
+      const int wpr = slices <= 64 ? 1 : slices <= 128 ? 2 : 4;
+      const uint32_t chunk_blocks = (uint32_t)ceil_div(chunks, 4 / wpr);
+      const dim3 grid(chunk_blocks + (uint32_t)ceil_div(n_rows, (4 / wpr) * kBlockRows));
+      hipLaunchKernelGGL((embedding_grad_kernel<V, O>), grid, dim3(256), 0, stream, (const V*)grad, ldg, keys, order, n,
+                         n_rows, width, (A)scale, padding, wpr, chunk_blocks, chunks, (O*)out, parts);
       FS_CHECK_MAIN_LAUNCH("embedding_grad_kernel");
       if (chunks > 0) {
         hipLaunchKernelGGL((embedding_grad_join_kernel<O, A>), dim3((uint32_t)chunks, (uint32_t)ceil_div(width, 256)),
-                           dim3(256), 0, stream, keys, n, n_rows, width, (A)scale, padding, parts, (O*)out);
+                           dim3(64 * kJoinWaves), 0, stream, keys, n, n_rows, width, (A)scale, padding, parts, (O*)out);
         FS_CHECK_LAUNCH("embedding_grad_join_kernel");
       }
       return FS_OK;

@@ -15,36 +15,36 @@
 namespace fs {
 namespace {
 
-template <class V, bool ALIGNED>
+template <class V>
 __global__ __launch_bounds__(256) void expert_dispatch_kernel(const V* __restrict__ x, int64_t ldx, int64_t n_tokens,
                                                               int slots, int64_t width, int lpr,
                                                               const int32_t* __restrict__ inverse,
                                                               const int32_t* __restrict__ routed_at,
                                                               V* __restrict__ out) {
-  constexpr int E = Slice<V>::n;
   const int lane = threadIdx.x & (lpr - 1);
   const int64_t t = (int64_t)blockIdx.x * (256 / lpr) + threadIdx.x / lpr;
   if (t >= n_tokens) return;
   const int routed = *routed_at;
   const V* row = x + t * ldx;
   const int32_t* inv = inverse + t * slots;
-  const int64_t full = width / E;
-  for (int64_t c = lane; c < full; c += lpr) {
-    const Slice<V> s = load_slice<ALIGNED>(row + c * E);
+  const int64_t slices = slices_of<V>(width);
+  for (int64_t c = lane; c < slices; c += lpr) {
+    const int64_t h = slice_start<V>(c, width);
+    uint4 s;  // (selected word by word: a choice between two slices went through memory)
+    __builtin_memcpy(&s, row + h, 16);
+#pragma unroll 4
     for (int j = 0; j < slots; ++j) {
-      const int at = inv[j];
-      Slice<V> o = s;
-      if (at >= routed)
-#pragma unroll
-        for (int e = 0; e < E; ++e) o.v[e] = (V)0;
-      store_slice<ALIGNED>(out + at * width + c * E, o);
+      const bool in = inv[j] < routed;
+      const uint4 o = make_uint4(in ? s.x : 0u, in ? s.y : 0u, in ? s.z : 0u, in ? s.w : 0u);
+      __builtin_memcpy(out + inv[j] * width + h, &o, 16);
     }
   }
-  for (int64_t h = full * E + lane; h < width; h += lpr)
-    for (int j = 0; j < slots; ++j) out[(int64_t)inv[j] * width + h] = inv[j] < routed ? row[h] : (V)0;
+  for (int64_t h = slices > 0 ? width : lane; h < width; h += lpr)
+    for (int j = 0; j < slots; ++j) out[inv[j] * width + h] = inv[j] < routed ? row[h] : (V)0;
 }
 
-template <class V, bool ALIGNED>
+// (a slot of no expert has a place, whose row is read and left out)
+template <class V>
 __global__ __launch_bounds__(256) void expert_combine_kernel(const V* __restrict__ rows, int64_t ldr, int64_t n_tokens,
                                                              int slots, int64_t width, int lpr,
                                                              const int32_t* __restrict__ inverse,
@@ -52,33 +52,38 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(const V* __restrict
                                                              const typename Elem<V>::acc* __restrict__ weights,
                                                              V* __restrict__ out) {
   using A = typename Elem<V>::acc;
-  constexpr int E = Slice<V>::n;
+  constexpr int E = Slice<V>::n, kAtOnce = 4;
   const int lane = threadIdx.x & (lpr - 1);
   const int64_t t = (int64_t)blockIdx.x * (256 / lpr) + threadIdx.x / lpr;
   if (t >= n_tokens) return;
   const int routed = *routed_at;
   const int32_t* inv = inverse + t * slots;
   const A* wt = weights != nullptr ? weights + t * slots : nullptr;
-  const int64_t full = width / E;
-  for (int64_t c = lane; c < full; c += lpr) {
-    A acc[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0;
-#pragma unroll 4
-    for (int j = 0; j < slots; ++j) {
-      const int at = inv[j];
-      if (at >= routed) continue;
+  const int64_t slices = slices_of<V>(width);
+  for (int64_t c = lane; c < slices; c += lpr) {
+    const int64_t h = slice_start<V>(c, width);
+    A acc[E] = {};
+    auto add = [&](int j, const Slice<V>& s) {
       const A w = wt != nullptr ? wt[j] : (A)1;
-      const Slice<V> s = load_slice<ALIGNED>(rows + at * ldr + c * E);
+      if (inv[j] < routed)
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += w * widen(s.v[e]);
+        for (int e = 0; e < E; ++e) acc[e] += w * widen(s.v[e]);
+    };
+    int j = 0;
+    for (; j + kAtOnce <= slots; j += kAtOnce) {
+      Slice<V> s[kAtOnce];
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) s[q] = load_slice(rows + inv[j + q] * ldr + h);
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) add(j + q, s[q]);
     }
+    for (; j < slots; ++j) add(j, load_slice(rows + inv[j] * ldr + h));
     Slice<V> o;
 #pragma unroll
     for (int e = 0; e < E; ++e) o.v[e] = (V)acc[e];
-    store_slice<ALIGNED>(out + t * width + c * E, o);
+    store_slice(out + t * width + h, o);
   }
-  for (int64_t h = full * E + lane; h < width; h += lpr) {
+  for (int64_t h = slices > 0 ? width : lane; h < width; h += lpr) {
     A acc = 0;
     for (int j = 0; j < slots; ++j)
       if (inv[j] < routed) acc += (wt != nullptr ? wt[j] : (A)1) * widen(rows[inv[j] * ldr + h]);
@@ -88,7 +93,7 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(const V* __restrict
 
 // One wave a slot: the token's gradient row, read by its slots in turn, comes
 // from cache after the first.
-template <class V, bool ALIGNED>
+template <class V>
 __global__ __launch_bounds__(256) void expert_combine_grad_kernel(
     const V* __restrict__ grad, int64_t ldg, const V* __restrict__ rows, int64_t ldr, int64_t n, int slots,
     int64_t width, const int32_t* __restrict__ inverse, const int32_t* __restrict__ routed_at,
@@ -105,27 +110,29 @@ __global__ __launch_bounds__(256) void expert_combine_grad_kernel(
   const V* g = grad + i / slots * ldg;
   const V* y = rows + at * ldr;
   V* o = grad_rows + at * width;
+  // (no overlapping slice at the end: an element counts once in the dot product)
   const int64_t full = width / E;
   A dot = 0;
-  for (int64_t c = lane; c < full; c += 64) {
-    Slice<V> out;
-    if (in) {
-      const Slice<V> sg = load_slice<ALIGNED>(g + c * E), sy = load_slice<ALIGNED>(y + c * E);
+  if (in) {
+#pragma unroll 2
+    for (int64_t c = lane; c < full; c += 64) {
+      const Slice<V> sg = load_slice(g + c * E), sy = load_slice(y + c * E);
+      Slice<V> out;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const A ge = widen(sg.v[e]);
         dot += ge * widen(sy.v[e]);
         out.v[e] = (V)(w * ge);
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) out.v[e] = (V)0;
+      store_slice(o + c * E, out);
     }
-    store_slice<ALIGNED>(o + c * E, out);
-  }
-  for (int64_t h = full * E + lane; h < width; h += 64) {
-    if (in) dot += widen(g[h]) * widen(y[h]);
-    o[h] = in ? (V)(w * widen(g[h])) : (V)0;
+    for (int64_t h = full * E + lane; h < width; h += 64) {
+      dot += widen(g[h]) * widen(y[h]);
+      o[h] = (V)(w * widen(g[h]));
+    }
+  } else {
+    for (int64_t c = lane; c < full; c += 64) store_slice(o + c * E, Slice<V>{});
+    for (int64_t h = full * E + lane; h < width; h += 64) o[h] = (V)0;
   }
   dot = wave_sum(dot);
   if (lane == 0) grad_w[i] = dot;
@@ -149,15 +156,10 @@ extern "C" int fs_expert_dispatch(int val_t, int64_t n_tokens, int slots, int64_
   if (!x || !inverse || !offsets || !out || ldx < 0) return fail(FS_E_INVALID, "fs_expert_dispatch: bad pointer or stride");
   return with_value_type(val_t, "fs_expert_dispatch", [&](auto v) -> int {
     using V = decltype(v);
-    const int64_t s = sizeof(V);
-    const int lpr = lanes_per_row(width / Slice<V>::n);
+    const int lpr = lanes_per_row(slices_of<V>(width));
     const dim3 grid((uint32_t)ceil_div(n_tokens, 256 / lpr));
-    if (aligned16(x, ldx * s) && aligned16(out, width * s))
-      hipLaunchKernelGGL((expert_dispatch_kernel<V, true>), grid, dim3(256), 0, stream, (const V*)x, ldx, n_tokens,
-                         slots, width, lpr, inverse, offsets + n_experts, (V*)out);
-    else
-      hipLaunchKernelGGL((expert_dispatch_kernel<V, false>), grid, dim3(256), 0, stream, (const V*)x, ldx, n_tokens,
-                         slots, width, lpr, inverse, offsets + n_experts, (V*)out);
+    hipLaunchKernelGGL((expert_dispatch_kernel<V>), grid, dim3(256), 0, stream, (const V*)x, ldx, n_tokens,
+                       slots, width, lpr, inverse, offsets + n_experts, (V*)out);
     FS_CHECK_MAIN_LAUNCH("expert_dispatch_kernel");
     return FS_OK;
   });
@@ -173,15 +175,10 @@ extern "C" int fs_expert_combine(int val_t, int64_t n_tokens, int slots, int64_t
   return with_value_type(val_t, "fs_expert_combine", [&](auto v) -> int {
     using V = decltype(v);
     using A = typename Elem<V>::acc;
-    const int64_t s = sizeof(V);
-    const int lpr = lanes_per_row(width / Slice<V>::n);
+    const int lpr = lanes_per_row(slices_of<V>(width));
     const dim3 grid((uint32_t)ceil_div(n_tokens, 256 / lpr));
-    if (aligned16(rows, ldr * s) && aligned16(out, width * s))
-      hipLaunchKernelGGL((expert_combine_kernel<V, true>), grid, dim3(256), 0, stream, (const V*)rows, ldr, n_tokens,
-                         slots, width, lpr, inverse, offsets + n_experts, (const A*)weights, (V*)out);
-    else
-      hipLaunchKernelGGL((expert_combine_kernel<V, false>), grid, dim3(256), 0, stream, (const V*)rows, ldr, n_tokens,
-                         slots, width, lpr, inverse, offsets + n_experts, (const A*)weights, (V*)out);
+    hipLaunchKernelGGL((expert_combine_kernel<V>), grid, dim3(256), 0, stream, (const V*)rows, ldr, n_tokens,
+                       slots, width, lpr, inverse, offsets + n_experts, (const A*)weights, (V*)out);
     FS_CHECK_MAIN_LAUNCH("expert_combine_kernel");
     return FS_OK;
   });
@@ -200,16 +197,11 @@ extern "C" int fs_expert_combine_grad(int val_t, int64_t n_tokens, int slots, in
   return with_value_type(val_t, "fs_expert_combine_grad", [&](auto v) -> int {
     using V = decltype(v);
     using A = typename Elem<V>::acc;
-    const int64_t s = sizeof(V), n = n_tokens * slots;
+    const int64_t n = n_tokens * slots;
     const dim3 grid((uint32_t)ceil_div(n, 4));
-    if (aligned16(grad, ldg * s) && aligned16(rows, ldr * s) && aligned16(grad_rows, width * s))
-      hipLaunchKernelGGL((expert_combine_grad_kernel<V, true>), grid, dim3(256), 0, stream, (const V*)grad, ldg,
-                         (const V*)rows, ldr, n, slots, width, inverse, offsets + n_experts, (const A*)weights,
-                         (V*)grad_rows, (A*)grad_weights);
-    else
-      hipLaunchKernelGGL((expert_combine_grad_kernel<V, false>), grid, dim3(256), 0, stream, (const V*)grad, ldg,
-                         (const V*)rows, ldr, n, slots, width, inverse, offsets + n_experts, (const A*)weights,
-                         (V*)grad_rows, (A*)grad_weights);
+    hipLaunchKernelGGL((expert_combine_grad_kernel<V>), grid, dim3(256), 0, stream, (const V*)grad, ldg,
+                       (const V*)rows, ldr, n, slots, width, inverse, offsets + n_experts, (const A*)weights,
+                       (V*)grad_rows, (A*)grad_weights);
     FS_CHECK_MAIN_LAUNCH("expert_combine_grad_kernel");
     return FS_OK;
   });

@@ -20,34 +20,35 @@ __device__ inline typename Elem<V>::acc widen(V v) {
   return (typename Elem<V>::acc)v;
 }
 
-// A lane's slice: 16 bytes of a row.  ALIGNED: rows start at multiples of 16
-// bytes; otherwise only elements are aligned, which the global load and store
-// instructions take as they are.
+// A lane's slice: 16 bytes of a row, at any element: the 16-byte load and store
+// instructions take addresses that only elements are aligned to (compiled alike
+// either way, so there is no variant for rows at multiples of 16 bytes).
 template <class V>
 struct Slice {
   static constexpr int n = 16 / (int)sizeof(V);
   V v[n];
 };
-template <bool ALIGNED, class V>
+template <class V>
 __device__ inline Slice<V> load_slice(const V* p) {
   Slice<V> s;
-  if constexpr (ALIGNED) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    __builtin_memcpy(&s, &u, 16);
-  } else {
-    __builtin_memcpy(&s, p, 16);
-  }
+  __builtin_memcpy(&s, p, 16);
   return s;
 }
-template <bool ALIGNED, class V>
+template <class V>
 __device__ inline void store_slice(V* p, const Slice<V>& s) {
-  if constexpr (ALIGNED) {
-    uint4 u;
-    __builtin_memcpy(&u, &s, 16);
-    *reinterpret_cast<uint4*>(p) = u;
-  } else {
-    __builtin_memcpy(p, &s, 16);
-  }
+  __builtin_memcpy(p, &s, 16);
+}
+// Slices of a row: the last one ends with the row and overlaps the one before
+// (its elements are computed twice, alike).  Rows shorter than a slice have
+// none; their elements are taken one by one.
+template <class V>
+__host__ __device__ inline int64_t slices_of(int64_t width) {
+  return width >= Slice<V>::n ? (width + Slice<V>::n - 1) / Slice<V>::n : 0;
+}
+template <class V>
+__device__ inline int64_t slice_start(int64_t c, int64_t width) {
+  const int64_t h = c * Slice<V>::n, last = width - Slice<V>::n;
+  return h < last ? h : last;
 }
 
 template <class A>
@@ -57,6 +58,7 @@ __device__ inline A wave_sum(A v) {
   return v;
 }
 
+// Whether rows `ld_bytes` apart all start at multiples of 16 bytes.
 inline bool aligned16(const void* p, int64_t ld_bytes) {
   return ((uintptr_t)p & 15) == 0 && (ld_bytes & 15) == 0;
 }

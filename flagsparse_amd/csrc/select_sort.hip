@@ -7,11 +7,12 @@
 // by this one routine (expert order; the embedding gradient's segments).
 //
 // Counting sort, least significant digit first: up to 10 key bits a pass, one
-// pass for experts, two for a vocabulary.  A pass is a count (digits of each
-// tile of 4096 positions) and a scatter, which ranks its tile stably: a wave
-// takes 64 positions at a time, the lanes with its digit found by ballots, and
-// waves own consecutive sub-tiles, so ranks need no order of atomics.  One tile
-// counts for itself and is one launch a pass.
+// pass for experts, two for a vocabulary.  A pass counts the digits of each tile
+// of 512 to 4096 positions, scans the counts, and scatters: a tile is ranked
+// stably, a wave taking 64 positions at a time, the lanes with its digit found
+// by ballots, and waves owning consecutive sub-tiles, so ranks need no order of
+// atomics.  One tile counts for itself and is one launch a pass; a few are
+// scanned by the scatter, two launches.
 #include "fs_common.hpp"
 #include "radix_tile.hpp"
 
@@ -20,14 +21,11 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
-constexpr int kChunks = 8;
-constexpr int kSub = 64 * kChunks;
-constexpr int kTile = kWaves * kSub;
 constexpr int kMaxBits = 10;
 constexpr int kMaxDigits = 1 << kMaxBits;
 // Up to this many tiles a scatter adds up the counts of the tiles before it
-// itself (reads all counts, 4 nd bytes a tile); more are scanned by launches.
-constexpr int64_t kSelfScanTiles = 512;
+// itself, in two rounds of loads; more are scanned by a launch of their own.
+constexpr int64_t kSelfScanTiles = 16;
 
 template <class Id>
 __device__ inline uint32_t key_of(Id id, uint32_t n_keys) {
@@ -43,16 +41,16 @@ __device__ inline uint32_t load_key(const void* __restrict__ src, int64_t i, uin
   else return key_of(static_cast<const Id*>(src)[i], n_keys);
 }
 
-template <class Id, bool KEYS>
+template <class Id, bool KEYS, int CH>
 __global__ __launch_bounds__(kThreads) void select_count_kernel(const void* __restrict__ src, int64_t n,
                                                                 uint32_t n_keys, int shift, int nd,
                                                                 uint32_t* __restrict__ cnt) {
   __shared__ uint32_t s_cnt[kMaxDigits];
   for (int d = threadIdx.x; d < nd; d += kThreads) s_cnt[d] = 0u;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kTile;
+  const int64_t base = (int64_t)blockIdx.x * (kThreads * CH);
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
+  for (int c = 0; c < CH; ++c) {
     const int64_t i = base + c * kThreads + threadIdx.x;
     if (i < n) atomicAdd(&s_cnt[(load_key<Id, KEYS>(src, i, n_keys) >> shift) & (uint32_t)(nd - 1)], 1u);
   }
@@ -61,36 +59,39 @@ __global__ __launch_bounds__(kThreads) void select_count_kernel(const void* __re
 }
 
 // mode 0: one tile; 1: the tiles before this one are added up here; 2: cnt
-// holds each tile's first place per digit.  LAST: writes order, inverse and
-// offsets, where asked for, besides the sorted keys.
-template <class Id, bool KEYS>
+// holds, per digit, the sum over the tiles before, and totals that over all.
+// Writes sorted keys, order, inverse and offsets where asked for.
+template <class Id, bool KEYS, int CH>
 __global__ __launch_bounds__(kThreads) void select_scatter_kernel(
     const void* __restrict__ src, const int32_t* __restrict__ pos_in, int64_t n, uint32_t n_keys, int shift, int nd,
-    const uint32_t* __restrict__ cnt, int64_t n_tiles, int mode, uint32_t* __restrict__ keys_out,
-    int32_t* __restrict__ pos_out, int32_t* __restrict__ inverse, int32_t* __restrict__ offsets) {
+    const uint32_t* __restrict__ cnt, const uint32_t* __restrict__ totals, int64_t n_tiles, int mode,
+    uint32_t* __restrict__ keys_out, int32_t* __restrict__ pos_out, int32_t* __restrict__ inverse, int32_t* __restrict__ offsets) {
   __shared__ uint32_t s_cnt[kWaves][kMaxDigits];
   __shared__ uint32_t s_base[kMaxDigits];
   __shared__ uint32_t s_part[2 * kThreads];
   __shared__ int64_t s_wave[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t tile = blockIdx.x;
-  const int64_t first = tile * kTile + w * kSub + lane;
+  const int64_t first = (tile * kWaves + w) * (64 * CH) + lane;
+  const int64_t wave_left = n - (first - lane);  // (the same for the whole wave)
   for (int d = tid; d < nd; d += kThreads)
     for (int k = 0; k < kWaves; ++k) s_cnt[k][d] = 0u;
 
-  uint32_t key[kChunks];
-  int32_t pos[kChunks];
+  uint32_t key[CH];
+  int32_t pos[CH];
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
+  for (int c = 0; c < CH; ++c) {
     const int64_t i = first + c * 64;
     key[c] = i < n ? load_key<Id, KEYS>(src, i, n_keys) : 0u;
     pos[c] = pos_in != nullptr && i < n ? pos_in[i] : (int32_t)i;
   }
   __syncthreads();
-  uint32_t rank[kChunks];
+  uint32_t rank[CH];
   const uint32_t mask = (uint32_t)(nd - 1);
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
+  for (int c = 0; c < CH; ++c) {
+    rank[c] = 0u;
+    if (c * 64 >= wave_left) continue;
     const bool active = first + c * 64 < n;
     const uint32_t digit = (key[c] >> shift) & mask;
     const uint64_t peers = match_lanes<kMaxBits>(digit, __ballot(active), mask);
@@ -114,62 +115,55 @@ __global__ __launch_bounds__(kThreads) void select_scatter_kernel(
     }
     s_base[d] = run;
   }
-  if (mode == 2) {
-    __syncthreads();
-    for (int d = tid; d < nd; d += kThreads) s_base[d] = cnt[tile * nd + d];
-  } else {
-    // per digit: all tiles' count (tot) and that of the tiles before (pre)
-    uint32_t tot[kMaxDigits / kThreads + 1], pre[kMaxDigits / kThreads + 1];
-    const int per = nd > kThreads ? nd / kThreads : 1;
-    if (mode == 1) {
-      const int groups = nd < kThreads ? kThreads / nd : 1;
-      for (int j = 0; j < per; ++j) {
-        const int d = nd < kThreads ? tid % nd : tid * per + j;
-        uint32_t a = 0u, b = 0u;
+  // per digit: the count of all tiles (tot) and of those before this one (pre)
+  uint32_t tot[kMaxDigits / kThreads], pre[kMaxDigits / kThreads];
+  const int per = nd > kThreads ? nd / kThreads : 1;
+  if (mode == 1) {
+    const int groups = nd < kThreads ? kThreads / nd : 1;
+    for (int j = 0; j < per; ++j) {
+      const int d = nd < kThreads ? tid % nd : tid * per + j;
+      uint32_t a = 0u, b = 0u;
 #pragma unroll 8
-        for (int64_t t = nd < kThreads ? tid / nd : 0; t < n_tiles; t += groups) {
-          const uint32_t v = cnt[t * nd + d];
-          a += v;
-          b += t < tile ? v : 0u;
-        }
-        tot[j] = a;
-        pre[j] = b;
+      for (int64_t t = nd < kThreads ? tid / nd : 0; t < n_tiles; t += groups) {
+        const uint32_t v = cnt[t * nd + d];
+        a += v;
+        b += t < tile ? v : 0u;
       }
-      if (groups > 1) {
-        s_part[tid] = tot[0];
-        s_part[kThreads + tid] = pre[0];
-        __syncthreads();
-        if (tid < nd)
-          for (int g = 1; g < groups; ++g) {
-            tot[0] += s_part[g * nd + tid];
-            pre[0] += s_part[kThreads + g * nd + tid];
-          }
-      }
-    } else {
-      __syncthreads();
-      for (int j = 0; j < per; ++j) {
-        const int d = tid * per + j;
-        tot[j] = d < nd ? s_base[d] : 0u;
-        pre[j] = 0u;
-      }
+      tot[j] = a;
+      pre[j] = b;
     }
-    int64_t mine = 0, all;
-    if (tid * per < nd)
-      for (int j = 0; j < per; ++j) mine += tot[j];
-    uint32_t run = (uint32_t)block_exclusive_scan(mine, s_wave, all);
-    if (tid * per < nd)
-      for (int j = 0; j < per; ++j) {
-        s_base[tid * per + j] = run + pre[j];
-        // one pass: the digit is the key
-        if (offsets != nullptr && tile == 0 && (uint32_t)(tid * per + j) <= n_keys) offsets[tid * per + j] = (int32_t)run;
-        run += tot[j];
-      }
+    if (groups > 1) {
+      s_part[tid] = tot[0];
+      s_part[kThreads + tid] = pre[0];
+      __syncthreads();
+      if (tid < nd)
+        for (int g = 1; g < groups; ++g) {
+          tot[0] += s_part[g * nd + tid];
+          pre[0] += s_part[kThreads + g * nd + tid];
+        }
+    }
+  } else {
+    __syncthreads();
+    for (int j = 0; j < per; ++j) {
+      const int d = tid * per + j;
+      tot[j] = d < nd ? (mode == 0 ? s_base[d] : totals[d]) : 0u;
+      pre[j] = d < nd && mode == 2 ? cnt[tile * nd + d] : 0u;
+    }
   }
+  int64_t mine = 0, all;
+  if (tid * per < nd)
+    for (int j = 0; j < per; ++j) mine += tot[j];
+  uint32_t run = (uint32_t)block_exclusive_scan(mine, s_wave, all);
+  if (tid * per < nd)
+    for (int j = 0; j < per; ++j) {
+      s_base[tid * per + j] = run + pre[j];
+      // one pass: the digit is the key
+      if (offsets != nullptr && tile == 0 && (uint32_t)(tid * per + j) <= n_keys) offsets[tid * per + j] = (int32_t)run;
+      run += tot[j];
+    }
   __syncthreads();
-  if (mode == 2 && offsets != nullptr && tile == 0)
-    for (uint32_t d = tid; d <= n_keys; d += kThreads) offsets[d] = (int32_t)s_base[d];
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
+  for (int c = 0; c < CH; ++c) {
     const int64_t i = first + c * 64;
     if (i >= n) continue;
     const uint32_t digit = (key[c] >> shift) & mask;
@@ -191,24 +185,33 @@ Passes passes_of(int64_t n_keys) {
   return {count, (bits + count - 1) / count};
 }
 
+// Positions a tile: 512, 1024, 2048 or 4096, the fewest that make at most 64
+// tiles (more tiles are more rows for the scan, fewer leave compute units idle).
+int chunks_of(int64_t n) {
+  int ch = 1;
+  while (ch < 8 && n > (int64_t)kThreads * ch * 64) ch *= 2;
+  return ch;
+}
+
 struct SortLayout {
-  size_t cnt, partial, totals, keys[2], pos[2], bytes;
+  size_t cnt, totals, keys[2], pos[2], bytes;
+  int ch;
+  int64_t tiles;
 };
 SortLayout sort_layout(int64_t n, int64_t n_keys) {
   const Passes p = passes_of(n_keys);
-  const int64_t tiles = ceil_div(n, kTile), nd = (int64_t)1 << p.bits;
   SortLayout l{};
+  l.ch = chunks_of(n);
+  l.tiles = ceil_div(n, (int64_t)kThreads * l.ch);
+  const int64_t nd = (int64_t)1 << p.bits;
   size_t at = 0;
   auto take = [&](size_t b) {
     const size_t a = at;
     at += (b + 255) / 256 * 256;
     return a;
   };
-  if (tiles > 1) l.cnt = take((size_t)(tiles * nd) * 4);
-  if (tiles > kSelfScanTiles) {
-    l.partial = take((size_t)(ceil_div(tiles, kWgScanTiles) * nd) * 4);
-    l.totals = take((size_t)nd * 4);
-  }
+  if (l.tiles > 1) l.cnt = take((size_t)(l.tiles * nd) * 4);
+  if (l.tiles > kSelfScanTiles) l.totals = take((size_t)nd * 4);
   // passes before the last write keys and positions, in turn
   for (int k = 0; k < 2 && k + 1 < p.count; ++k) {
     l.keys[k] = take((size_t)n * 4);
@@ -218,35 +221,46 @@ SortLayout sort_layout(int64_t n, int64_t n_keys) {
   return l;
 }
 
-template <class Id, bool KEYS>
-int sort_pass(const void* src, const int32_t* pos_in, int64_t n, uint32_t n_keys, int shift, int nd, uint8_t* ws,
-              const SortLayout& l, uint32_t* keys_out, int32_t* pos_out, int32_t* inverse, int32_t* offsets,
-              hipStream_t s) {
-  const int64_t tiles = ceil_div(n, kTile);
+struct PassArgs {
+  const void* src;
+  const int32_t* pos_in;
+  int64_t n;
+  uint32_t n_keys;
+  int shift, nd;
+  uint32_t* keys_out;
+  int32_t *pos_out, *inverse, *offsets;
+};
+
+template <class Id, bool KEYS, int CH>
+int sort_pass(const PassArgs& a, uint8_t* ws, const SortLayout& l, hipStream_t s) {
   uint32_t* cnt = reinterpret_cast<uint32_t*>(ws + l.cnt);
+  uint32_t* totals = reinterpret_cast<uint32_t*>(ws + l.totals);
   int mode = 0;
-  if (tiles > 1) {
-    hipLaunchKernelGGL((select_count_kernel<Id, KEYS>), dim3((uint32_t)tiles), dim3(kThreads), 0, s, src, n, n_keys,
-                       shift, nd, cnt);
+  if (l.tiles > 1) {
+    hipLaunchKernelGGL((select_count_kernel<Id, KEYS, CH>), dim3((uint32_t)l.tiles), dim3(kThreads), 0, s, a.src, a.n,
+                       a.n_keys, a.shift, a.nd, cnt);
     FS_CHECK_LAUNCH("select_count_kernel");
     mode = 1;
-    if (tiles > kSelfScanTiles) {
+    if (l.tiles > kSelfScanTiles) {
       mode = 2;
-      uint32_t* partial = reinterpret_cast<uint32_t*>(ws + l.partial);
-      uint32_t* totals = reinterpret_cast<uint32_t*>(ws + l.totals);
-      const int64_t blocks = ceil_div(tiles, kWgScanTiles);
-      hipLaunchKernelGGL(wg_scan_reduce_kernel, dim3((uint32_t)blocks), dim3(256), 0, s, cnt, tiles, nd, partial);
-      FS_CHECK_LAUNCH("wg_scan_reduce_kernel");
-      hipLaunchKernelGGL(wg_scan_column_kernel, dim3((uint32_t)nd), dim3(256), 0, s, partial, blocks, nd, totals);
+      hipLaunchKernelGGL(wg_scan_column_kernel, dim3((uint32_t)a.nd), dim3(256), 0, s, cnt, l.tiles, a.nd, totals);
       FS_CHECK_LAUNCH("wg_scan_column_kernel");
-      hipLaunchKernelGGL(wg_scan_down_kernel, dim3((uint32_t)blocks), dim3(256), 0, s, cnt, tiles, nd, partial, totals);
-      FS_CHECK_LAUNCH("wg_scan_down_kernel");
     }
   }
-  hipLaunchKernelGGL((select_scatter_kernel<Id, KEYS>), dim3((uint32_t)tiles), dim3(kThreads), 0, s, src, pos_in, n,
-                     n_keys, shift, nd, cnt, tiles, mode, keys_out, pos_out, inverse, offsets);
+  hipLaunchKernelGGL((select_scatter_kernel<Id, KEYS, CH>), dim3((uint32_t)l.tiles), dim3(kThreads), 0, s, a.src,
+                     a.pos_in, a.n, a.n_keys, a.shift, a.nd, cnt, totals, l.tiles, mode, a.keys_out, a.pos_out,
+                     a.inverse, a.offsets);
   FS_CHECK_MAIN_LAUNCH("select_scatter_kernel");
   return FS_OK;
+}
+template <class Id, bool KEYS>
+int sort_pass(const PassArgs& a, uint8_t* ws, const SortLayout& l, hipStream_t s) {
+  switch (l.ch) {
+    case 1: return sort_pass<Id, KEYS, 1>(a, ws, l, s);
+    case 2: return sort_pass<Id, KEYS, 2>(a, ws, l, s);
+    case 4: return sort_pass<Id, KEYS, 4>(a, ws, l, s);
+  }
+  return sort_pass<Id, KEYS, 8>(a, ws, l, s);
 }
 
 __global__ __launch_bounds__(256) void zero_offsets_kernel(int32_t* __restrict__ p, int64_t n) {
@@ -279,10 +293,10 @@ int select_sort(const void* ids, int id_t, int64_t n, int64_t n_keys, uint32_t* 
     uint32_t* ko = last ? keys_out : reinterpret_cast<uint32_t*>(ws + l.keys[k & 1]);
     int32_t* po = last ? order : reinterpret_cast<int32_t*>(ws + l.pos[k & 1]);
     int32_t* inv = last ? inverse : nullptr;
-    int rc;
-    if (k > 0) rc = sort_pass<int32_t, true>(src, pos, n, (uint32_t)n_keys, k * p.bits, nd, ws, l, ko, po, inv, offsets, s);
-    else if (id_t == FS_I64) rc = sort_pass<int64_t, false>(src, pos, n, (uint32_t)n_keys, 0, nd, ws, l, ko, po, inv, offsets, s);
-    else rc = sort_pass<int32_t, false>(src, pos, n, (uint32_t)n_keys, 0, nd, ws, l, ko, po, inv, offsets, s);
+    const PassArgs a{src, pos, n, (uint32_t)n_keys, k * p.bits, nd, ko, po, inv, offsets};
+    const int rc = k > 0            ? sort_pass<int32_t, true>(a, ws, l, s)
+                   : id_t == FS_I64 ? sort_pass<int64_t, false>(a, ws, l, s)
+                                    : sort_pass<int32_t, false>(a, ws, l, s);
     if (rc != FS_OK) return rc;
     src = ko;
     pos = po;
