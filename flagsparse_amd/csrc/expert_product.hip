@@ -120,11 +120,12 @@ struct Frags {
 #pragma unroll
     for (int j = 0; j < (KC ? 1 : F); ++j) at[j] = O::frag_offset(r0 + j * 16, lane);
   }
+  // (the first `some` of them)
   template <class X>
-  __device__ void read(uint32_t slice, X (&f)[F]) const {
+  __device__ void read(uint32_t slice, X (&f)[F], int some = F) const {
 #pragma unroll
     for (int j = 0; j < F; ++j)
-      f[j] = O::frag((const lds_byte*)(uintptr_t)(slice + at[KC ? 0 : j]) + (KC ? j * 16 * kRowBytes : 0));
+      if (j < some) f[j] = O::frag((const lds_byte*)(uintptr_t)(slice + at[KC ? 0 : j]) + (KC ? j * 16 * kRowBytes : 0));
   }
 };
 
@@ -307,6 +308,65 @@ __device__ inline bool find_tile(const ProductArgs& p, uint32_t nt, int lane, Ti
 
 enum Mode { kRowsTrans = 0, kRowsNon = 1, kMatrix = 2 };
 
+// A workgroup's tile: both operands, the result, and how much of it there is.
+template <class T>
+struct TileWork {
+  Source<T> a, b;
+  T* c;
+  int c_rows, c_cols;
+};
+
+template <class T, int MODE, int BM, int BN>
+__device__ inline bool tile_work(const ProductArgs& p, int lane, TileWork<T>& o) {
+  const uint32_t nt = (uint32_t)((p.n + BN - 1) / BN);
+  TileAt t;
+  if constexpr (MODE == kMatrix) {
+    // an expert's tiles over all XCDs: with an expert or two to an XCD the one
+    // with the most rows was waited for (1522 us with popularities log-normal,
+    // sigma 0.5, over 16 experts of 4096 x 4096; 1022 so)
+    const uint32_t mt = (uint32_t)((p.m + BM - 1) / BM), per = mt * nt;
+    t.expert = (int)(blockIdx.x / per);
+    tile_in_group((uint32_t)xcd_range_block(blockIdx.x % per, per), mt, nt, t);
+    const int64_t r0 = p.offsets[t.expert], m0 = (int64_t)t.m * BM;
+    o.a.k = o.b.k = p.offsets[t.expert + 1] - r0;
+    o.a.base = (const T*)p.a + r0 * p.lda + m0;
+    o.b.base = (const T*)p.b + r0 * p.ldb;
+    o.a.tile_rows = (int)(p.m - m0 < BM ? p.m - m0 : BM);
+    o.c = (T*)p.c + (int64_t)t.expert * p.c_expert + m0 * p.ldc;
+  } else {
+    if (!find_tile<BM>(p, nt, lane, t)) return false;
+    o.a.k = o.b.k = t.expert < p.n_experts ? p.k : 0;
+    o.a.base = (const T*)p.a + t.row0 * p.lda;
+    o.b.base = (const T*)p.b + (int64_t)t.expert * p.b_expert;
+    o.a.tile_rows = t.rows;
+    o.c = (T*)p.c + t.row0 * p.ldc;
+  }
+  const int64_t n0 = (int64_t)t.n * BN;
+  o.b.base += MODE == kRowsTrans ? n0 * p.ldb : n0;
+  o.b.tile_rows = (int)(p.n - n0 < BN ? p.n - n0 : BN);
+  o.a.ld = p.lda;
+  o.b.ld = p.ldb;
+  o.c += n0;
+  o.c_rows = o.a.tile_rows;
+  o.c_cols = o.b.tile_rows;
+  return true;
+}
+
+// Four neighbouring columns of a result row, from column n of the tile.
+template <class T>
+__device__ inline void store_four(T* row, int n, int cols, f32x4 v) {
+  T out[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = (T)v[e];
+  if (n + 4 <= cols) {
+    __builtin_memcpy(row + n, out, sizeof out);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (n + e < cols) row[n + e] = out[e];
+  }
+}
+
 template <class T, int MODE, bool DMA, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const ProductArgs p) {
   constexpr int THREADS = 64 * WM * WN;
@@ -319,42 +379,18 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
   __shared__ alignas(1024) uint8_t s_mem[kSlots][kSlot];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t nt = (uint32_t)((p.n + BN - 1) / BN);
-  TileAt t;
-  Source<T> sa, sb;
-  T* c;
-  int c_rows;
-  if constexpr (MODE == kMatrix) {
-    const uint32_t mt = (uint32_t)((p.m + BM - 1) / BM), id = (uint32_t)xcd_range_block(blockIdx.x, gridDim.x);
-    t.expert = (int)(id / (mt * nt));
-    tile_in_group(id % (mt * nt), mt, nt, t);
-    const int64_t r0 = p.offsets[t.expert], m0 = (int64_t)t.m * BM;
-    sa.k = sb.k = p.offsets[t.expert + 1] - r0;
-    sa.base = (const T*)p.a + r0 * p.lda + m0;
-    sb.base = (const T*)p.b + r0 * p.ldb;
-    sa.tile_rows = (int)(p.m - m0 < BM ? p.m - m0 : BM);
-    c = (T*)p.c + (int64_t)t.expert * p.c_expert + m0 * p.ldc;
-    c_rows = sa.tile_rows;
-  } else {
-    if (!find_tile<BM>(p, nt, lane, t)) return;
-    sa.k = sb.k = t.expert < p.n_experts ? p.k : 0;
-    sa.base = (const T*)p.a + t.row0 * p.lda;
-    sb.base = (const T*)p.b + (int64_t)t.expert * p.b_expert;
-    sa.tile_rows = c_rows = t.rows;
-    c = (T*)p.c + t.row0 * p.ldc;
-  }
-  const int64_t n0 = (int64_t)t.n * BN;
-  sb.base += BKC ? n0 * p.ldb : n0;
-  sb.tile_rows = (int)(p.n - n0 < BN ? p.n - n0 : BN);
-  sa.ld = p.lda;
-  sb.ld = p.ldb;
-  c += n0;
+  TileWork<T> work;
+  if (!tile_work<T, MODE, BM, BN>(p, lane, work)) return;
+  const Source<T>&sa = work.a, &sb = work.b;
 
   const int wm = w / WN, wn = w % WN;
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_byte*)&s_mem[0][0];
   Frags<OA, AKC, FM> from_a;
   Frags<OB, BKC, FN> from_b;
-  from_a.init(wm * (BM / WM), lane);
+  // 16-row blocks of a wave: half of what the tile has where two groups of waves
+  // share it (an expert's last tile may have few rows)
+  const int fm = WM * WN == 8 ? (work.c_rows + 31) / 32 : FM;
+  from_a.init(wm * fm * 16, lane);
   from_b.init(wn * (BN / WN), lane);
 
   f32x4 acc[FM][FN];
@@ -365,24 +401,19 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
 
   const int64_t steps = (sa.k + BK - 1) / BK;
   typename Mma<T>::frag fa[FM], fb[FN];
-  auto read_frags = [&](uint32_t slot) {
+  auto read_frags = [&](uint32_t slot, int some) {
     from_b.read(slot + OA::kBytes, fb);
-    from_a.read(slot, fa);
+    from_a.read(slot, fa, some);
   };
   auto multiply_row = [&](int i) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::run(fb[j], fa[i], acc[i][j]);
   };
   if constexpr (DMA) {
-    // Two groups of four waves, one wave a SIMD each, half a step apart: one
-    // multiplies and starts the loads of three steps ahead while the other
-    // reads fragments.  Every wave starts its share of every step's loads, also
-    // of the three steps past the last (zeros), so that counting the loads
-    // still under way tells which step has arrived.
-    static_assert(WM * WN == 8, "two waves a SIMD");
+    // Loads are started three steps ahead.  Every wave starts its share of every
+    // step's, also of the three steps past the last (zeros), so that counting
+    // those still under way tells which step has arrived.
     constexpr int kLoads = OA::kPieces + OB::kPieces;
-    static_assert(kLoads <= FM, "a load between the products of two rows");
-    const bool second = w >= 4;
     Dma<OA, T, AKC, THREADS> da;
     Dma<OB, T, BKC, THREADS> db;
     da.init(sa, tid);
@@ -408,27 +439,49 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) load(i);
     }
-    wait_loads<2 * kLoads>();
-    barrier();
-    if (second) barrier();
-    for (int64_t kt = 0; kt < steps; ++kt) {
-      read_frags(lds + (uint32_t)(kt & 3) * kSlot);
-      begin_loads(kt + 3);
-      wait_reads();
-      if (second) wait_loads<kLoads>();  // step kt + 1, which the first group reads next
+    if constexpr (WM * WN == 8) {
+      // Two groups of four waves, one wave a SIMD each, half a step apart: one
+      // multiplies, and starts loads in between, while the other reads fragments.
+      static_assert(kLoads <= FM, "a load between the products of two rows");
+      const bool second = w >= 4;
+      wait_loads<2 * kLoads>();
       barrier();
-      __builtin_amdgcn_s_setprio(1);
+      if (second) barrier();
+      auto run = [&](auto whole) {
+        for (int64_t kt = 0; kt < steps; ++kt) {
+          read_frags(lds + (uint32_t)(kt & 3) * kSlot, whole ? FM : fm);
+          begin_loads(kt + 3);
+          wait_reads();
+          if (second) wait_loads<kLoads>();  // step kt + 1, which the first group reads next
+          barrier();
+          __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        multiply_row(i);
-        if (i < kLoads) load(i);  // its slot was last read two phases ago
-        __builtin_amdgcn_sched_barrier(0);
+          for (int i = 0; i < FM; ++i) {
+            if (whole || i < fm) multiply_row(i);
+            if (i < kLoads) load(i);  // its slot was last read two phases ago
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          __builtin_amdgcn_s_setprio(0);
+          if (!second) wait_loads<2 * kLoads>();
+          barrier();
+        }
+      };
+      if (fm == FM) run(std::true_type{});
+      else run(std::false_type{});
+      if (!second) barrier();
+    } else {
+      for (int64_t kt = 0; kt < steps; ++kt) {
+        wait_reads();
+        wait_loads<2 * kLoads>();
+        barrier();  // step kt has arrived, step kt - 1 has been read
+        begin_loads(kt + 3);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) load(i);
+        read_frags(lds + (uint32_t)(kt & 3) * kSlot, FM);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) multiply_row(i);
       }
-      __builtin_amdgcn_s_setprio(0);
-      if (!second) wait_loads<2 * kLoads>();
-      barrier();
     }
-    if (!second) barrier();
     wait_loads<0>();
   } else {
     u32x4 ra[OA::kPieces], rb[OB::kPieces];
@@ -446,41 +499,131 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
       }
       // one barrier a step: the slot written next was last read before it
       __syncthreads();
-      read_frags(slot);
+      read_frags(slot, FM);
 #pragma unroll
       for (int i = 0; i < FM; ++i) multiply_row(i);
     }
   }
 
   // lane l holds row l % 16 and 4 neighbouring columns of each 16x16 result
-  const int cm = wm * (BM / WM) + (lane & 15), cn = wn * (BN / WN) + (lane >> 4) * 4;
+  const int cm = wm * fm * 16 + (lane & 15), cn = wn * (BN / WN) + (lane >> 4) * 4;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int m = cm + i * 16;
-    if (m >= c_rows) continue;
-    T* row = c + (int64_t)m * p.ldc;
+    if (i >= fm || m >= work.c_rows) continue;
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int n = cn + j * 16;
-      T out[4];
+    for (int j = 0; j < FN; ++j) store_four(work.c + (int64_t)m * p.ldc, cn + j * 16, work.c_cols, acc[i][j]);
+  }
+}
+
+// Few rows an expert: the matrices' bytes are what counts.  16 x 64 tiles, and
+// the four waves of a workgroup take every fourth step of k, each through slots
+// of its own and without barriers, so that many loads are under way; their sums
+// are added in wave order at the end.
+constexpr int kFewRows = 16, kFewCols = 64;
+template <class T, int MODE, bool DMA>
+__global__ __launch_bounds__(256) void expert_product_few_kernel(const ProductArgs p) {
+  constexpr bool BKC = MODE == kRowsTrans;
+  using OA = Operand<T, true, kFewRows, 64>;
+  using OB = Operand<T, BKC, kFewCols, 64>;
+  constexpr int BK = OA::BK, FN = kFewCols / 16, kWaves = 4;
+  constexpr int kSlots = DMA ? 4 : 1, kSlot = OA::kBytes + OB::kBytes;
+  static_assert(kSlots * kSlot >= FN * 64 * 16, "a wave's sums fit its slots");
+  __shared__ alignas(1024) uint8_t s_mem[kWaves][kSlots][kSlot];
+
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  TileWork<T> work;
+  if (!tile_work<T, MODE, kFewRows, kFewCols>(p, lane, work)) return;
+  const Source<T>&sa = work.a, &sb = work.b;
+  const uint32_t lds = (uint32_t)(uintptr_t)(lds_byte*)&s_mem[w][0][0];
+  Frags<OA, true, 1> from_a;
+  Frags<OB, BKC, FN> from_b;
+  from_a.init(0, lane);
+  from_b.init(0, lane);
+  f32x4 acc[FN];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] = (T)acc[i][j][e];
-      if constexpr (DMA) {  // (whole 16-byte pieces)
-        if (n < sb.tile_rows) __builtin_memcpy(__builtin_assume_aligned(row + n, sizeof out), out, sizeof out);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < sb.tile_rows) row[n + e] = out[e];
+  for (int j = 0; j < FN; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  typename Mma<T>::frag fa[1], fb[FN];
+  auto read_frags = [&](uint32_t slot) {
+    from_a.read(slot, fa);
+    from_b.read(slot + OA::kBytes, fb);
+  };
+  const int64_t steps = (sa.k + BK - 1) / BK;
+
+  if constexpr (DMA) {
+    constexpr int kLoads = OA::kPieces + OB::kPieces;
+    Dma<OA, T, true, 64> da;
+    Dma<OB, T, BKC, 64> db;
+    da.init(sa, lane);
+    db.init(sb, lane);
+    auto load = [&](int64_t i) {  // the wave's i-th step
+      const int64_t kt = w + i * kWaves, left = sa.k - kt * BK;
+      if (left < BK) {
+        da.cut(left, lane);
+        db.cut(left, lane);
       }
+      const u32x4 ra = da.at(kt), rb = db.at(kt);
+      const uint32_t next = lds + (uint32_t)(i & 3) * kSlot;
+#pragma unroll
+      for (int q = 0; q < OA::kPieces; ++q) da.issue(next, ra, q, 0);
+#pragma unroll
+      for (int q = 0; q < OB::kPieces; ++q) db.issue(next + OA::kBytes, rb, q, 0);
+    };
+    for (int i = 0; i < 3; ++i) load(i);
+    for (int64_t i = 0; w + i * kWaves < steps; ++i) {
+      wait_loads<2 * kLoads>();
+      read_frags(lds + (uint32_t)(i & 3) * kSlot);
+      load(i + 3);  // (into the slot read last time round)
+      wait_reads();
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[j] = Mma<T>::run(fb[j], fa[0], acc[j]);
+    }
+    wait_loads<0>();
+  } else {
+    u32x4 ra[2][OA::kPieces], rb[2][OB::kPieces];
+    auto load = [&](int64_t i, int q) {
+      if (w + i * kWaves >= steps) return;
+      load_pieces<OA, T, true>(sa, w + i * kWaves, lane, ra[q]);
+      load_pieces<OB, T, BKC>(sb, w + i * kWaves, lane, rb[q]);
+    };
+    auto step = [&](int64_t i, int q) {
+      if (w + i * kWaves >= steps) return;
+      store_pieces<OA>(lds, lane, ra[q], 64);
+      store_pieces<OB>(lds + OA::kBytes, lane, rb[q], 64);
+      load(i + 2, q);
+      wait_reads();  // (one wave: its own stores)
+      read_frags(lds);
+      wait_reads();
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[j] = Mma<T>::run(fb[j], fa[0], acc[j]);
+    };
+    load(0, 0);
+    load(1, 1);
+    for (int64_t i = 0; w + i * kWaves < steps; i += 2) {
+      step(i, 0);
+      step(i + 1, 1);
     }
   }
+
+#pragma unroll
+  for (int j = 0; j < FN; ++j) *(f32x4*)&s_mem[w][0][(j * 64 + lane) * 16] = acc[j];
+  __syncthreads();
+  f32x4 sum = *(const f32x4*)&s_mem[0][0][tid * 16];
+#pragma unroll
+  for (int k = 1; k < kWaves; ++k) sum += *(const f32x4*)&s_mem[k][0][tid * 16];
+  const int m = lane & 15;
+  if (m < work.c_rows) store_four(work.c + (int64_t)m * p.ldc, w * 16 + (lane >> 4) * 4, work.c_cols, sum);
+}
+
+template <int MODE, int BM, int BN>
+int64_t tiles_of(const ProductArgs& p) {
+  const int64_t nt = ceil_div(p.n, BN);
+  return MODE == kMatrix ? ceil_div(p.m, BM) * nt * p.n_experts : (p.n_rows / BM + p.n_experts + 1) * nt;
 }
 
 template <class T, int MODE, bool DMA, int BM, int BN, int WM, int WN>
 int launch_tiles(const ProductArgs& p, hipStream_t stream) {
-  const int64_t nt = ceil_div(p.n, BN);
-  const int64_t tiles = MODE == kMatrix ? ceil_div(p.m, BM) * nt * p.n_experts
-                                        : (p.n_rows / BM + p.n_experts + 1) * nt;
+  const int64_t tiles = tiles_of<MODE, BM, BN>(p);
   if (tiles > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
   hipLaunchKernelGGL((expert_product_kernel<T, MODE, DMA, BM, BN, WM, WN>), dim3((uint32_t)tiles),
                      dim3(64 * WM * WN), 0, stream, p);
@@ -488,16 +631,59 @@ int launch_tiles(const ProductArgs& p, hipStream_t stream) {
   return FS_OK;
 }
 
+template <class T, int MODE, bool DMA>
+int launch_few(const ProductArgs& p, hipStream_t stream) {
+  const int64_t tiles = tiles_of<MODE, kFewRows, kFewCols>(p);
+  if (tiles > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
+  hipLaunchKernelGGL((expert_product_few_kernel<T, MODE, DMA>), dim3((uint32_t)tiles), dim3(256), 0, stream, p);
+  FS_CHECK_MAIN_LAUNCH("expert_product_few_kernel");
+  return FS_OK;
+}
+
+// Which tiles.  The larger, the fewer times operands are read and the nearer to
+// the matrix cores' rate, if rows fill them and there are enough for the chip
+// (kFill).  us, bf16, 32 experts 2048 x 4096, rows an expert on average; tiles
+// few / 64 x 128 / 128 x 128 / 256 x 256:
+//   matrices (K, N)      4: 107  96  92  90     32: 154 106 105  95   128: 422 188 165 115
+//   (N, K), "trans"      4: 100 107 112 132     32: 164 114 119 138   128: 414 181 160 154
+//   matrix gradient                              32:  -  213 203 190   512:  -  516 457 395
+//   float32, (K, N)      8: 188 263 485 995     32: 302 276 486 993  1024:  - 2258 2093 2519 (16 experts)
+//   no whole 16 bytes    8: 141 148 188         32: 229 151 203       128: 595 317 277
+// Large tiles read whole lines of (K, N) matrices, which is why they serve few
+// rows too; of (N, K) ones they read 64 bytes of a row at a time.  One token
+// (8 experts of 64, 4096 columns): few 28, 64 x 128 23, 256 x 256 42; (1 of 8,
+// 4096 x 4096): 12, 28, 72.
+constexpr int64_t kFill = 256;
+
 template <class T, int MODE>
 int launch_product(const ProductArgs& p, hipStream_t stream) {
   // straight to LDS: whole 16-byte pieces, and offsets within a step that fit
   const int64_t s = sizeof(T), reach = MODE == kMatrix ? kRowBytes / s : 256;
   const bool dma = aligned16(p.a, p.lda * s) && aligned16(p.b, p.ldb * s) && p.b_expert * s % 16 == 0 &&
-                   aligned16(p.c, p.ldc * s) &&
                    (MODE == kMatrix ? p.m : p.k) * s % 16 == 0 && (MODE == kRowsTrans ? p.k : p.n) * s % 16 == 0 &&
                    reach * std::max(p.lda, p.ldb) * s < (int64_t)kInBuffer;
-  if (!dma) return launch_tiles<T, MODE, false, 128, 128, 2, 2>(p, stream);
-  return launch_tiles<T, MODE, true, 256, 256, 2, 4>(p, stream);
+  constexpr bool kHalf = sizeof(T) == 2;
+  if constexpr (MODE == kMatrix) {
+    if constexpr (kHalf)
+      if (dma && tiles_of<MODE, 256, 256>(p) >= kFill) return launch_tiles<T, MODE, true, 256, 256, 2, 4>(p, stream);
+    if (tiles_of<MODE, 128, 128>(p) >= kFill)
+      return dma ? launch_tiles<T, MODE, true, 128, 128, 2, 2>(p, stream)
+                 : launch_tiles<T, MODE, false, 128, 128, 2, 2>(p, stream);
+  } else {
+    const int64_t rows = p.n_rows / p.n_experts, active = std::min<int64_t>(p.n_rows, p.n_experts);
+    const int64_t tiles256 = ceil_div(p.n, 256) * std::max(active, p.n_rows / 256);
+    const int64_t tiles128 = ceil_div(p.n, 128) * std::max(active, p.n_rows / 128);
+    if constexpr (kHalf)
+      if (dma && (rows >= 112                ? tiles256 >= kFill
+                  : MODE == kRowsNon && rows >= 4 && tiles256 >= 2 * kFill))
+        return launch_tiles<T, MODE, true, 256, 256, 2, 4>(p, stream);
+    if (rows < (kHalf ? 12 : 20)) return dma ? launch_few<T, MODE, true>(p, stream) : launch_few<T, MODE, false>(p, stream);
+    if (rows >= (kHalf ? 40 : 768) && tiles128 >= kFill)
+      return dma ? launch_tiles<T, MODE, true, 128, 128, 2, 2>(p, stream)
+                 : launch_tiles<T, MODE, false, 128, 128, 2, 2>(p, stream);
+  }
+  return dma ? launch_tiles<T, MODE, true, 64, 128, 2, 2>(p, stream)
+             : launch_tiles<T, MODE, false, 64, 128, 2, 2>(p, stream);
 }
 
 template <int MODE>

@@ -99,6 +99,15 @@ def test_routed(dtype, op, n_tokens, slots, n_experts):
         _check(dtype, op, counts.tolist(), inner, outer, seed=outer)
 
 
+# enough and large enough tiles for the largest ones: of rows (first two), of the matrices' gradient (last)
+@pytest.mark.parametrize("counts,inner,outer", [((700, 1, 513, 900), 264, 5512), ((256, 0, 1024), 40, 12808),
+                                                ((300, 0, 5, 260), 2056, 2080)], ids=["rows", "short", "matrices"])
+@pytest.mark.parametrize("op", ["non", "trans"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_many_tiles(dtype, op, counts, inner, outer):
+    _check(dtype, op, counts, inner, outer, dropped=70)
+
+
 @pytest.mark.parametrize("op", ["non", "trans"])
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_neighbours_do_not_leak(dtype, op):
