@@ -102,7 +102,9 @@ EXPORTED_SYMBOLS = (
     "fs_expert_dispatch",
     "fs_expert_combine",
     "fs_expert_combine_grad",
+    "fs_expert_product_workspace_bytes",
     "fs_expert_product",
+    "fs_expert_product_grad_matrices_workspace_bytes",
     "fs_expert_product_grad_matrices",
 )
 
@@ -283,11 +285,15 @@ def _declare(lib):
     lib.fs_expert_combine_grad.restype = _i32
     lib.fs_expert_combine_grad.argtypes = [_i32, _i64, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
                                            _vp]
+    lib.fs_expert_product_workspace_bytes.restype = _sz
+    lib.fs_expert_product_workspace_bytes.argtypes = [_i32, _i32, _i64, _i64, _i64, _i64]
     lib.fs_expert_product.restype = _i32
-    lib.fs_expert_product.argtypes = [_i32, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp]
+    lib.fs_expert_product.argtypes = [_i32, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp]
+    lib.fs_expert_product_grad_matrices_workspace_bytes.restype = _sz
+    lib.fs_expert_product_grad_matrices_workspace_bytes.argtypes = [_i32, _i32, _i64, _i64, _i64, _i64]
     lib.fs_expert_product_grad_matrices.restype = _i32
     lib.fs_expert_product_grad_matrices.argtypes = [_i32, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp,
-                                                    _vp]
+                                                    _vp, _sz, _vp]
     lib.fs_last_kernel.restype = ctypes.c_char_p
     lib.fs_last_kernel.argtypes = []
 

@@ -245,6 +245,8 @@ struct ProductArgs {
   int64_t n_rows;          // rows of A
   int64_t m, n, k;         // m: of a matrix gradient; k: of a product of rows
   int n_experts;
+  int cus;                 // compute units
+  float* parts;            // room for the sums of split tiles, or null
 };
 
 struct TileAt {
@@ -264,51 +266,124 @@ __device__ inline void tile_in_group(uint32_t r, uint32_t mt, uint32_t nt, TileA
   t.n = (int)(g * kGroupN + q % gn);
 }
 
-__device__ inline int wave_scan(int v, int lane) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int u = __shfl_up(v, off);
-    if (lane >= off) v += u;
-  }
-  return v;
+enum Mode { kRowsTrans = 0, kRowsNon = 1, kMatrix = 2 };
+
+// The tiles of a call: `real` ones, of which the last `rest` are each shared by
+// `parts` workgroups, and those of rows of no expert, only written.
+struct TilePlan {
+  uint32_t real, zero, full, rest, parts;
+};
+
+// Tiles of a last round that leaves most of the chip idle are cut along k into
+// the parts that take the least time: a tile takes about 0.8 us a step, writing
+// and adding a tile's sums 0.085 us a part and tile, so parts^2 = 9 steps / rest.
+__host__ __device__ inline uint32_t parts_of(uint32_t rest, int64_t steps, uint32_t cus) {
+  uint32_t parts = 1;
+  while (rest > 0 && parts < 16 && (parts + 1) * rest <= cus &&
+         (int64_t)(parts + 1) * (parts + 1) * rest <= 9 * steps)
+    ++parts;
+  return parts;
 }
 
-// The workgroup's tile of a product of rows, or false.  All waves alike.
+// (All waves alike; so are the places below.)
+template <int MODE, int BM, int BN>
+__device__ inline TilePlan plan_tiles(const ProductArgs& p, int lane) {
+  const uint32_t nt = (uint32_t)((p.n + BN - 1) / BN);
+  TilePlan l;
+  int64_t steps;
+  constexpr int kStep = kRowBytes / 2;  // k of a step of 16-bit values: only they are split
+  if constexpr (MODE == kMatrix) {
+    l.real = (uint32_t)((p.m + BM - 1) / BM) * nt * (uint32_t)p.n_experts;
+    l.zero = 0;
+    steps = p.n_rows / p.n_experts / kStep;
+  } else {
+    int total = 0;
+    for (int e0 = 0; e0 < p.n_experts; e0 += 64) {
+      const int e = e0 + lane;
+      const int own = e < p.n_experts ? (p.offsets[e + 1] - p.offsets[e] + BM - 1) / BM : 0;
+      total += __builtin_amdgcn_readlane((int)wave_sum_scan((uint32_t)own), 63);
+    }
+    l.real = (uint32_t)total * nt;
+    l.zero = (uint32_t)((p.n_rows - p.offsets[p.n_experts] + BM - 1) / BM) * nt;
+    steps = p.k / kStep;
+  }
+  l.full = l.real;
+  l.rest = 0;
+  l.parts = 1;
+  if (p.parts != nullptr) {
+    const uint32_t rest = l.real % (uint32_t)p.cus, parts = parts_of(rest, steps, (uint32_t)p.cus);
+    if (parts > 1) {
+      l.rest = rest;
+      l.parts = parts;
+      l.full = l.real - rest;
+    }
+  }
+  return l;
+}
+
+// A workgroup's tile, or one part of it.
+struct Share {
+  uint32_t tile, part, parts, slot;
+};
+template <int MODE, int BM, int BN>
+__device__ inline bool find_share(const ProductArgs& p, const TilePlan& l, uint32_t block, Share& s) {
+  s.part = 0;
+  s.parts = 1;
+  if (block < l.full) {
+    if constexpr (MODE == kMatrix) {
+      // an expert's tiles over all XCDs: with an expert or two to an XCD the one
+      // with the most rows was waited for (1538 us with popularities log-normal,
+      // sigma 0.5, over 16 experts of 4096 x 4096; 1022 so)
+      const uint32_t per = (uint32_t)((p.m + BM - 1) / BM) * (uint32_t)((p.n + BN - 1) / BN);
+      const uint32_t first = block / per * per, here = l.full - first < per ? l.full - first : per;
+      s.tile = first + (uint32_t)xcd_range_block(block - first, here);
+    } else {
+      s.tile = (uint32_t)xcd_range_block(block, l.full);
+    }
+    return true;
+  }
+  block -= l.full;
+  if (block < l.rest * l.parts) {
+    s.tile = l.full + block % l.rest;
+    s.part = block / l.rest;
+    s.parts = l.parts;
+    s.slot = block % l.rest * l.parts + s.part;
+    return true;
+  }
+  block -= l.rest * l.parts;
+  s.tile = l.real + block;
+  return block < l.zero;
+}
+
+// Where tile `id` of a product of rows lies.
 template <int BM>
-__device__ inline bool find_tile(const ProductArgs& p, uint32_t nt, int lane, TileAt& t) {
+__device__ inline void find_tile(const ProductArgs& p, uint32_t nt, int lane, uint32_t id, TileAt& t) {
   const int E = p.n_experts;
-  auto tiles_of = [&](int e) {
-    if (e > E) return 0;
-    const int64_t a = p.offsets[e], b = e < E ? (int64_t)p.offsets[e + 1] : p.n_rows;
-    return (int)((b - a + BM - 1) / BM);
-  };
-  int total = 0;
-  for (int e = 0; e <= E; e += 64) total += __builtin_amdgcn_readlane(wave_scan(tiles_of(e + lane), lane), 63);
-  const uint32_t all = (uint32_t)total * nt;
-  if (blockIdx.x >= all) return false;
-  const uint32_t id = (uint32_t)xcd_range_block(blockIdx.x, all), q = id / nt;
+  const uint32_t q = id / nt;
   int before = 0;
-  for (int e = 0; e <= E; e += 64) {
-    const int own = tiles_of(e + lane), upto = wave_scan(own, lane) + before;
+  for (int e = 0;; e += 64) {
+    int own = 0;
+    if (e + lane <= E) {
+      const int64_t a = p.offsets[e + lane], b = e + lane < E ? (int64_t)p.offsets[e + lane + 1] : p.n_rows;
+      own = (int)((b - a + BM - 1) / BM);
+    }
+    const int upto = (int)wave_sum_scan((uint32_t)own) + before;
     const uint64_t m = __ballot((uint32_t)upto > q);
-    if (m != 0) {
-      const int l = __builtin_ctzll(m);
+    if (m != 0 || e + 64 > E) {  // (found: id is below the number of tiles)
+      const int l = m != 0 ? __builtin_ctzll(m) : 0;
       const int mt = __builtin_amdgcn_readlane(own, l), first = __builtin_amdgcn_readlane(upto, l) - mt;
       t.expert = e + l;
       tile_in_group(id - (uint32_t)first * nt, (uint32_t)mt, nt, t);
       const int64_t a = p.offsets[t.expert], b = t.expert < E ? (int64_t)p.offsets[t.expert + 1] : p.n_rows;
       t.row0 = a + (int64_t)t.m * BM;
       t.rows = (int)(b - t.row0 < BM ? b - t.row0 : BM);
-      return true;
+      return;
     }
     before = __builtin_amdgcn_readlane(upto, 63);
   }
-  return false;
 }
 
-enum Mode { kRowsTrans = 0, kRowsNon = 1, kMatrix = 2 };
-
-// A workgroup's tile: both operands, the result, and how much of it there is.
+// A tile: both operands, the result, and how much of it there is.
 template <class T>
 struct TileWork {
   Source<T> a, b;
@@ -317,16 +392,14 @@ struct TileWork {
 };
 
 template <class T, int MODE, int BM, int BN>
-__device__ inline bool tile_work(const ProductArgs& p, int lane, TileWork<T>& o) {
+__device__ inline TileWork<T> tile_work(const ProductArgs& p, int lane, uint32_t id) {
   const uint32_t nt = (uint32_t)((p.n + BN - 1) / BN);
+  TileWork<T> o;
   TileAt t;
   if constexpr (MODE == kMatrix) {
-    // an expert's tiles over all XCDs: with an expert or two to an XCD the one
-    // with the most rows was waited for (1522 us with popularities log-normal,
-    // sigma 0.5, over 16 experts of 4096 x 4096; 1022 so)
-    const uint32_t mt = (uint32_t)((p.m + BM - 1) / BM), per = mt * nt;
-    t.expert = (int)(blockIdx.x / per);
-    tile_in_group((uint32_t)xcd_range_block(blockIdx.x % per, per), mt, nt, t);
+    const uint32_t mt = (uint32_t)((p.m + BM - 1) / BM);
+    t.expert = (int)(id / (mt * nt));
+    tile_in_group(id % (mt * nt), mt, nt, t);
     const int64_t r0 = p.offsets[t.expert], m0 = (int64_t)t.m * BM;
     o.a.k = o.b.k = p.offsets[t.expert + 1] - r0;
     o.a.base = (const T*)p.a + r0 * p.lda + m0;
@@ -334,7 +407,7 @@ __device__ inline bool tile_work(const ProductArgs& p, int lane, TileWork<T>& o)
     o.a.tile_rows = (int)(p.m - m0 < BM ? p.m - m0 : BM);
     o.c = (T*)p.c + (int64_t)t.expert * p.c_expert + m0 * p.ldc;
   } else {
-    if (!find_tile<BM>(p, nt, lane, t)) return false;
+    find_tile<BM>(p, nt, lane, id, t);
     o.a.k = o.b.k = t.expert < p.n_experts ? p.k : 0;
     o.a.base = (const T*)p.a + t.row0 * p.lda;
     o.b.base = (const T*)p.b + (int64_t)t.expert * p.b_expert;
@@ -349,7 +422,7 @@ __device__ inline bool tile_work(const ProductArgs& p, int lane, TileWork<T>& o)
   o.c += n0;
   o.c_rows = o.a.tile_rows;
   o.c_cols = o.b.tile_rows;
-  return true;
+  return o;
 }
 
 // Four neighbouring columns of a result row, from column n of the tile.
@@ -379,8 +452,14 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
   __shared__ alignas(1024) uint8_t s_mem[kSlots][kSlot];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  TileWork<T> work;
-  if (!tile_work<T, MODE, BM, BN>(p, lane, work)) return;
+  const TilePlan plan = plan_tiles<MODE, BM, BN>(p, lane);
+  Share share;
+  if (!find_share<MODE, BM, BN>(p, plan, blockIdx.x, share)) return;
+  TileWork<T> work = tile_work<T, MODE, BM, BN>(p, lane, share.tile);
+  // the steps of this part of the tile
+  const int64_t all_steps = (work.a.k + BK - 1) / BK;
+  const int64_t first = all_steps * share.part / share.parts, steps = all_steps * (share.part + 1) / share.parts;
+  if (steps < all_steps) work.a.k = work.b.k = steps * BK;
   const Source<T>&sa = work.a, &sb = work.b;
 
   const int wm = w / WN, wn = w % WN;
@@ -399,7 +478,6 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  const int64_t steps = (sa.k + BK - 1) / BK;
   typename Mma<T>::frag fa[FM], fb[FN];
   auto read_frags = [&](uint32_t slot, int some) {
     from_b.read(slot + OA::kBytes, fb);
@@ -434,7 +512,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
       if (i < OA::kPieces) da.issue(next, rsrc_a, i, w);
       else db.issue(next + OA::kBytes, rsrc_b, i - OA::kPieces, w);
     };
-    for (int64_t kt = 0; kt < 3; ++kt) {
+    for (int64_t kt = first; kt < first + 3; ++kt) {
       begin_loads(kt);
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) load(i);
@@ -448,7 +526,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
       barrier();
       if (second) barrier();
       auto run = [&](auto whole) {
-        for (int64_t kt = 0; kt < steps; ++kt) {
+        for (int64_t kt = first; kt < steps; ++kt) {
           read_frags(lds + (uint32_t)(kt & 3) * kSlot, whole ? FM : fm);
           begin_loads(kt + 3);
           wait_reads();
@@ -470,7 +548,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
       else run(std::false_type{});
       if (!second) barrier();
     } else {
-      for (int64_t kt = 0; kt < steps; ++kt) {
+      for (int64_t kt = first; kt < steps; ++kt) {
         wait_reads();
         wait_loads<2 * kLoads>();
         barrier();  // step kt has arrived, step kt - 1 has been read
@@ -485,11 +563,11 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
     wait_loads<0>();
   } else {
     u32x4 ra[OA::kPieces], rb[OB::kPieces];
-    if (steps > 0) {
-      load_pieces<OA, T, AKC>(sa, 0, tid, ra);
-      load_pieces<OB, T, BKC>(sb, 0, tid, rb);
+    if (first < steps) {
+      load_pieces<OA, T, AKC>(sa, first, tid, ra);
+      load_pieces<OB, T, BKC>(sb, first, tid, rb);
     }
-    for (int64_t kt = 0; kt < steps; ++kt) {
+    for (int64_t kt = first; kt < steps; ++kt) {
       const uint32_t slot = lds + (uint32_t)(kt & 1) * kSlot;
       store_pieces<OA>(slot, tid, ra, THREADS);
       store_pieces<OB>(slot + OA::kBytes, tid, rb, THREADS);
@@ -505,6 +583,17 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
     }
   }
 
+  if constexpr (WM * WN == 8) {
+    if (share.parts > 1) {  // sums for the join, as the lanes hold them
+      f32x4* part = (f32x4*)p.parts + (int64_t)share.slot * (BM * BN / 4) + w * (FM * FN * 64) + lane;
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+        if (i < fm)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) part[(i * FN + j) * 64] = acc[i][j];
+      return;
+    }
+  }
   // lane l holds row l % 16 and 4 neighbouring columns of each 16x16 result
   const int cm = wm * fm * 16 + (lane & 15), cn = wn * (BN / WN) + (lane >> 4) * 4;
 #pragma unroll
@@ -513,6 +602,33 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
     if (i >= fm || m >= work.c_rows) continue;
 #pragma unroll
     for (int j = 0; j < FN; ++j) store_four(work.c + (int64_t)m * p.ldc, cn + j * 16, work.c_cols, acc[i][j]);
+  }
+}
+
+// Tiles cut along k: their parts are added in order.  A workgroup adds the i-th
+// 16-row block of each wave of one tile, then of others.
+template <class T, int MODE, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void expert_product_join_kernel(const ProductArgs p) {
+  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const TilePlan plan = plan_tiles<MODE, BM, BN>(p, lane);
+  for (uint32_t b = blockIdx.x; b < plan.rest * FM; b += gridDim.x) {
+    const uint32_t r = b / FM;
+    const int i = (int)(b % FM);
+    const TileWork<T> work = tile_work<T, MODE, BM, BN>(p, lane, plan.full + r);
+    const int fm = (work.c_rows + 31) / 32, m = ((w / WN) * fm + i) * 16 + (lane & 15);
+    if (i >= fm || m >= work.c_rows) continue;
+    const f32x4* part = (const f32x4*)p.parts + (int64_t)r * plan.parts * (BM * BN / 4) + w * (FM * FN * 64) +
+                        i * FN * 64 + lane;
+    f32x4 sum[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) sum[j] = part[j * 64];
+    for (uint32_t k = 1; k < plan.parts; ++k)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) sum[j] += part[(int64_t)k * (BM * BN / 4) + j * 64];
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+      store_four(work.c + (int64_t)m * p.ldc, (w % WN) * (BN / WN) + (lane >> 4) * 4 + j * 16, work.c_cols, sum[j]);
   }
 }
 
@@ -532,8 +648,10 @@ __global__ __launch_bounds__(256) void expert_product_few_kernel(const ProductAr
   __shared__ alignas(1024) uint8_t s_mem[kWaves][kSlots][kSlot];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  TileWork<T> work;
-  if (!tile_work<T, MODE, kFewRows, kFewCols>(p, lane, work)) return;
+  const TilePlan plan = plan_tiles<MODE, kFewRows, kFewCols>(p, lane);
+  Share share;
+  if (!find_share<MODE, kFewRows, kFewCols>(p, plan, blockIdx.x, share)) return;
+  const TileWork<T> work = tile_work<T, MODE, kFewRows, kFewCols>(p, lane, share.tile);
   const Source<T>&sa = work.a, &sb = work.b;
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_byte*)&s_mem[w][0][0];
   Frags<OA, true, 1> from_a;
@@ -621,18 +739,47 @@ int64_t tiles_of(const ProductArgs& p) {
   return MODE == kMatrix ? ceil_div(p.m, BM) * nt * p.n_experts : (p.n_rows / BM + p.n_experts + 1) * nt;
 }
 
+// Whether tiles of a last round may be split: of a matrix gradient it is known
+// here; of a product of rows, whose tiles are counted on the device, if tiles
+// take long beside the join that is then launched in any case, and rounds are
+// few.  us with and without: 4096 x 2 rows, 8 experts 4096 x 4096 bf16 272 and
+// 312, 8192 x 2 of 2048 x 2048 149 and 162, 4093 x 4 of 5120 x 2048 346 and 383.
+constexpr int kLarge = 256;
+template <int MODE>
+bool may_split(const ProductArgs& p) {
+  const int64_t tiles = ceil_div(p.n, kLarge);
+  if (MODE == kMatrix) {
+    const int64_t real = ceil_div(p.m, kLarge) * tiles * p.n_experts;
+    return real <= UINT32_MAX &&
+           parts_of((uint32_t)real % (uint32_t)p.cus, p.n_rows / p.n_experts / 32, (uint32_t)p.cus) > 1;
+  }
+  return p.n_rows / p.n_experts >= 112 && p.k >= 1536 && p.n_rows / kLarge * tiles < 8 * p.cus;
+}
+// The most sums that split tiles leave: one a compute unit.
+size_t parts_bytes(const ProductArgs& p) { return (size_t)p.cus * kLarge * kLarge * sizeof(float); }
+
 template <class T, int MODE, bool DMA, int BM, int BN, int WM, int WN>
-int launch_tiles(const ProductArgs& p, hipStream_t stream) {
-  const int64_t tiles = tiles_of<MODE, BM, BN>(p);
+int launch_tiles(ProductArgs p, hipStream_t stream) {
+  constexpr bool kSplit = WM * WN == 8;
+  if (!kSplit) p.parts = nullptr;
+  const int64_t tiles = tiles_of<MODE, BM, BN>(p) + (p.parts != nullptr ? p.cus : 0);
   if (tiles > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
   hipLaunchKernelGGL((expert_product_kernel<T, MODE, DMA, BM, BN, WM, WN>), dim3((uint32_t)tiles),
                      dim3(64 * WM * WN), 0, stream, p);
   FS_CHECK_MAIN_LAUNCH("expert_product_kernel");
+  if constexpr (kSplit) {
+    if (p.parts != nullptr) {
+      hipLaunchKernelGGL((expert_product_join_kernel<T, MODE, BM, BN, WM, WN>),
+                         dim3((uint32_t)p.cus), dim3(64 * WM * WN), 0, stream, p);
+      FS_CHECK_LAUNCH("expert_product_join_kernel");
+    }
+  }
   return FS_OK;
 }
 
 template <class T, int MODE, bool DMA>
-int launch_few(const ProductArgs& p, hipStream_t stream) {
+int launch_few(ProductArgs p, hipStream_t stream) {
+  p.parts = nullptr;
   const int64_t tiles = tiles_of<MODE, kFewRows, kFewCols>(p);
   if (tiles > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
   hipLaunchKernelGGL((expert_product_few_kernel<T, MODE, DMA>), dim3((uint32_t)tiles), dim3(256), 0, stream, p);
@@ -655,43 +802,59 @@ int launch_few(const ProductArgs& p, hipStream_t stream) {
 // 4096 x 4096): 12, 28, 72.
 constexpr int64_t kFill = 256;
 
+enum Tiles { kFew, kTiles64, kTiles128, kTiles256 };
+template <int MODE>
+Tiles choose_tiles(const ProductArgs& p, bool half, bool dma) {
+  if constexpr (MODE == kMatrix) {
+    if (half && dma && tiles_of<MODE, kLarge, kLarge>(p) >= kFill) return kTiles256;
+    return tiles_of<MODE, 128, 128>(p) >= kFill ? kTiles128 : kTiles64;
+  }
+  const int64_t rows = p.n_rows / p.n_experts, active = std::min<int64_t>(p.n_rows, p.n_experts);
+  const int64_t tiles256 = ceil_div(p.n, kLarge) * std::max(active, p.n_rows / kLarge);
+  const int64_t tiles128 = ceil_div(p.n, 128) * std::max(active, p.n_rows / 128);
+  if (half && dma && (rows >= 112 ? tiles256 >= kFill : MODE == kRowsNon && rows >= 4 && tiles256 >= 2 * kFill))
+    return kTiles256;
+  if (rows < (half ? 12 : 20)) return kFew;
+  return rows >= (half ? 40 : 768) && tiles128 >= kFill ? kTiles128 : kTiles64;
+}
+
 template <class T, int MODE>
-int launch_product(const ProductArgs& p, hipStream_t stream) {
+int launch_product(ProductArgs p, void* ws, size_t ws_bytes, hipStream_t stream) {
   // straight to LDS: whole 16-byte pieces, and offsets within a step that fit
-  const int64_t s = sizeof(T), reach = MODE == kMatrix ? kRowBytes / s : 256;
+  const int64_t s = sizeof(T), reach = MODE == kMatrix ? kRowBytes / s : kLarge;
   const bool dma = aligned16(p.a, p.lda * s) && aligned16(p.b, p.ldb * s) && p.b_expert * s % 16 == 0 &&
                    (MODE == kMatrix ? p.m : p.k) * s % 16 == 0 && (MODE == kRowsTrans ? p.k : p.n) * s % 16 == 0 &&
                    reach * std::max(p.lda, p.ldb) * s < (int64_t)kInBuffer;
-  constexpr bool kHalf = sizeof(T) == 2;
-  if constexpr (MODE == kMatrix) {
-    if constexpr (kHalf)
-      if (dma && tiles_of<MODE, 256, 256>(p) >= kFill) return launch_tiles<T, MODE, true, 256, 256, 2, 4>(p, stream);
-    if (tiles_of<MODE, 128, 128>(p) >= kFill)
+  switch (choose_tiles<MODE>(p, s == 2, dma)) {
+    case kFew:
+      if constexpr (MODE != kMatrix)
+        return dma ? launch_few<T, MODE, true>(p, stream) : launch_few<T, MODE, false>(p, stream);
+      break;
+    case kTiles64:
+      return dma ? launch_tiles<T, MODE, true, 64, 128, 2, 2>(p, stream)
+                 : launch_tiles<T, MODE, false, 64, 128, 2, 2>(p, stream);
+    case kTiles128:
       return dma ? launch_tiles<T, MODE, true, 128, 128, 2, 2>(p, stream)
                  : launch_tiles<T, MODE, false, 128, 128, 2, 2>(p, stream);
-  } else {
-    const int64_t rows = p.n_rows / p.n_experts, active = std::min<int64_t>(p.n_rows, p.n_experts);
-    const int64_t tiles256 = ceil_div(p.n, 256) * std::max(active, p.n_rows / 256);
-    const int64_t tiles128 = ceil_div(p.n, 128) * std::max(active, p.n_rows / 128);
-    if constexpr (kHalf)
-      if (dma && (rows >= 112                ? tiles256 >= kFill
-                  : MODE == kRowsNon && rows >= 4 && tiles256 >= 2 * kFill))
-        return launch_tiles<T, MODE, true, 256, 256, 2, 4>(p, stream);
-    if (rows < (kHalf ? 12 : 20)) return dma ? launch_few<T, MODE, true>(p, stream) : launch_few<T, MODE, false>(p, stream);
-    if (rows >= (kHalf ? 40 : 768) && tiles128 >= kFill)
-      return dma ? launch_tiles<T, MODE, true, 128, 128, 2, 2>(p, stream)
-                 : launch_tiles<T, MODE, false, 128, 128, 2, 2>(p, stream);
+    case kTiles256:
+      if constexpr (s == 2) {
+        if (may_split<MODE>(p)) {
+          if (ws == nullptr || ws_bytes < parts_bytes(p))
+            return fail(FS_E_WORKSPACE, "fs_expert_product: workspace too small");
+          p.parts = static_cast<float*>(ws);
+        }
+        return launch_tiles<T, MODE, true, kLarge, kLarge, 2, 4>(p, stream);
+      }
   }
-  return dma ? launch_tiles<T, MODE, true, 64, 128, 2, 2>(p, stream)
-             : launch_tiles<T, MODE, false, 64, 128, 2, 2>(p, stream);
+  return fail(FS_E_INVALID, "fs_expert_product: no tiles");
 }
 
 template <int MODE>
-int launch_product_type(int val_t, const ProductArgs& p, hipStream_t stream) {
+int launch_product_type(int val_t, const ProductArgs& p, void* ws, size_t ws_bytes, hipStream_t stream) {
   switch (val_t) {
-    case FS_F16: return launch_product<_Float16, MODE>(p, stream);
-    case FS_BF16: return launch_product<__bf16, MODE>(p, stream);
-    case FS_F32: return launch_product<float, MODE>(p, stream);
+    case FS_F16: return launch_product<_Float16, MODE>(p, ws, ws_bytes, stream);
+    case FS_BF16: return launch_product<__bf16, MODE>(p, ws, ws_bytes, stream);
+    case FS_F32: return launch_product<float, MODE>(p, ws, ws_bytes, stream);
   }
   return fail(FS_E_INVALID, "fs_expert_product: value types are FS_F16, FS_BF16 and FS_F32");
 }
@@ -703,18 +866,54 @@ int check_product(const char* who, int64_t n_rows, int64_t n_experts, int64_t a,
   return FS_OK;
 }
 
+// Compute units of the current device (cached per device id; threads that ask
+// at once store the same value).
+int compute_units() {
+  static std::atomic<int> cached[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  int v = cached[dev].load(std::memory_order_relaxed);
+  if (v == 0) {
+    if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0) v = 256;
+    cached[dev].store(v, std::memory_order_relaxed);
+  }
+  return v;
+}
+
+ProductArgs product_sizes(int trans, int64_t n_rows, int64_t n_experts, int64_t inner, int64_t outer, bool matrix) {
+  ProductArgs p{};
+  p.n_rows = n_rows;
+  p.n_experts = (int)n_experts;
+  p.m = trans ? outer : inner;
+  p.n = matrix && trans ? inner : outer;
+  p.k = inner;
+  p.cus = compute_units();
+  return p;
+}
+
 }  // namespace
 }  // namespace fs
 
+extern "C" size_t fs_expert_product_workspace_bytes(int val_t, int trans, int64_t n_rows, int64_t n_experts,
+                                                    int64_t inner, int64_t outer) {
+  using namespace fs;
+  if ((val_t != FS_F16 && val_t != FS_BF16) || check_product("", n_rows, n_experts, inner, outer, trans) != FS_OK ||
+      n_rows == 0 || outer == 0)
+    return 0;
+  const ProductArgs p = product_sizes(trans, n_rows, n_experts, inner, outer, false);
+  const Tiles t = trans ? choose_tiles<kRowsTrans>(p, true, true) : choose_tiles<kRowsNon>(p, true, true);
+  return t == kTiles256 && may_split<kRowsNon>(p) ? parts_bytes(p) : 0;
+}
+
 extern "C" int fs_expert_product(int val_t, int trans, int64_t n_rows, int64_t n_experts, int64_t inner, int64_t outer,
                                  const void* rows, int64_t ldr, const void* matrices, const int32_t* offsets, void* out,
-                                 hipStream_t stream) {
+                                 void* ws, size_t ws_bytes, hipStream_t stream) {
   using namespace fs;
   if (int rc = check_product("fs_expert_product", n_rows, n_experts, inner, outer, trans)) return rc;
   if (n_rows == 0 || outer == 0) return FS_OK;
   if (!offsets || !out || ldr < 0 || (inner > 0 && (!rows || !matrices)))
     return fail(FS_E_INVALID, "fs_expert_product: bad pointer or stride");
-  ProductArgs p{};
+  ProductArgs p = product_sizes(trans, n_rows, n_experts, inner, outer, false);
   p.a = rows;
   p.b = matrices;
   p.c = out;
@@ -723,34 +922,37 @@ extern "C" int fs_expert_product(int val_t, int trans, int64_t n_rows, int64_t n
   p.ldb = trans ? inner : outer;
   p.ldc = outer;
   p.b_expert = inner * outer;
-  p.n_rows = n_rows;
-  p.n = outer;
-  p.k = inner;
-  p.n_experts = (int)n_experts;
-  return trans ? launch_product_type<kRowsTrans>(val_t, p, stream) : launch_product_type<kRowsNon>(val_t, p, stream);
+  return trans ? launch_product_type<kRowsTrans>(val_t, p, ws, ws_bytes, stream)
+               : launch_product_type<kRowsNon>(val_t, p, ws, ws_bytes, stream);
+}
+
+extern "C" size_t fs_expert_product_grad_matrices_workspace_bytes(int val_t, int trans, int64_t n_rows,
+                                                                  int64_t n_experts, int64_t inner, int64_t outer) {
+  using namespace fs;
+  if ((val_t != FS_F16 && val_t != FS_BF16) || check_product("", n_rows, n_experts, inner, outer, trans) != FS_OK ||
+      inner == 0 || outer == 0)
+    return 0;
+  const ProductArgs p = product_sizes(trans, n_rows, n_experts, inner, outer, true);
+  return choose_tiles<kMatrix>(p, true, true) == kTiles256 && may_split<kMatrix>(p) ? parts_bytes(p) : 0;
 }
 
 extern "C" int fs_expert_product_grad_matrices(int val_t, int trans, int64_t n_rows, int64_t n_experts, int64_t inner,
                                                int64_t outer, const void* grad, int64_t ldg, const void* rows,
-                                               int64_t ldr, const int32_t* offsets, void* grad_matrices,
-                                               hipStream_t stream) {
+                                               int64_t ldr, const int32_t* offsets, void* grad_matrices, void* ws,
+                                               size_t ws_bytes, hipStream_t stream) {
   using namespace fs;
   if (int rc = check_product("fs_expert_product_grad_matrices", n_rows, n_experts, inner, outer, trans)) return rc;
   if (inner == 0 || outer == 0) return FS_OK;
   if (!offsets || !grad_matrices || ldg < 0 || ldr < 0 || (n_rows > 0 && (!grad || !rows)))
     return fail(FS_E_INVALID, "fs_expert_product_grad_matrices: bad pointer or stride");
-  ProductArgs p{};
+  ProductArgs p = product_sizes(trans, n_rows, n_experts, inner, outer, true);
   p.a = trans ? grad : rows;
   p.lda = trans ? ldg : ldr;
   p.b = trans ? rows : grad;
   p.ldb = trans ? ldr : ldg;
-  p.m = trans ? outer : inner;
-  p.n = trans ? inner : outer;
   p.c = grad_matrices;
   p.ldc = p.n;
   p.c_expert = inner * outer;
   p.offsets = offsets;
-  p.n_rows = n_rows;
-  p.n_experts = (int)n_experts;
-  return launch_product_type<kMatrix>(val_t, p, stream);
+  return launch_product_type<kMatrix>(val_t, p, ws, ws_bytes, stream);
 }

@@ -10,12 +10,14 @@
 // Products with the routing matrix, tokens by rows, and its transpose; all are
 // bound by the rows' bytes.  Sums run in slot order in 32 bits (64 for float64)
 // and are rounded once; a slot of no expert is left out, whatever its row holds.
+#include <type_traits>
+
 #include "select_rows.hpp"
 
 namespace fs {
 namespace {
 
-template <class V>
+template <class V, bool PAST>
 __global__ __launch_bounds__(256) void expert_dispatch_kernel(const V* __restrict__ x, int64_t ldx, int64_t n_tokens,
                                                               int slots, int64_t width, int lpr,
                                                               const int32_t* __restrict__ inverse,
@@ -35,8 +37,10 @@ __global__ __launch_bounds__(256) void expert_dispatch_kernel(const V* __restric
 #pragma unroll 4
     for (int j = 0; j < slots; ++j) {
       const bool in = inv[j] < routed;
-      const uint4 o = make_uint4(in ? s.x : 0u, in ? s.y : 0u, in ? s.z : 0u, in ? s.w : 0u);
-      __builtin_memcpy(out + inv[j] * width + h, &o, 16);
+      const uint4 words = make_uint4(in ? s.x : 0u, in ? s.y : 0u, in ? s.z : 0u, in ? s.w : 0u);
+      Slice<V> o;
+      __builtin_memcpy(&o, &words, 16);
+      store_slice<PAST>(out + inv[j] * width + h, o);
     }
   }
   for (int64_t h = slices > 0 ? width : lane; h < width; h += lpr)
@@ -44,7 +48,7 @@ __global__ __launch_bounds__(256) void expert_dispatch_kernel(const V* __restric
 }
 
 // (a slot of no expert has a place, whose row is read and left out)
-template <class V>
+template <class V, bool PAST>
 __global__ __launch_bounds__(256) void expert_combine_kernel(const V* __restrict__ rows, int64_t ldr, int64_t n_tokens,
                                                              int slots, int64_t width, int lpr,
                                                              const int32_t* __restrict__ inverse,
@@ -81,7 +85,7 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(const V* __restrict
     Slice<V> o;
 #pragma unroll
     for (int e = 0; e < E; ++e) o.v[e] = (V)acc[e];
-    store_slice(out + t * width + h, o);
+    store_slice<PAST>(out + t * width + h, o);
   }
   for (int64_t h = slices > 0 ? width : lane; h < width; h += lpr) {
     A acc = 0;
@@ -93,7 +97,7 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(const V* __restrict
 
 // One wave a slot: the token's gradient row, read by its slots in turn, comes
 // from cache after the first.
-template <class V>
+template <class V, bool PAST>
 __global__ __launch_bounds__(256) void expert_combine_grad_kernel(
     const V* __restrict__ grad, int64_t ldg, const V* __restrict__ rows, int64_t ldr, int64_t n, int slots,
     int64_t width, const int32_t* __restrict__ inverse, const int32_t* __restrict__ routed_at,
@@ -124,14 +128,14 @@ __global__ __launch_bounds__(256) void expert_combine_grad_kernel(
         dot += ge * widen(sy.v[e]);
         out.v[e] = (V)(w * ge);
       }
-      store_slice(o + c * E, out);
+      store_slice<PAST>(o + c * E, out);
     }
     for (int64_t h = full * E + lane; h < width; h += 64) {
       dot += widen(g[h]) * widen(y[h]);
       o[h] = (V)(w * widen(g[h]));
     }
   } else {
-    for (int64_t c = lane; c < full; c += 64) store_slice(o + c * E, Slice<V>{});
+    for (int64_t c = lane; c < full; c += 64) store_slice<PAST>(o + c * E, Slice<V>{});
     for (int64_t h = full * E + lane; h < width; h += 64) o[h] = (V)0;
   }
   dot = wave_sum(dot);
@@ -158,8 +162,12 @@ extern "C" int fs_expert_dispatch(int val_t, int64_t n_tokens, int slots, int64_
     using V = decltype(v);
     const int lpr = lanes_per_row(slices_of<V>(width));
     const dim3 grid((uint32_t)ceil_div(n_tokens, 256 / lpr));
-    hipLaunchKernelGGL((expert_dispatch_kernel<V>), grid, dim3(256), 0, stream, (const V*)x, ldx, n_tokens,
-                       slots, width, lpr, inverse, offsets + n_experts, (V*)out);
+    auto launch = [&](auto past) {
+      hipLaunchKernelGGL((expert_dispatch_kernel<V, decltype(past)::value>), grid, dim3(256), 0, stream, (const V*)x, ldx, n_tokens,
+                         slots, width, lpr, inverse, offsets + n_experts, (V*)out);
+    };
+    if (store_past_caches(n_tokens * (slots + 1) * width * (int64_t)sizeof(V), width * sizeof(V))) launch(std::true_type{});
+    else launch(std::false_type{});
     FS_CHECK_MAIN_LAUNCH("expert_dispatch_kernel");
     return FS_OK;
   });
@@ -177,8 +185,12 @@ extern "C" int fs_expert_combine(int val_t, int64_t n_tokens, int slots, int64_t
     using A = typename Elem<V>::acc;
     const int lpr = lanes_per_row(slices_of<V>(width));
     const dim3 grid((uint32_t)ceil_div(n_tokens, 256 / lpr));
-    hipLaunchKernelGGL((expert_combine_kernel<V>), grid, dim3(256), 0, stream, (const V*)rows, ldr, n_tokens,
-                       slots, width, lpr, inverse, offsets + n_experts, (const A*)weights, (V*)out);
+    auto launch = [&](auto past) {
+      hipLaunchKernelGGL((expert_combine_kernel<V, decltype(past)::value>), grid, dim3(256), 0, stream, (const V*)rows, ldr, n_tokens,
+                         slots, width, lpr, inverse, offsets + n_experts, (const A*)weights, (V*)out);
+    };
+    if (store_past_caches(n_tokens * (slots + 1) * width * (int64_t)sizeof(V), width * sizeof(V))) launch(std::true_type{});
+    else launch(std::false_type{});
     FS_CHECK_MAIN_LAUNCH("expert_combine_kernel");
     return FS_OK;
   });
@@ -199,9 +211,13 @@ extern "C" int fs_expert_combine_grad(int val_t, int64_t n_tokens, int slots, in
     using A = typename Elem<V>::acc;
     const int64_t n = n_tokens * slots;
     const dim3 grid((uint32_t)ceil_div(n, 4));
-    hipLaunchKernelGGL((expert_combine_grad_kernel<V>), grid, dim3(256), 0, stream, (const V*)grad, ldg,
-                       (const V*)rows, ldr, n, slots, width, inverse, offsets + n_experts, (const A*)weights,
-                       (V*)grad_rows, (A*)grad_weights);
+    auto launch = [&](auto past) {
+      hipLaunchKernelGGL((expert_combine_grad_kernel<V, decltype(past)::value>), grid, dim3(256), 0, stream, (const V*)grad, ldg,
+                         (const V*)rows, ldr, n, slots, width, inverse, offsets + n_experts, (const A*)weights,
+                         (V*)grad_rows, (A*)grad_weights);
+    };
+    if (store_past_caches((n_tokens + 2 * n) * width * (int64_t)sizeof(V), width * sizeof(V))) launch(std::true_type{});
+    else launch(std::false_type{});
     FS_CHECK_MAIN_LAUNCH("expert_combine_grad_kernel");
     return FS_OK;
   });

@@ -34,9 +34,29 @@ __device__ inline Slice<V> load_slice(const V* p) {
   __builtin_memcpy(&s, p, 16);
   return s;
 }
-template <class V>
+// PAST: past the caches (of their own kind, a choice at run time is compiled
+// into plain stores).
+template <bool PAST = false, class V>
 __device__ inline void store_slice(V* p, const Slice<V>& s) {
-  __builtin_memcpy(p, &s, 16);
+  if constexpr (PAST) {
+    typedef uint32_t words4 __attribute__((ext_vector_type(4)));
+    typedef words4 words __attribute__((aligned(2)));
+    words u;
+    __builtin_memcpy(&u, &s, 16);
+    __builtin_nontemporal_store(u, reinterpret_cast<words*>(p));
+  } else {
+    __builtin_memcpy(p, &s, 16);
+  }
+}
+// Whether a call that reads and writes `bytes` in all stores past the caches:
+// where that is more than the Infinity Cache holds, keeping results there only
+// drives out what is still to be read.  us with and without: dispatch 16384 x 8
+// of 2048 bf16 104 and 120, its 4096 tokens 26 and 24; combine 109 and 117;
+// combine_grad 4096 x 4 of 2048 f32 45 and 54; embedding gradient 65536 tokens
+// x 2048, 131072 rows bf16 191 and 239, 512 x 1024, 50000 rows f32 52 and 42.
+// (Rows of whole words: dispatch 2047 wide took 151 and 146.)
+inline bool store_past_caches(int64_t bytes, int64_t row_bytes) {
+  return bytes >= (int64_t)256 << 20 && row_bytes % 4 == 0;
 }
 // Slices of a row: the last one ends with the row and overlaps the one before
 // (its elements are computed twice, alike).  Rows shorter than a slice have
@@ -58,19 +78,25 @@ __device__ inline A wave_sum(A v) {
   return v;
 }
 
+// Inclusive sum over the lanes up to this one (row shifts, then row broadcasts;
+// lanes without a source read 0).
+template <int CTRL, int ROWS>
+__device__ inline uint32_t lane_shifted(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ inline uint32_t wave_sum_scan(uint32_t v) {
+  v += lane_shifted<0x111, 0xF>(v);  // row_shr:1
+  v += lane_shifted<0x112, 0xF>(v);  // row_shr:2
+  v += lane_shifted<0x114, 0xF>(v);  // row_shr:4
+  v += lane_shifted<0x118, 0xF>(v);  // row_shr:8
+  v += lane_shifted<0x142, 0xA>(v);  // row_bcast:15 -> rows 1, 3
+  v += lane_shifted<0x143, 0xC>(v);  // row_bcast:31 -> rows 2, 3
+  return v;
+}
+
 // Whether rows `ld_bytes` apart all start at multiples of 16 bytes.
 inline bool aligned16(const void* p, int64_t ld_bytes) {
   return ((uintptr_t)p & 15) == 0 && (ld_bytes & 15) == 0;
-}
-
-inline size_t value_bytes(int val_t) {
-  switch (val_t) {
-    case FS_F16:
-    case FS_BF16: return 2;
-    case FS_F32: return 4;
-    case FS_F64: return 8;
-  }
-  return 0;
 }
 
 // Threads of a workgroup of 256 that share a row of `slices` slices.

@@ -11,10 +11,12 @@
 // of 512 to 4096 positions, scans the counts, and scatters: a tile is ranked
 // stably, a wave taking 64 positions at a time, the lanes with its digit found
 // by ballots, and waves owning consecutive sub-tiles, so ranks need no order of
-// atomics.  One tile counts for itself and is one launch a pass; a few are
-// scanned by the scatter, two launches.
-#include "fs_common.hpp"
+// atomics.  Up to 4096 positions are sorted by one workgroup in one launch, all
+// passes through LDS.
+#include <type_traits>
+
 #include "radix_tile.hpp"
+#include "select_rows.hpp"
 
 namespace fs {
 namespace {
@@ -58,18 +60,19 @@ __global__ __launch_bounds__(kThreads) void select_count_kernel(const void* __re
   for (int d = threadIdx.x; d < nd; d += kThreads) cnt[(int64_t)blockIdx.x * nd + d] = s_cnt[d];
 }
 
-// mode 0: one tile; 1: the tiles before this one are added up here; 2: cnt
-// holds, per digit, the sum over the tiles before, and totals that over all.
+// scanned: cnt holds, per digit, the sum over the tiles before, and totals that
+// over all; otherwise the tiles' counts are added up here.
 // Writes sorted keys, order, inverse and offsets where asked for.
 template <class Id, bool KEYS, int CH>
 __global__ __launch_bounds__(kThreads) void select_scatter_kernel(
     const void* __restrict__ src, const int32_t* __restrict__ pos_in, int64_t n, uint32_t n_keys, int shift, int nd,
-    const uint32_t* __restrict__ cnt, const uint32_t* __restrict__ totals, int64_t n_tiles, int mode,
-    uint32_t* __restrict__ keys_out, int32_t* __restrict__ pos_out, int32_t* __restrict__ inverse, int32_t* __restrict__ offsets) {
+    const uint32_t* __restrict__ cnt, const uint32_t* __restrict__ totals, int64_t n_tiles, bool scanned,
+    uint32_t* __restrict__ keys_out, int32_t* __restrict__ pos_out, int32_t* __restrict__ inverse,
+    int32_t* __restrict__ offsets) {
   __shared__ uint32_t s_cnt[kWaves][kMaxDigits];
   __shared__ uint32_t s_base[kMaxDigits];
   __shared__ uint32_t s_part[2 * kThreads];
-  __shared__ int64_t s_wave[kWaves];
+  __shared__ uint32_t s_wave[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t tile = blockIdx.x;
   const int64_t first = (tile * kWaves + w) * (64 * CH) + lane;
@@ -85,6 +88,32 @@ __global__ __launch_bounds__(kThreads) void select_scatter_kernel(
     key[c] = i < n ? load_key<Id, KEYS>(src, i, n_keys) : 0u;
     pos[c] = pos_in != nullptr && i < n ? pos_in[i] : (int32_t)i;
   }
+  // per digit: the count of all tiles (tot) and of those before this one (pre),
+  // loaded before anything waits; a thread's digits are tid * per + j, or tid % nd
+  // with the tiles shared by groups of threads
+  uint32_t tot[kMaxDigits / kThreads] = {}, pre[kMaxDigits / kThreads] = {};
+  const int per = nd > kThreads ? nd / kThreads : 1, groups = nd < kThreads ? kThreads / nd : 1;
+  if (!scanned) {
+    for (int j = 0; j < per; ++j) {
+      const int d = groups > 1 ? tid % nd : tid * per + j;
+      uint32_t a = 0u, b = 0u;
+#pragma unroll 8
+      for (int64_t t = groups > 1 ? tid / nd : 0; t < n_tiles; t += groups) {
+        const uint32_t v = cnt[t * nd + d];
+        a += v;
+        b += t < tile ? v : 0u;
+      }
+      tot[j] = a;
+      pre[j] = b;
+    }
+  } else {
+    for (int j = 0; j < per; ++j)
+      if (tid * per + j < nd) {
+        tot[j] = totals[tid * per + j];
+        pre[j] = cnt[tile * nd + tid * per + j];
+      }
+  }
+
   __syncthreads();
   uint32_t rank[CH];
   const uint32_t mask = (uint32_t)(nd - 1);
@@ -104,56 +133,36 @@ __global__ __launch_bounds__(kThreads) void select_scatter_kernel(
     rank[c] = before + (uint32_t)below;
   }
   __syncthreads();
-  // counts of the waves -> places within the tile's run of each digit, and the
-  // first place of the run
+  // counts of the waves -> places within the tile's run of each digit
   for (int d = tid; d < nd; d += kThreads) {
-    uint32_t run = 0u;
+    uint32_t v[kWaves], run = 0u;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) v[k] = s_cnt[k][d];
+#pragma unroll
     for (int k = 0; k < kWaves; ++k) {
-      const uint32_t v = s_cnt[k][d];
       s_cnt[k][d] = run;
-      run += v;
+      run += v[k];
     }
-    s_base[d] = run;
   }
-  // per digit: the count of all tiles (tot) and of those before this one (pre)
-  uint32_t tot[kMaxDigits / kThreads], pre[kMaxDigits / kThreads];
-  const int per = nd > kThreads ? nd / kThreads : 1;
-  if (mode == 1) {
-    const int groups = nd < kThreads ? kThreads / nd : 1;
-    for (int j = 0; j < per; ++j) {
-      const int d = nd < kThreads ? tid % nd : tid * per + j;
-      uint32_t a = 0u, b = 0u;
-#pragma unroll 8
-      for (int64_t t = nd < kThreads ? tid / nd : 0; t < n_tiles; t += groups) {
-        const uint32_t v = cnt[t * nd + d];
-        a += v;
-        b += t < tile ? v : 0u;
-      }
-      tot[j] = a;
-      pre[j] = b;
-    }
-    if (groups > 1) {
-      s_part[tid] = tot[0];
-      s_part[kThreads + tid] = pre[0];
-      __syncthreads();
-      if (tid < nd)
-        for (int g = 1; g < groups; ++g) {
-          tot[0] += s_part[g * nd + tid];
-          pre[0] += s_part[kThreads + g * nd + tid];
-        }
-    }
-  } else {
+  if (!scanned && groups > 1) {
+    s_part[tid] = tot[0];
+    s_part[kThreads + tid] = pre[0];
     __syncthreads();
-    for (int j = 0; j < per; ++j) {
-      const int d = tid * per + j;
-      tot[j] = d < nd ? (mode == 0 ? s_base[d] : totals[d]) : 0u;
-      pre[j] = d < nd && mode == 2 ? cnt[tile * nd + d] : 0u;
-    }
+    if (tid < nd)
+      for (int g = 1; g < groups; ++g) {
+        tot[0] += s_part[g * nd + tid];
+        pre[0] += s_part[kThreads + g * nd + tid];
+      }
   }
-  int64_t mine = 0, all;
+  uint32_t mine = 0u;
   if (tid * per < nd)
     for (int j = 0; j < per; ++j) mine += tot[j];
-  uint32_t run = (uint32_t)block_exclusive_scan(mine, s_wave, all);
+  const uint32_t upto = wave_sum_scan(mine);
+  if (lane == 63) s_wave[w] = upto;
+  __syncthreads();
+  uint32_t run = upto - mine;
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) run += k < w ? s_wave[k] : 0u;
   if (tid * per < nd)
     for (int j = 0; j < per; ++j) {
       s_base[tid * per + j] = run + pre[j];
@@ -171,6 +180,102 @@ __global__ __launch_bounds__(kThreads) void select_scatter_kernel(
     if (keys_out != nullptr) keys_out[at] = key[c];
     if (pos_out != nullptr) pos_out[at] = pos[c];
     if (inverse != nullptr) inverse[pos[c]] = (int32_t)at;
+  }
+}
+
+// All of the sort by one workgroup of W waves, 64 CH positions each, W = 1..16.
+constexpr int kSmallWaves = 16, kSmallChunks = 4;
+constexpr int64_t kSmall = 64 * kSmallWaves * kSmallChunks;
+template <class Id, int CH>
+__global__ __launch_bounds__(64 * kSmallWaves) void select_small_kernel(
+    const Id* __restrict__ ids, int n, uint32_t n_keys, int bits, int passes, uint32_t* __restrict__ keys_out,
+    int32_t* __restrict__ order, int32_t* __restrict__ inverse, int32_t* __restrict__ offsets) {
+  __shared__ uint16_t s_cnt[kSmallWaves][kMaxDigits];
+  __shared__ uint32_t s_base[kMaxDigits];
+  __shared__ uint32_t s_wave[kSmallWaves];
+  __shared__ uint32_t s_key[64 * kSmallWaves * CH];
+  __shared__ uint16_t s_pos[64 * kSmallWaves * CH];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, threads = blockDim.x, waves = threads >> 6;
+  const int nd = 1 << bits, per = (nd + threads - 1) / threads;
+  const uint32_t mask = (uint32_t)(nd - 1);
+  uint32_t key[CH], rank[CH];
+  int pos[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int i = (w * CH + c) * 64 + lane;
+    key[c] = i < n ? key_of(ids[i], n_keys) : 0u;
+    pos[c] = i;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * bits;
+    for (int k = 0; k < waves; ++k)
+      for (int d = tid; d < nd; d += threads) s_cnt[k][d] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      rank[c] = 0u;
+      if ((w * CH + c) * 64 >= n) continue;
+      const bool active = (w * CH + c) * 64 + lane < n;
+      const uint32_t digit = (key[c] >> shift) & mask;
+      const uint64_t peers = match_lanes<kMaxBits>(digit, __ballot(active), mask);
+      const int below = count_below_t(peers);
+      uint32_t before = 0u;
+      if (active) before = s_cnt[w][digit];
+      wave_sync_t();
+      if (active && below == 0) s_cnt[w][digit] = (uint16_t)(before + (uint32_t)__popcll(peers));
+      wave_sync_t();
+      rank[c] = before + (uint32_t)below;
+    }
+    __syncthreads();
+    uint32_t mine = 0u;
+    for (int j = 0; j < per; ++j) {
+      const int d = tid * per + j;
+      if (d >= nd) break;
+      uint32_t v[kSmallWaves], run = 0u;
+#pragma unroll
+      for (int k = 0; k < kSmallWaves; ++k) v[k] = k < waves ? s_cnt[k][d] : 0u;
+#pragma unroll
+      for (int k = 0; k < kSmallWaves; ++k) {
+        if (k < waves) s_cnt[k][d] = (uint16_t)run;  // (at most 4096)
+        run += v[k];
+      }
+      s_base[d] = mine;  // within the thread's digits
+      mine += run;
+    }
+    const uint32_t upto = wave_sum_scan(mine);
+    if (lane == 63) s_wave[w] = upto;
+    __syncthreads();
+    uint32_t run = upto - mine;
+    for (int k = 0; k < w; ++k) run += s_wave[k];
+    for (int j = 0; j < per; ++j) {
+      const int d = tid * per + j;
+      if (d >= nd) break;
+      s_base[d] += run;
+      if (offsets != nullptr && (uint32_t)d <= n_keys) offsets[d] = (int32_t)s_base[d];  // (one pass: the digit is the key)
+    }
+    __syncthreads();
+    const bool last = pass + 1 == passes;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if ((w * CH + c) * 64 + lane >= n) continue;
+      const uint32_t digit = (key[c] >> shift) & mask, at = s_base[digit] + s_cnt[w][digit] + rank[c];
+      if (!last) {
+        s_key[at] = key[c];
+        s_pos[at] = (uint16_t)pos[c];
+      } else {
+        if (keys_out != nullptr) keys_out[at] = key[c];
+        if (order != nullptr) order[at] = pos[c];
+        if (inverse != nullptr) inverse[pos[c]] = (int32_t)at;
+      }
+    }
+    if (last) break;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int i = (w * CH + c) * 64 + lane;
+      key[c] = i < n ? s_key[i] : 0u;
+      pos[c] = i < n ? (int)s_pos[i] : 0;
+    }
   }
 }
 
@@ -201,6 +306,7 @@ struct SortLayout {
 SortLayout sort_layout(int64_t n, int64_t n_keys) {
   const Passes p = passes_of(n_keys);
   SortLayout l{};
+  if (n <= kSmall) return l;
   l.ch = chunks_of(n);
   l.tiles = ceil_div(n, (int64_t)kThreads * l.ch);
   const int64_t nd = (int64_t)1 << p.bits;
@@ -210,7 +316,7 @@ SortLayout sort_layout(int64_t n, int64_t n_keys) {
     at += (b + 255) / 256 * 256;
     return a;
   };
-  if (l.tiles > 1) l.cnt = take((size_t)(l.tiles * nd) * 4);
+  l.cnt = take((size_t)(l.tiles * nd) * 4);
   if (l.tiles > kSelfScanTiles) l.totals = take((size_t)nd * 4);
   // passes before the last write keys and positions, in turn
   for (int k = 0; k < 2 && k + 1 < p.count; ++k) {
@@ -235,20 +341,16 @@ template <class Id, bool KEYS, int CH>
 int sort_pass(const PassArgs& a, uint8_t* ws, const SortLayout& l, hipStream_t s) {
   uint32_t* cnt = reinterpret_cast<uint32_t*>(ws + l.cnt);
   uint32_t* totals = reinterpret_cast<uint32_t*>(ws + l.totals);
-  int mode = 0;
-  if (l.tiles > 1) {
-    hipLaunchKernelGGL((select_count_kernel<Id, KEYS, CH>), dim3((uint32_t)l.tiles), dim3(kThreads), 0, s, a.src, a.n,
-                       a.n_keys, a.shift, a.nd, cnt);
-    FS_CHECK_LAUNCH("select_count_kernel");
-    mode = 1;
-    if (l.tiles > kSelfScanTiles) {
-      mode = 2;
-      hipLaunchKernelGGL(wg_scan_column_kernel, dim3((uint32_t)a.nd), dim3(256), 0, s, cnt, l.tiles, a.nd, totals);
-      FS_CHECK_LAUNCH("wg_scan_column_kernel");
-    }
+  hipLaunchKernelGGL((select_count_kernel<Id, KEYS, CH>), dim3((uint32_t)l.tiles), dim3(kThreads), 0, s, a.src, a.n,
+                     a.n_keys, a.shift, a.nd, cnt);
+  FS_CHECK_LAUNCH("select_count_kernel");
+  const bool scanned = l.tiles > kSelfScanTiles;
+  if (scanned) {
+    hipLaunchKernelGGL(wg_scan_column_kernel, dim3((uint32_t)a.nd), dim3(256), 0, s, cnt, l.tiles, a.nd, totals);
+    FS_CHECK_LAUNCH("wg_scan_column_kernel");
   }
   hipLaunchKernelGGL((select_scatter_kernel<Id, KEYS, CH>), dim3((uint32_t)l.tiles), dim3(kThreads), 0, s, a.src,
-                     a.pos_in, a.n, a.n_keys, a.shift, a.nd, cnt, totals, l.tiles, mode, a.keys_out, a.pos_out,
+                     a.pos_in, a.n, a.n_keys, a.shift, a.nd, cnt, totals, l.tiles, scanned, a.keys_out, a.pos_out,
                      a.inverse, a.offsets);
   FS_CHECK_MAIN_LAUNCH("select_scatter_kernel");
   return FS_OK;
@@ -284,6 +386,21 @@ int select_sort(const void* ids, int id_t, int64_t n, int64_t n_keys, uint32_t* 
     return FS_OK;
   }
   const Passes p = passes_of(n_keys);
+  if (n <= kSmall) {
+    auto launch = [&](auto id, auto chunks) {
+      using Id = decltype(id);
+      constexpr int CH = decltype(chunks)::value;
+      hipLaunchKernelGGL((select_small_kernel<Id, CH>), dim3(1), dim3((uint32_t)(ceil_div(n, 64 * CH) * 64)), 0, s,
+                         (const Id*)ids, (int)n, (uint32_t)n_keys, p.bits, p.count, keys_out, order, inverse, offsets);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Four = std::integral_constant<int, kSmallChunks>;
+    const bool one = n <= 64 * kSmallWaves;
+    if (id_t == FS_I64) one ? launch(int64_t(0), One{}) : launch(int64_t(0), Four{});
+    else one ? launch(int32_t(0), One{}) : launch(int32_t(0), Four{});
+    FS_CHECK_MAIN_LAUNCH("select_small_kernel");
+    return FS_OK;
+  }
   const SortLayout l = sort_layout(n, n_keys);
   const int nd = 1 << p.bits;
   const void* src = ids;

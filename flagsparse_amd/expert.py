@@ -42,16 +42,28 @@ class PreparedExpertRoute:
               the number of slots that name one
     """
 
-    __slots__ = ("n_tokens", "slots", "num_experts", "order", "inverse", "offsets", "device")
+    __slots__ = ("n_tokens", "slots", "num_experts", "n_rows", "device", "_places", "_inverse_ptr", "_offsets_ptr")
 
-    def __init__(self, n_tokens, slots, num_experts, order, inverse, offsets):
-        self.n_tokens, self.slots, self.num_experts = n_tokens, slots, num_experts
-        self.order, self.inverse, self.offsets = order, inverse, offsets
-        self.device = offsets.device
+    def __init__(self, n_tokens, slots, num_experts, places):
+        n = n_tokens * slots
+        self.n_tokens, self.slots, self.num_experts, self.n_rows = n_tokens, slots, num_experts, n
+        self.device = places.device
+        # one int32 tensor: order, inverse, offsets (views of it cost more than the sort of a decode step)
+        self._places = places
+        start = places.data_ptr()
+        self._inverse_ptr, self._offsets_ptr = start + 4 * n, start + 8 * n
 
     @property
-    def n_rows(self):
-        return self.n_tokens * self.slots
+    def order(self):
+        return self._places[: self.n_rows]
+
+    @property
+    def inverse(self):
+        return self._places[self.n_rows : 2 * self.n_rows].view(self.n_tokens, self.slots)
+
+    @property
+    def offsets(self):
+        return self._places[2 * self.n_rows :]
 
 
 def prepare_expert_route(experts, num_experts):
@@ -75,18 +87,17 @@ def prepare_expert_route(experts, num_experts):
         raise ValueError("tokens * slots exceeds the int32 range")
     experts = experts.contiguous()
     device = experts.device
-    # one allocation for the three: the smallest calls are what it costs to make them
-    buf = torch.empty(2 * n + num_experts + 1, dtype=torch.int32, device=device)
-    order, inverse, offsets = buf[:n], buf[n : 2 * n].view(n_tokens, slots), buf[2 * n :]
+    places = torch.empty(2 * n + num_experts + 1, dtype=torch.int32, device=device)
+    route = PreparedExpertRoute(n_tokens, slots, num_experts, places)
     lib = _lib.lib()
     need = lib.fs_expert_route_workspace_bytes(n, num_experts)
     ws = _lib.workspace(need, device) if need else None
     _lib.check(
-        lib.fs_expert_route(_lib.INDEX_TYPE_CODES[experts.dtype], n, num_experts, _lib.ptr(experts), _lib.ptr(order),
-                            _lib.ptr(inverse), _lib.ptr(offsets), _lib.ptr(ws), need, _lib.stream_handle(device)),
+        lib.fs_expert_route(_lib.INDEX_TYPE_CODES[experts.dtype], n, num_experts, _lib.ptr(experts), places.data_ptr(),
+                            route._inverse_ptr, route._offsets_ptr, _lib.ptr(ws), need, _lib.stream_handle(device)),
         "fs_expert_route",
     )
-    return PreparedExpertRoute(n_tokens, slots, num_experts, order, inverse, offsets)
+    return route
 
 
 def _check_rows(rows, what, route, n_rows):
@@ -135,8 +146,8 @@ def _dispatch(x, route, out=None):
     result = _into(out, (route.n_rows, x.shape[1]), x)
     _lib.check(
         _lib.lib().fs_expert_dispatch(ROW_VALUE_CODES[x.dtype], route.n_tokens, route.slots, x.shape[1],
-                                      route.num_experts, _lib.ptr(x), ld, _lib.ptr(route.inverse),
-                                      _lib.ptr(route.offsets), _lib.ptr(result), _lib.stream_handle(x.device)),
+                                      route.num_experts, _lib.ptr(x), ld, route._inverse_ptr,
+                                      route._offsets_ptr, _lib.ptr(result), _lib.stream_handle(x.device)),
         "fs_expert_dispatch",
     )
     return _done(out, result)
@@ -148,8 +159,8 @@ def _combine(rows, route, weights, out=None):
     result = _into(out, (route.n_tokens, rows.shape[1]), rows)
     _lib.check(
         _lib.lib().fs_expert_combine(ROW_VALUE_CODES[rows.dtype], route.n_tokens, route.slots, rows.shape[1],
-                                     route.num_experts, _lib.ptr(rows), ld, _lib.ptr(route.inverse),
-                                     _lib.ptr(route.offsets), _lib.ptr(weights), _lib.ptr(result),
+                                     route.num_experts, _lib.ptr(rows), ld, route._inverse_ptr,
+                                     route._offsets_ptr, _lib.ptr(weights), _lib.ptr(result),
                                      _lib.stream_handle(rows.device)),
         "fs_expert_combine",
     )
@@ -250,7 +261,7 @@ def flagsparse_expert_combine_grad(grad, rows, route, weights):
     _lib.check(
         _lib.lib().fs_expert_combine_grad(ROW_VALUE_CODES[rows.dtype], route.n_tokens, route.slots, rows.shape[1],
                                           route.num_experts, _lib.ptr(grad), ldg, _lib.ptr(rows), ldr,
-                                          _lib.ptr(route.inverse), _lib.ptr(route.offsets), _lib.ptr(weights),
+                                          route._inverse_ptr, route._offsets_ptr, _lib.ptr(weights),
                                           _lib.ptr(grad_rows), _lib.ptr(grad_weights),
                                           _lib.stream_handle(rows.device)),
         "fs_expert_combine_grad",
@@ -297,10 +308,13 @@ def _product(rows, matrices, route, trans, inner, outer, out=None):
     rows, ld = row_major(rows)
     matrices, trans = _dense_matrices(matrices, trans)
     result = _into(out, (route.n_rows, outer), rows)
+    lib = _lib.lib()
+    sizes = (ROW_VALUE_CODES[rows.dtype], int(trans), route.n_rows, route.num_experts, inner, outer)
+    need = lib.fs_expert_product_workspace_bytes(*sizes)
+    ws = _lib.workspace(need, rows.device) if need else None
     _lib.check(
-        _lib.lib().fs_expert_product(ROW_VALUE_CODES[rows.dtype], int(trans), route.n_rows, route.num_experts, inner,
-                                     outer, _lib.ptr(rows), ld, _lib.ptr(matrices), _lib.ptr(route.offsets),
-                                     _lib.ptr(result), _lib.stream_handle(rows.device)),
+        lib.fs_expert_product(*sizes, _lib.ptr(rows), ld, _lib.ptr(matrices), route._offsets_ptr, _lib.ptr(result),
+                              _lib.ptr(ws), need, _lib.stream_handle(rows.device)),
         "fs_expert_product",
     )
     return _done(out, result)
@@ -311,10 +325,13 @@ def _product_grad_matrices(grad, rows, route, trans, inner, outer):
     rows, ldr = row_major(rows)
     shape = (route.num_experts, outer, inner) if trans else (route.num_experts, inner, outer)
     result = torch.empty(shape, dtype=rows.dtype, device=rows.device)
+    lib = _lib.lib()
+    sizes = (ROW_VALUE_CODES[rows.dtype], int(trans), route.n_rows, route.num_experts, inner, outer)
+    need = lib.fs_expert_product_grad_matrices_workspace_bytes(*sizes)
+    ws = _lib.workspace(need, rows.device) if need else None
     _lib.check(
-        _lib.lib().fs_expert_product_grad_matrices(
-            ROW_VALUE_CODES[rows.dtype], int(trans), route.n_rows, route.num_experts, inner, outer, _lib.ptr(grad), ldg,
-            _lib.ptr(rows), ldr, _lib.ptr(route.offsets), _lib.ptr(result), _lib.stream_handle(rows.device)),
+        lib.fs_expert_product_grad_matrices(*sizes, _lib.ptr(grad), ldg, _lib.ptr(rows), ldr, route._offsets_ptr,
+                                            _lib.ptr(result), _lib.ptr(ws), need, _lib.stream_handle(rows.device)),
         "fs_expert_product_grad_matrices",
     )
     return result

@@ -636,15 +636,21 @@ int fs_expert_combine_grad(int val_t, int64_t n_tokens, int slots, int64_t width
  * inner x outer each, or outer x inner with trans = 1.  The gradient of the
  * matrices, in their layout, sums rows[r]^T grad[r] (trans: grad[r]^T rows[r])
  * over each expert's rows; that of the rows is the product of grad with the
- * other trans, and inner and outer exchanged.
+ * other trans, and inner and outer exchanged.  The workspace takes the sums of
+ * tiles that several workgroups share (0 bytes for most sizes).
  */
+size_t fs_expert_product_workspace_bytes(int val_t, int trans, int64_t n_rows, int64_t n_experts,
+                                         int64_t inner, int64_t outer);
 int fs_expert_product(int val_t, int trans, int64_t n_rows, int64_t n_experts, int64_t inner,
                       int64_t outer, const void* rows, int64_t ldr, const void* matrices,
-                      const int32_t* offsets, void* out, hipStream_t stream);
+                      const int32_t* offsets, void* out, void* ws, size_t ws_bytes,
+                      hipStream_t stream);
+size_t fs_expert_product_grad_matrices_workspace_bytes(int val_t, int trans, int64_t n_rows,
+                                                       int64_t n_experts, int64_t inner, int64_t outer);
 int fs_expert_product_grad_matrices(int val_t, int trans, int64_t n_rows, int64_t n_experts,
                                     int64_t inner, int64_t outer, const void* grad, int64_t ldg,
                                     const void* rows, int64_t ldr, const int32_t* offsets,
-                                    void* grad_matrices, hipStream_t stream);
+                                    void* grad_matrices, void* ws, size_t ws_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

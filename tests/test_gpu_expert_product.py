@@ -99,9 +99,13 @@ def test_routed(dtype, op, n_tokens, slots, n_experts):
         _check(dtype, op, counts.tolist(), inner, outer, seed=outer)
 
 
-# enough and large enough tiles for the largest ones: of rows (first two), of the matrices' gradient (last)
+# enough and large enough tiles for the largest ones, of rows and of the matrices' gradient; the last two leave
+# a last round that is split
 @pytest.mark.parametrize("counts,inner,outer", [((700, 1, 513, 900), 264, 5512), ((256, 0, 1024), 40, 12808),
-                                                ((300, 0, 5, 260), 2056, 2080)], ids=["rows", "short", "matrices"])
+                                                ((300, 0, 5, 260), 2056, 2080),
+                                                ((1024, 1000, 300, 700), 1032, 5512),
+                                                ((900, 1400, 0, 1900), 2056, 2080)],
+                         ids=["rows", "short", "matrices", "rows_split", "matrices_split"])
 @pytest.mark.parametrize("op", ["non", "trans"])
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_many_tiles(dtype, op, counts, inner, outer):

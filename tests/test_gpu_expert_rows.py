@@ -202,8 +202,10 @@ def test_other_stream_and_graph():
 
 
 def test_kernel_names():
-    route, _, _ = _case((4, 2, 3, 0.0))
+    fs.prepare_expert_route(random_experts(5000, 1, 3, 1), 3)
     assert _lib.last_kernel() == "select_scatter_kernel"
+    route, _, _ = _case((4, 2, 3, 0.0))
+    assert _lib.last_kernel() == "select_small_kernel"
     x = randn((4, 8), torch.float32, 1)
     rows = fs.flagsparse_expert_dispatch(x, route)
     assert _lib.last_kernel() == "expert_dispatch_kernel"
