@@ -13,19 +13,24 @@ ROW_VALUE_CODES = {
 ROW_DTYPE_MESSAGE = "float16, bfloat16, float32, float64"
 
 
-def row_major(t):
+def row_major(t, width):
     """(t, stride of its rows) of a 2D tensor whose rows are contiguous; a copy
-    where they are not, or where rows overlap or run backwards."""
+    where they are not, or where rows overlap."""
     if t.is_contiguous():
-        return t, t.shape[1]
-    if t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
+        return t, width
+    if t.stride(1) == 1 and t.stride(0) >= width:
         return t, t.stride(0)
-    t = t.contiguous()
-    return t, t.shape[1]
+    return t.contiguous(), width
 
 
-def wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+recording = torch.is_grad_enabled
+
+
+def launch(function, device, *args):
+    """One call of a C entry point whose last argument is the stream."""
+    rc = function(*args, _lib.stream_handle(device))
+    if rc:
+        _lib.check(rc, function.__name__)
 
 
 def check_out(out, device, shape, dtype):

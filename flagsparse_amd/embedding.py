@@ -19,7 +19,7 @@ import torch
 
 from . import _lib
 from ._common import SUPPORTED_INDEX_DTYPES
-from ._rows import ROW_DTYPE_MESSAGE, ROW_VALUE_CODES, check_out, row_major, wants_grad
+from ._rows import ROW_DTYPE_MESSAGE, ROW_VALUE_CODES, check_out, launch, recording, row_major
 
 
 def _check_tokens(tokens, values, what):
@@ -45,18 +45,15 @@ def _normalize_padding(padding_idx, n_rows):
 
 
 def _lookup(table, tokens, scale, out=None):
-    n, (n_rows, width) = tokens.numel(), table.shape
-    table, ld = row_major(table)
-    tokens = tokens.contiguous()
+    n_rows, width = table.shape
+    table, ld = row_major(table, width)
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
     result = out
     if out is None or not out.is_contiguous():
-        result = torch.empty((*tokens.shape, width), dtype=table.dtype, device=table.device)
-    _lib.check(
-        _lib.lib().fs_embedding(ROW_VALUE_CODES[table.dtype], _lib.INDEX_TYPE_CODES[tokens.dtype], n, n_rows, width,
-                                _lib.ptr(table), ld, _lib.ptr(tokens), scale, _lib.ptr(result),
-                                _lib.stream_handle(table.device)),
-        "fs_embedding",
-    )
+        result = table.new_empty((*tokens.shape, width))
+    launch(_lib.lib().fs_embedding, table.device, ROW_VALUE_CODES[table.dtype], _lib.INDEX_TYPE_CODES[tokens.dtype],
+           tokens.numel(), n_rows, width, table.data_ptr(), ld, tokens.data_ptr(), scale, result.data_ptr())
     if out is not None and result is not out:
         out.copy_(result)
         return out
@@ -88,11 +85,12 @@ def flagsparse_embedding(table, tokens, scale=1.0, padding_idx=None, out=None):
     if table.ndim != 2:
         raise ValueError("table must be a 2D tensor: (rows, width)")
     scale = float(scale)
-    padding = _normalize_padding(padding_idx, table.shape[0])
-    if wants_grad(table):
+    if padding_idx is not None:
+        padding_idx = _normalize_padding(padding_idx, table.shape[0])
+    if table.requires_grad and recording():
         if out is not None:
             raise ValueError("out cannot be given where a gradient is recorded")
-        return _Embedding.apply(table, tokens, scale, None if padding < 0 else padding)
+        return _Embedding.apply(table, tokens, scale, padding_idx)
     if out is not None:
         check_out(out, table.device, (*tokens.shape, table.shape[1]), table.dtype)
     return _lookup(table, tokens, scale, out)
@@ -118,7 +116,7 @@ def flagsparse_embedding_grad(grad, tokens, num_rows, scale=1.0, padding_idx=Non
     n, width = tokens.numel(), grad.shape[-1]
     if out is not None:
         check_out(out, grad.device, (num_rows, width), dtype)
-    grad, ld = row_major(grad.reshape(n, width))
+    grad, ld = row_major(grad.reshape(n, width), width)
     tokens = tokens.contiguous()
     result = out
     if out is None or not out.is_contiguous():
@@ -126,12 +124,9 @@ def flagsparse_embedding_grad(grad, tokens, num_rows, scale=1.0, padding_idx=Non
     code = ROW_VALUE_CODES[grad.dtype]
     lib = _lib.lib()
     ws = _lib.workspace(lib.fs_embedding_grad_workspace_bytes(code, n, num_rows, width), grad.device)
-    _lib.check(
-        lib.fs_embedding_grad(code, ROW_VALUE_CODES[dtype], _lib.INDEX_TYPE_CODES[tokens.dtype], n, num_rows, width,
-                              _lib.ptr(grad), ld, _lib.ptr(tokens), float(scale), padding, _lib.ptr(result),
-                              _lib.ptr(ws), ws.numel(), _lib.stream_handle(grad.device)),
-        "fs_embedding_grad",
-    )
+    launch(lib.fs_embedding_grad, grad.device, code, ROW_VALUE_CODES[dtype], _lib.INDEX_TYPE_CODES[tokens.dtype], n,
+           num_rows, width, grad.data_ptr(), ld, tokens.data_ptr(), float(scale), padding, result.data_ptr(),
+           ws.data_ptr(), ws.numel())
     if out is not None and result is not out:
         out.copy_(result)
         return out

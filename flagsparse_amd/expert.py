@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from ._common import _INDEX_LIMIT_INT32, SUPPORTED_INDEX_DTYPES
-from ._rows import ROW_DTYPE_MESSAGE, ROW_VALUE_CODES, check_out, row_major, wants_grad
+from ._rows import ROW_DTYPE_MESSAGE, ROW_VALUE_CODES, check_out, launch, recording, row_major
 from .spmm_csr import _normalize_spmm_op, _spmm_op_transposes
 
 MAX_EXPERTS = 1023
@@ -59,7 +59,7 @@ class PreparedExpertRoute:
 
     @property
     def inverse(self):
-        return self._places[self.n_rows : 2 * self.n_rows].view(self.n_tokens, self.slots)
+        return self._places.as_strided((self.n_tokens, self.slots), (self.slots, 1), self.n_rows)
 
     @property
     def offsets(self):
@@ -92,11 +92,8 @@ def prepare_expert_route(experts, num_experts):
     lib = _lib.lib()
     need = lib.fs_expert_route_workspace_bytes(n, num_experts)
     ws = _lib.workspace(need, device) if need else None
-    _lib.check(
-        lib.fs_expert_route(_lib.INDEX_TYPE_CODES[experts.dtype], n, num_experts, _lib.ptr(experts), places.data_ptr(),
-                            route._inverse_ptr, route._offsets_ptr, _lib.ptr(ws), need, _lib.stream_handle(device)),
-        "fs_expert_route",
-    )
+    launch(lib.fs_expert_route, device, _lib.INDEX_TYPE_CODES[experts.dtype], n, num_experts, experts.data_ptr(),
+           places.data_ptr(), route._inverse_ptr, route._offsets_ptr, _lib.ptr(ws), need)
     return route
 
 
@@ -123,15 +120,15 @@ def _check_weights(weights, rows, route):
         raise TypeError(f"weights dtype must be {wide} for {rows.dtype} rows")
     if weights.device != route.device:
         raise ValueError("weights must be on the same CUDA device as the route")
-    if tuple(weights.shape) != (route.n_tokens, route.slots):
+    if weights.shape != (route.n_tokens, route.slots):
         raise ValueError(f"weights must have shape {(route.n_tokens, route.slots)}, got {tuple(weights.shape)}")
 
 
-def _into(out, shape, like):
+def _into(out, rows, width, like):
     """The tensor to write: out itself where it is contiguous."""
     if out is not None and out.is_contiguous():
         return out
-    return torch.empty(shape, dtype=like.dtype, device=like.device)
+    return like.new_empty((rows, width))
 
 
 def _done(out, result):
@@ -142,28 +139,23 @@ def _done(out, result):
 
 
 def _dispatch(x, route, out=None):
-    x, ld = row_major(x)
-    result = _into(out, (route.n_rows, x.shape[1]), x)
-    _lib.check(
-        _lib.lib().fs_expert_dispatch(ROW_VALUE_CODES[x.dtype], route.n_tokens, route.slots, x.shape[1],
-                                      route.num_experts, _lib.ptr(x), ld, route._inverse_ptr,
-                                      route._offsets_ptr, _lib.ptr(result), _lib.stream_handle(x.device)),
-        "fs_expert_dispatch",
-    )
+    width = x.shape[1]
+    x, ld = row_major(x, width)
+    result = _into(out, route.n_rows, width, x)
+    launch(_lib.lib().fs_expert_dispatch, route.device, ROW_VALUE_CODES[x.dtype], route.n_tokens, route.slots, width,
+           route.num_experts, x.data_ptr(), ld, route._inverse_ptr, route._offsets_ptr, result.data_ptr())
     return _done(out, result)
 
 
 def _combine(rows, route, weights, out=None):
-    rows, ld = row_major(rows)
-    weights = None if weights is None else weights.contiguous()
-    result = _into(out, (route.n_tokens, rows.shape[1]), rows)
-    _lib.check(
-        _lib.lib().fs_expert_combine(ROW_VALUE_CODES[rows.dtype], route.n_tokens, route.slots, rows.shape[1],
-                                     route.num_experts, _lib.ptr(rows), ld, route._inverse_ptr,
-                                     route._offsets_ptr, _lib.ptr(weights), _lib.ptr(result),
-                                     _lib.stream_handle(rows.device)),
-        "fs_expert_combine",
-    )
+    width = rows.shape[1]
+    rows, ld = row_major(rows, width)
+    if weights is not None and not weights.is_contiguous():
+        weights = weights.contiguous()
+    result = _into(out, route.n_tokens, width, rows)
+    launch(_lib.lib().fs_expert_combine, route.device, ROW_VALUE_CODES[rows.dtype], route.n_tokens, route.slots, width,
+           route.num_experts, rows.data_ptr(), ld, route._inverse_ptr, route._offsets_ptr,
+           None if weights is None else weights.data_ptr(), result.data_ptr())
     return _done(out, result)
 
 
@@ -203,7 +195,7 @@ def flagsparse_expert_dispatch(x, route, out=None):
     """
     n_tokens = route.n_tokens if isinstance(route, PreparedExpertRoute) else 0
     _check_rows(x, "x", route, n_tokens)
-    if wants_grad(x):
+    if x.requires_grad and recording():
         if out is not None:
             raise ValueError("out cannot be given where a gradient is recorded")
         return _Dispatch.apply(x, route)
@@ -231,7 +223,7 @@ def flagsparse_expert_combine(rows, route, weights=None, out=None):
     _check_rows(rows, "rows", route, n_rows)
     if weights is not None:
         _check_weights(weights, rows, route)
-    if wants_grad(rows, weights):
+    if (rows.requires_grad or (weights is not None and weights.requires_grad)) and recording():
         if out is not None:
             raise ValueError("out cannot be given where a gradient is recorded")
         return _Combine.apply(rows, route, weights)
@@ -253,19 +245,15 @@ def flagsparse_expert_combine_grad(grad, rows, route, weights):
     if grad.shape[1] != rows.shape[1]:
         raise ValueError(f"grad must have width {rows.shape[1]}, got {grad.shape[1]}")
     _check_weights(weights, rows, route)
-    grad, ldg = row_major(grad)
-    rows, ldr = row_major(rows)
+    width = rows.shape[1]
+    grad, ldg = row_major(grad, width)
+    rows, ldr = row_major(rows, width)
     weights = weights.contiguous()
-    grad_rows = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
-    grad_weights = torch.empty_like(weights)
-    _lib.check(
-        _lib.lib().fs_expert_combine_grad(ROW_VALUE_CODES[rows.dtype], route.n_tokens, route.slots, rows.shape[1],
-                                          route.num_experts, _lib.ptr(grad), ldg, _lib.ptr(rows), ldr,
-                                          route._inverse_ptr, route._offsets_ptr, _lib.ptr(weights),
-                                          _lib.ptr(grad_rows), _lib.ptr(grad_weights),
-                                          _lib.stream_handle(rows.device)),
-        "fs_expert_combine_grad",
-    )
+    grad_rows = rows.new_empty((route.n_rows, width))
+    grad_weights = weights.new_empty((route.n_tokens, route.slots))
+    launch(_lib.lib().fs_expert_combine_grad, route.device, ROW_VALUE_CODES[rows.dtype], route.n_tokens, route.slots,
+           width, route.num_experts, grad.data_ptr(), ldg, rows.data_ptr(), ldr, route._inverse_ptr, route._offsets_ptr,
+           weights.data_ptr(), grad_rows.data_ptr(), grad_weights.data_ptr())
     return grad_rows, grad_weights
 
 
@@ -305,35 +293,29 @@ def _dense_matrices(matrices, trans):
 
 
 def _product(rows, matrices, route, trans, inner, outer, out=None):
-    rows, ld = row_major(rows)
+    rows, ld = row_major(rows, inner)
     matrices, trans = _dense_matrices(matrices, trans)
-    result = _into(out, (route.n_rows, outer), rows)
+    result = _into(out, route.n_rows, outer, rows)
     lib = _lib.lib()
     sizes = (ROW_VALUE_CODES[rows.dtype], int(trans), route.n_rows, route.num_experts, inner, outer)
     need = lib.fs_expert_product_workspace_bytes(*sizes)
     ws = _lib.workspace(need, rows.device) if need else None
-    _lib.check(
-        lib.fs_expert_product(*sizes, _lib.ptr(rows), ld, _lib.ptr(matrices), route._offsets_ptr, _lib.ptr(result),
-                              _lib.ptr(ws), need, _lib.stream_handle(rows.device)),
-        "fs_expert_product",
-    )
+    launch(lib.fs_expert_product, route.device, *sizes, rows.data_ptr(), ld, matrices.data_ptr(), route._offsets_ptr,
+           result.data_ptr(), _lib.ptr(ws), need)
     return _done(out, result)
 
 
 def _product_grad_matrices(grad, rows, route, trans, inner, outer):
-    grad, ldg = row_major(grad)
-    rows, ldr = row_major(rows)
+    grad, ldg = row_major(grad, outer)
+    rows, ldr = row_major(rows, inner)
     shape = (route.num_experts, outer, inner) if trans else (route.num_experts, inner, outer)
-    result = torch.empty(shape, dtype=rows.dtype, device=rows.device)
+    result = rows.new_empty(shape)
     lib = _lib.lib()
     sizes = (ROW_VALUE_CODES[rows.dtype], int(trans), route.n_rows, route.num_experts, inner, outer)
     need = lib.fs_expert_product_grad_matrices_workspace_bytes(*sizes)
     ws = _lib.workspace(need, rows.device) if need else None
-    _lib.check(
-        lib.fs_expert_product_grad_matrices(*sizes, _lib.ptr(grad), ldg, _lib.ptr(rows), ldr, route._offsets_ptr,
-                                            _lib.ptr(result), _lib.ptr(ws), need, _lib.stream_handle(rows.device)),
-        "fs_expert_product_grad_matrices",
-    )
+    launch(lib.fs_expert_product_grad_matrices, route.device, *sizes, grad.data_ptr(), ldg, rows.data_ptr(), ldr,
+           route._offsets_ptr, result.data_ptr(), _lib.ptr(ws), need)
     return result
 
 
@@ -365,7 +347,7 @@ def flagsparse_expert_product(rows, matrices, route, op="non", out=None):
     for these real types).  Rows of no expert are zero.  Differentiable in both.
     """
     trans, inner, outer = _check_product(rows, matrices, route, op)
-    if wants_grad(rows, matrices):
+    if (rows.requires_grad or matrices.requires_grad) and recording():
         if out is not None:
             raise ValueError("out cannot be given where a gradient is recorded")
         return _Product.apply(rows, matrices, route, trans, inner, outer)
