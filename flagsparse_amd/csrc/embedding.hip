@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256) void embedding_kernel(const V* __restrict__ ta
                                                         typename Elem<V>::acc scale, V* __restrict__ out) {
   constexpr int E = Slice<V>::n;
   const int lane = threadIdx.x & (lpr - 1);
-  const int64_t t = (int64_t)blockIdx.x * (256 / lpr) + threadIdx.x / lpr;
+  const int64_t t = row_block() * (256 / lpr) + threadIdx.x / lpr;
   if (t >= n) return;
   const int64_t id = (int64_t)ids[t];
   const bool in = (uint64_t)id < (uint64_t)n_rows;
@@ -138,14 +138,15 @@ template <class V, class O, bool PAST>
 __global__ __launch_bounds__(256) void embedding_grad_kernel(
     const V* __restrict__ grad, int64_t ldg, const uint32_t* __restrict__ keys, const int32_t* __restrict__ order,
     int64_t n, int64_t n_rows, int64_t width, typename Elem<V>::acc scale, int64_t padding, int wpr, int block_rows,
-    uint32_t chunk_blocks, int64_t n_chunks, O* __restrict__ out, typename Elem<V>::acc* __restrict__ parts) {
+    int64_t chunk_blocks, int64_t n_chunks, O* __restrict__ out, typename Elem<V>::acc* __restrict__ parts) {
   using A = typename Elem<V>::acc;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t first = (int64_t)(w % wpr) * 64, stride = (int64_t)wpr * 64;
   const int groups = 4 / wpr;
 
-  if (blockIdx.x < chunk_blocks) {  // parts of long segments
-    const int64_t chunk = (int64_t)blockIdx.x * groups + w / wpr;
+  const int64_t block = row_block();
+  if (block < chunk_blocks) {  // parts of long segments
+    const int64_t chunk = block * groups + w / wpr;
     if (chunk >= n_chunks) return;
     const int64_t c0 = chunk * kLong;
     const int cnt = (int)(n - c0 < kLong ? n - c0 : kLong);
@@ -168,7 +169,7 @@ __global__ __launch_bounds__(256) void embedding_grad_kernel(
     return;
   }
 
-  const int64_t v0 = ((int64_t)(blockIdx.x - chunk_blocks) * groups + w / wpr) * block_rows;
+  const int64_t v0 = ((block - chunk_blocks) * groups + w / wpr) * block_rows;
   if (v0 >= n_rows) return;
   // a window of 64 sorted positions from the first row's on
   int64_t wb = wave_lower_bound(keys, n, (uint32_t)v0, lane);
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_grad_join_kernel(
   constexpr int C = 4, kAtOnce = 8;
   __shared__ A s_sum[kJoinWaves - 1][C][64];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t c0 = (int64_t)blockIdx.x * kLong;
+  const int64_t chunk = (int64_t)blockIdx.z * gridDim.x + blockIdx.x, c0 = chunk * kLong;
   if (c0 + kLong >= n) return;  // the last chunk starts none that leaves it
   const uint32_t kr = keys[c0 + kLong - 1];
   if (keys[c0 + kLong] != kr || (int64_t)kr >= n_rows || (int64_t)kr == padding) return;
@@ -225,14 +226,14 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_grad_join_kernel(
   const int f = __builtin_ctzll(__ballot(keys[c0 + lane] == kr));
   if (c0 + f + kLong >= n || keys[c0 + f + kLong] != kr) return;  // summed at once
   const int64_t end = wave_lower_bound(keys, n, kr + 1, lane);
-  const int64_t count = (end - 1) / kLong - blockIdx.x + 1;  // chunks that hold it
+  const int64_t count = (end - 1) / kLong - chunk + 1;  // chunks that hold it
   int64_t h[C];
 #pragma unroll
   for (int u = 0; u < C; ++u) {
     const int64_t own = (int64_t)blockIdx.y * 64 * C + u * 64 + lane;
     h[u] = own < width ? own : width - 1;
   }
-  auto part = [&](int64_t k) { return parts + ((blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * width; };
+  auto part = [&](int64_t k) { return parts + ((chunk + k) * 2 + (k == 0 ? 1 : 0)) * width; };
   A sum[C] = {};
   for (int64_t k = w; k < count; k += kJoinWaves * kAtOnce) {
     A v[kAtOnce][C];
@@ -277,7 +278,7 @@ GradLayout grad_layout(int val_t, int64_t n, int64_t n_rows, int64_t width) {
 }
 
 int check_sizes(const char* who, int64_t n, int64_t n_rows, int64_t width) {
-  if (n < 0 || n > INT32_MAX || n_rows < 0 || n_rows >= INT32_MAX || width < 0)
+  if (n < 0 || n > INT32_MAX || n_rows < 0 || n_rows >= INT32_MAX || width < 0 || width > 65535 * 256)
     return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
   return FS_OK;
 }
@@ -296,7 +297,7 @@ extern "C" int fs_embedding(int val_t, int id_t, int64_t n, int64_t n_rows, int6
     using V = decltype(v);
     using A = typename Elem<V>::acc;
     const int lpr = lanes_per_row(slices_of<V>(width));
-    const dim3 grid((uint32_t)ceil_div(n, 256 / lpr));
+    const dim3 grid = row_grid(ceil_div(n, 256 / lpr));
     auto launch = [&](auto id) {
       using Id = decltype(id);
       hipLaunchKernelGGL((embedding_kernel<V, Id>), grid, dim3(256), 0, stream, (const V*)table, ldt, n_rows,
@@ -346,8 +347,8 @@ extern "C" int fs_embedding_grad(int val_t, int out_t, int id_t, int64_t n, int6
       // up to 16 rows, so that workgroups fill the chip: 131072 tokens x 2048 of
       // 2000 rows, bf16, 206 us with 16, 168 with 4; 65536 of 131072: 238 and 267
       const int block_rows = (int)std::min<int64_t>(16, std::max<int64_t>(2, n_rows / (2048 * (4 / wpr))));
-      const uint32_t chunk_blocks = (uint32_t)ceil_div(chunks, 4 / wpr);
-      const dim3 grid(chunk_blocks + (uint32_t)ceil_div(n_rows, (4 / wpr) * block_rows));
+      const int64_t chunk_blocks = ceil_div(chunks, 4 / wpr);
+      const dim3 grid = row_grid(chunk_blocks + ceil_div(n_rows, (4 / wpr) * block_rows));
       auto launch = [&](auto past) {
         hipLaunchKernelGGL((embedding_grad_kernel<V, O, decltype(past)::value>), grid, dim3(256), 0, stream,
                            (const V*)grad, ldg, keys, order, n, n_rows, width, (A)scale, padding, wpr, block_rows,
@@ -358,7 +359,8 @@ extern "C" int fs_embedding_grad(int val_t, int out_t, int id_t, int64_t n, int6
       else launch(std::false_type{});
       FS_CHECK_MAIN_LAUNCH("embedding_grad_kernel");
       if (chunks > 0) {
-        hipLaunchKernelGGL((embedding_grad_join_kernel<O, A>), dim3((uint32_t)chunks, (uint32_t)ceil_div(width, 256)),
+        const dim3 x = row_grid(chunks);
+        hipLaunchKernelGGL((embedding_grad_join_kernel<O, A>), dim3(x.x, (uint32_t)ceil_div(width, 256), x.y),
                            dim3(64 * kJoinWaves), 0, stream, keys, n, n_rows, width, (A)scale, padding, parts, (O*)out);
         FS_CHECK_LAUNCH("embedding_grad_join_kernel");
       }

@@ -300,7 +300,7 @@ __device__ inline TilePlan plan_tiles(const ProductArgs& p, int lane) {
     int total = 0;
     for (int e0 = 0; e0 < p.n_experts; e0 += 64) {
       const int e = e0 + lane;
-      const int own = e < p.n_experts ? (p.offsets[e + 1] - p.offsets[e] + BM - 1) / BM : 0;
+      const int own = e < p.n_experts ? (int)(((int64_t)p.offsets[e + 1] - p.offsets[e] + BM - 1) / BM) : 0;
       total += __builtin_amdgcn_readlane((int)wave_sum_scan((uint32_t)own), 63);
     }
     l.real = (uint32_t)total * nt;
@@ -763,7 +763,7 @@ int launch_tiles(ProductArgs p, hipStream_t stream) {
   constexpr bool kSplit = WM * WN == 8;
   if (!kSplit) p.parts = nullptr;
   const int64_t tiles = tiles_of<MODE, BM, BN>(p) + (p.parts != nullptr ? p.cus : 0);
-  if (tiles > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
+  if (tiles * 64 * WM * WN > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
   hipLaunchKernelGGL((expert_product_kernel<T, MODE, DMA, BM, BN, WM, WN>), dim3((uint32_t)tiles),
                      dim3(64 * WM * WN), 0, stream, p);
   FS_CHECK_MAIN_LAUNCH("expert_product_kernel");
@@ -781,7 +781,7 @@ template <class T, int MODE, bool DMA>
 int launch_few(ProductArgs p, hipStream_t stream) {
   p.parts = nullptr;
   const int64_t tiles = tiles_of<MODE, kFewRows, kFewCols>(p);
-  if (tiles > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
+  if (tiles * 256 > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
   hipLaunchKernelGGL((expert_product_few_kernel<T, MODE, DMA>), dim3((uint32_t)tiles), dim3(256), 0, stream, p);
   FS_CHECK_MAIN_LAUNCH("expert_product_few_kernel");
   return FS_OK;

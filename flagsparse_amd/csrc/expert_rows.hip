@@ -24,7 +24,7 @@ __global__ __launch_bounds__(256) void expert_dispatch_kernel(const V* __restric
                                                               const int32_t* __restrict__ routed_at,
                                                               V* __restrict__ out) {
   const int lane = threadIdx.x & (lpr - 1);
-  const int64_t t = (int64_t)blockIdx.x * (256 / lpr) + threadIdx.x / lpr;
+  const int64_t t = row_block() * (256 / lpr) + threadIdx.x / lpr;
   if (t >= n_tokens) return;
   const int routed = *routed_at;
   const V* row = x + t * ldx;
@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(const V* __restrict
   using A = typename Elem<V>::acc;
   constexpr int E = Slice<V>::n, kAtOnce = 4;
   const int lane = threadIdx.x & (lpr - 1);
-  const int64_t t = (int64_t)blockIdx.x * (256 / lpr) + threadIdx.x / lpr;
+  const int64_t t = row_block() * (256 / lpr) + threadIdx.x / lpr;
   if (t >= n_tokens) return;
   const int routed = *routed_at;
   const int32_t* inv = inverse + t * slots;
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(256) void expert_combine_grad_kernel(
   using A = typename Elem<V>::acc;
   constexpr int E = Slice<V>::n;
   const int lane = threadIdx.x & 63;
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t i = row_block() * 4 + (threadIdx.x >> 6);
   if (i >= n) return;
   const int at = inverse[i];
   const bool in = at < *routed_at;
@@ -161,7 +161,7 @@ extern "C" int fs_expert_dispatch(int val_t, int64_t n_tokens, int slots, int64_
   return with_value_type(val_t, "fs_expert_dispatch", [&](auto v) -> int {
     using V = decltype(v);
     const int lpr = lanes_per_row(slices_of<V>(width));
-    const dim3 grid((uint32_t)ceil_div(n_tokens, 256 / lpr));
+    const dim3 grid = row_grid(ceil_div(n_tokens, 256 / lpr));
     auto launch = [&](auto past) {
       hipLaunchKernelGGL((expert_dispatch_kernel<V, decltype(past)::value>), grid, dim3(256), 0, stream, (const V*)x, ldx, n_tokens,
                          slots, width, lpr, inverse, offsets + n_experts, (V*)out);
@@ -184,7 +184,7 @@ extern "C" int fs_expert_combine(int val_t, int64_t n_tokens, int slots, int64_t
     using V = decltype(v);
     using A = typename Elem<V>::acc;
     const int lpr = lanes_per_row(slices_of<V>(width));
-    const dim3 grid((uint32_t)ceil_div(n_tokens, 256 / lpr));
+    const dim3 grid = row_grid(ceil_div(n_tokens, 256 / lpr));
     auto launch = [&](auto past) {
       hipLaunchKernelGGL((expert_combine_kernel<V, decltype(past)::value>), grid, dim3(256), 0, stream, (const V*)rows, ldr, n_tokens,
                          slots, width, lpr, inverse, offsets + n_experts, (const A*)weights, (V*)out);
@@ -210,7 +210,7 @@ extern "C" int fs_expert_combine_grad(int val_t, int64_t n_tokens, int slots, in
     using V = decltype(v);
     using A = typename Elem<V>::acc;
     const int64_t n = n_tokens * slots;
-    const dim3 grid((uint32_t)ceil_div(n, 4));
+    const dim3 grid = row_grid(ceil_div(n, 4));
     auto launch = [&](auto past) {
       hipLaunchKernelGGL((expert_combine_grad_kernel<V, decltype(past)::value>), grid, dim3(256), 0, stream, (const V*)grad, ldg,
                          (const V*)rows, ldr, n, slots, width, inverse, offsets + n_experts, (const A*)weights,

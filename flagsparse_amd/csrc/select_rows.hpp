@@ -106,6 +106,13 @@ inline int lanes_per_row(int64_t slices) {
   return l;
 }
 
+// Workgroups in two dimensions: a dimension of a grid holds below 2^32 threads.
+inline dim3 row_grid(int64_t blocks) {
+  const int64_t x = std::min<int64_t>(blocks, 1 << 22);
+  return dim3((uint32_t)x, (uint32_t)ceil_div(blocks, x));
+}
+__device__ inline int64_t row_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // Runs f with a value of the value type: real types only.
 template <class F>
 int with_value_type(int val_t, const char* who, F&& f) {

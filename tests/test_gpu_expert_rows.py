@@ -140,6 +140,20 @@ def test_offsets_past_32_bits():
     assert torch.equal(grad_w[-1], (x[-1, 0].float() ** 2 * width).expand(slots))
 
 
+def test_more_slots_than_one_grid_dimension_has_threads_for():
+    n_tokens = 34_000_000  # 68 M slots, a wave each: over 2^32 threads
+    experts = torch.zeros((n_tokens, 2), dtype=torch.int32, device=DEV)
+    experts[:, 1] = 1
+    experts[-3, 0] = -1
+    route = fs.prepare_expert_route(experts, 2)
+    assert route.offsets.tolist() == [0, n_tokens - 1, 2 * n_tokens - 1]
+    grad = torch.ones((n_tokens, 8), dtype=torch.float16, device=DEV)
+    rows = torch.full((2 * n_tokens, 8), 2.0, dtype=torch.float16, device=DEV)
+    grad_rows, grad_weights = fs.flagsparse_expert_combine_grad(grad, rows, route, torch.full((n_tokens, 2), 0.5, device=DEV))
+    assert bool((grad_rows[:-1] == 0.5).all()) and not bool(grad_rows[-1].any())
+    assert float(grad_weights[-3, 0]) == 0.0 and int((grad_weights == 16.0).sum()) == 2 * n_tokens - 1
+
+
 def test_autograd_matches_formula_and_differences():
     route, inverse, inside = _case((9, 3, 4, 0.2))
     x = randn((9, 5), torch.float64, 1).requires_grad_()
