@@ -48,7 +48,8 @@ class PreparedExpertRoute:
         n = n_tokens * slots
         self.n_tokens, self.slots, self.num_experts, self.n_rows = n_tokens, slots, num_experts, n
         self.device = places.device
-        # one int32 tensor: order, inverse, offsets (views of it cost more than the sort of a decode step)
+        # one int32 tensor: order, inverse, offsets and the sort's scratch (views of it cost more than the sort
+        # of a decode step)
         self._places = places
         start = places.data_ptr()
         self._inverse_ptr, self._offsets_ptr = start + 4 * n, start + 8 * n
@@ -63,7 +64,7 @@ class PreparedExpertRoute:
 
     @property
     def offsets(self):
-        return self._places[2 * self.n_rows :]
+        return self._places[2 * self.n_rows : 2 * self.n_rows + self.num_experts + 1]
 
 
 def prepare_expert_route(experts, num_experts):
@@ -87,13 +88,14 @@ def prepare_expert_route(experts, num_experts):
         raise ValueError("tokens * slots exceeds the int32 range")
     experts = experts.contiguous()
     device = experts.device
-    places = torch.empty(2 * n + num_experts + 1, dtype=torch.int32, device=device)
-    route = PreparedExpertRoute(n_tokens, slots, num_experts, places)
     lib = _lib.lib()
     need = lib.fs_expert_route_workspace_bytes(n, num_experts)
-    ws = _lib.workspace(need, device) if need else None
-    launch(lib.fs_expert_route, device, _lib.INDEX_TYPE_CODES[experts.dtype], n, num_experts, experts.data_ptr(),
-           places.data_ptr(), route._inverse_ptr, route._offsets_ptr, _lib.ptr(ws), need)
+    scratch = (2 * n + num_experts + 64) // 64 * 64  # 256-byte boundary behind the places
+    places = torch.empty(scratch + (need + 3) // 4, dtype=torch.int32, device=device)
+    route = PreparedExpertRoute(n_tokens, slots, num_experts, places)
+    start = places.data_ptr()
+    launch(lib.fs_expert_route, device, _lib.INDEX_TYPE_CODES[experts.dtype], n, num_experts, experts.data_ptr(), start,
+           route._inverse_ptr, route._offsets_ptr, start + 4 * scratch, need)
     return route
 
 
