@@ -76,10 +76,11 @@ struct Operand {
     else if constexpr (sizeof(T) == 4) return ((row >> 2) & 1) * 4;
     else return ((row & 3) + (kPerRow >= 16 ? ((row >> 3) & 1) * 4 : 0)) * 2;
   }
-  __device__ static int row_of(int i, int tid) { return (i * THREADS + tid) / kPerRow; }
-  __device__ static int piece_of(int i, int tid) {
-    return ((i * THREADS + tid) % kPerRow) ^ swizzle(row_of(i, tid));
-  }
+  // The q-th piece of the slice in LDS: its row, and which piece of it it is.
+  __device__ static int row_at(int q) { return q / kPerRow; }
+  __device__ static int piece_at(int q) { return (q % kPerRow) ^ swizzle(row_at(q)); }
+  __device__ static int row_of(int i, int tid) { return row_at(i * THREADS + tid); }
+  __device__ static int piece_of(int i, int tid) { return piece_at(i * THREADS + tid); }
 
   // Fragment of 16 tile rows from r0: lane l has tile row l % 16, k piece l / 16.
   __device__ static uint32_t frag_offset(int r0, int lane) {
@@ -170,20 +171,26 @@ __device__ inline void store_pieces(uint32_t lds, int tid, const u32x4 (&r)[O::k
   for (int i = 0; i < O::kPieces; ++i) *(lds_u32x4*)(lds_byte*)(uintptr_t)(lds + (uint32_t)(i * threads + tid) * 16) = r[i];
 }
 
-// The same pieces straight to LDS (buffer loads that write LDS, 64 lanes x 16
-// bytes from the address in M0): nothing in registers but an offset a piece.
-// Offsets below kInBuffer count from the step's base, which moves; a piece
-// outside the operand gets one beyond it, and the load writes zeros.
+// The same straight to LDS (buffer loads that write LDS, 64 lanes x WIDTH bytes
+// from the address in M0): nothing in registers but an offset a load.  WIDTH 16
+// takes whole pieces, 4 operands whose rows only start on whole words (2046 x
+// 4094 bf16, 32 experts, 8192 rows: 250 us, through registers 376, 2048 x 4096
+// with WIDTH 16 190); 16-bit rows off whole words go through registers.
+// Offsets below kInBuffer count from the step's base, which moves; a load
+// outside the operand gets one beyond it, and writes zeros.
 constexpr uint32_t kInBuffer = 1u << 30;
 
-__device__ inline void lds_dma16(uint32_t lds, uint32_t offset, u32x4 rsrc) {
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %1, %2, 0 offen lds"
-      :
-      : "s"(lds), "v"(offset), "s"(rsrc)
-      : "memory");  // (nothing else here uses M0)
+// (No register is written, so none is taken too early; M0 has no other use here.)
+template <int WIDTH>
+__device__ inline void lds_dma(uint32_t lds, uint32_t offset, u32x4 rsrc) {
+  if constexpr (WIDTH == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset),
+                 "s"(rsrc)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset),
+                 "s"(rsrc)
+                 : "memory");
 }
 __device__ inline u32x4 buffer_at(const void* p) {
   const uint64_t a = (uint64_t)(uintptr_t)p;
@@ -191,32 +198,36 @@ __device__ inline u32x4 buffer_at(const void* p) {
                (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)) & 0xffffu, kInBuffer, 0x00020000u};
 }
 
-template <class O, class T, bool KC, int THREADS>
+template <class O, class T, bool KC, int THREADS, int WIDTH>
 struct Dma {
-  uint32_t off[O::kPieces];
+  static constexpr int kLoads = O::kBytes / THREADS / WIDTH;  // a thread's, each step
+  uint32_t off[kLoads];
   const char* base;
   int64_t step;  // bytes from one step to the next
+  // the i-th load of thread tid: LDS row, and element in it
+  __device__ static int row(int i, int tid) { return O::row_at((i * THREADS + tid) * WIDTH / 16); }
+  __device__ static int element(int i, int tid) {
+    const int at = (i * THREADS + tid) * WIDTH;
+    return O::piece_at(at / 16) * O::E + at % 16 / (int)sizeof(T);
+  }
   __device__ void init(const Source<T>& s, int tid) {
     base = (const char*)s.base;
     step = KC ? (int64_t)kRowBytes : s.ld * (int64_t)sizeof(T) * O::BK;
 #pragma unroll
-    for (int i = 0; i < O::kPieces; ++i) {
-      const int row = O::row_of(i, tid), piece = O::piece_of(i, tid);
-      const bool in = KC ? row < s.tile_rows : piece * O::E < s.tile_rows;
-      off[i] = in ? (uint32_t)(row * s.ld * (int64_t)sizeof(T)) + (uint32_t)piece * 16u : 2u * kInBuffer;
+    for (int i = 0; i < kLoads; ++i) {
+      const bool in = (KC ? row(i, tid) : element(i, tid)) < s.tile_rows;
+      off[i] = in ? (uint32_t)((row(i, tid) * s.ld + element(i, tid)) * (int64_t)sizeof(T)) : 2u * kInBuffer;
     }
   }
   // Before the loads of a step that has only `left` of k (none or less: zeros).
   __device__ void cut(int64_t left, int tid) {
 #pragma unroll
-    for (int i = 0; i < O::kPieces; ++i) {
-      const int k0 = KC ? O::piece_of(i, tid) * O::E : O::row_of(i, tid);
-      if (k0 >= left) off[i] |= kInBuffer;
-    }
+    for (int i = 0; i < kLoads; ++i)
+      if ((KC ? element(i, tid) : row(i, tid)) >= left) off[i] |= kInBuffer;
   }
   __device__ u32x4 at(int64_t kt) const { return buffer_at(base + kt * step); }
   __device__ void issue(uint32_t lds, u32x4 rsrc, int i, int w) const {
-    lds_dma16(lds + (uint32_t)(i * THREADS + w * 64) * 16, off[i], rsrc);
+    lds_dma<WIDTH>(lds + (uint32_t)(i * THREADS + w * 64) * WIDTH, off[i], rsrc);
   }
 };
 
@@ -440,7 +451,7 @@ __device__ inline void store_four(T* row, int n, int cols, f32x4 v) {
   }
 }
 
-template <class T, int MODE, bool DMA, int BM, int BN, int WM, int WN>
+template <class T, int MODE, int WIDTH, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const ProductArgs p) {
   constexpr int THREADS = 64 * WM * WN;
   constexpr bool AKC = MODE != kMatrix, BKC = MODE == kRowsTrans;
@@ -448,7 +459,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
   using OB = Operand<T, BKC, BN, THREADS>;
   constexpr int BK = OA::BK;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  constexpr int kSlots = DMA ? 4 : 2, kSlot = OA::kBytes + OB::kBytes;
+  constexpr int kSlots = WIDTH ? 4 : 2, kSlot = OA::kBytes + OB::kBytes;
   __shared__ alignas(1024) uint8_t s_mem[kSlots][kSlot];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -487,13 +498,13 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::run(fb[j], fa[i], acc[i][j]);
   };
-  if constexpr (DMA) {
+  if constexpr (WIDTH != 0) {
     // Loads are started three steps ahead.  Every wave starts its share of every
     // step's, also of the three steps past the last (zeros), so that counting
     // those still under way tells which step has arrived.
-    constexpr int kLoads = OA::kPieces + OB::kPieces;
-    Dma<OA, T, AKC, THREADS> da;
-    Dma<OB, T, BKC, THREADS> db;
+    Dma<OA, T, AKC, THREADS, WIDTH> da;
+    Dma<OB, T, BKC, THREADS, WIDTH> db;
+    constexpr int kLoadsA = da.kLoads, kLoads = da.kLoads + db.kLoads;
     da.init(sa, tid);
     db.init(sb, tid);
     u32x4 rsrc_a, rsrc_b;
@@ -509,8 +520,8 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
       next = lds + (uint32_t)(kt & 3) * kSlot;
     };
     auto load = [&](int i) {
-      if (i < OA::kPieces) da.issue(next, rsrc_a, i, w);
-      else db.issue(next + OA::kBytes, rsrc_b, i - OA::kPieces, w);
+      if (i < kLoadsA) da.issue(next, rsrc_a, i, w);
+      else db.issue(next + OA::kBytes, rsrc_b, i - kLoadsA, w);
     };
     for (int64_t kt = first; kt < first + 3; ++kt) {
       begin_loads(kt);
@@ -520,7 +531,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
     if constexpr (WM * WN == 8) {
       // Two groups of four waves, one wave a SIMD each, half a step apart: one
       // multiplies, and starts loads in between, while the other reads fragments.
-      static_assert(kLoads <= FM, "a load between the products of two rows");
+      constexpr int kBetween = (kLoads + FM - 1) / FM;  // loads between the products of two rows
       const bool second = w >= 4;
       wait_loads<2 * kLoads>();
       barrier();
@@ -536,7 +547,9 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
 #pragma unroll
           for (int i = 0; i < FM; ++i) {
             if (whole || i < fm) multiply_row(i);
-            if (i < kLoads) load(i);  // its slot was last read two phases ago
+#pragma unroll
+            for (int q = 0; q < kBetween; ++q)
+              if (i * kBetween + q < kLoads) load(i * kBetween + q);  // the slot was last read two phases ago
             __builtin_amdgcn_sched_barrier(0);
           }
           __builtin_amdgcn_s_setprio(0);
@@ -637,13 +650,13 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_join_kernel(const
 // of its own and without barriers, so that many loads are under way; their sums
 // are added in wave order at the end.
 constexpr int kFewRows = 16, kFewCols = 64;
-template <class T, int MODE, bool DMA>
+template <class T, int MODE, int WIDTH>
 __global__ __launch_bounds__(256) void expert_product_few_kernel(const ProductArgs p) {
   constexpr bool BKC = MODE == kRowsTrans;
   using OA = Operand<T, true, kFewRows, 64>;
   using OB = Operand<T, BKC, kFewCols, 64>;
   constexpr int BK = OA::BK, FN = kFewCols / 16, kWaves = 4;
-  constexpr int kSlots = DMA ? 4 : 1, kSlot = OA::kBytes + OB::kBytes;
+  constexpr int kSlots = WIDTH ? 4 : 1, kSlot = OA::kBytes + OB::kBytes;
   static_assert(kSlots * kSlot >= FN * 64 * 16, "a wave's sums fit its slots");
   __shared__ alignas(1024) uint8_t s_mem[kWaves][kSlots][kSlot];
 
@@ -668,10 +681,10 @@ __global__ __launch_bounds__(256) void expert_product_few_kernel(const ProductAr
   };
   const int64_t steps = (sa.k + BK - 1) / BK;
 
-  if constexpr (DMA) {
-    constexpr int kLoads = OA::kPieces + OB::kPieces;
-    Dma<OA, T, true, 64> da;
-    Dma<OB, T, BKC, 64> db;
+  if constexpr (WIDTH != 0) {
+    Dma<OA, T, true, 64, WIDTH> da;
+    Dma<OB, T, BKC, 64, WIDTH> db;
+    constexpr int kLoads = da.kLoads + db.kLoads;
     da.init(sa, lane);
     db.init(sb, lane);
     auto load = [&](int64_t i) {  // the wave's i-th step
@@ -683,9 +696,9 @@ __global__ __launch_bounds__(256) void expert_product_few_kernel(const ProductAr
       const u32x4 ra = da.at(kt), rb = db.at(kt);
       const uint32_t next = lds + (uint32_t)(i & 3) * kSlot;
 #pragma unroll
-      for (int q = 0; q < OA::kPieces; ++q) da.issue(next, ra, q, 0);
+      for (int q = 0; q < da.kLoads; ++q) da.issue(next, ra, q, 0);
 #pragma unroll
-      for (int q = 0; q < OB::kPieces; ++q) db.issue(next + OA::kBytes, rb, q, 0);
+      for (int q = 0; q < db.kLoads; ++q) db.issue(next + OA::kBytes, rb, q, 0);
     };
     for (int i = 0; i < 3; ++i) load(i);
     for (int64_t i = 0; w + i * kWaves < steps; ++i) {
@@ -758,13 +771,13 @@ bool may_split(const ProductArgs& p) {
 // The most sums that split tiles leave: one a compute unit.
 size_t parts_bytes(const ProductArgs& p) { return (size_t)p.cus * kLarge * kLarge * sizeof(float); }
 
-template <class T, int MODE, bool DMA, int BM, int BN, int WM, int WN>
+template <class T, int MODE, int WIDTH, int BM, int BN, int WM, int WN>
 int launch_tiles(ProductArgs p, hipStream_t stream) {
   constexpr bool kSplit = WM * WN == 8;
   if (!kSplit) p.parts = nullptr;
   const int64_t tiles = tiles_of<MODE, BM, BN>(p) + (p.parts != nullptr ? p.cus : 0);
   if (tiles * 64 * WM * WN > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
-  hipLaunchKernelGGL((expert_product_kernel<T, MODE, DMA, BM, BN, WM, WN>), dim3((uint32_t)tiles),
+  hipLaunchKernelGGL((expert_product_kernel<T, MODE, WIDTH, BM, BN, WM, WN>), dim3((uint32_t)tiles),
                      dim3(64 * WM * WN), 0, stream, p);
   FS_CHECK_MAIN_LAUNCH("expert_product_kernel");
   if constexpr (kSplit) {
@@ -777,12 +790,12 @@ int launch_tiles(ProductArgs p, hipStream_t stream) {
   return FS_OK;
 }
 
-template <class T, int MODE, bool DMA>
+template <class T, int MODE, int WIDTH>
 int launch_few(ProductArgs p, hipStream_t stream) {
   p.parts = nullptr;
   const int64_t tiles = tiles_of<MODE, kFewRows, kFewCols>(p);
   if (tiles * 256 > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
-  hipLaunchKernelGGL((expert_product_few_kernel<T, MODE, DMA>), dim3((uint32_t)tiles), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((expert_product_few_kernel<T, MODE, WIDTH>), dim3((uint32_t)tiles), dim3(256), 0, stream, p);
   FS_CHECK_MAIN_LAUNCH("expert_product_few_kernel");
   return FS_OK;
 }
@@ -795,7 +808,7 @@ int launch_few(ProductArgs p, hipStream_t stream) {
 //   (N, K), "trans"      4: 100 107 112 132     32: 164 114 119 138   128: 414 181 160 154
 //   matrix gradient                              32:  -  213 203 190   512:  -  516 457 395
 //   float32, (K, N)      8: 188 263 485 995     32: 302 276 486 993  1024:  - 2258 2093 2519 (16 experts)
-//   no whole 16 bytes    8: 141 148 188         32: 229 151 203       128: 595 317 277
+//   no whole words       8: 141 148 188         32: 229 151 203       128: 595 317 277
 // Large tiles read whole lines of (K, N) matrices, which is why they serve few
 // rows too; of (N, K) ones they read 64 bytes of a row at a time.  One token
 // (8 experts of 64, 4096 columns): few 28, 64 x 128 23, 256 x 256 42; (1 of 8,
@@ -818,35 +831,40 @@ Tiles choose_tiles(const ProductArgs& p, bool half, bool dma) {
   return rows >= (half ? 40 : 768) && tiles128 >= kFill ? kTiles128 : kTiles64;
 }
 
-template <class T, int MODE>
+template <class T, int MODE, int WIDTH>
 int launch_product(ProductArgs p, void* ws, size_t ws_bytes, hipStream_t stream) {
-  // straight to LDS: whole 16-byte pieces, and offsets within a step that fit
-  const int64_t s = sizeof(T), reach = MODE == kMatrix ? kRowBytes / s : kLarge;
-  const bool dma = aligned16(p.a, p.lda * s) && aligned16(p.b, p.ldb * s) && p.b_expert * s % 16 == 0 &&
-                   (MODE == kMatrix ? p.m : p.k) * s % 16 == 0 && (MODE == kRowsTrans ? p.k : p.n) * s % 16 == 0 &&
-                   reach * std::max(p.lda, p.ldb) * s < (int64_t)kInBuffer;
-  switch (choose_tiles<MODE>(p, s == 2, dma)) {
+  switch (choose_tiles<MODE>(p, sizeof(T) == 2, WIDTH != 0)) {
     case kFew:
-      if constexpr (MODE != kMatrix)
-        return dma ? launch_few<T, MODE, true>(p, stream) : launch_few<T, MODE, false>(p, stream);
+      if constexpr (MODE != kMatrix) return launch_few<T, MODE, WIDTH>(p, stream);
       break;
-    case kTiles64:
-      return dma ? launch_tiles<T, MODE, true, 64, 128, 2, 2>(p, stream)
-                 : launch_tiles<T, MODE, false, 64, 128, 2, 2>(p, stream);
-    case kTiles128:
-      return dma ? launch_tiles<T, MODE, true, 128, 128, 2, 2>(p, stream)
-                 : launch_tiles<T, MODE, false, 128, 128, 2, 2>(p, stream);
+    case kTiles64: return launch_tiles<T, MODE, WIDTH, 64, 128, 2, 2>(p, stream);
+    case kTiles128: return launch_tiles<T, MODE, WIDTH, 128, 128, 2, 2>(p, stream);
     case kTiles256:
-      if constexpr (s == 2) {
+      if constexpr (sizeof(T) == 2 && WIDTH != 0) {
         if (may_split<MODE>(p)) {
           if (ws == nullptr || ws_bytes < parts_bytes(p))
             return fail(FS_E_WORKSPACE, "fs_expert_product: workspace too small");
           p.parts = static_cast<float*>(ws);
         }
-        return launch_tiles<T, MODE, true, kLarge, kLarge, 2, 4>(p, stream);
+        return launch_tiles<T, MODE, WIDTH, kLarge, kLarge, 2, 4>(p, stream);
       }
   }
   return fail(FS_E_INVALID, "fs_expert_product: no tiles");
+}
+
+template <class T, int MODE>
+int launch_product(const ProductArgs& p, void* ws, size_t ws_bytes, hipStream_t stream) {
+  // straight to LDS: rows and ends of rows on whole loads, and offsets within a
+  // step that fit
+  const int64_t s = sizeof(T), reach = MODE == kMatrix ? kRowBytes / s : kLarge;
+  auto whole = [&](int64_t width) {
+    const int64_t ends = (MODE == kMatrix ? p.m : p.k) | (MODE == kRowsTrans ? p.k : p.n);
+    return (((int64_t)(uintptr_t)p.a | (int64_t)(uintptr_t)p.b | (p.lda | p.ldb | p.b_expert | ends) * s) & (width - 1)) == 0;
+  };
+  const bool near = reach * std::max(p.lda, p.ldb) * s < (int64_t)kInBuffer;
+  if (near && whole(16)) return launch_product<T, MODE, 16>(p, ws, ws_bytes, stream);
+  if (near && whole(4)) return launch_product<T, MODE, 4>(p, ws, ws_bytes, stream);
+  return launch_product<T, MODE, 0>(p, ws, ws_bytes, stream);
 }
 
 template <int MODE>

@@ -99,13 +99,15 @@ def test_routed(dtype, op, n_tokens, slots, n_experts):
         _check(dtype, op, counts.tolist(), inner, outer, seed=outer)
 
 
-# enough and large enough tiles for the largest ones, of rows and of the matrices' gradient; the last two leave
-# a last round that is split
+# enough and large enough tiles for the largest ones, of rows and of the matrices' gradient; two leave a last
+# round that is split, two have rows of whole words but not of whole 16 bytes
 @pytest.mark.parametrize("counts,inner,outer", [((700, 1, 513, 900), 264, 5512), ((256, 0, 1024), 40, 12808),
                                                 ((300, 0, 5, 260), 2056, 2080),
                                                 ((1024, 1000, 300, 700), 1032, 5512),
-                                                ((900, 1400, 0, 1900), 2056, 2080)],
-                         ids=["rows", "short", "matrices", "rows_split", "matrices_split"])
+                                                ((900, 1400, 0, 1900), 2056, 2080),
+                                                ((700, 1, 513, 900), 266, 5510), ((300, 0, 5, 260), 2054, 2090)],
+                         ids=["rows", "short", "matrices", "rows_split", "matrices_split", "rows_words",
+                              "matrices_words"])
 @pytest.mark.parametrize("op", ["non", "trans"])
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_many_tiles(dtype, op, counts, inner, outer):
@@ -157,6 +159,21 @@ def test_strides_views_and_out():
     store = torch.empty(3 * 96 * 64 + 1, dtype=torch.bfloat16, device=DEV)
     off = store[1:].view(3, 96, 64).copy_(matrices)
     assert_sum(fs.flagsparse_expert_product(rows, off, route), want, mag, 96)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_rows_far_apart(dtype):
+    # a tile's rows further apart than the offsets of the loads that go straight to LDS
+    route = _route((200, 100))
+    store = torch.zeros((300, (1 << 22) // torch.empty(0, dtype=dtype).element_size() + 8), dtype=dtype, device=DEV)
+    rows, matrices = store[:, :40], randn((2, 40, 24), dtype, 2)
+    rows.copy_(randn((300, 40), dtype, 1))
+    want, mag = _oracle(rows, matrices, route, "non")
+    assert_sum(fs.flagsparse_expert_product(rows, matrices, route), want, mag, 40)
+    grad = randn((300, 24), dtype, 3)
+    _, got = fs.flagsparse_expert_product_grad(grad, rows, matrices, route)
+    want, mag = _oracle_matrices(grad, rows, matrices, route, "non")
+    assert_sum(got, want, mag, 200)
 
 
 def test_empty_sizes():
