@@ -257,6 +257,7 @@ struct ProductArgs {
   int64_t m, n, k;         // m: of a matrix gradient; k: of a product of rows
   int n_experts;
   int cus;                 // compute units
+  bool turn;               // whether tiles may begin at different steps
   float* parts;            // room for the sums of split tiles, or null
 };
 
@@ -507,6 +508,14 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
     constexpr int kLoadsA = da.kLoads, kLoads = da.kLoads + db.kLoads;
     da.init(sa, tid);
     db.init(sb, tid);
+    // With (N, K) matrices of few rows an expert, whose rows are read side by side
+    // 64 bytes at a time, tiles begin at different steps: beginning together they
+    // asked the same few memory channels where rows are 4 KB or 8 KB apart (64 and
+    // 128 rows for each of 32 experts, 2048 x 4096 bf16: 120 and 149 us, 109 and
+    // 124 so; from 512 rows on, where tiles share rows, 0.96 to 1.02 of the rate).
+    int64_t turn = 0;
+    if (MODE == kRowsTrans && p.turn && sa.k % BK == 0 && steps > first)
+      turn = (int64_t)(share.tile * 5u) % (steps - first);
     u32x4 rsrc_a, rsrc_b;
     uint32_t next;
     auto begin_loads = [&](int64_t kt) {
@@ -515,8 +524,9 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
         da.cut(left, tid);
         db.cut(left, tid);
       }
-      rsrc_a = da.at(kt);
-      rsrc_b = db.at(kt);
+      const int64_t at = kt >= steps ? kt : kt + turn < steps ? kt + turn : kt + turn - (steps - first);
+      rsrc_a = da.at(at);
+      rsrc_b = db.at(at);
       next = lds + (uint32_t)(kt & 3) * kSlot;
     };
     auto load = [&](int i) {
@@ -805,35 +815,38 @@ int launch_few(ProductArgs p, hipStream_t stream) {
 // (kFill).  us, bf16, 32 experts 2048 x 4096, rows an expert on average; tiles
 // few / 64 x 128 / 128 x 128 / 256 x 256:
 //   matrices (K, N)      4: 107  96  92  90     32: 154 106 105  95   128: 422 188 165 115
-//   (N, K), "trans"      4: 100 107 112 132     32: 164 114 119 138   128: 414 181 160 154
+//   (N, K), "trans"      8:  99  96             32:  -  104 106 103   128:  -   -  149 124
 //   matrix gradient                              32:  -  213 203 190   512:  -  516 457 395
 //   float32, (K, N)      8: 188 263 485 995     32: 302 276 486 993  1024:  - 2258 2093 2519 (16 experts)
 //   no whole words       8: 141 148 188         32: 229 151 203       128: 595 317 277
-// Large tiles read whole lines of (K, N) matrices, which is why they serve few
-// rows too; of (N, K) ones they read 64 bytes of a row at a time.  One token
-// (8 experts of 64, 4096 columns): few 28, 64 x 128 23, 256 x 256 42; (1 of 8,
-// 4096 x 4096): 12, 28, 72.
+//   whole words, (N, K)  8: 116 130
+// 1.5 rounds of large tiles lose to smaller ones (64 experts of 1536 columns, 8
+// rows: 87, 64 x 128 73).  One token (8 experts of 64, 4096 columns): few 23, 64
+// x 128 23, 256 x 256 42; (1 of 8, 4096 x 4096): 12, 28, 72; 16 tokens, 2 of 8,
+// 1024 x 1024: 9, 12.
 constexpr int64_t kFill = 256;
 
 enum Tiles { kFew, kTiles64, kTiles128, kTiles256 };
 template <int MODE>
-Tiles choose_tiles(const ProductArgs& p, bool half, bool dma) {
+Tiles choose_tiles(const ProductArgs& p, bool half, int width) {
   if constexpr (MODE == kMatrix) {
-    if (half && dma && tiles_of<MODE, kLarge, kLarge>(p) >= kFill) return kTiles256;
+    if (half && width != 0 && tiles_of<MODE, kLarge, kLarge>(p) >= kFill) return kTiles256;
     return tiles_of<MODE, 128, 128>(p) >= kFill ? kTiles128 : kTiles64;
   }
   const int64_t rows = p.n_rows / p.n_experts, active = std::min<int64_t>(p.n_rows, p.n_experts);
   const int64_t tiles256 = ceil_div(p.n, kLarge) * std::max(active, p.n_rows / kLarge);
   const int64_t tiles128 = ceil_div(p.n, 128) * std::max(active, p.n_rows / 128);
-  if (half && dma && (rows >= 112 ? tiles256 >= kFill : MODE == kRowsNon && rows >= 4 && tiles256 >= 2 * kFill))
+  const int64_t tiles64 = ceil_div(p.n, 128) * std::max(active, p.n_rows / 64);
+  if (half && width != 0 &&
+      (rows >= 112 ? tiles256 >= kFill : rows >= (MODE == kRowsNon ? 4 : 40) && tiles256 >= 2 * kFill))
     return kTiles256;
-  if (rows < (half ? 12 : 20)) return kFew;
+  if (rows < (!half ? 20 : width == 16 && tiles64 >= kFill ? 4 : 12)) return kFew;
   return rows >= (half ? 40 : 768) && tiles128 >= kFill ? kTiles128 : kTiles64;
 }
 
 template <class T, int MODE, int WIDTH>
 int launch_product(ProductArgs p, void* ws, size_t ws_bytes, hipStream_t stream) {
-  switch (choose_tiles<MODE>(p, sizeof(T) == 2, WIDTH != 0)) {
+  switch (choose_tiles<MODE>(p, sizeof(T) == 2, WIDTH)) {
     case kFew:
       if constexpr (MODE != kMatrix) return launch_few<T, MODE, WIDTH>(p, stream);
       break;
@@ -906,6 +919,7 @@ ProductArgs product_sizes(int trans, int64_t n_rows, int64_t n_experts, int64_t 
   p.n = matrix && trans ? inner : outer;
   p.k = inner;
   p.cus = compute_units();
+  p.turn = n_rows / n_experts <= 256;
   return p;
 }
 
@@ -919,7 +933,7 @@ extern "C" size_t fs_expert_product_workspace_bytes(int val_t, int trans, int64_
       n_rows == 0 || outer == 0)
     return 0;
   const ProductArgs p = product_sizes(trans, n_rows, n_experts, inner, outer, false);
-  const Tiles t = trans ? choose_tiles<kRowsTrans>(p, true, true) : choose_tiles<kRowsNon>(p, true, true);
+  const Tiles t = trans ? choose_tiles<kRowsTrans>(p, true, 16) : choose_tiles<kRowsNon>(p, true, 16);
   return t == kTiles256 && may_split<kRowsNon>(p) ? parts_bytes(p) : 0;
 }
 
@@ -951,7 +965,7 @@ extern "C" size_t fs_expert_product_grad_matrices_workspace_bytes(int val_t, int
       inner == 0 || outer == 0)
     return 0;
   const ProductArgs p = product_sizes(trans, n_rows, n_experts, inner, outer, true);
-  return choose_tiles<kMatrix>(p, true, true) == kTiles256 && may_split<kMatrix>(p) ? parts_bytes(p) : 0;
+  return choose_tiles<kMatrix>(p, true, 16) == kTiles256 && may_split<kMatrix>(p) ? parts_bytes(p) : 0;
 }
 
 extern "C" int fs_expert_product_grad_matrices(int val_t, int trans, int64_t n_rows, int64_t n_experts, int64_t inner,
