@@ -820,6 +820,10 @@ int launch_few(ProductArgs p, hipStream_t stream) {
 //   float32, (K, N)      8: 188 263 485 995     32: 302 276 486 993  1024:  - 2258 2093 2519 (16 experts)
 //   no whole words       8: 141 148 188         32: 229 151 203       128: 595 317 277
 //   whole words, (N, K)  8: 116 130
+// Large tiles too few to fill the chip, split along k (2048 rows of 4 experts
+// 4096 x 4096: 88, 128 x 128 118; 1024 x 2 of 8, 2048 x 2048: 50, 45), and of a
+// matrix gradient (16384 rows of 8, 1024 x 1024: 56, 42; of 4 x 8192 rows, 1024 x
+// 2048: 132, 146).
 // 1.5 rounds of large tiles lose to smaller ones (64 experts of 1536 columns, 8
 // rows: 87, 64 x 128 73).  One token (8 experts of 64, 4096 columns): few 23, 64
 // x 128 23, 256 x 256 42; (1 of 8, 4096 x 4096): 12, 28, 72; 16 tokens, 2 of 8,
@@ -829,8 +833,10 @@ constexpr int64_t kFill = 256;
 enum Tiles { kFew, kTiles64, kTiles128, kTiles256 };
 template <int MODE>
 Tiles choose_tiles(const ProductArgs& p, bool half, int width) {
+  // large tiles that do not fill the chip pay if their steps can be split
   if constexpr (MODE == kMatrix) {
-    if (half && width != 0 && tiles_of<MODE, kLarge, kLarge>(p) >= kFill) return kTiles256;
+    const int64_t tiles256 = tiles_of<MODE, kLarge, kLarge>(p);
+    if (half && width != 0 && (tiles256 >= 160 || (tiles256 >= 96 && p.n_rows / p.n_experts >= 6144))) return kTiles256;
     return tiles_of<MODE, 128, 128>(p) >= kFill ? kTiles128 : kTiles64;
   }
   const int64_t rows = p.n_rows / p.n_experts, active = std::min<int64_t>(p.n_rows, p.n_experts);
@@ -838,7 +844,8 @@ Tiles choose_tiles(const ProductArgs& p, bool half, int width) {
   const int64_t tiles128 = ceil_div(p.n, 128) * std::max(active, p.n_rows / 128);
   const int64_t tiles64 = ceil_div(p.n, 128) * std::max(active, p.n_rows / 64);
   if (half && width != 0 &&
-      (rows >= 112 ? tiles256 >= kFill : rows >= (MODE == kRowsNon ? 4 : 40) && tiles256 >= 2 * kFill))
+      (rows >= 112 ? tiles256 >= 160 || (p.k >= 1536 && tiles256 * p.k >= 192 * 1024)
+                   : rows >= (MODE == kRowsNon ? 4 : 40) && tiles256 >= 2 * kFill))
     return kTiles256;
   if (rows < (!half ? 20 : width == 16 && tiles64 >= kFill ? 4 : 12)) return kFew;
   return rows >= (half ? 40 : 768) && tiles128 >= kFill ? kTiles128 : kTiles64;
