@@ -18,6 +18,7 @@
 // How many rows an expert has is known on the device only: the grid is an upper
 // bound, each workgroup finds its tile from the offsets, and those beyond the
 // last tile leave.
+#include <initializer_list>
 #include <type_traits>
 
 #include "select_rows.hpp"
@@ -287,11 +288,15 @@ struct TilePlan {
 };
 
 // Tiles of a last round that leaves most of the chip idle are cut along k into
-// the parts that take the least time: a tile takes about 0.8 us a step, writing
-// and adding a tile's sums 0.085 us a part and tile, so parts^2 = 9 steps / rest.
-__host__ __device__ inline uint32_t parts_of(uint32_t rest, int64_t steps, uint32_t cus) {
+// the parts that take the least time: a large tile takes about 0.8 us a step,
+// writing and adding a tile's sums 0.085 us a part and tile, so parts^2 = 9 steps
+// / rest (smaller tiles: both in proportion).  `places`: tiles at a time.
+constexpr int kLarge = 256;
+constexpr uint32_t kMostParts = 32;
+__host__ __device__ inline uint32_t places_of(int cus, int bm) { return (uint32_t)cus * (bm == kLarge ? 1 : 2); }
+__host__ __device__ inline uint32_t parts_of(uint32_t rest, int64_t steps, uint32_t places) {
   uint32_t parts = 1;
-  while (rest > 0 && parts < 16 && (parts + 1) * rest <= cus &&
+  while (rest > 0 && parts < kMostParts && (parts + 1) * rest <= places &&
          (int64_t)(parts + 1) * (parts + 1) * rest <= 9 * steps)
     ++parts;
   return parts;
@@ -303,7 +308,7 @@ __device__ inline TilePlan plan_tiles(const ProductArgs& p, int lane) {
   const uint32_t nt = (uint32_t)((p.n + BN - 1) / BN);
   TilePlan l;
   int64_t steps;
-  constexpr int kStep = kRowBytes / 2;  // k of a step of 16-bit values: only they are split
+  constexpr int kStep = kRowBytes / 2;  // k of a step of 16-bit values
   if constexpr (MODE == kMatrix) {
     l.real = (uint32_t)((p.m + BM - 1) / BM) * nt * (uint32_t)p.n_experts;
     l.zero = 0;
@@ -323,7 +328,7 @@ __device__ inline TilePlan plan_tiles(const ProductArgs& p, int lane) {
   l.rest = 0;
   l.parts = 1;
   if (p.parts != nullptr) {
-    const uint32_t rest = l.real % (uint32_t)p.cus, parts = parts_of(rest, steps, (uint32_t)p.cus);
+    const uint32_t places = places_of(p.cus, BM), rest = l.real % places, parts = parts_of(rest, steps, places);
     if (parts > 1) {
       l.rest = rest;
       l.parts = parts;
@@ -480,7 +485,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
   Frags<OB, BKC, FN> from_b;
   // 16-row blocks of a wave: half of what the tile has where two groups of waves
   // share it (an expert's last tile may have few rows)
-  const int fm = WM * WN == 8 ? (work.c_rows + 31) / 32 : FM;
+  const int fm = BM == kLarge ? (work.c_rows + 31) / 32 : FM;
   from_a.init(wm * fm * 16, lane);
   from_b.init(wn * (BN / WN), lane);
 
@@ -606,7 +611,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
     }
   }
 
-  if constexpr (WM * WN == 8) {
+  if constexpr (BM == kLarge || MODE == kMatrix) {
     if (share.parts > 1) {  // sums for the join, as the lanes hold them
       f32x4* part = (f32x4*)p.parts + (int64_t)share.slot * (BM * BN / 4) + w * (FM * FN * 64) + lane;
 #pragma unroll
@@ -639,7 +644,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_join_kernel(const
     const uint32_t r = b / FM;
     const int i = (int)(b % FM);
     const TileWork<T> work = tile_work<T, MODE, BM, BN>(p, lane, plan.full + r);
-    const int fm = (work.c_rows + 31) / 32, m = ((w / WN) * fm + i) * 16 + (lane & 15);
+    const int fm = BM == kLarge ? (work.c_rows + 31) / 32 : FM, m = ((w / WN) * fm + i) * 16 + (lane & 15);
     if (i >= fm || m >= work.c_rows) continue;
     const f32x4* part = (const f32x4*)p.parts + (int64_t)r * plan.parts * (BM * BN / 4) + w * (FM * FN * 64) +
                         i * FN * 64 + lane;
@@ -763,37 +768,43 @@ int64_t tiles_of(const ProductArgs& p) {
 }
 
 // Whether tiles of a last round may be split: of a matrix gradient it is known
-// here; of a product of rows, whose tiles are counted on the device, if tiles
-// take long beside the join that is then launched in any case, and rounds are
-// few.  us with and without: 4096 x 2 rows, 8 experts 4096 x 4096 bf16 272 and
-// 312, 8192 x 2 of 2048 x 2048 149 and 162, 4093 x 4 of 5120 x 2048 346 and 383.
-constexpr int kLarge = 256;
-template <int MODE>
+// here; of a product of rows, whose tiles are counted on the device, large ones
+// if they take long beside the join that is then launched in any case, and rounds
+// are few.  us with and without: 4096 x 2 rows, 8 experts 4096 x 4096 bf16 272
+// and 312, 8192 x 2 of 2048 x 2048 149 and 162, 4093 x 4 of 5120 x 2048 346 and
+// 383; matrix gradients of 4 experts of 32768 rows, 256 x 320 89 and 226, of
+// 1024 rows 14 and 12: from 2048 rows on.
+template <int MODE, int BM, int BN>
 bool may_split(const ProductArgs& p) {
-  const int64_t tiles = ceil_div(p.n, kLarge);
+  const int64_t nt = ceil_div(p.n, BN), rows = p.n_rows / p.n_experts;
   if (MODE == kMatrix) {
-    const int64_t real = ceil_div(p.m, kLarge) * tiles * p.n_experts;
-    return real <= UINT32_MAX &&
-           parts_of((uint32_t)real % (uint32_t)p.cus, p.n_rows / p.n_experts / 32, (uint32_t)p.cus) > 1;
+    const int64_t real = ceil_div(p.m, BM) * nt * p.n_experts;
+    const uint32_t places = places_of(p.cus, BM);
+    return real <= INT32_MAX && (BM == kLarge || rows >= 2048) && parts_of((uint32_t)real % places, rows / 32, places) > 1;
   }
-  return p.n_rows / p.n_experts >= 112 && p.k >= 1536 && p.n_rows / kLarge * tiles < 8 * p.cus;
+  return BM == kLarge && rows >= 112 && p.k >= 1536 && p.n_rows / kLarge * nt < 8 * p.cus;
 }
-// The most sums that split tiles leave: one a compute unit.
-size_t parts_bytes(const ProductArgs& p) { return (size_t)p.cus * kLarge * kLarge * sizeof(float); }
+// The sums that split tiles leave: at most one a place.
+template <int MODE, int BM, int BN>
+size_t parts_bytes(const ProductArgs& p) {
+  return may_split<MODE, BM, BN>(p) ? (size_t)places_of(p.cus, BM) * BM * BN * sizeof(float) : 0;
+}
 
 template <class T, int MODE, int WIDTH, int BM, int BN, int WM, int WN>
-int launch_tiles(ProductArgs p, hipStream_t stream) {
-  constexpr bool kSplit = WM * WN == 8;
-  if (!kSplit) p.parts = nullptr;
-  const int64_t tiles = tiles_of<MODE, BM, BN>(p) + (p.parts != nullptr ? p.cus : 0);
+int launch_tiles(ProductArgs p, void* ws, size_t ws_bytes, hipStream_t stream) {
+  const size_t need = parts_bytes<MODE, BM, BN>(p);
+  if (need > 0 && (ws == nullptr || ws_bytes < need))
+    return fail(FS_E_WORKSPACE, "fs_expert_product: workspace too small");
+  p.parts = need > 0 ? static_cast<float*>(ws) : nullptr;
+  const int64_t tiles = tiles_of<MODE, BM, BN>(p) + (need > 0 ? places_of(p.cus, BM) : 0);
   if (tiles * 64 * WM * WN > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
   hipLaunchKernelGGL((expert_product_kernel<T, MODE, WIDTH, BM, BN, WM, WN>), dim3((uint32_t)tiles),
                      dim3(64 * WM * WN), 0, stream, p);
   FS_CHECK_MAIN_LAUNCH("expert_product_kernel");
-  if constexpr (kSplit) {
-    if (p.parts != nullptr) {
-      hipLaunchKernelGGL((expert_product_join_kernel<T, MODE, BM, BN, WM, WN>),
-                         dim3((uint32_t)p.cus), dim3(64 * WM * WN), 0, stream, p);
+  if constexpr (BM == kLarge || MODE == kMatrix) {
+    if (need > 0) {
+      hipLaunchKernelGGL((expert_product_join_kernel<T, MODE, BM, BN, WM, WN>), dim3((uint32_t)p.cus),
+                         dim3(64 * WM * WN), 0, stream, p);
       FS_CHECK_LAUNCH("expert_product_join_kernel");
     }
   }
@@ -852,24 +863,35 @@ Tiles choose_tiles(const ProductArgs& p, bool half, int width) {
 }
 
 template <class T, int MODE, int WIDTH>
-int launch_product(ProductArgs p, void* ws, size_t ws_bytes, hipStream_t stream) {
+int launch_product(const ProductArgs& p, void* ws, size_t ws_bytes, hipStream_t stream) {
   switch (choose_tiles<MODE>(p, sizeof(T) == 2, WIDTH)) {
     case kFew:
       if constexpr (MODE != kMatrix) return launch_few<T, MODE, WIDTH>(p, stream);
       break;
-    case kTiles64: return launch_tiles<T, MODE, WIDTH, 64, 128, 2, 2>(p, stream);
-    case kTiles128: return launch_tiles<T, MODE, WIDTH, 128, 128, 2, 2>(p, stream);
+    case kTiles64: return launch_tiles<T, MODE, WIDTH, 64, 128, 2, 2>(p, ws, ws_bytes, stream);
+    case kTiles128: return launch_tiles<T, MODE, WIDTH, 128, 128, 2, 2>(p, ws, ws_bytes, stream);
     case kTiles256:
-      if constexpr (sizeof(T) == 2 && WIDTH != 0) {
-        if (may_split<MODE>(p)) {
-          if (ws == nullptr || ws_bytes < parts_bytes(p))
-            return fail(FS_E_WORKSPACE, "fs_expert_product: workspace too small");
-          p.parts = static_cast<float*>(ws);
-        }
-        return launch_tiles<T, MODE, WIDTH, kLarge, kLarge, 2, 4>(p, stream);
-      }
+      if constexpr (sizeof(T) == 2 && WIDTH != 0)
+        return launch_tiles<T, MODE, WIDTH, kLarge, kLarge, 2, 4>(p, ws, ws_bytes, stream);
   }
   return fail(FS_E_INVALID, "fs_expert_product: no tiles");
+}
+
+// Workspace for any alignment of the operands.
+template <int MODE>
+size_t product_workspace(const ProductArgs& p, bool half) {
+  size_t most = 0;
+  for (int width : {16, 4, 0}) {
+    size_t need = 0;
+    switch (choose_tiles<MODE>(p, half, width)) {
+      case kFew: break;
+      case kTiles64: need = parts_bytes<MODE, 64, 128>(p); break;
+      case kTiles128: need = parts_bytes<MODE, 128, 128>(p); break;
+      case kTiles256: need = parts_bytes<MODE, kLarge, kLarge>(p);
+    }
+    most = std::max(most, need);
+  }
+  return most;
 }
 
 template <class T, int MODE>
@@ -936,12 +958,10 @@ ProductArgs product_sizes(int trans, int64_t n_rows, int64_t n_experts, int64_t 
 extern "C" size_t fs_expert_product_workspace_bytes(int val_t, int trans, int64_t n_rows, int64_t n_experts,
                                                     int64_t inner, int64_t outer) {
   using namespace fs;
-  if ((val_t != FS_F16 && val_t != FS_BF16) || check_product("", n_rows, n_experts, inner, outer, trans) != FS_OK ||
-      n_rows == 0 || outer == 0)
-    return 0;
+  if (check_product("", n_rows, n_experts, inner, outer, trans) != FS_OK || n_rows == 0 || outer == 0) return 0;
   const ProductArgs p = product_sizes(trans, n_rows, n_experts, inner, outer, false);
-  const Tiles t = trans ? choose_tiles<kRowsTrans>(p, true, 16) : choose_tiles<kRowsNon>(p, true, 16);
-  return t == kTiles256 && may_split<kRowsNon>(p) ? parts_bytes(p) : 0;
+  const bool half = val_t == FS_F16 || val_t == FS_BF16;
+  return trans ? product_workspace<kRowsTrans>(p, half) : product_workspace<kRowsNon>(p, half);
 }
 
 extern "C" int fs_expert_product(int val_t, int trans, int64_t n_rows, int64_t n_experts, int64_t inner, int64_t outer,
@@ -968,11 +988,9 @@ extern "C" int fs_expert_product(int val_t, int trans, int64_t n_rows, int64_t n
 extern "C" size_t fs_expert_product_grad_matrices_workspace_bytes(int val_t, int trans, int64_t n_rows,
                                                                   int64_t n_experts, int64_t inner, int64_t outer) {
   using namespace fs;
-  if ((val_t != FS_F16 && val_t != FS_BF16) || check_product("", n_rows, n_experts, inner, outer, trans) != FS_OK ||
-      inner == 0 || outer == 0)
-    return 0;
+  if (check_product("", n_rows, n_experts, inner, outer, trans) != FS_OK || inner == 0 || outer == 0) return 0;
   const ProductArgs p = product_sizes(trans, n_rows, n_experts, inner, outer, true);
-  return choose_tiles<kMatrix>(p, true, 16) == kTiles256 && may_split<kMatrix>(p) ? parts_bytes(p) : 0;
+  return product_workspace<kMatrix>(p, val_t == FS_F16 || val_t == FS_BF16);
 }
 
 extern "C" int fs_expert_product_grad_matrices(int val_t, int trans, int64_t n_rows, int64_t n_experts, int64_t inner,

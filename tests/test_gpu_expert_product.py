@@ -114,6 +114,15 @@ def test_many_tiles(dtype, op, counts, inner, outer):
     _check(dtype, op, counts, inner, outer, dropped=70)
 
 
+# many rows and small matrices: tiles of every size split along the rows
+@pytest.mark.parametrize("counts,inner,outer", [((5000, 0, 3300), 40, 24), ((2100, 2500, 1800), 136, 300),
+                                                ((4099, 3999), 65, 127), ((7000, 9000), 258, 202)], ids=str)
+@pytest.mark.parametrize("op", ["non", "trans"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_many_rows_small_matrices(dtype, op, counts, inner, outer):
+    _check(dtype, op, counts, inner, outer, dropped=9)
+
+
 @pytest.mark.parametrize("op", ["non", "trans"])
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_neighbours_do_not_leak(dtype, op):
