@@ -334,12 +334,14 @@ Passes passes_of(int64_t n_keys) {
   return {count, (bits + count - 1) / count};
 }
 
-// Positions a tile: 512, 1024, 2048 or 4096, the fewest that make at most 64
-// tiles (more tiles are more rows for the scan, fewer leave compute units idle).
+// Positions a tile: 512, 1024 or 2048, the fewest that make at most 64 tiles, or
+// 4096 from 256 tiles on (more tiles are more counts to scan, fewer leave compute
+// units idle).  us for slots of 64 experts, tiles of 2048 and 4096: 262144 10.5 and
+// 13.0, 524288 12.3 and 14.1; of 128, 2097152 25.5 and 22.0.
 int chunks_of(int64_t n) {
   int ch = 1;
-  while (ch < 8 && n > (int64_t)kThreads * ch * 64) ch *= 2;
-  return ch;
+  while (ch < 4 && n > (int64_t)kThreads * ch * 64) ch *= 2;
+  return n > (int64_t)kThreads * ch * 256 ? 2 * ch : ch;
 }
 
 struct SortLayout {
