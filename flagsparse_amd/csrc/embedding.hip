@@ -5,7 +5,8 @@
 // transposed product, grad_table[v] = scale * sum over the t with ids[t] = v of
 // grad[t]: positions sorted by token (select_sort.hip, stable), then one sum a
 // table row over its segment, in position order, so results do not change from
-// run to run.  Rows without tokens are written as zeros in the same pass.
+// run to run.  Rows without tokens are written as zeros in the same pass, of few
+// tokens beside their sort.
 //
 // A row of up to 64 tokens is summed at once.  A longer segment (tokens
 // follow a Zipf law: the first ones occur thousands of times in a batch) is cut
@@ -143,12 +144,14 @@ __device__ inline void sum_rows(const V* __restrict__ grad, int64_t ldg, int pos
 // block_rows rows one after the other.  Bound by the bytes where the table is
 // large: 65536 tokens of a Zipf law, 131072 rows of 2048 bf16, 806 MB, 174 us of
 // the call's 209 (4.6 TB/s; sort 22, join 11); 4095 tokens, 20011 rows of 1001
-// float32, 97 MB, 20 us of 38 (sort 13, join 4).
-template <class V, class O, bool PAST>
+// float32, 97 MB, 33 us in all (the sort and its zeros, the rows with tokens, join 4).
+// FILLED: rows below `filled` hold zeros already.
+template <class V, class O, bool PAST, bool FILLED>
 __global__ __launch_bounds__(256) void embedding_grad_kernel(
     const V* __restrict__ grad, int64_t ldg, const uint32_t* __restrict__ keys, const int32_t* __restrict__ order,
     int64_t n, int64_t n_rows, int64_t width, typename Elem<V>::acc scale, int64_t padding, int wpr, int block_rows,
-    int64_t chunk_blocks, int64_t n_chunks, O* __restrict__ out, typename Elem<V>::acc* __restrict__ parts) {
+    int64_t chunk_blocks, int64_t n_chunks, int64_t filled, O* __restrict__ out,
+    typename Elem<V>::acc* __restrict__ parts) {
   using A = typename Elem<V>::acc;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t first = (int64_t)(w % wpr) * 64, stride = (int64_t)wpr * 64;
@@ -197,6 +200,7 @@ __global__ __launch_bounds__(256) void embedding_grad_kernel(
       window();
     }
     uint64_t m = __ballot(kk == v);
+    if (FILLED && m == 0 && (int64_t)v < filled) continue;
     if (m >> 63) {  // the window may cut the segment: begin it there
       wb += __builtin_ctzll(m);
       window();
@@ -342,8 +346,12 @@ extern "C" int fs_embedding_grad(int val_t, int out_t, int id_t, int64_t n, int6
   uint8_t* w = static_cast<uint8_t*>(ws);
   uint32_t* keys = n > 0 ? reinterpret_cast<uint32_t*>(w + l.keys) : nullptr;
   int32_t* order = n > 0 ? reinterpret_cast<int32_t*>(w + l.order) : nullptr;
+  if (const int rc = with_value_type(val_t, "fs_embedding_grad", [](auto) -> int { return FS_OK; })) return rc;
+  int64_t filled = 0;  // rows that the sort's launches write zeros to
   if (n > 0) {
-    const int rc = select_sort(ids, id_t, n, n_rows, keys, order, nullptr, nullptr, w, stream);
+    const int64_t row_bytes = width * (out_t == FS_F64 ? 8 : out_t == FS_F32 ? 4 : 2);
+    filled = std::min(n_rows, select_sort_fill_bytes(n) / row_bytes);
+    const int rc = select_sort(ids, id_t, n, n_rows, keys, order, nullptr, nullptr, w, stream, out, filled * row_bytes);
     if (rc != FS_OK) return rc;
   }
   return with_value_type(val_t, "fs_embedding_grad", [&](auto v) -> int {
@@ -359,14 +367,14 @@ extern "C" int fs_embedding_grad(int val_t, int out_t, int id_t, int64_t n, int6
       const int block_rows = (int)std::min<int64_t>(16, std::max<int64_t>(2, n_rows / (2048 * (4 / wpr))));
       const int64_t chunk_blocks = ceil_div(chunks, 4 / wpr);
       const dim3 grid = row_grid(chunk_blocks + ceil_div(n_rows, (4 / wpr) * block_rows));
-      auto launch = [&](auto past) {
-        hipLaunchKernelGGL((embedding_grad_kernel<V, O, decltype(past)::value>), grid, dim3(256), 0, stream,
+      auto launch = [&](auto past, auto some) {
+        hipLaunchKernelGGL((embedding_grad_kernel<V, O, decltype(past)::value, decltype(some)::value>), grid, dim3(256), 0, stream,
                            (const V*)grad, ldg, keys, order, n, n_rows, width, (A)scale, padding, wpr, block_rows,
-                           chunk_blocks, chunks, (O*)out, parts);
+                           chunk_blocks, chunks, filled, (O*)out, parts);
       };
       if (store_past_caches((n * (int64_t)sizeof(V) + n_rows * (int64_t)sizeof(O)) * width, width * sizeof(O)))
-        launch(std::true_type{});
-      else launch(std::false_type{});
+        filled > 0 ? launch(std::true_type{}, std::true_type{}) : launch(std::true_type{}, std::false_type{});
+      else filled > 0 ? launch(std::false_type{}, std::true_type{}) : launch(std::false_type{}, std::false_type{});
       FS_CHECK_MAIN_LAUNCH("embedding_grad_kernel");
       if (chunks > 0) {
         const dim3 x = row_grid(chunks);

@@ -127,7 +127,8 @@ int with_value_type(int val_t, const char* who, F&& f) {
 
 // select_sort.hip
 size_t select_sort_bytes(int64_t n, int64_t n_keys);
+int64_t select_sort_fill_bytes(int64_t n);
 int select_sort(const void* ids, int id_t, int64_t n, int64_t n_keys, uint32_t* keys_out, int32_t* order,
-                int32_t* inverse, int32_t* offsets, uint8_t* ws, hipStream_t s);
+                int32_t* inverse, int32_t* offsets, uint8_t* ws, hipStream_t s, void* zeros, int64_t zero_bytes);
 
 }  // namespace fs

@@ -227,12 +227,26 @@ __global__ __launch_bounds__(kThreads) void select_scatter_kernel(
 }
 
 // All of the sort by one workgroup of W waves, 64 CH positions each, W = 1..16.
+// The others write zeros meanwhile, for the embedding gradient: as many bytes as
+// the sort hides (table gradients, us without and with: 4096 tokens of 32000 x 4096
+// bf16 78 and 61, 4095 of 20011 x 1001 f32 39 and 34, with twice the bytes 75 and 34;
+// 1 of 32000 x 1024 bf16 23 and 18, 512 of 50000 x 1024 f32 39 and 40).
 constexpr int kSmallWaves = 16, kSmallChunks = 4;
 constexpr int64_t kSmall = 64 * kSmallWaves * kSmallChunks;
+constexpr uint32_t kFillGroups = 512;
+template <bool PAST>
+__device__ inline void fill_zeros(uint8_t* __restrict__ p, int64_t bytes) {
+  const int64_t i = (int64_t)(blockIdx.x - 1) * blockDim.x + threadIdx.x, step = (int64_t)kFillGroups * blockDim.x;
+  const Slice<uint16_t> zero{};
+  for (int64_t q = i; q < bytes / 16; q += step) store_slice<PAST>(reinterpret_cast<uint16_t*>(p + q * 16), zero);
+  if (i < bytes % 16) p[bytes / 16 * 16 + i] = 0;
+}
 template <class Id, int CH>
 __global__ __launch_bounds__(64 * kSmallWaves) void select_small_kernel(
     const Id* __restrict__ ids, int n, uint32_t n_keys, int bits, int passes, uint32_t* __restrict__ keys_out,
-    int32_t* __restrict__ order, int32_t* __restrict__ inverse, int32_t* __restrict__ offsets) {
+    int32_t* __restrict__ order, int32_t* __restrict__ inverse, int32_t* __restrict__ offsets,
+    uint8_t* __restrict__ zeros, int64_t zero_bytes) {
+  if (blockIdx.x > 0) return fill_zeros<(CH > 1)>(zeros, zero_bytes);
   __shared__ uint16_t s_cnt[kSmallWaves][kMaxDigits];
   __shared__ uint32_t s_base[kMaxDigits];
   __shared__ uint32_t s_wave[kSmallWaves];
@@ -420,9 +434,17 @@ __global__ __launch_bounds__(256) void zero_offsets_kernel(int32_t* __restrict__
 
 size_t select_sort_bytes(int64_t n, int64_t n_keys) { return n > 0 ? sort_layout(n, n_keys).bytes : 0; }
 
-// keys_out, inverse and offsets may be null; offsets needs one pass.
+// The zeros that a sort can write beside its own work.  (Beside the launches of a
+// sort of many positions they cost more than they save: each launch's end waits for
+// them; 65536 tokens of 131072 x 2048 with 64 MB of them 208 us, without 164.)
+int64_t select_sort_fill_bytes(int64_t n) {
+  return n == 0 || n > kSmall ? 0 : (int64_t)(n > 64 * kSmallWaves ? 96 : 64) << 20;
+}
+
+// keys_out, inverse and offsets may be null; offsets needs one pass.  Also writes
+// zero_bytes zeros, at most select_sort_fill_bytes(n).
 int select_sort(const void* ids, int id_t, int64_t n, int64_t n_keys, uint32_t* keys_out, int32_t* order,
-                int32_t* inverse, int32_t* offsets, uint8_t* ws, hipStream_t s) {
+                int32_t* inverse, int32_t* offsets, uint8_t* ws, hipStream_t s, void* zeros, int64_t zero_bytes) {
   if (n == 0) {
     if (offsets != nullptr) {
       hipLaunchKernelGGL(zero_offsets_kernel, dim3((uint32_t)ceil_div(n_keys + 1, 256)), dim3(256), 0, s, offsets,
@@ -436,8 +458,9 @@ int select_sort(const void* ids, int id_t, int64_t n, int64_t n_keys, uint32_t* 
     auto launch = [&](auto id, auto chunks) {
       using Id = decltype(id);
       constexpr int CH = decltype(chunks)::value;
-      hipLaunchKernelGGL((select_small_kernel<Id, CH>), dim3(1), dim3((uint32_t)(ceil_div(n, 64 * CH) * 64)), 0, s,
-                         (const Id*)ids, (int)n, (uint32_t)n_keys, p.bits, p.count, keys_out, order, inverse, offsets);
+      hipLaunchKernelGGL((select_small_kernel<Id, CH>), dim3(zero_bytes > 0 ? 1 + kFillGroups : 1),
+                         dim3((uint32_t)(ceil_div(n, 64 * CH) * 64)), 0, s, (const Id*)ids, (int)n, (uint32_t)n_keys,
+                         p.bits, p.count, keys_out, order, inverse, offsets, static_cast<uint8_t*>(zeros), zero_bytes);
     };
     using One = std::integral_constant<int, 1>;
     using Four = std::integral_constant<int, kSmallChunks>;
@@ -488,5 +511,5 @@ extern "C" int fs_expert_route(int id_t, int64_t n, int64_t n_experts, const voi
   if (need > 0 && (ws == nullptr || ws_bytes < need))
     return fs::fail(FS_E_WORKSPACE, "fs_expert_route: workspace too small");
   return fs::select_sort(experts, id_t, n, n_experts, nullptr, order, inverse, offsets, static_cast<uint8_t*>(ws),
-                         stream);
+                         stream, nullptr, 0);
 }

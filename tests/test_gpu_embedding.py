@@ -147,6 +147,29 @@ def test_gradient_many_tiles_scanned_by_launches():
     assert torch.equal(got.cpu(), want)
 
 
+@pytest.mark.parametrize("n", [5, 300, 1025, 4096])
+@pytest.mark.parametrize("dtype", ROW_DTYPES, ids=ROW_IDS)
+def test_gradient_of_tables_larger_than_what_the_sort_zeroes(dtype, n):
+    """Beside a short sort the first 64 or 96 MB of the table are zeroed; the rows
+    after them are not, and rows have odd sizes and begin at one element."""
+    width = 1003
+    n_rows = (104 << 20) // (width * torch.empty(0, dtype=dtype).element_size())
+    g = torch.Generator().manual_seed(n)
+    tokens = torch.randint(0, n_rows, (n,), generator=g)
+    tokens[0], tokens[1], tokens[2], tokens[3] = 0, n_rows - 1, 7, n_rows - 2  # (7 and n_rows - 2: padding)
+    grad = torch.randint(-3, 4, (n, width), generator=g).to(dtype)  # sums of whole values: exact
+    for padding in (7, n_rows - 2):
+        room = torch.full((1 + n_rows * width,), float("nan"), dtype=dtype, device=DEV)
+        out = room[1:].view(n_rows, width)
+        fs.flagsparse_embedding_grad(grad.to(DEV), tokens.to(DEV), n_rows, padding_idx=padding, out=out)
+        rows, at = torch.unique(tokens, return_inverse=True)
+        want = torch.zeros(len(rows), width, dtype=torch.float64).index_add_(0, at, grad.double())
+        want[rows == padding] = 0
+        assert torch.equal(out[rows.to(DEV)].cpu().double(), want)
+        out[rows.to(DEV)] = 0
+        assert bool((out == 0).all()) and bool(torch.isnan(room[0]))
+
+
 @pytest.mark.parametrize("length", [1, 64, 65, 500])
 def test_gradient_padding_and_outside(length):
     ids = torch.cat([torch.full((length,), 3), torch.arange(8), torch.full((length,), -1), torch.full((length,), 8)])
