@@ -148,35 +148,65 @@ struct Source {
   int64_t k;      // k within it
 };
 
-// A thread's pieces of step kt in registers, zeros outside the operand.
+// The i-th piece of thread tid in step kt of an operand.
+template <class O, class T, bool KC>
+struct Piece {
+  const T* p;
+  int64_t left;  // elements of its row from its first on
+  __device__ Piece(const Source<T>& s, int64_t kt, int tid, int i) {
+    const int row = O::row_of(i, tid), piece = O::piece_of(i, tid);
+    const int64_t k0 = kt * O::BK;
+    const int64_t line = KC ? row : k0 + row;                            // row of memory
+    const int64_t first = KC ? k0 + (int64_t)piece * O::E : piece * O::E;  // element in it
+    p = s.base + line * s.ld + first;
+    left = line < (KC ? (int64_t)s.tile_rows : s.k) ? (KC ? s.k : (int64_t)s.tile_rows) - first : 0;
+  }
+};
+// A thread's pieces of step kt in registers, zeros outside the operand.  A piece
+// that its row ends in is taken element by element at the end of k, once; at the
+// end of the tile's columns, which is met in every step, it is loaded so that it
+// ends with the row, and shifted when it is stored (us, element by element and so:
+// two of 8 experts 4095 x 4095 bf16, (K, N), 39 and 22, matrix gradient of 4096 x
+// 2 rows, 8 of 1001 x 3001 122 and 97; for the end of k, (N, K), 56 and 70).
+template <class O, class T, bool KC>
+__device__ inline bool shifts(const Source<T>& s) {
+  return !KC && s.tile_rows >= O::E;
+}
 template <class O, class T, bool KC>
 __device__ inline void load_pieces(const Source<T>& s, int64_t kt, int tid, u32x4 (&r)[O::kPieces]) {
   constexpr int E = O::E;
+  const bool shift = shifts<O, T, KC>(s);
 #pragma unroll
   for (int i = 0; i < O::kPieces; ++i) {
-    const int row = O::row_of(i, tid), piece = O::piece_of(i, tid);
-    const int64_t k0 = kt * O::BK;
-    const int64_t line = KC ? row : k0 + row;                       // row of memory
-    const int64_t first = KC ? k0 + (int64_t)piece * E : piece * E;  // element in it
-    const bool in = KC ? row < s.tile_rows : k0 + row < s.k;
-    const int64_t left = (KC ? s.k : (int64_t)s.tile_rows) - first;
-    const T* p = s.base + line * s.ld + first;
+    const Piece<O, T, KC> a(s, kt, tid, i);
     u32x4 v = {0u, 0u, 0u, 0u};
-    if (in && left >= E) {
-      __builtin_memcpy(&v, p, 16);
-    } else if (in && left > 0) {
+    if (a.left >= E || (shift && a.left > 0)) {
+      __builtin_memcpy(&v, a.p - (!KC && a.left < E ? E - a.left : 0), 16);
+    } else if (a.left > 0) {
       T e[E];
 #pragma unroll
-      for (int q = 0; q < E; ++q) e[q] = q < left ? p[q] : (T)0;
+      for (int q = 0; q < E; ++q) e[q] = q < a.left ? a.p[q] : (T)0;
       __builtin_memcpy(&v, e, 16);
     }
     r[i] = v;
   }
 }
-template <class O>
-__device__ inline void store_pieces(uint32_t lds, int tid, const u32x4 (&r)[O::kPieces], int threads) {
+template <class O, class T, bool KC>
+__device__ inline void store_pieces(const Source<T>& s, int64_t kt, uint32_t lds, int tid, u32x4 (&r)[O::kPieces],
+                                    int threads) {
+  const bool shift = shifts<O, T, KC>(s);
 #pragma unroll
-  for (int i = 0; i < O::kPieces; ++i) *(lds_u32x4*)(lds_byte*)(uintptr_t)(lds + (uint32_t)(i * threads + tid) * 16) = r[i];
+  for (int i = 0; i < O::kPieces; ++i) {
+    u32x4 v = r[i];
+    const int64_t left = shift ? Piece<O, T, KC>(s, kt, tid, i).left : 0;
+    if (left > 0 && left < O::E) {
+      const unsigned bits = (unsigned)(O::E - left) * 8u * (unsigned)sizeof(T);  // 16 to 112
+      const uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+      const uint64_t x = bits < 64 ? lo >> bits | hi << (64 - bits) : hi >> (bits - 64), y = bits < 64 ? hi >> bits : 0;
+      v = u32x4{(uint32_t)x, (uint32_t)(x >> 32), (uint32_t)y, (uint32_t)(y >> 32)};
+    }
+    *(lds_u32x4*)(lds_byte*)(uintptr_t)(lds + (uint32_t)(i * threads + tid) * 16) = v;
+  }
 }
 
 // The same straight to LDS (buffer loads that write LDS, 64 lanes x WIDTH bytes
@@ -604,8 +634,8 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
     }
     for (int64_t kt = first; kt < steps; ++kt) {
       const uint32_t slot = lds + (uint32_t)(kt & 1) * kSlot;
-      store_pieces<OA>(slot, tid, ra, THREADS);
-      store_pieces<OB>(slot + OA::kBytes, tid, rb, THREADS);
+      store_pieces<OA, T, AKC>(sa, kt, slot, tid, ra, THREADS);
+      store_pieces<OB, T, BKC>(sb, kt, slot + OA::kBytes, tid, rb, THREADS);
       if (kt + 1 < steps) {
         load_pieces<OA, T, AKC>(sa, kt + 1, tid, ra);
         load_pieces<OB, T, BKC>(sb, kt + 1, tid, rb);
@@ -668,16 +698,16 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_join_kernel(const
 }
 
 // Few rows an expert: the matrices' bytes are what counts.  16 x 64 tiles, and
-// the four waves of a workgroup take every fourth step of k, each through slots
-// of its own and without barriers, so that many loads are under way; their sums
+// the waves of a workgroup take every fourth (or eighth) step of k, each through
+// slots of its own and without barriers, so that many loads are under way; their sums
 // are added in wave order at the end.
 constexpr int kFewRows = 16, kFewCols = 64;
-template <class T, int MODE, int WIDTH>
-__global__ __launch_bounds__(256) void expert_product_few_kernel(const ProductArgs p) {
+template <class T, int MODE, int WIDTH, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void expert_product_few_kernel(const ProductArgs p) {
   constexpr bool BKC = MODE == kRowsTrans;
   using OA = Operand<T, true, kFewRows, 64>;
   using OB = Operand<T, BKC, kFewCols, 64>;
-  constexpr int BK = OA::BK, FN = kFewCols / 16, kWaves = 4;
+  constexpr int BK = OA::BK, FN = kFewCols / 16;
   constexpr int kSlots = WIDTH ? 4 : 1, kSlot = OA::kBytes + OB::kBytes;
   static_assert(kSlots * kSlot >= FN * 64 * 16, "a wave's sums fit its slots");
   __shared__ alignas(1024) uint8_t s_mem[kWaves][kSlots][kSlot];
@@ -741,8 +771,8 @@ __global__ __launch_bounds__(256) void expert_product_few_kernel(const ProductAr
     };
     auto step = [&](int64_t i, int q) {
       if (w + i * kWaves >= steps) return;
-      store_pieces<OA>(lds, lane, ra[q], 64);
-      store_pieces<OB>(lds + OA::kBytes, lane, rb[q], 64);
+      store_pieces<OA, T, true>(sa, w + i * kWaves, lds, lane, ra[q], 64);
+      store_pieces<OB, T, BKC>(sb, w + i * kWaves, lds + OA::kBytes, lane, rb[q], 64);
       load(i + 2, q);
       wait_reads();  // (one wave: its own stores)
       read_frags(lds);
@@ -761,6 +791,7 @@ __global__ __launch_bounds__(256) void expert_product_few_kernel(const ProductAr
 #pragma unroll
   for (int j = 0; j < FN; ++j) *(f32x4*)&s_mem[w][0][(j * 64 + lane) * 16] = acc[j];
   __syncthreads();
+  if (w >= FN) return;
   f32x4 sum = *(const f32x4*)&s_mem[0][0][tid * 16];
 #pragma unroll
   for (int k = 1; k < kWaves; ++k) sum += *(const f32x4*)&s_mem[k][0][tid * 16];
@@ -822,8 +853,19 @@ template <class T, int MODE, int WIDTH>
 int launch_few(ProductArgs p, hipStream_t stream) {
   p.parts = nullptr;
   const int64_t tiles = tiles_of<MODE, kFewRows, kFewCols>(p);
-  if (tiles * 256 > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
-  hipLaunchKernelGGL((expert_product_few_kernel<T, MODE, WIDTH>), dim3((uint32_t)tiles), dim3(256), 0, stream, p);
+  if (tiles * 512 > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
+  // Eight waves where half of the chip has no tile, so that as many loads are under
+  // way (us with 4 and 8: one row, 4096 x 4096 f32 28 and 24; two of 8 experts
+  // 4095 x 4095 bf16, (K, N) 68 and 39, (N, K) 21 and 20; of 4096 x 4096 bf16, whose
+  // loads need no registers, 16.0 and 16.4).
+  if constexpr (sizeof(T) == 4 || WIDTH == 0) {
+    if (2 * ceil_div(p.n, kFewCols) * std::min<int64_t>(p.n_rows, p.n_experts) <= p.cus) {
+      hipLaunchKernelGGL((expert_product_few_kernel<T, MODE, WIDTH, 8>), dim3((uint32_t)tiles), dim3(512), 0, stream, p);
+      FS_CHECK_MAIN_LAUNCH("expert_product_few_kernel");
+      return FS_OK;
+    }
+  }
+  hipLaunchKernelGGL((expert_product_few_kernel<T, MODE, WIDTH, 4>), dim3((uint32_t)tiles), dim3(256), 0, stream, p);
   FS_CHECK_MAIN_LAUNCH("expert_product_few_kernel");
   return FS_OK;
 }
