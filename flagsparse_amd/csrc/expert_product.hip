@@ -43,6 +43,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) uint8_t lds_byte;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
 typedef __attribute__((address_space(3))) float lds_float;
 
 template <class T>
@@ -494,7 +496,7 @@ __device__ inline void store_four(T* row, int n, int cols, f32x4 v) {
   }
 }
 
-template <class T, int MODE, int WIDTH, int BM, int BN, int WM, int WN>
+template <class T, int MODE, int WIDTH, int BM, int BN, int WM, int WN, int SLOTS>
 __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const ProductArgs p) {
   constexpr int THREADS = 64 * WM * WN;
   constexpr bool AKC = MODE != kMatrix, BKC = MODE == kRowsTrans;
@@ -502,7 +504,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
   using OB = Operand<T, BKC, BN, THREADS>;
   constexpr int BK = OA::BK;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  constexpr int kSlots = WIDTH ? 4 : 2, kSlot = OA::kBytes + OB::kBytes;
+  constexpr int kSlots = WIDTH ? SLOTS : 2, kSlot = OA::kBytes + OB::kBytes, kAhead = SLOTS - 1;
   __shared__ alignas(1024) uint8_t s_mem[kSlots][kSlot];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -569,13 +571,13 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
       const int64_t at = kt >= steps ? kt : kt + turn < steps ? kt + turn : kt + turn - (steps - first);
       rsrc_a = da.at(at);
       rsrc_b = db.at(at);
-      next = lds + (uint32_t)(kt & 3) * kSlot;
+      next = lds + (uint32_t)(kt & kAhead) * kSlot;
     };
     auto load = [&](int i) {
       if (i < kLoadsA) da.issue(next, rsrc_a, i, w);
       else db.issue(next + OA::kBytes, rsrc_b, i - kLoadsA, w);
     };
-    for (int64_t kt = first; kt < first + 3; ++kt) {
+    for (int64_t kt = first; kt < first + kAhead; ++kt) {
       begin_loads(kt);
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) load(i);
@@ -615,12 +617,12 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
     } else {
       for (int64_t kt = first; kt < steps; ++kt) {
         wait_reads();
-        wait_loads<2 * kLoads>();
+        wait_loads<(kAhead - 1) * kLoads>();
         barrier();  // step kt has arrived, step kt - 1 has been read
-        begin_loads(kt + 3);
+        begin_loads(kt + kAhead);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) load(i);
-        read_frags(lds + (uint32_t)(kt & 3) * kSlot, FM);
+        read_frags(lds + (uint32_t)(kt & kAhead) * kSlot, FM);
 #pragma unroll
         for (int i = 0; i < FM; ++i) multiply_row(i);
       }
@@ -659,14 +661,48 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
       return;
     }
   }
-  // lane l holds row l % 16 and 4 neighbouring columns of each 16x16 result
-  const int cm = wm * fm * 16 + (lane & 15), cn = wn * (BN / WN) + (lane >> 4) * 4;
+  // Lane l holds row l % 16 and 4 neighbouring columns of each 16x16 result: by way
+  // of LDS a wave's 16 rows leave as whole 128-byte lines (STORES).
+  constexpr int kRow = 16 * FN * (int)sizeof(T), kPitch = kRow + 16, kLanes = kRow / 16, kOut = 16 / (int)sizeof(T);
+  static_assert(WM * WN * 16 * kPitch <= kSlots * kSlot, "the waves' rows fit the slots");
+  __syncthreads();  // (no wave reads or fills the slots any more)
+  lds_byte* own = (lds_byte*)(uintptr_t)lds + w * (16 * kPitch);
+  const int col = wn * (BN / WN) + lane % kLanes * kOut;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
-    const int m = cm + i * 16;
-    if (i >= fm || m >= work.c_rows) continue;
+    if (i >= fm) break;
 #pragma unroll
-    for (int j = 0; j < FN; ++j) store_four(work.c + (int64_t)m * p.ldc, cn + j * 16, work.c_cols, acc[i][j]);
+    for (int j = 0; j < FN; ++j) {
+      T out[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = (T)acc[i][j][e];
+      lds_byte* to = own + (lane & 15) * kPitch + (j * 16 + (lane >> 4) * 4) * (int)sizeof(T);
+      if constexpr (sizeof(T) == 2) {
+        u32x2 v;
+        __builtin_memcpy(&v, out, 8);
+        *(lds_u32x2*)to = v;
+      } else {
+        *(lds_u32x4*)to = __builtin_bit_cast(u32x4, acc[i][j]);
+      }
+    }
+    wait_reads();
+#pragma unroll
+    for (int q = 0; q < 16 * kLanes / 64; ++q) {
+      const int r = q * (64 / kLanes) + lane / kLanes, m = (wm * fm + i) * 16 + r;
+      const u32x4 v = *(const lds_u32x4*)(own + r * kPitch + lane % kLanes * 16);
+      if (m >= work.c_rows) continue;
+      T* row = work.c + (int64_t)m * p.ldc + col;
+      if (col + kOut <= work.c_cols) {
+        __builtin_memcpy(row, &v, 16);
+      } else {
+        T out[kOut];
+        __builtin_memcpy(out, &v, 16);
+#pragma unroll
+        for (int e = 0; e < kOut - 1; ++e)
+          if (col + e < work.c_cols) row[e] = out[e];
+      }
+    }
+    wait_reads();
   }
 }
 
@@ -836,8 +872,13 @@ int launch_tiles(ProductArgs p, void* ws, size_t ws_bytes, hipStream_t stream) {
   p.parts = need > 0 ? static_cast<float*>(ws) : nullptr;
   const int64_t tiles = tiles_of<MODE, BM, BN>(p) + (need > 0 ? places_of(p.cus, BM) : 0);
   if (tiles * 64 * WM * WN > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
-  hipLaunchKernelGGL((expert_product_kernel<T, MODE, WIDTH, BM, BN, WM, WN>), dim3((uint32_t)tiles),
-                     dim3(64 * WM * WN), 0, stream, p);
+  constexpr bool kShort = MODE == kMatrix && WIDTH != 0 && BM != kLarge;
+  if (kShort && p.n_rows / p.n_experts <= 4000)
+    hipLaunchKernelGGL((expert_product_kernel<T, MODE, WIDTH, BM, BN, WM, WN, kShort ? 2 : 4>), dim3((uint32_t)tiles),
+                       dim3(64 * WM * WN), 0, stream, p);
+  else
+    hipLaunchKernelGGL((expert_product_kernel<T, MODE, WIDTH, BM, BN, WM, WN, 4>), dim3((uint32_t)tiles),
+                       dim3(64 * WM * WN), 0, stream, p);
   FS_CHECK_MAIN_LAUNCH("expert_product_kernel");
   if constexpr (BM == kLarge || MODE == kMatrix) {
     if (need > 0) {
@@ -896,7 +937,7 @@ Tiles choose_tiles(const ProductArgs& p, bool half, int width) {
   // large tiles that do not fill the chip pay if their steps can be split
   if constexpr (MODE == kMatrix) {
     const int64_t tiles256 = tiles_of<MODE, kLarge, kLarge>(p);
-    if (half && width != 0 && (tiles256 >= 160 || (tiles256 >= 96 && p.n_rows / p.n_experts >= 6144))) return kTiles256;
+    if (half && width != 0 && p.n_rows / p.n_experts > 70 && (tiles256 >= 160 || (tiles256 >= 96 && p.n_rows / p.n_experts >= 6144))) return kTiles256;
     return tiles_of<MODE, 128, 128>(p) >= kFill ? kTiles128 : kTiles64;
   }
   const int64_t rows = p.n_rows / p.n_experts, active = std::min<int64_t>(p.n_rows, p.n_experts);
