@@ -496,7 +496,7 @@ __device__ inline void store_four(T* row, int n, int cols, f32x4 v) {
   }
 }
 
-template <class T, int MODE, int WIDTH, int BM, int BN, int WM, int WN, int SLOTS>
+template <class T, int MODE, int WIDTH, int BM, int BN, int WM, int WN, int SLOTS, bool PAST>
 __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const ProductArgs p) {
   constexpr int THREADS = 64 * WM * WN;
   constexpr bool AKC = MODE != kMatrix, BKC = MODE == kRowsTrans;
@@ -504,7 +504,8 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
   using OB = Operand<T, BKC, BN, THREADS>;
   constexpr int BK = OA::BK;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  constexpr int kSlots = WIDTH ? SLOTS : 2, kSlot = OA::kBytes + OB::kBytes, kAhead = SLOTS - 1;
+  constexpr int kSlots = WIDTH == 0 ? 2 : SLOTS, kSlot = OA::kBytes + OB::kBytes;
+  constexpr int kAhead = kSlots - 1;
   __shared__ alignas(1024) uint8_t s_mem[kSlots][kSlot];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -662,7 +663,12 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
     }
   }
   // Lane l holds row l % 16 and 4 neighbouring columns of each 16x16 result: by way
-  // of LDS a wave's 16 rows leave as whole 128-byte lines (STORES).
+  // of LDS a wave's 16 rows leave as lines of 128 or 256 bytes (us, 8 bytes a lane
+  // and so: 32768 rows of 16 experts 4096 x 4096 bf16 996 and 957, of 8 experts 256 x
+  // 1024 51 and 38, matrix gradient of 120 rows of 16 experts 4368 x 4032 191 and
+  // 125).  PAST: a matrix gradient's, where all lines are whole, go past the caches
+  // (256 rows of 32 experts 2048 x 4096 118 and 83, 2048 rows of 8 of 1024 x 1024 11.9
+  // and 10.3; lines in two parts, 64 experts 1800 x 1368, 66 and 148).
   constexpr int kRow = 16 * FN * (int)sizeof(T), kPitch = kRow + 16, kLanes = kRow / 16, kOut = 16 / (int)sizeof(T);
   static_assert(WM * WN * 16 * kPitch <= kSlots * kSlot, "the waves' rows fit the slots");
   __syncthreads();  // (no wave reads or fills the slots any more)
@@ -693,7 +699,7 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
       if (m >= work.c_rows) continue;
       T* row = work.c + (int64_t)m * p.ldc + col;
       if (col + kOut <= work.c_cols) {
-        __builtin_memcpy(row, &v, 16);
+        store_slice<PAST>(row, __builtin_bit_cast(Slice<T>, v));
       } else {
         T out[kOut];
         __builtin_memcpy(out, &v, 16);
@@ -864,6 +870,12 @@ size_t parts_bytes(const ProductArgs& p) {
   return may_split<MODE, BM, BN>(p) ? (size_t)places_of(p.cus, BM) * BM * BN * sizeof(float) : 0;
 }
 
+// Rows an expert up to which a matrix gradient's smaller tiles have two slots, so
+// that more workgroups share a compute unit: most of their time is the results' (us
+// with four and two: 127 rows of 64 experts 1800 x 1368 bf16 114 and 73, 256 of 32 of
+// 2048 x 4096 f32 279 and 191; 32768 an expert, 512 x 512 bf16 158 and 177).
+constexpr int64_t kShortRows = 1024;
+
 template <class T, int MODE, int WIDTH, int BM, int BN, int WM, int WN>
 int launch_tiles(ProductArgs p, void* ws, size_t ws_bytes, hipStream_t stream) {
   const size_t need = parts_bytes<MODE, BM, BN>(p);
@@ -872,13 +884,16 @@ int launch_tiles(ProductArgs p, void* ws, size_t ws_bytes, hipStream_t stream) {
   p.parts = need > 0 ? static_cast<float*>(ws) : nullptr;
   const int64_t tiles = tiles_of<MODE, BM, BN>(p) + (need > 0 ? places_of(p.cus, BM) : 0);
   if (tiles * 64 * WM * WN > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
-  constexpr bool kShort = MODE == kMatrix && WIDTH != 0 && BM != kLarge;
-  if (kShort && p.n_rows / p.n_experts <= 4000)
-    hipLaunchKernelGGL((expert_product_kernel<T, MODE, WIDTH, BM, BN, WM, WN, kShort ? 2 : 4>), dim3((uint32_t)tiles),
-                       dim3(64 * WM * WN), 0, stream, p);
-  else
-    hipLaunchKernelGGL((expert_product_kernel<T, MODE, WIDTH, BM, BN, WM, WN, 4>), dim3((uint32_t)tiles),
-                       dim3(64 * WM * WN), 0, stream, p);
+  auto launch = [&](auto slots, auto past) {
+    hipLaunchKernelGGL((expert_product_kernel<T, MODE, WIDTH, BM, BN, WM, WN, decltype(slots)::value, decltype(past)::value>),
+                       dim3((uint32_t)tiles), dim3(64 * WM * WN), 0, stream, p);
+  };
+  using Four = std::integral_constant<int, 4>;
+  using Two = std::integral_constant<int, MODE == kMatrix && WIDTH != 0 && BM != kLarge ? 2 : 4>;
+  using Past = std::integral_constant<bool, MODE == kMatrix>;
+  const bool past = MODE == kMatrix && ((uintptr_t)p.c | (size_t)p.ldc * sizeof(T)) % 128 == 0;
+  if (p.n_rows / p.n_experts <= kShortRows) past ? launch(Two{}, Past{}) : launch(Two{}, std::false_type{});
+  else past ? launch(Four{}, Past{}) : launch(Four{}, std::false_type{});
   FS_CHECK_MAIN_LAUNCH("expert_product_kernel");
   if constexpr (BM == kLarge || MODE == kMatrix) {
     if (need > 0) {
@@ -917,7 +932,8 @@ int launch_few(ProductArgs p, hipStream_t stream) {
 // few / 64 x 128 / 128 x 128 / 256 x 256:
 //   matrices (K, N)      4: 107  96  92  90     32: 154 106 105  95   128: 422 188 165 115
 //   (N, K), "trans"      8:  99  96             32:  -  104 106 103   128:  -   -  149 124
-//   matrix gradient                              32:  -  213 203 190   512:  -  516 457 395
+//   matrix gradient     350:  -   -  241 262   800:  -   -  528 434
+//   its whole words      75:  -   -  228 206   187:  -   -  310 265
 //   float32, (K, N)      8: 188 263 485 995     32: 302 276 486 993  1024:  - 2258 2093 2519 (16 experts)
 //   no whole words       8: 141 148 188         32: 229 151 203       128: 595 317 277
 //   whole words, (N, K)  8: 116 130
@@ -937,7 +953,7 @@ Tiles choose_tiles(const ProductArgs& p, bool half, int width) {
   // large tiles that do not fill the chip pay if their steps can be split
   if constexpr (MODE == kMatrix) {
     const int64_t tiles256 = tiles_of<MODE, kLarge, kLarge>(p);
-    if (half && width != 0 && p.n_rows / p.n_experts > 70 && (tiles256 >= 160 || (tiles256 >= 96 && p.n_rows / p.n_experts >= 6144))) return kTiles256;
+    if (half && width != 0 && p.n_rows / p.n_experts > (width == 16 ? 512 : 50) && (tiles256 >= 160 || (tiles256 >= 96 && p.n_rows / p.n_experts >= 6144))) return kTiles256;
     return tiles_of<MODE, 128, 128>(p) >= kFill ? kTiles128 : kTiles64;
   }
   const int64_t rows = p.n_rows / p.n_experts, active = std::min<int64_t>(p.n_rows, p.n_experts);
