@@ -363,8 +363,10 @@ extern "C" int fs_embedding_grad(int val_t, int out_t, int id_t, int64_t n, int6
       const int64_t chunks = n > kLong ? ceil_div(n, kLong) : 0, slices = slices_of<V>(width);
       const int wpr = slices <= 64 ? 1 : slices <= 128 ? 2 : 4;
       // up to 16 rows, so that workgroups fill the chip: 131072 tokens x 2048 of
-      // 2000 rows, bf16, 206 us with 16, 168 with 4; 65536 of 131072: 238 and 267
-      const int block_rows = (int)std::min<int64_t>(16, std::max<int64_t>(2, n_rows / (2048 * (4 / wpr))));
+      // 2000 rows, bf16, 206 us with 16, 168 with 4; 65536 of 131072: 238 and 267; of
+      // few tokens, found at once, up to 4: 1 of 262144 x 1024 121 and 105
+      const int64_t most = n <= 4096 ? 4 : 16;
+      const int block_rows = (int)std::min(most, std::max<int64_t>(2, n_rows / (2048 * (4 / wpr))));
       const int64_t chunk_blocks = ceil_div(chunks, 4 / wpr);
       const dim3 grid = row_grid(chunk_blocks + ceil_div(n_rows, (4 / wpr) * block_rows));
       auto launch = [&](auto past, auto some) {

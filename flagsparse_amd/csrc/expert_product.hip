@@ -20,9 +20,9 @@
 // last tile leave.
 //
 // Many rows: bound by the matrix instructions at the clock the card's power allows
-// (1.6 GHz here): bf16, 8192 x 8192 x 8192 1340 to 1440 TFLOP/s, 32768 rows of 16
-// experts 4096 x 4096 of unlike popularity 962 us, 1140 TFLOP/s; both gradients of
-// 16044 rows of 8 experts 2048 x 5120 f16 663 us, 1040 TFLOP/s.  Few rows: by the
+// (1.4 to 1.6 GHz): bf16, 8192 x 8192 x 8192 1340 to 1440 TFLOP/s, 32768 rows of 16
+// experts 4096 x 4096 of unlike popularity 957 us, 1150 TFLOP/s; both gradients of
+// 16044 rows of 8 experts 2048 x 5120 f16 647 us, 1060 TFLOP/s.  Few rows: by the
 // matrices' bytes, 64 rows of 25 of 32 experts 2048 x 4096 bf16 82 us, 420 MB at
 // 5.1 TB/s, the rate of a copy.
 #include <initializer_list>
