@@ -123,11 +123,14 @@ __device__ inline void store_sums(O* p, const A (&acc)[Slice<V>::n], A scale) {
   }
 }
 
-// A wave's share of one sum of rows: slices first, first + stride, ...
+// A wave's share of one sum of rows: slices first, first + stride, ...  A sum of
+// no rows is zero whatever the scale: infinite, NaN or negative ones give no NaN
+// and no -0 in table rows without tokens.
 template <bool PAST, class V, class O>
 __device__ inline void sum_rows(const V* __restrict__ grad, int64_t ldg, int pos, int t0, int t1, int64_t width,
                                 int64_t first, int64_t stride, int lane, typename Elem<V>::acc scale, O* out) {
   const int64_t slices = slices_of<V>(width);
+  if (t0 >= t1) scale = 0;
   typename Elem<V>::acc acc[Slice<V>::n];
   for (int64_t c = first; c < slices; c += stride) {  // (the same number of times for the lanes that go on)
     const int64_t h = slice_start<V>(c + lane < slices ? c + lane : slices - 1, width);
