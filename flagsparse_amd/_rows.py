@@ -33,6 +33,35 @@ def launch(function, device, *args):
         _lib.check(rc, function.__name__)
 
 
+def _span(t):
+    """Addresses from a tensor's first byte to behind its last."""
+    if t.numel() == 0:
+        return 0, 0
+    start = t.data_ptr()
+    last = sum((n - 1) * stride for n, stride in zip(t.shape, t.stride()))
+    return start, start + (last + 1) * t.element_size()
+
+
+def into(out, shape, like, *operands, dtype=None):
+    """The tensor that a kernel writes: ``out`` itself where it is contiguous and
+    shares no memory with an operand, which other workgroups would still read; a
+    new one, of ``dtype`` or ``like``'s, otherwise (``done`` copies it)."""
+    if out is not None and out.is_contiguous():
+        first, end = _span(out)
+        spans = (_span(t) for t in operands if t is not None)
+        if not any(first < b and a < end for a, b in spans):
+            return out
+    return like.new_empty(shape, dtype=dtype)
+
+
+def done(out, result):
+    """The result of a call: ``out``, with the result in it, where one was given."""
+    if out is not None and result is not out:
+        out.copy_(result)
+        return out
+    return result
+
+
 def check_out(out, device, shape, dtype):
     """Same checks and messages as the sparse products' (spmm_coo.py:619-625)."""
     if not isinstance(out, torch.Tensor):

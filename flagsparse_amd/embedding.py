@@ -19,7 +19,7 @@ import torch
 
 from . import _lib
 from ._common import SUPPORTED_INDEX_DTYPES
-from ._rows import ROW_DTYPE_MESSAGE, ROW_VALUE_CODES, check_out, launch, recording, row_major
+from ._rows import ROW_DTYPE_MESSAGE, ROW_VALUE_CODES, check_out, done, into, launch, recording, row_major
 
 
 def _check_tokens(tokens, values, what):
@@ -49,15 +49,10 @@ def _lookup(table, tokens, scale, out=None):
     table, ld = row_major(table, width)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
-    result = out
-    if out is None or not out.is_contiguous():
-        result = table.new_empty((*tokens.shape, width))
+    result = into(out, (*tokens.shape, width), table, table, tokens)
     launch(_lib.lib().fs_embedding, table.device, ROW_VALUE_CODES[table.dtype], _lib.INDEX_TYPE_CODES[tokens.dtype],
            tokens.numel(), n_rows, width, table.data_ptr(), ld, tokens.data_ptr(), scale, result.data_ptr())
-    if out is not None and result is not out:
-        out.copy_(result)
-        return out
-    return result
+    return done(out, result)
 
 
 class _Embedding(torch.autograd.Function):
@@ -118,19 +113,14 @@ def flagsparse_embedding_grad(grad, tokens, num_rows, scale=1.0, padding_idx=Non
         check_out(out, grad.device, (num_rows, width), dtype)
     grad, ld = row_major(grad.reshape(n, width), width)
     tokens = tokens.contiguous()
-    result = out
-    if out is None or not out.is_contiguous():
-        result = torch.empty((num_rows, width), dtype=dtype, device=grad.device)
+    result = into(out, (num_rows, width), grad, grad, tokens, dtype=dtype)
     code = ROW_VALUE_CODES[grad.dtype]
     lib = _lib.lib()
     ws = _lib.workspace(lib.fs_embedding_grad_workspace_bytes(code, n, num_rows, width), grad.device)
     launch(lib.fs_embedding_grad, grad.device, code, ROW_VALUE_CODES[dtype], _lib.INDEX_TYPE_CODES[tokens.dtype], n,
            num_rows, width, grad.data_ptr(), ld, tokens.data_ptr(), float(scale), padding, result.data_ptr(),
            ws.data_ptr(), ws.numel())
-    if out is not None and result is not out:
-        out.copy_(result)
-        return out
-    return result
+    return done(out, result)
 
 
 __all__ = ["flagsparse_embedding", "flagsparse_embedding_grad"]

@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from ._common import _INDEX_LIMIT_INT32, SUPPORTED_INDEX_DTYPES
-from ._rows import ROW_DTYPE_MESSAGE, ROW_VALUE_CODES, check_out, launch, recording, row_major
+from ._rows import ROW_DTYPE_MESSAGE, ROW_VALUE_CODES, check_out, done, into, launch, recording, row_major
 from .spmm_csr import _normalize_spmm_op, _spmm_op_transposes
 
 MAX_EXPERTS = 1023
@@ -126,27 +126,13 @@ def _check_weights(weights, rows, route):
         raise ValueError(f"weights must have shape {(route.n_tokens, route.slots)}, got {tuple(weights.shape)}")
 
 
-def _into(out, rows, width, like):
-    """The tensor to write: out itself where it is contiguous."""
-    if out is not None and out.is_contiguous():
-        return out
-    return like.new_empty((rows, width))
-
-
-def _done(out, result):
-    if out is not None and result is not out:
-        out.copy_(result)
-        return out
-    return result
-
-
 def _dispatch(x, route, out=None):
     width = x.shape[1]
     x, ld = row_major(x, width)
-    result = _into(out, route.n_rows, width, x)
+    result = into(out, (route.n_rows, width), x, x)
     launch(_lib.lib().fs_expert_dispatch, route.device, ROW_VALUE_CODES[x.dtype], route.n_tokens, route.slots, width,
            route.num_experts, x.data_ptr(), ld, route._inverse_ptr, route._offsets_ptr, result.data_ptr())
-    return _done(out, result)
+    return done(out, result)
 
 
 def _combine(rows, route, weights, out=None):
@@ -154,11 +140,11 @@ def _combine(rows, route, weights, out=None):
     rows, ld = row_major(rows, width)
     if weights is not None and not weights.is_contiguous():
         weights = weights.contiguous()
-    result = _into(out, route.n_tokens, width, rows)
+    result = into(out, (route.n_tokens, width), rows, rows, weights)
     launch(_lib.lib().fs_expert_combine, route.device, ROW_VALUE_CODES[rows.dtype], route.n_tokens, route.slots, width,
            route.num_experts, rows.data_ptr(), ld, route._inverse_ptr, route._offsets_ptr,
            None if weights is None else weights.data_ptr(), result.data_ptr())
-    return _done(out, result)
+    return done(out, result)
 
 
 class _Dispatch(torch.autograd.Function):
@@ -297,14 +283,14 @@ def _dense_matrices(matrices, trans):
 def _product(rows, matrices, route, trans, inner, outer, out=None):
     rows, ld = row_major(rows, inner)
     matrices, trans = _dense_matrices(matrices, trans)
-    result = _into(out, route.n_rows, outer, rows)
+    result = into(out, (route.n_rows, outer), rows, rows, matrices)
     lib = _lib.lib()
     sizes = (ROW_VALUE_CODES[rows.dtype], int(trans), route.n_rows, route.num_experts, inner, outer)
     need = lib.fs_expert_product_workspace_bytes(*sizes)
     ws = _lib.workspace(need, rows.device) if need else None
     launch(lib.fs_expert_product, route.device, *sizes, rows.data_ptr(), ld, matrices.data_ptr(), route._offsets_ptr,
            result.data_ptr(), _lib.ptr(ws), need)
-    return _done(out, result)
+    return done(out, result)
 
 
 def _product_grad_matrices(grad, rows, route, trans, inner, outer):
