@@ -55,11 +55,16 @@ def into(out, shape, like, *operands, dtype=None):
 
 
 def done(out, result):
-    """The result of a call: ``out``, with the result in it, where one was given."""
-    if out is not None and result is not out:
+    """The result of a call: ``out``, with the result in it, where one was given.
+    Autograd learns of the write, so a backward pass that still needs what ``out``
+    held raises."""
+    if out is None:
+        return result
+    if result is out:
+        torch.autograd.graph.increment_version(out)
+    else:
         out.copy_(result)
-        return out
-    return result
+    return out
 
 
 def check_out(out, device, shape, dtype):

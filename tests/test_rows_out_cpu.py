@@ -105,3 +105,17 @@ def test_the_result_reaches_out(monkeypatch, written):
     wide = torch.zeros(8, 16)
     expert._dispatch(torch.zeros(8, 8), _route(8), wide[:, ::2])
     assert torch.equal(wide[:, ::2], want) and not bool(wide[:, 1::2].any())
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_autograd_learns_of_the_write(written, name):
+    """A backward pass that needs the values which out= replaced raises, where the
+    kernel writes out itself and where the result is copied."""
+    x, tokens = torch.ones(8, 8), torch.arange(8)
+    for out in (torch.ones(8, 8), torch.ones(8, 16)[:, ::2], x):
+        factor = torch.ones(8, 8, requires_grad=True)
+        product = factor * out
+        with torch.no_grad():
+            _calls(x, out, tokens)[name]()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.sum().backward()
