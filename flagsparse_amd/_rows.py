@@ -77,3 +77,5 @@ def check_out(out, device, shape, dtype):
         raise ValueError("out must be on the same CUDA device as the inputs")
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
         raise ValueError("out shape/dtype must match result")
+    if out.requires_grad and recording():  # (its graph would be that of the values it held before)
+        raise ValueError("out cannot be given where a gradient is recorded")

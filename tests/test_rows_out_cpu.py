@@ -12,6 +12,7 @@ import torch
 import flagsparse_amd.embedding as embedding
 import flagsparse_amd.expert as expert
 from flagsparse_amd import _lib
+from flagsparse_amd._rows import check_out
 
 VALUE = 7.0
 
@@ -119,3 +120,14 @@ def test_autograd_learns_of_the_write(written, name):
             _calls(x, out, tokens)[name]()
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             product.sum().backward()
+
+
+def test_out_with_a_graph_is_refused(monkeypatch):
+    """out's graph would go on to give the gradient of the values it held before."""
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    held = torch.ones(8, 8, requires_grad=True) * 2.0
+    with pytest.raises(ValueError, match="out cannot be given where a gradient is recorded"):
+        check_out(held, held.device, (8, 8), torch.float32)
+    with torch.no_grad():
+        check_out(held, held.device, (8, 8), torch.float32)
+    check_out(held.detach(), held.device, (8, 8), torch.float32)
