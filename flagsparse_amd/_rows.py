@@ -1,6 +1,7 @@
 """Checks and layouts that the row operators share (embedding.py, expert.py)."""
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -24,6 +25,12 @@ def row_major(t, width):
 
 
 recording = torch.is_grad_enabled
+
+
+def refuse_tangent(t, what):
+    """The kernels would drop a forward-mode tangent without a word."""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{what} has a forward-mode tangent, which this operator does not propagate")
 
 
 def launch(function, device, *args):

@@ -19,7 +19,17 @@ import torch
 
 from . import _lib
 from ._common import SUPPORTED_INDEX_DTYPES
-from ._rows import ROW_DTYPE_MESSAGE, ROW_VALUE_CODES, check_out, done, into, launch, recording, row_major
+from ._rows import (
+    ROW_DTYPE_MESSAGE,
+    ROW_VALUE_CODES,
+    check_out,
+    done,
+    into,
+    launch,
+    recording,
+    refuse_tangent,
+    row_major,
+)
 
 
 def _check_tokens(tokens, values, what):
@@ -33,6 +43,7 @@ def _check_tokens(tokens, values, what):
         raise ValueError(f"{what} and tokens must be CUDA tensors")
     if values.device != tokens.device:
         raise ValueError(f"{what} and tokens must be on the same CUDA device")
+    refuse_tangent(values, what)
 
 
 def _normalize_padding(padding_idx, n_rows):

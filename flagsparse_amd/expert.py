@@ -27,7 +27,17 @@ import torch
 
 from . import _lib
 from ._common import _INDEX_LIMIT_INT32, SUPPORTED_INDEX_DTYPES
-from ._rows import ROW_DTYPE_MESSAGE, ROW_VALUE_CODES, check_out, done, into, launch, recording, row_major
+from ._rows import (
+    ROW_DTYPE_MESSAGE,
+    ROW_VALUE_CODES,
+    check_out,
+    done,
+    into,
+    launch,
+    recording,
+    refuse_tangent,
+    row_major,
+)
 from .spmm_csr import _normalize_spmm_op, _spmm_op_transposes
 
 MAX_EXPERTS = 1023
@@ -112,6 +122,7 @@ def _check_rows(rows, what, route, n_rows):
         raise ValueError(f"{what} must be on the same CUDA device as the route")
     if rows.ndim != 2 or rows.shape[0] != n_rows:
         raise ValueError(f"{what} must be a 2D tensor with {n_rows} rows, got shape {tuple(rows.shape)}")
+    refuse_tangent(rows, what)
 
 
 def _check_weights(weights, rows, route):
@@ -124,6 +135,7 @@ def _check_weights(weights, rows, route):
         raise ValueError("weights must be on the same CUDA device as the route")
     if weights.shape != (route.n_tokens, route.slots):
         raise ValueError(f"weights must have shape {(route.n_tokens, route.slots)}, got {tuple(weights.shape)}")
+    refuse_tangent(weights, "weights")
 
 
 def _dispatch(x, route, out=None):
@@ -263,6 +275,7 @@ def _check_product(rows, matrices, route, op):
     if matrices.ndim != 3 or matrices.shape[0] != route.num_experts:
         raise ValueError(f"matrices must be a 3D tensor with {route.num_experts} matrices, got shape "
                          f"{tuple(matrices.shape)}")
+    refuse_tangent(matrices, "matrices")
     trans = _spmm_op_transposes(_normalize_spmm_op(op))
     inner, outer = matrices.shape[2 if trans else 1], matrices.shape[1 if trans else 2]
     if rows.shape[1] != inner:
