@@ -323,7 +323,8 @@ def _product_grad_matrices(grad, rows, route, trans, inner, outer):
 class _Product(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, matrices, route, trans, inner, outer):
-        ctx.save_for_backward(rows, matrices)
+        # (each gradient reads the other operand only)
+        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, matrices if ctx.needs_input_grad[0] else None)
         ctx.route, ctx.sizes = route, (trans, inner, outer)
         return _product(rows, matrices, route, trans, inner, outer)
 
