@@ -100,11 +100,22 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(const V* __restrict
   }
 }
 
+// x * y rounded to A before it is rounded to a value type.  (Left to itself the
+// compiler turns some of a slice's products into instructions that round to 16
+// bits at once and others not, differently in each form of a kernel.)
+template <class A>
+__device__ inline A product(A x, A y) {
+  A p = x * y;
+  asm("" : "+v"(p));
+  return p;
+}
+
 // One wave a slot: the token's gradient row, read by its slots in turn, comes
 // from cache after the first.  The row of the gradient is written in the pass that
 // sums the weight's: 8191 x 8 slots, rows of 2560 f16, 714 MB, 138 us, 5.2 TB/s, the
-// rate of a copy.
-template <class V, bool PAST>
+// rate of a copy.  ROWS, DOTS: which of the two gradients are wanted; the rows are
+// read for the weights' alone, the weights for the rows' alone.
+template <class V, bool PAST, bool ROWS, bool DOTS>
 __global__ __launch_bounds__(256) void expert_combine_grad_kernel(
     const V* __restrict__ grad, int64_t ldg, const V* __restrict__ rows, int64_t ldr, int64_t n, int slots,
     int64_t width, const int32_t* __restrict__ inverse, const int32_t* __restrict__ routed_at,
@@ -117,36 +128,46 @@ __global__ __launch_bounds__(256) void expert_combine_grad_kernel(
   if (i >= n) return;
   const int at = inverse[i];
   const bool in = at < *routed_at;
-  const A w = in ? weights[i] : (A)0;
+  const A w = ROWS && in ? weights[i] : (A)0;
   const V* g = grad + i / slots * ldg;
-  const V* y = rows + at * ldr;
-  V* o = grad_rows + at * width;
+  const V* y = DOTS ? rows + at * ldr : nullptr;
+  V* o = ROWS ? grad_rows + at * width : nullptr;
   // (no overlapping slice at the end: an element counts once in the dot product)
   const int64_t full = width / E;
   A dot = 0;
   if (in) {
-#pragma unroll 2
-    for (int64_t c = lane; c < full; c += 64) {
-      const Slice<V> sg = load_slice(g + c * E), sy = load_slice(y + c * E);
+    // (two slices' loads in flight)
+    auto one = [&](int64_t c, const Slice<V>& sg, const Slice<V>& sy) {
       Slice<V> out;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const A ge = widen(sg.v[e]);
-        dot += ge * widen(sy.v[e]);
-        out.v[e] = (V)(w * ge);
+        if constexpr (DOTS) dot += ge * widen(sy.v[e]);
+        if constexpr (ROWS) out.v[e] = (V)product(w, ge);
       }
-      store_slice<PAST>(o + c * E, out);
+      if constexpr (ROWS) store_slice<PAST>(o + c * E, out);
+    };
+    auto of_grad = [&](int64_t c) { return load_slice(g + c * E); };
+    auto of_row = [&](int64_t c) { return DOTS ? load_slice(y + c * E) : Slice<V>{}; };
+    int64_t c = lane;
+    for (; c + 64 < full; c += 128) {
+      const Slice<V> g0 = of_grad(c), y0 = of_row(c), g1 = of_grad(c + 64), y1 = of_row(c + 64);
+      one(c, g0, y0);
+      one(c + 64, g1, y1);
     }
+    if (c < full) one(c, of_grad(c), of_row(c));
     for (int64_t h = full * E + lane; h < width; h += 64) {
-      dot += widen(g[h]) * widen(y[h]);
-      o[h] = (V)(w * widen(g[h]));
+      if constexpr (DOTS) dot += widen(g[h]) * widen(y[h]);
+      if constexpr (ROWS) o[h] = (V)product(w, widen(g[h]));
     }
-  } else {
+  } else if constexpr (ROWS) {
     for (int64_t c = lane; c < full; c += 64) store_slice<PAST>(o + c * E, Slice<V>{});
     for (int64_t h = full * E + lane; h < width; h += 64) o[h] = (V)0;
   }
-  dot = wave_sum(dot);
-  if (lane == 0) grad_w[i] = dot;
+  if constexpr (DOTS) {
+    dot = wave_sum(dot);
+    if (lane == 0) grad_w[i] = dot;
+  }
 }
 
 int check_rows(const char* who, int64_t n_tokens, int slots, int64_t width, int64_t n_experts) {
@@ -210,21 +231,30 @@ extern "C" int fs_expert_combine_grad(int val_t, int64_t n_tokens, int slots, in
   using namespace fs;
   if (int rc = check_rows("fs_expert_combine_grad", n_tokens, slots, width, n_experts)) return rc;
   if (n_tokens == 0) return FS_OK;
-  if (!inverse || !offsets || !weights || !grad_weights || ldg < 0 || ldr < 0 ||
-      (width > 0 && (!grad || !rows || !grad_rows)))
+  // (of no columns the rows' gradient is empty, and may be null where it is wanted)
+  const bool of_rows = grad_rows != nullptr, of_weights = grad_weights != nullptr;
+  if (!inverse || !offsets || ldg < 0 || ldr < 0 || (of_rows && !weights) ||
+      (width > 0 && (!grad || (of_weights && !rows) || (!of_rows && !of_weights))))
     return fail(FS_E_INVALID, "fs_expert_combine_grad: bad pointer or stride");
+  if (width == 0 && !of_weights) return FS_OK;
   return with_value_type(val_t, "fs_expert_combine_grad", [&](auto v) -> int {
     using V = decltype(v);
     using A = typename Elem<V>::acc;
     const int64_t n = n_tokens * slots;
     const dim3 grid = row_grid(ceil_div(n, 4));
-    auto launch = [&](auto past) {
-      hipLaunchKernelGGL((expert_combine_grad_kernel<V, decltype(past)::value>), grid, dim3(256), 0, stream, (const V*)grad, ldg,
-                         (const V*)rows, ldr, n, slots, width, inverse, offsets + n_experts, (const A*)weights,
-                         (V*)grad_rows, (A*)grad_weights);
+    auto launch = [&](auto past, auto want_rows, auto want_weights) {
+      hipLaunchKernelGGL((expert_combine_grad_kernel<V, decltype(past)::value, decltype(want_rows)::value,
+                                                     decltype(want_weights)::value>),
+                         grid, dim3(256), 0, stream, (const V*)grad, ldg, (const V*)rows, ldr, n, slots, width,
+                         inverse, offsets + n_experts, (const A*)weights, (V*)grad_rows, (A*)grad_weights);
     };
-    if (store_past_caches((n_tokens + 2 * n) * width * (int64_t)sizeof(V), width * sizeof(V))) launch(std::true_type{});
-    else launch(std::false_type{});
+    using Yes = std::true_type;
+    using No = std::false_type;
+    const int64_t moved = n_tokens + (of_rows ? n : 0) + (of_weights ? n : 0);
+    const bool past = store_past_caches(moved * width * (int64_t)sizeof(V), width * sizeof(V));
+    if (!of_rows) launch(No{}, No{}, Yes{});
+    else if (of_weights) past ? launch(Yes{}, Yes{}, Yes{}) : launch(No{}, Yes{}, Yes{});
+    else past ? launch(Yes{}, Yes{}, No{}) : launch(No{}, Yes{}, No{});
     FS_CHECK_MAIN_LAUNCH("expert_combine_grad_kernel");
     return FS_OK;
   });

@@ -159,6 +159,27 @@ def _combine(rows, route, weights, out=None):
     return done(out, result)
 
 
+def _combine_grad(grad, rows, route, weights):
+    """(gradient of the rows, which needs the weights, gradient of the weights, which
+    needs the rows): None for one whose operand is None."""
+    width = grad.shape[1]
+    grad, ldg = row_major(grad, width)
+    grad_rows = grad_weights = None
+    ldr = width
+    if weights is not None:
+        weights = weights.contiguous()
+        grad_rows = grad.new_empty((route.n_rows, width))
+    if rows is not None:
+        rows, ldr = row_major(rows, width)
+        wide = torch.float64 if rows.dtype == torch.float64 else torch.float32
+        grad_weights = grad.new_empty((route.n_tokens, route.slots), dtype=wide)
+    address = [None if t is None else t.data_ptr() for t in (rows, weights, grad_rows, grad_weights)]
+    launch(_lib.lib().fs_expert_combine_grad, route.device, ROW_VALUE_CODES[grad.dtype], route.n_tokens, route.slots,
+           width, route.num_experts, grad.data_ptr(), ldg, address[0], ldr, route._inverse_ptr, route._offsets_ptr,
+           *address[1:])
+    return grad_rows, grad_weights
+
+
 class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, route):
@@ -174,17 +195,18 @@ class _Dispatch(torch.autograd.Function):
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, route, weights):
-        ctx.route = route
-        ctx.save_for_backward(rows, weights)
+        ctx.route, ctx.weighted = route, weights is not None
+        # (each gradient reads the other operand only)
+        ctx.save_for_backward(rows if ctx.needs_input_grad[2] else None, weights if ctx.needs_input_grad[0] else None)
         return _combine(rows, route, weights)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        rows, weights = ctx.saved_tensors
-        if weights is None:
+        if not ctx.weighted:
             return _dispatch(grad, ctx.route), None, None
-        grad_rows, grad_weights = flagsparse_expert_combine_grad(grad, rows, ctx.route, weights)
+        rows, weights = ctx.saved_tensors
+        grad_rows, grad_weights = _combine_grad(grad, rows, ctx.route, weights)
         return grad_rows, None, grad_weights
 
 
@@ -245,16 +267,7 @@ def flagsparse_expert_combine_grad(grad, rows, route, weights):
     if grad.shape[1] != rows.shape[1]:
         raise ValueError(f"grad must have width {rows.shape[1]}, got {grad.shape[1]}")
     _check_weights(weights, rows, route)
-    width = rows.shape[1]
-    grad, ldg = row_major(grad, width)
-    rows, ldr = row_major(rows, width)
-    weights = weights.contiguous()
-    grad_rows = rows.new_empty((route.n_rows, width))
-    grad_weights = weights.new_empty((route.n_tokens, route.slots))
-    launch(_lib.lib().fs_expert_combine_grad, route.device, ROW_VALUE_CODES[rows.dtype], route.n_tokens, route.slots,
-           width, route.num_experts, grad.data_ptr(), ldg, rows.data_ptr(), ldr, route._inverse_ptr, route._offsets_ptr,
-           weights.data_ptr(), grad_rows.data_ptr(), grad_weights.data_ptr())
-    return grad_rows, grad_weights
+    return _combine_grad(grad, rows, route, weights)
 
 
 PRODUCT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)

@@ -618,7 +618,9 @@ int fs_expert_route(int id_t, int64_t n, int64_t n_experts, const void* experts,
  *                 of no expert left out; weights may be null (ones)
  *   combine_grad  grad_rows[inverse[t, j]] = weights[t, j] grad[t] and
  *                 grad_weights[t, j] = <grad[t], rows[inverse[t, j]]>; zeros for
- *                 slots of no expert
+ *                 slots of no expert.  Either result may be null where the other
+ *                 alone is wanted: the rows' reads no rows, the weights' no
+ *                 weights, which may then be null too
  */
 int fs_expert_dispatch(int val_t, int64_t n_tokens, int slots, int64_t width, int64_t n_experts,
                        const void* x, int64_t ldx, const int32_t* inverse, const int32_t* offsets,
