@@ -52,7 +52,8 @@ class PreparedExpertRoute:
               the number of slots that name one
     """
 
-    __slots__ = ("n_tokens", "slots", "num_experts", "n_rows", "device", "_places", "_inverse_ptr", "_offsets_ptr")
+    __slots__ = ("n_tokens", "slots", "num_experts", "n_rows", "device", "_places", "_inverse_ptr", "_offsets_ptr",
+                 "_stream")
 
     def __init__(self, n_tokens, slots, num_experts, places):
         n = n_tokens * slots
@@ -63,6 +64,7 @@ class PreparedExpertRoute:
         self._places = places
         start = places.data_ptr()
         self._inverse_ptr, self._offsets_ptr = start + 4 * n, start + 8 * n
+        self._stream = _lib.stream_handle(self.device)
 
     @property
     def order(self):
@@ -138,11 +140,23 @@ def _check_weights(weights, rows, route):
     refuse_tangent(weights, "weights")
 
 
+def _launch(function, route, *args):
+    """One call that reads a route's places.  A dropped route's memory waits for calls
+    still queued on other streams than its own: its next owner would overwrite the
+    places that they store to."""
+    stream = _lib.stream_handle(route.device)
+    if stream != route._stream:
+        route._places.record_stream(torch.cuda.current_stream(route.device))
+    rc = function(*args, stream)
+    if rc:
+        _lib.check(rc, function.__name__)
+
+
 def _dispatch(x, route, out=None):
     width = x.shape[1]
     x, ld = row_major(x, width)
     result = into(out, (route.n_rows, width), x, x)
-    launch(_lib.lib().fs_expert_dispatch, route.device, ROW_VALUE_CODES[x.dtype], route.n_tokens, route.slots, width,
+    _launch(_lib.lib().fs_expert_dispatch, route, ROW_VALUE_CODES[x.dtype], route.n_tokens, route.slots, width,
            route.num_experts, x.data_ptr(), ld, route._inverse_ptr, route._offsets_ptr, result.data_ptr())
     return done(out, result)
 
@@ -153,7 +167,7 @@ def _combine(rows, route, weights, out=None):
     if weights is not None and not weights.is_contiguous():
         weights = weights.contiguous()
     result = into(out, (route.n_tokens, width), rows, rows, weights)
-    launch(_lib.lib().fs_expert_combine, route.device, ROW_VALUE_CODES[rows.dtype], route.n_tokens, route.slots, width,
+    _launch(_lib.lib().fs_expert_combine, route, ROW_VALUE_CODES[rows.dtype], route.n_tokens, route.slots, width,
            route.num_experts, rows.data_ptr(), ld, route._inverse_ptr, route._offsets_ptr,
            None if weights is None else weights.data_ptr(), result.data_ptr())
     return done(out, result)
@@ -174,7 +188,7 @@ def _combine_grad(grad, rows, route, weights):
         wide = torch.float64 if rows.dtype == torch.float64 else torch.float32
         grad_weights = grad.new_empty((route.n_tokens, route.slots), dtype=wide)
     address = [None if t is None else t.data_ptr() for t in (rows, weights, grad_rows, grad_weights)]
-    launch(_lib.lib().fs_expert_combine_grad, route.device, ROW_VALUE_CODES[grad.dtype], route.n_tokens, route.slots,
+    _launch(_lib.lib().fs_expert_combine_grad, route, ROW_VALUE_CODES[grad.dtype], route.n_tokens, route.slots,
            width, route.num_experts, grad.data_ptr(), ldg, address[0], ldr, route._inverse_ptr, route._offsets_ptr,
            *address[1:])
     return grad_rows, grad_weights
@@ -314,7 +328,7 @@ def _product(rows, matrices, route, trans, inner, outer, out=None):
     sizes = (ROW_VALUE_CODES[rows.dtype], int(trans), route.n_rows, route.num_experts, inner, outer)
     need = lib.fs_expert_product_workspace_bytes(*sizes)
     ws = _lib.workspace(need, rows.device) if need else None
-    launch(lib.fs_expert_product, route.device, *sizes, rows.data_ptr(), ld, matrices.data_ptr(), route._offsets_ptr,
+    _launch(lib.fs_expert_product, route, *sizes, rows.data_ptr(), ld, matrices.data_ptr(), route._offsets_ptr,
            result.data_ptr(), _lib.ptr(ws), need)
     return done(out, result)
 
@@ -328,7 +342,7 @@ def _product_grad_matrices(grad, rows, route, trans, inner, outer):
     sizes = (ROW_VALUE_CODES[rows.dtype], int(trans), route.n_rows, route.num_experts, inner, outer)
     need = lib.fs_expert_product_grad_matrices_workspace_bytes(*sizes)
     ws = _lib.workspace(need, rows.device) if need else None
-    launch(lib.fs_expert_product_grad_matrices, route.device, *sizes, grad.data_ptr(), ldg, rows.data_ptr(), ldr,
+    _launch(lib.fs_expert_product_grad_matrices, route, *sizes, grad.data_ptr(), ldg, rows.data_ptr(), ldr,
            route._offsets_ptr, result.data_ptr(), _lib.ptr(ws), need)
     return result
 
