@@ -377,8 +377,13 @@ extern "C" int fs_embedding_grad(int val_t, int out_t, int id_t, int64_t n, int6
                            (const V*)grad, ldg, keys, order, n, n_rows, width, (A)scale, padding, wpr, block_rows,
                            chunk_blocks, chunks, filled, (O*)out, parts);
       };
-      if (store_past_caches((n * (int64_t)sizeof(V) + n_rows * (int64_t)sizeof(O)) * width, width * sizeof(O)))
-        filled > 0 ? launch(std::true_type{}, std::true_type{}) : launch(std::true_type{}, std::false_type{});
+      // past the caches only where a wave's slices leave as whole lines: a 32-bit result
+      // of 16-bit values leaves as every second 16 bytes at a time (us so and past the
+      // caches: 65536 tokens of 131072 x 2048 372 and 562, one token 201 and 527)
+      using Past = std::integral_constant<bool, sizeof(O) == sizeof(V)>;
+      const int64_t bytes = (n * (int64_t)sizeof(V) + n_rows * (int64_t)sizeof(O)) * width;
+      if (Past::value && store_past_caches(bytes, width * sizeof(O)))
+        filled > 0 ? launch(Past{}, std::true_type{}) : launch(Past{}, std::false_type{});
       else filled > 0 ? launch(std::false_type{}, std::true_type{}) : launch(std::false_type{}, std::false_type{});
       FS_CHECK_MAIN_LAUNCH("embedding_grad_kernel");
       if (chunks > 0) {
