@@ -664,11 +664,11 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
   }
   // Lane l holds row l % 16 and 4 neighbouring columns of each 16x16 result: by way
   // of LDS a wave's 16 rows leave as lines of 128 or 256 bytes (us, 8 bytes a lane
-  // and so: 32768 rows of 16 experts 4096 x 4096 bf16 996 and 957, of 8 experts 256 x
-  // 1024 51 and 38, matrix gradient of 120 rows of 16 experts 4368 x 4032 191 and
-  // 125).  PAST: a matrix gradient's, where all lines are whole, go past the caches
-  // (256 rows of 32 experts 2048 x 4096 118 and 83, 2048 rows of 8 of 1024 x 1024 11.9
-  // and 10.3; lines in two parts, 64 experts 1800 x 1368, 66 and 148).
+  // and so: 16 experts of 2048 rows, 4096 x 4096 bf16 996 and 957, 8 of 4096 rows, 256 x
+  // 1024 51 and 38, matrix gradient of 16 experts of 7 or 8 rows, 4368 x 4032 191 and
+  // 125).  PAST: a matrix gradient's, where all lines are whole, go past the caches (32
+  // experts of 8 rows, 2048 x 4096 116 and 84, of 256 rows 283 and 187, 8 of 256 rows,
+  // 1024 x 1024 10.4 and 9.1; lines in two parts, 64 of 2 rows, 1800 x 1368, 66 and 148).
   constexpr int kRow = 16 * FN * (int)sizeof(T), kPitch = kRow + 16, kLanes = kRow / 16, kOut = 16 / (int)sizeof(T);
   static_assert(WM * WN * 16 * kPitch <= kSlots * kSlot, "the waves' rows fit the slots");
   __syncthreads();  // (no wave reads or fills the slots any more)
@@ -870,11 +870,19 @@ size_t parts_bytes(const ProductArgs& p) {
   return may_split<MODE, BM, BN>(p) ? (size_t)places_of(p.cus, BM) * BM * BN * sizeof(float) : 0;
 }
 
-// Rows an expert up to which a matrix gradient's smaller tiles have two slots, so
-// that more workgroups share a compute unit: most of their time is the results' (us
-// with four and two: 127 rows of 64 experts 1800 x 1368 bf16 114 and 73, 256 of 32 of
-// 2048 x 4096 f32 279 and 191; 32768 an expert, 512 x 512 bf16 158 and 177).
-constexpr int64_t kShortRows = 1024;
+// Whether a matrix gradient's smaller tiles have two slots instead of four, so that
+// more workgroups share a compute unit: where there are more of them than places, with
+// 32-bit values (us with two and four: 32 experts of 64 rows, 2048 x 4096, 317 and 362,
+// of 4096 rows 15071 and 15853; 4 of 32768, 256 x 320, 295 and 307), and with 16-bit ones
+// of few rows, whose time is the results' (32 of 8 rows, 2048 x 4096, 83 and 115, of 320
+// 218 and 251; 16 of 384, 1024 x 2048 34 and 39, 64 of 384, 512 x 512 32 and 31, of 512 40
+// and 36).  With fewer, two slots only start loads later (4 of 1024 rows, 512 x 512 17.5
+// and 10.8, 1024 x 1024 19.3 and 14.9).
+constexpr int64_t kShortRows = 384;
+template <class T>
+bool two_slots(const ProductArgs& p, int64_t workgroups, uint32_t places) {
+  return workgroups > places && (sizeof(T) == 4 || p.n_rows / p.n_experts <= kShortRows);
+}
 
 template <class T, int MODE, int WIDTH, int BM, int BN, int WM, int WN>
 int launch_tiles(ProductArgs p, void* ws, size_t ws_bytes, hipStream_t stream) {
@@ -892,7 +900,7 @@ int launch_tiles(ProductArgs p, void* ws, size_t ws_bytes, hipStream_t stream) {
   using Two = std::integral_constant<int, MODE == kMatrix && WIDTH != 0 && BM != kLarge ? 2 : 4>;
   using Past = std::integral_constant<bool, MODE == kMatrix>;
   const bool past = MODE == kMatrix && ((uintptr_t)p.c | (size_t)p.ldc * sizeof(T)) % 128 == 0;
-  if (p.n_rows / p.n_experts <= kShortRows) past ? launch(Two{}, Past{}) : launch(Two{}, std::false_type{});
+  if (two_slots<T>(p, tiles, places_of(p.cus, BM))) past ? launch(Two{}, Past{}) : launch(Two{}, std::false_type{});
   else past ? launch(Four{}, Past{}) : launch(Four{}, std::false_type{});
   FS_CHECK_MAIN_LAUNCH("expert_product_kernel");
   if constexpr (BM == kLarge || MODE == kMatrix) {
@@ -928,19 +936,31 @@ int launch_few(ProductArgs p, hipStream_t stream) {
 
 // Which tiles.  The larger, the fewer times operands are read and the nearer to
 // the matrix cores' rate, if rows fill them and there are enough for the chip
-// (kFill).  us, bf16, 32 experts 2048 x 4096, rows an expert on average; tiles
-// few / 64 x 128 / 128 x 128 / 256 x 256:
-//   matrices (K, N)      4: 107  96  92  90     32: 154 106 105  95   128: 422 188 165 115
-//   (N, K), "trans"      8:  99  96             32:  -  104 106 103   128:  -   -  149 124
-//   matrix gradient     350:  -   -  241 262   800:  -   -  528 434
-//   its whole words      75:  -   -  228 206   187:  -   -  310 265
-//   float32, (K, N)      8: 188 263 485 995     32: 302 276 486 993  1024:  - 2258 2093 2519 (16 experts)
-//   no whole words       8: 141 148 188         32: 229 151 203       128: 595 317 277
-//   whole words, (N, K)  8: 116 130
-// Large tiles too few to fill the chip, split along k (2048 rows of 4 experts
-// 4096 x 4096: 88, 128 x 128 118; 1024 x 2 of 8, 2048 x 2048: 50, 45), and of a
-// matrix gradient (16384 rows of 8, 1024 x 1024: 56, 42; of 4 x 8192 rows, 1024 x
-// 2048: 132, 146).
+// (kFill).  us, 32 experts 2048 x 4096, bf16 where not said otherwise, rows an
+// expert, all alike; tiles few / 64 x 128 / 128 x 128 / 256 x 256:
+//   matrices (K, N)      2: 102  93  89  88     4: 104  95  91  88    32: 143 101 101  92
+//     unlike popularity  1:  60  64  64  74     2:  77  84  80  76     4:  82  89  85  78
+//   (N, K), "trans"      2:  96  93  95  97    16: 103  97  99  99    32: 146 101 104 102
+//                       48: 178 109 111 106   112:  -  178 127 122
+//   2046 x 4094, (K, N)  6: 103  89            12: 109  92
+//     (N, K)             6: 112 129            12: 121 134            16: 127 137
+//   2047 x 4095, (K, N)  6: 109  96            12: 117  98
+//     (N, K)             6: 129 155            12: 137 157            16: 142 157
+//   float32, (K, N)     16: 195 285 500        32: 263 286 504
+//     unlike popularity 32: 302 276 486       768:  - 1513 1498 (16 experts)
+//   matrix gradient    256:  -   -  188 194   384:  -   -  308 268   640:  -   -  412 365
+//     unlike popularity 320: -   -  226 221   384:  -   -  298 268   640:  -   -  451 363
+//     16 of 1024 x 2048 384: -   -   34  39   448:  -   -   44  43
+//     2046 x 4094       32:  -   -  176 186    48:  -   -  207 192    64:  -   -  208 194
+// Of products of rows, 8 experts of 1024 rows, 1024 columns of k, 128 / 256: with
+// 160 large tiles 39 / 32, 192 41 / 32, 128 26 / 29 (64 and 128 rows: 8 experts of 64
+// rows, 256 tiles of 128 17 / 18, of 96 rows 25 / 20, 128 tiles of 96 rows 13 / 15).
+// Fewer large tiles are split along k (8 experts of 1024 rows, popularities
+// unlike, and alike): k 1536, 128 tiles 49 / 42 to 47, alike 41 / 46; k 2048, 128 tiles
+// 62 / 51 to 55, 50 / 60, 96 tiles 44 to 48 / 56, 42 / 54; k 4096, 128 tiles 119 / 91 to 100,
+// 93 / 93, 64 tiles 68 / 63, 54 / 64.  A matrix gradient's along the rows (4 experts):
+// 96 tiles of 4096 rows 77 / 66, of 6144 115 / 87, of 1024 20 / 26; 64 tiles of 8192 rows
+// 96 / 83; 160 tiles of 1024 rows 26 / 27, of 4096 110 / 87.
 // 1.5 rounds of large tiles lose to smaller ones (64 experts of 1536 columns, 8
 // rows: 87, 64 x 128 73).  One token (8 experts of 64, 4096 columns): few 23, 64
 // x 128 23, 256 x 256 42; (1 of 8, 4096 x 4096): 12, 28, 72; 16 tokens, 2 of 8,
@@ -950,13 +970,15 @@ constexpr int64_t kFill = 256;
 enum Tiles { kFew, kTiles64, kTiles128, kTiles256 };
 template <int MODE>
 Tiles choose_tiles(const ProductArgs& p, bool half, int width) {
+  const int64_t rows = p.n_rows / p.n_experts, active = std::min<int64_t>(p.n_rows, p.n_experts);
   // large tiles that do not fill the chip pay if their steps can be split
   if constexpr (MODE == kMatrix) {
     const int64_t tiles256 = tiles_of<MODE, kLarge, kLarge>(p);
-    if (half && width != 0 && p.n_rows / p.n_experts > (width == 16 ? 512 : 50) && (tiles256 >= 160 || (tiles256 >= 96 && p.n_rows / p.n_experts >= 6144))) return kTiles256;
+    if (half && width != 0 && rows > (width == 16 ? kShortRows : 50) &&
+        (tiles256 >= 160 || (tiles256 >= 96 && rows >= 6144)))
+      return kTiles256;
     return tiles_of<MODE, 128, 128>(p) >= kFill ? kTiles128 : kTiles64;
   }
-  const int64_t rows = p.n_rows / p.n_experts, active = std::min<int64_t>(p.n_rows, p.n_experts);
   const int64_t tiles256 = ceil_div(p.n, kLarge) * std::max(active, p.n_rows / kLarge);
   const int64_t tiles128 = ceil_div(p.n, 128) * std::max(active, p.n_rows / 128);
   const int64_t tiles64 = ceil_div(p.n, 128) * std::max(active, p.n_rows / 64);
