@@ -11,7 +11,8 @@
 // A row of up to 64 tokens is summed at once.  A longer segment (tokens
 // follow a Zipf law: the first ones occur thousands of times in a batch) is cut
 // at multiples of 64 sorted positions; each chunk sums its part into the
-// workspace and a second launch adds a row's parts in order.
+// workspace, and in a second launch each of four waves adds every fourth of a
+// row's parts, and one the four sums, in a fixed order.
 #include <type_traits>
 
 #include "select_rows.hpp"
@@ -68,7 +69,7 @@ __device__ inline int64_t wave_lower_bound(const uint32_t* __restrict__ keys, in
 // Sum over the positions t0..t1 (held by the lanes) of the rows' slices from
 // element h, in position order, the loads of several rows in flight: six of
 // 16-bit values, for which eight leave registers for 5 waves a SIMD (65536 tokens
-// x 2048, inputs not in cache: 211 and 224 us; sixteen 511), eight of others.
+// x 2048, inputs not in cache: 214 and 224 us; sixteen 549), eight of others.
 template <class V>
 __device__ inline void sum_slices(const V* __restrict__ grad, int64_t ldg, int pos, int t0, int t1, int64_t h,
                                   typename Elem<V>::acc (&acc)[Slice<V>::n]) {
@@ -145,8 +146,8 @@ __device__ inline void sum_rows(const V* __restrict__ grad, int64_t ldg, int pos
 
 // wpr waves share a row (or a chunk), 64 slices each at a time, and go through
 // block_rows rows one after the other.  Bound by the bytes where the table is
-// large: 65536 tokens of a Zipf law, 131072 rows of 2048 bf16, 806 MB, 174 us of
-// the call's 209 (4.6 TB/s; sort 22, join 11); 4095 tokens, 20011 rows of 1001
+// large: 65536 tokens of a Zipf law, 131072 rows of 2048 bf16, 806 MB, 179 us of
+// the call's 213 (4.5 TB/s; sort 22, join 11); 4095 tokens, 20011 rows of 1001
 // float32, 97 MB, 33 us in all (the sort and its zeros, the rows with tokens, join 4).
 // FILLED: rows below `filled` hold zeros already.
 template <class V, class O, bool PAST, bool FILLED>
@@ -309,7 +310,8 @@ extern "C" int fs_embedding(int val_t, int id_t, int64_t n, int64_t n_rows, int6
   if (int rc = check_sizes("fs_embedding", n, n_rows, width)) return rc;
   if (id_t != FS_I32 && id_t != FS_I64) return fail(FS_E_INVALID, "fs_embedding: bad type code");
   if (n == 0 || width == 0) return FS_OK;
-  if ((n_rows > 0 && !table) || !ids || !out || ldt < 0) return fail(FS_E_INVALID, "fs_embedding: bad pointer or stride");
+  if ((n_rows > 0 && !table) || !ids || !out || ldt < 0)
+    return fail(FS_E_INVALID, "fs_embedding: bad pointer or stride");
   return with_value_type(val_t, "fs_embedding", [&](auto v) -> int {
     using V = decltype(v);
     using A = typename Elem<V>::acc;
@@ -365,17 +367,18 @@ extern "C" int fs_embedding_grad(int val_t, int out_t, int id_t, int64_t n, int6
       A* parts = n > 0 ? reinterpret_cast<A*>(w + l.parts) : nullptr;
       const int64_t chunks = n > kLong ? ceil_div(n, kLong) : 0, slices = slices_of<V>(width);
       const int wpr = slices <= 64 ? 1 : slices <= 128 ? 2 : 4;
-      // up to 16 rows, so that workgroups fill the chip: 131072 tokens x 2048 of
-      // 2000 rows, bf16, 206 us with 16, 168 with 4; 65536 of 131072: 238 and 267; of
-      // few tokens, found at once, up to 4: 1 of 262144 x 1024 121 and 105
+      // rows a workgroup, so that workgroups fill the chip (us with 16, 8, 4 and 2: 131072
+      // tokens of 2000 x 2048 bf16 204, 177, 166, 163, 20000 of 8000 x 1024 53, 46, 42, 41,
+      // 65536 of 131072 x 2048 214, 214, 236, 269); of few tokens, found at once, up to 4
+      // (1 of 262144 x 1024 118, 125, 103, 128)
       const int64_t most = n <= 4096 ? 4 : 16;
       const int block_rows = (int)std::min(most, std::max<int64_t>(2, n_rows / (2048 * (4 / wpr))));
       const int64_t chunk_blocks = ceil_div(chunks, 4 / wpr);
       const dim3 grid = row_grid(chunk_blocks + ceil_div(n_rows, (4 / wpr) * block_rows));
       auto launch = [&](auto past, auto some) {
-        hipLaunchKernelGGL((embedding_grad_kernel<V, O, decltype(past)::value, decltype(some)::value>), grid, dim3(256), 0, stream,
-                           (const V*)grad, ldg, keys, order, n, n_rows, width, (A)scale, padding, wpr, block_rows,
-                           chunk_blocks, chunks, filled, (O*)out, parts);
+        hipLaunchKernelGGL((embedding_grad_kernel<V, O, decltype(past)::value, decltype(some)::value>), grid,
+                           dim3(256), 0, stream, (const V*)grad, ldg, keys, order, n, n_rows, width, (A)scale,
+                           padding, wpr, block_rows, chunk_blocks, chunks, filled, (O*)out, parts);
       };
       // past the caches only where a wave's slices leave as whole lines: a 32-bit result
       // of 16-bit values leaves as every second 16 bytes at a time (us so and past the

@@ -52,12 +52,16 @@ struct Mma;
 template <>
 struct Mma<_Float16> {
   using frag = f16x8;
-  __device__ static f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  __device__ static f32x4 run(frag a, frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
 };
 template <>
 struct Mma<__bf16> {
   using frag = bf16x8;
-  __device__ static f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  __device__ static f32x4 run(frag a, frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
 };
 template <>
 struct Mma<float> {
@@ -136,7 +140,10 @@ struct Frags {
   __device__ void read(uint32_t slice, X (&f)[F], int some = F) const {
 #pragma unroll
     for (int j = 0; j < F; ++j)
-      if (j < some) f[j] = O::frag((const lds_byte*)(uintptr_t)(slice + at[KC ? 0 : j]) + (KC ? j * 16 * kRowBytes : 0));
+      if (j < some) {
+        const lds_byte* p = (const lds_byte*)(uintptr_t)(slice + at[KC ? 0 : j]);
+        f[j] = O::frag(p + (KC ? j * 16 * kRowBytes : 0));
+      }
   }
 };
 
@@ -545,9 +552,9 @@ __global__ __launch_bounds__(64 * WM * WN) void expert_product_kernel(const Prod
     for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::run(fb[j], fa[i], acc[i][j]);
   };
   if constexpr (WIDTH != 0) {
-    // Loads are started three steps ahead.  Every wave starts its share of every
-    // step's, also of the three steps past the last (zeros), so that counting
-    // those still under way tells which step has arrived.
+    // Loads are started kAhead steps ahead: three, or one with two slots.  Every
+    // wave starts its share of every step's, also of the kAhead steps past the last
+    // (zeros), so that counting those still under way tells which step has arrived.
     Dma<OA, T, AKC, THREADS, WIDTH> da;
     Dma<OB, T, BKC, THREADS, WIDTH> db;
     constexpr int kLoadsA = da.kLoads, kLoads = da.kLoads + db.kLoads;
@@ -860,7 +867,8 @@ bool may_split(const ProductArgs& p) {
   if (MODE == kMatrix) {
     const int64_t real = ceil_div(p.m, BM) * nt * p.n_experts;
     const uint32_t places = places_of(p.cus, BM);
-    return real <= INT32_MAX && (BM == kLarge || rows >= 2048) && parts_of((uint32_t)real % places, rows / 32, places) > 1;
+    return real <= INT32_MAX && (BM == kLarge || rows >= 2048) &&
+           parts_of((uint32_t)real % places, rows / 32, places) > 1;
   }
   return BM == kLarge && rows >= 112 && p.k >= 1536 && p.n_rows / kLarge * nt < 8 * p.cus;
 }
@@ -893,7 +901,8 @@ int launch_tiles(ProductArgs p, void* ws, size_t ws_bytes, hipStream_t stream) {
   const int64_t tiles = tiles_of<MODE, BM, BN>(p) + (need > 0 ? places_of(p.cus, BM) : 0);
   if (tiles * 64 * WM * WN > INT32_MAX) return fail(FS_E_INVALID, "fs_expert_product: too many tiles");
   auto launch = [&](auto slots, auto past) {
-    hipLaunchKernelGGL((expert_product_kernel<T, MODE, WIDTH, BM, BN, WM, WN, decltype(slots)::value, decltype(past)::value>),
+    hipLaunchKernelGGL((expert_product_kernel<T, MODE, WIDTH, BM, BN, WM, WN, decltype(slots)::value,
+                                              decltype(past)::value>),
                        dim3((uint32_t)tiles), dim3(64 * WM * WN), 0, stream, p);
   };
   using Four = std::integral_constant<int, 4>;
@@ -924,7 +933,8 @@ int launch_few(ProductArgs p, hipStream_t stream) {
   // loads need no registers, 16.0 and 16.4).
   if constexpr (sizeof(T) == 4 || WIDTH == 0) {
     if (2 * ceil_div(p.n, kFewCols) * std::min<int64_t>(p.n_rows, p.n_experts) <= p.cus) {
-      hipLaunchKernelGGL((expert_product_few_kernel<T, MODE, WIDTH, 8>), dim3((uint32_t)tiles), dim3(512), 0, stream, p);
+      hipLaunchKernelGGL((expert_product_few_kernel<T, MODE, WIDTH, 8>), dim3((uint32_t)tiles), dim3(512), 0, stream,
+                         p);
       FS_CHECK_MAIN_LAUNCH("expert_product_few_kernel");
       return FS_OK;
     }
@@ -1029,7 +1039,8 @@ int launch_product(const ProductArgs& p, void* ws, size_t ws_bytes, hipStream_t 
   const int64_t s = sizeof(T), reach = MODE == kMatrix ? kRowBytes / s : kLarge;
   auto whole = [&](int64_t width) {
     const int64_t ends = (MODE == kMatrix ? p.m : p.k) | (MODE == kRowsTrans ? p.k : p.n);
-    return (((int64_t)(uintptr_t)p.a | (int64_t)(uintptr_t)p.b | (p.lda | p.ldb | p.b_expert | ends) * s) & (width - 1)) == 0;
+    const int64_t starts = (int64_t)(uintptr_t)p.a | (int64_t)(uintptr_t)p.b;
+    return ((starts | (p.lda | p.ldb | p.b_expert | ends) * s) & (width - 1)) == 0;
   };
   const bool near = reach * std::max(p.lda, p.ldb) * s < (int64_t)kInBuffer;
   if (near && whole(16)) return launch_product<T, MODE, 16>(p, ws, ws_bytes, stream);

@@ -185,16 +185,18 @@ extern "C" int fs_expert_dispatch(int val_t, int64_t n_tokens, int slots, int64_
   using namespace fs;
   if (int rc = check_rows("fs_expert_dispatch", n_tokens, slots, width, n_experts)) return rc;
   if (n_tokens == 0 || width == 0) return FS_OK;
-  if (!x || !inverse || !offsets || !out || ldx < 0) return fail(FS_E_INVALID, "fs_expert_dispatch: bad pointer or stride");
+  if (!x || !inverse || !offsets || !out || ldx < 0)
+    return fail(FS_E_INVALID, "fs_expert_dispatch: bad pointer or stride");
   return with_value_type(val_t, "fs_expert_dispatch", [&](auto v) -> int {
     using V = decltype(v);
     const int lpr = lanes_per_row(slices_of<V>(width));
     const dim3 grid = row_grid(ceil_div(n_tokens, 256 / lpr));
     auto launch = [&](auto past) {
-      hipLaunchKernelGGL((expert_dispatch_kernel<V, decltype(past)::value>), grid, dim3(256), 0, stream, (const V*)x, ldx, n_tokens,
-                         slots, width, lpr, inverse, offsets + n_experts, (V*)out);
+      hipLaunchKernelGGL((expert_dispatch_kernel<V, decltype(past)::value>), grid, dim3(256), 0, stream,
+                         (const V*)x, ldx, n_tokens, slots, width, lpr, inverse, offsets + n_experts, (V*)out);
     };
-    if (store_past_caches(n_tokens * (slots + 1) * width * (int64_t)sizeof(V), width * sizeof(V))) launch(std::true_type{});
+    const int64_t row_bytes = width * (int64_t)sizeof(V);
+    if (store_past_caches(n_tokens * (slots + 1) * row_bytes, row_bytes)) launch(std::true_type{});
     else launch(std::false_type{});
     FS_CHECK_MAIN_LAUNCH("expert_dispatch_kernel");
     return FS_OK;
@@ -207,17 +209,20 @@ extern "C" int fs_expert_combine(int val_t, int64_t n_tokens, int slots, int64_t
   using namespace fs;
   if (int rc = check_rows("fs_expert_combine", n_tokens, slots, width, n_experts)) return rc;
   if (n_tokens == 0 || width == 0) return FS_OK;
-  if (!rows || !inverse || !offsets || !out || ldr < 0) return fail(FS_E_INVALID, "fs_expert_combine: bad pointer or stride");
+  if (!rows || !inverse || !offsets || !out || ldr < 0)
+    return fail(FS_E_INVALID, "fs_expert_combine: bad pointer or stride");
   return with_value_type(val_t, "fs_expert_combine", [&](auto v) -> int {
     using V = decltype(v);
     using A = typename Elem<V>::acc;
     const int lpr = lanes_per_row(slices_of<V>(width));
     const dim3 grid = row_grid(ceil_div(n_tokens, 256 / lpr));
     auto launch = [&](auto past) {
-      hipLaunchKernelGGL((expert_combine_kernel<V, decltype(past)::value>), grid, dim3(256), 0, stream, (const V*)rows, ldr, n_tokens,
-                         slots, width, lpr, inverse, offsets + n_experts, (const A*)weights, (V*)out);
+      hipLaunchKernelGGL((expert_combine_kernel<V, decltype(past)::value>), grid, dim3(256), 0, stream,
+                         (const V*)rows, ldr, n_tokens, slots, width, lpr, inverse, offsets + n_experts,
+                         (const A*)weights, (V*)out);
     };
-    if (store_past_caches(n_tokens * (slots + 1) * width * (int64_t)sizeof(V), width * sizeof(V))) launch(std::true_type{});
+    const int64_t row_bytes = width * (int64_t)sizeof(V);
+    if (store_past_caches(n_tokens * (slots + 1) * row_bytes, row_bytes)) launch(std::true_type{});
     else launch(std::false_type{});
     FS_CHECK_MAIN_LAUNCH("expert_combine_kernel");
     return FS_OK;

@@ -50,11 +50,13 @@ __device__ inline void store_slice(V* p, const Slice<V>& s) {
 }
 // Whether a call that reads and writes `bytes` in all stores past the caches:
 // where that is more than the Infinity Cache holds, keeping results there only
-// drives out what is still to be read.  us with and without: dispatch 16384 x 8
-// of 2048 bf16 104 and 120, its 4096 tokens 26 and 24; combine 109 and 117;
-// combine_grad 4096 x 4 of 2048 f32 45 and 54; embedding gradient 65536 tokens
-// x 2048, 131072 rows bf16 191 and 239, 512 x 1024, 50000 rows f32 52 and 42.
-// (Rows of whole words: dispatch 2047 wide took 151 and 146.)
+// drives out what is still to be read.  us with and without, inputs not in cache:
+// dispatch 16384 x 8 of 2048 bf16 103 and 110, its 4096 tokens 26 and 23; combine 108
+// and 117; embedding gradient 65536 tokens x 2048, 131072 rows bf16 214 and 228, 512 x
+// 1024, 50000 rows f32 42 and 43.  combine_grad gains where the call before left its
+// inputs in cache and loses where not: 4096 x 4 of 2048 f32 44 and 50, 60 and 51, 8191 x
+// 8 of 2560 f16 134 and 140, 137 and 135, 32768 x 8 of 4096 bf16 869 and 875.
+// (Rows of whole words: dispatch 2047 wide took 148 and 133.)
 inline bool store_past_caches(int64_t bytes, int64_t row_bytes) {
   return bytes >= (int64_t)256 << 20 && row_bytes % 4 == 0;
 }
@@ -92,11 +94,6 @@ __device__ inline uint32_t wave_sum_scan(uint32_t v) {
   v += lane_shifted<0x142, 0xA>(v);  // row_bcast:15 -> rows 1, 3
   v += lane_shifted<0x143, 0xC>(v);  // row_bcast:31 -> rows 2, 3
   return v;
-}
-
-// Whether rows `ld_bytes` apart all start at multiples of 16 bytes.
-inline bool aligned16(const void* p, int64_t ld_bytes) {
-  return ((uintptr_t)p & 15) == 0 && (ld_bytes & 15) == 0;
 }
 
 // Threads of a workgroup of 256 that share a row of `slices` slices.

@@ -591,9 +591,12 @@ int fs_embedding(int val_t, int id_t, int64_t n, int64_t n_rows, int64_t width,
                  const void* table, int64_t ldt, const void* ids, double scale,
                  void* out, hipStream_t stream);
 /*
- * Its gradient: out[v] = scale * (sum of grad[t] over ids[t] == v, in order of
- * t), every row of out written; row `padding` (-1: none) is zero.  out_t is
- * val_t, or FS_F32 for 16-bit values.
+ * Its gradient: out[v] = scale * (sum of grad[t] over ids[t] == v), every row of
+ * out written; row `padding` (-1: none) and rows that no id names are zero
+ * whatever the scale.  Up to 64 ids of a row are added in order of t, more in
+ * groups that end at multiples of 64 sorted positions, every fourth group after
+ * the other and the four sums at last: the same from run to run.  out_t is val_t,
+ * or FS_F32 for 16-bit values.
  */
 size_t fs_embedding_grad_workspace_bytes(int val_t, int64_t n, int64_t n_rows, int64_t width);
 int fs_embedding_grad(int val_t, int out_t, int id_t, int64_t n, int64_t n_rows, int64_t width,

@@ -33,11 +33,13 @@ def _route(n_tokens, slots=1, experts=2):
 def test_product_operand_with_a_gradient_may_change(launched, changed):
     rows, matrices = torch.ones(4, 8), torch.ones(2, 8, 8)
     t = (rows if changed == "rows" else matrices).requires_grad_() * 1.0
-    out = fs.flagsparse_expert_product(t if changed == "rows" else rows, t if changed == "matrices" else matrices, _route(4))
+    operands = (t, matrices) if changed == "rows" else (rows, t)
+    out = fs.flagsparse_expert_product(*operands, _route(4))
     t.mul_(2.0)
     out.sum().backward()  # reads the other one
     names = [name for name, _ in launched if not name.endswith("bytes")]
-    assert names == ["fs_expert_product", "fs_expert_product" if changed == "rows" else "fs_expert_product_grad_matrices"]
+    assert names == ["fs_expert_product",
+                     "fs_expert_product" if changed == "rows" else "fs_expert_product_grad_matrices"]
 
 
 def test_combine_operand_with_a_gradient_may_change(launched):
@@ -46,7 +48,8 @@ def test_combine_operand_with_a_gradient_may_change(launched):
     for changed in ("rows", "weights"):
         rows, weights = torch.ones(8, 8), torch.ones(4, 2)
         t = (rows if changed == "rows" else weights).requires_grad_() * 1.0
-        out = fs.flagsparse_expert_combine(t if changed == "rows" else rows, route, t if changed == "weights" else weights)
+        operands = (t, route, weights) if changed == "rows" else (rows, route, t)
+        out = fs.flagsparse_expert_combine(*operands)
         t.mul_(2.0)
         out.sum().backward()
         (_, _), (name, args) = launched

@@ -32,10 +32,10 @@ def _tokens(n, n_rows, seed):
 
 # gradient type, result type, width (rows of whole words that end off 16 bytes, and one that does not), tokens: after
 # a longer sort, and beside zeros that end inside the table
-@pytest.mark.parametrize("dtype,out,width", [(torch.float32, torch.float32, 1003), (torch.float16, torch.float32, 1003),
-                                             (torch.bfloat16, torch.float32, 520), (torch.bfloat16, torch.bfloat16, 1002),
-                                             (torch.float16, torch.float16, 2040), (torch.float64, torch.float64, 501),
-                                             (torch.float16, torch.float16, 1001)], ids=str)
+@pytest.mark.parametrize("dtype,out,width", [
+    (torch.float32, torch.float32, 1003), (torch.float16, torch.float32, 1003), (torch.bfloat16, torch.float32, 520),
+    (torch.bfloat16, torch.bfloat16, 1002), (torch.float16, torch.float16, 2040), (torch.float64, torch.float64, 501),
+    (torch.float16, torch.float16, 1001)], ids=str)
 @pytest.mark.parametrize("n", [3000, 20000])
 def test_gradient_past_the_caches(dtype, out, width, n):
     size = torch.empty(0, dtype=out).element_size()
