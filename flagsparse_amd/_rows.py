@@ -27,9 +27,14 @@ def row_major(t, width):
 recording = torch.is_grad_enabled
 
 
+def tangents():
+    """Whether operands may have forward-mode tangents."""
+    return forward_ad._current_level >= 0
+
+
 def refuse_tangent(t, what):
     """The kernels would drop a forward-mode tangent without a word."""
-    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+    if forward_ad.unpack_dual(t).tangent is not None:
         raise NotImplementedError(f"{what} has a forward-mode tangent, which this operator does not propagate")
 
 
@@ -49,24 +54,21 @@ def _span(t):
     return start, start + (last + 1) * t.element_size()
 
 
-def into(out, shape, like, *operands, dtype=None):
+def into(out, *operands):
     """The tensor that a kernel writes: ``out`` itself where it is contiguous and
     shares no memory with an operand, which other workgroups would still read; a
-    new one, of ``dtype`` or ``like``'s, otherwise (``done`` copies it)."""
-    if out is not None and out.is_contiguous():
+    new one otherwise (``done`` copies it)."""
+    if out.is_contiguous():
         first, end = _span(out)
         spans = (_span(t) for t in operands if t is not None)
         if not any(first < b and a < end for a, b in spans):
             return out
-    return like.new_empty(shape, dtype=dtype)
+    return out.new_empty(out.shape)
 
 
 def done(out, result):
-    """The result of a call: ``out``, with the result in it, where one was given.
-    Autograd learns of the write, so a backward pass that still needs what ``out``
-    held raises."""
-    if out is None:
-        return result
+    """``out``, with the result in it.  Autograd learns of the write, so a backward
+    pass that still needs what ``out`` held raises."""
     if result is out:
         torch.autograd.graph.increment_version(out)
     else:

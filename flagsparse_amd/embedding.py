@@ -29,6 +29,7 @@ from ._rows import (
     recording,
     refuse_tangent,
     row_major,
+    tangents,
 )
 
 
@@ -43,7 +44,8 @@ def _check_tokens(tokens, values, what):
         raise ValueError(f"{what} and tokens must be CUDA tensors")
     if values.device != tokens.device:
         raise ValueError(f"{what} and tokens must be on the same CUDA device")
-    refuse_tangent(values, what)
+    if tangents():
+        refuse_tangent(values, what)
 
 
 def _normalize_padding(padding_idx, n_rows):
@@ -60,10 +62,10 @@ def _lookup(table, tokens, scale, out=None):
     table, ld = row_major(table, width)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
-    result = into(out, (*tokens.shape, width), table, table, tokens)
+    result = table.new_empty((*tokens.shape, width)) if out is None else into(out, table, tokens)
     launch(_lib.lib().fs_embedding, table.device, ROW_VALUE_CODES[table.dtype], _lib.INDEX_TYPE_CODES[tokens.dtype],
            tokens.numel(), n_rows, width, table.data_ptr(), ld, tokens.data_ptr(), scale, result.data_ptr())
-    return done(out, result)
+    return result if out is None else done(out, result)
 
 
 class _Embedding(torch.autograd.Function):
@@ -124,14 +126,14 @@ def flagsparse_embedding_grad(grad, tokens, num_rows, scale=1.0, padding_idx=Non
         check_out(out, grad.device, (num_rows, width), dtype)
     grad, ld = row_major(grad.reshape(n, width), width)
     tokens = tokens.contiguous()
-    result = into(out, (num_rows, width), grad, grad, tokens, dtype=dtype)
+    result = grad.new_empty((num_rows, width), dtype=dtype) if out is None else into(out, grad, tokens)
     code = ROW_VALUE_CODES[grad.dtype]
     lib = _lib.lib()
     ws = _lib.workspace(lib.fs_embedding_grad_workspace_bytes(code, n, num_rows, width), grad.device)
     launch(lib.fs_embedding_grad, grad.device, code, ROW_VALUE_CODES[dtype], _lib.INDEX_TYPE_CODES[tokens.dtype], n,
            num_rows, width, grad.data_ptr(), ld, tokens.data_ptr(), float(scale), padding, result.data_ptr(),
            ws.data_ptr(), ws.numel())
-    return done(out, result)
+    return result if out is None else done(out, result)
 
 
 __all__ = ["flagsparse_embedding", "flagsparse_embedding_grad"]

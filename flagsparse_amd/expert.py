@@ -33,10 +33,10 @@ from ._rows import (
     check_out,
     done,
     into,
-    launch,
     recording,
     refuse_tangent,
     row_major,
+    tangents,
 )
 from .spmm_csr import _normalize_spmm_op, _spmm_op_transposes
 
@@ -55,7 +55,7 @@ class PreparedExpertRoute:
     __slots__ = ("n_tokens", "slots", "num_experts", "n_rows", "device", "_places", "_inverse_ptr", "_offsets_ptr",
                  "_stream")
 
-    def __init__(self, n_tokens, slots, num_experts, places):
+    def __init__(self, n_tokens, slots, num_experts, places, stream):
         n = n_tokens * slots
         self.n_tokens, self.slots, self.num_experts, self.n_rows = n_tokens, slots, num_experts, n
         self.device = places.device
@@ -64,7 +64,7 @@ class PreparedExpertRoute:
         self._places = places
         start = places.data_ptr()
         self._inverse_ptr, self._offsets_ptr = start + 4 * n, start + 8 * n
-        self._stream = _lib.stream_handle(self.device)
+        self._stream = stream  # the handle of the one that writes the places
 
     @property
     def order(self):
@@ -104,10 +104,13 @@ def prepare_expert_route(experts, num_experts):
     need = lib.fs_expert_route_workspace_bytes(n, num_experts)
     scratch = (2 * n + num_experts + 64) // 64 * 64  # 256-byte boundary behind the places
     places = torch.empty(scratch + (need + 3) // 4, dtype=torch.int32, device=device)
-    route = PreparedExpertRoute(n_tokens, slots, num_experts, places)
+    stream = _lib.stream_handle(device)
+    route = PreparedExpertRoute(n_tokens, slots, num_experts, places, stream)
     start = places.data_ptr()
-    launch(lib.fs_expert_route, device, _lib.INDEX_TYPE_CODES[experts.dtype], n, num_experts, experts.data_ptr(), start,
-           route._inverse_ptr, route._offsets_ptr, start + 4 * scratch, need)
+    rc = lib.fs_expert_route(_lib.INDEX_TYPE_CODES[experts.dtype], n, num_experts, experts.data_ptr(), start,
+                             route._inverse_ptr, route._offsets_ptr, start + 4 * scratch, need, stream)
+    if rc:
+        _lib.check(rc, "fs_expert_route")
     return route
 
 
@@ -124,7 +127,8 @@ def _check_rows(rows, what, route, n_rows):
         raise ValueError(f"{what} must be on the same CUDA device as the route")
     if rows.ndim != 2 or rows.shape[0] != n_rows:
         raise ValueError(f"{what} must be a 2D tensor with {n_rows} rows, got shape {tuple(rows.shape)}")
-    refuse_tangent(rows, what)
+    if tangents():
+        refuse_tangent(rows, what)
 
 
 def _check_weights(weights, rows, route):
@@ -137,7 +141,8 @@ def _check_weights(weights, rows, route):
         raise ValueError("weights must be on the same CUDA device as the route")
     if weights.shape != (route.n_tokens, route.slots):
         raise ValueError(f"weights must have shape {(route.n_tokens, route.slots)}, got {tuple(weights.shape)}")
-    refuse_tangent(weights, "weights")
+    if tangents():
+        refuse_tangent(weights, "weights")
 
 
 def _launch(function, route, *args):
@@ -155,10 +160,10 @@ def _launch(function, route, *args):
 def _dispatch(x, route, out=None):
     width = x.shape[1]
     x, ld = row_major(x, width)
-    result = into(out, (route.n_rows, width), x, x)
+    result = x.new_empty((route.n_rows, width)) if out is None else into(out, x)
     _launch(_lib.lib().fs_expert_dispatch, route, ROW_VALUE_CODES[x.dtype], route.n_tokens, route.slots, width,
            route.num_experts, x.data_ptr(), ld, route._inverse_ptr, route._offsets_ptr, result.data_ptr())
-    return done(out, result)
+    return result if out is None else done(out, result)
 
 
 def _combine(rows, route, weights, out=None):
@@ -166,11 +171,11 @@ def _combine(rows, route, weights, out=None):
     rows, ld = row_major(rows, width)
     if weights is not None and not weights.is_contiguous():
         weights = weights.contiguous()
-    result = into(out, (route.n_tokens, width), rows, rows, weights)
+    result = rows.new_empty((route.n_tokens, width)) if out is None else into(out, rows, weights)
     _launch(_lib.lib().fs_expert_combine, route, ROW_VALUE_CODES[rows.dtype], route.n_tokens, route.slots, width,
            route.num_experts, rows.data_ptr(), ld, route._inverse_ptr, route._offsets_ptr,
            None if weights is None else weights.data_ptr(), result.data_ptr())
-    return done(out, result)
+    return result if out is None else done(out, result)
 
 
 def _combine_grad(grad, rows, route, weights):
@@ -302,7 +307,8 @@ def _check_product(rows, matrices, route, op):
     if matrices.ndim != 3 or matrices.shape[0] != route.num_experts:
         raise ValueError(f"matrices must be a 3D tensor with {route.num_experts} matrices, got shape "
                          f"{tuple(matrices.shape)}")
-    refuse_tangent(matrices, "matrices")
+    if tangents():
+        refuse_tangent(matrices, "matrices")
     trans = _spmm_op_transposes(_normalize_spmm_op(op))
     inner, outer = matrices.shape[2 if trans else 1], matrices.shape[1 if trans else 2]
     if rows.shape[1] != inner:
@@ -323,14 +329,14 @@ def _dense_matrices(matrices, trans):
 def _product(rows, matrices, route, trans, inner, outer, out=None):
     rows, ld = row_major(rows, inner)
     matrices, trans = _dense_matrices(matrices, trans)
-    result = into(out, (route.n_rows, outer), rows, rows, matrices)
+    result = rows.new_empty((route.n_rows, outer)) if out is None else into(out, rows, matrices)
     lib = _lib.lib()
     sizes = (ROW_VALUE_CODES[rows.dtype], int(trans), route.n_rows, route.num_experts, inner, outer)
     need = lib.fs_expert_product_workspace_bytes(*sizes)
     ws = _lib.workspace(need, rows.device) if need else None
     _launch(lib.fs_expert_product, route, *sizes, rows.data_ptr(), ld, matrices.data_ptr(), route._offsets_ptr,
            result.data_ptr(), _lib.ptr(ws), need)
-    return done(out, result)
+    return result if out is None else done(out, result)
 
 
 def _product_grad_matrices(grad, rows, route, trans, inner, outer):

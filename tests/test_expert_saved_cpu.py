@@ -26,7 +26,7 @@ def launched(monkeypatch):
 
 def _route(n_tokens, slots=1, experts=2):
     n = n_tokens * slots
-    return PreparedExpertRoute(n_tokens, slots, experts, torch.zeros(2 * n + experts + 1, dtype=torch.int32))
+    return PreparedExpertRoute(n_tokens, slots, experts, torch.zeros(2 * n + experts + 1, dtype=torch.int32), 11)
 
 
 @pytest.mark.parametrize("changed", ["rows", "matrices"])

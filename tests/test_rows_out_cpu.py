@@ -41,7 +41,7 @@ def written(monkeypatch):
 
 def _route(n_tokens, slots=1, experts=2):
     n = n_tokens * slots
-    return expert.PreparedExpertRoute(n_tokens, slots, experts, torch.zeros(2 * n + experts + 1, dtype=torch.int32))
+    return expert.PreparedExpertRoute(n_tokens, slots, experts, torch.zeros(2 * n + experts + 1, dtype=torch.int32), 11)
 
 
 def _calls(x, out, tokens):

@@ -26,7 +26,7 @@ def launched(monkeypatch):
 
 
 def test_tangents_are_refused(launched):
-    tokens, route = torch.arange(4), PreparedExpertRoute(4, 1, 2, torch.zeros(11, dtype=torch.int32))
+    tokens, route = torch.arange(4), PreparedExpertRoute(4, 1, 2, torch.zeros(11, dtype=torch.int32), 11)
     x, w, m = torch.ones(4, 8), torch.ones(4, 1), torch.ones(2, 8, 8)
     calls = {
         "table": lambda t: fs.flagsparse_embedding(t(x), tokens),
