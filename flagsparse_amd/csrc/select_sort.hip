@@ -16,7 +16,7 @@
 //
 // Bound by launches and the latency of their steps, not by bytes: us, 64 x 8 slots
 // of 64 experts 5 (one launch), 131072 x 8 of 128 18 (16.8 MB; three launches),
-// 4095 tokens of 20011 13 (one launch), 65536 of 131072 20 (four).
+// 4095 tokens of 20011 13 (one launch), 65536 of 131072 22 (four).
 #include <type_traits>
 
 #include "radix_tile.hpp"

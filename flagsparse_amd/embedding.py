@@ -9,7 +9,8 @@ and 32-bit values are scaled and summed in float32 and rounded once.  Tokens:
 int32 or int64 of any shape.  A token outside [0, rows of the table) reads
 nothing: its result row is zero and its gradient goes nowhere (a process that
 holds a part of the vocabulary subtracts its first row from the tokens).
-Nothing synchronises, and sums run in a fixed order.
+Nothing synchronises, and sums run in a fixed order.  ``out`` may share memory
+with an operand.
 
 The reference has no counterpart; names, checks and errors follow its other
 operators (sparse_operations/spmm_coo.py:335-395, 619-625).
@@ -86,7 +87,7 @@ def flagsparse_embedding(table, tokens, scale=1.0, padding_idx=None, out=None):
     """scale * table[tokens]: tokens.shape + (width,), in the table's type.
 
     table is (rows, width).  padding_idx names a row whose gradient is zero
-    (the lookup reads it as any other).  Differentiable in `table`; `out`
+    (the lookup reads it as any other).  Differentiable once in `table`; `out`
     cannot be given then.
     """
     _check_tokens(tokens, table, "table")
@@ -109,7 +110,7 @@ def flagsparse_embedding_grad(grad, tokens, num_rows, scale=1.0, padding_idx=Non
 
     grad is tokens.shape + (width,).  dtype is the result's: grad's own, or
     float32 for 16-bit grad.  Rows that no token names, and padding_idx, are
-    zero.
+    zero.  Records no graph.
     """
     _check_tokens(tokens, grad, "grad")
     if grad.ndim != tokens.ndim + 1 or grad.shape[:-1] != tokens.shape:

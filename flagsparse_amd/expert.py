@@ -17,7 +17,9 @@ Products with the routing matrix, with a block-diagonal matrix and with the
 routing matrix's transpose (csrc/select_sort.hip, expert_rows.hip,
 expert_product.hip).  Values: float16, bfloat16, float32 (float64 too but for
 the product); sums run in 32 bits (64 for float64), in a fixed order, and are
-rounded once.  Routing weights are float32 (float64 with float64 rows).
+rounded once.  Routing weights are float32 (float64 with float64 rows).  The
+forward calls are differentiable once; the gradients called by name record no
+graph.  ``out`` may share memory with an operand.
 
 The reference has no counterpart; names, checks and errors follow its other
 operators (sparse_operations/spmm_coo.py:335-395, 619-625).
@@ -50,6 +52,9 @@ class PreparedExpertRoute:
     inverse   int32 (T, k): place of each slot
     offsets   int32 (num_experts + 1,): first place of each expert; the last is
               the number of slots that name one
+
+    It may be dropped while calls that use it are queued, on any stream; calls on
+    other streams than its own have to be ordered behind its preparation.
     """
 
     __slots__ = ("n_tokens", "slots", "num_experts", "n_rows", "device", "_places", "_inverse_ptr", "_offsets_ptr",

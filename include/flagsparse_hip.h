@@ -579,8 +579,8 @@ int fs_spmv_sell(int val_t, int sell_idx_t, int ptr_t, int layout, int64_t n_row
  * The reference has no counterpart of the entry points below.  Their value
  * types are FS_F16, FS_BF16, FS_F32 and FS_F64; sums run in 32 bits (64 for
  * FS_F64) in a fixed order and are rounded once.  Rows are contiguous; ld*
- * is the distance between rows in elements, results are dense.  Nothing
- * synchronises.
+ * is the distance between rows in elements, results are dense and share no
+ * memory with an operand.  Nothing synchronises.
  */
 
 /*
