@@ -68,6 +68,14 @@ from .alpha_spmm import (
     prepare_alpha_spmm_alg1_tle_opt,
     prepare_alpha_spmm_alg1_tle_opt2,
 )
+from .blocks import (
+    PreparedBlockSequences,
+    flagsparse_block_attention,
+    flagsparse_block_attention_grad,
+    flagsparse_block_means,
+    flagsparse_block_select,
+    prepare_block_sequences,
+)
 from .embedding import flagsparse_embedding, flagsparse_embedding_grad
 from .expert import (
     PreparedExpertRoute,

@@ -106,6 +106,12 @@ EXPORTED_SYMBOLS = (
     "fs_expert_product",
     "fs_expert_product_grad_matrices_workspace_bytes",
     "fs_expert_product_grad_matrices",
+    "fs_block_means",
+    "fs_block_select",
+    "fs_block_attention_workspace_bytes",
+    "fs_block_attention",
+    "fs_block_attention_grad_workspace_bytes",
+    "fs_block_attention_grad",
 )
 
 
@@ -130,6 +136,27 @@ class FsCsrPlan(ctypes.Structure):
         ("hist", ctypes.c_int64 * FS_HIST_BINS),
         ("part_bytes", ctypes.c_size_t),
         ("carry_bytes", ctypes.c_size_t),
+    ]
+
+
+class FsBlockSeqs(ctypes.Structure):
+    """Mirror of struct fs_block_seqs."""
+
+    _fields_ = [
+        ("n_seqs", ctypes.c_int64),
+        ("n_tokens", ctypes.c_int64),
+        ("n_rows", ctypes.c_int64),
+        ("q_offsets", ctypes.c_void_p),
+        ("k_offsets", ctypes.c_void_p),
+        ("k_lengths", ctypes.c_void_p),
+        ("pages", ctypes.c_void_p),
+        ("ld_pages", ctypes.c_int64),
+        ("pages_per_seq", ctypes.c_int64),
+        ("n_pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int32),
+        ("page_shift", ctypes.c_int32),
+        ("block", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
     ]
 
 
@@ -294,6 +321,22 @@ def _declare(lib):
     lib.fs_expert_product_grad_matrices.restype = _i32
     lib.fs_expert_product_grad_matrices.argtypes = [_i32, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp,
                                                     _vp, _sz, _vp]
+    lib.fs_block_means.restype = _i32
+    lib.fs_block_means.argtypes = [_i32, _vp, _i32, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp]
+    lib.fs_block_select.restype = _i32
+    lib.fs_block_select.argtypes = [_i32, _vp, _i32, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32,
+                                    _i32, _i32, _vp, _vp]
+    lib.fs_block_attention_workspace_bytes.restype = _sz
+    lib.fs_block_attention_workspace_bytes.argtypes = [_i32, _vp, _i32, _i32, _i32, _i32]
+    lib.fs_block_attention.restype = _i32
+    lib.fs_block_attention.argtypes = [_i32, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp,
+                                       _i64, _i64, _i64, _vp, _i64, _i64, _f64, _vp, _vp, _vp, _sz, _vp]
+    lib.fs_block_attention_grad_workspace_bytes.restype = _sz
+    lib.fs_block_attention_grad_workspace_bytes.argtypes = [_i32, _vp, _i32, _i32, _i32, _i32, _i32]
+    lib.fs_block_attention_grad.restype = _i32
+    lib.fs_block_attention_grad.argtypes = [_i32, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _i64, _vp, _i64,
+                                            _i64, _vp, _i64, _i64, _vp, _i64, _i64, _f64, _vp, _vp, _vp, _vp, _vp, _vp,
+                                            _sz, _vp]
     lib.fs_last_kernel.restype = ctypes.c_char_p
     lib.fs_last_kernel.argtypes = []
 

@@ -1,0 +1,561 @@
+// block_attention.hip — attention over the blocks of keys that each query selects.
+//
+//   out[t, h] = sum over j of softmax_j(scale <q[t, h], k[j]>) v[j]
+// over the keys j of the blocks that blocks[t, h / group] names, up to the query's
+// own position: a product of dense matrices sampled where the selection is, a softmax
+// along its rows, and the sparse matrix so made times the values, in one pass with the
+// running maximum and sum of each row.  A block named twice counts once.
+#include "block_walk.hpp"
+
+namespace fs {
+namespace {
+
+template <class T, int DP>
+struct Online {
+  typename Mma<T>::frag q[2][Rows<T, DP>::kFrags];
+  f32x4 o[2][DP / 16];  // columns 16 dt + 4 g .. of the lane's row
+  float m[2], l[2];     // maximum in powers of two, and the lane's own part of the sum
+};
+
+template <class T, int DP>
+__device__ inline void start(Online<T, DP>& st) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    st.m[i] = -INFINITY;
+    st.l[i] = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt) st.o[i][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+}
+
+// One step's keys and values taken into tiles 0 (A) and 1 (B).
+template <class T, int DP, bool A, bool B>
+__device__ inline void attend(Online<T, DP>& st, uint32_t kb, uint32_t vb,
+                              const bool (&sel)[2][Rows<T, DP>::kGroups],
+                              const int (&first)[Rows<T, DP>::kGroups], bool edge, uint32_t missing,
+                              const RowOf (&row)[2], float c, int lane) {
+  using R = Rows<T, DP>;
+  constexpr int G = R::kGroups, P = R::kUnit / 16;
+  f32x4 s[2][G];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr) s[i][gr] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int ks = 0; ks < R::kFrags; ++ks)
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr) {
+      const auto k = R::across(kb, gr * 16, ks, lane);
+      if (A) s[0][gr] = Mma<T>::run(k, st.q[0][ks], s[0][gr]);
+      if (B) s[1][gr] = Mma<T>::run(k, st.q[1][ks], s[1][gr]);
+    }
+  typename R::frag w[2][G / P];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (i == 0 ? !A : !B) continue;
+    float most = -INFINITY;
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        bool in = sel[i][gr];
+        if (edge) in = in && first[gr] + 4 * (lane >> 4) + r <= row[i].pos && !((missing >> gr) & 1u);
+        s[i][gr][r] = in ? s[i][gr][r] : -INFINITY;
+        most = fmaxf(most, s[i][gr][r]);
+      }
+    const float m = fmaxf(st.m[i], across_max(most) * c);
+    const float base = m == -INFINITY ? 0.0f : m;  // (a row without keys yet)
+    if (__ballot(m != st.m[i]) != 0) {
+      const float by = __builtin_amdgcn_exp2f(st.m[i] - base);
+      st.l[i] *= by;
+#pragma unroll
+      for (int dt = 0; dt < DP / 16; ++dt) st.o[i][dt] *= by;
+      st.m[i] = m;
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][gr][r], c, -base));
+        sum += x;
+        s[i][gr][r] = x;
+      }
+    st.l[i] += sum;
+    // weights, in [0, 1], in the values' type: off by half a unit in their last place
+    // each, the sum that they are divided by is not
+#pragma unroll
+    for (int u = 0; u < G / P; ++u) w[i][u] = R::rounded(&s[i][u * P]);
+  }
+#pragma unroll
+  for (int u = 0; u < G / P; ++u)
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt) {
+      const auto v = R::down(vb, u * R::kUnit, dt, lane);
+      if (A) st.o[0][dt] = Mma<T>::run(v, w[0][u], st.o[0][dt]);
+      if (B) st.o[1][dt] = Mma<T>::run(v, w[1][u], st.o[1][dt]);
+    }
+}
+
+// One row by a wave, key after key, without products of what is left out: a weight
+// of zero times a value that is not finite would be NaN.  Taken where a result is
+// not finite, whoever's it is.
+template <class T, int DP>
+__device__ __noinline__ void careful_row(const BlockArgs& p, const Sequence& sq, int seq, int64_t token, int head,
+                                         int in_group, int pos, int lane) {
+  const int hq = head * p.group + in_group, block = p.seqs.block, lg = p.lg_groups + 4;
+  const T* q = static_cast<const T*>(p.q) + token * p.q_token + (int64_t)hq * p.q_head;
+  const int32_t* ids = p.blocks + token * p.b_token + (int64_t)head * p.b_head;
+  const float c = p.scale * kLog2e;
+  float m = -INFINITY, l = 0.0f, o[(DP + 63) / 64];
+#pragma unroll
+  for (int i = 0; i < (DP + 63) / 64; ++i) o[i] = 0.0f;
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int e = 0; e < p.top; ++e) {
+      const int id = ids[e];
+      bool use = id >= 0 && id <= (pos >> lg);
+      for (int b = 0; b < e; ++b) use = use && ids[b] != id;
+      if (!use) continue;
+      for (int j0 = 0; j0 < block; j0 += 64) {
+        const int j = id * block + j0 + lane;
+        bool seen = j0 + lane < block && j <= pos && j < sq.keys;
+        float s = -INFINITY;
+        if (seen) {
+          const T* k = key_rows<T>(p.seqs, sq, seq, p.k, head, j & ~15);
+          seen = k != nullptr;
+          if (seen) {
+            k += (int64_t)(j & 15) * p.k.row;
+            s = 0.0f;
+            for (int d = 0; d < p.width; ++d) s = __builtin_fmaf((float)q[d], (float)k[d], s);
+          }
+        }
+        if (pass == 0) {
+          m = fmaxf(m, s);
+          continue;
+        }
+        const float w = seen ? __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -m)) : 0.0f;
+        l += w;
+        for (uint64_t left = __ballot(seen); left != 0; left &= left - 1) {
+          const int at = __builtin_ctzll(left), jj = id * block + j0 + at;
+          const float weight = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(w), at));
+          const T* v = key_rows<T>(p.seqs, sq, seq, p.v, head, jj & ~15) + (int64_t)(jj & 15) * p.v.row;
+#pragma unroll
+          for (int i = 0; i < (DP + 63) / 64; ++i)
+            if (i * 64 + lane < p.width) o[i] = __builtin_fmaf(weight, (float)v[i * 64 + lane], o[i]);
+        }
+      }
+    }
+    if (pass == 0) {
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+      m = m == -INFINITY ? 0.0f : m * c;
+    }
+  }
+  l = wave_sum(l);
+  const int64_t at = token * p.heads * p.group + hq;
+  T* out = static_cast<T*>(p.out) + at * p.width;
+#pragma unroll
+  for (int i = 0; i < (DP + 63) / 64; ++i)
+    if (i * 64 + lane < p.width) out[i * 64 + lane] = (T)(l == 0.0f ? 0.0f : o[i] / l);
+  if (p.lse != nullptr && lane == 0) p.lse[at] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * kLn2;
+}
+
+// Many queries.
+template <class T, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void block_attention_kernel(const BlockArgs p) {
+  using R = Rows<T, DP>;
+  __shared__ alignas(1024) uint8_t s_kv[2][2][R::kBytes];
+  __shared__ WalkMemory<WAVES> s_walk;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  WalkTile t;
+  if (!walk_tile<WAVES>(p, lane, t)) return;
+  RowOf row[2];
+  rows_of<WAVES>(p, t, w, lane, row);
+  Online<T, DP> st;
+  start(st);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    load_row<T, DP>(static_cast<const T*>(p.q) + (int64_t)(t.token0 + row[i].token) * p.q_token +
+                        (int64_t)(t.head * p.group + row[i].head) * p.q_head,
+                    row[i].in, p.width, lane, st.q[i]);
+  const float c = p.scale * kLog2e;
+  walk_blocks<T, DP, WAVES>(
+      p, t, row, s_walk, s_kv, tid, w, lane,
+      [&](const Step<T, DP>& now, const bool(&sel)[2][R::kGroups], bool a, bool b, bool edge, uint32_t kb, uint32_t vb) {
+        if (a && b) attend<T, DP, true, true>(st, kb, vb, sel, now.first, edge, now.missing, row, c, lane);
+        else if (a) attend<T, DP, true, false>(st, kb, vb, sel, now.first, edge, now.missing, row, c, lane);
+        else attend<T, DP, false, true>(st, kb, vb, sel, now.first, edge, now.missing, row, c, lane);
+      });
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float l = across_sum(st.l[i]), by = l > 0.0f ? 1.0f / l : 0.0f;
+    bool bad = !__builtin_isfinite(l);
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bad |= !__builtin_isfinite(st.o[i][dt][r]);
+    uint64_t rows = __ballot(bad && row[i].in);
+    rows = (rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xffffu;
+    const int64_t at = (int64_t)(t.token0 + row[i].token) * p.heads * p.group + t.head * p.group + row[i].head;
+    if (row[i].in && !((rows >> (lane & 15)) & 1)) {
+      store_row<T, DP>(static_cast<T*>(p.out) + at * p.width, st.o[i], by, p.width, lane);
+      if (p.lse != nullptr && lane < 16) p.lse[at] = l > 0.0f ? (st.m[i] + __builtin_log2f(l)) * kLn2 : -INFINITY;
+    }
+    for (; rows != 0; rows &= rows - 1) {
+      const int r = __builtin_ctzll(rows), tok = __builtin_amdgcn_readlane(row[i].token, r);
+      careful_row<T, DP>(p, t.sq, t.seq, t.token0 + tok, t.head, __builtin_amdgcn_readlane(row[i].head, r),
+                         t.pos0 + tok, lane);
+    }
+  }
+}
+
+// Few queries: a workgroup takes one token's rows of a group, up to 32 of them, and
+// its waves the steps of the token's own blocks in turn, each with keys and values of
+// its own in LDS; their states are joined at the end, with `splits` workgroups a
+// token those by the next kernel.
+constexpr int kFewWaves = 4;
+
+template <class T, int DP>
+struct FewShape {
+  static constexpr int kWaves = DP * (int)sizeof(T) > 256 ? 2 : kFewWaves;
+};
+// (floats of a split's part: maximum and sum of 32 rows, then the rows)
+template <int DP>
+__host__ __device__ constexpr int part_floats() { return 64 + 32 * DP; }
+
+struct FewPlace {
+  int64_t token;
+  int head, chunk, split;
+};
+__device__ inline FewPlace few_place(const BlockArgs& p, int64_t at) {
+  FewPlace f;
+  f.split = (int)(at % p.splits);
+  at /= p.splits;
+  const int chunks = (p.group + 31) / 32;
+  f.chunk = (int)(at % chunks);
+  at /= chunks;
+  f.head = (int)(at % p.heads);
+  f.token = at / p.heads;
+  return f;
+}
+// Sequence and position of a token; false: of none.
+__device__ inline bool token_at(const fs_block_seqs& s, int64_t token, int lane, int& seq, Sequence& sq, int& pos) {
+  if (s.q_offsets == nullptr) {
+    seq = (int)token;
+  } else {
+    seq = (int)s.n_seqs;
+    for (int64_t b0 = 0; b0 < s.n_seqs; b0 += 64) {
+      const int64_t b = b0 + lane;
+      bool mine = false;
+      if (b < s.n_seqs) {
+        const Sequence q = sequence_at(s, (int)b);
+        mine = token >= q.first && token < q.first + q.count;
+      }
+      const uint64_t m = __ballot(mine);
+      if (m != 0) {
+        seq = (int)b0 + __builtin_ctzll(m);
+        break;
+      }
+    }
+  }
+  if (seq >= s.n_seqs) return false;
+  sq = sequence_at(s, seq);
+  pos = sq.keys - sq.count + (int)(token - sq.first);
+  return true;
+}
+
+// Rows of one token and chunk from the states of `n` waves or splits: part(i) gives
+// the i-th one's 32 maxima, 32 sums and 32 rows.
+template <class T, int DP, int THREADS, class Part>
+__device__ inline void join_rows(const BlockArgs& p, const FewPlace& f, int seq, const Sequence& sq, int pos, int n,
+                                 int tid, int* s_bad, Part part) {
+  const int rows = p.group - f.chunk * 32 < 32 ? p.group - f.chunk * 32 : 32;
+  const int fours = p.width / 4;
+  int any = 0;
+  if (tid < 32) s_bad[tid] = 0;
+  __syncthreads();
+  for (int e = tid; e < rows * fours; e += THREADS) {
+    const int r = e / fours, d = (e - r * fours) * 4;
+    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < n; ++i) m = fmaxf(m, part(i)[r]);
+    const float base = m == -INFINITY ? 0.0f : m;
+    for (int i = 0; i < n; ++i) {
+      const float* x = part(i);
+      const float by = __builtin_amdgcn_exp2f(x[r] - base);
+      l = __builtin_fmaf(by, x[32 + r], l);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = __builtin_fmaf(by, x[64 + r * DP + d + j], o[j]);
+    }
+    const float by = l > 0.0f ? 1.0f / l : 0.0f;
+    bool bad = !__builtin_isfinite(l);
+    T out[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bad |= !__builtin_isfinite(o[j]);
+      out[j] = (T)(o[j] * by);
+    }
+    const int64_t at = (f.token * p.heads + f.head) * p.group + f.chunk * 32 + r;
+    __builtin_memcpy(static_cast<T*>(p.out) + at * p.width + d, out, sizeof out);
+    if (p.lse != nullptr && d == 0) p.lse[at] = l > 0.0f ? (m + __builtin_log2f(l)) * kLn2 : -INFINITY;
+    if (bad) any = s_bad[r] = 1;
+  }
+  if (!__syncthreads_or(any)) return;
+  __threadfence();  // the rows above are written before they are written again
+  __syncthreads();
+  for (int r = tid >> 6; r < rows; r += THREADS / 64)
+    if (s_bad[r]) careful_row<T, DP>(p, sq, seq, f.token, f.head, f.chunk * 32 + r, pos, tid & 63);
+}
+
+template <class T, int DP>
+__device__ inline void zero_rows(const BlockArgs& p, const FewPlace& f, int tid, int threads) {
+  const int rows = p.group - f.chunk * 32 < 32 ? p.group - f.chunk * 32 : 32;
+  const int64_t at = (f.token * p.heads + f.head) * p.group + f.chunk * 32;
+  for (int e = tid; e < rows * p.width; e += threads) static_cast<T*>(p.out)[at * p.width + e] = (T)0.0f;
+  if (p.lse != nullptr && tid < rows) p.lse[at + tid] = -INFINITY;
+}
+
+template <class T, int DP, bool TWO>
+__global__ __launch_bounds__((64 * FewShape<T, DP>::kWaves)) void block_attention_few_kernel(const BlockArgs p) {
+  using R = Rows<T, DP>;
+  constexpr int WAVES = FewShape<T, DP>::kWaves, THREADS = 64 * WAVES, G = R::kGroups;
+  static_assert(part_floats<DP>() * 4 <= 2 * R::kBytes, "a wave's state fits where its keys were");
+  __shared__ alignas(1024) uint8_t s_kv[WAVES][2][R::kBytes];
+  __shared__ int s_ids[kMostTop];
+  __shared__ int s_count, s_bad[32];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const FewPlace f = few_place(p, row_block());
+  if (f.token >= p.seqs.n_tokens) return;
+  int seq, pos;
+  Sequence sq;
+  if (!token_at(p.seqs, f.token, lane, seq, sq, pos)) {
+    if (f.split == 0) zero_rows<T, DP>(p, f, tid, THREADS);
+    return;
+  }
+  const int block = p.seqs.block, lg = p.lg_groups + 4;
+  const int32_t* ids = p.blocks + f.token * p.b_token + (int64_t)f.head * p.b_head;
+  for (int e = tid; e < p.top; e += THREADS) {
+    const int id = ids[e];
+    s_ids[e] = id >= 0 && id <= (pos >> lg) ? id : -1;
+  }
+  __syncthreads();
+  if (w == 0) {  // those that are blocks, each once
+    int count = 0;
+    for (int e0 = 0; e0 < p.top; e0 += 64) {
+      const int e = e0 + lane, id = e < p.top ? s_ids[e] : -1;
+      bool use = id >= 0;
+      for (int b = 0; b < count; ++b) use = use && s_ids[b] != id;
+      for (int b = 0; b < 63; ++b) {
+        const int other = __builtin_amdgcn_readlane(id, b);
+        use = use && !(b < lane && other == id);
+      }
+      const uint64_t m = __ballot(use);
+      if (use) s_ids[count + __builtin_popcountll(m & (((uint64_t)1 << lane) - 1))] = id;
+      count += __builtin_popcountll(m);
+    }
+    if (lane == 0) s_count = count;
+  }
+  RowOf row[2];
+  Online<T, DP> st;
+  start(st);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = f.chunk * 32 + i * 16 + (lane & 15);
+    row[i].in = r < p.group;
+    row[i].head = row[i].in ? r : 0;
+    row[i].token = 0;
+    row[i].pos = row[i].in ? pos : -1;
+    if (i == 0 || TWO)
+      load_row<T, DP>(static_cast<const T*>(p.q) + f.token * p.q_token +
+                          (int64_t)(f.head * p.group + row[i].head) * p.q_head,
+                      row[i].in, p.width, lane, st.q[i]);
+  }
+  __syncthreads();
+  const int count = s_count, steps = ((count << p.lg_groups) + G - 1) / G;
+  const float c = p.scale * kLog2e;
+  const uint32_t kb = lds_address(s_kv[w][0]), vb = lds_address(s_kv[w][1]);
+  for (int s = f.split * WAVES + w; s < steps; s += WAVES * p.splits) {
+    int first[G];
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr) {
+      const int q = s * G + gr, e = q >> p.lg_groups;
+      const int id = __builtin_amdgcn_readfirstlane(e < count ? s_ids[e] : -1);
+      first[gr] = id >= 0 ? id * block + (q & ((1 << p.lg_groups) - 1)) * 16 : -1;
+    }
+    auto entry = [&](int gr) {
+      int x = first[0];
+#pragma unroll
+      for (int i = 1; i < G; ++i) x = gr == i ? first[i] : x;
+      return x;
+    };
+    wait_reads();  // the step before has read its rows
+    load_rows<T, DP, 1>(p, p.k, sq, seq, f.head, kb, 0, lane, entry);
+    load_rows<T, DP, 1>(p, p.v, sq, seq, f.head, vb, 0, lane, entry);
+    const uint32_t missing = missing_pages<T, DP>(p, sq, seq, entry);
+    bool sel[2][G];
+    bool edge = missing != 0;
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr) {
+      sel[0][gr] = row[0].in && first[gr] >= 0;
+      sel[1][gr] = row[1].in && first[gr] >= 0;
+      edge |= first[gr] + 15 > pos;
+    }
+    wait_loads<0>();
+    attend<T, DP, true, TWO>(st, kb, vb, sel, first, edge, missing, row, c, lane);
+  }
+  wait_reads();
+  float* mine = reinterpret_cast<float*>(s_kv[w][0]);
+#pragma unroll
+  for (int i = 0; i < (TWO ? 2 : 1); ++i) {
+    const int r = i * 16 + (lane & 15);
+    const float l = across_sum(st.l[i]);
+    if (lane < 16) {
+      mine[r] = st.m[i];
+      mine[32 + r] = l;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt)
+      *reinterpret_cast<f32x4*>(&mine[64 + r * DP + dt * 16 + (lane >> 4) * 4]) = st.o[i][dt];
+  }
+  __syncthreads();
+  if (p.splits == 1) {
+    join_rows<T, DP, THREADS>(p, f, seq, sq, pos, WAVES, tid, s_bad,
+                              [&](int i) { return reinterpret_cast<const float*>(s_kv[i][0]); });
+    return;
+  }
+  // joined over the waves, into the split's part
+  float* part = p.parts + row_block() * part_floats<DP>();
+  const int rows = TWO ? 32 : 16;
+  for (int e = tid; e < rows * (DP / 4); e += THREADS) {
+    const int r = e / (DP / 4), d = e % (DP / 4) * 4;
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) m = fmaxf(m, reinterpret_cast<const float*>(s_kv[i][0])[r]);
+    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+      const float* x = reinterpret_cast<const float*>(s_kv[i][0]);
+      const float by = __builtin_amdgcn_exp2f(x[r] - base);
+      l = __builtin_fmaf(by, x[32 + r], l);
+      o += by * *reinterpret_cast<const f32x4*>(&x[64 + r * DP + d]);
+    }
+    if (d == 0) {
+      part[r] = m;
+      part[32 + r] = l;
+    }
+    *reinterpret_cast<f32x4*>(&part[64 + r * DP + d]) = o;
+  }
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__(128) void block_attention_join_kernel(const BlockArgs p) {
+  __shared__ int s_bad[32];
+  const int64_t at = row_block();
+  const FewPlace f = few_place(p, at * p.splits);
+  if (f.token >= p.seqs.n_tokens) return;
+  int seq, pos;
+  Sequence sq;
+  if (!token_at(p.seqs, f.token, threadIdx.x & 63, seq, sq, pos)) return;  // (zeros are there already)
+  join_rows<T, DP, 128>(p, f, seq, sq, pos, p.splits, threadIdx.x, s_bad, [&](int i) {
+    return p.parts + (at * p.splits + i) * part_floats<DP>();
+  });
+}
+
+// A few rows' kernel up to this many (token, key-value head) pairs.
+constexpr int64_t kFewPairs = 4096;
+
+struct Plan {
+  bool few;
+  int splits;
+  int64_t groups;  // (token, head, chunk) triples of the few rows' kernel
+  size_t bytes;
+};
+Plan plan_of(int val_t, int64_t tokens, int heads, int group, int width, int block, int top) {
+  Plan o{};
+  o.few = tokens * heads <= kFewPairs;
+  o.groups = tokens * heads * ((group + 31) / 32);
+  o.splits = 1;
+  if (o.few) {
+    const int bytes = (width <= 64 ? 64 : width <= 128 ? 128 : 256) * (val_t == FS_F32 ? 4 : 2);
+    const int waves = bytes > 256 ? 2 : kFewWaves, keys = val_t == FS_F32 ? 32 : 64;
+    const int64_t steps = ceil_div((int64_t)top * block, keys);
+    // until a wave has one step, or there are two workgroups a compute unit
+    while ((int64_t)o.splits * waves < steps && o.groups * o.splits < 512 && o.splits < 64) o.splits *= 2;
+    if (o.splits > 1)
+      o.bytes = (size_t)(o.groups * o.splits) * (64 + 32 * (width <= 64 ? 64 : width <= 128 ? 128 : 256)) * 4;
+  }
+  return o;
+}
+
+}  // namespace
+}  // namespace fs
+
+extern "C" size_t fs_block_attention_workspace_bytes(int val_t, const fs_block_seqs* seqs, int heads, int group,
+                                                     int width, int top) {
+  using namespace fs;
+  if (block_sizes_fault("", val_t, seqs, heads, group, width) != FS_OK || top < 1 || top > kMostTop) return 0;
+  return plan_of(val_t, seqs->n_tokens, heads, group, width, seqs->block, top).bytes;
+}
+
+extern "C" int fs_block_attention(int val_t, const fs_block_seqs* seqs, int heads, int group, int width, int top,
+                                  const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_page,
+                                  int64_t k_row, int64_t k_head, const void* v, int64_t v_page, int64_t v_row,
+                                  int64_t v_head, const int32_t* blocks, int64_t b_token, int64_t b_head, double scale,
+                                  void* out, float* lse, void* ws, size_t ws_bytes, hipStream_t stream) {
+  using namespace fs;
+  const char* who = "fs_block_attention";
+  if (const int rc = block_sizes_fault(who, val_t, seqs, heads, group, width)) return rc;
+  if (top < 1 || top > kMostTop) return fail(FS_E_INVALID, std::string(who) + ": top out of range");
+  if (seqs->n_tokens == 0) return FS_OK;
+  const int64_t size = val_t == FS_F32 ? 4 : 2;
+  if (!q || !k || !v || !blocks || !out || q_token < 0 || q_head < 0 || b_token < 0 || b_head < 0)
+    return fail(FS_E_INVALID, std::string(who) + ": bad pointer or stride");
+  if (!block_rows_fit(k, k_page, k_row, k_head, size) || !block_rows_fit(v, v_page, v_row, v_head, size))
+    return fail(FS_E_INVALID, std::string(who) + ": keys and values need rows at multiples of 16 bytes");
+  if (!(scale > 0.0) || !(scale < 1e30)) return fail(FS_E_INVALID, std::string(who) + ": scale must be positive");
+  const Plan plan = plan_of(val_t, seqs->n_tokens, heads, group, width, seqs->block, top);
+  if (plan.bytes > 0 && (ws == nullptr || ws_bytes < plan.bytes))
+    return fail(FS_E_WORKSPACE, std::string(who) + ": workspace too small");
+  BlockArgs p{};
+  p.seqs = *seqs;
+  p.k = RowLayout{k, k_page, k_row, k_head};
+  p.v = RowLayout{v, v_page, v_row, v_head};
+  p.q = q;
+  p.q_token = q_token;
+  p.q_head = q_head;
+  p.out = out;
+  p.lse = lse;
+  p.blocks = blocks;
+  p.b_token = b_token;
+  p.b_head = b_head;
+  p.top = top;
+  p.heads = heads;
+  p.group = group;
+  p.width = width;
+  p.lg_groups = __builtin_ctz((unsigned)seqs->block) - 4;
+  p.scale = (float)scale;
+  p.splits = plan.splits;
+  p.parts = static_cast<float*>(ws);
+  return with_block_width(val_t, width, who, [&](auto val, auto dp) -> int {
+    using T = decltype(val);
+    constexpr int DP = decltype(dp)::value;
+    if (plan.few) {
+      const dim3 grid = row_grid(plan.groups * plan.splits), threads(64 * FewShape<T, DP>::kWaves);
+      if (group > 16) hipLaunchKernelGGL((block_attention_few_kernel<T, DP, true>), grid, threads, 0, stream, p);
+      else hipLaunchKernelGGL((block_attention_few_kernel<T, DP, false>), grid, threads, 0, stream, p);
+      FS_CHECK_MAIN_LAUNCH("block_attention_few_kernel");
+      if (plan.splits > 1) {
+        hipLaunchKernelGGL((block_attention_join_kernel<T, DP>), row_grid(plan.groups), dim3(128), 0, stream, p);
+        FS_CHECK_LAUNCH("block_attention_join_kernel");
+      }
+      return FS_OK;
+    }
+    constexpr int WAVES = 4;
+    p.tiles = block_tiles(*seqs, tokens_of<WAVES>(group));
+    if (p.tiles * heads > kMostWorkgroups) return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
+    hipLaunchKernelGGL((block_attention_kernel<T, DP, WAVES>), dim3((uint32_t)(p.tiles * heads)), dim3(64 * WAVES), 0,
+                       stream, p);
+    FS_CHECK_MAIN_LAUNCH("block_attention_kernel");
+    return FS_OK;
+  });
+}

@@ -1,0 +1,928 @@
+// block_attention_grad.hip — gradients of the attention over selected blocks.
+//
+// With S = scale Q K^T on the selection, P = exp(S - lse) its rows' softmax, which
+// the forward pass's lse gives again without their sums, and G the gradient of the
+// result O:
+//   dV = P^T G          dP = G V^T          dS = P (dP - <G, O>)
+//   dQ = scale dS K     dK = scale dS^T Q
+// The queries' gradient walks a workgroup's blocks as the forward pass does.  The
+// keys' and values' need the selection's transpose, the tokens of each block: the
+// entries sorted by block (select_sort.hip), in pieces of about the same length,
+// since the first block has every token and most have few.  A workgroup takes one
+// piece and 32 or 64 of a block's keys; pieces of one block leave their sums in the
+// workspace, which are added in order, so no atomics' order shows.
+#include "block_walk.hpp"
+
+namespace fs {
+namespace {
+
+constexpr int kAmaxParts = 256;
+
+// dS of 16-bit floats, whose small values have few bits: G and <G, O> are multiplied
+// by the power of two that brings G's largest value to [1, 2), and the gradients
+// divided by it in 32 bits.  (bfloat16 and float32 have the exponents.)
+template <class T>
+constexpr bool kFactored = std::is_same_v<T, _Float16>;
+
+__device__ inline float factor_of(float most) {
+  const uint32_t e = (__float_as_uint(most) >> 23) & 255u;
+  return e == 0u || e >= 254u ? 1.0f : __uint_as_float((254u - e) << 23);
+}
+template <class T>
+__device__ inline float read_factor(const float* parts, int lane) {
+  if constexpr (!kFactored<T>) {
+    return 1.0f;
+  } else {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kAmaxParts / 64; ++i) m = fmaxf(m, parts[i * 64 + lane]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+    return factor_of(m);
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void block_amax_kernel(const T* x, int64_t n, float* parts) {
+  __shared__ float s_max[4];
+  float m = 0.0f;
+  const int64_t step = (int64_t)gridDim.x * 256 * Slice<T>::n;
+  for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * Slice<T>::n; at < n; at += step) {
+    // (n is a multiple of 8)
+    const Slice<T> v = load_slice(x + at);
+#pragma unroll
+    for (int e = 0; e < Slice<T>::n; ++e) m = fmaxf(m, fabsf((float)v.v[e]));
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+  if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) parts[blockIdx.x] = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+}
+
+// ---- gradient of the queries ------------------------------------------------------
+
+template <class T, int DP>
+struct QueryGrad {
+  typename Mma<T>::frag q[2][Rows<T, DP>::kFrags], g[2][Rows<T, DP>::kFrags];
+  f32x4 d[2][DP / 16];
+  float lse[2], delta[2];  // in powers of two; times the factor
+};
+
+template <class T, int DP, bool A, bool B>
+__device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, const bool (&sel)[2][Rows<T, DP>::kGroups],
+                            const int (&first)[Rows<T, DP>::kGroups], bool edge, uint32_t missing,
+                            const RowOf (&row)[2], float c, float factor, int lane) {
+  using R = Rows<T, DP>;
+  constexpr int G = R::kGroups, P = R::kUnit / 16;
+  f32x4 s[2][G], dp[2][G];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr) s[i][gr] = dp[i][gr] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int ks = 0; ks < R::kFrags; ++ks)
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr) {
+      const auto k = R::across(kb, gr * 16, ks, lane);
+      if (A) s[0][gr] = Mma<T>::run(k, st.q[0][ks], s[0][gr]);
+      if (B) s[1][gr] = Mma<T>::run(k, st.q[1][ks], s[1][gr]);
+      const auto v = R::across(vb, gr * 16, ks, lane);
+      if (A) dp[0][gr] = Mma<T>::run(v, st.g[0][ks], dp[0][gr]);
+      if (B) dp[1][gr] = Mma<T>::run(v, st.g[1][ks], dp[1][gr]);
+    }
+  typename R::frag w[2][G / P];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (i == 0 ? !A : !B) continue;
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        bool in = sel[i][gr];
+        if (edge) in = in && first[gr] + 4 * (lane >> 4) + r <= row[i].pos && !((missing >> gr) & 1u);
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][gr][r], c, -st.lse[i]));
+        const float y = x * __builtin_fmaf(dp[i][gr][r], factor, -st.delta[i]);
+        s[i][gr][r] = in ? y : 0.0f;
+      }
+    // (dS in the values' type, rounded once)
+#pragma unroll
+    for (int u = 0; u < G / P; ++u) w[i][u] = R::rounded(&s[i][u * P]);
+  }
+#pragma unroll
+  for (int u = 0; u < G / P; ++u)
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt) {
+      const auto k = R::down(kb, u * R::kUnit, dt, lane);
+      if (A) st.d[0][dt] = Mma<T>::run(k, w[0][u], st.d[0][dt]);
+      if (B) st.d[1][dt] = Mma<T>::run(k, w[1][u], st.d[1][dt]);
+    }
+}
+
+struct GradArgs {
+  BlockArgs b;  // q, k, v, blocks; out: the queries' gradient
+  const void* grad;
+  const void* o;
+  const float* lse;
+  float* delta;        // <G, O> of each row
+  const float* amax;   // float16
+  const int32_t* order;
+  const int4* pieces;  // key, first entry, one behind the last, place of its sums or -1
+  const int32_t* n_pieces;
+  const int2* sums;    // of each key: place of its first sums, and their number
+  float* parts;
+  void* dk;
+  void* dv;
+  int lists;           // selections a token: heads, or 1 where the heads share one
+  int key_blocks;      // blocks that keys may name, of all sequences
+  uint32_t per_group;  // 2^32 / group, rounded up
+};
+
+// A row without what is left out, see careful_row.
+template <class T, int DP>
+__device__ __noinline__ void careful_query(const GradArgs& a, const Sequence& sq, int seq, int64_t token, int head,
+                                           int in_group, int pos, float lse, float delta, int lane) {
+  const BlockArgs& p = a.b;
+  const int hq = head * p.group + in_group, block = p.seqs.block, lg = p.lg_groups + 4;
+  const int64_t at = token * p.heads * p.group + hq;
+  const T* q = static_cast<const T*>(p.q) + token * p.q_token + (int64_t)hq * p.q_head;
+  const T* g = static_cast<const T*>(a.grad) + at * p.width;
+  const int32_t* ids = p.blocks + token * p.b_token + (int64_t)head * p.b_head;
+  const float c = p.scale * kLog2e;
+  float d[(DP + 63) / 64];
+#pragma unroll
+  for (int i = 0; i < (DP + 63) / 64; ++i) d[i] = 0.0f;
+  for (int e = 0; e < p.top; ++e) {
+    const int id = ids[e];
+    bool use = id >= 0 && id <= (pos >> lg);
+    for (int b = 0; b < e; ++b) use = use && ids[b] != id;
+    if (!use) continue;
+    for (int j0 = 0; j0 < block; j0 += 64) {
+      const int j = id * block + j0 + lane;
+      const bool seen = j0 + lane < block && j <= pos && j < sq.keys;
+      float w = 0.0f;
+      if (seen) {
+        const T* k = key_rows<T>(p.seqs, sq, seq, p.k, head, j & ~15) + (int64_t)(j & 15) * p.k.row;
+        const T* v = key_rows<T>(p.seqs, sq, seq, p.v, head, j & ~15) + (int64_t)(j & 15) * p.v.row;
+        float s = 0.0f, y = 0.0f;
+        for (int x = 0; x < p.width; ++x) {
+          s = __builtin_fmaf((float)q[x], (float)k[x], s);
+          y = __builtin_fmaf((float)g[x], (float)v[x], y);
+        }
+        w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -lse)) * (y - delta);
+      }
+      for (uint64_t left = __ballot(seen); left != 0; left &= left - 1) {
+        const int l = __builtin_ctzll(left), jj = id * block + j0 + l;
+        const float weight = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(w), l));
+        const T* k = key_rows<T>(p.seqs, sq, seq, p.k, head, jj & ~15) + (int64_t)(jj & 15) * p.k.row;
+#pragma unroll
+        for (int i = 0; i < (DP + 63) / 64; ++i)
+          if (i * 64 + lane < p.width) d[i] = __builtin_fmaf(weight, (float)k[i * 64 + lane], d[i]);
+      }
+    }
+  }
+  T* out = static_cast<T*>(p.out) + at * p.width;
+#pragma unroll
+  for (int i = 0; i < (DP + 63) / 64; ++i)
+    if (i * 64 + lane < p.width) out[i * 64 + lane] = (T)(d[i] * p.scale);
+}
+
+template <class T, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void block_query_grad_kernel(const GradArgs a) {
+  using R = Rows<T, DP>;
+  __shared__ alignas(1024) uint8_t s_kv[2][2][R::kBytes];
+  __shared__ WalkMemory<WAVES> s_walk;
+  const BlockArgs& p = a.b;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  WalkTile t;
+  if (!walk_tile<WAVES>(p, lane, t)) return;
+  RowOf row[2];
+  rows_of<WAVES>(p, t, w, lane, row);
+  const float factor = read_factor<T>(a.amax, lane);
+  QueryGrad<T, DP> st;
+  float delta[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int hq = t.head * p.group + row[i].head;
+    const int64_t at = (int64_t)(t.token0 + row[i].token) * p.heads * p.group + hq;
+    load_row<T, DP>(static_cast<const T*>(p.q) + (int64_t)(t.token0 + row[i].token) * p.q_token + (int64_t)hq * p.q_head,
+                    row[i].in, p.width, lane, st.q[i]);
+    load_row<T, DP>(static_cast<const T*>(a.grad) + at * p.width, row[i].in, p.width, lane, st.g[i]);
+    typename R::frag o[R::kFrags];
+    load_row<T, DP>(static_cast<const T*>(a.o) + at * p.width, row[i].in, p.width, lane, o);
+    float sum = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < R::kFrags; ++ks)
+#pragma unroll
+      for (int e = 0; e < 16 / (int)sizeof(T); ++e) sum = __builtin_fmaf((float)st.g[i][ks][e], (float)o[ks][e], sum);
+    delta[i] = across_sum(sum);
+    st.delta[i] = delta[i] * factor;
+    st.lse[i] = row[i].in ? a.lse[at] * kLog2e : 0.0f;
+    if (row[i].in && lane < 16) a.delta[at] = delta[i];
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt) st.d[i][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const float c = p.scale * kLog2e;
+  walk_blocks<T, DP, WAVES>(
+      p, t, row, s_walk, s_kv, tid, w, lane,
+      [&](const Step<T, DP>& now, const bool(&sel)[2][R::kGroups], bool x, bool y, bool edge, uint32_t kb, uint32_t vb) {
+        if (x && y) take<T, DP, true, true>(st, kb, vb, sel, now.first, edge, now.missing, row, c, factor, lane);
+        else if (x) take<T, DP, true, false>(st, kb, vb, sel, now.first, edge, now.missing, row, c, factor, lane);
+        else take<T, DP, false, true>(st, kb, vb, sel, now.first, edge, now.missing, row, c, factor, lane);
+      });
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    bool bad = false;
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bad |= !__builtin_isfinite(st.d[i][dt][r]);
+    uint64_t rows = __ballot(bad && row[i].in);
+    rows = (rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xffffu;
+    const int64_t at = (int64_t)(t.token0 + row[i].token) * p.heads * p.group + t.head * p.group + row[i].head;
+    if (row[i].in && !((rows >> (lane & 15)) & 1))
+      store_row<T, DP>(static_cast<T*>(p.out) + at * p.width, st.d[i], p.scale / factor, p.width, lane);
+    for (; rows != 0; rows &= rows - 1) {
+      const int r = __builtin_ctzll(rows), tok = __builtin_amdgcn_readlane(row[i].token, r);
+      auto of = [&](float x) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), r)); };
+      careful_query<T, DP>(a, t.sq, t.seq, t.token0 + tok, t.head, __builtin_amdgcn_readlane(row[i].head, r),
+                           t.pos0 + tok, of(st.lse[i]), of(delta[i]), lane);
+    }
+  }
+}
+
+// ---- the selection's transpose ----------------------------------------------------
+
+// Number of a sequence's first block among all blocks: those of one sequence are
+// consecutive, and no two sequences share one, without their lengths' sum.
+__device__ inline int first_block(const fs_block_seqs& s, int b, int lg_block) {
+  return (clamp_to(s.k_offsets[b], 0, s.n_rows) >> lg_block) + b;
+}
+
+// The key that each entry of the selection is sorted by, head by head and block by
+// block; one too large for entries that name nothing or the same block again.  A
+// wave takes a token.  Also zeros the gradients of rows of no sequence.
+__global__ __launch_bounds__(256) void block_keys_kernel(const BlockArgs p, int lists, int key_blocks, int32_t* keys,
+                                                         uint32_t* dk, uint32_t* dv, int64_t row_words) {
+  const int lane = threadIdx.x & 63, lg = p.lg_groups + 4;
+  const int64_t waves = (int64_t)gridDim.x * 4, first = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int n_keys = lists * key_blocks;
+  for (int64_t token = first; token < p.seqs.n_tokens; token += waves) {
+    int seq, pos, base = 0;
+    Sequence sq;
+    const bool some = [&] {
+      seq = (int)p.seqs.n_seqs;
+      if (p.seqs.q_offsets == nullptr) {
+        seq = (int)token;
+      } else {
+        for (int64_t b0 = 0; b0 < p.seqs.n_seqs; b0 += 64) {
+          bool mine = false;
+          if (b0 + lane < p.seqs.n_seqs) {
+            const Sequence q = sequence_at(p.seqs, (int)b0 + lane);
+            mine = token >= q.first && token < q.first + q.count;
+          }
+          const uint64_t m = __ballot(mine);
+          if (m != 0) {
+            seq = (int)b0 + __builtin_ctzll(m);
+            break;
+          }
+        }
+      }
+      return seq < p.seqs.n_seqs;
+    }();
+    pos = -1;
+    if (some) {
+      sq = sequence_at(p.seqs, seq);
+      pos = sq.keys - sq.count + (int)(token - sq.first);
+      base = first_block(p.seqs, seq, lg);
+    }
+    for (int e = lane; e < lists * p.top; e += 64) {
+      const int list = e / p.top, at = e - list * p.top;
+      const int32_t* ids = p.blocks + token * p.b_token + (int64_t)list * p.b_head;
+      const int id = ids[at];
+      bool use = id >= 0 && id <= (pos >> lg);
+      for (int b = 0; b < at; ++b) use = use && ids[b] != id;
+      const int64_t key = (int64_t)list * key_blocks + base + id;
+      keys[token * lists * p.top + e] = use && base + id < key_blocks ? (int32_t)key : n_keys;
+    }
+  }
+  const int64_t head = p.seqs.n_seqs > 0 ? clamp_to(p.seqs.k_offsets[0], 0, p.seqs.n_rows) : 0;
+  const int64_t tail = p.seqs.n_seqs > 0 ? clamp_to(p.seqs.k_offsets[p.seqs.n_seqs], 0, p.seqs.n_rows) : 0;
+  const int64_t threads = (int64_t)gridDim.x * 256, me = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  for (int64_t i = me; i < head * row_words; i += threads) dk[i] = dv[i] = 0u;
+  for (int64_t i = tail * row_words + me; i < p.seqs.n_rows * row_words; i += threads) dk[i] = dv[i] = 0u;
+}
+
+// First sorted entry of each key.
+__global__ __launch_bounds__(256) void block_lists_kernel(const uint32_t* keys, int64_t n, int n_keys, int32_t* starts) {
+  const int k = (int)(blockIdx.x * 256 + threadIdx.x);
+  if (k > n_keys) return;
+  int64_t lo = 0, hi = n;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (keys[mid] < (uint32_t)k) lo = mid + 1;
+    else hi = mid;
+  }
+  starts[k] = (int32_t)lo;
+}
+
+// Lists cut into pieces of `most` entries at most, one at least, and places for the
+// sums of those with more than one.  One workgroup.
+__global__ __launch_bounds__(1024) void block_pieces_kernel(const int32_t* starts, int n_keys, int most, int4* pieces,
+                                                            int2* sums, int32_t* n_pieces) {
+  __shared__ uint32_t s_total[2][16];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  uint32_t at = 0, place = 0;
+  for (int k0 = 0; k0 < n_keys; k0 += 1024) {
+    const int k = k0 + tid;
+    const int from = k < n_keys ? starts[k] : 0, to = k < n_keys ? starts[k + 1] : 0;
+    const uint32_t n = k < n_keys ? (uint32_t)(to > from ? (to - from + most - 1) / most : 1) : 0u;
+    const uint32_t shared = n > 1 ? n : 0u;
+    const uint32_t upto = wave_sum_scan(n), upto2 = wave_sum_scan(shared);
+    if (lane == 63) {
+      s_total[0][w] = upto;
+      s_total[1][w] = upto2;
+    }
+    __syncthreads();
+    uint32_t mine = at + upto - n, mine2 = place + upto2 - shared;
+    for (int i = 0; i < 16; ++i) {
+      if (i < w) {
+        mine += s_total[0][i];
+        mine2 += s_total[1][i];
+      }
+      at += s_total[0][i];
+      place += s_total[1][i];
+    }
+    if (k < n_keys) {
+      sums[k] = int2{(int)mine2, (int)shared};
+      // (of like length)
+      const int each = n > 0 ? (int)((to - from + (int)n - 1) / (int)n) : 0;
+      for (uint32_t i = 0; i < n; ++i) {
+        const int a = from + (int)i * each < to ? from + (int)i * each : to;
+        const int b = a + each < to ? a + each : to;
+        pieces[mine + i] = int4{k, a, b, n > 1 ? (int)(mine2 + i) : -1};
+      }
+    }
+    __syncthreads();
+  }
+  if (tid == 0) *n_pieces = (int32_t)at;
+}
+
+// ---- gradients of keys and values -------------------------------------------------
+
+// KT tiles of 16 keys a wave, KW waves over the keys, RW over the rows.
+template <class T, int DP, int BK>
+struct KeyShape {
+  static constexpr bool kWide = DP * (int)sizeof(T) > 256;
+  static constexpr int KT = kWide ? 1 : 2;
+  static constexpr int KW = BK / (16 * KT);
+  static constexpr int RW = 4 / KW;
+  static constexpr int kStep = 32 * RW;  // rows a step
+};
+
+struct KeyPlace {
+  int seq, head, first;  // position of the first key
+  Sequence sq;
+};
+
+// 4 rows' numbers, by a lane's group.
+struct RowStats {
+  float lse[128], delta[128];
+  int pos[128];
+};
+
+template <class T, int DP>
+__device__ __noinline__ void careful_key(const GradArgs& a, const KeyPlace& at, const int32_t* tokens, int rows, int j,
+                                         float (&k_sum)[(DP + 63) / 64], float (&v_sum)[(DP + 63) / 64], int lane) {
+  const BlockArgs& p = a.b;
+  const float c = p.scale * kLog2e;
+  constexpr int N = (DP + 63) / 64;
+#pragma unroll
+  for (int i = 0; i < N; ++i) k_sum[i] = v_sum[i] = 0.0f;
+  if (j >= at.sq.keys) return;
+  const T* k = static_cast<const T*>(p.k.base) + (at.sq.row0 + j) * p.k.row + at.head * p.k.head;
+  const T* v = static_cast<const T*>(p.v.base) + (at.sq.row0 + j) * p.v.row + at.head * p.v.head;
+  for (int r0 = 0; r0 < rows; r0 += 64) {
+    const int r = r0 + lane;
+    float x = 0.0f, y = 0.0f;
+    bool seen = false;
+    int64_t row = 0, q_row = 0;
+    if (r < rows) {
+      const int token = tokens[r / p.group], hq = at.head * p.group + r % p.group;
+      seen = at.sq.keys - at.sq.count + token - at.sq.first >= j;
+      row = (int64_t)token * p.heads * p.group + hq;
+      q_row = token * p.q_token + hq * p.q_head;
+      if (seen) {
+        const T* q = static_cast<const T*>(p.q) + q_row;
+        const T* g = static_cast<const T*>(a.grad) + row * p.width;
+        float s = 0.0f, d = 0.0f;
+        for (int i = 0; i < p.width; ++i) {
+          s = __builtin_fmaf((float)q[i], (float)k[i], s);
+          d = __builtin_fmaf((float)g[i], (float)v[i], d);
+        }
+        x = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -a.lse[row] * kLog2e));
+        y = x * (d - a.delta[row]);
+      }
+    }
+    for (uint64_t left = __ballot(seen); left != 0; left &= left - 1) {
+      const int l = __builtin_ctzll(left);
+      const float wx = __shfl(x, l), wy = __shfl(y, l);
+      const T* g = static_cast<const T*>(a.grad) + __shfl(row, l) * p.width;
+      const T* q = static_cast<const T*>(p.q) + __shfl(q_row, l);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i * 64 + lane < p.width) {
+          v_sum[i] = __builtin_fmaf(wx, (float)g[i * 64 + lane], v_sum[i]);
+          k_sum[i] = __builtin_fmaf(wy, (float)q[i * 64 + lane], k_sum[i]);
+        }
+    }
+  }
+}
+
+constexpr int kMostEntries = 1024;  // of a piece
+
+template <class T, int DP, int BK>
+__global__ __launch_bounds__(256) void block_key_grad_kernel(const GradArgs a) {
+  using R = Rows<T, DP>;
+  using S = KeyShape<T, DP, BK>;
+  constexpr int KT = S::KT, KW = S::KW, RW = S::RW, STEP = S::kStep, F = R::kFrags;
+  constexpr int kSlot = STEP * R::kRow, P = R::kUnit / 16;
+  constexpr int kJoin = (RW - 1) * KW * KT * 16 * DP * 4 * 2;
+  constexpr int kMemory = 4 * kSlot > kJoin ? 4 * kSlot : kJoin;
+  __shared__ alignas(1024) uint8_t s_mem[kMemory];
+  __shared__ RowStats s_stats[2];
+  __shared__ int32_t s_token[kMostEntries];
+  __shared__ int s_bad;
+  const BlockArgs& p = a.b;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kw = w % KW, rw = w / KW;
+  const int lg_block = p.lg_groups + 4, parts = p.seqs.block / BK, shared = p.heads / a.lists;
+  int64_t at = xcd_range_block(blockIdx.x, gridDim.x);
+  const int part = (int)(at % parts);
+  at /= parts;
+  const int copy = (int)(at % shared);
+  at /= shared;
+  if (at >= *a.n_pieces) return;
+  const int4 piece = a.pieces[at];
+  KeyPlace o;
+  const int list = piece.x / a.key_blocks, number = piece.x - list * a.key_blocks;
+  o.head = a.lists == 1 ? copy : list;
+  o.seq = -1;
+  for (int64_t b0 = 0; b0 < p.seqs.n_seqs; b0 += 64) {
+    bool mine = false;
+    if (b0 + lane < p.seqs.n_seqs) {
+      const Sequence q = sequence_at(p.seqs, (int)b0 + lane);
+      const int f = first_block(p.seqs, (int)b0 + lane, lg_block);
+      mine = number >= f && number - f < ((q.keys + p.seqs.block - 1) >> lg_block);
+    }
+    const uint64_t m = __ballot(mine);
+    if (m != 0) {
+      o.seq = (int)b0 + __builtin_ctzll(m);
+      break;
+    }
+  }
+  if (o.seq < 0) return;  // a number that no sequence's block has
+  o.sq = sequence_at(p.seqs, o.seq);
+  o.first = ((number - first_block(p.seqs, o.seq, lg_block)) << lg_block) + part * BK;
+  const int entries = piece.z - piece.y, rows = entries * p.group;
+  for (int e = tid; e < entries; e += 256) s_token[e] = a.order[piece.y + e] / (a.lists * p.top);
+  if (tid == 0) s_bad = 0;
+
+  // the wave's keys and values, as second operands
+  typename R::frag kf[KT][F], vf[KT][F];
+#pragma unroll
+  for (int n = 0; n < KT; ++n) {
+    const int j = o.first + (kw * KT + n) * 16 + (lane & 15);
+    const bool in = j < o.sq.keys;
+    load_row<T, DP>(static_cast<const T*>(p.k.base) + (o.sq.row0 + j) * p.k.row + o.head * p.k.head, in, p.width, lane,
+                    kf[n]);
+    load_row<T, DP>(static_cast<const T*>(p.v.base) + (o.sq.row0 + j) * p.v.row + o.head * p.v.head, in, p.width, lane,
+                    vf[n]);
+  }
+  f32x4 dk[KT][DP / 16], dv[KT][DP / 16];
+#pragma unroll
+  for (int n = 0; n < KT; ++n)
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt) dk[n][dt] = dv[n][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const float factor = read_factor<T>(a.amax, lane);
+  const float c = p.scale * kLog2e;
+  const int offset = o.sq.keys - o.sq.count - o.sq.first;  // of positions from tokens
+  __syncthreads();
+
+  const int steps = (rows + STEP - 1) / STEP;
+  auto place = [&](int r, int& token, int& hq) {
+    const int e = (int)__umulhi((uint32_t)r, a.per_group);
+    const int entry = p.group == 1 ? r : e;
+    token = s_token[entry];
+    hq = o.head * p.group + r - entry * p.group;
+  };
+  float n_lse = 0.0f, n_delta = 0.0f;
+  int n_pos = 0;
+  auto issue = [&](int s) {
+    constexpr int kLoads = kSlot / 1024 / 4;
+    static_assert(kSlot % 4096 == 0, "whole loads a wave");
+    const uint32_t qb = lds_address(s_mem) + (uint32_t)((s & 1) * 2 * kSlot), gb = qb + kSlot;
+    const int lr = R::lane_row(lane), pos = lane % R::kPieces;
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      const int r0 = (w * kLoads + n) * R::kAtOnce;
+      const int at_step = s * STEP + r0 + lr;
+      int token, hq;
+      place(at_step < rows ? at_step : rows - 1, token, hq);  // (past the end: some row of the list, left out below)
+      const int piece16 = pos ^ R::swizzle((r0 + lr) & 15);
+      const bool in = piece16 * 16 < p.width * (int)sizeof(T);
+      const int64_t d = in ? piece16 * (16 / (int)sizeof(T)) : 0;
+      const T* q = static_cast<const T*>(p.q) + token * p.q_token + hq * p.q_head + d;
+      const T* g = static_cast<const T*>(a.grad) + ((int64_t)token * p.heads * p.group + hq) * p.width + d;
+      lds_dma_at((uint32_t)__builtin_amdgcn_readfirstlane((int)(qb + (uint32_t)r0 * R::kRow)), q);
+      lds_dma_at((uint32_t)__builtin_amdgcn_readfirstlane((int)(gb + (uint32_t)r0 * R::kRow)), g);
+    }
+    if (tid < STEP) {
+      const int r = s * STEP + tid;
+      int token, hq;
+      place(r < rows ? r : rows - 1, token, hq);
+      const int64_t row = (int64_t)token * p.heads * p.group + hq;
+      n_lse = a.lse[row];
+      n_delta = a.delta[row];
+      n_pos = r < rows ? token + offset : INT32_MIN;
+    }
+  };
+  if (steps > 0) issue(0);
+  for (int s = 0; s < steps; ++s) {
+    RowStats& stats = s_stats[s & 1];
+    if (tid < STEP) {
+      stats.lse[tid] = n_lse * kLog2e;
+      stats.delta[tid] = n_delta * factor;
+      stats.pos[tid] = n_pos;
+    }
+    wait_loads<0>();
+    wait_reads();
+    barrier();
+    if (s + 1 < steps) issue(s + 1);
+    const uint32_t qb = lds_address(s_mem) + (uint32_t)((s & 1) * 2 * kSlot) + (uint32_t)(rw * 32 * R::kRow);
+    const uint32_t gb = qb + kSlot;
+    f32x4 x[2][KT], y[2][KT];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < KT; ++n) x[m][n] = y[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int ks = 0; ks < F; ++ks)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const auto q = R::across(qb, m * 16, ks, lane);
+        const auto g = R::across(gb, m * 16, ks, lane);
+#pragma unroll
+        for (int n = 0; n < KT; ++n) {
+          x[m][n] = Mma<T>::run(q, kf[n][ks], x[m][n]);
+          y[m][n] = Mma<T>::run(g, vf[n][ks], y[m][n]);
+        }
+      }
+    typename R::frag pf[KT][2 / P], sf[KT][2 / P];
+    f32x4 wx[KT][2], wy[KT][2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const int r0 = rw * 32 + m * 16 + (lane >> 4) * 4;
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(&stats.lse[r0]);
+      const f32x4 delta = *reinterpret_cast<const f32x4*>(&stats.delta[r0]);
+      const int4 pos = *reinterpret_cast<const int4*>(&stats.pos[r0]);
+      const int row_pos[4] = {pos.x, pos.y, pos.z, pos.w};
+#pragma unroll
+      for (int n = 0; n < KT; ++n) {
+        const int j = o.first + (kw * KT + n) * 16 + (lane & 15);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          // (keys behind the last one are behind every position, rows past the list's
+          // end before every key)
+          const bool in = j <= row_pos[r];
+          const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(x[m][n][r], c, -lse[r]));
+          const float v = u * __builtin_fmaf(y[m][n][r], factor, -delta[r]);
+          wx[n][m][r] = in ? u : 0.0f;
+          wy[n][m][r] = in ? v : 0.0f;
+        }
+      }
+    }
+    // (P and dS in the values' type, each rounded once)
+#pragma unroll
+    for (int n = 0; n < KT; ++n)
+#pragma unroll
+      for (int u = 0; u < 2 / P; ++u) {
+        pf[n][u] = R::rounded(&wx[n][u * P]);
+        sf[n][u] = R::rounded(&wy[n][u * P]);
+      }
+#pragma unroll
+    for (int u = 0; u < 2 / P; ++u)
+#pragma unroll
+      for (int dt = 0; dt < DP / 16; ++dt) {
+        const auto g = R::down(gb, u * R::kUnit, dt, lane);
+        const auto q = R::down(qb, u * R::kUnit, dt, lane);
+#pragma unroll
+        for (int n = 0; n < KT; ++n) {
+          dv[n][dt] = Mma<T>::run(g, pf[n][u], dv[n][dt]);
+          dk[n][dt] = Mma<T>::run(q, sf[n][u], dk[n][dt]);
+        }
+      }
+  }
+  // sums of the waves over the rows
+  wait_reads();
+  __syncthreads();
+  float* s_join = reinterpret_cast<float*>(s_mem);
+  constexpr int kWaveSums = KT * 16 * DP * 2;
+  if (rw > 0) {
+    float* mine = s_join + ((rw - 1) * KW + kw) * kWaveSums;
+#pragma unroll
+    for (int n = 0; n < KT; ++n)
+#pragma unroll
+      for (int dt = 0; dt < DP / 16; ++dt) {
+        float* e = mine + ((n * (DP / 16) + dt) * 2) * 256 + lane * 4;
+        *reinterpret_cast<f32x4*>(e) = dk[n][dt];
+        *reinterpret_cast<f32x4*>(e + 256) = dv[n][dt];
+      }
+  }
+  __syncthreads();
+  bool bad = false;
+  if (rw == 0) {
+#pragma unroll
+    for (int i = 1; i < RW; ++i) {
+      const float* other = s_join + ((i - 1) * KW + kw) * kWaveSums;
+#pragma unroll
+      for (int n = 0; n < KT; ++n)
+#pragma unroll
+        for (int dt = 0; dt < DP / 16; ++dt) {
+          const float* e = other + ((n * (DP / 16) + dt) * 2) * 256 + lane * 4;
+          dk[n][dt] += *reinterpret_cast<const f32x4*>(e);
+          dv[n][dt] += *reinterpret_cast<const f32x4*>(e + 256);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < KT; ++n)
+#pragma unroll
+      for (int dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bad |= !__builtin_isfinite(dk[n][dt][r]) || !__builtin_isfinite(dv[n][dt][r]);
+    if (__ballot(bad) != 0 && lane == 0) s_bad = 1;
+  }
+  __syncthreads();
+  const bool again = s_bad != 0;
+  const int64_t place_of = piece.w >= 0 ? ((int64_t)piece.w * shared + copy) * p.seqs.block + part * BK : 0;
+  const float by = p.scale / factor;
+  if (!again) {
+    if (rw == 0) {
+#pragma unroll
+      for (int n = 0; n < KT; ++n) {
+        const int jj = (kw * KT + n) * 16 + (lane & 15), j = o.first + jj;
+        if (piece.w >= 0) {
+          float* sums = a.parts + (place_of + jj) * 2 * DP;
+#pragma unroll
+          for (int dt = 0; dt < DP / 16; ++dt) {
+            *reinterpret_cast<f32x4*>(sums + dt * 16 + (lane >> 4) * 4) = dk[n][dt] * by;
+            *reinterpret_cast<f32x4*>(sums + DP + dt * 16 + (lane >> 4) * 4) = dv[n][dt];
+          }
+        } else if (j < o.sq.keys) {
+          const int64_t row = ((o.sq.row0 + j) * p.heads + o.head) * p.width;
+          store_row<T, DP>(static_cast<T*>(a.dk) + row, dk[n], by, p.width, lane);
+          store_row<T, DP>(static_cast<T*>(a.dv) + row, dv[n], 1.0f, p.width, lane);
+        }
+      }
+    }
+    return;
+  }
+  // a sum that is not finite: each key by itself, without products of what it is not seen by
+  for (int jj = w; jj < BK; jj += 4) {
+    const int j = o.first + jj;
+    constexpr int N = (DP + 63) / 64;
+    float k_sum[N], v_sum[N];
+    careful_key<T, DP>(a, o, s_token, rows, j, k_sum, v_sum, lane);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int d = i * 64 + lane;
+      if (piece.w >= 0) {
+        float* sums = a.parts + (place_of + jj) * 2 * DP;
+        sums[d] = k_sum[i] * p.scale;
+        sums[DP + d] = v_sum[i];
+      } else if (j < o.sq.keys && d < p.width) {
+        const int64_t row = ((o.sq.row0 + j) * p.heads + o.head) * p.width;
+        static_cast<T*>(a.dk)[row + d] = (T)(k_sum[i] * p.scale);
+        static_cast<T*>(a.dv)[row + d] = (T)v_sum[i];
+      }
+    }
+  }
+}
+
+// Sums of a block's pieces, in order: a workgroup 16 keys of one.
+template <class T, int DP>
+__global__ __launch_bounds__(256) void block_key_join_kernel(const GradArgs a) {
+  const BlockArgs& p = a.b;
+  const int lane = threadIdx.x & 63, lg_block = p.lg_groups + 4, shared = p.heads / a.lists;
+  int64_t at = row_block();
+  const int group = (int)(at & ((1 << p.lg_groups) - 1));
+  at >>= p.lg_groups;
+  const int copy = (int)(at % shared), key = (int)(at / shared);
+  if (key >= a.lists * a.key_blocks) return;
+  const int2 sums = a.sums[key];
+  if (sums.y == 0) return;
+  const int list = key / a.key_blocks, number = key - list * a.key_blocks;
+  const int head = a.lists == 1 ? copy : list;
+  for (int64_t b0 = 0; b0 < p.seqs.n_seqs; b0 += 64) {
+    bool mine = false;
+    if (b0 + lane < p.seqs.n_seqs) {
+      const Sequence q = sequence_at(p.seqs, (int)b0 + lane);
+      const int f = first_block(p.seqs, (int)b0 + lane, lg_block);
+      mine = number >= f && number - f < ((q.keys + p.seqs.block - 1) >> lg_block);
+    }
+    const uint64_t m = __ballot(mine);
+    if (m == 0) continue;
+    const int seq = (int)b0 + __builtin_ctzll(m);
+    const Sequence sq = sequence_at(p.seqs, seq);
+    const int first = ((number - first_block(p.seqs, seq, lg_block)) << lg_block) + group * 16;
+    for (int e = threadIdx.x; e < 16 * (DP / 4) * 2; e += 256) {
+      const int d = e % (DP / 4) * 4, which = e / (DP / 4) % 2, jj = e / (DP / 4) / 2, j = first + jj;
+      if (d >= p.width || j >= sq.keys) continue;
+      f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int i = 0; i < sums.y; ++i)
+        sum += *reinterpret_cast<const f32x4*>(
+            a.parts + ((((int64_t)(sums.x + i) * shared + copy) * p.seqs.block + group * 16 + jj) * 2 + which) * DP + d);
+      T out[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) out[r] = (T)sum[r];
+      const int64_t row = ((sq.row0 + j) * p.heads + head) * p.width + d;
+      __builtin_memcpy(static_cast<T*>(which ? a.dv : a.dk) + row, out, sizeof out);
+    }
+    return;
+  }
+}
+
+// ---- host -------------------------------------------------------------------------
+
+struct GradPlan {
+  int64_t entries;  // of the selection
+  int64_t key_blocks, n_keys;
+  int64_t pieces, places;  // at most
+  int most;                // entries a piece
+  size_t sort, keys, sorted, order, starts, list, sums, count, delta, amax, parts, bytes;
+};
+GradPlan grad_plan(int64_t tokens, int64_t rows, int64_t n_seqs, int block, int heads, int group, int lists, int width,
+                   int top) {
+  GradPlan l{};
+  l.entries = tokens * lists * top;
+  l.key_blocks = rows / block + n_seqs + 1;
+  l.n_keys = l.key_blocks * lists;
+  // pieces enough for a few rounds of the chip, and long enough that their sums cost little
+  const int64_t shared = heads / lists, parts = std::max(1, block / 64);
+  int64_t most = ceil_div(l.entries * shared * parts, 2048);
+  most = std::max<int64_t>(most, ceil_div(512, group));
+  l.most = (int)std::min<int64_t>(most, kMostEntries);
+  l.pieces = l.entries / l.most + l.n_keys;
+  l.places = 2 * (l.entries / l.most) + 2;
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t a = at;
+    at += up(n);
+    return a;
+  };
+  l.sort = take(select_sort_bytes(l.entries, l.n_keys));
+  l.keys = take((size_t)l.entries * 4);
+  l.sorted = take((size_t)l.entries * 4);
+  l.order = take((size_t)l.entries * 4);
+  l.starts = take((size_t)(l.n_keys + 1) * 4);
+  l.list = take((size_t)l.pieces * 16);
+  l.sums = take((size_t)l.n_keys * 8);
+  l.count = take(4);
+  l.delta = take((size_t)tokens * heads * group * 4);
+  l.amax = take(kAmaxParts * 4);
+  const int dp = width <= 64 ? 64 : width <= 128 ? 128 : 256;
+  l.parts = take((size_t)(l.places * shared) * block * 2 * dp * 4);
+  l.bytes = at;
+  return l;
+}
+
+int grad_fault(const char* who, int val_t, const fs_block_seqs* seqs, int heads, int group, int width, int lists,
+               int top) {
+  if (const int rc = block_sizes_fault(who, val_t, seqs, heads, group, width)) return rc;
+  if (seqs->pages != nullptr) return fail(FS_E_INVALID, std::string(who) + ": keys of a cache have no gradient");
+  if (top < 1 || top > kMostTop) return fail(FS_E_INVALID, std::string(who) + ": top out of range");
+  if (lists != 1 && lists != heads) return fail(FS_E_INVALID, std::string(who) + ": lists is 1 or the heads");
+  const int64_t blocks = (seqs->n_rows / seqs->block + seqs->n_seqs + 1) * lists;
+  if (seqs->n_tokens * lists * top > INT32_MAX || blocks >= INT32_MAX)
+    return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
+  return FS_OK;
+}
+
+}  // namespace
+}  // namespace fs
+
+extern "C" size_t fs_block_attention_grad_workspace_bytes(int val_t, const fs_block_seqs* seqs, int heads, int group,
+                                                          int width, int lists, int top) {
+  using namespace fs;
+  if (grad_fault("", val_t, seqs, heads, group, width, lists, top) != FS_OK) return 0;
+  return grad_plan(seqs->n_tokens, seqs->n_rows, seqs->n_seqs, seqs->block, heads, group, lists, width, top).bytes;
+}
+
+extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int heads, int group, int width, int lists,
+                                       int top, const void* grad, const void* q, int64_t q_token, int64_t q_head,
+                                       const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                                       int64_t v_head, const int32_t* blocks, int64_t b_token, int64_t b_head,
+                                       double scale, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                                       void* ws, size_t ws_bytes, hipStream_t stream) {
+  using namespace fs;
+  const char* who = "fs_block_attention_grad";
+  if (const int rc = grad_fault(who, val_t, seqs, heads, group, width, lists, top)) return rc;
+  const int64_t size = val_t == FS_F32 ? 4 : 2, tokens = seqs->n_tokens;
+  if (tokens == 0 && seqs->n_rows == 0) return FS_OK;
+  if ((tokens > 0 && (!grad || !q || !blocks || !out || !lse || !dq)) || !k || !v || (seqs->n_rows > 0 && (!dk || !dv)) ||
+      q_token < 0 || q_head < 0 || b_token < 0 || b_head < 0)
+    return fail(FS_E_INVALID, std::string(who) + ": bad pointer or stride");
+  if (!block_rows_fit(k, 0, k_row, k_head, size) || !block_rows_fit(v, 0, v_row, v_head, size) ||
+      (((int64_t)(uintptr_t)q | (int64_t)(uintptr_t)grad | q_token * size | q_head * size) & 15) != 0)
+    return fail(FS_E_INVALID, std::string(who) + ": queries, keys, values and grad need rows at multiples of 16 bytes");
+  if (!(scale > 0.0) || !(scale < 1e30)) return fail(FS_E_INVALID, std::string(who) + ": scale must be positive");
+  const GradPlan l = grad_plan(tokens, seqs->n_rows, seqs->n_seqs, seqs->block, heads, group, lists, width, top);
+  if (ws == nullptr || ws_bytes < l.bytes) return fail(FS_E_WORKSPACE, std::string(who) + ": workspace too small");
+  uint8_t* m = static_cast<uint8_t*>(ws);
+  GradArgs a{};
+  BlockArgs& p = a.b;
+  p.seqs = *seqs;
+  p.k = RowLayout{k, 0, k_row, k_head};
+  p.v = RowLayout{v, 0, v_row, v_head};
+  p.q = q;
+  p.q_token = q_token;
+  p.q_head = q_head;
+  p.out = dq;
+  p.blocks = blocks;
+  p.b_token = b_token;
+  p.b_head = b_head;
+  p.top = top;
+  p.heads = heads;
+  p.group = group;
+  p.width = width;
+  p.lg_groups = __builtin_ctz((unsigned)seqs->block) - 4;
+  p.scale = (float)scale;
+  a.grad = grad;
+  a.o = out;
+  a.lse = lse;
+  a.delta = reinterpret_cast<float*>(m + l.delta);
+  float* amax = reinterpret_cast<float*>(m + l.amax);
+  a.amax = amax;
+  a.order = reinterpret_cast<int32_t*>(m + l.order);
+  a.pieces = reinterpret_cast<int4*>(m + l.list);
+  a.n_pieces = reinterpret_cast<int32_t*>(m + l.count);
+  a.sums = reinterpret_cast<int2*>(m + l.sums);
+  a.parts = reinterpret_cast<float*>(m + l.parts);
+  a.dk = dk;
+  a.dv = dv;
+  a.lists = lists;
+  a.key_blocks = (int)l.key_blocks;
+  a.per_group = group == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + group - 1) / group);
+  int32_t* keys = reinterpret_cast<int32_t*>(m + l.keys);
+  uint32_t* sorted = reinterpret_cast<uint32_t*>(m + l.sorted);
+  int32_t* starts = reinterpret_cast<int32_t*>(m + l.starts);
+
+  hipLaunchKernelGGL(block_keys_kernel, dim3((uint32_t)std::min<int64_t>(ceil_div(std::max<int64_t>(tokens, 4), 4), 4096)),
+                     dim3(256), 0, stream, p, lists, (int)l.key_blocks, keys, static_cast<uint32_t*>(dk),
+                     static_cast<uint32_t*>(dv), (int64_t)heads * width * size / 4);
+  FS_CHECK_LAUNCH("block_keys_kernel");
+  if (l.entries > 0) {
+    if (const int rc = select_sort(keys, FS_I32, l.entries, l.n_keys, sorted, reinterpret_cast<int32_t*>(m + l.order),
+                                   nullptr, nullptr, m + l.sort, stream, nullptr, 0))
+      return rc;
+  }
+  hipLaunchKernelGGL(block_lists_kernel, dim3((uint32_t)ceil_div(l.n_keys + 1, 256)), dim3(256), 0, stream, sorted,
+                     l.entries, (int)l.n_keys, starts);
+  FS_CHECK_LAUNCH("block_lists_kernel");
+  hipLaunchKernelGGL(block_pieces_kernel, dim3(1), dim3(1024), 0, stream, starts, (int)l.n_keys, l.most,
+                     const_cast<int4*>(a.pieces), const_cast<int2*>(a.sums), const_cast<int32_t*>(a.n_pieces));
+  FS_CHECK_LAUNCH("block_pieces_kernel");
+  return with_block_width(val_t, width, who, [&](auto val, auto dp) -> int {
+    using T = decltype(val);
+    constexpr int DP = decltype(dp)::value, WAVES = 4;
+    if (tokens > 0) {
+      if constexpr (kFactored<T>) {
+        hipLaunchKernelGGL((block_amax_kernel<T>), dim3(kAmaxParts), dim3(256), 0, stream, static_cast<const T*>(grad),
+                           tokens * heads * group * width, amax);
+        FS_CHECK_LAUNCH("block_amax_kernel");
+      }
+      p.tiles = block_tiles(*seqs, tokens_of<WAVES>(group));
+      if (p.tiles * heads > kMostWorkgroups) return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
+      hipLaunchKernelGGL((block_query_grad_kernel<T, DP, WAVES>), dim3((uint32_t)(p.tiles * heads)), dim3(64 * WAVES), 0,
+                         stream, a);
+      FS_CHECK_MAIN_LAUNCH("block_query_grad_kernel");
+    }
+    const int64_t shared = heads / lists;
+    auto keys_of = [&](auto bk) -> int {
+      constexpr int BK = decltype(bk)::value;
+      const int64_t groups = l.pieces * shared * (seqs->block / BK);
+      if (groups > kMostWorkgroups) return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
+      hipLaunchKernelGGL((block_key_grad_kernel<T, DP, BK>), dim3((uint32_t)groups), dim3(256), 0, stream, a);
+      FS_CHECK_LAUNCH("block_key_grad_kernel");
+      return FS_OK;
+    };
+    if (const int rc = seqs->block == 32 ? keys_of(std::integral_constant<int, 32>{})
+                                         : keys_of(std::integral_constant<int, 64>{}))
+      return rc;
+    hipLaunchKernelGGL((block_key_join_kernel<T, DP>), row_grid((l.n_keys * shared) << p.lg_groups), dim3(256), 0, stream,
+                       a);
+    FS_CHECK_LAUNCH("block_key_join_kernel");
+    return FS_OK;
+  });
+}

@@ -1,0 +1,363 @@
+// block_tile.hpp — what the kernels over selected blocks share (block_*.hip): where
+// sequences, pages and blocks lie, a tile of keys or values in LDS, fragments of it,
+// and the softmax of a tile of queries.
+//
+// A matrix instruction takes 16 keys by 16 query rows.  Scores come transposed,
+// keys down and queries across (K Q^T): a lane then holds scores of one query, so
+// its maximum and sum need two exchanges between lanes and no more, and the scores
+// of 4 keys in a row that it holds are, as they lie, the second operand of the
+// product with the values (V^T P^T), whose first operand the LDS read transposes.
+#pragma once
+
+#include <type_traits>
+
+#include "matrix_core.hpp"
+#include "select_rows.hpp"
+
+namespace fs {
+namespace {
+
+constexpr int kMostTop = 128;  // blocks that a query may select
+
+// ---- sequences, pages -----------------------------------------------------------
+
+__device__ inline int clamp_to(int64_t v, int64_t lo, int64_t hi) { return (int)(v < lo ? lo : v > hi ? hi : v); }
+
+// Query tokens and keys of sequence b; of n_seqs the tokens behind the last
+// sequence, without keys.  Offsets are on the device and unchecked: whatever they
+// hold, tokens and rows are within their arrays.
+struct Sequence {
+  int first, count;  // tokens
+  int keys;
+  int64_t row0;  // of the keys, packed
+};
+__device__ inline Sequence sequence_at(const fs_block_seqs& s, int b) {
+  Sequence o;
+  o.keys = 0;
+  o.row0 = 0;
+  if (s.q_offsets == nullptr) {
+    o.first = b;
+    o.count = b < s.n_seqs ? 1 : 0;
+  } else {
+    o.first = b == 0 ? 0 : clamp_to(s.q_offsets[b], 0, s.n_tokens);
+    o.count = (b < s.n_seqs ? clamp_to(s.q_offsets[b + 1], o.first, s.n_tokens) : (int)s.n_tokens) - o.first;
+  }
+  if (b < s.n_seqs) {
+    if (s.pages != nullptr) {
+      const int64_t most = s.pages_per_seq * s.page_size;
+      o.keys = clamp_to(s.k_lengths[b], 0, most < INT32_MAX ? most : INT32_MAX);
+    } else {
+      o.row0 = clamp_to(s.k_offsets[b], 0, s.n_rows);
+      o.keys = clamp_to(s.k_offsets[b + 1], o.row0, s.n_rows) - (int)o.row0;
+    }
+  }
+  return o;
+}
+
+// The sequence and tile of tile i, `per` tokens a tile: sequences in order, the
+// tokens behind the last one as one more.  false: there is no such tile.
+// (All lanes alike.)
+__device__ inline bool find_tile(const fs_block_seqs& s, int per, int64_t i, int lane, int& seq, int& tile) {
+  if (s.q_offsets == nullptr) {
+    seq = (int)i;
+    tile = 0;
+    return i < s.n_seqs;
+  }
+  int64_t before = 0;
+  for (int64_t b0 = 0; b0 <= s.n_seqs; b0 += 64) {
+    const int64_t b = b0 + lane;
+    const int own = b <= s.n_seqs ? (sequence_at(s, (int)b).count + per - 1) / per : 0;
+    const int64_t upto = (int64_t)wave_sum_scan((uint32_t)own) + before;
+    const uint64_t m = __ballot(upto > i);
+    if (m != 0) {
+      const int l = __builtin_ctzll(m);
+      seq = (int)b0 + l;
+      tile = (int)(i - before) - (__builtin_amdgcn_readlane((int)(upto - before), l) - __builtin_amdgcn_readlane(own, l));
+      return true;
+    }
+    before += __builtin_amdgcn_readlane((int)(upto - before), 63);
+  }
+  return false;
+}
+
+// A cache's or packed rows' layout: distances in elements.
+struct RowLayout {
+  const void* base;
+  int64_t page, row, head;
+};
+
+// First element of 16 keys that begin at position j (a multiple of 16) of a
+// sequence, or null where their page is outside the cache.
+template <class T>
+__device__ inline const T* key_rows(const fs_block_seqs& s, const Sequence& q, int seq, const RowLayout& l, int head,
+                                    int j) {
+  const T* base = static_cast<const T*>(l.base) + (int64_t)head * l.head;
+  if (s.pages == nullptr) return base + (q.row0 + j) * l.row;
+  const int64_t at = j >> s.page_shift;
+  if (at >= s.pages_per_seq) return nullptr;
+  const int64_t page = s.pages[(int64_t)seq * s.ld_pages + at];
+  if (page < 0 || page >= s.n_pages) return nullptr;
+  return base + page * l.page + (int64_t)(j & (s.page_size - 1)) * l.row;
+}
+
+// ---- tiles in LDS ---------------------------------------------------------------
+
+typedef __attribute__((address_space(3))) uint32_t lds_word;
+typedef __attribute__((address_space(3))) const uint8_t clds_byte;
+
+__device__ inline uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+
+// Rows of DP elements (a head's width, filled up), 16-byte pieces exchanged within
+// a row so that neither a fragment of 16 rows by one piece nor a transposing read
+// of 4 rows by 32 bytes meets a bank twice.
+template <class T, int DP>
+struct Rows {
+  static constexpr int kRow = DP * (int)sizeof(T);  // bytes: 128, 256 or 512
+  static constexpr int kPieces = kRow / 16;
+  static constexpr int kUnit = sizeof(T) == 2 ? 32 : 16;  // rows that one product over rows takes
+  static constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // keys a step
+  static constexpr int kGroups = kKeys / 16;
+  static constexpr int kBytes = kKeys * kRow;
+  static constexpr int kFrags = kRow / 64;     // fragments of 16 rows
+  static constexpr int kTiles = DP / 16;       // tiles of 16 columns
+  using frag = typename Mma<T>::frag;
+
+  __device__ static int swizzle(int row) {
+    if constexpr (sizeof(T) == 4) return ((row >> 2) & 3) * 4 + (row & 3);
+    else if constexpr (kRow == 128) return ((row >> 1) & 3) * 2 + ((row >> 3) & 1);
+    else return (row & 7) * 2 + ((row >> 3) & 1);
+  }
+
+  // One load instruction: 64 lanes' pieces of kAtOnce rows.
+  static constexpr int kAtOnce = 64 / kPieces;
+  __device__ static int lane_row(int lane) { return lane / kPieces; }
+
+  // Fragment of rows r0 .. r0 + 15 (a multiple of 16), column piece 4 ks + lane / 16.
+  __device__ static frag across(uint32_t lds, int r0, int ks, int lane) {
+    const int i = lane & 15, g = lane >> 4;
+    const uint32_t at = lds + (uint32_t)(r0 * kRow) + (uint32_t)(i * kRow) +
+                        (uint32_t)(((ks << 2) ^ (g ^ swizzle(i))) << 4);
+    const u32x4 v = *(const lds_u32x4*)(lds_byte*)(uintptr_t)at;
+    frag f;
+    __builtin_memcpy(&f, &v, 16);
+    return f;
+  }
+  // Fragment of columns 16 dt .. 16 dt + 15 over kUnit rows from r0: lane i of its
+  // 16 has column i of rows 4 g .. 4 g + 3 (16-bit values: and of those 16 further).
+  __device__ static frag down(uint32_t lds, int r0, int dt, int lane) {
+    const int i = lane & 15, g = lane >> 4;
+    frag f;
+    if constexpr (sizeof(T) == 2) {
+      const int r = 4 * g + (i >> 2);
+      const uint32_t at = lds + (uint32_t)(r0 * kRow) + (uint32_t)(r * kRow) +
+                          (uint32_t)((((dt << 1) ^ ((i & 3) >> 1) ^ swizzle(r)) << 4) + (i & 1) * 8);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_byte*)(uintptr_t)at);
+      const s16x4 hi =
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_byte*)(uintptr_t)(at + 16 * kRow));
+      __builtin_memcpy(&f, &lo, 8);
+      __builtin_memcpy((char*)&f + 8, &hi, 8);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * g + j;
+        const uint32_t at = lds + (uint32_t)(r0 * kRow) + (uint32_t)(r * kRow) +
+                            (uint32_t)((((dt << 2) + (i >> 2)) ^ swizzle(r)) << 4) + (uint32_t)(i & 3) * 4;
+        f[j] = *(const lds_float*)(lds_byte*)(uintptr_t)at;
+      }
+    }
+    return f;
+  }
+  // The other operand: values of kUnit rows that products of 16 rows left, rounded
+  // to the value type.
+  __device__ static frag rounded(const f32x4* s) {
+    frag f;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[j] = (T)s[0][j];
+        f[4 + j] = (T)s[1][j];
+      }
+    } else {
+      f = s[0];
+    }
+    return f;
+  }
+};
+
+// The largest, and the sum, of a value over the four lanes of a query.
+__device__ inline float across_max(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ inline float across_sum(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+// What the kernels of queries take.
+struct BlockArgs {
+  fs_block_seqs seqs;
+  RowLayout k, v;
+  const void* q;
+  int64_t q_token, q_head;  // distances in elements
+  void* out;                // tokens x heads * group x width, dense
+  float* lse;               // tokens x heads * group; may be null
+  const int32_t* blocks;
+  int64_t b_token, b_head;
+  int top, heads, group, width;
+  int lg_groups;  // log2 of a block's groups of 16 keys
+  float scale;
+  int64_t tiles;  // workgroups a head
+  int splits;
+  float* parts;
+  // gradients
+  const void* grad;
+  const void* o;
+  const float* lse_in;
+  float* delta;
+  const float* factor;
+};
+
+// The loads of one step's keys or values: rows of `lds`, zeros past the sequence's
+// keys, past the width and for pages outside the cache.  Wave w of WAVES takes its
+// share.  entry(group) gives the block of a group of 16 keys, negative for none.
+template <class T, int DP, int WAVES, class Entry>
+__device__ inline void load_rows(const BlockArgs& p, const RowLayout& l, const Sequence& sq, int seq, int head,
+                                 uint32_t lds, int w, int lane, Entry entry) {
+  using R = Rows<T, DP>;
+  constexpr int kLoads = R::kBytes / 1024 / WAVES;
+  static_assert(R::kBytes % (1024 * WAVES) == 0, "whole loads a wave");
+  const int r = R::lane_row(lane), pos = lane % R::kPieces;
+#pragma unroll
+  for (int n = 0; n < kLoads; ++n) {
+    const int row0 = (w * kLoads + n) * R::kAtOnce, gr = row0 / 16;
+    const int first = entry(gr);  // position of the group's first key
+    const int row = row0 % 16 + r;
+    const int piece = pos ^ R::swizzle(row);
+    const T* base = first >= 0 ? key_rows<T>(p.seqs, sq, seq, l, head, first) : nullptr;
+    const bool in = base != nullptr && first + row < sq.keys && piece * 16 < p.width * (int)sizeof(T);
+    const uint32_t off = in ? (uint32_t)(row * l.row * (int64_t)sizeof(T)) + (uint32_t)piece * 16 : 2u * kInBuffer;
+    lds_dma<16>((uint32_t)__builtin_amdgcn_readfirstlane((int)(lds + (uint32_t)row0 * R::kRow)), off,
+                buffer_at(base != nullptr ? base : l.base));
+  }
+}
+
+// Which groups of 16 keys of a step lie in pages outside the cache, a bit each.
+template <class T, int DP, class Entry>
+__device__ inline uint32_t missing_pages(const BlockArgs& p, const Sequence& sq, int seq, Entry entry) {
+  uint32_t m = 0;
+  if (p.seqs.pages != nullptr) {
+#pragma unroll
+    for (int gr = 0; gr < Rows<T, DP>::kGroups; ++gr) {
+      const int first = entry(gr);
+      if (first >= 0 && key_rows<T>(p.seqs, sq, seq, p.k, 0, first) == nullptr) m |= 1u << gr;
+    }
+  }
+  return m;
+}
+
+// 16 query rows of a wave: lanes with the same lane % 16 hold one row's state.
+struct RowOf {
+  int token;  // within the workgroup's tile
+  int head;   // within the group
+  int pos;    // its position; -1 and less: before the first key
+  bool in;
+};
+
+// Fragments of a lane's row of a dense or strided array, zeros outside.
+template <class T, int DP>
+__device__ inline void load_row(const T* row, bool in, int width, int lane,
+                                typename Mma<T>::frag (&f)[Rows<T, DP>::kFrags]) {
+#pragma unroll
+  for (int ks = 0; ks < Rows<T, DP>::kFrags; ++ks) {
+    const int piece = ks * 4 + (lane >> 4);
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (in && piece * 16 < width * (int)sizeof(T)) __builtin_memcpy(&v, (const char*)row + piece * 16, 16);
+    __builtin_memcpy(&f[ks], &v, 16);
+  }
+}
+
+// Columns 16 dt + 4 g .. + 3 of a lane's row.
+template <class T, int DP>
+__device__ inline void store_row(T* row, const f32x4 (&o)[DP / 16], float by, int width, int lane) {
+#pragma unroll
+  for (int dt = 0; dt < DP / 16; ++dt) {
+    const int d = dt * 16 + (lane >> 4) * 4;
+    if (d < width) {  // (a multiple of 4)
+      T e[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) e[j] = (T)(o[dt][j] * by);
+      __builtin_memcpy(row + d, e, sizeof e);
+    }
+  }
+}
+
+// ---- host side ------------------------------------------------------------------
+
+constexpr int64_t kMostWorkgroups = ((int64_t)1 << 32) / 512 - 1;  // of 256 threads, in one dimension
+
+inline int64_t block_tiles(const fs_block_seqs& s, int per) {
+  return s.q_offsets == nullptr ? s.n_seqs : s.n_tokens / per + s.n_seqs + 1;
+}
+
+inline int block_seqs_fault(const char* who, const fs_block_seqs* s) {
+  auto refuse = [&](const char* text) { return fail(FS_E_INVALID, std::string(who) + ": " + text); };
+  if (s == nullptr) return refuse("null pointer");
+  if (s->n_seqs < 0 || s->n_seqs > INT32_MAX / 2 || s->n_tokens < 0 || s->n_tokens > INT32_MAX || s->n_rows < 0 ||
+      s->n_rows > INT32_MAX)
+    return refuse("sizes out of range");
+  if (s->block < 32 || s->block > 1024 || (s->block & (s->block - 1)) != 0)
+    return refuse("blocks are of 32, 64, 128, 256, 512 or 1024 keys");
+  if (s->q_offsets == nullptr && s->n_tokens != s->n_seqs) return refuse("without offsets a sequence has one token");
+  if (s->pages != nullptr) {
+    if (s->k_lengths == nullptr && s->n_seqs > 0) return refuse("null pointer");
+    if (s->page_size < 16 || s->page_size > (1 << 20) || (s->page_size & (s->page_size - 1)) != 0 ||
+        s->page_shift != __builtin_ctz((unsigned)s->page_size))
+      return refuse("pages are of a power of two of rows, 16 at least");
+    if (s->n_pages < 0 || s->pages_per_seq < 0 || s->ld_pages < 0) return refuse("sizes out of range");
+  } else if (s->k_offsets == nullptr && s->n_seqs > 0) {
+    return refuse("null pointer");
+  }
+  return FS_OK;
+}
+
+inline int block_sizes_fault(const char* who, int val_t, const fs_block_seqs* s, int heads, int group, int width) {
+  if (const int rc = block_seqs_fault(who, s)) return rc;
+  auto refuse = [&](const char* text) { return fail(FS_E_INVALID, std::string(who) + ": " + text); };
+  if (val_t != FS_F16 && val_t != FS_BF16 && val_t != FS_F32) return refuse("value types are FS_F16, FS_BF16 and FS_F32");
+  if (heads < 1 || heads > 65535 || group < 1 || group > 128) return refuse("heads out of range");
+  if (width < 8 || width % 8 != 0 || width > (val_t == FS_F32 ? 128 : 256)) return refuse("width out of range");
+  return FS_OK;
+}
+
+// Whether loads of 16 bytes can take the rows, and the distances of 64 of them fit.
+inline bool block_rows_fit(const void* base, int64_t page, int64_t row, int64_t head, int64_t size) {
+  if (page < 0 || row < 0 || head < 0 || row > ((int64_t)1 << 22)) return false;
+  return (((int64_t)(uintptr_t)base | page * size | row * size | head * size) & 15) == 0;
+}
+
+// Runs f with a value of the value type and the width filled up.
+template <class F>
+int with_block_width(int val_t, int width, const char* who, F&& f) {
+  auto by_width = [&](auto v) -> int {
+    using T = decltype(v);
+    if (width <= 64) return f(v, std::integral_constant<int, 64>{});
+    if (width <= 128) return f(v, std::integral_constant<int, 128>{});
+    if constexpr (sizeof(T) == 2) return f(v, std::integral_constant<int, 256>{});
+    return fail(FS_E_INVALID, std::string(who) + ": width out of range");
+  };
+  if (val_t == FS_F16) return by_width((_Float16)0);
+  if (val_t == FS_BF16) return by_width((__bf16)0);
+  return by_width(0.0f);
+}
+
+}  // namespace
+}  // namespace fs

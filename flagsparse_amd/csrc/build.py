@@ -24,7 +24,8 @@ BUILD_DIR = os.path.join(HERE, "_build")
 
 SOURCES = ["abi.cpp", "spmv.hip", "spmv_opt.hip", "spmv_scatter.hip", "spmv_gather.hip", "spmm.hip", "spmm_group.hip",
            "spmm_half.hip", "transpose.hip", "sell.hip", "select_sort.hip", "embedding.hip", "expert_rows.hip",
-           "expert_product.hip"]
+           "expert_product.hip", "block_means.hip",
+           "block_select.hip", "block_attention.hip", "block_attention_grad.hip"]
 # the measurement-only library (bench.py --gather-floor), with its own copy of
 # the error reporting
 DIAG_OUT = os.path.join(PKG, "libflagsparse_diag.so")

@@ -28,50 +28,13 @@
 #include <initializer_list>
 #include <type_traits>
 
+#include "matrix_core.hpp"
 #include "select_rows.hpp"
 
 namespace fs {
 namespace {
 
 constexpr int kRowBytes = 64;  // k of one step, of an operand contiguous in k
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) uint8_t lds_byte;
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
-typedef __attribute__((address_space(3))) float lds_float;
-
-template <class T>
-struct Mma;
-template <>
-struct Mma<_Float16> {
-  using frag = f16x8;
-  __device__ static f32x4 run(frag a, frag b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-  }
-};
-template <>
-struct Mma<__bf16> {
-  using frag = bf16x8;
-  __device__ static f32x4 run(frag a, frag b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-  }
-};
-template <>
-struct Mma<float> {
-  using frag = f32x4;  // four steps of one k a lane
-  __device__ static f32x4 run(frag a, frag b, f32x4 c) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-    return c;
-  }
-};
 
 // One operand's slice in LDS, and the way there.  KC: contiguous in k, R rows
 // of the tile by 64 bytes of k; otherwise BK rows of k by R elements.
@@ -225,26 +188,6 @@ __device__ inline void store_pieces(const Source<T>& s, int64_t kt, uint32_t lds
 // with WIDTH 16 190); 16-bit rows off whole words go through registers.
 // Offsets below kInBuffer count from the step's base, which moves; a load
 // outside the operand gets one beyond it, and writes zeros.
-constexpr uint32_t kInBuffer = 1u << 30;
-
-// (No register is written, so none is taken too early; M0 has no other use here.)
-template <int WIDTH>
-__device__ inline void lds_dma(uint32_t lds, uint32_t offset, u32x4 rsrc) {
-  if constexpr (WIDTH == 16)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset),
-                 "s"(rsrc)
-                 : "memory");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset),
-                 "s"(rsrc)
-                 : "memory");
-}
-__device__ inline u32x4 buffer_at(const void* p) {
-  const uint64_t a = (uint64_t)(uintptr_t)p;
-  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
-               (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)) & 0xffffu, kInBuffer, 0x00020000u};
-}
-
 template <class O, class T, bool KC, int THREADS, int WIDTH>
 struct Dma {
   static constexpr int kLoads = O::kBytes / THREADS / WIDTH;  // a thread's, each step
@@ -277,21 +220,6 @@ struct Dma {
     lds_dma<WIDTH>(lds + (uint32_t)(i * THREADS + w * 64) * WIDTH, off[i], rsrc);
   }
 };
-
-// Waits and the barrier, which nothing is moved across.
-template <int LEFT>
-__device__ inline void wait_loads() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
-}
-__device__ inline void wait_reads() {
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-}
-__device__ inline void barrier() {
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_barrier" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-}
 
 struct ProductArgs {
   const void* a;

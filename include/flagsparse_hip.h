@@ -658,6 +658,96 @@ int fs_expert_product_grad_matrices(int val_t, int trans, int64_t n_rows, int64_
                                     const void* rows, int64_t ldr, const int32_t* offsets,
                                     void* grad_matrices, void* ws, size_t ws_bytes, hipStream_t stream);
 
+/* ---- attention over selected blocks of keys ----
+ *
+ * The reference has no counterpart.  Values are FS_F16, FS_BF16 or FS_F32; sums,
+ * maxima and softmax statistics are held in 32 bits, in a fixed order.
+ *
+ * Sequences: n_seqs of them, the query tokens of sequence b are q_offsets[b] to
+ * q_offsets[b + 1] - 1 of n_tokens, or, without q_offsets, token b alone.  They are
+ * the sequence's last positions: token i of n has position keys - n + i (below
+ * zero: before the first key) and sees the keys up to its own position.  The keys
+ * are the rows k_offsets[b] to k_offsets[b + 1] - 1 of n_rows packed rows; or, with
+ * pages, the first k_lengths[b] rows of the pages that pages[b * ld_pages + ...]
+ * (pages_per_seq of them) names, page_size rows each, of a cache of n_pages.
+ * Block i of a sequence is its keys i * block to (i + 1) * block - 1.
+ * Offsets begin at 0 and do not decrease; all of them, the lengths and the pages
+ * are on the device and are not checked, but whatever they hold nothing outside the
+ * arrays is read or written.  A page outside the cache holds no keys; tokens
+ * behind the last sequence have none.
+ */
+typedef struct fs_block_seqs {
+  int64_t n_seqs, n_tokens, n_rows; /* n_rows: packed rows of keys */
+  const int32_t* q_offsets;         /* n_seqs + 1, or null */
+  const int32_t* k_offsets;         /* n_seqs + 1; packed rows */
+  const int32_t* k_lengths;         /* n_seqs; pages */
+  const int32_t* pages;
+  int64_t ld_pages, pages_per_seq, n_pages;
+  int32_t page_size, page_shift;    /* a power of two, 16 or more; its logarithm */
+  int32_t block, reserved;          /* 32, 64, ..., 1024 */
+} fs_block_seqs;
+
+/*
+ * The mean of each block's keys (of those it holds; zero where it holds none), summed in 32 bits, to
+ * out[b * m_seq + i * m_block + h * m_head], i < most, of heads rows of width
+ * elements a key.  With start (n_seqs), only blocks that hold a key at start[b] or
+ * behind it are written; blocks without keys never are.
+ */
+int fs_block_means(int val_t, const fs_block_seqs* seqs, int heads, int width, const void* k,
+                   int64_t k_page, int64_t k_row, int64_t k_head, const int32_t* start,
+                   int64_t most, void* out, int64_t m_seq, int64_t m_block, int64_t m_head,
+                   hipStream_t stream);
+/*
+ * The blocks of each token and key-value head, out (tokens x heads x top), ascending,
+ * -1 behind them: the sequence's first `first` blocks and the `recent` ones up to the
+ * token's own, and of the others before those that have the largest scores
+ * <sum of the group's q[t], means[b, i, h]>, computed in 64 bits; equal ones by
+ * their number, not-a-numbers last.  Blocks from `most` on have no score.
+ * first + recent <= top <= 128, recent >= 1.  Means of blocks in front of the recent
+ * ones alone are read.
+ */
+int fs_block_select(int val_t, const fs_block_seqs* seqs, int heads, int group, int width,
+                    const void* q, int64_t q_token, int64_t q_head, const void* means,
+                    int64_t most, int64_t m_seq, int64_t m_block, int64_t m_head, int top,
+                    int first, int recent, int32_t* out, hipStream_t stream);
+/*
+ * out[t, h] = softmax over the keys j that token t's blocks hold (scale <q[t, h],
+ * k[j, h / group]>) times v[j, h / group], for the heads * group heads h of a
+ * token: blocks[t * b_token + (h / group) * b_head + i], i < top <= 128, names
+ * blocks of t's sequence.  A block named twice counts once, a negative one or one
+ * behind the token's own not at all; a token without keys gets zeros.  out is
+ * dense, tokens x heads * group x width; lse (may be null) gets the logarithm of the
+ * sum of the exponentials, minus infinity without keys.  Strides are in elements;
+ * rows of width elements are contiguous, those of keys and values at multiples of
+ * 16 bytes; width is a multiple of 8, up to 256 (FS_F32: 128); group <= 128.
+ * k_page and v_page are read with pages alone.
+ */
+size_t fs_block_attention_workspace_bytes(int val_t, const fs_block_seqs* seqs, int heads,
+                                          int group, int width, int top);
+int fs_block_attention(int val_t, const fs_block_seqs* seqs, int heads, int group, int width,
+                       int top, const void* q, int64_t q_token, int64_t q_head, const void* k,
+                       int64_t k_page, int64_t k_row, int64_t k_head, const void* v,
+                       int64_t v_page, int64_t v_row, int64_t v_head, const int32_t* blocks,
+                       int64_t b_token, int64_t b_head, double scale, void* out, float* lse,
+                       void* ws, size_t ws_bytes, hipStream_t stream);
+/*
+ * Its gradients in queries, keys and values of packed rows, from grad, out and lse
+ * (dense; out and lse as fs_block_attention wrote them).  dq is dense, tokens x
+ * heads * group x width; dk and dv are n_rows x heads x width, zero in rows of no
+ * sequence and of keys that no token sees.  lists is heads, or 1 where the heads
+ * share a selection.  Rows of queries and of grad lie at multiples of 16 bytes too.
+ * tokens * lists * top is below 2^31.
+ */
+size_t fs_block_attention_grad_workspace_bytes(int val_t, const fs_block_seqs* seqs, int heads,
+                                               int group, int width, int lists, int top);
+int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int heads, int group, int width,
+                            int lists, int top, const void* grad, const void* q, int64_t q_token,
+                            int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                            const void* v, int64_t v_row, int64_t v_head, const int32_t* blocks,
+                            int64_t b_token, int64_t b_head, double scale, const void* out,
+                            const float* lse, void* dq, void* dk, void* dv, void* ws,
+                            size_t ws_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
