@@ -246,9 +246,11 @@ def prepare(case, seed):
     if own:
         import flagsparse_amd as fs
 
+        # (the selection reads no keys, only how many there are)
+        paged = "pages" in a
         state["seqs"] = fs.prepare_block_sequences(case["block"], q_offsets=a["q_offsets"],
-                                                   k_offsets=a.get("k_offsets"), pages=a.get("pages"),
-                                                   k_lengths=a["k_lengths"] if case["page"] else None)
+                                                   k_offsets=None if paged else _offsets(lengths),
+                                                   pages=a.get("pages"), k_lengths=a["k_lengths"] if paged else None)
     else:
         state["seq"], state["pos"] = _positions(lengths, new)
     if case["call"] == "means":
