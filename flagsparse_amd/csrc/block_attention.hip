@@ -10,98 +10,97 @@
 namespace fs {
 namespace {
 
+// A wave's 16 rows: a lane has a part of row lane % 16.
 template <class T, int DP>
 struct Online {
-  typename Mma<T>::frag q[2][Rows<T, DP>::kFrags];
-  f32x4 o[2][DP / 16];  // columns 16 dt + 4 g .. of the lane's row
-  float m[2], l[2];     // maximum in powers of two, and the lane's own part of the sum
+  typename Mma<T>::frag q[Rows<T, DP>::kFrags];
+  f32x4 o[DP / 16];  // columns 16 dt + 4 g ..
+  float m, l;        // maximum in powers of two, and the lane's own part of the sum
 };
 
 template <class T, int DP>
 __device__ inline void start(Online<T, DP>& st) {
+  st.m = -INFINITY;
+  st.l = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    st.m[i] = -INFINITY;
-    st.l[i] = 0.0f;
-#pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt) st.o[i][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  for (int dt = 0; dt < DP / 16; ++dt) st.o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
-// One step's keys and values taken into tiles 0 (A) and 1 (B).
-template <class T, int DP, bool A, bool B>
-__device__ inline void attend(Online<T, DP>& st, uint32_t kb, uint32_t vb,
-                              const bool (&sel)[2][Rows<T, DP>::kGroups],
-                              const int (&first)[Rows<T, DP>::kGroups], bool edge, uint32_t missing,
-                              const RowOf (&row)[2], float c, int lane) {
+// The maximum follows the scores only where it grows by more than this, in powers of
+// two: weights are 2^8 at most, and rescaling is left out of most steps.
+constexpr float kSlack = 8.0f;
+
+// One step's keys and values.
+template <class T, int DP>
+__device__ inline void attend(Online<T, DP>& st, uint32_t kb, uint32_t vb, uint32_t sel, const Halves& now, bool some,
+                              bool edge, uint32_t missing, const RowOf& row, float c, int lane) {
   using R = Rows<T, DP>;
   constexpr int G = R::kGroups, P = R::kUnit / 16;
-  f32x4 s[2][G];
+  f32x4 s[G];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int gr = 0; gr < G; ++gr) s[i][gr] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int gr = 0; gr < G; ++gr) s[gr] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int ks = 0; ks < R::kFrags; ++ks)
 #pragma unroll
+    for (int gr = 0; gr < G; ++gr) s[gr] = Mma<T>::run(R::across(kb, gr * 16, ks, lane), st.q[ks], s[gr]);
+  if (edge) {
+#pragma unroll
     for (int gr = 0; gr < G; ++gr) {
-      const auto k = R::across(kb, gr * 16, ks, lane);
-      if (A) s[0][gr] = Mma<T>::run(k, st.q[0][ks], s[0][gr]);
-      if (B) s[1][gr] = Mma<T>::run(k, st.q[1][ks], s[1][gr]);
+      const int last = (missing >> gr) & 1u ? -1 : row.pos - now.of<T, DP>(gr) - 4 * (lane >> 4);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[gr][r] = r <= last ? s[gr][r] : -INFINITY;
     }
-  typename R::frag w[2][G / P];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (i == 0 ? !A : !B) continue;
-    float most = -INFINITY;
-#pragma unroll
-    for (int gr = 0; gr < G; ++gr)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        bool in = sel[i][gr];
-        if (edge) in = in && first[gr] + 4 * (lane >> 4) + r <= row[i].pos && !((missing >> gr) & 1u);
-        s[i][gr][r] = in ? s[i][gr][r] : -INFINITY;
-        most = fmaxf(most, s[i][gr][r]);
-      }
-    const float m = fmaxf(st.m[i], across_max(most) * c);
-    const float base = m == -INFINITY ? 0.0f : m;  // (a row without keys yet)
-    if (__ballot(m != st.m[i]) != 0) {
-      const float by = __builtin_amdgcn_exp2f(st.m[i] - base);
-      st.l[i] *= by;
-#pragma unroll
-      for (int dt = 0; dt < DP / 16; ++dt) st.o[i][dt] *= by;
-      st.m[i] = m;
-    }
-    float sum = 0.0f;
-#pragma unroll
-    for (int gr = 0; gr < G; ++gr)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][gr][r], c, -base));
-        sum += x;
-        s[i][gr][r] = x;
-      }
-    st.l[i] += sum;
-    // weights, in [0, 1], in the values' type: off by half a unit in their last place
-    // each, the sum that they are divided by is not
-#pragma unroll
-    for (int u = 0; u < G / P; ++u) w[i][u] = R::rounded(&s[i][u * P]);
   }
+  if (some) {
 #pragma unroll
-  for (int u = 0; u < G / P; ++u)
+    for (int gr = 0; gr < G; ++gr) {
+      const bool in = (sel >> (gr / (G / 2))) & 1u;
 #pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt) {
-      const auto v = R::down(vb, u * R::kUnit, dt, lane);
-      if (A) st.o[0][dt] = Mma<T>::run(v, w[0][u], st.o[0][dt]);
-      if (B) st.o[1][dt] = Mma<T>::run(v, w[1][u], st.o[1][dt]);
+      for (int r = 0; r < 4; ++r) s[gr][r] = in ? s[gr][r] : -INFINITY;
     }
+  }
+  float most = -INFINITY;
+#pragma unroll
+  for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) most = fmaxf(most, s[gr][r]);
+  most = across_max(most) * c;
+  if (__ballot(most > st.m + kSlack) != 0) {
+    // (a row without keys yet: its maximum stays at minus infinity, its sums are zero)
+    const float m = fmaxf(st.m, most);
+    const float by = __builtin_amdgcn_exp2f(st.m - (m == -INFINITY ? 0.0f : m));
+    st.l *= by;
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt) st.o[dt] *= by;
+    st.m = m;
+  }
+  const float base = st.m == -INFINITY ? 0.0f : st.m;
+  float sum = 0.0f;
+#pragma unroll
+  for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[gr][r], c, -base));
+      sum += x;
+      s[gr][r] = x;
+    }
+  st.l += sum;
+  // weights in the values' type: off by half a unit in their last place each, the sum
+  // that they are divided by is not
+#pragma unroll
+  for (int u = 0; u < G / P; ++u) {
+    const auto w = R::rounded(&s[u * P]);
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt)
+      st.o[dt] = Mma<T>::run(R::down(vb, u * R::kUnit, dt, lane), w, st.o[dt]);
+  }
 }
 
 // One row by a wave, key after key, without products of what is left out: a weight
 // of zero times a value that is not finite would be NaN.  Taken where a result is
 // not finite, whoever's it is.
 template <class T, int DP>
-__device__ __noinline__ void careful_row(const BlockArgs& p, const Sequence& sq, int seq, int64_t token, int head,
+__device__ __forceinline__ void careful_row(const BlockArgs& p, const Sequence& sq, int seq, int64_t token, int head,
                                          int in_group, int pos, int lane) {
   const int hq = head * p.group + in_group, block = p.seqs.block, lg = p.lg_groups + 4;
   const T* q = static_cast<const T*>(p.q) + token * p.q_token + (int64_t)hq * p.q_head;
@@ -160,7 +159,7 @@ __device__ __noinline__ void careful_row(const BlockArgs& p, const Sequence& sq,
   if (p.lse != nullptr && lane == 0) p.lse[at] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * kLn2;
 }
 
-// Many queries.
+// Many queries.  A row whose result is not finite is left to the next kernel.
 template <class T, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void block_attention_kernel(const BlockArgs p) {
   using R = Rows<T, DP>;
@@ -169,47 +168,46 @@ __global__ __launch_bounds__(64 * WAVES) void block_attention_kernel(const Block
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   WalkTile t;
   if (!walk_tile<WAVES>(p, lane, t)) return;
-  RowOf row[2];
-  rows_of<WAVES>(p, t, w, lane, row);
+  const RowOf row = row_of(p, t, w, lane);
   Online<T, DP> st;
   start(st);
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    load_row<T, DP>(static_cast<const T*>(p.q) + (int64_t)(t.token0 + row[i].token) * p.q_token +
-                        (int64_t)(t.head * p.group + row[i].head) * p.q_head,
-                    row[i].in, p.width, lane, st.q[i]);
+  const int64_t at = (int64_t)(t.token0 + row.token) * p.heads * p.group + t.head * p.group + row.head;
+  load_row<T, DP>(static_cast<const T*>(p.q) + (int64_t)(t.token0 + row.token) * p.q_token +
+                      (int64_t)(t.head * p.group + row.head) * p.q_head,
+                  row.in, p.width, lane, st.q);
   const float c = p.scale * kLog2e;
-  walk_blocks<T, DP, WAVES>(
-      p, t, row, s_walk, s_kv, tid, w, lane,
-      [&](const Step<T, DP>& now, const bool(&sel)[2][R::kGroups], bool a, bool b, bool edge, uint32_t kb, uint32_t vb) {
-        if (a && b) attend<T, DP, true, true>(st, kb, vb, sel, now.first, edge, now.missing, row, c, lane);
-        else if (a) attend<T, DP, true, false>(st, kb, vb, sel, now.first, edge, now.missing, row, c, lane);
-        else attend<T, DP, false, true>(st, kb, vb, sel, now.first, edge, now.missing, row, c, lane);
-      });
+  walk_blocks<T, DP, WAVES>(p, t, row, s_walk, s_kv, tid, w, lane,
+                            [&](const Halves& now, uint32_t sel, bool some, bool edge, uint32_t missing, uint32_t kb,
+                                uint32_t vb) { attend<T, DP>(st, kb, vb, sel, now, some, edge, missing, row, c, lane); });
+  const float l = across_sum(st.l), by = l > 0.0f ? 1.0f / l : 0.0f;
+  bool bad = !__builtin_isfinite(l);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float l = across_sum(st.l[i]), by = l > 0.0f ? 1.0f / l : 0.0f;
-    bool bad = !__builtin_isfinite(l);
+  for (int dt = 0; dt < DP / 16; ++dt)
 #pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) bad |= !__builtin_isfinite(st.o[i][dt][r]);
-    uint64_t rows = __ballot(bad && row[i].in);
-    rows = (rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xffffu;
-    const int64_t at = (int64_t)(t.token0 + row[i].token) * p.heads * p.group + t.head * p.group + row[i].head;
-    if (row[i].in && !((rows >> (lane & 15)) & 1)) {
-      store_row<T, DP>(static_cast<T*>(p.out) + at * p.width, st.o[i], by, p.width, lane);
-      if (p.lse != nullptr && lane < 16) p.lse[at] = l > 0.0f ? (st.m[i] + __builtin_log2f(l)) * kLn2 : -INFINITY;
-    }
-    for (; rows != 0; rows &= rows - 1) {
-      const int r = __builtin_ctzll(rows), tok = __builtin_amdgcn_readlane(row[i].token, r);
-      careful_row<T, DP>(p, t.sq, t.seq, t.token0 + tok, t.head, __builtin_amdgcn_readlane(row[i].head, r),
-                         t.pos0 + tok, lane);
-    }
+    for (int r = 0; r < 4; ++r) bad |= !__builtin_isfinite(st.o[dt][r]);
+  const uint64_t rows = __ballot(bad && row.in);
+  if (row.in) {
+    store_row<T, DP>(static_cast<T*>(p.out) + at * p.width, st.o, by, p.width, lane);
+    if (p.lse != nullptr && lane < 16) p.lse[at] = l > 0.0f ? (st.m + __builtin_log2f(l)) * kLn2 : -INFINITY;
+  }
+  if (lane == 0)
+    p.again[(int64_t)blockIdx.x * WAVES + w] = (uint32_t)(rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xffffu;
+}
+
+// Those rows, key after key.
+template <class T, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void block_attention_again_kernel(const BlockArgs p) {
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  WalkTile t;
+  if (!walk_tile<WAVES>(p, lane, t)) return;
+  uint32_t rows = alike((int)p.again[(int64_t)blockIdx.x * WAVES + w]);
+  for (; rows != 0; rows &= rows - 1) {
+    const int r = w * 16 + __builtin_ctz(rows), tok = r / p.group;
+    careful_row<T, DP>(p, t.sq, t.seq, t.token0 + tok, t.head, r - tok * p.group, t.pos0 + tok, lane);
   }
 }
 
-// Few queries: a workgroup takes one token's rows of a group, up to 32 of them, and
+// Few queries: a workgroup takes one token's rows of a group, up to 16 of them, and
 // its waves the steps of the token's own blocks in turn, each with keys and values of
 // its own in LDS; their states are joined at the end, with `splits` workgroups a
 // token those by the next kernel.
@@ -219,9 +217,9 @@ template <class T, int DP>
 struct FewShape {
   static constexpr int kWaves = DP * (int)sizeof(T) > 256 ? 2 : kFewWaves;
 };
-// (floats of a split's part: maximum and sum of 32 rows, then the rows)
+// (floats of a split's part: maximum and sum of 16 rows, then the rows)
 template <int DP>
-__host__ __device__ constexpr int part_floats() { return 64 + 32 * DP; }
+__host__ __device__ constexpr int part_floats() { return 32 + 16 * DP; }
 
 struct FewPlace {
   int64_t token;
@@ -231,7 +229,7 @@ __device__ inline FewPlace few_place(const BlockArgs& p, int64_t at) {
   FewPlace f;
   f.split = (int)(at % p.splits);
   at /= p.splits;
-  const int chunks = (p.group + 31) / 32;
+  const int chunks = (p.group + 15) / 16;
   f.chunk = (int)(at % chunks);
   at /= chunks;
   f.head = (int)(at % p.heads);
@@ -259,20 +257,20 @@ __device__ inline bool token_at(const fs_block_seqs& s, int64_t token, int lane,
     }
   }
   if (seq >= s.n_seqs) return false;
-  sq = sequence_at(s, seq);
+  sq = sequence_of(s, seq);
   pos = sq.keys - sq.count + (int)(token - sq.first);
   return true;
 }
 
 // Rows of one token and chunk from the states of `n` waves or splits: part(i) gives
-// the i-th one's 32 maxima, 32 sums and 32 rows.
+// the i-th one's 16 maxima, 16 sums and 16 rows.
 template <class T, int DP, int THREADS, class Part>
 __device__ inline void join_rows(const BlockArgs& p, const FewPlace& f, int seq, const Sequence& sq, int pos, int n,
                                  int tid, int* s_bad, Part part) {
-  const int rows = p.group - f.chunk * 32 < 32 ? p.group - f.chunk * 32 : 32;
+  const int rows = p.group - f.chunk * 16 < 16 ? p.group - f.chunk * 16 : 16;
   const int fours = p.width / 4;
   int any = 0;
-  if (tid < 32) s_bad[tid] = 0;
+  if (tid < 16) s_bad[tid] = 0;
   __syncthreads();
   for (int e = tid; e < rows * fours; e += THREADS) {
     const int r = e / fours, d = (e - r * fours) * 4;
@@ -282,9 +280,9 @@ __device__ inline void join_rows(const BlockArgs& p, const FewPlace& f, int seq,
     for (int i = 0; i < n; ++i) {
       const float* x = part(i);
       const float by = __builtin_amdgcn_exp2f(x[r] - base);
-      l = __builtin_fmaf(by, x[32 + r], l);
+      l = __builtin_fmaf(by, x[16 + r], l);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = __builtin_fmaf(by, x[64 + r * DP + d + j], o[j]);
+      for (int j = 0; j < 4; ++j) o[j] = __builtin_fmaf(by, x[32 + r * DP + d + j], o[j]);
     }
     const float by = l > 0.0f ? 1.0f / l : 0.0f;
     bool bad = !__builtin_isfinite(l);
@@ -294,7 +292,7 @@ __device__ inline void join_rows(const BlockArgs& p, const FewPlace& f, int seq,
       bad |= !__builtin_isfinite(o[j]);
       out[j] = (T)(o[j] * by);
     }
-    const int64_t at = (f.token * p.heads + f.head) * p.group + f.chunk * 32 + r;
+    const int64_t at = (f.token * p.heads + f.head) * p.group + f.chunk * 16 + r;
     __builtin_memcpy(static_cast<T*>(p.out) + at * p.width + d, out, sizeof out);
     if (p.lse != nullptr && d == 0) p.lse[at] = l > 0.0f ? (m + __builtin_log2f(l)) * kLn2 : -INFINITY;
     if (bad) any = s_bad[r] = 1;
@@ -303,25 +301,25 @@ __device__ inline void join_rows(const BlockArgs& p, const FewPlace& f, int seq,
   __threadfence();  // the rows above are written before they are written again
   __syncthreads();
   for (int r = tid >> 6; r < rows; r += THREADS / 64)
-    if (s_bad[r]) careful_row<T, DP>(p, sq, seq, f.token, f.head, f.chunk * 32 + r, pos, tid & 63);
+    if (s_bad[r]) careful_row<T, DP>(p, sq, seq, f.token, f.head, f.chunk * 16 + r, pos, tid & 63);
 }
 
 template <class T, int DP>
 __device__ inline void zero_rows(const BlockArgs& p, const FewPlace& f, int tid, int threads) {
-  const int rows = p.group - f.chunk * 32 < 32 ? p.group - f.chunk * 32 : 32;
-  const int64_t at = (f.token * p.heads + f.head) * p.group + f.chunk * 32;
+  const int rows = p.group - f.chunk * 16 < 16 ? p.group - f.chunk * 16 : 16;
+  const int64_t at = (f.token * p.heads + f.head) * p.group + f.chunk * 16;
   for (int e = tid; e < rows * p.width; e += threads) static_cast<T*>(p.out)[at * p.width + e] = (T)0.0f;
   if (p.lse != nullptr && tid < rows) p.lse[at + tid] = -INFINITY;
 }
 
-template <class T, int DP, bool TWO>
+template <class T, int DP>
 __global__ __launch_bounds__((64 * FewShape<T, DP>::kWaves)) void block_attention_few_kernel(const BlockArgs p) {
   using R = Rows<T, DP>;
-  constexpr int WAVES = FewShape<T, DP>::kWaves, THREADS = 64 * WAVES, G = R::kGroups;
+  constexpr int WAVES = FewShape<T, DP>::kWaves, THREADS = 64 * WAVES;
   static_assert(part_floats<DP>() * 4 <= 2 * R::kBytes, "a wave's state fits where its keys were");
   __shared__ alignas(1024) uint8_t s_kv[WAVES][2][R::kBytes];
   __shared__ int s_ids[kMostTop];
-  __shared__ int s_count, s_bad[32];
+  __shared__ int s_count, s_bad[16];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const FewPlace f = few_place(p, row_block());
   if (f.token >= p.seqs.n_tokens) return;
@@ -331,7 +329,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP>::kWaves)) void block_attentio
     if (f.split == 0) zero_rows<T, DP>(p, f, tid, THREADS);
     return;
   }
-  const int block = p.seqs.block, lg = p.lg_groups + 4;
+  const int lg = p.lg_groups + 4;
   const int32_t* ids = p.blocks + f.token * p.b_token + (int64_t)f.head * p.b_head;
   for (int e = tid; e < p.top; e += THREADS) {
     const int id = ids[e];
@@ -354,68 +352,53 @@ __global__ __launch_bounds__((64 * FewShape<T, DP>::kWaves)) void block_attentio
     }
     if (lane == 0) s_count = count;
   }
-  RowOf row[2];
+  RowOf row;
+  row.in = f.chunk * 16 + (lane & 15) < p.group;
+  row.head = row.in ? f.chunk * 16 + (lane & 15) : 0;
+  row.token = 0;
+  row.pos = row.in ? pos : -1;
   Online<T, DP> st;
   start(st);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = f.chunk * 32 + i * 16 + (lane & 15);
-    row[i].in = r < p.group;
-    row[i].head = row[i].in ? r : 0;
-    row[i].token = 0;
-    row[i].pos = row[i].in ? pos : -1;
-    if (i == 0 || TWO)
-      load_row<T, DP>(static_cast<const T*>(p.q) + f.token * p.q_token +
-                          (int64_t)(f.head * p.group + row[i].head) * p.q_head,
-                      row[i].in, p.width, lane, st.q[i]);
-  }
+  load_row<T, DP>(static_cast<const T*>(p.q) + f.token * p.q_token + (int64_t)(f.head * p.group + row.head) * p.q_head,
+                  row.in, p.width, lane, st.q);
   __syncthreads();
-  const int count = s_count, steps = ((count << p.lg_groups) + G - 1) / G;
+  constexpr int kHalf = R::kKeys / 2;
+  const int lg_halves = lg - (kHalf == 32 ? 5 : 4);
+  const int count = alike(s_count), steps = ((count << lg_halves) + 1) / 2;
   const float c = p.scale * kLog2e;
   const uint32_t kb = lds_address(s_kv[w][0]), vb = lds_address(s_kv[w][1]);
+  KeySource<T, DP, 1> src;
+  src.init(p, sq, seq, f.head, 0, lane);
   for (int s = f.split * WAVES + w; s < steps; s += WAVES * p.splits) {
-    int first[G];
+    Halves now;
+    uint32_t sel = 0;
+    bool edge = false;
 #pragma unroll
-    for (int gr = 0; gr < G; ++gr) {
-      const int q = s * G + gr, e = q >> p.lg_groups;
-      const int id = __builtin_amdgcn_readfirstlane(e < count ? s_ids[e] : -1);
-      first[gr] = id >= 0 ? id * block + (q & ((1 << p.lg_groups) - 1)) * 16 : -1;
+    for (int h = 0; h < 2; ++h) {
+      const int at = 2 * s + h, e = at >> lg_halves;
+      const int id = alike(e < count ? s_ids[e] : -1);
+      now.first[h] = id >= 0 ? (id << lg) + (at & ((1 << lg_halves) - 1)) * kHalf : -1;
+      sel |= now.first[h] >= 0 && row.in ? 1u << h : 0u;
+      edge |= now.first[h] + kHalf - 1 > pos;
     }
-    auto entry = [&](int gr) {
-      int x = first[0];
-#pragma unroll
-      for (int i = 1; i < G; ++i) x = gr == i ? first[i] : x;
-      return x;
-    };
+    auto first = [&](int gr) { return now.of<T, DP>(gr); };
     wait_reads();  // the step before has read its rows
-    load_rows<T, DP, 1>(p, p.k, sq, seq, f.head, kb, 0, lane, entry);
-    load_rows<T, DP, 1>(p, p.v, sq, seq, f.head, vb, 0, lane, entry);
-    const uint32_t missing = missing_pages<T, DP>(p, sq, seq, entry);
-    bool sel[2][G];
-    bool edge = missing != 0;
-#pragma unroll
-    for (int gr = 0; gr < G; ++gr) {
-      sel[0][gr] = row[0].in && first[gr] >= 0;
-      sel[1][gr] = row[1].in && first[gr] >= 0;
-      edge |= first[gr] + 15 > pos;
-    }
+    src.load(kb, vb, 0, first);
+    const uint32_t missing = src.missing(first);
     wait_loads<0>();
-    attend<T, DP, true, TWO>(st, kb, vb, sel, first, edge, missing, row, c, lane);
+    attend<T, DP>(st, kb, vb, sel, now, true, edge || missing != 0, missing, row, c, lane);
   }
   wait_reads();
   float* mine = reinterpret_cast<float*>(s_kv[w][0]);
-#pragma unroll
-  for (int i = 0; i < (TWO ? 2 : 1); ++i) {
-    const int r = i * 16 + (lane & 15);
-    const float l = across_sum(st.l[i]);
-    if (lane < 16) {
-      mine[r] = st.m[i];
-      mine[32 + r] = l;
-    }
-#pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt)
-      *reinterpret_cast<f32x4*>(&mine[64 + r * DP + dt * 16 + (lane >> 4) * 4]) = st.o[i][dt];
+  const int r16 = lane & 15;
+  const float sum = across_sum(st.l);
+  if (lane < 16) {
+    mine[r16] = st.m;
+    mine[16 + r16] = sum;
   }
+#pragma unroll
+  for (int dt = 0; dt < DP / 16; ++dt)
+    *reinterpret_cast<f32x4*>(&mine[32 + r16 * DP + dt * 16 + (lane >> 4) * 4]) = st.o[dt];
   __syncthreads();
   if (p.splits == 1) {
     join_rows<T, DP, THREADS>(p, f, seq, sq, pos, WAVES, tid, s_bad,
@@ -424,8 +407,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP>::kWaves)) void block_attentio
   }
   // joined over the waves, into the split's part
   float* part = p.parts + row_block() * part_floats<DP>();
-  const int rows = TWO ? 32 : 16;
-  for (int e = tid; e < rows * (DP / 4); e += THREADS) {
+  for (int e = tid; e < 16 * (DP / 4); e += THREADS) {
     const int r = e / (DP / 4), d = e % (DP / 4) * 4;
     float m = -INFINITY, l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -436,20 +418,20 @@ __global__ __launch_bounds__((64 * FewShape<T, DP>::kWaves)) void block_attentio
     for (int i = 0; i < WAVES; ++i) {
       const float* x = reinterpret_cast<const float*>(s_kv[i][0]);
       const float by = __builtin_amdgcn_exp2f(x[r] - base);
-      l = __builtin_fmaf(by, x[32 + r], l);
-      o += by * *reinterpret_cast<const f32x4*>(&x[64 + r * DP + d]);
+      l = __builtin_fmaf(by, x[16 + r], l);
+      o += by * *reinterpret_cast<const f32x4*>(&x[32 + r * DP + d]);
     }
     if (d == 0) {
       part[r] = m;
-      part[32 + r] = l;
+      part[16 + r] = l;
     }
-    *reinterpret_cast<f32x4*>(&part[64 + r * DP + d]) = o;
+    *reinterpret_cast<f32x4*>(&part[32 + r * DP + d]) = o;
   }
 }
 
 template <class T, int DP>
 __global__ __launch_bounds__(128) void block_attention_join_kernel(const BlockArgs p) {
-  __shared__ int s_bad[32];
+  __shared__ int s_bad[16];
   const int64_t at = row_block();
   const FewPlace f = few_place(p, at * p.splits);
   if (f.token >= p.seqs.n_tokens) return;
@@ -461,6 +443,8 @@ __global__ __launch_bounds__(128) void block_attention_join_kernel(const BlockAr
   });
 }
 
+constexpr int kWaves = 8;  // of the many rows' kernel
+
 // A few rows' kernel up to this many (token, key-value head) pairs.
 constexpr int64_t kFewPairs = 4096;
 
@@ -470,10 +454,12 @@ struct Plan {
   int64_t groups;  // (token, head, chunk) triples of the few rows' kernel
   size_t bytes;
 };
-Plan plan_of(int val_t, int64_t tokens, int heads, int group, int width, int block, int top) {
+Plan plan_of(int val_t, const fs_block_seqs& s, int heads, int group, int width, int top) {
   Plan o{};
+  const int64_t tokens = s.n_tokens;
+  const int block = s.block;
   o.few = tokens * heads <= kFewPairs;
-  o.groups = tokens * heads * ((group + 31) / 32);
+  o.groups = tokens * heads * ((group + 15) / 16);
   o.splits = 1;
   if (o.few) {
     const int bytes = (width <= 64 ? 64 : width <= 128 ? 128 : 256) * (val_t == FS_F32 ? 4 : 2);
@@ -482,7 +468,9 @@ Plan plan_of(int val_t, int64_t tokens, int heads, int group, int width, int blo
     // until a wave has one step, or there are two workgroups a compute unit
     while ((int64_t)o.splits * waves < steps && o.groups * o.splits < 512 && o.splits < 64) o.splits *= 2;
     if (o.splits > 1)
-      o.bytes = (size_t)(o.groups * o.splits) * (64 + 32 * (width <= 64 ? 64 : width <= 128 ? 128 : 256)) * 4;
+      o.bytes = (size_t)(o.groups * o.splits) * (32 + 16 * (width <= 64 ? 64 : width <= 128 ? 128 : 256)) * 4;
+  } else {
+    o.bytes = (size_t)(block_tiles(s, tokens_of<kWaves>(group)) * heads) * kWaves * 4;
   }
   return o;
 }
@@ -494,7 +482,7 @@ extern "C" size_t fs_block_attention_workspace_bytes(int val_t, const fs_block_s
                                                      int width, int top) {
   using namespace fs;
   if (block_sizes_fault("", val_t, seqs, heads, group, width) != FS_OK || top < 1 || top > kMostTop) return 0;
-  return plan_of(val_t, seqs->n_tokens, heads, group, width, seqs->block, top).bytes;
+  return plan_of(val_t, *seqs, heads, group, width, top).bytes;
 }
 
 extern "C" int fs_block_attention(int val_t, const fs_block_seqs* seqs, int heads, int group, int width, int top,
@@ -513,7 +501,7 @@ extern "C" int fs_block_attention(int val_t, const fs_block_seqs* seqs, int head
   if (!block_rows_fit(k, k_page, k_row, k_head, size) || !block_rows_fit(v, v_page, v_row, v_head, size))
     return fail(FS_E_INVALID, std::string(who) + ": keys and values need rows at multiples of 16 bytes");
   if (!(scale > 0.0) || !(scale < 1e30)) return fail(FS_E_INVALID, std::string(who) + ": scale must be positive");
-  const Plan plan = plan_of(val_t, seqs->n_tokens, heads, group, width, seqs->block, top);
+  const Plan plan = plan_of(val_t, *seqs, heads, group, width, top);
   if (plan.bytes > 0 && (ws == nullptr || ws_bytes < plan.bytes))
     return fail(FS_E_WORKSPACE, std::string(who) + ": workspace too small");
   BlockArgs p{};
@@ -536,13 +524,13 @@ extern "C" int fs_block_attention(int val_t, const fs_block_seqs* seqs, int head
   p.scale = (float)scale;
   p.splits = plan.splits;
   p.parts = static_cast<float*>(ws);
+  p.again = static_cast<uint32_t*>(ws);
   return with_block_width(val_t, width, who, [&](auto val, auto dp) -> int {
     using T = decltype(val);
     constexpr int DP = decltype(dp)::value;
     if (plan.few) {
       const dim3 grid = row_grid(plan.groups * plan.splits), threads(64 * FewShape<T, DP>::kWaves);
-      if (group > 16) hipLaunchKernelGGL((block_attention_few_kernel<T, DP, true>), grid, threads, 0, stream, p);
-      else hipLaunchKernelGGL((block_attention_few_kernel<T, DP, false>), grid, threads, 0, stream, p);
+      hipLaunchKernelGGL((block_attention_few_kernel<T, DP>), grid, threads, 0, stream, p);
       FS_CHECK_MAIN_LAUNCH("block_attention_few_kernel");
       if (plan.splits > 1) {
         hipLaunchKernelGGL((block_attention_join_kernel<T, DP>), row_grid(plan.groups), dim3(128), 0, stream, p);
@@ -550,12 +538,13 @@ extern "C" int fs_block_attention(int val_t, const fs_block_seqs* seqs, int head
       }
       return FS_OK;
     }
-    constexpr int WAVES = 4;
-    p.tiles = block_tiles(*seqs, tokens_of<WAVES>(group));
+    p.tiles = block_tiles(*seqs, tokens_of<kWaves>(group));
     if (p.tiles * heads > kMostWorkgroups) return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
-    hipLaunchKernelGGL((block_attention_kernel<T, DP, WAVES>), dim3((uint32_t)(p.tiles * heads)), dim3(64 * WAVES), 0,
-                       stream, p);
+    const dim3 grid((uint32_t)(p.tiles * heads)), threads(64 * kWaves);
+    hipLaunchKernelGGL((block_attention_kernel<T, DP, kWaves>), grid, threads, 0, stream, p);
     FS_CHECK_MAIN_LAUNCH("block_attention_kernel");
+    hipLaunchKernelGGL((block_attention_again_kernel<T, DP, kWaves>), grid, threads, 0, stream, p);
+    FS_CHECK_LAUNCH("block_attention_again_kernel");
     return FS_OK;
   });
 }

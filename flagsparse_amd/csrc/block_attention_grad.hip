@@ -16,7 +16,7 @@
 namespace fs {
 namespace {
 
-constexpr int kAmaxParts = 256;
+constexpr int kAmaxParts = 256, kQueryWaves = 8;
 
 // dS of 16-bit floats, whose small values have few bits: G and <G, O> are multiplied
 // by the power of two that brings G's largest value to [1, 2), and the gradients
@@ -64,59 +64,57 @@ __global__ __launch_bounds__(256) void block_amax_kernel(const T* x, int64_t n, 
 
 template <class T, int DP>
 struct QueryGrad {
-  typename Mma<T>::frag q[2][Rows<T, DP>::kFrags], g[2][Rows<T, DP>::kFrags];
-  f32x4 d[2][DP / 16];
-  float lse[2], delta[2];  // in powers of two; times the factor
+  typename Mma<T>::frag q[Rows<T, DP>::kFrags], g[Rows<T, DP>::kFrags];
+  f32x4 d[DP / 16];
+  float lse, delta;  // in powers of two; times the factor
 };
 
-template <class T, int DP, bool A, bool B>
-__device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, const bool (&sel)[2][Rows<T, DP>::kGroups],
-                            const int (&first)[Rows<T, DP>::kGroups], bool edge, uint32_t missing,
-                            const RowOf (&row)[2], float c, float factor, int lane) {
+template <class T, int DP>
+__device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, uint32_t sel, const Halves& now, bool some,
+                            bool edge, const RowOf& row, float c, float factor, int lane) {
   using R = Rows<T, DP>;
   constexpr int G = R::kGroups, P = R::kUnit / 16;
-  f32x4 s[2][G], dp[2][G];
+  f32x4 s[G], dp[G];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int gr = 0; gr < G; ++gr) s[i][gr] = dp[i][gr] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int gr = 0; gr < G; ++gr) s[gr] = dp[gr] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int ks = 0; ks < R::kFrags; ++ks)
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) {
-      const auto k = R::across(kb, gr * 16, ks, lane);
-      if (A) s[0][gr] = Mma<T>::run(k, st.q[0][ks], s[0][gr]);
-      if (B) s[1][gr] = Mma<T>::run(k, st.q[1][ks], s[1][gr]);
-      const auto v = R::across(vb, gr * 16, ks, lane);
-      if (A) dp[0][gr] = Mma<T>::run(v, st.g[0][ks], dp[0][gr]);
-      if (B) dp[1][gr] = Mma<T>::run(v, st.g[1][ks], dp[1][gr]);
+      s[gr] = Mma<T>::run(R::across(kb, gr * 16, ks, lane), st.q[ks], s[gr]);
+      dp[gr] = Mma<T>::run(R::across(vb, gr * 16, ks, lane), st.g[ks], dp[gr]);
     }
-  typename R::frag w[2][G / P];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (i == 0 ? !A : !B) continue;
+  for (int gr = 0; gr < G; ++gr)
 #pragma unroll
-    for (int gr = 0; gr < G; ++gr)
+    for (int r = 0; r < 4; ++r) {
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[gr][r], c, -st.lse));
+      s[gr][r] = x * __builtin_fmaf(dp[gr][r], factor, -st.delta);
+    }
+  if (edge) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        bool in = sel[i][gr];
-        if (edge) in = in && first[gr] + 4 * (lane >> 4) + r <= row[i].pos && !((missing >> gr) & 1u);
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][gr][r], c, -st.lse[i]));
-        const float y = x * __builtin_fmaf(dp[i][gr][r], factor, -st.delta[i]);
-        s[i][gr][r] = in ? y : 0.0f;
-      }
-    // (dS in the values' type, rounded once)
+    for (int gr = 0; gr < G; ++gr) {
+      const int last = row.pos - now.of<T, DP>(gr) - 4 * (lane >> 4);
 #pragma unroll
-    for (int u = 0; u < G / P; ++u) w[i][u] = R::rounded(&s[i][u * P]);
+      for (int r = 0; r < 4; ++r) s[gr][r] = r <= last ? s[gr][r] : 0.0f;
+    }
   }
+  if (some) {
 #pragma unroll
-  for (int u = 0; u < G / P; ++u)
+    for (int gr = 0; gr < G; ++gr) {
+      const bool in = (sel >> (gr / (G / 2))) & 1u;
 #pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt) {
-      const auto k = R::down(kb, u * R::kUnit, dt, lane);
-      if (A) st.d[0][dt] = Mma<T>::run(k, w[0][u], st.d[0][dt]);
-      if (B) st.d[1][dt] = Mma<T>::run(k, w[1][u], st.d[1][dt]);
+      for (int r = 0; r < 4; ++r) s[gr][r] = in ? s[gr][r] : 0.0f;
     }
+  }
+  // (dS in the values' type, rounded once)
+#pragma unroll
+  for (int u = 0; u < G / P; ++u) {
+    const auto w = R::rounded(&s[u * P]);
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt)
+      st.d[dt] = Mma<T>::run(R::down(kb, u * R::kUnit, dt, lane), w, st.d[dt]);
+  }
 }
 
 struct GradArgs {
@@ -140,7 +138,7 @@ struct GradArgs {
 
 // A row without what is left out, see careful_row.
 template <class T, int DP>
-__device__ __noinline__ void careful_query(const GradArgs& a, const Sequence& sq, int seq, int64_t token, int head,
+__device__ __forceinline__ void careful_query(const GradArgs& a, const Sequence& sq, int seq, int64_t token, int head,
                                            int in_group, int pos, float lse, float delta, int lane) {
   const BlockArgs& p = a.b;
   const int hq = head * p.group + in_group, block = p.seqs.block, lg = p.lg_groups + 4;
@@ -196,58 +194,57 @@ __global__ __launch_bounds__(64 * WAVES) void block_query_grad_kernel(const Grad
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   WalkTile t;
   if (!walk_tile<WAVES>(p, lane, t)) return;
-  RowOf row[2];
-  rows_of<WAVES>(p, t, w, lane, row);
+  const RowOf row = row_of(p, t, w, lane);
   const float factor = read_factor<T>(a.amax, lane);
   QueryGrad<T, DP> st;
-  float delta[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int hq = t.head * p.group + row[i].head;
-    const int64_t at = (int64_t)(t.token0 + row[i].token) * p.heads * p.group + hq;
-    load_row<T, DP>(static_cast<const T*>(p.q) + (int64_t)(t.token0 + row[i].token) * p.q_token + (int64_t)hq * p.q_head,
-                    row[i].in, p.width, lane, st.q[i]);
-    load_row<T, DP>(static_cast<const T*>(a.grad) + at * p.width, row[i].in, p.width, lane, st.g[i]);
+  const int hq = t.head * p.group + row.head;
+  const int64_t at = (int64_t)(t.token0 + row.token) * p.heads * p.group + hq;
+  load_row<T, DP>(static_cast<const T*>(p.q) + (int64_t)(t.token0 + row.token) * p.q_token + (int64_t)hq * p.q_head,
+                  row.in, p.width, lane, st.q);
+  load_row<T, DP>(static_cast<const T*>(a.grad) + at * p.width, row.in, p.width, lane, st.g);
+  {
     typename R::frag o[R::kFrags];
-    load_row<T, DP>(static_cast<const T*>(a.o) + at * p.width, row[i].in, p.width, lane, o);
+    load_row<T, DP>(static_cast<const T*>(a.o) + at * p.width, row.in, p.width, lane, o);
     float sum = 0.0f;
 #pragma unroll
     for (int ks = 0; ks < R::kFrags; ++ks)
 #pragma unroll
-      for (int e = 0; e < 16 / (int)sizeof(T); ++e) sum = __builtin_fmaf((float)st.g[i][ks][e], (float)o[ks][e], sum);
-    delta[i] = across_sum(sum);
-    st.delta[i] = delta[i] * factor;
-    st.lse[i] = row[i].in ? a.lse[at] * kLog2e : 0.0f;
-    if (row[i].in && lane < 16) a.delta[at] = delta[i];
-#pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt) st.d[i][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int e = 0; e < 16 / (int)sizeof(T); ++e) sum = __builtin_fmaf((float)st.g[ks][e], (float)o[ks][e], sum);
+    sum = across_sum(sum);
+    if (row.in && lane < 16) a.delta[at] = sum;
+    st.delta = sum * factor;
+    st.lse = row.in ? a.lse[at] * kLog2e : 0.0f;
   }
+#pragma unroll
+  for (int dt = 0; dt < DP / 16; ++dt) st.d[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   const float c = p.scale * kLog2e;
-  walk_blocks<T, DP, WAVES>(
-      p, t, row, s_walk, s_kv, tid, w, lane,
-      [&](const Step<T, DP>& now, const bool(&sel)[2][R::kGroups], bool x, bool y, bool edge, uint32_t kb, uint32_t vb) {
-        if (x && y) take<T, DP, true, true>(st, kb, vb, sel, now.first, edge, now.missing, row, c, factor, lane);
-        else if (x) take<T, DP, true, false>(st, kb, vb, sel, now.first, edge, now.missing, row, c, factor, lane);
-        else take<T, DP, false, true>(st, kb, vb, sel, now.first, edge, now.missing, row, c, factor, lane);
-      });
+  walk_blocks<T, DP, WAVES>(p, t, row, s_walk, s_kv, tid, w, lane,
+                            [&](const Halves& now, uint32_t sel, bool some, bool edge, uint32_t, uint32_t kb,
+                                uint32_t vb) { take<T, DP>(st, kb, vb, sel, now, some, edge, row, c, factor, lane); });
+  bool bad = false;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    bool bad = false;
+  for (int dt = 0; dt < DP / 16; ++dt)
 #pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) bad |= !__builtin_isfinite(st.d[i][dt][r]);
-    uint64_t rows = __ballot(bad && row[i].in);
-    rows = (rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xffffu;
-    const int64_t at = (int64_t)(t.token0 + row[i].token) * p.heads * p.group + t.head * p.group + row[i].head;
-    if (row[i].in && !((rows >> (lane & 15)) & 1))
-      store_row<T, DP>(static_cast<T*>(p.out) + at * p.width, st.d[i], p.scale / factor, p.width, lane);
-    for (; rows != 0; rows &= rows - 1) {
-      const int r = __builtin_ctzll(rows), tok = __builtin_amdgcn_readlane(row[i].token, r);
-      auto of = [&](float x) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), r)); };
-      careful_query<T, DP>(a, t.sq, t.seq, t.token0 + tok, t.head, __builtin_amdgcn_readlane(row[i].head, r),
-                           t.pos0 + tok, of(st.lse[i]), of(delta[i]), lane);
-    }
+    for (int r = 0; r < 4; ++r) bad |= !__builtin_isfinite(st.d[dt][r]);
+  const uint64_t rows = __ballot(bad && row.in);
+  if (row.in) store_row<T, DP>(static_cast<T*>(p.out) + at * p.width, st.d, p.scale / factor, p.width, lane);
+  if (lane == 0)
+    p.again[(int64_t)blockIdx.x * WAVES + w] = (uint32_t)(rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xffffu;
+}
+
+// Rows whose gradient is not finite, key after key.
+template <class T, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void block_query_grad_again_kernel(const GradArgs a) {
+  const BlockArgs& p = a.b;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  WalkTile t;
+  if (!walk_tile<WAVES>(p, lane, t)) return;
+  uint32_t rows = alike((int)p.again[(int64_t)blockIdx.x * WAVES + w]);
+  for (; rows != 0; rows &= rows - 1) {
+    const int r = w * 16 + __builtin_ctz(rows), tok = r / p.group, in_group = r - tok * p.group;
+    const int64_t at = (int64_t)(t.token0 + tok) * p.heads * p.group + t.head * p.group + in_group;
+    careful_query<T, DP>(a, t.sq, t.seq, t.token0 + tok, t.head, in_group, t.pos0 + tok, a.lse[at] * kLog2e, a.delta[at],
+                         lane);
   }
 }
 
@@ -392,7 +389,7 @@ struct RowStats {
 };
 
 template <class T, int DP>
-__device__ __noinline__ void careful_key(const GradArgs& a, const KeyPlace& at, const int32_t* tokens, int rows, int j,
+__device__ __forceinline__ void careful_key(const GradArgs& a, const KeyPlace& at, const int32_t* tokens, int rows, int j,
                                          float (&k_sum)[(DP + 63) / 64], float (&v_sum)[(DP + 63) / 64], int lane) {
   const BlockArgs& p = a.b;
   const float c = p.scale * kLog2e;
@@ -482,7 +479,7 @@ __global__ __launch_bounds__(256) void block_key_grad_kernel(const GradArgs a) {
     }
   }
   if (o.seq < 0) return;  // a number that no sequence's block has
-  o.sq = sequence_at(p.seqs, o.seq);
+  o.sq = sequence_of(p.seqs, o.seq);
   o.first = ((number - first_block(p.seqs, o.seq, lg_block)) << lg_block) + part * BK;
   const int entries = piece.z - piece.y, rows = entries * p.group;
   for (int e = tid; e < entries; e += 256) s_token[e] = a.order[piece.y + e] / (a.lists * p.top);
@@ -759,11 +756,12 @@ struct GradPlan {
   int64_t key_blocks, n_keys;
   int64_t pieces, places;  // at most
   int most;                // entries a piece
-  size_t sort, keys, sorted, order, starts, list, sums, count, delta, amax, parts, bytes;
+  size_t again, sort, keys, sorted, order, starts, list, sums, count, delta, amax, parts, bytes;
 };
-GradPlan grad_plan(int64_t tokens, int64_t rows, int64_t n_seqs, int block, int heads, int group, int lists, int width,
-                   int top) {
+GradPlan grad_plan(const fs_block_seqs& s, int heads, int group, int lists, int width, int top) {
   GradPlan l{};
+  const int64_t tokens = s.n_tokens, rows = s.n_rows, n_seqs = s.n_seqs;
+  const int block = s.block;
   l.entries = tokens * lists * top;
   l.key_blocks = rows / block + n_seqs + 1;
   l.n_keys = l.key_blocks * lists;
@@ -781,6 +779,7 @@ GradPlan grad_plan(int64_t tokens, int64_t rows, int64_t n_seqs, int block, int 
     at += up(n);
     return a;
   };
+  l.again = take((size_t)(block_tiles(s, tokens_of<kQueryWaves>(group)) * heads) * kQueryWaves * 4);
   l.sort = take(select_sort_bytes(l.entries, l.n_keys));
   l.keys = take((size_t)l.entries * 4);
   l.sorted = take((size_t)l.entries * 4);
@@ -816,7 +815,7 @@ extern "C" size_t fs_block_attention_grad_workspace_bytes(int val_t, const fs_bl
                                                           int width, int lists, int top) {
   using namespace fs;
   if (grad_fault("", val_t, seqs, heads, group, width, lists, top) != FS_OK) return 0;
-  return grad_plan(seqs->n_tokens, seqs->n_rows, seqs->n_seqs, seqs->block, heads, group, lists, width, top).bytes;
+  return grad_plan(*seqs, heads, group, lists, width, top).bytes;
 }
 
 extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int heads, int group, int width, int lists,
@@ -837,11 +836,12 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
       (((int64_t)(uintptr_t)q | (int64_t)(uintptr_t)grad | q_token * size | q_head * size) & 15) != 0)
     return fail(FS_E_INVALID, std::string(who) + ": queries, keys, values and grad need rows at multiples of 16 bytes");
   if (!(scale > 0.0) || !(scale < 1e30)) return fail(FS_E_INVALID, std::string(who) + ": scale must be positive");
-  const GradPlan l = grad_plan(tokens, seqs->n_rows, seqs->n_seqs, seqs->block, heads, group, lists, width, top);
+  const GradPlan l = grad_plan(*seqs, heads, group, lists, width, top);
   if (ws == nullptr || ws_bytes < l.bytes) return fail(FS_E_WORKSPACE, std::string(who) + ": workspace too small");
   uint8_t* m = static_cast<uint8_t*>(ws);
   GradArgs a{};
   BlockArgs& p = a.b;
+  p.again = reinterpret_cast<uint32_t*>(m + l.again);
   p.seqs = *seqs;
   p.k = RowLayout{k, 0, k_row, k_head};
   p.v = RowLayout{v, 0, v_row, v_head};
@@ -895,7 +895,7 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
   FS_CHECK_LAUNCH("block_pieces_kernel");
   return with_block_width(val_t, width, who, [&](auto val, auto dp) -> int {
     using T = decltype(val);
-    constexpr int DP = decltype(dp)::value, WAVES = 4;
+    constexpr int DP = decltype(dp)::value, WAVES = kQueryWaves;
     if (tokens > 0) {
       if constexpr (kFactored<T>) {
         hipLaunchKernelGGL((block_amax_kernel<T>), dim3(kAmaxParts), dim3(256), 0, stream, static_cast<const T*>(grad),
@@ -907,6 +907,9 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
       hipLaunchKernelGGL((block_query_grad_kernel<T, DP, WAVES>), dim3((uint32_t)(p.tiles * heads)), dim3(64 * WAVES), 0,
                          stream, a);
       FS_CHECK_MAIN_LAUNCH("block_query_grad_kernel");
+      hipLaunchKernelGGL((block_query_grad_again_kernel<T, DP, WAVES>), dim3((uint32_t)(p.tiles * heads)),
+                         dim3(64 * WAVES), 0, stream, a);
+      FS_CHECK_LAUNCH("block_query_grad_again_kernel");
     }
     const int64_t shared = heads / lists;
     auto keys_of = [&](auto bk) -> int {

@@ -31,6 +31,7 @@ struct Sequence {
   int keys;
   int64_t row0;  // of the keys, packed
 };
+__device__ inline int alike(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ inline Sequence sequence_at(const fs_block_seqs& s, int b) {
   Sequence o;
   o.keys = 0;
@@ -51,6 +52,16 @@ __device__ inline Sequence sequence_at(const fs_block_seqs& s, int b) {
       o.keys = clamp_to(s.k_offsets[b + 1], o.row0, s.n_rows) - (int)o.row0;
     }
   }
+  return o;
+}
+
+// The same of a b that all lanes have, in scalar registers.
+__device__ inline Sequence sequence_of(const fs_block_seqs& s, int b) {
+  Sequence o = sequence_at(s, alike(b));
+  o.first = alike(o.first);
+  o.count = alike(o.count);
+  o.keys = alike(o.keys);
+  o.row0 = alike((int)o.row0);
   return o;
 }
 
@@ -215,54 +226,110 @@ struct BlockArgs {
   int top, heads, group, width;
   int lg_groups;  // log2 of a block's groups of 16 keys
   float scale;
-  int64_t tiles;  // workgroups a head
+  int64_t tiles;    // workgroups a head
+  uint32_t* again;  // many rows: a word a wave, its rows whose result is not finite
   int splits;
   float* parts;
-  // gradients
-  const void* grad;
-  const void* o;
-  const float* lse_in;
-  float* delta;
-  const float* factor;
 };
 
-// The loads of one step's keys or values: rows of `lds`, zeros past the sequence's
-// keys, past the width and for pages outside the cache.  Wave w of WAVES takes its
-// share.  entry(group) gives the block of a group of 16 keys, negative for none.
-template <class T, int DP, int WAVES, class Entry>
-__device__ inline void load_rows(const BlockArgs& p, const RowLayout& l, const Sequence& sq, int seq, int head,
-                                 uint32_t lds, int w, int lane, Entry entry) {
+// Keys and values of one sequence and head, and a lane's part of the loads of a step:
+// wave w of WAVES takes kLoads instructions for the keys and as many for the values.
+template <class T, int DP, int WAVES>
+struct KeySource {
   using R = Rows<T, DP>;
-  constexpr int kLoads = R::kBytes / 1024 / WAVES;
+  static constexpr int kLoads = R::kBytes / 1024 / WAVES;
+  static constexpr int kOffsets = kLoads * R::kAtOnce < 16 ? kLoads : 16 / R::kAtOnce;
   static_assert(R::kBytes % (1024 * WAVES) == 0, "whole loads a wave");
-  const int r = R::lane_row(lane), pos = lane % R::kPieces;
-#pragma unroll
-  for (int n = 0; n < kLoads; ++n) {
-    const int row0 = (w * kLoads + n) * R::kAtOnce, gr = row0 / 16;
-    const int first = entry(gr);  // position of the group's first key
-    const int row = row0 % 16 + r;
-    const int piece = pos ^ R::swizzle(row);
-    const T* base = first >= 0 ? key_rows<T>(p.seqs, sq, seq, l, head, first) : nullptr;
-    const bool in = base != nullptr && first + row < sq.keys && piece * 16 < p.width * (int)sizeof(T);
-    const uint32_t off = in ? (uint32_t)(row * l.row * (int64_t)sizeof(T)) + (uint32_t)piece * 16 : 2u * kInBuffer;
-    lds_dma<16>((uint32_t)__builtin_amdgcn_readfirstlane((int)(lds + (uint32_t)row0 * R::kRow)), off,
-                buffer_at(base != nullptr ? base : l.base));
-  }
-}
+  const char *k, *v;
+  uint32_t k_row, v_row;      // bytes
+  uint32_t k_off[kOffsets], v_off[kOffsets];
+  const int32_t* table;       // the sequence's pages, or null
+  int64_t k_page, v_page, n_pages;
+  int per_seq, shift, keys;
+  int row;  // the lane's, of the first load
 
-// Which groups of 16 keys of a step lie in pages outside the cache, a bit each.
-template <class T, int DP, class Entry>
-__device__ inline uint32_t missing_pages(const BlockArgs& p, const Sequence& sq, int seq, Entry entry) {
-  uint32_t m = 0;
-  if (p.seqs.pages != nullptr) {
+  __device__ void init(const BlockArgs& p, const Sequence& sq, int seq, int head, int w, int lane) {
+    k = static_cast<const char*>(p.k.base) + (head * p.k.head + sq.row0 * p.k.row) * (int64_t)sizeof(T);
+    v = static_cast<const char*>(p.v.base) + (head * p.v.head + sq.row0 * p.v.row) * (int64_t)sizeof(T);
+    k_row = (uint32_t)(p.k.row * (int64_t)sizeof(T));
+    v_row = (uint32_t)(p.v.row * (int64_t)sizeof(T));
+    keys = sq.keys;
+    table = p.seqs.pages == nullptr ? nullptr : p.seqs.pages + (int64_t)seq * p.seqs.ld_pages;
+    k_page = p.k.page * (int64_t)sizeof(T);
+    v_page = p.v.page * (int64_t)sizeof(T);
+    n_pages = p.seqs.n_pages;
+    per_seq = (int)p.seqs.pages_per_seq;
+    shift = p.seqs.page_shift;
+    row = w * kLoads * R::kAtOnce % 16 + R::lane_row(lane);
 #pragma unroll
-    for (int gr = 0; gr < Rows<T, DP>::kGroups; ++gr) {
-      const int first = entry(gr);
-      if (first >= 0 && key_rows<T>(p.seqs, sq, seq, p.k, 0, first) == nullptr) m |= 1u << gr;
+    for (int n = 0; n < kOffsets; ++n) {
+      const int r = row + n * R::kAtOnce, piece = (lane % R::kPieces) ^ R::swizzle(r);
+      const bool in = piece * 16 < p.width * (int)sizeof(T);
+      k_off[n] = in ? (uint32_t)r * k_row + (uint32_t)piece * 16 : 2u * kInBuffer;
+      v_off[n] = in ? (uint32_t)r * v_row + (uint32_t)piece * 16 : 2u * kInBuffer;
     }
   }
-  return m;
-}
+  // The page of the 16 keys from position j on; negative: outside the cache.
+  __device__ int64_t page_of(int j) const {
+    const int at = j >> shift;
+    const int64_t page = at < per_seq ? table[at] : -1;
+    return page < n_pages ? page : -1;
+  }
+  // One step's keys to LDS at kb, values at vb, zeros past the sequence's end, past the
+  // width and for pages outside the cache.  first(group): the position of a group's
+  // first key, negative for none.  (All lanes alike but for the rows.)
+  template <class First>
+  __device__ void load(uint32_t kb, uint32_t vb, int w, First first) const {
+    constexpr int kAGroup = 16 / R::kAtOnce;  // loads
+    const char *k0 = k, *v0 = v;
+    int j = -1;
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      const int row0 = (w * kLoads + n) * R::kAtOnce;
+      if (n % kAGroup == 0) {
+        j = first(row0 / 16);
+        k0 = k;
+        v0 = v;
+        if (j >= 0) {
+          int64_t jj = j;
+          if (table != nullptr) {
+            const int64_t page = page_of(j);
+            if (page < 0) {
+              j = -1;
+            } else {
+              k0 += page * k_page;
+              v0 += page * v_page;
+              jj = j & ((1 << shift) - 1);
+            }
+          }
+          if (j >= 0) {
+            k0 += jj * k_row;
+            v0 += jj * v_row;
+          }
+        }
+      }
+      // (rows of the group that are keys)
+      const int left = j >= 0 ? keys - j : 0;
+      const bool in = row + n % kAGroup * R::kAtOnce < left;
+      const uint32_t to = (uint32_t)row0 * R::kRow;
+      lds_dma<16>((uint32_t)alike((int)(kb + to)), in ? k_off[n % kOffsets] : 2u * kInBuffer, buffer_at(k0));
+      lds_dma<16>((uint32_t)alike((int)(vb + to)), in ? v_off[n % kOffsets] : 2u * kInBuffer, buffer_at(v0));
+    }
+  }
+  // Which groups of a step lie in pages outside the cache, a bit each.
+  template <class First>
+  __device__ uint32_t missing(First first) const {
+    uint32_t m = 0;
+    if (table != nullptr) {
+#pragma unroll
+      for (int gr = 0; gr < R::kGroups; ++gr) {
+        const int j = first(gr);
+        if (j >= 0 && page_of(j) < 0) m |= 1u << gr;
+      }
+    }
+    return m;
+  }
+};
 
 // 16 query rows of a wave: lanes with the same lane % 16 hold one row's state.
 struct RowOf {
@@ -270,6 +337,18 @@ struct RowOf {
   int head;   // within the group
   int pos;    // its position; -1 and less: before the first key
   bool in;
+};
+
+// A step's two halves: the position of each one's first key (negative: none).
+struct Halves {
+  int first[2];
+  template <class T, int DP>
+  __device__ int of(int group) const {
+    constexpr int kHalf = Rows<T, DP>::kGroups / 2;
+    const bool second = group >= kHalf;
+    const int f = second ? first[1] : first[0];
+    return f < 0 ? -1 : f + (group - (second ? kHalf : 0)) * 16;
+  }
 };
 
 // Fragments of a lane's row of a dense or strided array, zeros outside.

@@ -3,7 +3,7 @@
 // (block_attention.hip, block_attention_grad.hip).
 //
 // A workgroup takes consecutive tokens of a sequence, all heads of one group, 16
-// rows a tile and two tiles a wave.  Tokens near each other select many of the same
+// rows a wave.  Tokens near each other select many of the same
 // blocks: a table in LDS holds, for each block of a window of the sequence, a bit
 // for each token that selects it.  The blocks with a bit are walked in order, keys
 // and values loaded once for the workgroup, and a wave takes part with the tiles
@@ -34,7 +34,7 @@ struct WalkTile {
 };
 
 template <int WAVES>
-__host__ __device__ inline int tokens_of(int group) { return WAVES * 32 / group; }
+__host__ __device__ inline int tokens_of(int group) { return WAVES * 16 / group; }
 
 // Head by head over the XCDs (each has its keys and values in a cache of its own), a
 // head's last tiles first: they have the most blocks to choose from.
@@ -45,7 +45,7 @@ __device__ inline bool walk_tile(const BlockArgs& p, int lane, WalkTile& t) {
   t.per = tokens_of<WAVES>(p.group);
   int tile;
   if (!find_tile(p.seqs, t.per, p.tiles - 1 - at % p.tiles, lane, t.seq, tile)) return false;
-  t.sq = sequence_at(p.seqs, t.seq);
+  t.sq = sequence_of(p.seqs, t.seq);
   const int first = tile * t.per;
   t.token0 = t.sq.first + first;
   t.tokens = t.sq.count - first < t.per ? t.sq.count - first : t.per;
@@ -53,41 +53,35 @@ __device__ inline bool walk_tile(const BlockArgs& p, int lane, WalkTile& t) {
   return true;
 }
 
-// The rows of a wave's two tiles.
-template <int WAVES>
-__device__ inline void rows_of(const BlockArgs& p, const WalkTile& t, int w, int lane, RowOf (&row)[2]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = w * 32 + i * 16 + (lane & 15);
-    row[i].token = r / p.group;
-    row[i].head = r % p.group;
-    row[i].in = row[i].token < t.tokens;
-    if (!row[i].in) row[i].token = 0;
-    row[i].pos = row[i].in ? t.pos0 + row[i].token : -1;
-  }
+// A lane's row.
+__device__ inline RowOf row_of(const BlockArgs& p, const WalkTile& t, int w, int lane) {
+  RowOf o;
+  const int r = w * 16 + (lane & 15);
+  o.token = r / p.group;
+  o.head = r - o.token * p.group;
+  o.in = o.token < t.tokens;
+  if (!o.in) o.token = 0;
+  o.pos = o.in ? t.pos0 + o.token : -1;
+  return o;
 }
 
-// One step's groups of 16 keys: the position of each one's first key (negative:
-// none), and its block's place in the window.
-template <class T, int DP>
-struct Step {
-  static constexpr int kGroups = Rows<T, DP>::kGroups;
-  int first[kGroups], slot[kGroups];
-  uint32_t missing;
-};
-
+// A lane's selection in a step has a bit for each half.
 template <class T, int DP, int WAVES, class Body>
-__device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const RowOf (&row)[2],
+__device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const RowOf& row,
                                    WalkMemory<WAVES>& mem, uint8_t (&kv)[2][2][Rows<T, DP>::kBytes], int tid, int w,
                                    int lane, Body body) {
   using R = Rows<T, DP>;
-  constexpr int THREADS = 64 * WAVES, G = R::kGroups;
-  const int block = p.seqs.block, lg_block = p.lg_groups + 4;
+  constexpr int THREADS = 64 * WAVES, kHalf = R::kKeys / 2;
+  const int lg_block = p.lg_groups + 4;
+  const int lg_halves = lg_block - (kHalf == 32 ? 5 : 4);  // of a block's halves of a step
   const int words = (t.per + 31) / 32, window = kMaskWords / words;
   const int last = t.pos0 + t.tokens - 1;
   const int n_blocks = last < 0 ? 0 : (last >> lg_block) + 1;
   const int entries = t.tokens * p.top;
   const int32_t* ids = p.blocks + (int64_t)t.token0 * p.b_token + (int64_t)t.head * p.b_head;
+  KeySource<T, DP, WAVES> src;
+  src.init(p, t.sq, t.seq, t.head, w, lane);
+  const uint32_t kv0 = lds_address(kv);
 
   for (int w0 = 0; w0 < n_blocks; w0 += window) {
     __syncthreads();
@@ -104,14 +98,14 @@ __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const 
     __syncthreads();
     // the blocks with a bit, in order
     const int each = (here + THREADS - 1) / THREADS;
-    uint32_t mine = 0;
-    for (int i = 0; i < each; ++i) {
-      const int b = tid * each + i;
+    auto named = [&](int b) {
       uint32_t any = 0;
       if (b < here)
         for (int k = 0; k < words; ++k) any |= mem.mask[b * words + k];
-      mine += any != 0;
-    }
+      return any != 0;
+    };
+    uint32_t mine = 0;
+    for (int i = 0; i < each; ++i) mine += named(tid * each + i);
     const uint32_t upto = wave_sum_scan(mine);
     if (lane == 63) mem.total[w] = upto;
     __syncthreads();
@@ -122,66 +116,51 @@ __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const 
       if (i < w) at += mem.total[i];
       count += (int)mem.total[i];
     }
-    for (int i = 0; i < each; ++i) {
-      const int b = tid * each + i;
-      uint32_t any = 0;
-      if (b < here)
-        for (int k = 0; k < words; ++k) any |= mem.mask[b * words + k];
-      if (any != 0) mem.list[at++] = (uint16_t)b;
-    }
+    count = alike(count);
+    for (int i = 0; i < each; ++i)
+      if (named(tid * each + i)) mem.list[at++] = (uint16_t)(tid * each + i);
     __syncthreads();
 
-    const int steps = ((count << p.lg_groups) + G - 1) / G;
-    Step<T, DP> next;
+    const int steps = ((count << lg_halves) + 1) / 2;
+    Halves next;
+    int next_slot[2];
+    uint32_t next_missing;
     auto prepare = [&](int s) {
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) {
-        const int q = s * G + gr, e = q >> p.lg_groups;
-        const bool in = e < count;
-        const int slot = __builtin_amdgcn_readfirstlane(in ? (int)mem.list[e] : 0);
-        next.slot[gr] = slot;
-        next.first[gr] = in ? (w0 + slot) * block + (q & ((1 << p.lg_groups) - 1)) * 16 : -1;
+      for (int h = 0; h < 2; ++h) {
+        const int q = 2 * s + h, e = q >> lg_halves;
+        const int slot = alike((int)mem.list[e < count ? e : 0]);
+        next_slot[h] = slot;
+        next.first[h] = e < count ? ((w0 + slot) << lg_block) + (q & ((1 << lg_halves) - 1)) * kHalf : -1;
       }
-      auto entry = [&](int gr) {
-        int f = next.first[0];
-#pragma unroll
-        for (int i = 1; i < G; ++i) f = gr == i ? next.first[i] : f;
-        return f;
-      };
-      next.missing = missing_pages<T, DP>(p, t.sq, t.seq, entry);
-      load_rows<T, DP, WAVES>(p, p.k, t.sq, t.seq, t.head, lds_address(kv[s & 1][0]), w, lane, entry);
-      load_rows<T, DP, WAVES>(p, p.v, t.sq, t.seq, t.head, lds_address(kv[s & 1][1]), w, lane, entry);
+      auto first = [&](int gr) { return next.of<T, DP>(gr); };
+      next_missing = src.missing(first);
+      const uint32_t to = kv0 + (uint32_t)((s & 1) * 2 * R::kBytes);
+      src.load(to, to + R::kBytes, w, first);
     };
     prepare(0);
     for (int s = 0; s < steps; ++s) {
-      const Step<T, DP> now = next;
+      const Halves now = next;
+      const int slot[2] = {next_slot[0], next_slot[1]};
+      const uint32_t missing = next_missing;
       wait_loads<0>();
       wait_reads();
       barrier();  // the step's rows are there, and nobody reads the other slot any more
       if (s + 1 < steps) prepare(s + 1);
-      bool sel[2][G];
-      bool any[2] = {false, false};
+      uint32_t sel = 0;
+      bool edge = missing != 0;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-          if (gr > 0 && p.lg_groups >= (G == 4 ? 2 : 1)) {
-            sel[i][gr] = sel[i][0];
-            continue;
-          }
-          const uint32_t bits = mem.mask[now.slot[gr] * words + (row[i].token >> 5)];
-          sel[i][gr] = now.first[gr] >= 0 && row[i].in && ((bits >> (row[i].token & 31)) & 1u);
-          any[i] |= sel[i][gr];
-        }
-      const bool a = __ballot(any[0]) != 0, b = __ballot(any[1]) != 0;
-      if (!a && !b) continue;
-      // keys behind a row's own position, or in no page of the cache
-      bool edge = now.missing != 0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) edge |= sel[i][gr] && now.first[gr] + 15 > row[i].pos;
-      body(now, sel, a, b, __ballot(edge) != 0, lds_address(kv[s & 1][0]), lds_address(kv[s & 1][1]));
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t bits = mem.mask[slot[h] * words + (row.token >> 5)];
+        const bool in = (now.first[h] >= 0) & row.in & (((bits >> (row.token & 31)) & 1u) != 0u);
+        sel |= in ? 1u << h : 0u;
+        // keys behind a row's own position
+        edge |= in & (now.first[h] + kHalf - 1 > row.pos);
+      }
+      if (__ballot(sel != 0u) == 0) continue;
+      const bool some = __ballot(sel != 3u) != 0;  // not all
+      const uint32_t kb = kv0 + (uint32_t)((s & 1) * 2 * R::kBytes);
+      body(now, sel, some, __ballot(edge) != 0, missing, kb, kb + R::kBytes);
     }
     wait_loads<0>();
   }
