@@ -31,18 +31,18 @@ __device__ inline void start(Online<T, DP>& st) {
 constexpr float kSlack = 8.0f;
 
 // One step's keys and values.
-template <class T, int DP>
+template <class T, int DP, int AHEAD, class Wait>
 __device__ inline void attend(Online<T, DP>& st, uint32_t kb, uint32_t vb, uint32_t sel, const Halves& now, bool some,
-                              bool edge, uint32_t missing, const RowOf& row, float c, int lane) {
+                              bool edge, uint32_t missing, const RowOf& row, float c, int lane, Wait values) {
   using R = Rows<T, DP>;
   constexpr int G = R::kGroups, P = R::kUnit / 16;
   f32x4 s[G];
 #pragma unroll
   for (int gr = 0; gr < G; ++gr) s[gr] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int ks = 0; ks < R::kFrags; ++ks)
-#pragma unroll
-    for (int gr = 0; gr < G; ++gr) s[gr] = Mma<T>::run(R::across(kb, gr * 16, ks, lane), st.q[ks], s[gr]);
+  products<T, DP, AHEAD>(kb, st.q, s, lane);
+  values();  // are there: they are read while the weights are computed
+  Columns<T, DP, AHEAD> v;
+  v.read(vb, 0, lane);
   if (edge) {
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) {
@@ -87,13 +87,10 @@ __device__ inline void attend(Online<T, DP>& st, uint32_t kb, uint32_t vb, uint3
   st.l += sum;
   // weights in the values' type: off by half a unit in their last place each, the sum
   // that they are divided by is not
+  typename R::frag w[G / P];
 #pragma unroll
-  for (int u = 0; u < G / P; ++u) {
-    const auto w = R::rounded(&s[u * P]);
-#pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt)
-      st.o[dt] = Mma<T>::run(R::down(vb, u * R::kUnit, dt, lane), w, st.o[dt]);
-  }
+  for (int u = 0; u < G / P; ++u) w[u] = R::rounded(&s[u * P]);
+  v.add(vb, w, st.o, lane);
 }
 
 // One row by a wave, key after key, without products of what is left out: a weight
@@ -160,14 +157,25 @@ __device__ __forceinline__ void careful_row(const BlockArgs& p, const Sequence& 
 }
 
 // Many queries.  A row whose result is not finite is left to the next kernel.
-template <class T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void block_attention_kernel(const BlockArgs p) {
-  using R = Rows<T, DP>;
-  __shared__ alignas(1024) uint8_t s_kv[2][2][R::kBytes];
-  __shared__ WalkMemory<WAVES> s_walk;
+// Waves that read, by the bytes of a row.
+constexpr int many_readers(int row) { return row <= 256 ? 12 : 6; }
+template <class T, int DP>
+struct ManyShape : WalkShape<T, DP, many_readers(DP * (int)sizeof(T)), (DP * sizeof(T) > 256 ? 1 : 2)> {
+  static constexpr int kAhead = DP * sizeof(T) == 256 ? 4 : 8;
+};
+
+template <class T, int DP>
+__global__ __launch_bounds__((ManyShape<T, DP>::kThreads)) void block_attention_kernel(const BlockArgs p) {
+  using Shape = ManyShape<T, DP>;
+  __shared__ typename Shape::Memory mem;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   WalkTile t;
-  if (!walk_tile<WAVES>(p, lane, t)) return;
+  if (!walk_tile(p, lane, t)) return;
+  walk_start<Shape>(mem, tid);
+  if (w >= Shape::kReaders) {
+    walk_loads<T, DP, Shape>(p, t, mem, lds_address(&mem), tid, w, lane);
+    return;
+  }
   const RowOf row = row_of(p, t, w, lane);
   Online<T, DP> st;
   start(st);
@@ -176,9 +184,11 @@ __global__ __launch_bounds__(64 * WAVES) void block_attention_kernel(const Block
                       (int64_t)(t.head * p.group + row.head) * p.q_head,
                   row.in, p.width, lane, st.q);
   const float c = p.scale * kLog2e;
-  walk_blocks<T, DP, WAVES>(p, t, row, s_walk, s_kv, tid, w, lane,
+  walk_blocks<T, DP, Shape, false>(p, t, row, mem, lds_address(&mem), tid, w, lane,
                             [&](const Halves& now, uint32_t sel, bool some, bool edge, uint32_t missing, uint32_t kb,
-                                uint32_t vb) { attend<T, DP>(st, kb, vb, sel, now, some, edge, missing, row, c, lane); });
+                                uint32_t vb, auto values) {
+                              attend<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, missing, row, c, lane, values);
+                            });
   const float l = across_sum(st.l), by = l > 0.0f ? 1.0f / l : 0.0f;
   bool bad = !__builtin_isfinite(l);
 #pragma unroll
@@ -191,16 +201,16 @@ __global__ __launch_bounds__(64 * WAVES) void block_attention_kernel(const Block
     if (p.lse != nullptr && lane < 16) p.lse[at] = l > 0.0f ? (st.m + __builtin_log2f(l)) * kLn2 : -INFINITY;
   }
   if (lane == 0)
-    p.again[(int64_t)blockIdx.x * WAVES + w] = (uint32_t)(rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xffffu;
+    p.again[(int64_t)blockIdx.x * Shape::kReaders + w] = (uint32_t)(rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xffffu;
 }
 
 // Those rows, key after key.
-template <class T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void block_attention_again_kernel(const BlockArgs p) {
+template <class T, int DP>
+__global__ __launch_bounds__((64 * ManyShape<T, DP>::kReaders)) void block_attention_again_kernel(const BlockArgs p) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   WalkTile t;
-  if (!walk_tile<WAVES>(p, lane, t)) return;
-  uint32_t rows = alike((int)p.again[(int64_t)blockIdx.x * WAVES + w]);
+  uint32_t rows = alike((int)p.again[(int64_t)blockIdx.x * ManyShape<T, DP>::kReaders + w]);
+  if (rows == 0 || !walk_tile(p, lane, t)) return;
   for (; rows != 0; rows &= rows - 1) {
     const int r = w * 16 + __builtin_ctz(rows), tok = r / p.group;
     careful_row<T, DP>(p, t.sq, t.seq, t.token0 + tok, t.head, r - tok * p.group, t.pos0 + tok, lane);
@@ -367,8 +377,9 @@ __global__ __launch_bounds__((64 * FewShape<T, DP>::kWaves)) void block_attentio
   const int count = alike(s_count), steps = ((count << lg_halves) + 1) / 2;
   const float c = p.scale * kLog2e;
   const uint32_t kb = lds_address(s_kv[w][0]), vb = lds_address(s_kv[w][1]);
-  KeySource<T, DP, 1> src;
-  src.init(p, sq, seq, f.head, 0, lane);
+  KeySource<T, DP> keys, values;
+  keys.init(p, p.k, sq, seq, f.head, lane);
+  values.init(p, p.v, sq, seq, f.head, lane);
   for (int s = f.split * WAVES + w; s < steps; s += WAVES * p.splits) {
     Halves now;
     uint32_t sel = 0;
@@ -381,12 +392,15 @@ __global__ __launch_bounds__((64 * FewShape<T, DP>::kWaves)) void block_attentio
       sel |= now.first[h] >= 0 && row.in ? 1u << h : 0u;
       edge |= now.first[h] + kHalf - 1 > pos;
     }
-    auto first = [&](int gr) { return now.of<T, DP>(gr); };
+    typename KeySource<T, DP>::Place k_place, v_place;
+    keys.find(now, k_place);
+    values.find(now, v_place);
     wait_reads();  // the step before has read its rows
-    src.load(kb, vb, 0, first);
-    const uint32_t missing = src.missing(first);
-    wait_loads<0>();
-    attend<T, DP>(st, kb, vb, sel, now, true, edge || missing != 0, missing, row, c, lane);
+    keys.load(kb, k_place, lane);
+    values.load(vb, v_place, lane);
+    wait_loads<KeySource<T, DP>::kLoads>();
+    attend<T, DP, 16>(st, kb, vb, sel, now, true, edge || k_place.missing != 0, k_place.missing, row, c, lane,
+                  [] { wait_loads<0>(); });
   }
   wait_reads();
   float* mine = reinterpret_cast<float*>(s_kv[w][0]);
@@ -443,8 +457,6 @@ __global__ __launch_bounds__(128) void block_attention_join_kernel(const BlockAr
   });
 }
 
-constexpr int kWaves = 8;  // of the many rows' kernel
-
 // A few rows' kernel up to this many (token, key-value head) pairs.
 constexpr int64_t kFewPairs = 4096;
 
@@ -452,6 +464,8 @@ struct Plan {
   bool few;
   int splits;
   int64_t groups;  // (token, head, chunk) triples of the few rows' kernel
+  int readers, per;
+  int64_t tiles;
   size_t bytes;
 };
 Plan plan_of(int val_t, const fs_block_seqs& s, int heads, int group, int width, int top) {
@@ -470,7 +484,10 @@ Plan plan_of(int val_t, const fs_block_seqs& s, int heads, int group, int width,
     if (o.splits > 1)
       o.bytes = (size_t)(o.groups * o.splits) * (32 + 16 * (width <= 64 ? 64 : width <= 128 ? 128 : 256)) * 4;
   } else {
-    o.bytes = (size_t)(block_tiles(s, tokens_of<kWaves>(group)) * heads) * kWaves * 4;
+    o.readers = many_readers((width <= 64 ? 64 : width <= 128 ? 128 : 256) * (val_t == FS_F32 ? 4 : 2));
+    o.per = o.readers * 16 / group;
+    o.tiles = block_tiles(s, o.per);
+    o.bytes = (size_t)(o.tiles * heads) * o.readers * 4;
   }
   return o;
 }
@@ -538,12 +555,13 @@ extern "C" int fs_block_attention(int val_t, const fs_block_seqs* seqs, int head
       }
       return FS_OK;
     }
-    p.tiles = block_tiles(*seqs, tokens_of<kWaves>(group));
+    p.tiles = plan.tiles;
+    p.per = plan.per;
     if (p.tiles * heads > kMostWorkgroups) return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
-    const dim3 grid((uint32_t)(p.tiles * heads)), threads(64 * kWaves);
-    hipLaunchKernelGGL((block_attention_kernel<T, DP, kWaves>), grid, threads, 0, stream, p);
+    const dim3 grid((uint32_t)(p.tiles * heads));
+    hipLaunchKernelGGL((block_attention_kernel<T, DP>), grid, dim3(ManyShape<T, DP>::kThreads), 0, stream, p);
     FS_CHECK_MAIN_LAUNCH("block_attention_kernel");
-    hipLaunchKernelGGL((block_attention_again_kernel<T, DP, kWaves>), grid, threads, 0, stream, p);
+    hipLaunchKernelGGL((block_attention_again_kernel<T, DP>), grid, dim3(64 * ManyShape<T, DP>::kReaders), 0, stream, p);
     FS_CHECK_LAUNCH("block_attention_again_kernel");
     return FS_OK;
   });

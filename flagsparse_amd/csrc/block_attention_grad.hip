@@ -16,7 +16,10 @@
 namespace fs {
 namespace {
 
-constexpr int kAmaxParts = 256, kQueryWaves = 8;
+constexpr int kAmaxParts = 256;
+
+// Waves that read, of the queries' gradient, by the bytes of a row.
+constexpr int query_readers(int row) { return row <= 128 ? 12 : row <= 256 ? 8 : 6; }
 
 // dS of 16-bit floats, whose small values have few bits: G and <G, O> are multiplied
 // by the power of two that brings G's largest value to [1, 2), and the gradients
@@ -69,21 +72,19 @@ struct QueryGrad {
   float lse, delta;  // in powers of two; times the factor
 };
 
-template <class T, int DP>
+template <class T, int DP, int AHEAD, class Wait>
 __device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, uint32_t sel, const Halves& now, bool some,
-                            bool edge, const RowOf& row, float c, float factor, int lane) {
+                            bool edge, const RowOf& row, float c, float factor, int lane, Wait values) {
   using R = Rows<T, DP>;
   constexpr int G = R::kGroups, P = R::kUnit / 16;
   f32x4 s[G], dp[G];
 #pragma unroll
   for (int gr = 0; gr < G; ++gr) s[gr] = dp[gr] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int ks = 0; ks < R::kFrags; ++ks)
-#pragma unroll
-    for (int gr = 0; gr < G; ++gr) {
-      s[gr] = Mma<T>::run(R::across(kb, gr * 16, ks, lane), st.q[ks], s[gr]);
-      dp[gr] = Mma<T>::run(R::across(vb, gr * 16, ks, lane), st.g[ks], dp[gr]);
-    }
+  products<T, DP, AHEAD>(kb, st.q, s, lane);
+  values();  // are there
+  products<T, DP, AHEAD>(vb, st.g, dp, lane);
+  Columns<T, DP, AHEAD> k;
+  k.read(kb, 0, lane);
 #pragma unroll
   for (int gr = 0; gr < G; ++gr)
 #pragma unroll
@@ -108,13 +109,10 @@ __device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, uint
     }
   }
   // (dS in the values' type, rounded once)
+  typename R::frag w[G / P];
 #pragma unroll
-  for (int u = 0; u < G / P; ++u) {
-    const auto w = R::rounded(&s[u * P]);
-#pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt)
-      st.d[dt] = Mma<T>::run(R::down(kb, u * R::kUnit, dt, lane), w, st.d[dt]);
-  }
+  for (int u = 0; u < G / P; ++u) w[u] = R::rounded(&s[u * P]);
+  k.add(kb, w, st.d, lane);
 }
 
 struct GradArgs {
@@ -185,15 +183,25 @@ __device__ __forceinline__ void careful_query(const GradArgs& a, const Sequence&
     if (i * 64 + lane < p.width) out[i * 64 + lane] = (T)(d[i] * p.scale);
 }
 
-template <class T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void block_query_grad_kernel(const GradArgs a) {
+template <class T, int DP>
+struct QueryGradShape : WalkShape<T, DP, query_readers(DP * (int)sizeof(T)), (DP * sizeof(T) > 256 ? 1 : 2)> {
+  static constexpr int kAhead = 8;
+};
+
+template <class T, int DP>
+__global__ __launch_bounds__((QueryGradShape<T, DP>::kThreads)) void block_query_grad_kernel(const GradArgs a) {
   using R = Rows<T, DP>;
-  __shared__ alignas(1024) uint8_t s_kv[2][2][R::kBytes];
-  __shared__ WalkMemory<WAVES> s_walk;
+  using Shape = QueryGradShape<T, DP>;
+  __shared__ typename Shape::Memory mem;
   const BlockArgs& p = a.b;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   WalkTile t;
-  if (!walk_tile<WAVES>(p, lane, t)) return;
+  if (!walk_tile(p, lane, t)) return;
+  walk_start<Shape>(mem, tid);
+  if (w >= Shape::kReaders) {
+    walk_loads<T, DP, Shape>(p, t, mem, lds_address(&mem), tid, w, lane);
+    return;
+  }
   const RowOf row = row_of(p, t, w, lane);
   const float factor = read_factor<T>(a.amax, lane);
   QueryGrad<T, DP> st;
@@ -218,9 +226,9 @@ __global__ __launch_bounds__(64 * WAVES) void block_query_grad_kernel(const Grad
 #pragma unroll
   for (int dt = 0; dt < DP / 16; ++dt) st.d[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   const float c = p.scale * kLog2e;
-  walk_blocks<T, DP, WAVES>(p, t, row, s_walk, s_kv, tid, w, lane,
-                            [&](const Halves& now, uint32_t sel, bool some, bool edge, uint32_t, uint32_t kb,
-                                uint32_t vb) { take<T, DP>(st, kb, vb, sel, now, some, edge, row, c, factor, lane); });
+  walk_blocks<T, DP, Shape, false>(p, t, row, mem, lds_address(&mem), tid, w, lane,
+                            [&](const Halves& now, uint32_t sel, bool some, bool edge, uint32_t, uint32_t kb, uint32_t vb,
+                                auto values) { take<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, row, c, factor, lane, values); });
   bool bad = false;
 #pragma unroll
   for (int dt = 0; dt < DP / 16; ++dt)
@@ -229,17 +237,17 @@ __global__ __launch_bounds__(64 * WAVES) void block_query_grad_kernel(const Grad
   const uint64_t rows = __ballot(bad && row.in);
   if (row.in) store_row<T, DP>(static_cast<T*>(p.out) + at * p.width, st.d, p.scale / factor, p.width, lane);
   if (lane == 0)
-    p.again[(int64_t)blockIdx.x * WAVES + w] = (uint32_t)(rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xffffu;
+    p.again[(int64_t)blockIdx.x * Shape::kReaders + w] = (uint32_t)(rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xffffu;
 }
 
 // Rows whose gradient is not finite, key after key.
-template <class T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void block_query_grad_again_kernel(const GradArgs a) {
+template <class T, int DP>
+__global__ __launch_bounds__((64 * QueryGradShape<T, DP>::kReaders)) void block_query_grad_again_kernel(const GradArgs a) {
   const BlockArgs& p = a.b;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   WalkTile t;
-  if (!walk_tile<WAVES>(p, lane, t)) return;
-  uint32_t rows = alike((int)p.again[(int64_t)blockIdx.x * WAVES + w]);
+  uint32_t rows = alike((int)p.again[(int64_t)blockIdx.x * QueryGradShape<T, DP>::kReaders + w]);
+  if (rows == 0 || !walk_tile(p, lane, t)) return;
   for (; rows != 0; rows &= rows - 1) {
     const int r = w * 16 + __builtin_ctz(rows), tok = r / p.group, in_group = r - tok * p.group;
     const int64_t at = (int64_t)(t.token0 + tok) * p.heads * p.group + t.head * p.group + in_group;
@@ -756,9 +764,11 @@ struct GradPlan {
   int64_t key_blocks, n_keys;
   int64_t pieces, places;  // at most
   int most;                // entries a piece
+  int per;                 // tokens a workgroup of the queries' gradient
+  int64_t tiles;
   size_t again, sort, keys, sorted, order, starts, list, sums, count, delta, amax, parts, bytes;
 };
-GradPlan grad_plan(const fs_block_seqs& s, int heads, int group, int lists, int width, int top) {
+GradPlan grad_plan(int val_t, const fs_block_seqs& s, int heads, int group, int lists, int width, int top) {
   GradPlan l{};
   const int64_t tokens = s.n_tokens, rows = s.n_rows, n_seqs = s.n_seqs;
   const int block = s.block;
@@ -779,7 +789,11 @@ GradPlan grad_plan(const fs_block_seqs& s, int heads, int group, int lists, int 
     at += up(n);
     return a;
   };
-  l.again = take((size_t)(block_tiles(s, tokens_of<kQueryWaves>(group)) * heads) * kQueryWaves * 4);
+  const int dp = width <= 64 ? 64 : width <= 128 ? 128 : 256;
+  const int readers = query_readers(dp * (val_t == FS_F32 ? 4 : 2));
+  l.per = readers * 16 / group;
+  l.tiles = block_tiles(s, l.per);
+  l.again = take((size_t)(l.tiles * heads) * readers * 4);
   l.sort = take(select_sort_bytes(l.entries, l.n_keys));
   l.keys = take((size_t)l.entries * 4);
   l.sorted = take((size_t)l.entries * 4);
@@ -790,7 +804,6 @@ GradPlan grad_plan(const fs_block_seqs& s, int heads, int group, int lists, int 
   l.count = take(4);
   l.delta = take((size_t)tokens * heads * group * 4);
   l.amax = take(kAmaxParts * 4);
-  const int dp = width <= 64 ? 64 : width <= 128 ? 128 : 256;
   l.parts = take((size_t)(l.places * shared) * block * 2 * dp * 4);
   l.bytes = at;
   return l;
@@ -815,7 +828,7 @@ extern "C" size_t fs_block_attention_grad_workspace_bytes(int val_t, const fs_bl
                                                           int width, int lists, int top) {
   using namespace fs;
   if (grad_fault("", val_t, seqs, heads, group, width, lists, top) != FS_OK) return 0;
-  return grad_plan(*seqs, heads, group, lists, width, top).bytes;
+  return grad_plan(val_t, *seqs, heads, group, lists, width, top).bytes;
 }
 
 extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int heads, int group, int width, int lists,
@@ -836,7 +849,7 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
       (((int64_t)(uintptr_t)q | (int64_t)(uintptr_t)grad | q_token * size | q_head * size) & 15) != 0)
     return fail(FS_E_INVALID, std::string(who) + ": queries, keys, values and grad need rows at multiples of 16 bytes");
   if (!(scale > 0.0) || !(scale < 1e30)) return fail(FS_E_INVALID, std::string(who) + ": scale must be positive");
-  const GradPlan l = grad_plan(*seqs, heads, group, lists, width, top);
+  const GradPlan l = grad_plan(val_t, *seqs, heads, group, lists, width, top);
   if (ws == nullptr || ws_bytes < l.bytes) return fail(FS_E_WORKSPACE, std::string(who) + ": workspace too small");
   uint8_t* m = static_cast<uint8_t*>(ws);
   GradArgs a{};
@@ -895,20 +908,21 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
   FS_CHECK_LAUNCH("block_pieces_kernel");
   return with_block_width(val_t, width, who, [&](auto val, auto dp) -> int {
     using T = decltype(val);
-    constexpr int DP = decltype(dp)::value, WAVES = kQueryWaves;
+    constexpr int DP = decltype(dp)::value;
     if (tokens > 0) {
       if constexpr (kFactored<T>) {
         hipLaunchKernelGGL((block_amax_kernel<T>), dim3(kAmaxParts), dim3(256), 0, stream, static_cast<const T*>(grad),
                            tokens * heads * group * width, amax);
         FS_CHECK_LAUNCH("block_amax_kernel");
       }
-      p.tiles = block_tiles(*seqs, tokens_of<WAVES>(group));
+      p.tiles = l.tiles;
+      p.per = l.per;
       if (p.tiles * heads > kMostWorkgroups) return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
-      hipLaunchKernelGGL((block_query_grad_kernel<T, DP, WAVES>), dim3((uint32_t)(p.tiles * heads)), dim3(64 * WAVES), 0,
-                         stream, a);
+      const dim3 grid((uint32_t)(p.tiles * heads));
+      hipLaunchKernelGGL((block_query_grad_kernel<T, DP>), grid, dim3(QueryGradShape<T, DP>::kThreads), 0, stream, a);
       FS_CHECK_MAIN_LAUNCH("block_query_grad_kernel");
-      hipLaunchKernelGGL((block_query_grad_again_kernel<T, DP, WAVES>), dim3((uint32_t)(p.tiles * heads)),
-                         dim3(64 * WAVES), 0, stream, a);
+      hipLaunchKernelGGL((block_query_grad_again_kernel<T, DP>), grid, dim3(64 * QueryGradShape<T, DP>::kReaders), 0,
+                         stream, a);
       FS_CHECK_LAUNCH("block_query_grad_again_kernel");
     }
     const int64_t shared = heads / lists;

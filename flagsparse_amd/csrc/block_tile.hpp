@@ -197,6 +197,59 @@ struct Rows {
   }
 };
 
+// Reads of LDS run ahead of the products that use them, AHEAD fragments at a time:
+// left to itself the compiler waits for each by itself.
+__device__ inline void fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// s[gr] += rows 16 gr .. of the tile at lds times the lane's row, in f: scores, or
+// products of values with a gradient.
+template <class T, int DP, int AHEAD>
+__device__ inline void products(uint32_t lds, const typename Mma<T>::frag (&f)[Rows<T, DP>::kFrags],
+                                f32x4 (&s)[Rows<T, DP>::kGroups], int lane) {
+  using R = Rows<T, DP>;
+  constexpr int G = R::kGroups, F = R::kFrags, kStep = AHEAD / G < F ? AHEAD / G : F;  // fragments' columns at a time
+#pragma unroll
+  for (int k0 = 0; k0 < F; k0 += kStep) {
+    typename R::frag x[kStep][G];
+#pragma unroll
+    for (int ks = 0; ks < kStep; ++ks)
+#pragma unroll
+      for (int gr = 0; gr < G; ++gr) x[ks][gr] = R::across(lds, gr * 16, k0 + ks, lane);
+    fence();
+#pragma unroll
+    for (int ks = 0; ks < kStep; ++ks)
+#pragma unroll
+      for (int gr = 0; gr < G; ++gr) s[gr] = Mma<T>::run(x[ks][gr], f[k0 + ks], s[gr]);
+  }
+}
+// Columns of the tile: the first operands of the products over its rows.
+template <class T, int DP, int AHEAD>
+struct Columns {
+  using R = Rows<T, DP>;
+  static constexpr int kUnits = R::kKeys / R::kUnit, kAll = kUnits * (DP / 16), kStep = kAll < AHEAD ? kAll : AHEAD;
+  typename R::frag x[kStep];
+  __device__ void read(uint32_t lds, int first, int lane) {
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) {
+      const int at = first + i;
+      x[i] = R::down(lds, at / (DP / 16) * R::kUnit, at % (DP / 16), lane);
+    }
+    fence();
+  }
+  // o[dt] += columns times w, after read(lds, 0): what is left is read here.
+  __device__ void add(uint32_t lds, const typename R::frag (&w)[kUnits], f32x4 (&o)[DP / 16], int lane) {
+#pragma unroll
+    for (int first = 0; first < kAll; first += kStep) {
+      if (first > 0) read(lds, first, lane);
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        const int at = first + i;
+        o[at % (DP / 16)] = Mma<T>::run(x[i], w[at / (DP / 16)], o[at % (DP / 16)]);
+      }
+    }
+  }
+};
+
 // The largest, and the sum, of a value over the four lanes of a query.
 __device__ inline float across_max(float x) {
   auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -227,116 +280,10 @@ struct BlockArgs {
   int lg_groups;  // log2 of a block's groups of 16 keys
   float scale;
   int64_t tiles;    // workgroups a head
+  int per;          // tokens a workgroup
   uint32_t* again;  // many rows: a word a wave, its rows whose result is not finite
   int splits;
   float* parts;
-};
-
-// Keys and values of one sequence and head, and a lane's part of the loads of a step:
-// wave w of WAVES takes kLoads instructions for the keys and as many for the values.
-template <class T, int DP, int WAVES>
-struct KeySource {
-  using R = Rows<T, DP>;
-  static constexpr int kLoads = R::kBytes / 1024 / WAVES;
-  static constexpr int kOffsets = kLoads * R::kAtOnce < 16 ? kLoads : 16 / R::kAtOnce;
-  static_assert(R::kBytes % (1024 * WAVES) == 0, "whole loads a wave");
-  const char *k, *v;
-  uint32_t k_row, v_row;      // bytes
-  uint32_t k_off[kOffsets], v_off[kOffsets];
-  const int32_t* table;       // the sequence's pages, or null
-  int64_t k_page, v_page, n_pages;
-  int per_seq, shift, keys;
-  int row;  // the lane's, of the first load
-
-  __device__ void init(const BlockArgs& p, const Sequence& sq, int seq, int head, int w, int lane) {
-    k = static_cast<const char*>(p.k.base) + (head * p.k.head + sq.row0 * p.k.row) * (int64_t)sizeof(T);
-    v = static_cast<const char*>(p.v.base) + (head * p.v.head + sq.row0 * p.v.row) * (int64_t)sizeof(T);
-    k_row = (uint32_t)(p.k.row * (int64_t)sizeof(T));
-    v_row = (uint32_t)(p.v.row * (int64_t)sizeof(T));
-    keys = sq.keys;
-    table = p.seqs.pages == nullptr ? nullptr : p.seqs.pages + (int64_t)seq * p.seqs.ld_pages;
-    k_page = p.k.page * (int64_t)sizeof(T);
-    v_page = p.v.page * (int64_t)sizeof(T);
-    n_pages = p.seqs.n_pages;
-    per_seq = (int)p.seqs.pages_per_seq;
-    shift = p.seqs.page_shift;
-    row = w * kLoads * R::kAtOnce % 16 + R::lane_row(lane);
-#pragma unroll
-    for (int n = 0; n < kOffsets; ++n) {
-      const int r = row + n * R::kAtOnce, piece = (lane % R::kPieces) ^ R::swizzle(r);
-      const bool in = piece * 16 < p.width * (int)sizeof(T);
-      k_off[n] = in ? (uint32_t)r * k_row + (uint32_t)piece * 16 : 2u * kInBuffer;
-      v_off[n] = in ? (uint32_t)r * v_row + (uint32_t)piece * 16 : 2u * kInBuffer;
-    }
-  }
-  // The page of the 16 keys from position j on; negative: outside the cache.
-  __device__ int64_t page_of(int j) const {
-    const int at = j >> shift;
-    const int64_t page = at < per_seq ? table[at] : -1;
-    return page < n_pages ? page : -1;
-  }
-  // One step's keys to LDS at kb, values at vb, zeros past the sequence's end, past the
-  // width and for pages outside the cache.  first(group): the position of a group's
-  // first key, negative for none.  (All lanes alike but for the rows.)
-  template <class First>
-  __device__ void load(uint32_t kb, uint32_t vb, int w, First first) const {
-    constexpr int kAGroup = 16 / R::kAtOnce;  // loads
-    const char *k0 = k, *v0 = v;
-    int j = -1;
-#pragma unroll
-    for (int n = 0; n < kLoads; ++n) {
-      const int row0 = (w * kLoads + n) * R::kAtOnce;
-      if (n % kAGroup == 0) {
-        j = first(row0 / 16);
-        k0 = k;
-        v0 = v;
-        if (j >= 0) {
-          int64_t jj = j;
-          if (table != nullptr) {
-            const int64_t page = page_of(j);
-            if (page < 0) {
-              j = -1;
-            } else {
-              k0 += page * k_page;
-              v0 += page * v_page;
-              jj = j & ((1 << shift) - 1);
-            }
-          }
-          if (j >= 0) {
-            k0 += jj * k_row;
-            v0 += jj * v_row;
-          }
-        }
-      }
-      // (rows of the group that are keys)
-      const int left = j >= 0 ? keys - j : 0;
-      const bool in = row + n % kAGroup * R::kAtOnce < left;
-      const uint32_t to = (uint32_t)row0 * R::kRow;
-      lds_dma<16>((uint32_t)alike((int)(kb + to)), in ? k_off[n % kOffsets] : 2u * kInBuffer, buffer_at(k0));
-      lds_dma<16>((uint32_t)alike((int)(vb + to)), in ? v_off[n % kOffsets] : 2u * kInBuffer, buffer_at(v0));
-    }
-  }
-  // Which groups of a step lie in pages outside the cache, a bit each.
-  template <class First>
-  __device__ uint32_t missing(First first) const {
-    uint32_t m = 0;
-    if (table != nullptr) {
-#pragma unroll
-      for (int gr = 0; gr < R::kGroups; ++gr) {
-        const int j = first(gr);
-        if (j >= 0 && page_of(j) < 0) m |= 1u << gr;
-      }
-    }
-    return m;
-  }
-};
-
-// 16 query rows of a wave: lanes with the same lane % 16 hold one row's state.
-struct RowOf {
-  int token;  // within the workgroup's tile
-  int head;   // within the group
-  int pos;    // its position; -1 and less: before the first key
-  bool in;
 };
 
 // A step's two halves: the position of each one's first key (negative: none).
@@ -349,6 +296,109 @@ struct Halves {
     const int f = second ? first[1] : first[0];
     return f < 0 ? -1 : f + (group - (second ? kHalf : 0)) * 16;
   }
+};
+
+// Keys, or values, of one sequence and head, and a wave's loads of a step of them.
+template <class T, int DP>
+struct KeySource {
+  using R = Rows<T, DP>;
+  static constexpr int kLoads = R::kBytes / 1024, kGroups = R::kGroups;
+  static constexpr int kAGroup = 16 / R::kAtOnce;  // loads of 16 rows
+  const char* base;
+  uint32_t row;           // bytes
+  uint32_t off[kAGroup];  // a lane's, within 16 rows
+  // the sequence's pages, or null (constant for the call: scalar loads, which leave the
+  // count of loads under way alone)
+  typedef const __attribute__((address_space(4))) int32_t Constant;
+  Constant* table;
+  int64_t page, n_pages;
+  int per_seq, shift, keys;
+
+  __device__ void init(const BlockArgs& p, const RowLayout& l, const Sequence& sq, int seq, int head, int lane) {
+    base = static_cast<const char*>(l.base) + (head * l.head + sq.row0 * l.row) * (int64_t)sizeof(T);
+    row = (uint32_t)(l.row * (int64_t)sizeof(T));
+    keys = sq.keys;
+    table = p.seqs.pages == nullptr ? nullptr : (Constant*)(p.seqs.pages + (int64_t)seq * p.seqs.ld_pages);
+    page = l.page * (int64_t)sizeof(T);
+    n_pages = p.seqs.n_pages;
+    per_seq = (int)p.seqs.pages_per_seq;
+    shift = p.seqs.page_shift;
+#pragma unroll
+    for (int n = 0; n < kAGroup; ++n) {
+      const int r = R::lane_row(lane) + n * R::kAtOnce, piece = (lane % R::kPieces) ^ R::swizzle(r);
+      const bool in = piece * 16 < p.width * (int)sizeof(T);
+      off[n] = in ? (uint32_t)r * row + (uint32_t)piece * 16 : 2u * kInBuffer;
+    }
+  }
+  // Where a step lies.  `whole`: all its rows are keys and one behind the other, from
+  // first.at[0] on; otherwise the first byte of each group of 16 keys, and how many of
+  // its rows are keys.  Bits of the groups whose page is outside the cache.
+  struct Place {
+    const char* at[kGroups];
+    int left[kGroups];
+    uint32_t missing;
+    bool whole;
+  };
+  // The step whose rows are keys j .. j + kKeys - 1 of the page `id` (without pages: 0).
+  __device__ const char* rows_at(int64_t id, int j) const {
+    return table == nullptr ? base + (int64_t)j * row : base + id * page + (int64_t)(j & ((1 << shift) - 1)) * row;
+  }
+  __device__ void find(const Halves& h, Place& o) const {
+    o.missing = 0;
+    o.whole = false;
+#pragma unroll
+    for (int gr = 0; gr < kGroups; ++gr) {
+      const int j = h.of<T, DP>(gr);
+      o.at[gr] = base;
+      o.left[gr] = 0;
+      if (j >= 0 && j < keys) {
+        if (table == nullptr) {
+          o.at[gr] = base + (int64_t)j * row;
+          o.left[gr] = keys - j;
+        } else {
+          const int t = j >> shift;
+          const int64_t id = t < per_seq ? table[t] : -1;
+          if (id >= 0 && id < n_pages) {
+            o.at[gr] = rows_at(id, j);
+            o.left[gr] = keys - j;
+          } else {
+            o.missing |= 1u << gr;
+          }
+        }
+      }
+    }
+  }
+  // One step to LDS, zeros past the sequence's end, past the width and for pages outside
+  // the cache.
+  __device__ void load(uint32_t lds, const Place& o, int lane) const {
+    if (o.whole) {
+      const u32x4 rsrc = buffer_at(o.at[0]);
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr)
+#pragma unroll
+        for (int n = 0; n < kAGroup; ++n)
+          lds_dma_shifted(lds + (uint32_t)(gr * 16 * R::kRow + n * 1024), off[n], rsrc, (uint32_t)(gr * 16) * row);
+      return;
+    }
+#pragma unroll
+    for (int gr = 0; gr < kGroups; ++gr) {
+      const u32x4 rsrc = buffer_at(o.at[gr]);
+      const uint32_t to = lds + (uint32_t)(gr * 16 * R::kRow);
+#pragma unroll
+      for (int n = 0; n < kAGroup; ++n) {
+        const bool in = R::lane_row(lane) + n * R::kAtOnce < o.left[gr];
+        lds_dma<16>(to + (uint32_t)n * 1024, in ? off[n] : 2u * kInBuffer, rsrc);
+      }
+    }
+  }
+};
+
+// 16 query rows of a wave: lanes with the same lane % 16 hold one row's state.
+struct RowOf {
+  int token;  // within the workgroup's tile
+  int head;   // within the group
+  int pos;    // its position; -1 and less: before the first key
+  bool in;
 };
 
 // Fragments of a lane's row of a dense or strided array, zeros outside.

@@ -3,12 +3,24 @@
 // (block_attention.hip, block_attention_grad.hip).
 //
 // A workgroup takes consecutive tokens of a sequence, all heads of one group, 16
-// rows a wave.  Tokens near each other select many of the same
-// blocks: a table in LDS holds, for each block of a window of the sequence, a bit
-// for each token that selects it.  The blocks with a bit are walked in order, keys
-// and values loaded once for the workgroup, and a wave takes part with the tiles
-// that have a token of the block.
+// rows a wave.  Tokens near each other select many of the same blocks: a table in LDS
+// holds, for each block of a window of the sequence, a bit for each token that selects
+// it.  The blocks with a bit are walked in order, keys and values loaded once for the
+// workgroup, and a wave takes part where one of its tokens selects the block.
+//
+// Which waves take part differs from block to block, so the waves do not meet at a
+// barrier: some waves load, in pairs, one the keys and one the values of a step, into a
+// ring of slots, the pairs in turn, and the others follow each at its own pace.  A
+// loader says in LDS which step a slot holds; a wave that has read it adds one to the
+// slot's count, and a slot is loaded again when all that take part have.  Every wait
+// ends: each wave goes through its steps in order; the first step that is not yet read
+// by all waits for its loaders alone, who wait for the readers of the step that had its
+// slot before, an earlier one; and a loader that waits has announced what it has loaded.
+// A loader is one wave, which issues an instruction in four or five cycles: what it
+// needs is laid out 64 blocks at a time, a lane each.
 #pragma once
+
+#include <cstddef>
 
 #include "block_tile.hpp"
 
@@ -17,11 +29,23 @@ namespace {
 
 constexpr int kMaskWords = 2048;
 
-template <int WAVES>
-struct WalkMemory {
-  uint32_t mask[kMaskWords];
-  uint16_t list[kMaskWords];
-  uint32_t total[WAVES];
+// Waves that read, pairs that load, and slots by what LDS holds.
+template <class T, int DP, int READERS, int PAIRS>
+struct WalkShape {
+  static constexpr int kReaders = READERS, kPairs = PAIRS, kWaves = READERS + 2 * PAIRS, kThreads = 64 * kWaves;
+  static constexpr int kBytes = Rows<T, DP>::kBytes;
+  static constexpr int kSlots = kBytes > 16384 ? 2 : 4;
+  static_assert(kSlots % PAIRS == 0, "a slot is one pair's");
+  struct alignas(1024) Memory {
+    uint8_t kv[kSlots][2][kBytes];  // (first: kv0 in what follows is its address)
+    uint32_t mask[kMaskWords];
+    uint64_t part[READERS][kMaskWords / 64];  // units that a wave takes part in
+    uint16_t list[kMaskWords];
+    uint32_t total[kWaves];
+    uint32_t ready[2][kSlots];  // 1 + the step that a slot holds; of the keys, of the values
+    uint32_t missing[kSlots];
+    uint32_t done[kSlots];
+  };
 };
 
 // What a workgroup works on.
@@ -30,25 +54,19 @@ struct WalkTile {
   int seq, head;
   int token0, tokens;  // of all tokens; how many
   int pos0;            // position of the first
-  int per;             // tokens a full tile
 };
-
-template <int WAVES>
-__host__ __device__ inline int tokens_of(int group) { return WAVES * 16 / group; }
 
 // Head by head over the XCDs (each has its keys and values in a cache of its own), a
 // head's last tiles first: they have the most blocks to choose from.
-template <int WAVES>
 __device__ inline bool walk_tile(const BlockArgs& p, int lane, WalkTile& t) {
   const int64_t at = xcd_range_block(blockIdx.x, gridDim.x);
   t.head = (int)(at / p.tiles);
-  t.per = tokens_of<WAVES>(p.group);
   int tile;
-  if (!find_tile(p.seqs, t.per, p.tiles - 1 - at % p.tiles, lane, t.seq, tile)) return false;
+  if (!find_tile(p.seqs, p.per, p.tiles - 1 - at % p.tiles, lane, t.seq, tile)) return false;
   t.sq = sequence_of(p.seqs, t.seq);
-  const int first = tile * t.per;
+  const int first = alike(tile) * p.per;
   t.token0 = t.sq.first + first;
-  t.tokens = t.sq.count - first < t.per ? t.sq.count - first : t.per;
+  t.tokens = t.sq.count - first < p.per ? t.sq.count - first : p.per;
   t.pos0 = t.sq.keys - t.sq.count + first;
   return true;
 }
@@ -65,23 +83,50 @@ __device__ inline RowOf row_of(const BlockArgs& p, const WalkTile& t, int w, int
   return o;
 }
 
-// A lane's selection in a step has a bit for each half.
-template <class T, int DP, int WAVES, class Body>
-__device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const RowOf& row,
-                                   WalkMemory<WAVES>& mem, uint8_t (&kv)[2][2][Rows<T, DP>::kBytes], int tid, int w,
-                                   int lane, Body body) {
+// Words in LDS that other waves of the workgroup write, by their addresses.
+__device__ inline uint32_t look(uint32_t at) { return (uint32_t)alike((int)*(volatile lds_word*)(uintptr_t)at); }
+__device__ inline void tell(uint32_t at, uint32_t v) { *(volatile lds_word*)(uintptr_t)at = v; }
+__device__ inline void in_order() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+template <class Shape>
+__device__ inline void walk_start(typename Shape::Memory& mem, int tid) {
+  if (tid < Shape::kSlots) mem.ready[0][tid] = mem.ready[1][tid] = mem.done[tid] = 0u;
+}
+
+// The walk of a wave that loads (LOADS) or reads: body(...) takes a step.  Both kinds
+// meet at the same barriers; each has code of its own, so that a loader's holds no rows.
+template <class T, int DP, class Shape, bool LOADS, class Body>
+__device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const RowOf& row, typename Shape::Memory& mem,
+                                   uint32_t kv0, int tid, int w, int lane, Body body) {
   using R = Rows<T, DP>;
-  constexpr int THREADS = 64 * WAVES, kHalf = R::kKeys / 2;
+  constexpr int THREADS = Shape::kThreads, READERS = Shape::kReaders, S = Shape::kSlots, kHalf = R::kKeys / 2;
+  constexpr int kLoads = KeySource<T, DP>::kLoads;
   const int lg_block = p.lg_groups + 4;
   const int lg_halves = lg_block - (kHalf == 32 ? 5 : 4);  // of a block's halves of a step
-  const int words = (t.per + 31) / 32, window = kMaskWords / words;
+  // a unit: a block, or two of half a step
+  const bool pairs = lg_halves == 0;
+  const int lg_steps = pairs ? 0 : lg_halves - 1;  // of a unit
+  const int words = (p.per + 31) / 32, window = kMaskWords / words;
   const int last = t.pos0 + t.tokens - 1;
   const int n_blocks = last < 0 ? 0 : (last >> lg_block) + 1;
   const int entries = t.tokens * p.top;
   const int32_t* ids = p.blocks + (int64_t)t.token0 * p.b_token + (int64_t)t.head * p.b_head;
-  KeySource<T, DP, WAVES> src;
-  src.init(p, t.sq, t.seq, t.head, w, lane);
-  const uint32_t kv0 = lds_address(kv);
+  // the words that hold the wave's tokens, and their bits
+  const int t_lo = w * 16 / p.group, t_hi = (w * 16 + 15) / p.group;
+  const int word_lo = t_lo >> 5, word_hi = t_hi >> 5;
+  const uint32_t bits_lo = word_lo == word_hi ? (uint32_t)(((uint64_t)1 << (t_hi - t_lo + 1)) - 1) << (t_lo & 31)
+                                              : ~0u << (t_lo & 31);
+  const uint32_t bits_hi = word_lo == word_hi ? 0u : (uint32_t)(((uint64_t)1 << ((t_hi & 31) + 1)) - 1);
+  const uint32_t ready0 = kv0 + (uint32_t)offsetof(typename Shape::Memory, ready);
+  const uint32_t missing0 = kv0 + (uint32_t)offsetof(typename Shape::Memory, missing);
+  const uint32_t done0 = kv0 + (uint32_t)offsetof(typename Shape::Memory, done);
+  uint32_t base = 0;  // steps of the windows before
+  uint32_t expected[S / Shape::kPairs];  // readings of a loader's slots so far
+#pragma unroll
+  for (int i = 0; i < S / Shape::kPairs; ++i) expected[i] = 0u;
 
   for (int w0 = 0; w0 < n_blocks; w0 += window) {
     __syncthreads();
@@ -112,7 +157,7 @@ __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const 
     uint32_t at = upto - mine;
     int count = 0;
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) {
+    for (int i = 0; i < Shape::kWaves; ++i) {
       if (i < w) at += mem.total[i];
       count += (int)mem.total[i];
     }
@@ -120,50 +165,173 @@ __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const 
     for (int i = 0; i < each; ++i)
       if (named(tid * each + i)) mem.list[at++] = (uint16_t)(tid * each + i);
     __syncthreads();
-
-    const int steps = ((count << lg_halves) + 1) / 2;
-    Halves next;
-    int next_slot[2];
-    uint32_t next_missing;
-    auto prepare = [&](int s) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int q = 2 * s + h, e = q >> lg_halves;
-        const int slot = alike((int)mem.list[e < count ? e : 0]);
-        next_slot[h] = slot;
-        next.first[h] = e < count ? ((w0 + slot) << lg_block) + (q & ((1 << lg_halves) - 1)) * kHalf : -1;
+    const int units = pairs ? (count + 1) / 2 : count;
+    if constexpr (!LOADS) {
+      for (int u0 = 0; u0 < units; u0 += 64) {
+        uint32_t any = 0;
+        for (int h = 0; h < (pairs ? 2 : 1); ++h) {
+          const int e = pairs ? 2 * (u0 + lane) + h : u0 + lane;
+          if (e < count) {
+            const uint32_t* m = &mem.mask[mem.list[e] * words];
+            if (word_lo < words) any |= m[word_lo] & bits_lo;
+            if (word_hi < words) any |= m[word_hi] & bits_hi;
+          }
+        }
+        const uint64_t m = __ballot(any != 0);
+        if (lane == 0) mem.part[w][u0 >> 6] = m;
       }
-      auto first = [&](int gr) { return next.of<T, DP>(gr); };
-      next_missing = src.missing(first);
-      const uint32_t to = kv0 + (uint32_t)((s & 1) * 2 * R::kBytes);
-      src.load(to, to + R::kBytes, w, first);
-    };
-    prepare(0);
-    for (int s = 0; s < steps; ++s) {
-      const Halves now = next;
-      const int slot[2] = {next_slot[0], next_slot[1]};
-      const uint32_t missing = next_missing;
-      wait_loads<0>();
-      wait_reads();
-      barrier();  // the step's rows are there, and nobody reads the other slot any more
-      if (s + 1 < steps) prepare(s + 1);
-      uint32_t sel = 0;
-      bool edge = missing != 0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t bits = mem.mask[slot[h] * words + (row.token >> 5)];
-        const bool in = (now.first[h] >= 0) & row.in & (((bits >> (row.token & 31)) & 1u) != 0u);
-        sel |= in ? 1u << h : 0u;
-        // keys behind a row's own position
-        edge |= in & (now.first[h] + kHalf - 1 > row.pos);
-      }
-      if (__ballot(sel != 0u) == 0) continue;
-      const bool some = __ballot(sel != 3u) != 0;  // not all
-      const uint32_t kb = kv0 + (uint32_t)((s & 1) * 2 * R::kBytes);
-      body(now, sel, some, __ballot(edge) != 0, missing, kb, kb + R::kBytes);
     }
-    wait_loads<0>();
+    __syncthreads();
+
+    // the halves of step ss of unit u
+    auto halves_of = [&](int u, int ss, int (&slot)[2]) {
+      Halves o;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int e = pairs ? 2 * u + h : u;
+        slot[h] = h == 1 && !pairs ? slot[0] : alike((int)mem.list[e < count ? e : 0]);
+        o.first[h] = e < count ? ((w0 + slot[h]) << lg_block) + (pairs ? 0 : (2 * ss + h) * kHalf) : -1;
+      }
+      return o;
+    };
+
+    const uint32_t steps = (uint32_t)units << lg_steps;
+    if constexpr (LOADS) {
+      constexpr uint32_t PAIRS = Shape::kPairs, OWN = S / PAIRS;  // slots of this pair
+      const int which = (w - READERS) & 1;                        // 0: keys, 1: values
+      const uint32_t pair = (uint32_t)(w - READERS) >> 1;
+      KeySource<T, DP> src;
+      src.init(p, which ? p.v : p.k, t.sq, t.seq, t.head, lane);
+      // a block's rows are one behind the other in packed rows and in a page that holds it
+      const bool together = !pairs && (src.table == nullptr || src.shift >= lg_block);
+      const uint32_t ready = ready0 + 4 * (uint32_t)(which * S);
+      uint32_t step = base + (pair + PAIRS - base % PAIRS) % PAIRS, told = step;
+      auto announce = [&] {  // the first step under way
+        if (step - told == PAIRS) wait_loads<0>();
+        else wait_loads<kLoads>();
+        if (lane == 0) tell(ready + 4 * (told % S), told + 1);
+        told += PAIRS;
+      };
+      uint32_t readers = 0;             // of 64 units, a lane each
+      uint32_t at_lo = 0, at_hi = 0;    // their blocks' first bytes
+      int first = 0, chunk = -1;        // their first keys
+      uint64_t here = 0;                // those whose page is in the cache
+      for (; step - base < steps; step += PAIRS) {
+        const uint32_t x = step - base;
+        const int u = (int)(x >> lg_steps), ss = (int)(x & ((1u << lg_steps) - 1u)), uu = u & 63;
+        if (u >> 6 != chunk) {
+          chunk = u >> 6;
+          readers = 0;
+#pragma unroll
+          for (int r = 0; r < READERS; ++r) readers += (uint32_t)(mem.part[r][chunk] >> lane) & 1u;
+          const int mine = chunk * 64 + lane;
+          first = mine < units ? (w0 + (int)mem.list[pairs ? 0 : mine]) << lg_block : 0;
+          int64_t page = 0;
+          if (together && src.table != nullptr) {
+            const int nth = first >> src.shift;
+            page = nth < src.per_seq ? p.seqs.pages[(int64_t)t.seq * p.seqs.ld_pages + nth] : -1;
+            if (page >= src.n_pages) page = -1;
+          }
+          const uint64_t bytes = (uint64_t)(uintptr_t)src.rows_at(page < 0 ? 0 : page, first);
+          at_lo = (uint32_t)bytes;
+          at_hi = (uint32_t)(bytes >> 32);
+          here = __ballot(page >= 0);
+        }
+        typename KeySource<T, DP>::Place place;
+        const int j = __builtin_amdgcn_readlane(first, uu) + ss * R::kKeys;
+        place.missing = 0;
+        place.whole = together && j + R::kKeys <= src.keys && ((here >> uu) & 1u);
+        if (place.whole) {
+          const uint64_t bytes = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_hi, uu) << 32 |
+                                 (uint32_t)__builtin_amdgcn_readlane((int)at_lo, uu);
+          place.at[0] = (const char*)(uintptr_t)(bytes + (uint64_t)((uint32_t)(ss * R::kKeys)) * src.row);
+        } else {
+          int slot[2];
+          src.find(halves_of(u, ss, slot), place);
+        }
+        const uint32_t i = step % S, own = i / PAIRS;
+        uint32_t want = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < OWN; ++k)
+          if (k == own) want = expected[k];
+        while (look(done0 + 4 * i) != want) {
+          if (told != step) announce();
+          else __builtin_amdgcn_s_sleep(1);
+        }
+        in_order();
+        if (which == 0 && lane == 0) tell(missing0 + 4 * i, place.missing);
+        src.load(kv0 + (2 * i + (uint32_t)which) * Shape::kBytes, place, lane);
+        const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)readers, uu);
+#pragma unroll
+        for (uint32_t k = 0; k < OWN; ++k)
+          if (k == own) expected[k] += n;
+        // two steps under way
+        if (step - told == PAIRS) {
+          step += PAIRS;
+          announce();
+          step -= PAIRS;
+        }
+      }
+      while (told != step) announce();
+    } else {
+      // (a wave of one token takes part with all its rows)
+      const bool alone = t_lo == t_hi && !pairs;
+      for (int u0 = 0; u0 < units; u0 += 64) {
+        uint64_t left = mem.part[w][u0 >> 6];
+        left = (uint64_t)(uint32_t)alike((int)(uint32_t)left) | (uint64_t)(uint32_t)alike((int)(uint32_t)(left >> 32)) << 32;
+        const int mine = u0 + lane < units ? (int)mem.list[pairs ? 0 : u0 + lane] : 0;  // 64 units' blocks
+        for (; left != 0; left &= left - 1) {
+          const int uu = __builtin_ctzll(left), u = u0 + uu;
+          for (int ss = 0; ss < 1 << lg_steps; ++ss) {
+            Halves now;
+            int slot[2];
+            if (pairs) {
+              now = halves_of(u, ss, slot);
+            } else {
+              slot[0] = slot[1] = __builtin_amdgcn_readlane(mine, uu);
+              now.first[0] = ((w0 + slot[0]) << lg_block) + 2 * ss * kHalf;
+              now.first[1] = now.first[0] + kHalf;
+            }
+            uint32_t sel = 0;
+            bool edge = false;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              bool in = row.in;
+              if (!alone) {
+                const uint32_t bits = mem.mask[slot[h] * words + (row.token >> 5)];
+                in = (now.first[h] >= 0) & row.in & (((bits >> (row.token & 31)) & 1u) != 0u);
+              }
+              sel |= in ? 1u << h : 0u;
+              // keys behind a row's own position
+              edge |= in & (now.first[h] + kHalf - 1 > row.pos);
+            }
+            const bool some = __ballot(sel != 3u) != 0;  // not all
+            const uint32_t step = base + ((uint32_t)u << lg_steps) + (uint32_t)ss;
+            const uint32_t i = step % S;
+            while (look(ready0 + 4 * i) != step + 1) __builtin_amdgcn_s_sleep(1);
+            in_order();
+            const uint32_t missing = p.seqs.pages != nullptr ? look(missing0 + 4 * i) : 0u;
+            body(now, sel, some, __ballot(edge) != 0 || missing != 0, missing, kv0 + 2 * i * Shape::kBytes,
+                 kv0 + (2 * i + 1) * Shape::kBytes, [&] {
+                   while (look(ready0 + 4 * (S + i)) != step + 1) __builtin_amdgcn_s_sleep(1);
+                   in_order();
+                 });
+            wait_reads();
+            if (lane == 0)
+              __hip_atomic_fetch_add((lds_word*)(uintptr_t)(done0 + 4 * i), 1u, __ATOMIC_RELAXED,
+                                     __HIP_MEMORY_SCOPE_WORKGROUP);
+          }
+        }
+      }
+    }
+    base += steps;
   }
+}
+
+template <class T, int DP, class Shape>
+__device__ inline void walk_loads(const BlockArgs& p, const WalkTile& t, typename Shape::Memory& mem, uint32_t kv0,
+                                  int tid, int w, int lane) {
+  walk_blocks<T, DP, Shape, true>(p, t, RowOf{}, mem, kv0, tid, w, lane, [] {});
 }
 
 }  // namespace

@@ -61,6 +61,13 @@ __device__ inline void lds_dma(uint32_t lds, uint32_t offset, u32x4 rsrc) {
                  "s"(rsrc)
                  : "memory");
 }
+// 16 bytes a lane, from base + offset + shift (a scalar, in bytes, not part of what is
+// compared with the buffer's end).
+__device__ inline void lds_dma_shifted(uint32_t lds, uint32_t offset, u32x4 rsrc, uint32_t shift) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset),
+               "s"(rsrc), "s"(shift)
+               : "memory");
+}
 // The same from an address a lane.
 __device__ inline void lds_dma_at(uint32_t lds, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
