@@ -32,7 +32,7 @@ constexpr float kSlack = 8.0f;
 
 // One step's keys and values.
 template <class T, int DP, int AHEAD, class Wait>
-__device__ inline void attend(Online<T, DP>& st, uint32_t kb, uint32_t vb, uint32_t sel, const Halves& now, bool some,
+__device__ inline void attend(Online<T, DP>& st, uint32_t kb, uint32_t vb, bool sel, int now, bool some,
                               bool edge, uint32_t missing, const RowOf& row, float c, int lane, Wait values) {
   using R = Rows<T, DP>;
   constexpr int G = R::kGroups, P = R::kUnit / 16;
@@ -46,18 +46,16 @@ __device__ inline void attend(Online<T, DP>& st, uint32_t kb, uint32_t vb, uint3
   if (edge) {
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) {
-      const int last = (missing >> gr) & 1u ? -1 : row.pos - now.of<T, DP>(gr) - 4 * (lane >> 4);
+      const int last = (missing >> gr) & 1u ? -1 : row.pos - now - 16 * gr - 4 * (lane >> 4);
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[gr][r] = r <= last ? s[gr][r] : -INFINITY;
     }
   }
   if (some) {
 #pragma unroll
-    for (int gr = 0; gr < G; ++gr) {
-      const bool in = (sel >> (gr / (G / 2))) & 1u;
+    for (int gr = 0; gr < G; ++gr)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s[gr][r] = in ? s[gr][r] : -INFINITY;
-    }
+      for (int r = 0; r < 4; ++r) s[gr][r] = sel ? s[gr][r] : -INFINITY;
   }
   float most = -INFINITY;
 #pragma unroll
@@ -161,7 +159,7 @@ __device__ __forceinline__ void careful_row(const BlockArgs& p, const Sequence& 
 constexpr int many_readers(int row) { return row <= 256 ? 12 : 6; }
 template <class T, int DP>
 struct ManyShape : WalkShape<T, DP, many_readers(DP * (int)sizeof(T)), (DP * sizeof(T) > 256 ? 1 : 2)> {
-  static constexpr int kAhead = DP * sizeof(T) == 256 ? 4 : 8;
+  static constexpr int kAhead = 8;
 };
 
 template <class T, int DP>
@@ -185,7 +183,7 @@ __global__ __launch_bounds__((ManyShape<T, DP>::kThreads)) void block_attention_
                   row.in, p.width, lane, st.q);
   const float c = p.scale * kLog2e;
   walk_blocks<T, DP, Shape, false>(p, t, row, mem, lds_address(&mem), tid, w, lane,
-                            [&](const Halves& now, uint32_t sel, bool some, bool edge, uint32_t missing, uint32_t kb,
+                            [&](int now, bool sel, bool some, bool edge, uint32_t missing, uint32_t kb,
                                 uint32_t vb, auto values) {
                               attend<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, missing, row, c, lane, values);
                             });
@@ -221,11 +219,11 @@ __global__ __launch_bounds__((64 * ManyShape<T, DP>::kReaders)) void block_atten
 // its waves the steps of the token's own blocks in turn, each with keys and values of
 // its own in LDS; their states are joined at the end, with `splits` workgroups a
 // token those by the next kernel.
-constexpr int kFewWaves = 4;
+constexpr int kFewWaves = 8;
 
 template <class T, int DP>
 struct FewShape {
-  static constexpr int kWaves = DP * (int)sizeof(T) > 256 ? 2 : kFewWaves;
+  static constexpr int kWaves = DP * (int)sizeof(T) > 256 ? kFewWaves / 2 : kFewWaves;
 };
 // (floats of a split's part: maximum and sum of 16 rows, then the rows)
 template <int DP>
@@ -372,26 +370,15 @@ __global__ __launch_bounds__((64 * FewShape<T, DP>::kWaves)) void block_attentio
   load_row<T, DP>(static_cast<const T*>(p.q) + f.token * p.q_token + (int64_t)(f.head * p.group + row.head) * p.q_head,
                   row.in, p.width, lane, st.q);
   __syncthreads();
-  constexpr int kHalf = R::kKeys / 2;
-  const int lg_halves = lg - (kHalf == 32 ? 5 : 4);
-  const int count = alike(s_count), steps = ((count << lg_halves) + 1) / 2;
+  const int lg_steps = lg - 5, steps = alike(s_count) << lg_steps;
   const float c = p.scale * kLog2e;
   const uint32_t kb = lds_address(s_kv[w][0]), vb = lds_address(s_kv[w][1]);
   KeySource<T, DP> keys, values;
   keys.init(p, p.k, sq, seq, f.head, lane);
   values.init(p, p.v, sq, seq, f.head, lane);
   for (int s = f.split * WAVES + w; s < steps; s += WAVES * p.splits) {
-    Halves now;
-    uint32_t sel = 0;
-    bool edge = false;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = 2 * s + h, e = at >> lg_halves;
-      const int id = alike(e < count ? s_ids[e] : -1);
-      now.first[h] = id >= 0 ? (id << lg) + (at & ((1 << lg_halves) - 1)) * kHalf : -1;
-      sel |= now.first[h] >= 0 && row.in ? 1u << h : 0u;
-      edge |= now.first[h] + kHalf - 1 > pos;
-    }
+    const int now = (alike(s_ids[s >> lg_steps]) << lg) + (s & ((1 << lg_steps) - 1)) * R::kKeys;
+    const bool edge = now + R::kKeys - 1 > pos;
     typename KeySource<T, DP>::Place k_place, v_place;
     keys.find(now, k_place);
     values.find(now, v_place);
@@ -399,7 +386,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP>::kWaves)) void block_attentio
     keys.load(kb, k_place, lane);
     values.load(vb, v_place, lane);
     wait_loads<KeySource<T, DP>::kLoads>();
-    attend<T, DP, 16>(st, kb, vb, sel, now, true, edge || k_place.missing != 0, k_place.missing, row, c, lane,
+    attend<T, DP, 8>(st, kb, vb, row.in, now, true, edge || k_place.missing != 0, k_place.missing, row, c, lane,
                   [] { wait_loads<0>(); });
   }
   wait_reads();
@@ -477,8 +464,8 @@ Plan plan_of(int val_t, const fs_block_seqs& s, int heads, int group, int width,
   o.splits = 1;
   if (o.few) {
     const int bytes = (width <= 64 ? 64 : width <= 128 ? 128 : 256) * (val_t == FS_F32 ? 4 : 2);
-    const int waves = bytes > 256 ? 2 : kFewWaves, keys = val_t == FS_F32 ? 32 : 64;
-    const int64_t steps = ceil_div((int64_t)top * block, keys);
+    const int waves = bytes > 256 ? kFewWaves / 2 : kFewWaves;
+    const int64_t steps = (int64_t)top * block / 32;
     // until a wave has one step, or there are two workgroups a compute unit
     while ((int64_t)o.splits * waves < steps && o.groups * o.splits < 512 && o.splits < 64) o.splits *= 2;
     if (o.splits > 1)

@@ -73,7 +73,7 @@ struct QueryGrad {
 };
 
 template <class T, int DP, int AHEAD, class Wait>
-__device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, uint32_t sel, const Halves& now, bool some,
+__device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, bool sel, int now, bool some,
                             bool edge, const RowOf& row, float c, float factor, int lane, Wait values) {
   using R = Rows<T, DP>;
   constexpr int G = R::kGroups, P = R::kUnit / 16;
@@ -95,18 +95,16 @@ __device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, uint
   if (edge) {
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) {
-      const int last = row.pos - now.of<T, DP>(gr) - 4 * (lane >> 4);
+      const int last = row.pos - now - 16 * gr - 4 * (lane >> 4);
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[gr][r] = r <= last ? s[gr][r] : 0.0f;
     }
   }
   if (some) {
 #pragma unroll
-    for (int gr = 0; gr < G; ++gr) {
-      const bool in = (sel >> (gr / (G / 2))) & 1u;
+    for (int gr = 0; gr < G; ++gr)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s[gr][r] = in ? s[gr][r] : 0.0f;
-    }
+      for (int r = 0; r < 4; ++r) s[gr][r] = sel ? s[gr][r] : 0.0f;
   }
   // (dS in the values' type, rounded once)
   typename R::frag w[G / P];
@@ -227,7 +225,7 @@ __global__ __launch_bounds__((QueryGradShape<T, DP>::kThreads)) void block_query
   for (int dt = 0; dt < DP / 16; ++dt) st.d[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   const float c = p.scale * kLog2e;
   walk_blocks<T, DP, Shape, false>(p, t, row, mem, lds_address(&mem), tid, w, lane,
-                            [&](const Halves& now, uint32_t sel, bool some, bool edge, uint32_t, uint32_t kb, uint32_t vb,
+                            [&](int now, bool sel, bool some, bool edge, uint32_t, uint32_t kb, uint32_t vb,
                                 auto values) { take<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, row, c, factor, lane, values); });
   bool bad = false;
 #pragma unroll

@@ -128,7 +128,7 @@ struct Rows {
   static constexpr int kRow = DP * (int)sizeof(T);  // bytes: 128, 256 or 512
   static constexpr int kPieces = kRow / 16;
   static constexpr int kUnit = sizeof(T) == 2 ? 32 : 16;  // rows that one product over rows takes
-  static constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;  // keys a step
+  static constexpr int kKeys = 32;                         // keys a step
   static constexpr int kGroups = kKeys / 16;
   static constexpr int kBytes = kKeys * kRow;
   static constexpr int kFrags = kRow / 64;     // fragments of 16 rows
@@ -286,18 +286,6 @@ struct BlockArgs {
   float* parts;
 };
 
-// A step's two halves: the position of each one's first key (negative: none).
-struct Halves {
-  int first[2];
-  template <class T, int DP>
-  __device__ int of(int group) const {
-    constexpr int kHalf = Rows<T, DP>::kGroups / 2;
-    const bool second = group >= kHalf;
-    const int f = second ? first[1] : first[0];
-    return f < 0 ? -1 : f + (group - (second ? kHalf : 0)) * 16;
-  }
-};
-
 // Keys, or values, of one sequence and head, and a wave's loads of a step of them.
 template <class T, int DP>
 struct KeySource {
@@ -331,39 +319,38 @@ struct KeySource {
     }
   }
   // Where a step lies.  `whole`: all its rows are keys and one behind the other, from
-  // first.at[0] on; otherwise the first byte of each group of 16 keys, and how many of
-  // its rows are keys.  Bits of the groups whose page is outside the cache.
+  // at[0] on; otherwise the first byte of each group of 16 keys, and how many of its rows
+  // are keys.  Bits of the groups whose page is outside the cache.
   struct Place {
     const char* at[kGroups];
     int left[kGroups];
     uint32_t missing;
     bool whole;
   };
-  // The step whose rows are keys j .. j + kKeys - 1 of the page `id` (without pages: 0).
+  // Key j on, of the page `id` (without pages: any).
   __device__ const char* rows_at(int64_t id, int j) const {
     return table == nullptr ? base + (int64_t)j * row : base + id * page + (int64_t)(j & ((1 << shift) - 1)) * row;
   }
-  __device__ void find(const Halves& h, Place& o) const {
+  __device__ void find(int first, Place& o) const {
     o.missing = 0;
     o.whole = false;
 #pragma unroll
     for (int gr = 0; gr < kGroups; ++gr) {
-      const int j = h.of<T, DP>(gr);
+      const int j = first + gr * 16;
       o.at[gr] = base;
       o.left[gr] = 0;
-      if (j >= 0 && j < keys) {
-        if (table == nullptr) {
-          o.at[gr] = base + (int64_t)j * row;
+      if (j < keys) {
+        int64_t id = 0;
+        if (table != nullptr) {
+          const int t = j >> shift;
+          id = t < per_seq ? table[t] : -1;
+          if (id >= n_pages) id = -1;
+        }
+        if (id >= 0) {
+          o.at[gr] = rows_at(id, j);
           o.left[gr] = keys - j;
         } else {
-          const int t = j >> shift;
-          const int64_t id = t < per_seq ? table[t] : -1;
-          if (id >= 0 && id < n_pages) {
-            o.at[gr] = rows_at(id, j);
-            o.left[gr] = keys - j;
-          } else {
-            o.missing |= 1u << gr;
-          }
+          o.missing |= 1u << gr;
         }
       }
     }

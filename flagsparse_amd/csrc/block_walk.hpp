@@ -34,12 +34,12 @@ template <class T, int DP, int READERS, int PAIRS>
 struct WalkShape {
   static constexpr int kReaders = READERS, kPairs = PAIRS, kWaves = READERS + 2 * PAIRS, kThreads = 64 * kWaves;
   static constexpr int kBytes = Rows<T, DP>::kBytes;
-  static constexpr int kSlots = kBytes > 16384 ? 2 : 4;
+  static constexpr int kSlots = kBytes > 8192 ? 4 : 8;
   static_assert(kSlots % PAIRS == 0, "a slot is one pair's");
   struct alignas(1024) Memory {
     uint8_t kv[kSlots][2][kBytes];  // (first: kv0 in what follows is its address)
     uint32_t mask[kMaskWords];
-    uint64_t part[READERS][kMaskWords / 64];  // units that a wave takes part in
+    uint64_t part[READERS][kMaskWords / 64];  // listed blocks that a wave takes part in
     uint16_t list[kMaskWords];
     uint32_t total[kWaves];
     uint32_t ready[2][kSlots];  // 1 + the step that a slot holds; of the keys, of the values
@@ -102,13 +102,9 @@ template <class T, int DP, class Shape, bool LOADS, class Body>
 __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const RowOf& row, typename Shape::Memory& mem,
                                    uint32_t kv0, int tid, int w, int lane, Body body) {
   using R = Rows<T, DP>;
-  constexpr int THREADS = Shape::kThreads, READERS = Shape::kReaders, S = Shape::kSlots, kHalf = R::kKeys / 2;
+  constexpr int THREADS = Shape::kThreads, READERS = Shape::kReaders, S = Shape::kSlots;
   constexpr int kLoads = KeySource<T, DP>::kLoads;
-  const int lg_block = p.lg_groups + 4;
-  const int lg_halves = lg_block - (kHalf == 32 ? 5 : 4);  // of a block's halves of a step
-  // a unit: a block, or two of half a step
-  const bool pairs = lg_halves == 0;
-  const int lg_steps = pairs ? 0 : lg_halves - 1;  // of a unit
+  const int lg_block = p.lg_groups + 4, lg_steps = lg_block - 5;  // of a block
   const int words = (p.per + 31) / 32, window = kMaskWords / words;
   const int last = t.pos0 + t.tokens - 1;
   const int n_blocks = last < 0 ? 0 : (last >> lg_block) + 1;
@@ -165,17 +161,13 @@ __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const 
     for (int i = 0; i < each; ++i)
       if (named(tid * each + i)) mem.list[at++] = (uint16_t)(tid * each + i);
     __syncthreads();
-    const int units = pairs ? (count + 1) / 2 : count;
     if constexpr (!LOADS) {
-      for (int u0 = 0; u0 < units; u0 += 64) {
+      for (int u0 = 0; u0 < count; u0 += 64) {
         uint32_t any = 0;
-        for (int h = 0; h < (pairs ? 2 : 1); ++h) {
-          const int e = pairs ? 2 * (u0 + lane) + h : u0 + lane;
-          if (e < count) {
-            const uint32_t* m = &mem.mask[mem.list[e] * words];
-            if (word_lo < words) any |= m[word_lo] & bits_lo;
-            if (word_hi < words) any |= m[word_hi] & bits_hi;
-          }
+        if (u0 + lane < count) {
+          const uint32_t* m = &mem.mask[mem.list[u0 + lane] * words];
+          if (word_lo < words) any |= m[word_lo] & bits_lo;
+          if (word_hi < words) any |= m[word_hi] & bits_hi;
         }
         const uint64_t m = __ballot(any != 0);
         if (lane == 0) mem.part[w][u0 >> 6] = m;
@@ -183,36 +175,26 @@ __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const 
     }
     __syncthreads();
 
-    // the halves of step ss of unit u
-    auto halves_of = [&](int u, int ss, int (&slot)[2]) {
-      Halves o;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int e = pairs ? 2 * u + h : u;
-        slot[h] = h == 1 && !pairs ? slot[0] : alike((int)mem.list[e < count ? e : 0]);
-        o.first[h] = e < count ? ((w0 + slot[h]) << lg_block) + (pairs ? 0 : (2 * ss + h) * kHalf) : -1;
-      }
-      return o;
-    };
-
-    const uint32_t steps = (uint32_t)units << lg_steps;
+    const uint32_t steps = (uint32_t)count << lg_steps;
     if constexpr (LOADS) {
       constexpr uint32_t PAIRS = Shape::kPairs, OWN = S / PAIRS;  // slots of this pair
+      constexpr uint32_t DEEP = OWN < 3 ? 2 : 3;                  // steps under way
       const int which = (w - READERS) & 1;                        // 0: keys, 1: values
       const uint32_t pair = (uint32_t)(w - READERS) >> 1;
       KeySource<T, DP> src;
       src.init(p, which ? p.v : p.k, t.sq, t.seq, t.head, lane);
       // a block's rows are one behind the other in packed rows and in a page that holds it
-      const bool together = !pairs && (src.table == nullptr || src.shift >= lg_block);
+      const bool together = src.table == nullptr || src.shift >= lg_block;
       const uint32_t ready = ready0 + 4 * (uint32_t)(which * S);
       uint32_t step = base + (pair + PAIRS - base % PAIRS) % PAIRS, told = step;
-      auto announce = [&] {  // the first step under way
-        if (step - told == PAIRS) wait_loads<0>();
-        else wait_loads<kLoads>();
+      auto announce = [&](uint32_t end) {  // the first step under way, of those before `end`
+        if (end - told == PAIRS) wait_loads<0>();
+        else if (DEEP == 2 || end - told == 2 * PAIRS) wait_loads<kLoads>();
+        else wait_loads<DEEP == 2 ? 0 : 2 * kLoads>();
         if (lane == 0) tell(ready + 4 * (told % S), told + 1);
         told += PAIRS;
       };
-      uint32_t readers = 0;             // of 64 units, a lane each
+      uint32_t readers = 0;             // of 64 blocks, a lane each
       uint32_t at_lo = 0, at_hi = 0;    // their blocks' first bytes
       int first = 0, chunk = -1;        // their first keys
       uint64_t here = 0;                // those whose page is in the cache
@@ -225,7 +207,7 @@ __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const 
 #pragma unroll
           for (int r = 0; r < READERS; ++r) readers += (uint32_t)(mem.part[r][chunk] >> lane) & 1u;
           const int mine = chunk * 64 + lane;
-          first = mine < units ? (w0 + (int)mem.list[pairs ? 0 : mine]) << lg_block : 0;
+          first = mine < count ? (w0 + (int)mem.list[mine]) << lg_block : 0;
           int64_t page = 0;
           if (together && src.table != nullptr) {
             const int nth = first >> src.shift;
@@ -246,8 +228,7 @@ __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const 
                                  (uint32_t)__builtin_amdgcn_readlane((int)at_lo, uu);
           place.at[0] = (const char*)(uintptr_t)(bytes + (uint64_t)((uint32_t)(ss * R::kKeys)) * src.row);
         } else {
-          int slot[2];
-          src.find(halves_of(u, ss, slot), place);
+          src.find(j, place);
         }
         const uint32_t i = step % S, own = i / PAIRS;
         uint32_t want = 0;
@@ -255,7 +236,7 @@ __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const 
         for (uint32_t k = 0; k < OWN; ++k)
           if (k == own) want = expected[k];
         while (look(done0 + 4 * i) != want) {
-          if (told != step) announce();
+          if (told != step) announce(step);
           else __builtin_amdgcn_s_sleep(1);
         }
         in_order();
@@ -265,53 +246,30 @@ __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const 
 #pragma unroll
         for (uint32_t k = 0; k < OWN; ++k)
           if (k == own) expected[k] += n;
-        // two steps under way
-        if (step - told == PAIRS) {
-          step += PAIRS;
-          announce();
-          step -= PAIRS;
-        }
+        if (step + PAIRS - told == DEEP * PAIRS) announce(step + PAIRS);
       }
-      while (told != step) announce();
+      while (told != step) announce(step);
     } else {
       // (a wave of one token takes part with all its rows)
-      const bool alone = t_lo == t_hi && !pairs;
-      for (int u0 = 0; u0 < units; u0 += 64) {
+      const bool alone = t_lo == t_hi;
+      for (int u0 = 0; u0 < count; u0 += 64) {
         uint64_t left = mem.part[w][u0 >> 6];
         left = (uint64_t)(uint32_t)alike((int)(uint32_t)left) | (uint64_t)(uint32_t)alike((int)(uint32_t)(left >> 32)) << 32;
-        const int mine = u0 + lane < units ? (int)mem.list[pairs ? 0 : u0 + lane] : 0;  // 64 units' blocks
+        const int mine = u0 + lane < count ? (int)mem.list[u0 + lane] : 0;  // 64 blocks
         for (; left != 0; left &= left - 1) {
-          const int uu = __builtin_ctzll(left), u = u0 + uu;
+          const int uu = __builtin_ctzll(left), u = u0 + uu, nth = __builtin_amdgcn_readlane(mine, uu);
+          bool sel = row.in;
+          if (!alone) sel &= ((mem.mask[nth * words + (row.token >> 5)] >> (row.token & 31)) & 1u) != 0u;
+          const bool some = __ballot(sel) != ~0ull;  // not all
           for (int ss = 0; ss < 1 << lg_steps; ++ss) {
-            Halves now;
-            int slot[2];
-            if (pairs) {
-              now = halves_of(u, ss, slot);
-            } else {
-              slot[0] = slot[1] = __builtin_amdgcn_readlane(mine, uu);
-              now.first[0] = ((w0 + slot[0]) << lg_block) + 2 * ss * kHalf;
-              now.first[1] = now.first[0] + kHalf;
-            }
-            uint32_t sel = 0;
-            bool edge = false;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              bool in = row.in;
-              if (!alone) {
-                const uint32_t bits = mem.mask[slot[h] * words + (row.token >> 5)];
-                in = (now.first[h] >= 0) & row.in & (((bits >> (row.token & 31)) & 1u) != 0u);
-              }
-              sel |= in ? 1u << h : 0u;
-              // keys behind a row's own position
-              edge |= in & (now.first[h] + kHalf - 1 > row.pos);
-            }
-            const bool some = __ballot(sel != 3u) != 0;  // not all
+            const int now = ((w0 + nth) << lg_block) + ss * R::kKeys;
+            const bool edge = __ballot(sel & (now + R::kKeys - 1 > row.pos)) != 0;  // keys behind a row's position
             const uint32_t step = base + ((uint32_t)u << lg_steps) + (uint32_t)ss;
             const uint32_t i = step % S;
             while (look(ready0 + 4 * i) != step + 1) __builtin_amdgcn_s_sleep(1);
             in_order();
             const uint32_t missing = p.seqs.pages != nullptr ? look(missing0 + 4 * i) : 0u;
-            body(now, sel, some, __ballot(edge) != 0 || missing != 0, missing, kv0 + 2 * i * Shape::kBytes,
+            body(now, sel, some, edge || missing != 0, missing, kv0 + 2 * i * Shape::kBytes,
                  kv0 + (2 * i + 1) * Shape::kBytes, [&] {
                    while (look(ready0 + 4 * (S + i)) != step + 1) __builtin_amdgcn_s_sleep(1);
                    in_order();
