@@ -158,7 +158,7 @@ __device__ __forceinline__ void careful_row(const BlockArgs& p, const Sequence& 
 // Waves that read, by the bytes of a row.
 constexpr int many_readers(int row) { return row <= 256 ? 12 : 6; }
 template <class T, int DP>
-struct ManyShape : WalkShape<T, DP, many_readers(DP * (int)sizeof(T)), (DP * sizeof(T) > 256 ? 1 : 2)> {
+struct ManyShape : WalkShape<T, DP, many_readers(DP * (int)sizeof(T)), (DP * sizeof(T) > 256 ? 2 : 4)> {
   static constexpr int kAhead = 8;
 };
 

@@ -182,7 +182,7 @@ __device__ __forceinline__ void careful_query(const GradArgs& a, const Sequence&
 }
 
 template <class T, int DP>
-struct QueryGradShape : WalkShape<T, DP, query_readers(DP * (int)sizeof(T)), (DP * sizeof(T) > 256 ? 1 : 2)> {
+struct QueryGradShape : WalkShape<T, DP, query_readers(DP * (int)sizeof(T)), (DP * sizeof(T) > 256 ? 2 : 4)> {
   static constexpr int kAhead = 8;
 };
 

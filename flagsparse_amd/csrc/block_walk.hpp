@@ -9,15 +9,16 @@
 // workgroup, and a wave takes part where one of its tokens selects the block.
 //
 // Which waves take part differs from block to block, so the waves do not meet at a
-// barrier: some waves load, in pairs, one the keys and one the values of a step, into a
-// ring of slots, the pairs in turn, and the others follow each at its own pace.  A
-// loader says in LDS which step a slot holds; a wave that has read it adds one to the
-// slot's count, and a slot is loaded again when all that take part have.  Every wait
-// ends: each wave goes through its steps in order; the first step that is not yet read
-// by all waits for its loaders alone, who wait for the readers of the step that had its
-// slot before, an earlier one; and a loader that waits has announced what it has loaded.
-// A loader is one wave, which issues an instruction in four or five cycles: what it
-// needs is laid out 64 blocks at a time, a lane each.
+// barrier: some waves load, a step each in turn, into a ring of slots, and the others
+// follow each at its own pace.  A loader says in LDS which step a slot holds; a wave that
+// has read it adds one to the slot's count, and a slot is loaded again when all that take
+// part have.  Every wait ends: each wave goes through its steps in order, and the first
+// step that is not yet read by all waits for its loader alone, which waits for the
+// readers of the step that had its slot before, an earlier one.
+// A loader is one wave, which issues an instruction in some cycles: what it needs is laid
+// out 64 blocks at a time, a lane each.  It announces a step before it goes on to its
+// next: us with one, two and three steps of a loader under way, 16384 tokens of 4 x 16
+// heads 1778, 1827, 1870, chunks of 4 x 512 tokens 428, 442, 458.
 #pragma once
 
 #include <cstddef>
@@ -29,13 +30,13 @@ namespace {
 
 constexpr int kMaskWords = 2048;
 
-// Waves that read, pairs that load, and slots by what LDS holds.
-template <class T, int DP, int READERS, int PAIRS>
+// Waves that read and that load, and slots by what LDS holds.
+template <class T, int DP, int READERS, int LOADERS>
 struct WalkShape {
-  static constexpr int kReaders = READERS, kPairs = PAIRS, kWaves = READERS + 2 * PAIRS, kThreads = 64 * kWaves;
+  static constexpr int kReaders = READERS, kLoaders = LOADERS, kWaves = READERS + LOADERS, kThreads = 64 * kWaves;
   static constexpr int kBytes = Rows<T, DP>::kBytes;
   static constexpr int kSlots = kBytes > 8192 ? 4 : 8;
-  static_assert(kSlots % PAIRS == 0, "a slot is one pair's");
+  static_assert(kSlots % LOADERS == 0, "a slot is one loader's");
   struct alignas(1024) Memory {
     uint8_t kv[kSlots][2][kBytes];  // (first: kv0 in what follows is its address)
     uint32_t mask[kMaskWords];
@@ -120,9 +121,9 @@ __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const 
   const uint32_t missing0 = kv0 + (uint32_t)offsetof(typename Shape::Memory, missing);
   const uint32_t done0 = kv0 + (uint32_t)offsetof(typename Shape::Memory, done);
   uint32_t base = 0;  // steps of the windows before
-  uint32_t expected[S / Shape::kPairs];  // readings of a loader's slots so far
+  uint32_t expected[S / Shape::kLoaders];  // readings of a loader's slots so far
 #pragma unroll
-  for (int i = 0; i < S / Shape::kPairs; ++i) expected[i] = 0u;
+  for (int i = 0; i < S / Shape::kLoaders; ++i) expected[i] = 0u;
 
   for (int w0 = 0; w0 < n_blocks; w0 += window) {
     __syncthreads();
@@ -177,29 +178,20 @@ __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const 
 
     const uint32_t steps = (uint32_t)count << lg_steps;
     if constexpr (LOADS) {
-      constexpr uint32_t PAIRS = Shape::kPairs, OWN = S / PAIRS;  // slots of this pair
-      constexpr uint32_t DEEP = OWN < 3 ? 2 : 3;                  // steps under way
-      const int which = (w - READERS) & 1;                        // 0: keys, 1: values
-      const uint32_t pair = (uint32_t)(w - READERS) >> 1;
-      KeySource<T, DP> src;
-      src.init(p, which ? p.v : p.k, t.sq, t.seq, t.head, lane);
+      constexpr uint32_t LOADERS = Shape::kLoaders, OWN = S / LOADERS;  // slots of this one
+      const uint32_t nth = (uint32_t)(w - READERS);
+      KeySource<T, DP> k, v;
+      k.init(p, p.k, t.sq, t.seq, t.head, lane);
+      v.init(p, p.v, t.sq, t.seq, t.head, lane);
       // a block's rows are one behind the other in packed rows and in a page that holds it
-      const bool together = src.table == nullptr || src.shift >= lg_block;
-      const uint32_t ready = ready0 + 4 * (uint32_t)(which * S);
-      uint32_t step = base + (pair + PAIRS - base % PAIRS) % PAIRS, told = step;
-      auto announce = [&](uint32_t end) {  // the first step under way, of those before `end`
-        if (end - told == PAIRS) wait_loads<0>();
-        else if (DEEP == 2 || end - told == 2 * PAIRS) wait_loads<kLoads>();
-        else wait_loads<DEEP == 2 ? 0 : 2 * kLoads>();
-        if (lane == 0) tell(ready + 4 * (told % S), told + 1);
-        told += PAIRS;
-      };
-      uint32_t readers = 0;             // of 64 blocks, a lane each
-      uint32_t at_lo = 0, at_hi = 0;    // their blocks' first bytes
-      int first = 0, chunk = -1;        // their first keys
-      uint64_t here = 0;                // those whose page is in the cache
-      for (; step - base < steps; step += PAIRS) {
-        const uint32_t x = step - base;
+      const bool together = k.table == nullptr || k.shift >= lg_block;
+      uint32_t readers = 0;  // of 64 blocks, a lane each
+      int first = 0;         // their first keys
+      uint64_t k_at = 0, v_at = 0;
+      uint64_t here = 0;     // those whose page is in the cache
+      int chunk = -1;
+      for (uint32_t x = (nth + LOADERS - base % LOADERS) % LOADERS; x < steps; x += LOADERS) {
+        const uint32_t step = base + x;
         const int u = (int)(x >> lg_steps), ss = (int)(x & ((1u << lg_steps) - 1u)), uu = u & 63;
         if (u >> 6 != chunk) {
           chunk = u >> 6;
@@ -209,46 +201,51 @@ __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const 
           const int mine = chunk * 64 + lane;
           first = mine < count ? (w0 + (int)mem.list[mine]) << lg_block : 0;
           int64_t page = 0;
-          if (together && src.table != nullptr) {
-            const int nth = first >> src.shift;
-            page = nth < src.per_seq ? p.seqs.pages[(int64_t)t.seq * p.seqs.ld_pages + nth] : -1;
-            if (page >= src.n_pages) page = -1;
+          if (together && k.table != nullptr) {
+            const int at = first >> k.shift;
+            page = at < k.per_seq ? p.seqs.pages[(int64_t)t.seq * p.seqs.ld_pages + at] : -1;
+            if (page >= k.n_pages) page = -1;
           }
-          const uint64_t bytes = (uint64_t)(uintptr_t)src.rows_at(page < 0 ? 0 : page, first);
-          at_lo = (uint32_t)bytes;
-          at_hi = (uint32_t)(bytes >> 32);
+          k_at = (uint64_t)(uintptr_t)k.rows_at(page < 0 ? 0 : page, first);
+          v_at = (uint64_t)(uintptr_t)v.rows_at(page < 0 ? 0 : page, first);
           here = __ballot(page >= 0);
         }
-        typename KeySource<T, DP>::Place place;
+        typename KeySource<T, DP>::Place k_place, v_place;
         const int j = __builtin_amdgcn_readlane(first, uu) + ss * R::kKeys;
-        place.missing = 0;
-        place.whole = together && j + R::kKeys <= src.keys && ((here >> uu) & 1u);
-        if (place.whole) {
-          const uint64_t bytes = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_hi, uu) << 32 |
-                                 (uint32_t)__builtin_amdgcn_readlane((int)at_lo, uu);
-          place.at[0] = (const char*)(uintptr_t)(bytes + (uint64_t)((uint32_t)(ss * R::kKeys)) * src.row);
+        k_place.missing = 0;
+        k_place.whole = v_place.whole = together && j + R::kKeys <= k.keys && ((here >> uu) & 1u);
+        if (k_place.whole) {
+          auto at = [&](uint64_t a, uint32_t row) {
+            const uint64_t bytes = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(a >> 32), uu) << 32 |
+                                   (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)a, uu);
+            return (const char*)(uintptr_t)(bytes + (uint64_t)((uint32_t)(ss * R::kKeys)) * row);
+          };
+          k_place.at[0] = at(k_at, k.row);
+          v_place.at[0] = at(v_at, v.row);
         } else {
-          src.find(j, place);
+          k.find(j, k_place);
+          v.find(j, v_place);
         }
-        const uint32_t i = step % S, own = i / PAIRS;
+        const uint32_t i = step % S, own = i / LOADERS;
         uint32_t want = 0;
 #pragma unroll
-        for (uint32_t k = 0; k < OWN; ++k)
-          if (k == own) want = expected[k];
-        while (look(done0 + 4 * i) != want) {
-          if (told != step) announce(step);
-          else __builtin_amdgcn_s_sleep(1);
-        }
+        for (uint32_t n = 0; n < OWN; ++n)
+          if (n == own) want = expected[n];
+        while (look(done0 + 4 * i) != want) __builtin_amdgcn_s_sleep(1);
         in_order();
-        if (which == 0 && lane == 0) tell(missing0 + 4 * i, place.missing);
-        src.load(kv0 + (2 * i + (uint32_t)which) * Shape::kBytes, place, lane);
-        const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)readers, uu);
+        if (lane == 0) tell(missing0 + 4 * i, k_place.missing);
+        const uint32_t to = kv0 + 2 * i * Shape::kBytes;
+        k.load(to, k_place, lane);
+        v.load(to + Shape::kBytes, v_place, lane);
+        const uint32_t n_readers = (uint32_t)__builtin_amdgcn_readlane((int)readers, uu);
 #pragma unroll
-        for (uint32_t k = 0; k < OWN; ++k)
-          if (k == own) expected[k] += n;
-        if (step + PAIRS - told == DEEP * PAIRS) announce(step + PAIRS);
+        for (uint32_t n = 0; n < OWN; ++n)
+          if (n == own) expected[n] += n_readers;
+        wait_loads<kLoads>();  // the keys' are done
+        if (lane == 0) tell(ready0 + 4 * i, step + 1);
+        wait_loads<0>();
+        if (lane == 0) tell(ready0 + 4 * (S + i), step + 1);
       }
-      while (told != step) announce(step);
     } else {
       // (a wave of one token takes part with all its rows)
       const bool alone = t_lo == t_hi;
