@@ -93,6 +93,22 @@ def test_select(sizes, dtype):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", BLOCK_DTYPES, ids=BLOCK_IDS)
+@pytest.mark.parametrize("sizes", [(4, 64, 64, 8, 1, 1), (16, 128, 32, 100, 3, 4), (1, 80, 64, 4, 1, 3)],
+                         ids=lambda c: "x".join(map(str, c)))
+def test_select_of_single_tokens(sizes, dtype):
+    """One query a sequence, without offsets: each wave takes a part of the blocks."""
+    group, width, block, top, first, recent = sizes
+    lengths = [0, 1, block * 3, 20011, 70000 if block == 64 else 9000, 640]
+    most = -(-max(lengths) // block)
+    q = randn((6, 2 * group, width), dtype, 3)
+    means = randn((6, most, 2, width), dtype, 4)
+    case = Case([1] * 6, lengths, 1, 1, 8, block, torch.float16, 5, page=64, single=True)
+    got = fs.flagsparse_block_select(q, means, case.seqs, top, first, recent)
+    seq, pos = list(range(6)), [n - 1 for n in lengths]
+    assert torch.equal(got, select_oracle(q, means, seq, pos, block, top, first, recent))
+
+
 def test_select_wide():
     case = Case([70], [4000], 1, 1, 8, 32, torch.float16, 5)
     for dtype in BLOCK_DTYPES[:2]:
@@ -105,7 +121,7 @@ def test_select_wide():
 @pytest.mark.parametrize("tokens", [1, 20])
 def test_select_ties_and_what_is_not_a_number(tokens):
     """Equal scores go to the lower block, both zeros are equal, NaN comes last."""
-    case = Case([tokens], [64 * 40], 1, 1, 8, 64, torch.float16, 6)
+    case = Case([tokens], [64 * 40], 1, 1, 8, 64, torch.float16, 6, single=tokens == 1)
     q = torch.ones((tokens, 1, 8), device="cuda")
     means = torch.zeros((1, 40, 1, 8), device="cuda")
     means[0, 5:20] = 1.0
