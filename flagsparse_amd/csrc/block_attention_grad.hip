@@ -373,13 +373,11 @@ __global__ __launch_bounds__(1024) void block_pieces_kernel(const int32_t* start
 
 // ---- gradients of keys and values -------------------------------------------------
 
-// KT tiles of 16 keys a wave, KW waves over the keys, RW over the rows.
+// 16 keys a wave, KW waves over the keys, RW over the rows.
 template <class T, int DP, int BK>
 struct KeyShape {
-  static constexpr bool kWide = DP * (int)sizeof(T) > 256;
-  static constexpr int KT = kWide ? 1 : 2;
-  static constexpr int KW = BK / (16 * KT);
-  static constexpr int RW = 4 / KW;
+  static constexpr int kWaves = DP * (int)sizeof(T) > 256 ? 4 : 8, kThreads = 64 * kWaves;
+  static constexpr int KT = 1, KW = BK / (16 * KT), RW = kWaves / KW;
   static constexpr int kStep = 32 * RW;  // rows a step
 };
 
@@ -445,10 +443,11 @@ __device__ __forceinline__ void careful_key(const GradArgs& a, const KeyPlace& a
 constexpr int kMostEntries = 1024;  // of a piece
 
 template <class T, int DP, int BK>
-__global__ __launch_bounds__(256) void block_key_grad_kernel(const GradArgs a) {
+__global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_grad_kernel(const GradArgs a) {
   using R = Rows<T, DP>;
   using S = KeyShape<T, DP, BK>;
   constexpr int KT = S::KT, KW = S::KW, RW = S::RW, STEP = S::kStep, F = R::kFrags;
+  constexpr int WAVES = S::kWaves, THREADS = S::kThreads;
   constexpr int kSlot = STEP * R::kRow, P = R::kUnit / 16;
   constexpr int kJoin = (RW - 1) * KW * KT * 16 * DP * 4 * 2;
   constexpr int kMemory = 4 * kSlot > kJoin ? 4 * kSlot : kJoin;
@@ -488,7 +487,7 @@ __global__ __launch_bounds__(256) void block_key_grad_kernel(const GradArgs a) {
   o.sq = sequence_of(p.seqs, o.seq);
   o.first = ((number - first_block(p.seqs, o.seq, lg_block)) << lg_block) + part * BK;
   const int entries = piece.z - piece.y, rows = entries * p.group;
-  for (int e = tid; e < entries; e += 256) s_token[e] = a.order[piece.y + e] / (a.lists * p.top);
+  for (int e = tid; e < entries; e += THREADS) s_token[e] = a.order[piece.y + e] / (a.lists * p.top);
   if (tid == 0) s_bad = 0;
 
   // the wave's keys and values, as second operands
@@ -522,8 +521,8 @@ __global__ __launch_bounds__(256) void block_key_grad_kernel(const GradArgs a) {
   float n_lse = 0.0f, n_delta = 0.0f;
   int n_pos = 0;
   auto issue = [&](int s) {
-    constexpr int kLoads = kSlot / 1024 / 4;
-    static_assert(kSlot % 4096 == 0, "whole loads a wave");
+    constexpr int kLoads = kSlot / 1024 / WAVES;
+    static_assert(kSlot % (1024 * WAVES) == 0, "whole loads a wave");
     const uint32_t qb = lds_address(s_mem) + (uint32_t)((s & 1) * 2 * kSlot), gb = qb + kSlot;
     const int lr = R::lane_row(lane), pos = lane % R::kPieces;
 #pragma unroll
@@ -691,7 +690,7 @@ __global__ __launch_bounds__(256) void block_key_grad_kernel(const GradArgs a) {
     return;
   }
   // a sum that is not finite: each key by itself, without products of what it is not seen by
-  for (int jj = w; jj < BK; jj += 4) {
+  for (int jj = w; jj < BK; jj += WAVES) {
     const int j = o.first + jj;
     constexpr int N = (DP + 63) / 64;
     float k_sum[N], v_sum[N];
@@ -928,7 +927,8 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
       constexpr int BK = decltype(bk)::value;
       const int64_t groups = l.pieces * shared * (seqs->block / BK);
       if (groups > kMostWorkgroups) return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
-      hipLaunchKernelGGL((block_key_grad_kernel<T, DP, BK>), dim3((uint32_t)groups), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((block_key_grad_kernel<T, DP, BK>), dim3((uint32_t)groups), dim3(KeyShape<T, DP, BK>::kThreads), 0,
+                         stream, a);
       FS_CHECK_LAUNCH("block_key_grad_kernel");
       return FS_OK;
     };
