@@ -151,4 +151,10 @@ __all__ = [
     "flagsparse_expert_combine_grad",
     "flagsparse_expert_product",
     "flagsparse_expert_product_grad",
+    "PreparedBlockSequences",
+    "prepare_block_sequences",
+    "flagsparse_block_means",
+    "flagsparse_block_select",
+    "flagsparse_block_attention",
+    "flagsparse_block_attention_grad",
 ]
