@@ -192,20 +192,18 @@ def _scale_of(scale, width):
 def _described(seqs, n_tokens, k):
     """The C entry points' description of the sequences; without k, which the selection
     does not read, their lengths alone."""
-    c = _lib.FsBlockSeqs()
-    c.n_seqs, c.n_tokens, c.block = seqs.n_seqs, n_tokens, seqs.block_size
-    if seqs.q_offsets is not None:
-        c.q_offsets = seqs.q_offsets.data_ptr()
+    q_offsets = seqs.q_offsets
     if seqs.pages is None:
-        c.k_offsets = seqs.k_offsets.data_ptr()
-        c.n_rows = _INT32_MAX if k is None else k.shape[0]
+        c = _lib.FsBlockSeqs(seqs.n_seqs, n_tokens, _INT32_MAX if k is None else k.shape[0],
+                             None if q_offsets is None else q_offsets.data_ptr(), seqs.k_offsets.data_ptr(), None, None,
+                             0, 0, 0, 0, 0, seqs.block_size)
     else:
+        pages, page = seqs.pages, 1 << 20 if k is None else k.shape[1]
         # (an empty table has no address of its own: any other will do, nothing is read)
-        c.pages = seqs.pages.data_ptr() or seqs.k_lengths.data_ptr() or 16
-        c.k_lengths = seqs.k_lengths.data_ptr()
-        c.ld_pages, c.pages_per_seq = seqs.pages.stride(0), seqs.pages.shape[1]
-        page = 1 << 20 if k is None else k.shape[1]
-        c.n_pages, c.page_size, c.page_shift = 0 if k is None else k.shape[0], page, page.bit_length() - 1
+        c = _lib.FsBlockSeqs(seqs.n_seqs, n_tokens, 0, None if q_offsets is None else q_offsets.data_ptr(), None,
+                             seqs.k_lengths.data_ptr(), pages.data_ptr() or seqs.k_lengths.data_ptr() or 16,
+                             pages.stride(0), pages.shape[1], 0 if k is None else k.shape[0], page,
+                             page.bit_length() - 1, seqs.block_size)
     return ctypes.byref(c)
 
 

@@ -33,16 +33,16 @@ constexpr float kSlack = 8.0f;
 // One step's keys and values.
 template <class T, int DP, int AHEAD, class Wait>
 __device__ inline void attend(Online<T, DP>& st, uint32_t kb, uint32_t vb, bool sel, int now, bool some,
-                              bool edge, uint32_t missing, const RowOf& row, float c, int lane, Wait values) {
+                              bool edge, uint32_t missing, const RowOf& row, float c, int used, int lane, Wait values) {
   using R = Rows<T, DP>;
   constexpr int G = R::kGroups, P = R::kUnit / 16;
   f32x4 s[G];
 #pragma unroll
   for (int gr = 0; gr < G; ++gr) s[gr] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  products<T, DP, AHEAD>(kb, st.q, s, lane);
+  products<T, DP, AHEAD>(kb, st.q, s, used, lane);
   values();  // are there: they are read while the weights are computed
   Columns<T, DP, AHEAD> v;
-  v.read(vb, 0, lane);
+  v.read(vb, 0, used, lane);
   if (edge) {
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) {
@@ -88,7 +88,7 @@ __device__ inline void attend(Online<T, DP>& st, uint32_t kb, uint32_t vb, bool 
   typename R::frag w[G / P];
 #pragma unroll
   for (int u = 0; u < G / P; ++u) w[u] = R::rounded(&s[u * P]);
-  v.add(vb, w, st.o, lane);
+  v.add(vb, w, st.o, used, lane);
 }
 
 // One row by a wave, key after key, without products of what is left out: a weight
@@ -182,10 +182,11 @@ __global__ __launch_bounds__((ManyShape<T, DP>::kThreads)) void block_attention_
                       (int64_t)(t.head * p.group + row.head) * p.q_head,
                   row.in, p.width, lane, st.q);
   const float c = p.scale * kLog2e;
+  const int used = (p.width + 15) / 16;
   walk_blocks<T, DP, Shape, false>(p, t, row, mem, lds_address(&mem), tid, w, lane,
                             [&](int now, bool sel, bool some, bool edge, uint32_t missing, uint32_t kb,
                                 uint32_t vb, auto values) {
-                              attend<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, missing, row, c, lane, values);
+                              attend<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, missing, row, c, used, lane, values);
                             });
   const float l = across_sum(st.l), by = l > 0.0f ? 1.0f / l : 0.0f;
   bool bad = !__builtin_isfinite(l);
@@ -372,6 +373,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP>::kWaves)) void block_attentio
   __syncthreads();
   const int lg_steps = lg - 5, steps = alike(s_count) << lg_steps;
   const float c = p.scale * kLog2e;
+  const int used = (p.width + 15) / 16;
   const uint32_t kb = lds_address(s_kv[w][0]), vb = lds_address(s_kv[w][1]);
   KeySource<T, DP> keys, values;
   keys.init(p, p.k, sq, seq, f.head, lane);
@@ -386,7 +388,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP>::kWaves)) void block_attentio
     keys.load(kb, k_place, lane);
     values.load(vb, v_place, lane);
     wait_loads<KeySource<T, DP>::kLoads>();
-    attend<T, DP, 8>(st, kb, vb, row.in, now, true, edge || k_place.missing != 0, k_place.missing, row, c, lane,
+    attend<T, DP, 8>(st, kb, vb, row.in, now, true, edge || k_place.missing != 0, k_place.missing, row, c, used, lane,
                   [] { wait_loads<0>(); });
   }
   wait_reads();
@@ -466,8 +468,10 @@ Plan plan_of(int val_t, const fs_block_seqs& s, int heads, int group, int width,
     const int bytes = (width <= 64 ? 64 : width <= 128 ? 128 : 256) * (val_t == FS_F32 ? 4 : 2);
     const int waves = bytes > 256 ? kFewWaves / 2 : kFewWaves;
     const int64_t steps = (int64_t)top * block / 32;
-    // until a wave has one step, or there are two workgroups a compute unit
-    while ((int64_t)o.splits * waves < steps && o.groups * o.splits < 512 && o.splits < 64) o.splits *= 2;
+    // until a wave has four steps, or there are two workgroups a compute unit (us with four
+    // and with one, where the join is a launch of its own: one token of 8 x 4 heads, 16
+    // blocks of 64 keys 20.7 and 24.8)
+    while ((int64_t)o.splits * waves * 4 < steps && o.groups * o.splits < 512 && o.splits < 64) o.splits *= 2;
     if (o.splits > 1)
       o.bytes = (size_t)(o.groups * o.splits) * (32 + 16 * (width <= 64 ? 64 : width <= 128 ? 128 : 256)) * 4;
   } else {

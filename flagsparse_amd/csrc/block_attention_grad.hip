@@ -74,17 +74,17 @@ struct QueryGrad {
 
 template <class T, int DP, int AHEAD, class Wait>
 __device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, bool sel, int now, bool some,
-                            bool edge, const RowOf& row, float c, float factor, int lane, Wait values) {
+                            bool edge, const RowOf& row, float c, float factor, int used, int lane, Wait values) {
   using R = Rows<T, DP>;
   constexpr int G = R::kGroups, P = R::kUnit / 16;
   f32x4 s[G], dp[G];
 #pragma unroll
   for (int gr = 0; gr < G; ++gr) s[gr] = dp[gr] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  products<T, DP, AHEAD>(kb, st.q, s, lane);
+  products<T, DP, AHEAD>(kb, st.q, s, used, lane);
   values();  // are there
-  products<T, DP, AHEAD>(vb, st.g, dp, lane);
+  products<T, DP, AHEAD>(vb, st.g, dp, used, lane);
   Columns<T, DP, AHEAD> k;
-  k.read(kb, 0, lane);
+  k.read(kb, 0, used, lane);
 #pragma unroll
   for (int gr = 0; gr < G; ++gr)
 #pragma unroll
@@ -110,7 +110,7 @@ __device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, bool
   typename R::frag w[G / P];
 #pragma unroll
   for (int u = 0; u < G / P; ++u) w[u] = R::rounded(&s[u * P]);
-  k.add(kb, w, st.d, lane);
+  k.add(kb, w, st.d, used, lane);
 }
 
 struct GradArgs {
@@ -224,9 +224,10 @@ __global__ __launch_bounds__((QueryGradShape<T, DP>::kThreads)) void block_query
 #pragma unroll
   for (int dt = 0; dt < DP / 16; ++dt) st.d[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   const float c = p.scale * kLog2e;
+  const int used = (p.width + 15) / 16;
   walk_blocks<T, DP, Shape, false>(p, t, row, mem, lds_address(&mem), tid, w, lane,
                             [&](int now, bool sel, bool some, bool edge, uint32_t, uint32_t kb, uint32_t vb,
-                                auto values) { take<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, row, c, factor, lane, values); });
+                                auto values) { take<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, row, c, factor, used, lane, values); });
   bool bad = false;
 #pragma unroll
   for (int dt = 0; dt < DP / 16; ++dt)
@@ -511,7 +512,7 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
   const int offset = o.sq.keys - o.sq.count - o.sq.first;  // of positions from tokens
   __syncthreads();
 
-  const int steps = (rows + STEP - 1) / STEP;
+  const int steps = (rows + STEP - 1) / STEP, used = (p.width + 15) / 16;
   auto place = [&](int r, int& token, int& hq) {
     const int e = (int)__umulhi((uint32_t)r, a.per_group);
     const int entry = p.group == 1 ? r : e;
@@ -569,7 +570,8 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
 #pragma unroll
       for (int n = 0; n < KT; ++n) x[m][n] = y[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int ks = 0; ks < F; ++ks)
+    for (int ks = 0; ks < F; ++ks) {
+      if (leave_out<T>(ks, used)) break;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         const auto q = R::across(qb, m * 16, ks, lane);
@@ -580,6 +582,7 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
           y[m][n] = Mma<T>::run(g, vf[n][ks], y[m][n]);
         }
       }
+    }
     typename R::frag pf[KT][2 / P], sf[KT][2 / P];
     f32x4 wx[KT][2], wy[KT][2];
 #pragma unroll
@@ -616,6 +619,7 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
     for (int u = 0; u < 2 / P; ++u)
 #pragma unroll
       for (int dt = 0; dt < DP / 16; ++dt) {
+        if (leave_out<T>(dt, used)) break;
         const auto g = R::down(gb, u * R::kUnit, dt, lane);
         const auto q = R::down(qb, u * R::kUnit, dt, lane);
 #pragma unroll

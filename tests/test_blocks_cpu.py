@@ -261,7 +261,7 @@ def test_workspace_sizes():
         return lib.fs_block_attention_workspace_bytes(f16, ctypes.byref(c), heads, 4, 128, top)
 
     assert need(64, 16) == 0  # workgroups enough without splitting
-    assert need(1, 16) > 0  # one token's blocks over several
+    assert need(1, 128) > 0  # one token with many blocks: several share them
     assert need(0, 16) == 0
     assert need(16384, 16) < 1 << 20  # a word a wave
     c = _described(n_tokens=8192, n_rows=8192, n_seqs=1)
