@@ -168,7 +168,7 @@ __global__ __launch_bounds__((ManyShape<T, DP>::kThreads)) void block_attention_
   __shared__ typename Shape::Memory mem;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   WalkTile t;
-  if (!walk_tile(p, lane, t)) return;
+  if (!walk_tile(p, blockIdx.x, lane, t)) return;
   walk_start<Shape>(mem, tid);
   if (w >= Shape::kReaders) {
     walk_loads<T, DP, Shape>(p, t, mem, lds_address(&mem), tid, w, lane);
@@ -209,7 +209,7 @@ __global__ __launch_bounds__((64 * ManyShape<T, DP>::kReaders)) void block_atten
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   WalkTile t;
   uint32_t rows = alike((int)p.again[(int64_t)blockIdx.x * ManyShape<T, DP>::kReaders + w]);
-  if (rows == 0 || !walk_tile(p, lane, t)) return;
+  if (rows == 0 || !walk_tile(p, blockIdx.x, lane, t)) return;
   for (; rows != 0; rows &= rows - 1) {
     const int r = w * 16 + __builtin_ctz(rows), tok = r / p.group;
     careful_row<T, DP>(p, t.sq, t.seq, t.token0 + tok, t.head, r - tok * p.group, t.pos0 + tok, lane);

@@ -45,22 +45,20 @@ __device__ inline float read_factor(const float* parts, int lane) {
   }
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void block_amax_kernel(const T* x, int64_t n, float* parts) {
+// One of kAmaxParts workgroups' largest value of n, a multiple of 8.
+__device__ inline void amax_part(const _Float16* x, int64_t n, float* parts, uint32_t block) {
   __shared__ float s_max[4];
   float m = 0.0f;
-  const int64_t step = (int64_t)gridDim.x * 256 * Slice<T>::n;
-  for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * Slice<T>::n; at < n; at += step) {
-    // (n is a multiple of 8)
-    const Slice<T> v = load_slice(x + at);
+  for (int64_t at = ((int64_t)block * 256 + threadIdx.x) * 8; at < n; at += (int64_t)kAmaxParts * 256 * 8) {
+    const Slice<_Float16> v = load_slice(x + at);
 #pragma unroll
-    for (int e = 0; e < Slice<T>::n; ++e) m = fmaxf(m, fabsf((float)v.v[e]));
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf((float)v.v[e]));
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
   if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
   __syncthreads();
-  if (threadIdx.x == 0) parts[blockIdx.x] = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+  if (threadIdx.x == 0) parts[block] = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
 }
 
 // ---- gradient of the queries ------------------------------------------------------
@@ -194,7 +192,10 @@ __global__ __launch_bounds__((QueryGradShape<T, DP>::kThreads)) void block_query
   const BlockArgs& p = a.b;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   WalkTile t;
-  if (!walk_tile(p, lane, t)) return;
+  if (!walk_tile(p, blockIdx.x, lane, t)) {
+    if (tid < Shape::kReaders) p.again[(int64_t)blockIdx.x * Shape::kReaders + tid] = 0u;
+    return;
+  }
   walk_start<Shape>(mem, tid);
   if (w >= Shape::kReaders) {
     walk_loads<T, DP, Shape>(p, t, mem, lds_address(&mem), tid, w, lane);
@@ -239,19 +240,22 @@ __global__ __launch_bounds__((QueryGradShape<T, DP>::kThreads)) void block_query
     p.again[(int64_t)blockIdx.x * Shape::kReaders + w] = (uint32_t)(rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xffffu;
 }
 
-// Rows whose gradient is not finite, key after key.
+// Rows whose gradient is not finite, key after key: those of one workgroup of the kernel
+// above, by `waves` waves.
 template <class T, int DP>
-__global__ __launch_bounds__((64 * QueryGradShape<T, DP>::kReaders)) void block_query_grad_again_kernel(const GradArgs a) {
+__device__ inline void queries_again(const GradArgs& a, uint32_t block, int w, int waves, int lane) {
   const BlockArgs& p = a.b;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  WalkTile t;
-  uint32_t rows = alike((int)p.again[(int64_t)blockIdx.x * QueryGradShape<T, DP>::kReaders + w]);
-  if (rows == 0 || !walk_tile(p, lane, t)) return;
-  for (; rows != 0; rows &= rows - 1) {
-    const int r = w * 16 + __builtin_ctz(rows), tok = r / p.group, in_group = r - tok * p.group;
-    const int64_t at = (int64_t)(t.token0 + tok) * p.heads * p.group + t.head * p.group + in_group;
-    careful_query<T, DP>(a, t.sq, t.seq, t.token0 + tok, t.head, in_group, t.pos0 + tok, a.lse[at] * kLog2e, a.delta[at],
-                         lane);
+  constexpr int READERS = QueryGradShape<T, DP>::kReaders;
+  for (; w < READERS; w += waves) {
+    uint32_t rows = (uint32_t)alike((int)p.again[(int64_t)block * READERS + w]);
+    WalkTile t;
+    if (rows == 0 || !walk_tile(p, block, lane, t)) continue;
+    for (; rows != 0; rows &= rows - 1) {
+      const int r = w * 16 + __builtin_ctz(rows), tok = r / p.group, in_group = r - tok * p.group;
+      const int64_t at = (int64_t)(t.token0 + tok) * p.heads * p.group + t.head * p.group + in_group;
+      careful_query<T, DP>(a, t.sq, t.seq, t.token0 + tok, t.head, in_group, t.pos0 + tok, a.lse[at] * kLog2e, a.delta[at],
+                           lane);
+    }
   }
 }
 
@@ -265,9 +269,12 @@ __device__ inline int first_block(const fs_block_seqs& s, int b, int lg_block) {
 
 // The key that each entry of the selection is sorted by, head by head and block by
 // block; one too large for entries that name nothing or the same block again.  A
-// wave takes a token.  Also zeros the gradients of rows of no sequence.
+// wave takes a token.  Also zeros the gradients of rows of no sequence and, of float16,
+// finds the largest value of the gradient.
 __global__ __launch_bounds__(256) void block_keys_kernel(const BlockArgs p, int lists, int key_blocks, int32_t* keys,
-                                                         uint32_t* dk, uint32_t* dv, int64_t row_words) {
+                                                         uint32_t* dk, uint32_t* dv, int64_t row_words,
+                                                         const _Float16* grad, int64_t values, float* amax) {
+  if (grad != nullptr && blockIdx.x < kAmaxParts) amax_part(grad, values, amax, blockIdx.x);
   const int lane = threadIdx.x & 63, lg = p.lg_groups + 4;
   const int64_t waves = (int64_t)gridDim.x * 4, first = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int n_keys = lists * key_blocks;
@@ -318,28 +325,40 @@ __global__ __launch_bounds__(256) void block_keys_kernel(const BlockArgs p, int 
 }
 
 // First sorted entry of each key.
-__global__ __launch_bounds__(256) void block_lists_kernel(const uint32_t* keys, int64_t n, int n_keys, int32_t* starts) {
-  const int k = (int)(blockIdx.x * 256 + threadIdx.x);
-  if (k > n_keys) return;
+__device__ inline int32_t first_of(const uint32_t* keys, int64_t n, uint32_t k) {
   int64_t lo = 0, hi = n;
   while (lo < hi) {
     const int64_t mid = (lo + hi) >> 1;
-    if (keys[mid] < (uint32_t)k) lo = mid + 1;
+    if (keys[mid] < k) lo = mid + 1;
     else hi = mid;
   }
-  starts[k] = (int32_t)lo;
+  return (int32_t)lo;
+}
+__global__ __launch_bounds__(256) void block_lists_kernel(const uint32_t* keys, int64_t n, int n_keys, int32_t* starts) {
+  const int k = (int)(blockIdx.x * 256 + threadIdx.x);
+  if (k <= n_keys) starts[k] = first_of(keys, n, (uint32_t)k);
 }
 
 // Lists cut into pieces of `most` entries at most, one at least, and places for the
-// sums of those with more than one.  One workgroup.
-__global__ __launch_bounds__(1024) void block_pieces_kernel(const int32_t* starts, int n_keys, int most, int4* pieces,
-                                                            int2* sums, int32_t* n_pieces) {
+// sums of those with more than one.  One workgroup; up to kFewKeys keys it finds the
+// lists itself (FIND), which saves a launch.
+constexpr int kFewKeys = 2048;
+template <bool FIND>
+__global__ __launch_bounds__(1024) void block_pieces_kernel(const uint32_t* keys, int64_t entries, const int32_t* starts,
+                                                            int n_keys, int most, int4* pieces, int2* sums,
+                                                            int32_t* n_pieces) {
   __shared__ uint32_t s_total[2][16];
+  __shared__ int32_t s_first[FIND ? kFewKeys + 1 : 1];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  if constexpr (FIND) {
+    for (int k = tid; k <= n_keys; k += 1024) s_first[k] = first_of(keys, entries, (uint32_t)k);
+    __syncthreads();
+  }
+  auto first = [&](int k) { return FIND ? s_first[FIND ? k : 0] : starts[k]; };
   uint32_t at = 0, place = 0;
   for (int k0 = 0; k0 < n_keys; k0 += 1024) {
     const int k = k0 + tid;
-    const int from = k < n_keys ? starts[k] : 0, to = k < n_keys ? starts[k + 1] : 0;
+    const int from = k < n_keys ? first(k) : 0, to = k < n_keys ? first(k + 1) : 0;
     const uint32_t n = k < n_keys ? (uint32_t)(to > from ? (to - from + most - 1) / most : 1) : 0u;
     const uint32_t shared = n > 1 ? n : 0u;
     const uint32_t upto = wave_sum_scan(n), upto2 = wave_sum_scan(shared);
@@ -715,12 +734,17 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
   }
 }
 
-// Sums of a block's pieces, in order: a workgroup 16 keys of one.
+// Sums of a block's pieces, in order: a workgroup 16 keys of one.  The first `again`
+// workgroups take the queries' rows that are not finite.
 template <class T, int DP>
-__global__ __launch_bounds__(256) void block_key_join_kernel(const GradArgs a) {
+__global__ __launch_bounds__(256) void block_key_join_kernel(const GradArgs a, int64_t again) {
   const BlockArgs& p = a.b;
   const int lane = threadIdx.x & 63, lg_block = p.lg_groups + 4, shared = p.heads / a.lists;
-  int64_t at = row_block();
+  int64_t at = row_block() - again;
+  if (at < 0) {
+    queries_again<T, DP>(a, (uint32_t)(at + again), __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), 4, lane);
+    return;
+  }
   const int group = (int)(at & ((1 << p.lg_groups) - 1));
   at >>= p.lg_groups;
   const int copy = (int)(at % shared), key = (int)(at / shared);
@@ -892,39 +916,42 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
   uint32_t* sorted = reinterpret_cast<uint32_t*>(m + l.sorted);
   int32_t* starts = reinterpret_cast<int32_t*>(m + l.starts);
 
-  hipLaunchKernelGGL(block_keys_kernel, dim3((uint32_t)std::min<int64_t>(ceil_div(std::max<int64_t>(tokens, 4), 4), 4096)),
+  const bool factored = val_t == FS_F16 && tokens > 0;
+  const int64_t key_groups = std::min<int64_t>(ceil_div(std::max<int64_t>(tokens, 4), 4), 4096);
+  hipLaunchKernelGGL(block_keys_kernel, dim3((uint32_t)(factored ? std::max<int64_t>(key_groups, kAmaxParts) : key_groups)),
                      dim3(256), 0, stream, p, lists, (int)l.key_blocks, keys, static_cast<uint32_t*>(dk),
-                     static_cast<uint32_t*>(dv), (int64_t)heads * width * size / 4);
+                     static_cast<uint32_t*>(dv), (int64_t)heads * width * size / 4,
+                     factored ? static_cast<const _Float16*>(grad) : nullptr, tokens * heads * group * width, amax);
   FS_CHECK_LAUNCH("block_keys_kernel");
   if (l.entries > 0) {
     if (const int rc = select_sort(keys, FS_I32, l.entries, l.n_keys, sorted, reinterpret_cast<int32_t*>(m + l.order),
                                    nullptr, nullptr, m + l.sort, stream, nullptr, 0))
       return rc;
   }
-  hipLaunchKernelGGL(block_lists_kernel, dim3((uint32_t)ceil_div(l.n_keys + 1, 256)), dim3(256), 0, stream, sorted,
-                     l.entries, (int)l.n_keys, starts);
-  FS_CHECK_LAUNCH("block_lists_kernel");
-  hipLaunchKernelGGL(block_pieces_kernel, dim3(1), dim3(1024), 0, stream, starts, (int)l.n_keys, l.most,
-                     const_cast<int4*>(a.pieces), const_cast<int2*>(a.sums), const_cast<int32_t*>(a.n_pieces));
+  int4* pieces = const_cast<int4*>(a.pieces);
+  int2* sums = const_cast<int2*>(a.sums);
+  int32_t* n_pieces = const_cast<int32_t*>(a.n_pieces);
+  if (l.n_keys <= kFewKeys) {
+    hipLaunchKernelGGL((block_pieces_kernel<true>), dim3(1), dim3(1024), 0, stream, sorted, l.entries, starts,
+                       (int)l.n_keys, l.most, pieces, sums, n_pieces);
+  } else {
+    hipLaunchKernelGGL(block_lists_kernel, dim3((uint32_t)ceil_div(l.n_keys + 1, 256)), dim3(256), 0, stream, sorted,
+                       l.entries, (int)l.n_keys, starts);
+    FS_CHECK_LAUNCH("block_lists_kernel");
+    hipLaunchKernelGGL((block_pieces_kernel<false>), dim3(1), dim3(1024), 0, stream, sorted, l.entries, starts,
+                       (int)l.n_keys, l.most, pieces, sums, n_pieces);
+  }
   FS_CHECK_LAUNCH("block_pieces_kernel");
   return with_block_width(val_t, width, who, [&](auto val, auto dp) -> int {
     using T = decltype(val);
     constexpr int DP = decltype(dp)::value;
     if (tokens > 0) {
-      if constexpr (kFactored<T>) {
-        hipLaunchKernelGGL((block_amax_kernel<T>), dim3(kAmaxParts), dim3(256), 0, stream, static_cast<const T*>(grad),
-                           tokens * heads * group * width, amax);
-        FS_CHECK_LAUNCH("block_amax_kernel");
-      }
       p.tiles = l.tiles;
       p.per = l.per;
       if (p.tiles * heads > kMostWorkgroups) return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
       const dim3 grid((uint32_t)(p.tiles * heads));
       hipLaunchKernelGGL((block_query_grad_kernel<T, DP>), grid, dim3(QueryGradShape<T, DP>::kThreads), 0, stream, a);
       FS_CHECK_MAIN_LAUNCH("block_query_grad_kernel");
-      hipLaunchKernelGGL((block_query_grad_again_kernel<T, DP>), grid, dim3(64 * QueryGradShape<T, DP>::kReaders), 0,
-                         stream, a);
-      FS_CHECK_LAUNCH("block_query_grad_again_kernel");
     }
     const int64_t shared = heads / lists;
     auto keys_of = [&](auto bk) -> int {
@@ -939,8 +966,9 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
     if (const int rc = seqs->block == 32 ? keys_of(std::integral_constant<int, 32>{})
                                          : keys_of(std::integral_constant<int, 64>{}))
       return rc;
-    hipLaunchKernelGGL((block_key_join_kernel<T, DP>), row_grid((l.n_keys * shared) << p.lg_groups), dim3(256), 0, stream,
-                       a);
+    const int64_t again = tokens > 0 ? p.tiles * heads : 0;
+    hipLaunchKernelGGL((block_key_join_kernel<T, DP>), row_grid(again + ((l.n_keys * shared) << p.lg_groups)), dim3(256), 0,
+                       stream, a, again);
     FS_CHECK_LAUNCH("block_key_join_kernel");
     return FS_OK;
   });

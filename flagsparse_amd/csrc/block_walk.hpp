@@ -59,8 +59,8 @@ struct WalkTile {
 
 // Head by head over the XCDs (each has its keys and values in a cache of its own), a
 // head's last tiles first: they have the most blocks to choose from.
-__device__ inline bool walk_tile(const BlockArgs& p, int lane, WalkTile& t) {
-  const int64_t at = xcd_range_block(blockIdx.x, gridDim.x);
+__device__ inline bool walk_tile(const BlockArgs& p, uint32_t block, int lane, WalkTile& t) {
+  const int64_t at = xcd_range_block(block, (uint32_t)(p.tiles * p.heads));
   t.head = (int)(at / p.tiles);
   int tile;
   if (!find_tile(p.seqs, p.per, p.tiles - 1 - at % p.tiles, lane, t.seq, tile)) return false;
