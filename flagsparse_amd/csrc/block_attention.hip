@@ -5,6 +5,15 @@
 // own position: a product of dense matrices sampled where the selection is, a softmax
 // along its rows, and the sparse matrix so made times the values, in one pass with the
 // running maximum and sum of each row.  A block named twice counts once.
+//
+// Many queries (block_walk.hpp): 16384 tokens of 4 x 16 heads of 128, 16 blocks of 64
+// keys, bf16 1617 us, 320 TFLOP/s; 4 x 512 tokens of 4 x 8 heads over 16384 keys in pages
+// of 16, 32 blocks, f16 398 us.  Ten tokens beside each other select 80 different blocks
+// of 256, so a block has two or three readers, and what bounds it is the way of a step
+// through a slot (load, announcement, reading): the matrix instructions are busy for 15%
+// of the cycles, LDS for 25, and without its loads or without its products it takes nine
+// tenths as long.  Few queries: 64 tokens of 8 x 8 heads over as many caches 53 us, 262 MB
+// at 4.9 TB/s, a copy's rate.
 #include "block_walk.hpp"
 
 namespace fs {
