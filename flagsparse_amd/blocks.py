@@ -182,6 +182,12 @@ def _check_blocks(blocks, q, heads):
         raise ValueError(f"blocks must name 1 to {MAX_SELECTED_BLOCKS} blocks a query, got {blocks.shape[2]}")
 
 
+def _check_gradient(group, width, dtype):
+    """A workgroup of the queries' gradient holds a group's rows: 96 where they are wide."""
+    if group > 96 and width * dtype.itemsize > 256:
+        raise ValueError(f"gradients of rows of more than 256 bytes need groups of up to 96 heads, got {group}")
+
+
 def _scale_of(scale, width):
     scale = width**-0.5 if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
@@ -425,6 +431,7 @@ def flagsparse_block_attention(q, k, v, blocks, seqs, scale=None, out=None, retu
             raise ValueError("out cannot be given where a gradient is recorded")
         if seqs.pages is not None:
             raise ValueError("keys and values of a cache have no gradient: detach them, and q")
+        _check_gradient(group, width, q.dtype)
         result, lse = _BlockAttention.apply(q, k, v, blocks, seqs, scale)
     else:
         if out is not None:
@@ -437,11 +444,13 @@ def flagsparse_block_attention_grad(grad, q, k, v, blocks, seqs, out, lse, scale
     """Gradients of ``flagsparse_block_attention`` in q, k and v, of packed rows.
 
     grad has q's shape; out and lse are the forward call's results.  Rows of no
-    sequence get zeros.  Records no graph.
+    sequence get zeros.  Rows of more than 256 bytes take groups of up to 96 heads.
+    Records no graph.
     """
     heads, group, width = _check_attention(q, k, v, blocks, seqs)
     if seqs.pages is not None:
         raise ValueError("keys and values of a cache have no gradient")
+    _check_gradient(group, width, q.dtype)
     for t, what in ((grad, "grad"), (out, "out")):
         _check_values(t, what, seqs, 3)
         if t.dtype != q.dtype:

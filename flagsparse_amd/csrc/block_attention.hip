@@ -470,7 +470,9 @@ Plan plan_of(int val_t, const fs_block_seqs& s, int heads, int group, int width,
   Plan o{};
   const int64_t tokens = s.n_tokens;
   const int block = s.block;
-  o.few = tokens * heads <= kFewPairs;
+  o.readers = many_readers((width <= 64 ? 64 : width <= 128 ? 128 : 256) * (val_t == FS_F32 ? 4 : 2));
+  // (a group whose rows do not fit a workgroup of the other kernel, too)
+  o.few = tokens * heads <= kFewPairs || o.readers * 16 < group;
   o.groups = tokens * heads * ((group + 15) / 16);
   o.splits = 1;
   if (o.few) {
@@ -484,7 +486,6 @@ Plan plan_of(int val_t, const fs_block_seqs& s, int heads, int group, int width,
     if (o.splits > 1)
       o.bytes = (size_t)(o.groups * o.splits) * (32 + 16 * (width <= 64 ? 64 : width <= 128 ? 128 : 256)) * 4;
   } else {
-    o.readers = many_readers((width <= 64 ? 64 : width <= 128 ? 128 : 256) * (val_t == FS_F32 ? 4 : 2));
     o.per = o.readers * 16 / group;
     o.tiles = block_tiles(s, o.per);
     o.bytes = (size_t)(o.tiles * heads) * o.readers * 4;

@@ -847,6 +847,8 @@ int grad_fault(const char* who, int val_t, const fs_block_seqs* seqs, int heads,
   if (const int rc = block_sizes_fault(who, val_t, seqs, heads, group, width)) return rc;
   if (seqs->pages != nullptr) return fail(FS_E_INVALID, std::string(who) + ": keys of a cache have no gradient");
   if (top < 1 || top > kMostTop) return fail(FS_E_INVALID, std::string(who) + ": top out of range");
+  const int row = (width <= 64 ? 64 : width <= 128 ? 128 : 256) * (val_t == FS_F32 ? 4 : 2);
+  if (group > query_readers(row) * 16) return fail(FS_E_INVALID, std::string(who) + ": heads out of range for this width");
   if (lists != 1 && lists != heads) return fail(FS_E_INVALID, std::string(who) + ": lists is 1 or the heads");
   const int64_t blocks = (seqs->n_rows / seqs->block + seqs->n_seqs + 1) * lists;
   if (seqs->n_tokens * lists * top > INT32_MAX || blocks >= INT32_MAX)

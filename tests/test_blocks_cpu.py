@@ -125,6 +125,9 @@ def test_operands_are_checked():
         attend(leaf, cache, cache, ids, _seqs(2, paged=True))
     grad = fs.flagsparse_block_attention_grad
     lse = _fake((5, 6), torch.float32)
+    with pytest.raises(ValueError, match="groups of up to 96 heads, got 97"):
+        wide, keys = _fake((5, 97, 256)), _fake((40, 1, 256))
+        grad(wide, wide, keys, keys, ids[:, :1], seqs, wide, _fake((5, 97), torch.float32))
     with pytest.raises(ValueError, match="keys and values of a cache have no gradient"):
         cache = _fake((4, 16, 3, 64))
         grad(q, q, cache, cache, ids, _seqs(2, paged=True), q, lse)
@@ -223,6 +226,7 @@ def test_c_refusals_without_touching_the_gpu():
     many = _described(n_tokens=100000, n_rows=100000)
     need = lib.fs_block_attention_workspace_bytes(f16, ctypes.byref(many), 3, 2, 64, 4)
     assert need > 0
+    assert lib.fs_block_attention_workspace_bytes(f16, ctypes.byref(many), 3, 128, 256, 4) == 0  # a token's rows are many
     refused(attend(many, ws=FAKE, need=need - 1), "workspace too small", _lib.FS_E_WORKSPACE)
 
     def grad(c, lists=3, top=4, q=FAKE, ws=FAKE, need=1 << 40, dk=FAKE):
@@ -230,6 +234,10 @@ def test_c_refusals_without_touching_the_gpu():
                                            FAKE, 192, 64, FAKE, 12, 4, 0.125, FAKE, FAKE, FAKE, dk, FAKE, ws, need, None)
 
     refused(grad(_described(**paged)), "no gradient")
+    c = _described()
+    refused(lib.fs_block_attention_grad(f16, ctypes.byref(c), 1, 97, 256, 1, 4, FAKE, FAKE, 384, 64, FAKE, 256, 256, FAKE,
+                                        256, 256, FAKE, 4, 0, 0.125, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 40, None),
+            "heads out of range for this width")
     refused(grad(_described(), lists=2), "lists is 1 or the heads")
     refused(grad(_described(), q=FAKE + 4), "multiples of 16 bytes")
     refused(grad(_described(), dk=None), "bad pointer")

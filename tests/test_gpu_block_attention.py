@@ -116,3 +116,25 @@ def test_grad_wide(width, block, dtype):
     found = oracle(case, blocks, 0.07, grad)
     for t, name in zip(got, ("dq", "dk", "dv")):
         assert_within(t, found, name)
+
+
+@pytest.mark.parametrize("tokens", [3, 70])
+@pytest.mark.parametrize("group", [96, 97, 128])
+@pytest.mark.parametrize("width", [128, 256])
+def test_large_groups(tokens, group, width):
+    """One key-value head of many query heads: a token's rows take several waves, or more than a workgroup has."""
+    case = Case([tokens], [tokens + 130], 64 if tokens > 3 else 1, group, width, 64, torch.bfloat16, 11)
+    if tokens > 3:
+        assert tokens * case.heads > 4096
+    blocks = random_blocks([tokens], [tokens + 130], case.heads, 3, 64, 12)
+    out, lse = fs.flagsparse_block_attention(case.q, case.k, case.v, blocks, case.seqs, return_lse=True)
+    found = oracle(case, blocks, width**-0.5)
+    assert_within(lse, found, "lse")
+    assert_within(out, found, "out")
+    if tokens > 3 or (group > 96 and width > 128):  # (the gradient of such groups is refused)
+        return
+    grad = randn(case.q.shape, torch.bfloat16, 13)
+    got = fs.flagsparse_block_attention_grad(grad, case.q, case.k, case.v, blocks, case.seqs, out, lse)
+    found = oracle(case, blocks, width**-0.5, grad)
+    for t, name in zip(got, ("dq", "dk", "dv")):
+        assert_within(t, found, name)
