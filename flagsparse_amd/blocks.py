@@ -45,6 +45,7 @@ BLOCK_VALUE_CODES = {
     torch.float32: _lib.FS_F32,
 }
 _INT32_MAX = 2**31 - 1
+_MAX_KEYS = _INT32_MAX - 2047
 
 
 class PreparedBlockSequences:
@@ -151,7 +152,7 @@ def _check_keys(k, what, seqs):
         page = k.shape[1]
         if page < 16 or page > 1 << 20 or page & (page - 1):
             raise ValueError(f"pages must have a power of two of rows, at least 16, got {page}")
-    elif k.shape[0] > _INT32_MAX:
+    elif k.shape[0] > _MAX_KEYS:
         raise ValueError(f"{what} rows exceed the int32 range")
 
 
@@ -200,7 +201,7 @@ def _described(seqs, n_tokens, k):
     does not read, their lengths alone."""
     q_offsets = seqs.q_offsets
     if seqs.pages is None:
-        c = _lib.FsBlockSeqs(seqs.n_seqs, n_tokens, _INT32_MAX if k is None else k.shape[0],
+        c = _lib.FsBlockSeqs(seqs.n_seqs, n_tokens, _MAX_KEYS if k is None else k.shape[0],
                              None if q_offsets is None else q_offsets.data_ptr(), seqs.k_offsets.data_ptr(), None, None,
                              0, 0, 0, 0, 0, seqs.block_size)
     else:

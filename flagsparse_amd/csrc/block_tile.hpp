@@ -18,6 +18,8 @@ namespace fs {
 namespace {
 
 constexpr int kMostTop = 128;  // blocks that a query may select
+// Keys of a sequence, so that the position behind its last block fits 32 bits too.
+constexpr int64_t kMostKeys = INT32_MAX - 2047;
 
 // ---- sequences, pages -----------------------------------------------------------
 
@@ -46,7 +48,7 @@ __device__ inline Sequence sequence_at(const fs_block_seqs& s, int b) {
   if (b < s.n_seqs) {
     if (s.pages != nullptr) {
       const int64_t most = s.pages_per_seq * s.page_size;
-      o.keys = clamp_to(s.k_lengths[b], 0, most < INT32_MAX ? most : INT32_MAX);
+      o.keys = clamp_to(s.k_lengths[b], 0, most < kMostKeys ? most : kMostKeys);
     } else {
       o.row0 = clamp_to(s.k_offsets[b], 0, s.n_rows);
       o.keys = clamp_to(s.k_offsets[b + 1], o.row0, s.n_rows) - (int)o.row0;
@@ -438,7 +440,7 @@ inline int block_seqs_fault(const char* who, const fs_block_seqs* s) {
   auto refuse = [&](const char* text) { return fail(FS_E_INVALID, std::string(who) + ": " + text); };
   if (s == nullptr) return refuse("null pointer");
   if (s->n_seqs < 0 || s->n_seqs > INT32_MAX / 2 || s->n_tokens < 0 || s->n_tokens > INT32_MAX || s->n_rows < 0 ||
-      s->n_rows > INT32_MAX)
+      s->n_rows > kMostKeys)
     return refuse("sizes out of range");
   if (s->block < 32 || s->block > 1024 || (s->block & (s->block - 1)) != 0)
     return refuse("blocks are of 32, 64, 128, 256, 512 or 1024 keys");

@@ -205,6 +205,7 @@ def test_c_refusals_without_touching_the_gpu():
     refused(attend(_described(), val=f64), "value types are")
     refused(attend(_described(n_seqs=-1)), "sizes out of range")
     refused(attend(_described(n_rows=1 << 31)), "sizes out of range")
+    refused(attend(_described(n_rows=(1 << 31) - 2047)), "sizes out of range")  # the end of its last block
     refused(attend(_described(block=48)), "blocks are of")
     refused(attend(_described(q_offsets=None)), "without offsets a sequence has one token")
     refused(attend(_described(k_offsets=None)), "null pointer")
