@@ -430,7 +430,7 @@ __device__ inline void store_row(T* row, const f32x4 (&o)[DP / 16], float by, in
 
 // ---- host side ------------------------------------------------------------------
 
-constexpr int64_t kMostWorkgroups = ((int64_t)1 << 32) / 512 - 1;  // of 256 threads, in one dimension
+constexpr int64_t kMostWorkgroups = ((int64_t)1 << 32) / 1024 - 1;  // of up to 1024 threads, in one dimension
 
 inline int64_t block_tiles(const fs_block_seqs& s, int per) {
   return s.q_offsets == nullptr ? s.n_seqs : s.n_tokens / per + s.n_seqs + 1;

@@ -230,6 +230,9 @@ def test_c_refusals_without_touching_the_gpu():
     assert lib.fs_block_attention_workspace_bytes(f16, ctypes.byref(many), 3, 128, 256, 4) == 0  # a token's rows are many
     refused(attend(many, ws=FAKE, need=need - 1), "workspace too small", _lib.FS_E_WORKSPACE)
 
+    most = _described(n_tokens=1 << 27)  # more workgroups of 1024 threads than a launch can have
+    refused(attend(most, heads=2, group=12, ws=FAKE, need=1 << 40), "sizes out of range")
+
     def grad(c, lists=3, top=4, q=FAKE, ws=FAKE, need=1 << 40, dk=FAKE):
         return lib.fs_block_attention_grad(f16, ctypes.byref(c), 3, 2, 64, lists, top, FAKE, q, 384, 64, FAKE, 192, 64,
                                            FAKE, 192, 64, FAKE, 12, 4, 0.125, FAKE, FAKE, FAKE, dk, FAKE, ws, need, None)
