@@ -138,3 +138,20 @@ def test_large_groups(tokens, group, width):
     found = oracle(case, blocks, width**-0.5, grad)
     for t, name in zip(got, ("dq", "dk", "dv")):
         assert_within(t, found, name)
+
+
+@pytest.mark.parametrize("group", [1, 3])
+def test_many_blocks_in_several_windows(group):
+    """More blocks than a workgroup's table holds at a time."""
+    tokens, length = 2100, 60000
+    case = Case([tokens], [length], 2, group, 32, 32, torch.bfloat16, 14)
+    blocks = random_blocks([tokens], [length], 2, 5, 32, 15)
+    out, lse = fs.flagsparse_block_attention(case.q, case.k, case.v, blocks, case.seqs, return_lse=True)
+    rows = torch.arange(0, tokens, 97)
+    for t in rows.tolist():
+        p = length - tokens + t
+        one = Case([1], [p + 1], 2, group, 32, 32, torch.bfloat16, 14)
+        one.q, one.packed_k, one.packed_v = case.q[t : t + 1], case.packed_k[: p + 1], case.packed_v[: p + 1]
+        found = oracle(one, blocks[t : t + 1], 32**-0.5)
+        assert_within(lse[t : t + 1], found, "lse")
+        assert_within(out[t : t + 1], found, "out")
