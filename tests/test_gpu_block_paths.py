@@ -420,3 +420,61 @@ def test_prompt_then_decode_with_summaries_kept():
         case.q, case.packed_k, case.packed_v = q[rows], k[: at + new], v[: at + new]
         assert_within(out, oracle(case, blocks, width**-0.5), "out")
         at += new
+
+
+@pytest.mark.parametrize("tokens", [2, 1100], ids=["few", "many"])
+@pytest.mark.parametrize("page", [0, 64], ids=["rows", "pages"])
+def test_keys_behind_32_bits(page, tokens):
+    """Keys 4.3 billion elements into their array: bit for bit those of a short one."""
+    heads, width, block, length = 4, 128, 64, 1500
+    case = Case([tokens], [length], heads, 1, width, block, torch.bfloat16, 21)
+    blocks = random_blocks([tokens], [length], heads, 5, block, 22)
+    want, want_lse = _attend(case, blocks, return_lse=True)
+    want_means = fs.flagsparse_block_means(case.k, case.seqs, 24)
+    rows = 2**32 // (heads * width) + 20000 // block * block
+    k = torch.zeros((rows, heads, width), dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    k[-length:], v[-length:] = case.k, case.v
+    if page:
+        at = rows // page * page - 1536
+        k[at : at + length], v[at : at + length] = case.k, case.v
+        table = (torch.arange(24, dtype=torch.int32) + at // page)[None].cuda()
+        seqs = fs.prepare_block_sequences(block, offsets([tokens]), pages=table,
+                                          k_lengths=torch.tensor([length], dtype=torch.int32).cuda())
+        k, v = (x[: rows // page * page].view(-1, page, heads, width) for x in (k, v))
+    else:
+        seqs = fs.prepare_block_sequences(block, offsets([0, tokens]), k_offsets=offsets([rows - length, length]))
+    out, lse = fs.flagsparse_block_attention(case.q, k, v, blocks, seqs, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    if page:
+        assert torch.equal(fs.flagsparse_block_means(k, seqs, 24), want_means)
+        return
+    grad = randn(case.q.shape, torch.bfloat16, 23)
+    want_grads = fs.flagsparse_block_attention_grad(grad, case.q, case.k, case.v, blocks, case.seqs, want, want_lse)
+    grads = fs.flagsparse_block_attention_grad(grad, case.q, k, v, blocks, seqs, out, lse)
+    assert torch.equal(grads[0], want_grads[0])
+    for got, of in zip(grads[1:], want_grads[1:]):
+        assert torch.equal(got[-length:], of)
+        assert not got[:-length].any()
+
+
+def test_one_sequence_of_millions_of_keys():
+    """Blocks at both ends of a sequence of 8.4 million keys; its blocks are selected by means."""
+    heads, width, block, n = 4, 128, 64, 131072 + 7
+    length = n * block - 9
+    k = torch.zeros((n * block, heads, width), dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    near = Case([3], [9 * block - 9], heads, 2, width, block, torch.bfloat16, 24)
+    k[:block], v[:block] = near.k[:block], near.v[:block]
+    k[length - near.rows + block : length], v[length - near.rows + block : length] = near.k[block:], near.v[block:]
+    k, v = k[:length], v[:length]
+    seqs = fs.prepare_block_sequences(block, offsets([3]), k_offsets=offsets([length]))
+    ids = torch.tensor([[0, 3, 5, 8], [0, 1, 7, 8], [0, 2, 4, 6]], dtype=torch.int32)[:, None].expand(3, heads, 4).contiguous().cuda()
+    far = torch.where(ids > 0, ids + (n - 9), ids)
+    want = fs.flagsparse_block_attention(near.q, near.k, near.v, ids, near.seqs)
+    assert torch.equal(fs.flagsparse_block_attention(near.q, k, v, far, seqs), want)
+    means = fs.flagsparse_block_means(k, seqs, n)
+    assert torch.equal(means[:, [0, *range(n - 8, n)]], fs.flagsparse_block_means(near.k, near.seqs, 9))
+    assert not means[:, 1 : n - 8].any()
+    got = fs.flagsparse_block_select(near.q, means, seqs, 6)
+    assert torch.equal(got, select_oracle(near.q, means, [0] * 3, [length - 3, length - 2, length - 1], block, 6, 1, 1))
