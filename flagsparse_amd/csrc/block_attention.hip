@@ -38,6 +38,11 @@ __device__ inline void start(Online<T, DP>& st) {
 // The maximum follows the scores only where it grows by more than this, in powers of
 // two: weights are 2^8 at most, and rescaling is left out of most steps.
 constexpr float kSlack = 8.0f;
+// float16's weights times 2^7, so up to 2^15: its last step is then 2^-32 of the weight
+// of the largest score instead of 2^-25, and the small weights of 131072 keys, the most
+// that a query selects, are not lost together.  Their sum has the factor too.
+template <class T>
+constexpr float kLift = std::is_same_v<T, _Float16> ? 7.0f : 0.0f;
 
 // One step's keys and values.
 template <class T, int DP, int AHEAD, class Wait>
@@ -81,7 +86,7 @@ __device__ inline void attend(Online<T, DP>& st, uint32_t kb, uint32_t vb, bool 
     for (int dt = 0; dt < DP / 16; ++dt) st.o[dt] *= by;
     st.m = m;
   }
-  const float base = st.m == -INFINITY ? 0.0f : st.m;
+  const float base = (st.m == -INFINITY ? 0.0f : st.m) - kLift<T>;
   float sum = 0.0f;
 #pragma unroll
   for (int gr = 0; gr < G; ++gr)
@@ -206,7 +211,7 @@ __global__ __launch_bounds__((ManyShape<T, DP>::kThreads)) void block_attention_
   const uint64_t rows = __ballot(bad && row.in);
   if (row.in) {
     store_row<T, DP>(static_cast<T*>(p.out) + at * p.width, st.o, by, p.width, lane);
-    if (p.lse != nullptr && lane < 16) p.lse[at] = l > 0.0f ? (st.m + __builtin_log2f(l)) * kLn2 : -INFINITY;
+    if (p.lse != nullptr && lane < 16) p.lse[at] = l > 0.0f ? (st.m - kLift<T> + __builtin_log2f(l)) * kLn2 : -INFINITY;
   }
   if (lane == 0)
     p.again[(int64_t)blockIdx.x * Shape::kReaders + w] = (uint32_t)(rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xffffu;
@@ -312,7 +317,7 @@ __device__ inline void join_rows(const BlockArgs& p, const FewPlace& f, int seq,
     }
     const int64_t at = (f.token * p.heads + f.head) * p.group + f.chunk * 16 + r;
     __builtin_memcpy(static_cast<T*>(p.out) + at * p.width + d, out, sizeof out);
-    if (p.lse != nullptr && d == 0) p.lse[at] = l > 0.0f ? (m + __builtin_log2f(l)) * kLn2 : -INFINITY;
+    if (p.lse != nullptr && d == 0) p.lse[at] = l > 0.0f ? (m - kLift<T> + __builtin_log2f(l)) * kLn2 : -INFINITY;
     if (bad) any = s_bad[r] = 1;
   }
   if (!__syncthreads_or(any)) return;
