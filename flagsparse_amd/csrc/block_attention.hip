@@ -45,9 +45,10 @@ template <class T>
 constexpr float kLift = std::is_same_v<T, _Float16> ? 7.0f : 0.0f;
 
 // One step's keys and values.
-template <class T, int DP, int AHEAD, class Wait>
+template <class T, int DP, int AHEAD, class Wait, class Done>
 __device__ inline void attend(Online<T, DP>& st, uint32_t kb, uint32_t vb, bool sel, int now, bool some,
-                              bool edge, uint32_t missing, const RowOf& row, float c, int used, int lane, Wait values) {
+                              bool edge, uint32_t missing, const RowOf& row, float c, int used, int lane, Wait values,
+                              Done done) {
   using R = Rows<T, DP>;
   constexpr int G = R::kGroups, P = R::kUnit / 16;
   f32x4 s[G];
@@ -97,12 +98,11 @@ __device__ inline void attend(Online<T, DP>& st, uint32_t kb, uint32_t vb, bool 
       s[gr][r] = x;
     }
   st.l += sum;
-  // weights in the values' type: off by half a unit in their last place each, the sum
-  // that they are divided by is not
-  typename R::frag w[G / P];
+  // weights in two parts of the values' type: together off by 2^-16 (float16: 2^-22) of each
+  typename R::Halves w[G / P];
 #pragma unroll
-  for (int u = 0; u < G / P; ++u) w[u] = R::rounded(&s[u * P]);
-  v.add(vb, w, st.o, used, lane);
+  for (int u = 0; u < G / P; ++u) w[u] = R::halves(&s[u * P]);
+  v.add(vb, w, st.o, used, lane, done);
 }
 
 // One row by a wave, key after key, without products of what is left out: a weight
@@ -199,8 +199,9 @@ __global__ __launch_bounds__((ManyShape<T, DP>::kThreads)) void block_attention_
   const int used = (p.width + 15) / 16;
   walk_blocks<T, DP, Shape, false>(p, t, row, mem, lds_address(&mem), tid, w, lane,
                             [&](int now, bool sel, bool some, bool edge, uint32_t missing, uint32_t kb,
-                                uint32_t vb, auto values) {
-                              attend<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, missing, row, c, used, lane, values);
+                                uint32_t vb, auto values, auto done) {
+                              attend<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, missing, row, c, used, lane, values,
+                                                           done);
                             });
   const float l = across_sum(st.l), by = l > 0.0f ? 1.0f / l : 0.0f;
   bool bad = !__builtin_isfinite(l);
@@ -403,7 +404,7 @@ __global__ __launch_bounds__((64 * FewShape<T, DP>::kWaves)) void block_attentio
     values.load(vb, v_place, lane);
     wait_loads<KeySource<T, DP>::kLoads>();
     attend<T, DP, 8>(st, kb, vb, row.in, now, true, edge || k_place.missing != 0, k_place.missing, row, c, used, lane,
-                  [] { wait_loads<0>(); });
+                  [] { wait_loads<0>(); }, [] {});
   }
   wait_reads();
   float* mine = reinterpret_cast<float*>(s_kv[w][0]);

@@ -233,8 +233,11 @@ __global__ __launch_bounds__((QueryGradShape<T, DP>::kThreads)) void block_query
   const float c = p.scale * kLog2e;
   const int used = (p.width + 15) / 16;
   walk_blocks<T, DP, Shape, false>(p, t, row, mem, lds_address(&mem), tid, w, lane,
-                            [&](int now, bool sel, bool some, bool edge, uint32_t, uint32_t kb, uint32_t vb,
-                                auto values) { take<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, row, c, factor, used, lane, values); });
+                            [&](int now, bool sel, bool some, bool edge, uint32_t, uint32_t kb, uint32_t vb, auto values,
+                                auto done) {
+                              take<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, row, c, factor, used, lane, values);
+                              done();
+                            });
   bool bad = false;
 #pragma unroll
   for (int dt = 0; dt < DP / 16; ++dt)

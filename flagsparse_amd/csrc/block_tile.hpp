@@ -197,6 +197,36 @@ struct Rows {
     }
     return f;
   }
+  // The same in two parts of 16 bits, the second what rounding to the first leaves out:
+  // 16 bits of a bfloat16 value and 22 of a float16 one, for 32-bit sums, instead of 8 and
+  // 11.  A product takes two instructions; the fragment of rows beside it is read once.
+  static constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
+  struct Halves {
+    frag part[kParts];
+  };
+  __device__ static Halves halves(const f32x4* s) {
+    Halves o;
+    o.part[0] = rounded(s);
+    if constexpr (kParts == 2) {
+      uint32_t pair[4];
+      __builtin_memcpy(pair, &o.part[0], 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // (from the pairs as they are: by elements the compiler rounds a second time)
+        float first, second;
+        if constexpr (std::is_same_v<T, __bf16>) {
+          first = __uint_as_float(pair[j] << 16);
+          second = __uint_as_float(pair[j] & 0xffff0000u);
+        } else {
+          first = (float)o.part[0][2 * j];
+          second = (float)o.part[0][2 * j + 1];
+        }
+        o.part[1][2 * j] = (T)(s[j >> 1][2 * (j & 1)] - first);
+        o.part[1][2 * j + 1] = (T)(s[j >> 1][2 * (j & 1) + 1] - second);
+      }
+    }
+    return o;
+  }
 };
 
 // Reads of LDS run ahead of the products that use them, AHEAD fragments at a time:
@@ -257,6 +287,26 @@ struct Columns {
         const int at = first + i;
         if (!leave_out<T>(at % (DP / 16), used))
           o[at % (DP / 16)] = Mma<T>::run(x[i], w[at / (DP / 16)], o[at % (DP / 16)]);
+      }
+    }
+  }
+  // The same with w in parts; done() once all is read, before the last products: nobody
+  // waits for those.
+  template <class Done>
+  __device__ void add(uint32_t lds, const typename R::Halves (&w)[kUnits], f32x4 (&o)[DP / 16], int used, int lane,
+                      Done done) {
+#pragma unroll
+    for (int first = 0; first < kAll; first += kStep) {
+      if (first > 0) read(lds, first, used, lane);
+      if (first + kStep == kAll) done();
+#pragma unroll
+      for (int n = 0; n < R::kParts; ++n) {
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) {
+          const int at = first + i;
+          if (!leave_out<T>(at % (DP / 16), used))
+            o[at % (DP / 16)] = Mma<T>::run(x[i], w[at / (DP / 16)].part[n], o[at % (DP / 16)]);
+        }
       }
     }
   }

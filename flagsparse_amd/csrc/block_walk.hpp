@@ -97,7 +97,8 @@ __device__ inline void walk_start(typename Shape::Memory& mem, int tid) {
   if (tid < Shape::kSlots) mem.ready[0][tid] = mem.ready[1][tid] = mem.done[tid] = 0u;
 }
 
-// The walk of a wave that loads (LOADS) or reads: body(...) takes a step.  Both kinds
+// The walk of a wave that loads (LOADS) or reads: body(...) takes a step, calls values()
+// before it reads the values and done() once, when it has read all.  Both kinds
 // meet at the same barriers; each has code of its own, so that a loader's holds no rows.
 template <class T, int DP, class Shape, bool LOADS, class Body>
 __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const RowOf& row, typename Shape::Memory& mem,
@@ -266,15 +267,20 @@ __device__ inline void walk_blocks(const BlockArgs& p, const WalkTile& t, const 
             while (look(ready0 + 4 * i) != step + 1) __builtin_amdgcn_s_sleep(1);
             in_order();
             const uint32_t missing = p.seqs.pages != nullptr ? look(missing0 + 4 * i) : 0u;
-            body(now, sel, some, edge || missing != 0, missing, kv0 + 2 * i * Shape::kBytes,
-                 kv0 + (2 * i + 1) * Shape::kBytes, [&] {
-                   while (look(ready0 + 4 * (S + i)) != step + 1) __builtin_amdgcn_s_sleep(1);
-                   in_order();
-                 });
-            wait_reads();
-            if (lane == 0)
-              __hip_atomic_fetch_add((lds_word*)(uintptr_t)(done0 + 4 * i), 1u, __ATOMIC_RELAXED,
-                                     __HIP_MEMORY_SCOPE_WORKGROUP);
+            body(
+                now, sel, some, edge || missing != 0, missing, kv0 + 2 * i * Shape::kBytes,
+                kv0 + (2 * i + 1) * Shape::kBytes,
+                [&] {
+                  while (look(ready0 + 4 * (S + i)) != step + 1) __builtin_amdgcn_s_sleep(1);
+                  in_order();
+                },
+                [&] {
+                  wait_reads();
+                  if (lane == 0)
+                    __hip_atomic_fetch_add((lds_word*)(uintptr_t)(done0 + 4 * i), 1u, __ATOMIC_RELAXED,
+                                           __HIP_MEMORY_SCOPE_WORKGROUP);
+                  in_order();
+                });
           }
         }
       }

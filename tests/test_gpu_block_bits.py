@@ -8,9 +8,31 @@ import torch
 
 import flagsparse_amd as fs
 
-from ._blocks_helpers import BLOCK_DTYPES, BLOCK_IDS, Case
+from ._blocks_bounds import attention_bounds, worst
+from ._blocks_helpers import BLOCK_DTYPES, BLOCK_IDS, Case, random_blocks
 
 pytestmark = pytest.mark.gpu
+
+SIZES = [
+    # new, lengths, heads, group, width, block, top, page
+    ([5, 3], [700, 65], 2, 4, 64, 32, 4, 0),
+    ([1, 1], [90, 300], 2, 16, 128, 64, 2, 16),
+    ([4], [90], 1, 3, 32, 32, 2, 0),
+    ([1100], [1150], 4, 3, 32, 32, 2, 0),
+    ([600, 450], [600, 700], 4, 8, 128, 64, 2, 16),
+    ([1030], [1030], 4, 2, 64, 32, 5, 32),
+]
+
+
+@pytest.mark.parametrize("dtype", BLOCK_DTYPES, ids=BLOCK_IDS)
+@pytest.mark.parametrize("sizes", SIZES, ids=["x".join(map(str, c[2:])) for c in SIZES])
+def test_weights_keep_their_bits(sizes, dtype):
+    new, lengths, heads, group, width, block, top, page = sizes
+    case = Case(new, lengths, heads, group, width, block, dtype, 90, page)
+    blocks = random_blocks(new, lengths, heads, top, block, 91)
+    got = fs.flagsparse_block_attention(case.q, case.k, case.v, blocks, case.seqs)
+    off = worst(got, *attention_bounds(case, blocks, width**-0.5))
+    assert off <= 1.0, f"{off} times the bound"
 
 
 @pytest.mark.parametrize("dtype", BLOCK_DTYPES, ids=BLOCK_IDS)
