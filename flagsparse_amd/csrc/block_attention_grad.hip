@@ -22,50 +22,37 @@
 namespace fs {
 namespace {
 
-constexpr int kAmaxParts = 256;
-
 // Waves that read, of the queries' gradient, by the bytes of a row.
 constexpr int query_readers(int row) { return row <= 128 ? 12 : row <= 256 ? 8 : 6; }
 
-// dS of 16-bit floats, whose small values have few bits: G and <G, O> are multiplied
-// by the power of two that brings G's largest value to [1, 2), and the gradients
-// divided by it in 32 bits.  (bfloat16 and float32 have the exponents.)
+// dS of float16, whose small values have few bits, times a power of two: of a query's
+// own in its gradient, of a key's own in the key's.  It follows the largest value so far,
+// as the softmax's maximum does, and keeps it between 2^8 and 2^15; what is summed up is
+// scaled again where it changes, and the gradients are divided by it in 32 bits.  So
+// neither rows whose gradient is small beside others' nor small weights lose bits.
+// (bfloat16 and float32 have the exponents.)
 template <class T>
 constexpr bool kFactored = std::is_same_v<T, _Float16>;
+constexpr float kFirstFactor = 0x1p100f;
 
-__device__ inline float factor_of(float most) {
-  const uint32_t e = (__float_as_uint(most) >> 23) & 255u;
-  return e == 0u || e >= 254u ? 1.0f : __uint_as_float((254u - e) << 23);
+// `most`: the largest value of a step, of the lane's query or key.  Not finite: the sum
+// will not be either, whatever the factor.
+template <int N>
+__device__ inline void follow(float most, float& factor, f32x4 (&sum)[N]) {
+  const bool grown = most * factor > 0x1p15f && most < INFINITY;
+  if (__ballot(grown) == 0) return;
+  const int at = (int)((__float_as_uint(factor) >> 23) & 255u);
+  const int to = grown ? 262 - (int)((__float_as_uint(most) >> 23) & 255u) : at;  // most: [2^8, 2^9)
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sum[n][r] = __builtin_amdgcn_ldexpf(sum[n][r], to - at);
+  factor = __uint_as_float((uint32_t)to << 23);
 }
+
+// P of float16 in the values' gradient: times 2^15, at most.
 template <class T>
-__device__ inline float read_factor(const float* parts, int lane) {
-  if constexpr (!kFactored<T>) {
-    return 1.0f;
-  } else {
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kAmaxParts / 64; ++i) m = fmaxf(m, parts[i * 64 + lane]);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-    return factor_of(m);
-  }
-}
-
-// One of kAmaxParts workgroups' largest value of n, a multiple of 8.
-__device__ inline void amax_part(const _Float16* x, int64_t n, float* parts, uint32_t block) {
-  __shared__ float s_max[4];
-  float m = 0.0f;
-  for (int64_t at = ((int64_t)block * 256 + threadIdx.x) * 8; at < n; at += (int64_t)kAmaxParts * 256 * 8) {
-    const Slice<_Float16> v = load_slice(x + at);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf((float)v.v[e]));
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-  if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) parts[block] = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-}
+constexpr float kWeightLift = std::is_same_v<T, _Float16> ? 15.0f : 0.0f;
 
 // ---- gradient of the queries ------------------------------------------------------
 
@@ -73,12 +60,13 @@ template <class T, int DP>
 struct QueryGrad {
   typename Mma<T>::frag q[Rows<T, DP>::kFrags], g[Rows<T, DP>::kFrags];
   f32x4 d[DP / 16];
-  float lse, delta;  // in powers of two; times the factor
+  float lse, delta;  // in powers of two; <G, O>
+  float factor;
 };
 
 template <class T, int DP, int AHEAD, class Wait>
 __device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, bool sel, int now, bool some,
-                            bool edge, const RowOf& row, float c, float factor, int used, int lane, Wait values) {
+                            bool edge, const RowOf& row, float c, int used, int lane, Wait values) {
   using R = Rows<T, DP>;
   constexpr int G = R::kGroups, P = R::kUnit / 16;
   f32x4 s[G], dp[G];
@@ -94,7 +82,7 @@ __device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, bool
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[gr][r], c, -st.lse));
-      s[gr][r] = x * __builtin_fmaf(dp[gr][r], factor, -st.delta);
+      s[gr][r] = x * (dp[gr][r] - st.delta);
     }
   if (edge) {
 #pragma unroll
@@ -110,6 +98,16 @@ __device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, bool
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[gr][r] = sel ? s[gr][r] : 0.0f;
   }
+  if constexpr (kFactored<T>) {
+    float most = 0.0f;
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(s[gr][r]));
+    follow(across_max(most), st.factor, st.d);
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr) s[gr] *= st.factor;
+  }
   // (dS in the values' type, rounded once)
   typename R::frag w[G / P];
 #pragma unroll
@@ -123,7 +121,6 @@ struct GradArgs {
   const void* o;
   const float* lse;
   float* delta;        // <G, O> of each row
-  const float* amax;   // float16
   const int32_t* order;
   const int4* pieces;  // key, first entry, one behind the last, place of its sums or -1
   const int32_t* n_pieces;
@@ -208,8 +205,8 @@ __global__ __launch_bounds__((QueryGradShape<T, DP>::kThreads)) void block_query
     return;
   }
   const RowOf row = row_of(p, t, w, lane);
-  const float factor = read_factor<T>(a.amax, lane);
   QueryGrad<T, DP> st;
+  st.factor = kFactored<T> ? kFirstFactor : 1.0f;
   const int hq = t.head * p.group + row.head;
   const int64_t at = (int64_t)(t.token0 + row.token) * p.heads * p.group + hq;
   load_row<T, DP>(static_cast<const T*>(p.q) + (int64_t)(t.token0 + row.token) * p.q_token + (int64_t)hq * p.q_head,
@@ -225,7 +222,7 @@ __global__ __launch_bounds__((QueryGradShape<T, DP>::kThreads)) void block_query
       for (int e = 0; e < 16 / (int)sizeof(T); ++e) sum = __builtin_fmaf((float)st.g[ks][e], (float)o[ks][e], sum);
     sum = across_sum(sum);
     if (row.in && lane < 16) a.delta[at] = sum;
-    st.delta = sum * factor;
+    st.delta = sum;
     st.lse = row.in ? a.lse[at] * kLog2e : 0.0f;
   }
 #pragma unroll
@@ -235,7 +232,7 @@ __global__ __launch_bounds__((QueryGradShape<T, DP>::kThreads)) void block_query
   walk_blocks<T, DP, Shape, false>(p, t, row, mem, lds_address(&mem), tid, w, lane,
                             [&](int now, bool sel, bool some, bool edge, uint32_t, uint32_t kb, uint32_t vb, auto values,
                                 auto done) {
-                              take<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, row, c, factor, used, lane, values);
+                              take<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, row, c, used, lane, values);
                               done();
                             });
   bool bad = false;
@@ -244,7 +241,7 @@ __global__ __launch_bounds__((QueryGradShape<T, DP>::kThreads)) void block_query
 #pragma unroll
     for (int r = 0; r < 4; ++r) bad |= !__builtin_isfinite(st.d[dt][r]);
   const uint64_t rows = __ballot(bad && row.in);
-  if (row.in) store_row<T, DP>(static_cast<T*>(p.out) + at * p.width, st.d, p.scale / factor, p.width, lane);
+  if (row.in) store_row<T, DP>(static_cast<T*>(p.out) + at * p.width, st.d, p.scale / st.factor, p.width, lane);
   if (lane == 0)
     p.again[(int64_t)blockIdx.x * Shape::kReaders + w] = (uint32_t)(rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xffffu;
 }
@@ -278,12 +275,9 @@ __device__ inline int first_block(const fs_block_seqs& s, int b, int lg_block) {
 
 // The key that each entry of the selection is sorted by, head by head and block by
 // block; one too large for entries that name nothing or the same block again.  A
-// wave takes a token.  Also zeros the gradients of rows of no sequence and, of float16,
-// finds the largest value of the gradient.
+// wave takes a token.  Also zeros the gradients of rows of no sequence.
 __global__ __launch_bounds__(256) void block_keys_kernel(const BlockArgs p, int lists, int key_blocks, int32_t* keys,
-                                                         uint32_t* dk, uint32_t* dv, int64_t row_words,
-                                                         const _Float16* grad, int64_t values, float* amax) {
-  if (grad != nullptr && blockIdx.x < kAmaxParts) amax_part(grad, values, amax, blockIdx.x);
+                                                         uint32_t* dk, uint32_t* dv, int64_t row_words) {
   const int lane = threadIdx.x & 63, lg = p.lg_groups + 4;
   const int64_t waves = (int64_t)gridDim.x * 4, first = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int n_keys = lists * key_blocks;
@@ -537,7 +531,9 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
   for (int n = 0; n < KT; ++n)
 #pragma unroll
     for (int dt = 0; dt < DP / 16; ++dt) dk[n][dt] = dv[n][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const float factor = read_factor<T>(a.amax, lane);
+  float factor[KT];  // of the lane's keys
+#pragma unroll
+  for (int n = 0; n < KT; ++n) factor[n] = kFactored<T> ? kFirstFactor : 1.0f;
   const float c = p.scale * kLog2e;
   const int offset = o.sq.keys - o.sq.count - o.sq.first;  // of positions from tokens
   __syncthreads();
@@ -584,8 +580,8 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
   for (int s = 0; s < steps; ++s) {
     RowStats& stats = s_stats[s & 1];
     if (tid < STEP) {
-      stats.lse[tid] = n_lse * kLog2e;
-      stats.delta[tid] = n_delta * factor;
+      stats.lse[tid] = n_lse * kLog2e - kWeightLift<T>;
+      stats.delta[tid] = n_delta;
       stats.pos[tid] = n_pos;
     }
     wait_loads<0>();
@@ -631,10 +627,23 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
           // end before every key)
           const bool in = j <= row_pos[r];
           const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(x[m][n][r], c, -lse[r]));
-          const float v = u * __builtin_fmaf(y[m][n][r], factor, -delta[r]);
+          const float v = u * (y[m][n][r] - delta[r]);
           wx[n][m][r] = in ? u : 0.0f;
           wy[n][m][r] = in ? v : 0.0f;
         }
+      }
+    }
+    if constexpr (kFactored<T>) {
+#pragma unroll
+      for (int n = 0; n < KT; ++n) {
+        float most = 0.0f;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(wy[n][m][r]));
+        follow(across_max(most), factor[n], dk[n]);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) wy[n][m] *= factor[n];
       }
     }
     // (P and dS in the values' type, each rounded once)
@@ -657,6 +666,17 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
           dv[n][dt] = Mma<T>::run(g, pf[n][u], dv[n][dt]);
           dk[n][dt] = Mma<T>::run(q, sf[n][u], dk[n][dt]);
         }
+      }
+  }
+  if constexpr (kFactored<T>) {
+    constexpr float kDown = 0x1p-15f;
+    static_assert(kWeightLift<T> == 15.0f);
+#pragma unroll
+    for (int n = 0; n < KT; ++n)
+#pragma unroll
+      for (int dt = 0; dt < DP / 16; ++dt) {
+        dk[n][dt] *= kDown / factor[n];
+        dv[n][dt] *= kDown;
       }
   }
   // sums of the waves over the rows
@@ -701,7 +721,6 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
   __syncthreads();
   const bool again = s_bad != 0;
   const int64_t place_of = piece.w >= 0 ? ((int64_t)piece.w * shared + copy) * p.seqs.block + part * BK : 0;
-  const float by = p.scale / factor;
   if (!again) {
     if (rw == 0) {
 #pragma unroll
@@ -711,12 +730,12 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
           float* sums = a.parts + (place_of + jj) * 2 * DP;
 #pragma unroll
           for (int dt = 0; dt < DP / 16; ++dt) {
-            *reinterpret_cast<f32x4*>(sums + dt * 16 + (lane >> 4) * 4) = dk[n][dt] * by;
+            *reinterpret_cast<f32x4*>(sums + dt * 16 + (lane >> 4) * 4) = dk[n][dt] * p.scale;
             *reinterpret_cast<f32x4*>(sums + DP + dt * 16 + (lane >> 4) * 4) = dv[n][dt];
           }
         } else if (j < o.sq.keys) {
           const int64_t row = ((o.sq.row0 + j) * p.heads + o.head) * p.width;
-          store_row<T, DP>(static_cast<T*>(a.dk) + row, dk[n], by, p.width, lane);
+          store_row<T, DP>(static_cast<T*>(a.dk) + row, dk[n], p.scale, p.width, lane);
           store_row<T, DP>(static_cast<T*>(a.dv) + row, dv[n], 1.0f, p.width, lane);
         }
       }
@@ -802,7 +821,7 @@ struct GradPlan {
   int most;                // entries a piece
   int per;                 // tokens a workgroup of the queries' gradient
   int64_t tiles;
-  size_t again, sort, keys, sorted, order, starts, list, sums, count, delta, amax, parts, bytes;
+  size_t again, sort, keys, sorted, order, starts, list, sums, count, delta, parts, bytes;
 };
 GradPlan grad_plan(int val_t, const fs_block_seqs& s, int heads, int group, int lists, int width, int top) {
   GradPlan l{};
@@ -839,7 +858,6 @@ GradPlan grad_plan(int val_t, const fs_block_seqs& s, int heads, int group, int 
   l.sums = take((size_t)l.n_keys * 8);
   l.count = take(4);
   l.delta = take((size_t)tokens * heads * group * 4);
-  l.amax = take(kAmaxParts * 4);
   l.parts = take((size_t)(l.places * shared) * block * 2 * dp * 4);
   l.bytes = at;
   return l;
@@ -913,8 +931,6 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
   a.o = out;
   a.lse = lse;
   a.delta = reinterpret_cast<float*>(m + l.delta);
-  float* amax = reinterpret_cast<float*>(m + l.amax);
-  a.amax = amax;
   a.order = reinterpret_cast<int32_t*>(m + l.order);
   a.pieces = reinterpret_cast<int4*>(m + l.list);
   a.n_pieces = reinterpret_cast<int32_t*>(m + l.count);
@@ -929,12 +945,9 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
   uint32_t* sorted = reinterpret_cast<uint32_t*>(m + l.sorted);
   int32_t* starts = reinterpret_cast<int32_t*>(m + l.starts);
 
-  const bool factored = val_t == FS_F16 && tokens > 0;
   const int64_t key_groups = std::min<int64_t>(ceil_div(std::max<int64_t>(tokens, 4), 4), 4096);
-  hipLaunchKernelGGL(block_keys_kernel, dim3((uint32_t)(factored ? std::max<int64_t>(key_groups, kAmaxParts) : key_groups)),
-                     dim3(256), 0, stream, p, lists, (int)l.key_blocks, keys, static_cast<uint32_t*>(dk),
-                     static_cast<uint32_t*>(dv), (int64_t)heads * width * size / 4,
-                     factored ? static_cast<const _Float16*>(grad) : nullptr, tokens * heads * group * width, amax);
+  hipLaunchKernelGGL(block_keys_kernel, dim3((uint32_t)key_groups), dim3(256), 0, stream, p, lists, (int)l.key_blocks, keys,
+                     static_cast<uint32_t*>(dk), static_cast<uint32_t*>(dv), (int64_t)heads * width * size / 4);
   FS_CHECK_LAUNCH("block_keys_kernel");
   if (l.entries > 0) {
     if (const int rc = select_sort(keys, FS_I32, l.entries, l.n_keys, sorted, reinterpret_cast<int32_t*>(m + l.order),

@@ -8,10 +8,12 @@ import torch
 
 import flagsparse_amd as fs
 
-from ._blocks_bounds import attention_bounds, worst
-from ._blocks_helpers import BLOCK_DTYPES, BLOCK_IDS, Case, random_blocks
+from ._blocks_bounds import attention_bounds, gradient_bounds, worst
+from ._blocks_helpers import BLOCK_DTYPES, BLOCK_IDS, Case, random_blocks, randn
+from ._rows_helpers import UNIT
 
 pytestmark = pytest.mark.gpu
+INF = float("inf")
 
 SIZES = [
     # new, lengths, heads, group, width, block, top, page
@@ -57,3 +59,52 @@ def test_many_small_weights_add_up(tokens, dtype):
     # scores off by some 2^-24 of 26, sums of 8192 terms, one rounding, float16's last step
     bound = want * (2.0**-16 + 2 * 8192 * 2.0**-24) + torch.finfo(dtype).eps / 2 * want + 2.0**-25
     assert float((got.double() - want).abs().max()) <= bound
+
+
+def _gradients(case, blocks, grad):
+    out, lse = fs.flagsparse_block_attention(case.q, case.k, case.v, blocks, case.seqs, return_lse=True)
+    return out, lse, fs.flagsparse_block_attention_grad(grad, case.q, case.k, case.v, blocks, case.seqs, out, lse)
+
+
+@pytest.mark.parametrize("tokens", [90, 700])
+@pytest.mark.parametrize("large", [2.0**13, INF, float("nan")], ids=["2^13", "inf", "nan"])
+@pytest.mark.parametrize("dtype", BLOCK_DTYPES, ids=BLOCK_IDS)
+def test_small_gradients_beside_large_ones(dtype, large, tokens):
+    """Gradients of 2^-13 beside a row 2^26 times as large, or one that is not finite: what
+    that row has no part in keeps its bits."""
+    case = Case([tokens], [tokens], 2, 2, 64, 32, dtype, 96)
+    blocks = random_blocks([tokens], [tokens], 2, 2, 32, 97)
+    grad = randn(case.q.shape, dtype, 98) * 2.0**-13
+    row = tokens - 20
+    grad[row] = randn(case.q.shape[1:], dtype, 99) * (large if large < INF else 1.0)
+    shown = grad.clone()
+    if not large < INF:
+        grad[row] = large
+    out, lse, got = _gradients(case, blocks, grad)
+    found = gradient_bounds(case, blocks, 64**-0.5, shown, out, lse, UNIT[dtype])
+    reached = case.seen(blocks)[:, row].t()[:, :, None].expand(case.packed_k.shape)
+    rows = torch.arange(tokens, device="cuda") == row
+    off = {}
+    for t, name, apart in zip(got, ("dq", "dk", "dv"), (rows, reached, reached)):
+        want, bound = found[name]
+        if not large < INF:
+            assert not torch.isfinite(t[apart]).any()
+            t, want, bound = t[~apart], want[~apart], bound[~apart]
+        off[name] = worst(t, want, bound)
+    assert max(off.values()) <= 1.0, off
+
+
+@pytest.mark.parametrize("size", [2.0**-14, 1.0, 2.0**13])
+@pytest.mark.parametrize("width", [64, 128])
+def test_float16_gradients_of_small_weights(width, size):
+    """Scores that differ by 60 and more: weights down to 2^-90, and gradients of scores
+    that grow from step to step."""
+    case = Case([200], [200], 2, 2, width, 32, torch.float16, 100)
+    case.q *= 4.0
+    case.packed_k *= torch.linspace(0.0, 3.0, 200, device="cuda")[:, None, None].half()
+    blocks = random_blocks([200], [200], 2, 4, 32, 101)
+    grad = randn(case.q.shape, torch.float16, 102) * size
+    out, lse, got = _gradients(case, blocks, grad)
+    found = gradient_bounds(case, blocks, width**-0.5, grad, out, lse, UNIT[torch.float16])
+    off = {name: worst(t, *found[name]) for t, name in zip(got, ("dq", "dk", "dv"))}
+    assert max(off.values()) <= 1.0, off
