@@ -64,9 +64,9 @@ struct QueryGrad {
   float factor;
 };
 
-template <class T, int DP, int AHEAD, class Wait>
+template <class T, int DP, int AHEAD, class Wait, class Done>
 __device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, bool sel, int now, bool some,
-                            bool edge, const RowOf& row, float c, int used, int lane, Wait values) {
+                            bool edge, const RowOf& row, float c, int used, int lane, Wait values, Done done) {
   using R = Rows<T, DP>;
   constexpr int G = R::kGroups, P = R::kUnit / 16;
   f32x4 s[G], dp[G];
@@ -108,11 +108,11 @@ __device__ inline void take(QueryGrad<T, DP>& st, uint32_t kb, uint32_t vb, bool
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) s[gr] *= st.factor;
   }
-  // (dS in the values' type, rounded once)
-  typename R::frag w[G / P];
+  // dS in two parts of the values' type, as the forward pass's weights
+  typename R::Halves w[G / P];
 #pragma unroll
-  for (int u = 0; u < G / P; ++u) w[u] = R::rounded(&s[u * P]);
-  k.add(kb, w, st.d, used, lane);
+  for (int u = 0; u < G / P; ++u) w[u] = R::halves(&s[u * P]);
+  k.add(kb, w, st.d, used, lane, done);
 }
 
 struct GradArgs {
@@ -232,8 +232,8 @@ __global__ __launch_bounds__((QueryGradShape<T, DP>::kThreads)) void block_query
   walk_blocks<T, DP, Shape, false>(p, t, row, mem, lds_address(&mem), tid, w, lane,
                             [&](int now, bool sel, bool some, bool edge, uint32_t, uint32_t kb, uint32_t vb, auto values,
                                 auto done) {
-                              take<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, row, c, used, lane, values);
-                              done();
+                              take<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, row, c, used, lane, values,
+                                                         done);
                             });
   bool bad = false;
 #pragma unroll
@@ -609,7 +609,7 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
         }
       }
     }
-    typename R::frag pf[KT][2 / P], sf[KT][2 / P];
+    typename R::Halves pf[KT][2 / P], sf[KT][2 / P];
     f32x4 wx[KT][2], wy[KT][2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -646,13 +646,13 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
         for (int m = 0; m < 2; ++m) wy[n][m] *= factor[n];
       }
     }
-    // (P and dS in the values' type, each rounded once)
+    // P and dS in two parts of the values' type
 #pragma unroll
     for (int n = 0; n < KT; ++n)
 #pragma unroll
       for (int u = 0; u < 2 / P; ++u) {
-        pf[n][u] = R::rounded(&wx[n][u * P]);
-        sf[n][u] = R::rounded(&wy[n][u * P]);
+        pf[n][u] = R::halves(&wx[n][u * P]);
+        sf[n][u] = R::halves(&wy[n][u * P]);
       }
 #pragma unroll
     for (int u = 0; u < 2 / P; ++u)
@@ -662,10 +662,12 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
         const auto g = R::down(gb, u * R::kUnit, dt, lane);
         const auto q = R::down(qb, u * R::kUnit, dt, lane);
 #pragma unroll
-        for (int n = 0; n < KT; ++n) {
-          dv[n][dt] = Mma<T>::run(g, pf[n][u], dv[n][dt]);
-          dk[n][dt] = Mma<T>::run(q, sf[n][u], dk[n][dt]);
-        }
+        for (int i = 0; i < R::kParts; ++i)
+#pragma unroll
+          for (int n = 0; n < KT; ++n) {
+            dv[n][dt] = Mma<T>::run(g, pf[n][u].part[i], dv[n][dt]);
+            dk[n][dt] = Mma<T>::run(q, sf[n][u].part[i], dk[n][dt]);
+          }
       }
   }
   if constexpr (kFactored<T>) {

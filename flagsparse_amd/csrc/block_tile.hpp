@@ -276,22 +276,8 @@ struct Columns {
     }
     fence();
   }
-  // o[dt] += columns times w, after read(lds, 0): what is left is read here.
-  __device__ void add(uint32_t lds, const typename R::frag (&w)[kUnits], f32x4 (&o)[DP / 16], int used,
-                      int lane) {
-#pragma unroll
-    for (int first = 0; first < kAll; first += kStep) {
-      if (first > 0) read(lds, first, used, lane);
-#pragma unroll
-      for (int i = 0; i < kStep; ++i) {
-        const int at = first + i;
-        if (!leave_out<T>(at % (DP / 16), used))
-          o[at % (DP / 16)] = Mma<T>::run(x[i], w[at / (DP / 16)], o[at % (DP / 16)]);
-      }
-    }
-  }
-  // The same with w in parts; done() once all is read, before the last products: nobody
-  // waits for those.
+  // o[dt] += columns times w, after read(lds, 0): what is left is read here.  done() once
+  // all is read, before the last products: nobody waits for those.
   template <class Done>
   __device__ void add(uint32_t lds, const typename R::Halves (&w)[kUnits], f32x4 (&o)[DP / 16], int used, int lane,
                       Done done) {

@@ -1,5 +1,5 @@
-"""Bounds of the operators over blocks as near as 32-bit arithmetic comes: weights
-keep the bits of two 16-bit parts, so that what a 16-bit result is
+"""Bounds of the operators over blocks as near as 32-bit arithmetic comes: weights and
+gradients of scores keep the bits of two 16-bit parts, so that what a 16-bit result is
 off by is its own rounding, next to which the rest is small."""
 
 import math
@@ -62,12 +62,12 @@ def attention_bounds(case, blocks, scale):
     return x.by_token(out), x.by_token(err + u * (out.abs() + err) + TINY[case.dtype])
 
 
-def gradient_bounds(case, blocks, scale, grad, out, lse, parts=None):
+def gradient_bounds(case, blocks, scale, grad, out, lse):
     """{name: (gradient in 64 bits, bound)} of the call with these results of the forward
-    pass, as they were rounded.  `parts`: what weights and gradients of scores are off by."""
+    pass, as they were rounded."""
     x = _Pairs(case, blocks, scale)
     dtype = case.dtype
-    u, parts = UNIT[dtype], _parts(dtype) if parts is None else parts
+    u, parts = UNIT[dtype], _parts(dtype)
     g, o = x.by_head(grad), x.by_head(out)
     lse = lse.double().view(x.T, x.H, x.G).permute(1, 2, 0)[..., None]
     shown = torch.where(torch.isinf(lse), 0.0, lse)

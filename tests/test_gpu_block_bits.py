@@ -10,7 +10,6 @@ import flagsparse_amd as fs
 
 from ._blocks_bounds import attention_bounds, gradient_bounds, worst
 from ._blocks_helpers import BLOCK_DTYPES, BLOCK_IDS, Case, random_blocks, randn
-from ._rows_helpers import UNIT
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -66,6 +65,28 @@ def _gradients(case, blocks, grad):
     return out, lse, fs.flagsparse_block_attention_grad(grad, case.q, case.k, case.v, blocks, case.seqs, out, lse)
 
 
+GRAD = [
+    # new, lengths, heads, group, width, block, top
+    ([90], [90], 2, 2, 32, 32, 2),
+    ([70, 0, 30], [70, 0, 45], 2, 3, 64, 64, 1),
+    ([100], [180], 1, 4, 128, 64, 2),
+    ([129, 40], [129, 40], 2, 1, 80, 32, 3),
+]
+
+
+@pytest.mark.parametrize("dtype", BLOCK_DTYPES, ids=BLOCK_IDS)
+@pytest.mark.parametrize("sizes", GRAD, ids=["x".join(map(str, c[2:])) for c in GRAD])
+def test_gradients_keep_their_bits(sizes, dtype):
+    new, lengths, heads, group, width, block, top = sizes
+    case = Case(new, lengths, heads, group, width, block, dtype, 93)
+    blocks = random_blocks(new, lengths, heads, top, block, 94)
+    grad = randn(case.q.shape, dtype, 95)
+    out, lse, got = _gradients(case, blocks, grad)
+    found = gradient_bounds(case, blocks, width**-0.5, grad, out, lse)
+    off = {name: worst(t, *found[name]) for t, name in zip(got, ("dq", "dk", "dv"))}
+    assert max(off.values()) <= 1.0, off
+
+
 @pytest.mark.parametrize("tokens", [90, 700])
 @pytest.mark.parametrize("large", [2.0**13, INF, float("nan")], ids=["2^13", "inf", "nan"])
 @pytest.mark.parametrize("dtype", BLOCK_DTYPES, ids=BLOCK_IDS)
@@ -81,7 +102,7 @@ def test_small_gradients_beside_large_ones(dtype, large, tokens):
     if not large < INF:
         grad[row] = large
     out, lse, got = _gradients(case, blocks, grad)
-    found = gradient_bounds(case, blocks, 64**-0.5, shown, out, lse, UNIT[dtype])
+    found = gradient_bounds(case, blocks, 64**-0.5, shown, out, lse)
     reached = case.seen(blocks)[:, row].t()[:, :, None].expand(case.packed_k.shape)
     rows = torch.arange(tokens, device="cuda") == row
     off = {}
@@ -105,6 +126,6 @@ def test_float16_gradients_of_small_weights(width, size):
     blocks = random_blocks([200], [200], 2, 4, 32, 101)
     grad = randn(case.q.shape, torch.float16, 102) * size
     out, lse, got = _gradients(case, blocks, grad)
-    found = gradient_bounds(case, blocks, width**-0.5, grad, out, lse, UNIT[torch.float16])
+    found = gradient_bounds(case, blocks, width**-0.5, grad, out, lse)
     off = {name: worst(t, *found[name]) for t, name in zip(got, ("dq", "dk", "dv"))}
     assert max(off.values()) <= 1.0, off
