@@ -419,9 +419,10 @@ def flagsparse_block_attention(q, k, v, blocks, seqs, scale=None, out=None, retu
     (T, 1, top) for all heads alike, names blocks of the query's sequence: one
     named twice counts once, a negative one or one behind the query's own not at
     all.  Within its blocks a query sees the keys up to its own position; one that
-    sees none gets zeros.  scale is width ** -0.5 unless given.  With return_lse
-    also the logarithm of the sum of the exponentials, (T, heads * group) float32,
-    minus infinity without keys; it carries no gradient.
+    sees none gets zeros, one whose scores are all minus infinity not-a-numbers.
+    scale is width ** -0.5 unless given.  With return_lse also the logarithm of the
+    sum of the exponentials, (T, heads * group) float32, minus infinity for both; it
+    carries no gradient.
 
     Differentiable in q, k and v of packed rows.
     """

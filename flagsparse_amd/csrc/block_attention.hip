@@ -107,7 +107,8 @@ __device__ inline void attend(Online<T, DP>& st, uint32_t kb, uint32_t vb, bool 
 
 // One row by a wave, key after key, without products of what is left out: a weight
 // of zero times a value that is not finite would be NaN.  Taken where a result is
-// not finite, whoever's it is.
+// not finite, whoever's it is, and where a sum of weights is zero: of a row without keys,
+// which is zero, or of one whose scores are all minus infinity, which is not a number.
 template <class T, int DP>
 __device__ __forceinline__ void careful_row(const BlockArgs& p, const Sequence& sq, int seq, int64_t token, int head,
                                          int in_group, int pos, int lane) {
@@ -115,6 +116,7 @@ __device__ __forceinline__ void careful_row(const BlockArgs& p, const Sequence& 
   const T* q = static_cast<const T*>(p.q) + token * p.q_token + (int64_t)hq * p.q_head;
   const int32_t* ids = p.blocks + token * p.b_token + (int64_t)head * p.b_head;
   const float c = p.scale * kLog2e;
+  bool any = false;  // key is seen
   float m = -INFINITY, l = 0.0f, o[(DP + 63) / 64];
 #pragma unroll
   for (int i = 0; i < (DP + 63) / 64; ++i) o[i] = 0.0f;
@@ -122,7 +124,7 @@ __device__ __forceinline__ void careful_row(const BlockArgs& p, const Sequence& 
     for (int e = 0; e < p.top; ++e) {
       const int id = ids[e];
       bool use = id >= 0 && id <= (pos >> lg);
-      for (int b = 0; b < e; ++b) use = use && ids[b] != id;
+      for (int b = 0; use && b < e; ++b) use = ids[b] != id;
       if (!use) continue;
       for (int j0 = 0; j0 < block; j0 += 64) {
         const int j = id * block + j0 + lane;
@@ -138,6 +140,7 @@ __device__ __forceinline__ void careful_row(const BlockArgs& p, const Sequence& 
           }
         }
         if (pass == 0) {
+          any |= __ballot(seen) != 0;
           m = fmaxf(m, s);
           continue;
         }
@@ -164,7 +167,7 @@ __device__ __forceinline__ void careful_row(const BlockArgs& p, const Sequence& 
   T* out = static_cast<T*>(p.out) + at * p.width;
 #pragma unroll
   for (int i = 0; i < (DP + 63) / 64; ++i)
-    if (i * 64 + lane < p.width) out[i * 64 + lane] = (T)(l == 0.0f ? 0.0f : o[i] / l);
+    if (i * 64 + lane < p.width) out[i * 64 + lane] = (T)(any ? o[i] / l : 0.0f);
   if (p.lse != nullptr && lane == 0) p.lse[at] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * kLn2;
 }
 
@@ -197,14 +200,16 @@ __global__ __launch_bounds__((ManyShape<T, DP>::kThreads)) void block_attention_
                   row.in, p.width, lane, st.q);
   const float c = p.scale * kLog2e;
   const int used = (p.width + 15) / 16;
+  bool saw = false;  // a block, though its pages may be missing
   walk_blocks<T, DP, Shape, false>(p, t, row, mem, lds_address(&mem), tid, w, lane,
                             [&](int now, bool sel, bool some, bool edge, uint32_t missing, uint32_t kb,
                                 uint32_t vb, auto values, auto done) {
+                              saw |= sel;
                               attend<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, missing, row, c, used, lane, values,
                                                            done);
                             });
   const float l = across_sum(st.l), by = l > 0.0f ? 1.0f / l : 0.0f;
-  bool bad = !__builtin_isfinite(l);
+  bool bad = !__builtin_isfinite(l) || (l == 0.0f && saw);
 #pragma unroll
   for (int dt = 0; dt < DP / 16; ++dt)
 #pragma unroll
@@ -309,7 +314,7 @@ __device__ inline void join_rows(const BlockArgs& p, const FewPlace& f, int seq,
       for (int j = 0; j < 4; ++j) o[j] = __builtin_fmaf(by, x[32 + r * DP + d + j], o[j]);
     }
     const float by = l > 0.0f ? 1.0f / l : 0.0f;
-    bool bad = !__builtin_isfinite(l);
+    bool bad = !__builtin_isfinite(l) || (l == 0.0f && pos >= 0);
     T out[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

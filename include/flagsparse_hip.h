@@ -715,9 +715,10 @@ int fs_block_select(int val_t, const fs_block_seqs* seqs, int heads, int group, 
  * k[j, h / group]>) times v[j, h / group], for the heads * group heads h of a
  * token: blocks[t * b_token + (h / group) * b_head + i], i < top <= 128, names
  * blocks of t's sequence.  A block named twice counts once, a negative one or one
- * behind the token's own not at all; a token without keys gets zeros.  out is
+ * behind the token's own not at all; a token without keys gets zeros, one whose scores
+ * are all minus infinity not-a-numbers.  out is
  * dense, tokens x heads * group x width; lse (may be null) gets the logarithm of the
- * sum of the exponentials, minus infinity without keys.  Strides are in elements;
+ * sum of the exponentials, minus infinity for both.  Strides are in elements;
  * rows of width elements are contiguous, those of keys and values at multiples of
  * 16 bytes; width is a multiple of 8, up to 256 (FS_F32: 128); group <= 128.
  * k_page and v_page are read with pages alone.
