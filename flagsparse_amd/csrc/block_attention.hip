@@ -200,16 +200,21 @@ __global__ __launch_bounds__((ManyShape<T, DP>::kThreads)) void block_attention_
                   row.in, p.width, lane, st.q);
   const float c = p.scale * kLog2e;
   const int used = (p.width + 15) / 16;
-  bool saw = false;  // a block, though its pages may be missing
   walk_blocks<T, DP, Shape, false>(p, t, row, mem, lds_address(&mem), tid, w, lane,
                             [&](int now, bool sel, bool some, bool edge, uint32_t missing, uint32_t kb,
                                 uint32_t vb, auto values, auto done) {
-                              saw |= sel;
                               attend<T, DP, Shape::kAhead>(st, kb, vb, sel, now, some, edge, missing, row, c, used, lane, values,
                                                            done);
                             });
   const float l = across_sum(st.l), by = l > 0.0f ? 1.0f / l : 0.0f;
-  bool bad = !__builtin_isfinite(l) || (l == 0.0f && saw);
+  bool bad = !__builtin_isfinite(l);
+  if (__ballot(l == 0.0f && row.pos >= 0) != 0) {  // (looked up here: a bit kept in the walk costs it 1.5%)
+    const int32_t* ids = p.blocks + (int64_t)(t.token0 + row.token) * p.b_token + (int64_t)t.head * p.b_head;
+    for (int e = 0; e < p.top; ++e) {
+      const int id = ids[e];
+      bad |= l == 0.0f && id >= 0 && id <= (row.pos >> (p.lg_groups + 4));
+    }
+  }
 #pragma unroll
   for (int dt = 0; dt < DP / 16; ++dt)
 #pragma unroll
