@@ -364,7 +364,8 @@ __global__ __launch_bounds__(1024) void block_pieces_kernel(const uint32_t* keys
   for (int k0 = 0; k0 < n_keys; k0 += 1024) {
     const int k = k0 + tid;
     const int from = k < n_keys ? first(k) : 0, to = k < n_keys ? first(k + 1) : 0;
-    const uint32_t n = k < n_keys ? (uint32_t)(to > from ? (to - from + most - 1) / most : 1) : 0u;
+    const uint32_t length = to > from ? (uint32_t)(to - from) : 0u;
+    const uint32_t n = k < n_keys ? (length > 0u ? (length + (uint32_t)most - 1u) / (uint32_t)most : 1u) : 0u;
     const uint32_t shared = n > 1 ? n : 0u;
     const uint32_t upto = wave_sum_scan(n), upto2 = wave_sum_scan(shared);
     if (lane == 63) {
@@ -384,11 +385,10 @@ __global__ __launch_bounds__(1024) void block_pieces_kernel(const uint32_t* keys
     if (k < n_keys) {
       sums[k] = int2{(int)mine2, (int)shared};
       // (of like length)
-      const int each = n > 0 ? (int)((to - from + (int)n - 1) / (int)n) : 0;
+      const uint32_t each = (length + n - 1u) / n;
       for (uint32_t i = 0; i < n; ++i) {
-        const int a = from + (int)i * each < to ? from + (int)i * each : to;
-        const int b = a + each < to ? a + each : to;
-        pieces[mine + i] = int4{k, a, b, n > 1 ? (int)(mine2 + i) : -1};
+        const uint32_t a = i * each < length ? i * each : length, b = length - a < each ? length : a + each;
+        pieces[mine + i] = int4{k, from + (int)a, from + (int)b, n > 1 ? (int)(mine2 + i) : -1};
       }
     }
     __syncthreads();
@@ -404,6 +404,8 @@ struct KeyShape {
   static constexpr int kWaves = DP * (int)sizeof(T) > 256 ? 4 : 8, kThreads = 64 * kWaves;
   static constexpr int KT = 1, KW = BK / (16 * KT), RW = kWaves / KW;
   static constexpr int kStep = 32 * RW;  // rows a step
+  // waves a SIMD: of rows of 128 bytes two workgroups share a compute unit
+  static constexpr int kOccupancy = DP * (int)sizeof(T) <= 128 ? 4 : 1;
 };
 
 struct KeyPlace {
@@ -418,7 +420,7 @@ struct RowStats {
 };
 
 template <class T, int DP>
-__device__ __forceinline__ void careful_key(const GradArgs& a, const KeyPlace& at, const int32_t* tokens, int rows, int j,
+__device__ __forceinline__ void careful_key(const GradArgs& a, const KeyPlace& at, const int32_t* order, int64_t rows, int j,
                                          float (&k_sum)[(DP + 63) / 64], float (&v_sum)[(DP + 63) / 64], int lane) {
   const BlockArgs& p = a.b;
   const float c = p.scale * kLog2e;
@@ -428,13 +430,13 @@ __device__ __forceinline__ void careful_key(const GradArgs& a, const KeyPlace& a
   if (j >= at.sq.keys) return;
   const T* k = static_cast<const T*>(p.k.base) + (at.sq.row0 + j) * p.k.row + at.head * p.k.head;
   const T* v = static_cast<const T*>(p.v.base) + (at.sq.row0 + j) * p.v.row + at.head * p.v.head;
-  for (int r0 = 0; r0 < rows; r0 += 64) {
-    const int r = r0 + lane;
+  for (int64_t r0 = 0; r0 < rows; r0 += 64) {
+    const int64_t r = r0 + lane;
     float x = 0.0f, y = 0.0f;
     bool seen = false;
     int64_t row = 0, q_row = 0;
     if (r < rows) {
-      const int token = tokens[r / p.group], hq = at.head * p.group + r % p.group;
+      const int token = order[r / p.group] / (a.lists * p.top), hq = at.head * p.group + (int)(r % p.group);
       seen = at.sq.keys - at.sq.count + token - at.sq.first >= j;
       row = (int64_t)token * p.heads * p.group + hq;
       q_row = token * p.q_token + hq * p.q_head;
@@ -465,10 +467,10 @@ __device__ __forceinline__ void careful_key(const GradArgs& a, const KeyPlace& a
   }
 }
 
-constexpr int kMostEntries = 1024;  // of a piece
+constexpr int kWindow = 1024;  // entries of a piece whose tokens LDS holds at a time
 
 template <class T, int DP, int BK>
-__global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_grad_kernel(const GradArgs a) {
+__global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads), (KeyShape<T, DP, BK>::kOccupancy)) void block_key_grad_kernel(const GradArgs a) {
   using R = Rows<T, DP>;
   using S = KeyShape<T, DP, BK>;
   constexpr int KT = S::KT, KW = S::KW, RW = S::RW, STEP = S::kStep, F = R::kFrags;
@@ -478,7 +480,7 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
   constexpr int kMemory = 4 * kSlot > kJoin ? 4 * kSlot : kJoin;
   __shared__ alignas(1024) uint8_t s_mem[kMemory];
   __shared__ RowStats s_stats[2];
-  __shared__ int32_t s_token[kMostEntries];
+  __shared__ int32_t s_token[kWindow];
   __shared__ int s_bad;
   const BlockArgs& p = a.b;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -511,8 +513,7 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
   if (o.seq < 0) return;  // a number that no sequence's block has
   o.sq = sequence_of(p.seqs, o.seq);
   o.first = ((number - first_block(p.seqs, o.seq, lg_block)) << lg_block) + part * BK;
-  const int entries = piece.z - piece.y, rows = entries * p.group;
-  for (int e = tid; e < entries; e += THREADS) s_token[e] = a.order[piece.y + e] / (a.lists * p.top);
+  const int entries = piece.z - piece.y;
   if (tid == 0) s_bad = 0;
 
   // the wave's keys and values, as second operands
@@ -536,9 +537,8 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
   for (int n = 0; n < KT; ++n) factor[n] = kFactored<T> ? kFirstFactor : 1.0f;
   const float c = p.scale * kLog2e;
   const int offset = o.sq.keys - o.sq.count - o.sq.first;  // of positions from tokens
-  __syncthreads();
-
-  const int steps = (rows + STEP - 1) / STEP, used = (p.width + 15) / 16;
+  const int used = (p.width + 15) / 16;
+  int rows = 0;  // of a window
   auto place = [&](int r, int& token, int& hq) {
     const int e = (int)__umulhi((uint32_t)r, a.per_group);
     const int entry = p.group == 1 ? r : e;
@@ -576,99 +576,108 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
       n_pos = r < rows ? token + offset : INT32_MIN;
     }
   };
-  if (steps > 0) issue(0);
-  for (int s = 0; s < steps; ++s) {
-    RowStats& stats = s_stats[s & 1];
-    if (tid < STEP) {
-      stats.lse[tid] = n_lse * kLog2e - kWeightLift<T>;
-      stats.delta[tid] = n_delta;
-      stats.pos[tid] = n_pos;
-    }
-    wait_loads<0>();
-    wait_reads();
-    barrier();
-    if (s + 1 < steps) issue(s + 1);
-    const uint32_t qb = lds_address(s_mem) + (uint32_t)((s & 1) * 2 * kSlot) + (uint32_t)(rw * 32 * R::kRow);
-    const uint32_t gb = qb + kSlot;
-    f32x4 x[2][KT], y[2][KT];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int n = 0; n < KT; ++n) x[m][n] = y[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int ks = 0; ks < F; ++ks) {
-      if (leave_out<T>(ks, used)) break;
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const auto q = R::across(qb, m * 16, ks, lane);
-        const auto g = R::across(gb, m * 16, ks, lane);
-#pragma unroll
-        for (int n = 0; n < KT; ++n) {
-          x[m][n] = Mma<T>::run(q, kf[n][ks], x[m][n]);
-          y[m][n] = Mma<T>::run(g, vf[n][ks], y[m][n]);
-        }
+  for (int e0 = 0; e0 < entries; e0 += kWindow) {
+    const int here = entries - e0 < kWindow ? entries - e0 : kWindow;
+    wait_reads();  // (the window before has been read)
+    __syncthreads();
+    for (int e = tid; e < here; e += THREADS) s_token[e] = a.order[piece.y + e0 + e] / (a.lists * p.top);
+    __syncthreads();
+    rows = here * p.group;
+    const int steps = (rows + STEP - 1) / STEP;
+    issue(0);
+    for (int s = 0; s < steps; ++s) {
+      RowStats& stats = s_stats[s & 1];
+      if (tid < STEP) {
+        stats.lse[tid] = n_lse * kLog2e - kWeightLift<T>;
+        stats.delta[tid] = n_delta;
+        stats.pos[tid] = n_pos;
       }
-    }
-    typename R::Halves pf[KT][2 / P], sf[KT][2 / P];
-    f32x4 wx[KT][2], wy[KT][2];
+      wait_loads<0>();
+      wait_reads();
+      barrier();
+      if (s + 1 < steps) issue(s + 1);
+      const uint32_t qb = lds_address(s_mem) + (uint32_t)((s & 1) * 2 * kSlot) + (uint32_t)(rw * 32 * R::kRow);
+      const uint32_t gb = qb + kSlot;
+      f32x4 x[2][KT], y[2][KT];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      const int r0 = rw * 32 + m * 16 + (lane >> 4) * 4;
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(&stats.lse[r0]);
-      const f32x4 delta = *reinterpret_cast<const f32x4*>(&stats.delta[r0]);
-      const int4 pos = *reinterpret_cast<const int4*>(&stats.pos[r0]);
-      const int row_pos[4] = {pos.x, pos.y, pos.z, pos.w};
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int n = 0; n < KT; ++n) {
-        const int j = o.first + (kw * KT + n) * 16 + (lane & 15);
+        for (int n = 0; n < KT; ++n) x[m][n] = y[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          // (keys behind the last one are behind every position, rows past the list's
-          // end before every key)
-          const bool in = j <= row_pos[r];
-          const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(x[m][n][r], c, -lse[r]));
-          const float v = u * (y[m][n][r] - delta[r]);
-          wx[n][m][r] = in ? u : 0.0f;
-          wy[n][m][r] = in ? v : 0.0f;
-        }
-      }
-    }
-    if constexpr (kFactored<T>) {
+      for (int ks = 0; ks < F; ++ks) {
+        if (leave_out<T>(ks, used)) break;
 #pragma unroll
-      for (int n = 0; n < KT; ++n) {
-        float most = 0.0f;
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(wy[n][m][r]));
-        follow(across_max(most), factor[n], dk[n]);
-#pragma unroll
-        for (int m = 0; m < 2; ++m) wy[n][m] *= factor[n];
-      }
-    }
-    // P and dS in two parts of the values' type
-#pragma unroll
-    for (int n = 0; n < KT; ++n)
-#pragma unroll
-      for (int u = 0; u < 2 / P; ++u) {
-        pf[n][u] = R::halves(&wx[n][u * P]);
-        sf[n][u] = R::halves(&wy[n][u * P]);
-      }
-#pragma unroll
-    for (int u = 0; u < 2 / P; ++u)
-#pragma unroll
-      for (int dt = 0; dt < DP / 16; ++dt) {
-        if (leave_out<T>(dt, used)) break;
-        const auto g = R::down(gb, u * R::kUnit, dt, lane);
-        const auto q = R::down(qb, u * R::kUnit, dt, lane);
-#pragma unroll
-        for (int i = 0; i < R::kParts; ++i)
+        for (int m = 0; m < 2; ++m) {
+          const auto q = R::across(qb, m * 16, ks, lane);
+          const auto g = R::across(gb, m * 16, ks, lane);
 #pragma unroll
           for (int n = 0; n < KT; ++n) {
-            dv[n][dt] = Mma<T>::run(g, pf[n][u].part[i], dv[n][dt]);
-            dk[n][dt] = Mma<T>::run(q, sf[n][u].part[i], dk[n][dt]);
+            x[m][n] = Mma<T>::run(q, kf[n][ks], x[m][n]);
+            y[m][n] = Mma<T>::run(g, vf[n][ks], y[m][n]);
           }
+        }
       }
+      typename R::Halves pf[KT][2 / P], sf[KT][2 / P];
+      f32x4 wx[KT][2], wy[KT][2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const int r0 = rw * 32 + m * 16 + (lane >> 4) * 4;
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(&stats.lse[r0]);
+        const f32x4 delta = *reinterpret_cast<const f32x4*>(&stats.delta[r0]);
+        const int4 pos = *reinterpret_cast<const int4*>(&stats.pos[r0]);
+        const int row_pos[4] = {pos.x, pos.y, pos.z, pos.w};
+#pragma unroll
+        for (int n = 0; n < KT; ++n) {
+          const int j = o.first + (kw * KT + n) * 16 + (lane & 15);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            // (keys behind the last one are behind every position, rows past the list's
+            // end before every key)
+            const bool in = j <= row_pos[r];
+            const float u = __builtin_amdgcn_exp2f(__builtin_fmaf(x[m][n][r], c, -lse[r]));
+            const float v = u * (y[m][n][r] - delta[r]);
+            wx[n][m][r] = in ? u : 0.0f;
+            wy[n][m][r] = in ? v : 0.0f;
+          }
+        }
+      }
+      if constexpr (kFactored<T>) {
+#pragma unroll
+        for (int n = 0; n < KT; ++n) {
+          float most = 0.0f;
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(wy[n][m][r]));
+          follow(across_max(most), factor[n], dk[n]);
+#pragma unroll
+          for (int m = 0; m < 2; ++m) wy[n][m] *= factor[n];
+        }
+      }
+      // P and dS in two parts of the values' type
+#pragma unroll
+      for (int n = 0; n < KT; ++n)
+#pragma unroll
+        for (int u = 0; u < 2 / P; ++u) {
+          pf[n][u] = R::halves(&wx[n][u * P]);
+          sf[n][u] = R::halves(&wy[n][u * P]);
+        }
+#pragma unroll
+      for (int u = 0; u < 2 / P; ++u)
+#pragma unroll
+        for (int dt = 0; dt < DP / 16; ++dt) {
+          if (leave_out<T>(dt, used)) break;
+          const auto g = R::down(gb, u * R::kUnit, dt, lane);
+          const auto q = R::down(qb, u * R::kUnit, dt, lane);
+#pragma unroll
+          for (int i = 0; i < R::kParts; ++i)
+#pragma unroll
+            for (int n = 0; n < KT; ++n) {
+              dv[n][dt] = Mma<T>::run(g, pf[n][u].part[i], dv[n][dt]);
+              dk[n][dt] = Mma<T>::run(q, sf[n][u].part[i], dk[n][dt]);
+            }
+        }
+    }
   }
   if constexpr (kFactored<T>) {
     constexpr float kDown = 0x1p-15f;
@@ -749,7 +758,7 @@ __global__ __launch_bounds__((KeyShape<T, DP, BK>::kThreads)) void block_key_gra
     const int j = o.first + jj;
     constexpr int N = (DP + 63) / 64;
     float k_sum[N], v_sum[N];
-    careful_key<T, DP>(a, o, s_token, rows, j, k_sum, v_sum, lane);
+    careful_key<T, DP>(a, o, a.order + piece.y, (int64_t)entries * p.group, j, k_sum, v_sum, lane);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int d = i * 64 + lane;
@@ -832,11 +841,11 @@ GradPlan grad_plan(int val_t, const fs_block_seqs& s, int heads, int group, int 
   l.entries = tokens * lists * top;
   l.key_blocks = rows / block + n_seqs + 1;
   l.n_keys = l.key_blocks * lists;
-  // pieces enough for a few rounds of the chip, and long enough that their sums cost little
+  // pieces enough for a few rounds of the chip, and long enough that their sums cost little;
+  // so many at most, whatever the sizes: their sums are the workspace's largest part
   const int64_t shared = heads / lists, parts = std::max(1, block / 64);
-  int64_t most = ceil_div(l.entries * shared * parts, 2048);
-  most = std::max<int64_t>(most, ceil_div(512, group));
-  l.most = (int)std::min<int64_t>(most, kMostEntries);
+  const int64_t most = std::max<int64_t>(ceil_div(l.entries * shared * parts, 2048), ceil_div(512, group));
+  l.most = (int)std::min<int64_t>(most, INT32_MAX);
   l.pieces = l.entries / l.most + l.n_keys;
   l.places = 2 * (l.entries / l.most) + 2;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };

@@ -279,3 +279,18 @@ def test_workspace_sizes():
     c = _described(n_tokens=8192, n_rows=8192, n_seqs=1)
     grads = lib.fs_block_attention_grad_workspace_bytes(f16, ctypes.byref(c), 4, 8, 128, 4, 16)
     assert 8192 * 4 * 16 * 4 * 3 < grads < 1 << 30
+
+
+@pytest.mark.parametrize("tokens, top, block", [(32768, 16, 64), (131072, 32, 128), (131072, 16, 1024), (1 << 20, 16, 64)])
+@pytest.mark.parametrize("lists", [1, 8])
+def test_workspace_of_gradients_of_many_tokens(tokens, top, block, lists):
+    """What grows with the tokens is some words an entry and a number a row; the sums of
+    pieces do not."""
+    lib = _lib.load_library()
+    heads, group, width = 8, 8, 128
+    c = _described(n_tokens=tokens, n_rows=tokens, n_seqs=1, block=block)
+    need = lib.fs_block_attention_grad_workspace_bytes(_lib.FS_BF16, ctypes.byref(c), heads, group, width, lists, top)
+    entries = tokens * lists * top
+    # (a sort in passes has as many words again)
+    growing = entries * 4 * 8 + tokens * heads * group * 4 * 2 + 64 * (tokens // block + 2048) * lists
+    assert 0 < need < growing + (320 << 20)

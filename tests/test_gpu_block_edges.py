@@ -6,7 +6,8 @@ import torch
 
 import flagsparse_amd as fs
 
-from ._blocks_helpers import BLOCK_DTYPES, BLOCK_IDS, Case, assert_within, oracle, random_blocks, randn
+from ._blocks_bounds import gradient_bounds, worst
+from ._blocks_helpers import BLOCK_DTYPES, BLOCK_IDS, Case, oracle, random_blocks, randn
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -51,3 +52,39 @@ def test_scores_that_are_all_minus_infinity(dtype, tokens, page):
     dq, _, dv = fs.flagsparse_block_attention_grad(grad, case.q, case.k, case.v, blocks, case.seqs, out, lse)
     assert bool(torch.isnan(dq[rows]).all())
     assert bool(torch.isnan(dv[64:128][case.seen(blocks)[:, bad.any(0), 64:128].any(1).t()]).all())
+
+
+@pytest.mark.parametrize("bad", [None, float("nan")], ids=["finite", "nan"])
+@pytest.mark.parametrize("dtype", BLOCK_DTYPES, ids=BLOCK_IDS)
+def test_lists_of_more_entries_than_a_window_holds(dtype, bad):
+    """One selection for eight heads, blocks of 1024 keys: the first block's list has 9000
+    tokens, in pieces of more than 1024."""
+    tokens, heads, width, block = 9000, 8, 16, 1024
+    case = Case([tokens], [tokens], heads, 1, width, block, dtype, 63)
+    blocks = torch.zeros((tokens, 1, 2), dtype=torch.int32)
+    blocks[:, 0, 1] = torch.arange(tokens) // block
+    blocks = blocks.cuda()
+    assert tokens * 2 * heads * (block // 64) > 2048 * 1024  # entries a piece
+    grad = randn(case.q.shape, dtype, 64)
+    out, lse = fs.flagsparse_block_attention(case.q, case.k, case.v, blocks, case.seqs, return_lse=True)
+    given = grad.clone()
+    row = 5000  # sees the keys below 1024 and from 4096 on
+    if bad is not None:
+        grad[row], given[row] = 0.0, bad
+    got = fs.flagsparse_block_attention_grad(given, case.q, case.k, case.v, blocks, case.seqs, out, lse)
+    for h in (0, 5):
+        one = Case([tokens], [tokens], 1, 1, width, block, dtype, 63)
+        one.q, one.packed_k, one.packed_v = (t[:, h : h + 1] for t in (case.q, case.packed_k, case.packed_v))
+        part = slice(h, h + 1)
+        found = gradient_bounds(one, blocks, width**-0.5, grad[:, part], out[:, part], lse[:, part])
+        keys = torch.zeros(tokens, dtype=torch.bool, device="cuda")
+        rows = keys.clone()
+        if bad is not None:
+            keys[:1024] = keys[4096 : row + 1] = True
+            rows[row] = True
+        for t, name, apart in zip(got, ("dq", "dk", "dv"), (rows, keys, keys)):
+            want, bound = found[name]
+            assert bool(torch.isnan(t[:, part][apart]).all())
+            off = worst(t[:, part][~apart], want[~apart], bound[~apart])
+            assert off <= 1.0, (name, h, off)
+        del found
