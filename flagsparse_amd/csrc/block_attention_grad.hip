@@ -825,6 +825,9 @@ __global__ __launch_bounds__(256) void block_key_join_kernel(const GradArgs a, i
 
 // ---- host -------------------------------------------------------------------------
 
+// Keys of a workgroup of the keys' gradient.
+constexpr int keys_at_once(int block) { return block == 32 ? 32 : 64; }
+
 struct GradPlan {
   int64_t entries;  // of the selection
   int64_t key_blocks, n_keys;
@@ -884,6 +887,11 @@ int grad_fault(const char* who, int val_t, const fs_block_seqs* seqs, int heads,
   if (lists != 1 && lists != heads) return fail(FS_E_INVALID, std::string(who) + ": lists is 1 or the heads");
   const int64_t blocks = (seqs->n_rows / seqs->block + seqs->n_seqs + 1) * lists;
   if (seqs->n_tokens * lists * top > INT32_MAX || blocks >= INT32_MAX)
+    return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
+  // (here, before anything is launched)
+  const GradPlan l = grad_plan(val_t, *seqs, heads, group, lists, width, top);
+  if (l.tiles * heads > kMostWorkgroups ||
+      l.pieces * (heads / lists) * (seqs->block / keys_at_once(seqs->block)) > kMostWorkgroups)
     return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
   return FS_OK;
 }
@@ -985,7 +993,6 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
     if (tokens > 0) {
       p.tiles = l.tiles;
       p.per = l.per;
-      if (p.tiles * heads > kMostWorkgroups) return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
       const dim3 grid((uint32_t)(p.tiles * heads));
       hipLaunchKernelGGL((block_query_grad_kernel<T, DP>), grid, dim3(QueryGradShape<T, DP>::kThreads), 0, stream, a);
       FS_CHECK_MAIN_LAUNCH("block_query_grad_kernel");
@@ -994,14 +1001,13 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
     auto keys_of = [&](auto bk) -> int {
       constexpr int BK = decltype(bk)::value;
       const int64_t groups = l.pieces * shared * (seqs->block / BK);
-      if (groups > kMostWorkgroups) return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
       hipLaunchKernelGGL((block_key_grad_kernel<T, DP, BK>), dim3((uint32_t)groups), dim3(KeyShape<T, DP, BK>::kThreads), 0,
                          stream, a);
       FS_CHECK_LAUNCH("block_key_grad_kernel");
       return FS_OK;
     };
-    if (const int rc = seqs->block == 32 ? keys_of(std::integral_constant<int, 32>{})
-                                         : keys_of(std::integral_constant<int, 64>{}))
+    if (const int rc = keys_at_once(seqs->block) == 32 ? keys_of(std::integral_constant<int, 32>{})
+                                                       : keys_of(std::integral_constant<int, 64>{}))
       return rc;
     const int64_t again = tokens > 0 ? p.tiles * heads : 0;
     hipLaunchKernelGGL((block_key_join_kernel<T, DP>), row_grid(again + ((l.n_keys * shared) << p.lg_groups)), dim3(256), 0,

@@ -294,3 +294,17 @@ def test_workspace_of_gradients_of_many_tokens(tokens, top, block, lists):
     # (a sort in passes has as many words again)
     growing = entries * 4 * 8 + tokens * heads * group * 4 * 2 + 64 * (tokens // block + 2048) * lists
     assert 0 < need < growing + (320 << 20)
+
+
+@pytest.mark.parametrize("sizes", [dict(n_tokens=1 << 26, n_rows=40), dict(n_tokens=64, n_rows=1 << 29)],
+                         ids=["queries", "keys"])
+def test_gradients_refuse_launches_that_are_too_large_before_the_first(sizes):
+    """More workgroups than a launch can have, of the queries' or of the keys' kernel."""
+    lib = _lib.load_library()
+    c = _described(**sizes)
+    need = lib.fs_block_attention_grad_workspace_bytes(_lib.FS_F16, ctypes.byref(c), 16, 4, 64, 1, 4)
+    rc = lib.fs_block_attention_grad(_lib.FS_F16, ctypes.byref(c), 16, 4, 64, 1, 4, FAKE, FAKE, 4096, 64, FAKE, 1024, 64,
+                                     FAKE, 1024, 64, FAKE, 4, 0, 0.125, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE,
+                                     1 << 50, None)
+    assert rc == _lib.FS_E_INVALID and "sizes out of range" in lib.fs_last_error().decode(), lib.fs_last_error()
+    assert need == 0
