@@ -362,7 +362,8 @@ def _attention(q, k, v, blocks, seqs, scale, out=None, want_lse=False):
     return (result if out is None else done(out, result)), lse
 
 
-def _attention_grad(grad, q, k, v, blocks, seqs, scale, out, lse):
+def _attention_grad(grad, q, k, v, blocks, seqs, scale, out, lse, queries=True, keys=True):
+    """(dq, dk, dv): None for the queries', or for the keys' and values', where not wanted."""
     heads, width = k.shape[-2:]
     group = q.shape[1] // heads
     grad, out, lse = (t.contiguous() for t in (grad, out, lse))
@@ -374,7 +375,8 @@ def _attention_grad(grad, q, k, v, blocks, seqs, scale, out, lse):
     v, (_, v_row, v_head) = _cache_rows(v)
     if blocks.stride(2) != 1:
         blocks = blocks.contiguous()
-    dq, dk, dv = grad.new_empty(q.shape), grad.new_empty(k.shape), grad.new_empty(v.shape)
+    dq = grad.new_empty(q.shape) if queries else None
+    dk, dv = (grad.new_empty(k.shape), grad.new_empty(v.shape)) if keys else (None, None)
     top, lib, code = blocks.shape[2], _lib.lib(), BLOCK_VALUE_CODES[q.dtype]
     lists = blocks.shape[1]
     if q.shape[0] * lists * top > _INT32_MAX:
@@ -407,8 +409,9 @@ class _BlockAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _):
         q, k, v, blocks, out, lse, _, _ = ctx.saved_tensors
-        dq, dk, dv = _attention_grad(grad, q, k, v, blocks, ctx.seqs, ctx.scale, out, lse)
-        return dq, dk, dv, None, None, None
+        of_q, of_k, of_v = ctx.needs_input_grad[:3]
+        dq, dk, dv = _attention_grad(grad, q, k, v, blocks, ctx.seqs, ctx.scale, out, lse, of_q, of_k or of_v)
+        return dq, dk if of_k else None, dv if of_v else None, None, None, None
 
 
 def flagsparse_block_attention(q, k, v, blocks, seqs, scale=None, out=None, return_lse=False):

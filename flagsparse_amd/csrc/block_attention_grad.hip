@@ -199,9 +199,10 @@ __global__ __launch_bounds__((QueryGradShape<T, DP>::kThreads)) void block_query
     if (tid < Shape::kReaders) p.again[(int64_t)blockIdx.x * Shape::kReaders + tid] = 0u;
     return;
   }
+  const bool all = p.out != nullptr;  // or <G, O> alone, for the keys
   walk_start<Shape>(mem, tid);
   if (w >= Shape::kReaders) {
-    walk_loads<T, DP, Shape>(p, t, mem, lds_address(&mem), tid, w, lane);
+    if (all) walk_loads<T, DP, Shape>(p, t, mem, lds_address(&mem), tid, w, lane);
     return;
   }
   const RowOf row = row_of(p, t, w, lane);
@@ -222,6 +223,7 @@ __global__ __launch_bounds__((QueryGradShape<T, DP>::kThreads)) void block_query
       for (int e = 0; e < 16 / (int)sizeof(T); ++e) sum = __builtin_fmaf((float)st.g[ks][e], (float)o[ks][e], sum);
     sum = across_sum(sum);
     if (row.in && lane < 16) a.delta[at] = sum;
+    if (!all) return;
     st.delta = sum;
     st.lse = row.in ? a.lse[at] * kLog2e : 0.0f;
   }
@@ -786,6 +788,7 @@ __global__ __launch_bounds__(256) void block_key_join_kernel(const GradArgs a, i
     queries_again<T, DP>(a, (uint32_t)(at + again), __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), 4, lane);
     return;
   }
+  if (a.dk == nullptr) return;
   const int group = (int)(at & ((1 << p.lg_groups) - 1));
   at >>= p.lg_groups;
   const int copy = (int)(at % shared), key = (int)(at / shared);
@@ -917,8 +920,9 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
   if (const int rc = grad_fault(who, val_t, seqs, heads, group, width, lists, top)) return rc;
   const int64_t size = val_t == FS_F32 ? 4 : 2, tokens = seqs->n_tokens;
   if (tokens == 0 && seqs->n_rows == 0) return FS_OK;
-  if ((tokens > 0 && (!grad || !q || !blocks || !out || !lse || !dq)) || !k || !v || (seqs->n_rows > 0 && (!dk || !dv)) ||
-      q_token < 0 || q_head < 0 || b_token < 0 || b_head < 0)
+  const bool queries = tokens > 0 && dq != nullptr, of_keys = seqs->n_rows > 0 && dk != nullptr;
+  if ((tokens > 0 && (!grad || !q || !blocks || !out || !lse)) || !k || !v || (seqs->n_rows > 0 && !dk != !dv) ||
+      (!queries && !of_keys) || q_token < 0 || q_head < 0 || b_token < 0 || b_head < 0)
     return fail(FS_E_INVALID, std::string(who) + ": bad pointer or stride");
   if (!block_rows_fit(k, 0, k_row, k_head, size) || !block_rows_fit(v, 0, v_row, v_head, size) ||
       (((int64_t)(uintptr_t)q | (int64_t)(uintptr_t)grad | q_token * size | q_head * size) & 15) != 0)
@@ -964,29 +968,31 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
   uint32_t* sorted = reinterpret_cast<uint32_t*>(m + l.sorted);
   int32_t* starts = reinterpret_cast<int32_t*>(m + l.starts);
 
-  const int64_t key_groups = std::min<int64_t>(ceil_div(std::max<int64_t>(tokens, 4), 4), 4096);
-  hipLaunchKernelGGL(block_keys_kernel, dim3((uint32_t)key_groups), dim3(256), 0, stream, p, lists, (int)l.key_blocks, keys,
-                     static_cast<uint32_t*>(dk), static_cast<uint32_t*>(dv), (int64_t)heads * width * size / 4);
-  FS_CHECK_LAUNCH("block_keys_kernel");
-  if (l.entries > 0) {
-    if (const int rc = select_sort(keys, FS_I32, l.entries, l.n_keys, sorted, reinterpret_cast<int32_t*>(m + l.order),
-                                   nullptr, nullptr, m + l.sort, stream, nullptr, 0))
-      return rc;
+  if (of_keys) {
+    const int64_t key_groups = std::min<int64_t>(ceil_div(std::max<int64_t>(tokens, 4), 4), 4096);
+    hipLaunchKernelGGL(block_keys_kernel, dim3((uint32_t)key_groups), dim3(256), 0, stream, p, lists, (int)l.key_blocks, keys,
+                       static_cast<uint32_t*>(dk), static_cast<uint32_t*>(dv), (int64_t)heads * width * size / 4);
+    FS_CHECK_LAUNCH("block_keys_kernel");
+    if (l.entries > 0) {
+      if (const int rc = select_sort(keys, FS_I32, l.entries, l.n_keys, sorted, reinterpret_cast<int32_t*>(m + l.order),
+                                     nullptr, nullptr, m + l.sort, stream, nullptr, 0))
+        return rc;
+    }
+    int4* pieces = const_cast<int4*>(a.pieces);
+    int2* sums = const_cast<int2*>(a.sums);
+    int32_t* n_pieces = const_cast<int32_t*>(a.n_pieces);
+    if (l.n_keys <= kFewKeys && l.entries <= kFewEntries) {
+      hipLaunchKernelGGL((block_pieces_kernel<true>), dim3(1), dim3(1024), 0, stream, sorted, l.entries, starts,
+                         (int)l.n_keys, l.most, pieces, sums, n_pieces);
+    } else {
+      hipLaunchKernelGGL(block_lists_kernel, dim3((uint32_t)ceil_div(l.n_keys + 1, 256)), dim3(256), 0, stream, sorted,
+                         l.entries, (int)l.n_keys, starts);
+      FS_CHECK_LAUNCH("block_lists_kernel");
+      hipLaunchKernelGGL((block_pieces_kernel<false>), dim3(1), dim3(1024), 0, stream, sorted, l.entries, starts,
+                         (int)l.n_keys, l.most, pieces, sums, n_pieces);
+    }
+    FS_CHECK_LAUNCH("block_pieces_kernel");
   }
-  int4* pieces = const_cast<int4*>(a.pieces);
-  int2* sums = const_cast<int2*>(a.sums);
-  int32_t* n_pieces = const_cast<int32_t*>(a.n_pieces);
-  if (l.n_keys <= kFewKeys && l.entries <= kFewEntries) {
-    hipLaunchKernelGGL((block_pieces_kernel<true>), dim3(1), dim3(1024), 0, stream, sorted, l.entries, starts,
-                       (int)l.n_keys, l.most, pieces, sums, n_pieces);
-  } else {
-    hipLaunchKernelGGL(block_lists_kernel, dim3((uint32_t)ceil_div(l.n_keys + 1, 256)), dim3(256), 0, stream, sorted,
-                       l.entries, (int)l.n_keys, starts);
-    FS_CHECK_LAUNCH("block_lists_kernel");
-    hipLaunchKernelGGL((block_pieces_kernel<false>), dim3(1), dim3(1024), 0, stream, sorted, l.entries, starts,
-                       (int)l.n_keys, l.most, pieces, sums, n_pieces);
-  }
-  FS_CHECK_LAUNCH("block_pieces_kernel");
   return with_block_width(val_t, width, who, [&](auto val, auto dp) -> int {
     using T = decltype(val);
     constexpr int DP = decltype(dp)::value;
@@ -997,7 +1003,7 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
       hipLaunchKernelGGL((block_query_grad_kernel<T, DP>), grid, dim3(QueryGradShape<T, DP>::kThreads), 0, stream, a);
       FS_CHECK_MAIN_LAUNCH("block_query_grad_kernel");
     }
-    const int64_t shared = heads / lists;
+    const int64_t shared = of_keys ? heads / lists : 0;
     auto keys_of = [&](auto bk) -> int {
       constexpr int BK = decltype(bk)::value;
       const int64_t groups = l.pieces * shared * (seqs->block / BK);
@@ -1006,10 +1012,12 @@ extern "C" int fs_block_attention_grad(int val_t, const fs_block_seqs* seqs, int
       FS_CHECK_LAUNCH("block_key_grad_kernel");
       return FS_OK;
     };
-    if (const int rc = keys_at_once(seqs->block) == 32 ? keys_of(std::integral_constant<int, 32>{})
-                                                       : keys_of(std::integral_constant<int, 64>{}))
-      return rc;
-    const int64_t again = tokens > 0 ? p.tiles * heads : 0;
+    if (of_keys) {
+      const int rc = keys_at_once(seqs->block) == 32 ? keys_of(std::integral_constant<int, 32>{})
+                                                     : keys_of(std::integral_constant<int, 64>{});
+      if (rc != FS_OK) return rc;
+    }
+    const int64_t again = queries ? p.tiles * heads : 0;
     hipLaunchKernelGGL((block_key_join_kernel<T, DP>), row_grid(again + ((l.n_keys * shared) << p.lg_groups)), dim3(256), 0,
                        stream, a, again);
     FS_CHECK_LAUNCH("block_key_join_kernel");

@@ -735,7 +735,8 @@ int fs_block_attention(int val_t, const fs_block_seqs* seqs, int heads, int grou
  * Its gradients in queries, keys and values of packed rows, from grad, out and lse
  * (dense; out and lse as fs_block_attention wrote them).  dq is dense, tokens x
  * heads * group x width; dk and dv are n_rows x heads x width, zero in rows of no
- * sequence and of keys that no token sees.  lists is heads, or 1 where the heads
+ * sequence and of keys that no token sees.  dq may be null, or both dk and dv: what is
+ * for them alone is left out.  lists is heads, or 1 where the heads
  * share a selection.  group is up to 96 where a row, filled up to 64, 128 or 256
  * elements, has more than 256 bytes.  Rows of queries and of grad lie at multiples of 16 bytes too.
  * tokens * lists * top is below 2^31.

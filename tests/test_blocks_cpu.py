@@ -308,3 +308,20 @@ def test_gradients_refuse_launches_that_are_too_large_before_the_first(sizes):
                                      1 << 50, None)
     assert rc == _lib.FS_E_INVALID and "sizes out of range" in lib.fs_last_error().decode(), lib.fs_last_error()
     assert need == 0
+
+
+def test_gradients_of_keys_and_values_go_together():
+    lib = _lib.load_library()
+
+    def refused(dq, dk, dv):
+        c = _described()
+        rc = lib.fs_block_attention_grad(_lib.FS_F16, ctypes.byref(c), 3, 2, 64, 3, 4, FAKE, FAKE, 384, 64, FAKE, 192, 64,
+                                         FAKE, 192, 64, FAKE, 12, 4, 0.125, FAKE, FAKE, dq, dk, dv, FAKE, 0, None)
+        text = lib.fs_last_error().decode()
+        return rc == _lib.FS_E_INVALID and "bad pointer" in text, text
+
+    for given in ((FAKE, FAKE, None), (FAKE, None, FAKE), (None, FAKE, None), (None, None, None)):
+        assert refused(*given)[0], given
+    for given in ((FAKE, FAKE, FAKE), (FAKE, None, None), (None, FAKE, FAKE)):  # (the workspace is)
+        bad, text = refused(*given)
+        assert not bad and "workspace too small" in text, given

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import flagsparse_amd as fs
+from flagsparse_amd import blocks as block_module
 
 from ._blocks_bounds import gradient_bounds, worst
 from ._blocks_helpers import BLOCK_DTYPES, BLOCK_IDS, Case, oracle, random_blocks, randn
@@ -88,3 +89,22 @@ def test_lists_of_more_entries_than_a_window_holds(dtype, bad):
             off = worst(t[:, part][~apart], want[~apart], bound[~apart])
             assert off <= 1.0, (name, h, off)
         del found
+
+
+@pytest.mark.parametrize("wanted", ["q", "k", "v", "kv", "qv"])
+@pytest.mark.parametrize("tokens", [70, 1500])
+def test_gradients_that_are_not_wanted_are_not_computed(tokens, wanted, monkeypatch):
+    case = Case([tokens, 30], [tokens + 40, 30], 4, 2, 64, 64, torch.bfloat16, 65, tail=3, key_tail=4)
+    blocks = random_blocks([tokens, 30], [tokens + 40, 30], 4, 3, 64, 66, extra=3)
+    grad = randn(case.q.shape, torch.bfloat16, 67)
+    out, lse = fs.flagsparse_block_attention(case.q, case.k, case.v, blocks, case.seqs, return_lse=True)
+    want = dict(zip("qkv", fs.flagsparse_block_attention_grad(grad, case.q, case.k, case.v, blocks, case.seqs, out, lse)))
+    computed = []
+    inner = block_module._attention_grad
+    monkeypatch.setattr(block_module, "_attention_grad", lambda *a, **b: computed.append(inner(*a, **b)) or computed[-1])
+    leaves = {n: t.clone().requires_grad_(n in wanted) for n, t in zip("qkv", (case.q, case.k, case.v))}
+    result = fs.flagsparse_block_attention(*leaves.values(), blocks, case.seqs)
+    got = torch.autograd.grad(result, [leaves[n] for n in wanted], grad)
+    assert all(torch.equal(g, want[n]) for g, n in zip(got, wanted))
+    dq, dk, dv = computed.pop()
+    assert (dq is None) == ("q" not in wanted) and (dk is None) == (dv is None) == (wanted == "q")
