@@ -5,10 +5,10 @@ import pytest
 import torch
 
 import flagsparse_amd as fs
-from flagsparse_amd import blocks as block_module
+from flagsparse_amd import _lib, blocks as block_module
 
-from ._blocks_bounds import gradient_bounds, worst
-from ._blocks_helpers import BLOCK_DTYPES, BLOCK_IDS, Case, oracle, random_blocks, randn
+from ._blocks_bounds import attention_bounds, gradient_bounds, worst
+from ._blocks_helpers import BLOCK_DTYPES, BLOCK_IDS, Case, offsets, oracle, random_blocks, randn
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -108,3 +108,131 @@ def test_gradients_that_are_not_wanted_are_not_computed(tokens, wanted, monkeypa
     assert all(torch.equal(g, want[n]) for g, n in zip(got, wanted))
     dq, dk, dv = computed.pop()
     assert (dq is None) == ("q" not in wanted) and (dk is None) == (dv is None) == (wanted == "q")
+
+
+WINDOWS = [
+    # dtype, group, width, context: more blocks of 32 keys than a workgroup's table holds at a time
+    (torch.float16, 1, 64, 30000),
+    (torch.bfloat16, 3, 64, 30000),
+    (torch.bfloat16, 1, 128, 40000),
+    (torch.float32, 1, 64, 40000),
+    (torch.float32, 1, 128, 50000),
+]
+
+
+@pytest.mark.parametrize("sizes", WINDOWS, ids=["x".join(map(str, c)).replace("torch.", "") for c in WINDOWS])
+def test_gradients_in_several_windows(sizes):
+    dtype, group, width, context = sizes
+    tokens = 250
+    case = Case([tokens], [context], 2, group, width, 32, dtype, 68)
+    blocks = random_blocks([tokens], [context], 2, 6, 32, 69)
+    grad = randn(case.q.shape, dtype, 70)
+    out, lse = fs.flagsparse_block_attention(case.q, case.k, case.v, blocks, case.seqs, return_lse=True)
+    got = fs.flagsparse_block_attention_grad(grad, case.q, case.k, case.v, blocks, case.seqs, out, lse)
+    found = gradient_bounds(case, blocks, width**-0.5, grad, out, lse)
+    off = {name: worst(t, *found[name]) for t, name in zip(got, ("dq", "dk", "dv"))}
+    assert max(off.values()) <= 1.0, off
+
+
+LARGE_BLOCKS = [
+    ([700, 3], [1500, 600], 2, 3, 64, 512, 2),
+    ([1100, 90], [1100, 2100], 4, 2, 128, 1024, 2),
+    ([5], [2600], 2, 4, 80, 512, 3),
+]
+
+
+@pytest.mark.parametrize("dtype", BLOCK_DTYPES, ids=BLOCK_IDS)
+@pytest.mark.parametrize("sizes", LARGE_BLOCKS, ids=["x".join(map(str, c[2:])) for c in LARGE_BLOCKS])
+def test_large_blocks(sizes, dtype):
+    new, lengths, heads, group, width, block, top = sizes
+    case = Case(new, lengths, heads, group, width, block, dtype, 71, tail=2, key_tail=3)
+    blocks = random_blocks(new, lengths, heads, top, block, 72, extra=2)
+    grad = randn(case.q.shape, dtype, 73)
+    out, lse = fs.flagsparse_block_attention(case.q, case.k, case.v, blocks, case.seqs, return_lse=True)
+    got = fs.flagsparse_block_attention_grad(grad, case.q, case.k, case.v, blocks, case.seqs, out, lse)
+    found = gradient_bounds(case, blocks, width**-0.5, grad, out, lse)
+    off = {name: worst(t, *found[name]) for t, name in zip(got, ("dq", "dk", "dv"))}
+    off["out"] = worst(out, *attention_bounds(case, blocks, width**-0.5))
+    assert max(off.values()) <= 1.0, off
+    means = fs.flagsparse_block_means(case.k, case.seqs, max_blocks=6)
+    at = 0
+    for b, n in enumerate(lengths):
+        for i in range(6):
+            rows = case.packed_k[at + min(i * block, n) : at + min((i + 1) * block, n)].double()
+            want = rows.mean(0) if rows.shape[0] else torch.zeros_like(means[b, i]).double()
+            size = rows.abs().sum(0) / max(1, rows.shape[0])
+            # sums of `block` terms in 32 bits, one division, one rounding
+            bound = (block + 2) * 2.0**-24 * size + torch.finfo(dtype).eps / 2 * (want.abs() + size * 2.0**-13) + 2.0**-25
+            assert bool(((means[b, i].double() - want).abs() <= bound).all())
+        at += n
+
+
+class _Guarded:
+    """A tensor's copy in the middle of a larger one, whose other values are kept in mind."""
+
+    def __init__(self, t, around):
+        self.whole = torch.full((t.numel() + 8192,), around, dtype=t.dtype, device="cuda")
+        self.middle = self.whole[4096 : 4096 + t.numel()].view(t.shape)
+        self.middle.copy_(t)
+        self.around = around
+
+    def untouched(self):
+        sides = torch.cat([self.whole[:4096], self.whole[-4096:]])
+        return bool((torch.isnan(sides) if self.around != self.around else sides == self.around).all())
+
+
+@pytest.mark.parametrize("tokens", [(40, 30), (1500, 30)], ids=["few", "many"])
+@pytest.mark.parametrize("which", ["queries", "keys", "below", "falling"])
+def test_lengths_beyond_the_arrays_touch_nothing_around_them(which, tokens):
+    """Offsets far past the arrays and below zero: what they say there is not there, and the
+    results are those of the offsets brought into range, unless they fall: sequences then
+    lie over each other."""
+    heads, group, width, block, top = 4, 2, 64, 64, 4
+    total, rows = sum(tokens), tokens[0] + 660
+    lengths = [tokens[0] + 360, 300]
+    wild = torch.tensor([0, 2**31 - 1, 5] if which == "falling" else [0, 2**31 - 9, 2**31 - 1], dtype=torch.int32).cuda()
+    if which == "queries":  # all tokens are the first sequence's
+        q_offsets, k_offsets, new, lengths = wild, offsets(lengths), [total, 0], lengths
+    elif which == "keys":  # all rows are
+        q_offsets, k_offsets, new, lengths = offsets(tokens), wild, list(tokens), [rows, 0]
+    elif which == "falling":
+        q_offsets, k_offsets, new = wild, wild, [total, 0]
+    else:  # no sequence has any
+        q_offsets, k_offsets, new, lengths = -wild, -wild, [0, 0], [0, 0]
+    case = Case(new, lengths, heads, group, width, block, torch.bfloat16, 74, tail=total - sum(new),
+                key_tail=rows - sum(lengths))
+    blocks = random_blocks([total], [rows], heads, top, block, 75)
+    nan = float("nan")
+    q, k, v, grad = (_Guarded(t, nan) for t in (case.q, case.packed_k, case.packed_v, randn(case.q.shape, torch.bfloat16, 76)))
+    ids = _Guarded(blocks, 1)
+    out, dq = (_Guarded(torch.zeros_like(case.q), 7.0) for _ in range(2))
+    dk, dv = (_Guarded(torch.zeros_like(case.packed_k), 7.0) for _ in range(2))
+    seqs = fs.prepare_block_sequences(block, q_offsets, k_offsets=k_offsets)
+    _, lse = fs.flagsparse_block_attention(q.middle, k.middle, v.middle, ids.middle, seqs, out=out.middle, return_lse=True)
+    # (by the C entry, whose results lie where they are put)
+    lib, described = _lib.lib(), block_module._described(seqs, total, k.middle)
+    need = lib.fs_block_attention_grad_workspace_bytes(_lib.FS_BF16, described, heads, group, width, heads, top)
+    ws = _Guarded(torch.zeros(need, dtype=torch.uint8, device="cuda"), 7)
+    token, row = heads * group * width, heads * width
+    rc = lib.fs_block_attention_grad(
+        _lib.FS_BF16, described, heads, group, width, heads, top, grad.middle.data_ptr(), q.middle.data_ptr(), token, width,
+        k.middle.data_ptr(), row, width, v.middle.data_ptr(), row, width, ids.middle.data_ptr(), heads * top, top,
+        width**-0.5, out.middle.data_ptr(), lse.data_ptr(), dq.middle.data_ptr(), dk.middle.data_ptr(),
+        dv.middle.data_ptr(), ws.middle.data_ptr(), need, _lib.stream_handle(q.middle.device))
+    assert rc == _lib.FS_OK, lib.fs_last_error()
+    means = _Guarded(torch.zeros((2, 9, heads, width), dtype=torch.bfloat16, device="cuda"), 7.0)
+    fs.flagsparse_block_means(k.middle, seqs, out=means.middle)
+    chosen = _Guarded(torch.zeros((total, heads, 5), dtype=torch.int32, device="cuda"), 7)
+    fs.flagsparse_block_select(q.middle, means.middle, seqs, 5, out=chosen.middle)
+    torch.cuda.synchronize()
+    for t in (q, k, v, grad, ids, out, dq, dk, dv, ws, means, chosen):
+        assert t.untouched()
+    if which == "falling":
+        return
+    if which != "keys":  # (the selection has no keys: it takes the lengths as they are)
+        assert torch.equal(chosen.middle, fs.flagsparse_block_select(case.q, means.middle, case.seqs, 5))
+    assert torch.equal(means.middle, fs.flagsparse_block_means(case.packed_k, case.seqs, max_blocks=9))
+    assert worst(out.middle, *attention_bounds(case, blocks, width**-0.5)) <= 1.0
+    found = gradient_bounds(case, blocks, width**-0.5, grad.middle, out.middle, lse)
+    for t, name in ((dq, "dq"), (dk, "dk"), (dv, "dv")):
+        assert worst(t.middle, *found[name]) <= 1.0, name
