@@ -471,8 +471,26 @@ __global__ __launch_bounds__(128) void block_attention_join_kernel(const BlockAr
   });
 }
 
-// A few rows' kernel up to this many (token, key-value head) pairs.
-constexpr int64_t kFewPairs = 4096;
+// The few rows' kernel takes each (token, key-value head, 16 of the group) by itself: its
+// time goes with their number and their width.  The other one's hardly changes until the
+// chip has a workgroup for each compute unit, and falls with the group, as fewer tokens
+// share a walk.  us of both (few, many), bf16, widths of 128, 16 blocks of 64 of 8192 to
+// 16384 keys, by token and head:
+//   group 1   2048 124, 371; 4096 239, 375   (of 64 sequences 326, 308)
+//   group 4   2048 124, 205; 4096 240, 206   (of 64 sequences 330, 256)
+//   group 16  1024 66, 99; 2048 126, 99; 4096 241, 177   (of 64 sequences 2048 175, 175)
+//   group 64  64 29, 39; 192 70, 60; 400 104, 60
+//   group 8, 64 blocks  2048 281, 345; 4096 552, 357
+//   group 4, width 256  1600 199, 205; 2048 230, 203;  width 64 (f16) 4096 106, 136
+//   group 4, f32  2048 344, 632; 4096 681, 637
+// Even at about 6500 of widths of 128 by the root of the group; never above 4096.
+constexpr int64_t kFewMost = 4096, kEven = 6500;
+inline bool few_rows(int64_t tokens, int heads, int group, int width) {
+  const int64_t all = tokens * heads * ((group + 15) / 16);
+  if (all > kFewMost) return false;
+  const int64_t wide = all * (width <= 64 ? 64 : width <= 128 ? 128 : 256);
+  return wide * wide * group <= (kEven * 128) * (kEven * 128);
+}
 
 struct Plan {
   bool few;
@@ -488,7 +506,7 @@ Plan plan_of(int val_t, const fs_block_seqs& s, int heads, int group, int width,
   const int block = s.block;
   o.readers = many_readers((width <= 64 ? 64 : width <= 128 ? 128 : 256) * (val_t == FS_F32 ? 4 : 2));
   // (a group whose rows do not fit a workgroup of the other kernel, too)
-  o.few = tokens * heads <= kFewPairs || o.readers * 16 < group;
+  o.few = few_rows(tokens, heads, group, width) || o.readers * 16 < group;
   o.groups = tokens * heads * ((group + 15) / 16);
   o.splits = 1;
   if (o.few) {

@@ -167,6 +167,17 @@ def test_large_blocks(sizes, dtype):
         at += n
 
 
+@pytest.mark.parametrize("tokens", [405, 407], ids=["few", "many"])
+@pytest.mark.parametrize("page", [0, 32])
+def test_either_side_of_the_rule(tokens, page):
+    """Groups of 16 and four heads of 128: 1625 tokens and heads go to the one kernel, more to the other."""
+    case = Case([tokens - 5, 5], [tokens + 30, 100], 4, 16, 128, 64, torch.float16, 77, page)
+    blocks = random_blocks([tokens - 5, 5], [tokens + 30, 100], 4, 3, 64, 78)
+    out, lse = fs.flagsparse_block_attention(case.q, case.k, case.v, blocks, case.seqs, return_lse=True)
+    assert _lib.last_kernel() == ("block_attention_few_kernel" if tokens * 4 <= 1625 else "block_attention_kernel")
+    assert worst(out, *attention_bounds(case, blocks, 128**-0.5)) <= 1.0
+
+
 class _Guarded:
     """A tensor's copy in the middle of a larger one, whose other values are kept in mind."""
 
