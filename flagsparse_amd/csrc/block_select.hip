@@ -160,7 +160,7 @@ __device__ inline int keep_best_of_row(uint64_t* keys, int32_t* ids, int kept, i
   return keep_best(key, id, used, want, keys, ids, lane);
 }
 
-// SINGLE: a workgroup takes one token, where sequences have few.
+// SINGLE: a workgroup takes one token, where few have many blocks.
 template <class T, int DP, bool SINGLE>
 __global__ __launch_bounds__((64 * kSelectWaves), (SINGLE || DP > 128 ? 2 : 4)) void block_select_kernel(const SelectArgs p) {
   constexpr int E = 16 / (int)sizeof(T), J = DP * (int)sizeof(T) / 64, W = kSelectWaves, kEach = kTokens / W;
@@ -366,16 +366,31 @@ extern "C" int fs_block_select(int val_t, const fs_block_seqs* seqs, int heads, 
   p.first = first;
   p.recent = recent;
   p.lg_block = __builtin_ctz((unsigned)seqs->block);
-  // one token a workgroup where a tile of 16 would hold four at most
-  const bool single = seqs->n_tokens <= 4 * seqs->n_seqs;
+  // One token a workgroup, its blocks over the waves, where they are many and the tokens
+  // few (or alone in their tile of 16 in any case).  us of both (single, tiles), bf16, 8
+  // heads of 128:
+  //   256 blocks   1 token 20, 13; 32 sequences of one 22, 13, of two 28, 16
+  //   512 blocks   1 token 22, 21; of 16 sequences two 23, 27
+  //   768 blocks   1 token 24, 30; of 16 sequences four 38, 38
+  //   1024 blocks  1 token 27, 38; 32 sequences of one 32, 41, of two 47, 50, of four 77, 52
+  // Widths above 128, whose means fill a wave's registers: 1024 blocks, 1 token 56, 59; 16
+  // sequences of one 75, 61, of four 133, 70, so tiles always.
+  const bool single = most >= 640 && width <= 128 &&
+                      (seqs->n_tokens <= seqs->n_seqs || seqs->n_tokens * heads <= 512);
   p.tiles = block_tiles(*seqs, single ? 1 : kTokens);
   if (p.tiles * heads > kMostWorkgroups) return fail(FS_E_INVALID, std::string(who) + ": sizes out of range");
   return with_block_width(val_t, width, who, [&](auto val, auto dp) -> int {
     using T = decltype(val);
     constexpr int DP = decltype(dp)::value;
     const dim3 grid((uint32_t)(p.tiles * heads)), threads(64 * kSelectWaves);
-    if (single) hipLaunchKernelGGL((block_select_kernel<T, DP, true>), grid, threads, 0, stream, p);
-    else hipLaunchKernelGGL((block_select_kernel<T, DP, false>), grid, threads, 0, stream, p);
+    if constexpr (DP <= 128) {
+      if (single) {
+        hipLaunchKernelGGL((block_select_kernel<T, DP, true>), grid, threads, 0, stream, p);
+        FS_CHECK_MAIN_LAUNCH("block_select_kernel (single tokens)");
+        return FS_OK;
+      }
+    }
+    hipLaunchKernelGGL((block_select_kernel<T, DP, false>), grid, threads, 0, stream, p);
     FS_CHECK_MAIN_LAUNCH("block_select_kernel");
     return FS_OK;
   });
