@@ -386,7 +386,7 @@ extern "C" int fs_block_select(int val_t, const fs_block_seqs* seqs, int heads, 
     if constexpr (DP <= 128) {
       if (single) {
         hipLaunchKernelGGL((block_select_kernel<T, DP, true>), grid, threads, 0, stream, p);
-        FS_CHECK_MAIN_LAUNCH("block_select_kernel (single tokens)");
+        FS_CHECK_MAIN_LAUNCH("block_select_single_kernel");
         return FS_OK;
       }
     }

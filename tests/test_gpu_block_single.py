@@ -9,7 +9,7 @@ from flagsparse_amd import _lib
 from ._blocks_helpers import BLOCK_DTYPES, BLOCK_IDS, Case, randn, select_oracle
 
 pytestmark = pytest.mark.gpu
-SINGLE = "block_select_kernel (single tokens)"
+SINGLE = "block_select_single_kernel"
 
 SIZES = [
     # new, lengths, heads, group, width, block, top, first, recent
