@@ -3,8 +3,9 @@
 //
 // One pass over the keys: a wave takes one head of a block, as many rows at a time
 // as its 64 lanes have 16-byte slices for, sums in 32 bits and adds its rows' sums at
-// the end, in a fixed order.  216 MB of f16 keys 36 us, 6.0 TB/s; the blocks of 64 new
-// keys 10 us, a chain of four dependent loads behind the launch.
+// the end, in a fixed order.  216 MB of f16 keys 47 us, 4.6 TB/s (36 us where they lie in
+// the 256 MB cache).  The blocks of 64 new keys 10 us: a lane looks up the page of each
+// of its 16 rows and loads the row, one after the other, and waits for both.
 #include "block_tile.hpp"
 
 namespace fs {
@@ -70,7 +71,6 @@ __global__ __launch_bounds__(256) void block_means_kernel(const MeansArgs p) {
     for (int e = 0; e < E; ++e) sum[e] = 0.0f;
     int held = 0;  // rows that are in the cache
     if (mine < groups) {
-#pragma unroll 4
       for (int r = mine; r < rows; r += groups) {
         const T* row = key_rows<T>(p.seqs, q, seq, p.k, head, (j0 + r) & ~15);
         if (row != nullptr) {
