@@ -6,14 +6,20 @@
 // along its rows, and the sparse matrix so made times the values, in one pass with the
 // running maximum and sum of each row.  A block named twice counts once.
 //
+// Weights of 16-bit values go through the matrix cores in two parts (Rows::halves), so that
+// results are off by their own rounding alone.  In one part, 8 bits of bfloat16, errors are
+// 1.4 times as large, and 16384 tokens take 1631 us instead of 1729.
+//
 // Many queries (block_walk.hpp): 16384 tokens of 4 x 16 heads of 128, 16 blocks of 64
-// keys, bf16 1617 us, 320 TFLOP/s; 4 x 512 tokens of 4 x 8 heads over 16384 keys in pages
-// of 16, 32 blocks, f16 398 us.  Ten tokens beside each other select 80 different blocks
-// of 256, so a block has two or three readers, and what bounds it is the way of a step
-// through a slot (load, announcement, reading): the matrix instructions are busy for 15%
-// of the cycles, LDS for 25, and without its loads or without its products it takes nine
-// tenths as long.  Few queries: 64 tokens of 8 x 8 heads over as many caches 53 us, 262 MB
-// at 4.9 TB/s, a copy's rate.
+// keys, bf16 1729 us, 299 TFLOP/s; 4 x 512 tokens of 4 x 8 heads over 16384 keys in pages
+// of 16, 32 blocks, f16 443 us.  The 12 tokens (24 of groups of 8) of a workgroup select 79
+// (172) different blocks of 256, so a step has 2.4 (3.6) of its twelve readers, and what
+// bounds it is a step's way through a slot (load, announcement, reading): 1240 (1570)
+// cycles, where a reader's matrix instructions take 384.  Those are busy for 18% (16%) of
+// the cycles, LDS for 26% (21%); waves wait for half of theirs.  Of rows of 128 16-bit
+// values the kernel fills its 128 registers (float16 spills two, outside the steps, and
+// both 47 scalars).  Few queries: 64 tokens of 8 x 8 heads over as many caches 61 us, 262
+// MB at 4.3 TB/s.
 #include "block_walk.hpp"
 
 namespace fs {
@@ -172,7 +178,8 @@ __device__ __forceinline__ void careful_row(const BlockArgs& p, const Sequence& 
 }
 
 // Many queries.  A row whose result is not finite is left to the next kernel.
-// Waves that read, by the bytes of a row.
+// Waves that read, by the bytes of a row: with the loaders the 16 waves that have 128
+// registers each, or, of rows of 512 bytes, which need 208, the 8 that have 256.
 constexpr int many_readers(int row) { return row <= 256 ? 12 : 6; }
 template <class T, int DP>
 struct ManyShape : WalkShape<T, DP, many_readers(DP * (int)sizeof(T)), (DP * sizeof(T) > 256 ? 2 : 4)> {
@@ -513,9 +520,9 @@ Plan plan_of(int val_t, const fs_block_seqs& s, int heads, int group, int width,
     const int bytes = (width <= 64 ? 64 : width <= 128 ? 128 : 256) * (val_t == FS_F32 ? 4 : 2);
     const int waves = bytes > 256 ? kFewWaves / 2 : kFewWaves;
     const int64_t steps = (int64_t)top * block / 32;
-    // until a wave has four steps, or there are two workgroups a compute unit (us with four
-    // and with one, where the join is a launch of its own: one token of 8 x 4 heads, 16
-    // blocks of 64 keys 20.7 and 24.8)
+    // until a wave has four steps, or there are two workgroups a compute unit: the join is a
+    // launch of its own (us with four, with one and with 16, one token of 8 x 4 heads of 128,
+    // blocks of 64 keys: 16 blocks 20, 24, 20; 64 blocks 25, 25, 36; 128 blocks 29, 36, 50)
     while ((int64_t)o.splits * waves * 4 < steps && o.groups * o.splits < 512 && o.splits < 64) o.splits *= 2;
     if (o.splits > 1)
       o.bytes = (size_t)(o.groups * o.splits) * (32 + 16 * (width <= 64 ? 64 : width <= 128 ? 128 : 256)) * 4;

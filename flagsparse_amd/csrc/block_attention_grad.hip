@@ -12,17 +12,24 @@
 // piece and 32 or 64 of a block's keys; pieces of one block leave their sums in the
 // workspace, which are added in order, so no atomics' order shows.
 //
-// 8192 tokens of 4 x 8 heads of 128, 16 blocks of 64 keys, bf16: 1427 us, 219 TFLOP/s; the
-// queries' part 735 (bound as the forward pass is, by what its waves wait for each other),
-// the keys' 680: eight waves of 16 keys, so that two are on a SIMD (four waves of 32 keys,
-// one on each, 775), LDS busy for half of the time, as each wave reads all rows both
-// ways; joining the pieces' sums 69, sorting and cutting the lists 45.
+// P and dS of 16-bit values go through the matrix cores in two parts (Rows::halves), as
+// the forward pass's weights do: in one, errors are 1.4 times as large and the case below
+// takes 1437 us.
+//
+// 8192 tokens of 4 x 8 heads of 128, 16 blocks of 64 keys, bf16: 1556 us, 201 TFLOP/s; kernels
+// under the profiler: the queries' part 770, bound as the forward pass is, by what its waves wait for each other
+// (matrix instructions busy for 21% of the cycles, LDS for 31%), the keys' 724: eight
+// waves of 16 keys, so that two are on a SIMD (four of 32 keys, one on each, took 14%
+// longer), which wait for 47% of their cycles, for a step's rows and at its barrier
+// (matrix instructions 22%, LDS 26%), joining the pieces' sums 70, sorting and cutting the
+// lists 40.  The queries' gradient alone 732, the keys' and values' 865.
 #include "block_walk.hpp"
 
 namespace fs {
 namespace {
 
-// Waves that read, of the queries' gradient, by the bytes of a row.
+// Waves that read, of the queries' gradient, by the bytes of a row: with the loaders as
+// many as have the registers that they need, 128, 168 or 256.
 constexpr int query_readers(int row) { return row <= 128 ? 12 : row <= 256 ? 8 : 6; }
 
 // dS of float16, whose small values have few bits, times a power of two: of a query's
@@ -847,8 +854,12 @@ GradPlan grad_plan(int val_t, const fs_block_seqs& s, int heads, int group, int 
   l.entries = tokens * lists * top;
   l.key_blocks = rows / block + n_seqs + 1;
   l.n_keys = l.key_blocks * lists;
-  // pieces enough for a few rounds of the chip, and long enough that their sums cost little;
-  // so many at most, whatever the sizes: their sums are the workspace's largest part
+  // Pieces enough for a few rounds of the chip, and long enough that their sums cost little;
+  // so many at most, whatever the sizes: their sums are the workspace's largest part.  us
+  // with 2048 pieces, with 1024 and with 4096: 8192 tokens of 4 x 8 heads 1563, 1587, 1643;
+  // 2048 of 4 x 16 594, 557, 727; 4 x 2048 of 8 x 1 370, 348, 366; f32, 8192 of 4 x 8 10787,
+  // 11587, 10417.  With 512 rows a piece at least, 256 and 1024: 1024 tokens of 4 x 4 heads
+  // 148, 162, 143, f32 621, 601, 699.
   const int64_t shared = heads / lists, parts = std::max(1, block / 64);
   const int64_t most = std::max<int64_t>(ceil_div(l.entries * shared * parts, 2048), ceil_div(512, group));
   l.most = (int)std::min<int64_t>(most, INT32_MAX);

@@ -12,10 +12,11 @@
 // first, then bit by bit.  Of single tokens each wave takes a part of the blocks, and
 // one the best of all parts.  Ties go to the lower block.
 //
-// 16384 tokens of 4 x 16 heads of 128, 256 blocks, bf16 152 us (the queries alone are 268
+// 16384 tokens of 4 x 16 heads of 128, 256 blocks, bf16 151 us (the queries alone are 268
 // MB, 52 us at a copy's rate; the rest is the limits, a wave's two tokens one after the
-// other); 32 single tokens of 8 x 4 heads over 1024 blocks 32 us, bound by the latency of
-// a wave's dozen loads of means and its two searches.
+// other); 32 single tokens of 8 x 4 heads over 1024 blocks 33 us, bound by the latency of
+// a wave's loads of means, its search, and up to seven searches more of the wave that
+// joins the parts.  Widths of 256: 32 single tokens over 1024 blocks 67 us.
 #include "block_tile.hpp"
 
 namespace fs {

@@ -235,7 +235,7 @@ __device__ inline void fence() { __builtin_amdgcn_sched_barrier(0); }
 
 // Of 32-bit values, whose products are eight times as slow, columns past the width are
 // left out: `used` counts the 16 columns at a time that are not (float32, 3 sequences of
-// 2501 tokens and fewer, 12 heads of 80 columns: 315 us, without this 382).
+// 2501 tokens and fewer, 12 heads of 80 columns: 314 us, without this 385).
 template <class T>
 __device__ inline bool leave_out(int at, int used) { return sizeof(T) == 4 && at >= used; }
 
