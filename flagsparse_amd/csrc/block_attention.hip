@@ -490,11 +490,17 @@ __global__ __launch_bounds__(128) void block_attention_join_kernel(const BlockAr
 //   group 8, 64 blocks  2048 281, 345; 4096 552, 357
 //   group 4, width 256  1600 199, 205; 2048 230, 203;  width 64 (f16) 4096 106, 136
 //   group 4, f32  2048 344, 632; 4096 681, 637
-// Even at about 6500 of widths of 128 by the root of the group; never above 4096.
+// Even at about 6500 of widths of 128 by the root of the group; never above 4096.  Of
+// single tokens nothing is shared, unless 16 of the group at a time share a token's blocks,
+// and of two a sequence little (8 heads, group 8):
+//   of one a sequence  4096 290, 388; 16384 1713, 2275;  group 64 128 55, 41
+//   of two             2048 189, 214; 4096 376, 422; 16384 1203, 990;  width 256 2048 345, 304
 constexpr int64_t kFewMost = 4096, kEven = 6500;
-inline bool few_rows(int64_t tokens, int heads, int group, int width) {
-  const int64_t all = tokens * heads * ((group + 15) / 16);
+inline bool few_rows(const fs_block_seqs& s, int heads, int group, int width) {
+  const int64_t all = s.n_tokens * heads * ((group + 15) / 16);
+  if (group <= 16 && s.n_tokens <= s.n_seqs) return true;
   if (all > kFewMost) return false;
+  if (group <= 16 && width <= 128 && s.n_tokens <= 2 * s.n_seqs) return true;
   const int64_t wide = all * (width <= 64 ? 64 : width <= 128 ? 128 : 256);
   return wide * wide * group <= (kEven * 128) * (kEven * 128);
 }
@@ -513,7 +519,7 @@ Plan plan_of(int val_t, const fs_block_seqs& s, int heads, int group, int width,
   const int block = s.block;
   o.readers = many_readers((width <= 64 ? 64 : width <= 128 ? 128 : 256) * (val_t == FS_F32 ? 4 : 2));
   // (a group whose rows do not fit a workgroup of the other kernel, too)
-  o.few = few_rows(tokens, heads, group, width) || o.readers * 16 < group;
+  o.few = few_rows(s, heads, group, width) || o.readers * 16 < group;
   o.groups = tokens * heads * ((group + 15) / 16);
   o.splits = 1;
   if (o.few) {

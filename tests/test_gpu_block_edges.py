@@ -178,6 +178,26 @@ def test_either_side_of_the_rule(tokens, page):
     assert worst(out, *attention_bounds(case, blocks, 128**-0.5)) <= 1.0
 
 
+@pytest.mark.parametrize("page", [0, 16], ids=["rows", "pages"])
+@pytest.mark.parametrize("group, kernel", [(2, "few_"), (17, "")])
+def test_single_tokens_of_many_sequences(page, group, kernel):
+    """A decode step of 1200 sequences: no two tokens share a block."""
+    n, heads = 1200, 4
+    lengths = [(7 * i) % 23 for i in range(n)]
+    case = Case([1] * n, lengths, heads, group, 32, 32, torch.bfloat16, 79, page, single=True)
+    blocks = torch.zeros((n, 1, 1), dtype=torch.int32, device="cuda")
+    out, lse = fs.flagsparse_block_attention(case.q, case.k, case.v, blocks, case.seqs, return_lse=True)
+    assert _lib.last_kernel() == f"block_attention_{kernel}kernel"
+    for b in range(0, n, 61):
+        one = Case([1], [lengths[b]], heads, group, 32, 32, torch.bfloat16, 79)
+        rows = slice(sum(lengths[:b]), sum(lengths[: b + 1]))
+        one.q, one.packed_k, one.packed_v = case.q[b : b + 1], case.packed_k[rows], case.packed_v[rows]
+        if lengths[b] == 0:
+            assert not out[b].any() and bool((lse[b] == -INF).all())
+        else:
+            assert worst(out[b : b + 1], *attention_bounds(one, blocks[b : b + 1], 32**-0.5)) <= 1.0
+
+
 class _Guarded:
     """A tensor's copy in the middle of a larger one, whose other values are kept in mind."""
 
