@@ -267,3 +267,38 @@ def test_lengths_beyond_the_arrays_touch_nothing_around_them(which, tokens):
     found = gradient_bounds(case, blocks, width**-0.5, grad.middle, out.middle, lse)
     for t, name in ((dq, "dq"), (dk, "dk"), (dv, "dv")):
         assert worst(t.middle, *found[name]) <= 1.0, name
+
+
+@pytest.mark.parametrize("wanted", ["q", "kv"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["f16", "f32"])
+def test_a_captured_backward_of_some_leaves(dtype, wanted):
+    """Captured alone, replayed with other values, eager passes in between; on a stream of its own."""
+    case = Case([300, 70], [300, 90], 2, 3, 64, 64, dtype, 80)
+    blocks = random_blocks([300, 70], [300, 90], 2, 3, 64, 81)
+    leaves = {n: t.clone().requires_grad_(n in wanted) for n, t in zip("qkv", (case.q, case.k, case.v))}
+    grad = randn(case.q.shape, dtype, 82)
+
+    def step():
+        out = fs.flagsparse_block_attention(*leaves.values(), blocks, case.seqs)
+        return torch.autograd.grad(out, [leaves[n] for n in wanted], grad)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for turn in range(4):
+        size = 2.0 ** (6 * turn - 12)
+        grad.copy_(randn(case.q.shape, dtype, 83 + turn) * size)
+        with torch.no_grad():
+            leaves["v"].copy_(randn(case.v.shape, dtype, 90 + turn))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in held]
+        with torch.cuda.stream(side):
+            want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
